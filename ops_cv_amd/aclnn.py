@@ -456,6 +456,79 @@ def upsample_bilinear2d_backward(grad_out, input_size, align_corners=False, scal
                                                                 out, workspace, _raw(stream), channels_last, out_dtype)
 
 
+# ----------------------------------------------------------------------------------------------------
+# operators on token sequences (include/opscv_tokens.h)
+# ----------------------------------------------------------------------------------------------------
+
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BASE, ROTARY_BY_PARTS = 0, 1, 2, 3
+NO_WINDOW = 2 ** 63 - 1
+
+
+def residual_norm(x, weight, residual=None, eps=1e-6, need_rstd=False, out=None, sum_out=None, rstd_out=None,
+                  stream=None, workspace=None):
+    """Both phases of opscvResidualNorm: root-mean-square norm of x, or of x + residual, times weight, over the last
+    dimension.  Returns (out, sum, rstd): sum is x + residual (None without a residual), rstd what the backward call
+    reads (None unless need_rstd)."""
+    return (_helpers or _native()).residual_norm(x, weight, residual, eps, False, need_rstd, out, None, sum_out, rstd_out,
+                                                 workspace, _raw(stream))
+
+
+def residual_norm_int8(x, weight, residual=None, eps=1e-6, need_rstd=False, out=None, scale_out=None, sum_out=None,
+                       rstd_out=None, stream=None, workspace=None):
+    """residual_norm with the result in 8 bits; returns (out, scale, sum, rstd).  out * scale[..., None] stands for the
+    norm."""
+    return (_helpers or _native()).residual_norm(x, weight, residual, eps, True, need_rstd, out, scale_out, sum_out,
+                                                 rstd_out, workspace, _raw(stream))
+
+
+def residual_norm_backward(grad_y, sum_in, weight, rstd, grad_sum=None, need_weight=True, grad_x=None, grad_weight=None,
+                           stream=None, workspace=None):
+    """Both phases of opscvResidualNormBackward; returns (grad_x, grad_weight).  sum_in and rstd are what the forward call
+    returned (sum_in = x without a residual), grad_sum the gradient that reaches the sum on its other way.  grad_x is the
+    gradient of x and of the residual alike; grad_weight is None unless need_weight."""
+    return (_helpers or _native()).residual_norm_backward(grad_y, sum_in, weight, rstd, grad_sum, need_weight, grad_x,
+                                                          grad_weight, workspace, _raw(stream))
+
+
+def rotary_table(like, positions, rot, base=10000.0, scaling=ROTARY_PLAIN, factor=1.0, original_length=0, magnitude=1.0,
+                 out=None, stream=None, workspace=None):
+    """Both phases of opscvRotaryTable: cosines and sines of `positions` positions, float32 (positions, rot), on the device
+    of the tensor `like`."""
+    return (_helpers or _native()).rotary_table(like, positions, rot, base, scaling, factor, original_length, magnitude,
+                                                out, workspace, _raw(stream))
+
+
+def rotary(query, key, table, positions=None, interleaved=False, inverse=False, query_out=None, key_out=None, stream=None,
+           workspace=None):
+    """Both phases of opscvRotary on (batch, tokens, heads, d) tensors; returns (query_out, key_out).  key may be None.
+    The outputs may be the inputs.  inverse gives the gradient's way back."""
+    return (_helpers or _native()).rotary(query, key, table, positions, interleaved, inverse, query_out, key_out,
+                                          workspace, _raw(stream))
+
+
+def _scale(scale, query):
+    return query.shape[-1] ** -0.5 if scale is None else scale
+
+
+def window_attention(query, key, value, scale=None, left=NO_WINDOW, right=0, sinks=0, q_lengths=None, kv_lengths=None,
+                     need_lse=False, out=None, lse=None, stream=None, workspace=None):
+    """Both phases of opscvWindowAttention; returns (out, lse), lse None unless need_lse.  query is (batch, tokens, heads,
+    d), key and value (batch, kv_tokens, kv_heads, d); query i of a sequence stands at p = kv_length - q_length + i and
+    sees the keys j <= p + right with j >= p - left or j < sinks.  scale defaults to d ** -0.5."""
+    return (_helpers or _native()).window_attention(query, key, value, _scale(scale, query), left, right, sinks, q_lengths,
+                                                    kv_lengths, need_lse, out, lse, workspace, _raw(stream))
+
+
+def window_attention_backward(grad_out, query, key, value, out, lse, scale=None, left=NO_WINDOW, right=0, sinks=0,
+                              q_lengths=None, kv_lengths=None, grad_query=None, grad_key=None, grad_value=None,
+                              stream=None, workspace=None):
+    """Both phases of opscvWindowAttentionBackward; returns (grad_query, grad_key, grad_value).  out and lse are what the
+    forward call returned for the same arguments."""
+    return (_helpers or _native()).window_attention_backward(grad_out, query, key, value, out, lse, _scale(scale, query),
+                                                             left, right, sinks, q_lengths, kv_lengths, grad_query,
+                                                             grad_key, grad_value, workspace, _raw(stream))
+
+
 def grid_sampler2d_taps(grid, h_in, w_in, interpolation_mode=0, padding_mode=0, align_corners=False, stream=None):
     """Per-pixel tap records (numpy structured array) computed on the device by the kernels' coordinate stage."""
     import numpy as np

@@ -6,6 +6,7 @@
 #include <vector>
 
 #include "opscv_acl_base.h"
+#include "token_args.hpp"
 
 constexpr int kMaxDims = 8;
 
@@ -81,7 +82,8 @@ struct StridedView {
 };
 
 enum class OpKind : int { Nop = 0, GridSampler2D = 1, Resize = 2, ResizeGrad = 3, GridSampler3D = 4, GridSampler2DGrad = 5,
-                          GridSampler3DGrad = 6 };
+                          GridSampler3DGrad = 6, ResidualNorm = 7, ResidualNormGrad = 8, RotaryTable = 9, Rotary = 10,
+                          WindowAttention = 11, WindowAttentionGrad = 12 };
 
 // Where a kernel operand lives: the tensor's own memory (contiguous view) or a slice of the caller's
 // workspace, known only as an offset until the second phase receives the workspace address.
@@ -217,19 +219,29 @@ struct aclOpExecutor {
     opscv::GridSampler3DArgs gs3;
     opscv::GridSamplerGradArgs gsg;
     opscv::GridSampler3DGradArgs gsg3;
+    opscv::NormArgs norm;
+    opscv::NormGradArgs norm_grad;
+    opscv::RotaryTableArgs rotary_table;
+    opscv::RotaryArgs rotary;
+    opscv::AttentionArgs attention;
     int want_out0 = 1, want_out1 = 0;  // which outputs the operator produces (backward output mask)
     opscv::PlannedPtr in0, in1, out0;  // input/self, grid, out
     opscv::PlannedPtr in2, out1;       // third input and second output of the operators that have them
     opscv::PlannedPtr scratch;         // kernel scratch inside the workspace (operators that use one)
+    // operands of the operators on token sequences, by the slots of opscv_tokens.cpp; bit i of `required`: operand i has
+    // elements, so its address must not be NULL
+    static constexpr int kOperands = 12;
+    opscv::PlannedPtr operands[kOperands];
+    uint32_t required = 0;
     // packing work: views gathered into the workspace before the kernel, scattered after it
     struct Pack {
         opscv::StridedView view;
         uint64_t ws_offset = 0;
         int elem_bytes = 0;
     };
-    // at most three inputs and two outputs per operator; fixed storage, so that planning never touches the heap
+    // at most five inputs and four outputs per operator; fixed storage, so that planning never touches the heap
     struct PackList {
-        static constexpr int kCapacity = 4;
+        static constexpr int kCapacity = 5;
         Pack items[kCapacity];
         int count = 0;
         // false when the list is full (the entry is dropped: the caller must fail the plan)

@@ -1,0 +1,448 @@
+// Attention forward: softmax over the keys that a query sees, in one pass over them with a running maximum and sum.
+//
+// The rows of a workgroup are queries of all heads that share a key head (row r: query r / G of head r % G of the group),
+// so a tile of keys and values in LDS serves them all, and their windows span few keys beyond one query's.  A wavefront
+// has 32 rows, one per lane of a half:
+//   S' = K Q'        (32 keys x 32 rows; K from LDS in "row" order, Q in registers)
+//   m, l             running maximum of a row and sum of exp2(S c - m), c = scale log2 e; a row's keys are spread over two
+//                    lanes, which exchange their maxima
+//   O' = O' f + V' P (head features x 32 rows; V from LDS in "column" order, P are S's registers, rounded to the type)
+// m, l and O stay in 32 bits; P is rounded to the type as the matrix instructions want it.
+#pragma once
+
+#include <atomic>
+
+#include "attention_plan.hpp"
+#include "attention_tile.hpp"
+#include "fast_div.hpp"
+#include "kernels.hpp"
+
+namespace opscv {
+namespace att {
+
+struct ForwardLaunch {
+    AttentionArgs a;
+    FastDiv group;    // heads that share a key head
+    uint32_t rows;    // queries times those
+    uint32_t tiles, splits, kv_heads;
+    uint32_t blocks;  // workgroups with work
+};
+
+// Workgroups go round the eight XCDs; this gives every XCD a run of neighbouring numbers, so that the tiles of rows that
+// read the same keys share an L2.
+static __device__ __forceinline__ uint32_t xcd_order(uint32_t index, uint32_t count)
+{
+    const uint32_t each = (count + 7) / 8;
+    return (index & 7u) * each + (index >> 3);
+}
+
+// Keys that a range of rows sees, as tiles: the first `sink_tiles` start at key 0, the others at `first`.
+struct KeyRange {
+    int first, end;  // window
+    int sink_end;    // sinks in front of it
+    int sink_tiles, tiles;
+};
+
+template <int KEYS>
+static __device__ __forceinline__ KeyRange key_range(int p_low, int p_high, int kv_len, int left, int right, int sinks)
+{
+    KeyRange k;
+    k.end = min(max(p_high + right + 1, 0), kv_len);
+    k.first = min(max(p_low - left, 0), k.end);
+    k.sink_end = min(sinks, k.first);
+    k.sink_tiles = (k.sink_end + KEYS - 1) / KEYS;
+    if (k.sink_tiles > 0 && k.first <= k.sink_tiles * KEYS) {  // the window starts among them: one run of tiles
+        k.first = 0;
+        k.sink_tiles = 0;
+    }
+    k.tiles = k.sink_tiles + (k.end - k.first + KEYS - 1) / KEYS;
+    return k;
+}
+
+template <typename T, int NB, bool FEW, bool VEC>
+__global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads(), 1) void attention_kernel(
+    ForwardLaunch p)
+{
+    constexpr int kPitch = pitch_of(NB);
+    constexpr ForwardShape kShape = forward_shape(sizeof(T), kPitch, FEW);
+    constexpr int kKeys = kShape.keys, kSubs = kKeys / kBlock, kGroupThreads = 64 * kShape.row_waves;
+    typedef Tile<T, kPitch> L;
+    extern __shared__ __align__(16) char lds[];
+
+    const AttentionArgs& a = p.a;
+    const uint32_t index = xcd_order(blockIdx.x, p.blocks);
+    if (index >= p.blocks || (blockIdx.x >> 3) >= (p.blocks + 7) / 8) {
+        return;
+    }
+    const uint32_t tile = index % p.tiles, rest = index / p.tiles;
+    const uint32_t split = rest % p.splits, bh = rest / p.splits;
+    const uint32_t b = bh / p.kv_heads, kv_head = bh % p.kv_heads;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
+    const int h = lane >> 5, own = lane & 31;
+    const int row_wave = wave % kShape.row_waves, key_wave = wave / kShape.row_waves;
+    const int gt = row_wave * 64 + lane;
+    const int d = (int)a.d, left = (int)a.left, right = (int)a.right, sinks = (int)a.sinks;
+    const Sequence seq = sequence_at(a, b);
+
+    // the row of this lane; rows past the last repeat it and are not written
+    const uint32_t row0 = tile * kShape.rows(), wave_row0 = row0 + row_wave * kBlock;
+    const uint32_t row = min(wave_row0 + own, p.rows - 1);
+    const int query = (int)fast_div(row, p.group), in_group = (int)(row - (uint32_t)query * p.group.div);
+    const int head = (int)(kv_head * p.group.div) + in_group;
+    const int pos = query < seq.q_len ? seq.first + query : INT32_MIN / 2;  // a padding query sees nothing
+
+    // queries of the workgroup and of the wavefront
+    const auto query_of = [&](uint32_t r) { return (int)fast_div(min(r, p.rows - 1), p.group); };
+    const int block_low = query_of(row0), block_high = min(query_of(row0 + kShape.rows() - 1), seq.q_len - 1);
+    KeyRange range = key_range<kKeys>(seq.first + block_low, seq.first + block_high, seq.kv_len, left, right, sinks);
+    if (block_high < block_low) {
+        range.tiles = 0;
+    }
+    const int wave_low = seq.first + query_of(wave_row0), wave_high = seq.first + query_of(wave_row0 + kBlock - 1);
+    const bool wave_whole = query_of(wave_row0 + kBlock - 1) < seq.q_len;
+    const int t_begin = (int)((int64_t)range.tiles * split / p.splits);
+    const int t_end = (int)((int64_t)range.tiles * (split + 1) / p.splits);
+
+    Frag<T> q[2 * NB];
+    {
+        const T* const src = (const T*)a.q.ptr + (int64_t)b * a.q.stride[0] + (int64_t)query * a.q.stride[1] +
+                             (int64_t)head * a.q.stride[2];
+#pragma unroll
+        for (int i = 0; i < 2 * NB; i++) {
+            q[i] = global_row<T, VEC>(src, 16 * i + 8 * h, d);
+        }
+    }
+    const T* const k_base = (const T*)a.k.ptr + (int64_t)b * a.k.stride[0] + (int64_t)kv_head * a.k.stride[2];
+    const T* const v_base = (const T*)a.v.ptr + (int64_t)b * a.v.stride[0] + (int64_t)kv_head * a.v.stride[2];
+    const uint32_t k_pitch = (uint32_t)(a.k.stride[1] * (int64_t)sizeof(T));
+    const uint32_t v_pitch = (uint32_t)(a.v.stride[1] * (int64_t)sizeof(T));
+
+    T* const ring = reinterpret_cast<T*>(lds) + (size_t)key_wave * (kShape.stages * 2 * kKeys * kPitch);
+    const auto key_of = [&](int t) { return t < range.sink_tiles ? t * kKeys : range.first + (t - range.sink_tiles) * kKeys; };
+    const auto end_of = [&](int t) { return t < range.sink_tiles ? range.sink_end : range.end; };
+    const auto fetch = [&](int t, int buffer) {
+        const int key0 = key_of(t), rows = end_of(t) - key0;
+        T* const k_tile = ring + buffer * (2 * kKeys * kPitch);
+        stage<T, kPitch, kKeys, kGroupThreads, VEC>(k_tile, k_base + (int64_t)key0 * a.k.stride[1], gt, d, [&](int r) {
+            return r < rows ? (uint32_t)r * k_pitch : kOutside;
+        });
+        stage<T, kPitch, kKeys, kGroupThreads, VEC>(k_tile + kKeys * kPitch, v_base + (int64_t)key0 * a.v.stride[1], gt, d,
+                                                    [&](int r) { return r < rows ? (uint32_t)r * v_pitch : kOutside; });
+    };
+    constexpr int kInFlight = 2 * kKeys * L::kChunks / kGroupThreads;  // loads of one fetch, a wavefront
+    const auto group_barrier = [&]() {
+        if constexpr (kShape.row_waves > 1) {
+            __syncthreads();
+        } else {
+            // one wavefront: its LDS operations stay in order; what it has read is back before the place is filled again
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+        }
+    };
+
+    const float c = a.scale * kLog2e;
+    float most = -INFINITY, total = 0.0f;  // `total`: of this lane's keys only
+    acc_t o[NB];
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        o[i] = zeros();
+    }
+
+    int buffer = 0;
+    if (t_begin + key_wave < t_end) {
+        fetch(t_begin + key_wave, 0);
+    }
+    for (int t = t_begin + key_wave; t < t_end; t += kShape.key_waves) {
+        const bool more = t + kShape.key_waves < t_end;
+        if (kShape.stages == 2 && more) {
+            fetch(t + kShape.key_waves, buffer ^ 1);
+            if constexpr (VEC) {
+                __builtin_amdgcn_s_waitcnt((kInFlight & 15) | ((kInFlight >> 4) << 14) | 0xf70);  // vmcnt(kInFlight)
+            }
+        } else if constexpr (VEC) {
+            __builtin_amdgcn_s_waitcnt(0xf70);  // vmcnt(0)
+        }
+        group_barrier();
+        const T* const k_tile = ring + buffer * (2 * kKeys * kPitch);
+        const T* const v_tile = k_tile + kKeys * kPitch;
+        const int key0 = key_of(t), end = end_of(t);
+
+        acc_t s[kSubs];
+#pragma unroll
+        for (int j = 0; j < kSubs; j++) {
+            s[j] = zeros();
+#pragma unroll
+            for (int i = 0; i < 2 * NB; i++) {
+                s[j] = Mma<T>::mul(L::row(k_tile, j * kBlock + own, 2 * i + h), q[i], s[j]);
+            }
+        }
+        const bool all_seen = wave_whole && key0 + kKeys <= end && key0 + kKeys - 1 <= wave_low + right &&
+                              (key0 >= wave_high - left || key0 + kKeys <= sinks);
+        if (!all_seen) {
+#pragma unroll
+            for (int j = 0; j < kSubs; j++) {
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int key = key0 + j * kBlock + 8 * (r / 4) + 4 * h + r % 4;
+                    s[j][r] = (key < end && sees(pos, key, left, right, sinks)) ? s[j][r] : -INFINITY;
+                }
+            }
+        }
+        float high = s[0][0];
+#pragma unroll
+        for (int j = 0; j < kSubs; j++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                high = fmaxf(high, s[j][r]);
+            }
+        }
+        high = fmaxf(high, other_half(high)) * c;
+        const float now = fmaxf(most, high);
+        const float base = now == -INFINITY ? 0.0f : now;  // rows that have seen nothing yet: exp2(-inf - 0) = 0
+        if (__any(now > most)) {
+            const float fade = exp2f(most - base);
+            total *= fade;
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    o[i][r] *= fade;
+                }
+            }
+        }
+        most = now;
+#pragma unroll
+        for (int j = 0; j < kSubs; j++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                s[j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], c, -base));
+                total += s[j][r];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kSubs; j++) {
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+                const Frag<T> w = operand<T>(s[j], g);
+#pragma unroll
+                for (int i = 0; i < NB; i++) {
+                    o[i] = Mma<T>::mul(L::column(v_tile, j * kBlock + 16 * g, i, lane), w, o[i]);
+                }
+            }
+        }
+        group_barrier();
+        if (kShape.stages == 1 && more) {
+            fetch(t + kShape.key_waves, 0);
+        }
+        buffer ^= kShape.stages - 1;
+    }
+    total += other_half(total);
+
+    // join the wavefronts that shared the keys: every one leaves its sums in LDS, [feature][row], and takes a share of
+    // the features for all of them
+    constexpr int kJoin = kShape.key_waves;
+    float* const sums = reinterpret_cast<float*>(lds);
+    if constexpr (kJoin > 1) {
+        constexpr int kWaveFloats = (NB * kBlock + 2) * kBlock;
+        __syncthreads();
+        float* const mine = sums + wave * kWaveFloats;
+        if (h == 0) {
+            mine[own] = most;
+            mine[kBlock + own] = total;
+        }
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                mine[(2 + i * kBlock + 8 * (r / 4) + 4 * h + r % 4) * kBlock + own] = o[i][r];
+            }
+        }
+        __syncthreads();
+        float high = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kJoin; w++) {
+            high = fmaxf(high, sums[w * kWaveFloats + own]);
+        }
+        const float base = high == -INFINITY ? 0.0f : high;
+        float share[kJoin];
+        total = 0.0f;
+        most = high;
+#pragma unroll
+        for (int w = 0; w < kJoin; w++) {
+            share[w] = exp2f(sums[w * kWaveFloats + own] - base);
+            total += share[w] * sums[w * kWaveFloats + kBlock + own];
+        }
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+            if (i % kJoin == wave) {
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    float x = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < kJoin; w++) {
+                        x += share[w] * sums[w * kWaveFloats + (2 + i * kBlock + 8 * (r / 4) + 4 * h + r % 4) * kBlock + own];
+                    }
+                    o[i][r] = x;
+                }
+            }
+        }
+    }
+
+    if (wave_row0 + own >= p.rows) {
+        return;
+    }
+    const bool first_wave = kJoin == 1 || wave == 0;
+    if (p.splits > 1) {
+        float* const part = a.scratch + (((int64_t)bh * p.splits + split) * p.rows + row) * partial_floats(d);
+        if (first_wave && h == 0) {
+            part[0] = most;
+            part[1] = total;
+        }
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+            if (kJoin == 1 || i % kJoin == wave) {
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const int at = i * kBlock + 8 * (r / 4) + 4 * h;
+                    if (at < d) {  // rows of partial results have room for whole groups of four
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            part[2 + at + e] = o[i][r + e];
+                        }
+                    }
+                }
+            }
+        }
+        return;
+    }
+    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    if (first_wave && h == 0 && a.lse.ptr != nullptr) {
+        ((float*)a.lse.ptr)[(int64_t)b * a.lse.stride[0] + (int64_t)head * a.lse.stride[1] +
+                            (int64_t)query * a.lse.stride[2]] =
+            total == 0.0f ? -INFINITY : (most + log2f(total)) * kLn2;
+    }
+    T* const out = (T*)a.out.ptr + (int64_t)b * a.out.stride[0] + (int64_t)query * a.out.stride[1] +
+                   (int64_t)head * a.out.stride[2];
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        if (kJoin == 1 || i % kJoin == wave) {
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                put4<T, VEC>(out, i * kBlock + 8 * (r / 4) + 4 * h, d, o[i][r] * inverse, o[i][r + 1] * inverse,
+                             o[i][r + 2] * inverse, o[i][r + 3] * inverse);
+            }
+        }
+    }
+}
+
+// Joins the parts of a split: four features of a row a thread.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void attention_join_kernel(ForwardLaunch p, uint32_t quads, uint32_t total)
+{
+    const AttentionArgs& a = p.a;
+    const uint32_t index = blockIdx.x * 256u + threadIdx.x;
+    if (index >= total) {
+        return;
+    }
+    const uint32_t quad = index % quads, rest = index / quads;
+    const uint32_t row = rest % p.rows, bh = rest / p.rows;
+    const uint32_t b = bh / p.kv_heads, kv_head = bh % p.kv_heads;
+    const int d = (int)a.d;
+    const int64_t step = partial_floats(d) * (int64_t)p.rows;
+    const float* const part = a.scratch + ((int64_t)bh * p.splits * p.rows + row) * partial_floats(d);
+    float high = -INFINITY;
+    for (uint32_t s = 0; s < p.splits; s++) {
+        high = fmaxf(high, part[s * step]);
+    }
+    const float base = high == -INFINITY ? 0.0f : high;
+    float sum = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t s = 0; s < p.splits; s++) {
+        const float* const at = part + s * step;
+        const float share = exp2f(at[0] - base);
+        sum += share * at[1];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            x[e] += share * at[2 + 4 * quad + e];
+        }
+    }
+    const uint32_t query = fast_div(row, p.group), head = kv_head * p.group.div + (row - query * p.group.div);
+    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (quad == 0 && a.lse.ptr != nullptr) {
+        ((float*)a.lse.ptr)[(int64_t)b * a.lse.stride[0] + (int64_t)head * a.lse.stride[1] +
+                            (int64_t)query * a.lse.stride[2]] =
+            sum == 0.0f ? -INFINITY : (high + log2f(sum)) * kLn2;
+    }
+    T* const out = (T*)a.out.ptr + (int64_t)b * a.out.stride[0] + (int64_t)query * a.out.stride[1] +
+                   (int64_t)head * a.out.stride[2];
+    put4<T, VEC>(out, (int)(4 * quad), d, x[0] * inverse, x[1] * inverse, x[2] * inverse, x[3] * inverse);
+}
+
+template <typename T, int NB, bool FEW, bool VEC>
+hipError_t run_forward_shape(const ForwardLaunch& p, hipStream_t stream)
+{
+    constexpr ForwardShape kShape = forward_shape(sizeof(T), pitch_of(NB), FEW);
+    constexpr int kTiles = kShape.key_waves * kShape.stages * 2 * kShape.keys * pitch_of(NB) * (int)sizeof(T);
+    constexpr int kJoin = kShape.key_waves > 1 ? kShape.key_waves * (NB * kBlock + 2) * kBlock * 4 : 0;
+    constexpr int kBytes = kTiles > kJoin ? kTiles : kJoin;
+    static_assert(kBytes <= 160 * 1024, "LDS of a CU");
+    static std::atomic<uint32_t> done{0};
+    const auto kernel = attention_kernel<T, NB, FEW, VEC>;
+    if (kBytes > 64 * 1024) {
+        if (const hipError_t e = allow_dynamic_lds((const void*)kernel, kBytes, done); e != hipSuccess) {
+            return e;
+        }
+    }
+    hipLaunchKernelGGL(kernel, dim3((p.blocks + 7) / 8 * 8), dim3(kShape.threads()), kBytes, stream, p);
+    return hipGetLastError();
+}
+
+template <typename T, bool VEC>
+hipError_t run_forward(const AttentionArgs& a, hipStream_t stream)
+{
+    const ForwardPlan plan = plan_forward(a);
+    if (plan.blocks > INT32_MAX / 1024 || (plan.splits > 1 && a.scratch == nullptr)) {
+        return hipErrorInvalidValue;
+    }
+    ForwardLaunch p;
+    p.a = a;
+    p.group = make_fast_div((uint32_t)(a.heads / a.kv_heads));
+    p.rows = (uint32_t)plan.rows;
+    p.tiles = (uint32_t)plan.tiles;
+    p.splits = (uint32_t)plan.splits;
+    p.kv_heads = (uint32_t)a.kv_heads;
+    p.blocks = (uint32_t)plan.blocks;
+    const int nb = VEC ? blocks_of(a.d) : (a.d <= 128 ? 4 : 8);  // odd sizes: two widths serve them all
+    hipError_t e = hipErrorInvalidValue;
+    const auto pick = [&](auto few) {
+        constexpr bool kFew = decltype(few)::value;
+        switch (nb) {
+            case 8: e = run_forward_shape<T, 8, kFew, VEC>(p, stream); break;
+            case 4: e = run_forward_shape<T, 4, kFew, VEC>(p, stream); break;
+            default:
+                if constexpr (VEC) {
+                    e = nb == 3 ? run_forward_shape<T, 3, kFew, VEC>(p, stream) : run_forward_shape<T, 2, kFew, VEC>(p, stream);
+                }
+                break;
+        }
+    };
+    plan.few_rows ? pick(std::true_type()) : pick(std::false_type());
+    if (e != hipSuccess || plan.splits == 1) {
+        return e;
+    }
+    const int64_t quads = (a.d + 3) / 4, total = a.batch * a.kv_heads * plan.rows * quads;
+    if (total > INT32_MAX) {
+        return hipErrorInvalidValue;
+    }
+    hipLaunchKernelGGL((attention_join_kernel<T, VEC>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, stream, p,
+                       (uint32_t)quads, (uint32_t)total);
+    return hipGetLastError();
+}
+
+}  // namespace att
+
+// one translation unit a type
+hipError_t run_attention_f32(const AttentionArgs& a, bool vectors, hipStream_t stream);
+hipError_t run_attention_f16(const AttentionArgs& a, bool vectors, hipStream_t stream);
+hipError_t run_attention_bf16(const AttentionArgs& a, bool vectors, hipStream_t stream);
+
+}  // namespace opscv

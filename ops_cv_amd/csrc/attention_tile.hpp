@@ -1,0 +1,311 @@
+// Tiles of attention on the matrix cores: fragments, staging through LDS, and what a query sees.
+//
+// Every product is made of 32 x 32 results over 16 terms: result[m][n] += sum over slots of A[m][slot] B[slot][n].  Lane l
+// holds row m = l % 32 of A (or column n of B) and the eight slots (h, 0..7) of its half h = l / 32; of the result it
+// holds column n = l % 32 and rows m = 8 (r / 4) + 4 h + r % 4 for r = 0..15.  16-bit types take one instruction
+// (32x32x16); FLOAT takes eight of 32x32x2, one for each slot of a lane, so the three types share all code.
+//
+// Which term a slot stands for is free as long as A and B agree.  Two orders are used: "row": slot (h, e) is term
+// 8 h + e, for operands whose terms lie side by side in memory; "column": slot (h, e) is term 4 h + e % 4 + 8 (e / 4),
+// the order in which a result of the instruction holds its rows.  So eight registers of one product's result are, rounded
+// to the type, the B operand of the next product as they stand, and nothing moves between lanes.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "acl_types.hpp"
+
+namespace opscv {
+namespace att {
+
+typedef float acc_t __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr uint32_t kOutside = 0x80000000u;  // an offset past every buffer: the load returns zeros
+constexpr int kBufferFlags = 0x00027000;    // raw buffer, 32-bit elements
+
+template <typename T>
+struct Mma;
+
+template <>
+struct Mma<__bf16> {
+    typedef bf16x8 Frag;
+    static __device__ __forceinline__ acc_t mul(Frag a, Frag b, acc_t c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+};
+
+template <>
+struct Mma<_Float16> {
+    typedef f16x8 Frag;
+    static __device__ __forceinline__ acc_t mul(Frag a, Frag b, acc_t c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+};
+
+template <>
+struct Mma<float> {
+    typedef f32x8 Frag;
+    static __device__ __forceinline__ acc_t mul(Frag a, Frag b, acc_t c)
+    {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+        }
+        return c;
+    }
+};
+
+template <typename T>
+using Frag = typename Mma<T>::Frag;
+
+static __device__ __forceinline__ acc_t zeros()
+{
+    acc_t z;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        z[i] = 0.0f;
+    }
+    return z;
+}
+
+// registers 8 g .. 8 g + 7 of a result as an operand, rounded to the type (to nearest: the products that follow take the
+// type's numbers, and their sums stay in 32 bits)
+template <typename T>
+static __device__ __forceinline__ Frag<T> operand(const acc_t& x, int g)
+{
+    Frag<T> f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        f[e] = (T)x[8 * g + e];
+    }
+    return f;
+}
+
+// x of the other half's lane with the same l % 32
+static __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+
+// ---------------------------------------------------------------------------------------------------------------- LDS
+//
+// A tile is rows of PITCH elements (a power of two, the head size rounded up) in 16-byte chunks; chunk c of row r lies at
+// place c ^ swizzle(r).  The swizzle spreads both ways of reading over the 64 banks: whole rows by neighbouring lanes
+// (16 rows of one chunk number fall on 16 places of a 256-byte span) and columns (four neighbouring rows of the same 64
+// bytes fall on the four quarters of such a span).
+
+template <typename T, int PITCH>
+struct Tile {
+    static constexpr int kPerChunk = 16 / (int)sizeof(T);
+    static constexpr int kChunks = PITCH / kPerChunk;  // of a row: 8 or more
+    static_assert(kChunks >= 8 && (kChunks & (kChunks - 1)) == 0, "rows of a power of two, 128 bytes or more");
+
+    static __device__ __forceinline__ int swizzle(int row)
+    {
+        return kChunks == 8 ? ((((row >> 1) & 1) << 2) | ((row >> 2) & 3)) : (((row & 3) << 2) | ((row >> 2) & 3));
+    }
+
+    static constexpr int bytes(int rows) { return rows * PITCH * (int)sizeof(T); }
+
+    // eight elements from element 8 c of a row on: an operand in "row" order, m or n = the row
+    static __device__ __forceinline__ Frag<T> row(const T* tile, int r, int c)
+    {
+        const T* const at = tile + r * PITCH;
+        if constexpr (sizeof(T) == 2) {
+            return *reinterpret_cast<const Frag<T>*>(at + ((c ^ swizzle(r)) * 8));
+        } else {
+            typedef float f32x4 __attribute__((ext_vector_type(4)));
+            const f32x4 a = *reinterpret_cast<const f32x4*>(at + (((2 * c) ^ swizzle(r)) * 4));
+            const f32x4 b = *reinterpret_cast<const f32x4*>(at + (((2 * c + 1) ^ swizzle(r)) * 4));
+            Frag<T> f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                f[e] = a[e];
+                f[4 + e] = b[e];
+            }
+            return f;
+        }
+    }
+
+    // element 32 block + l % 32 of rows base + 4 h + {0..3, 8..11}: an operand in "column" order, m or n = the element
+    static __device__ __forceinline__ Frag<T> column(const T* tile, int base, int block, int lane)
+    {
+        const int h = lane >> 5;
+        if constexpr (sizeof(T) == 2) {
+            // Sixteen lanes together read four rows of sixteen elements, eight bytes a lane (row i / 4, elements
+            // 4 (i % 4) .. + 3), and the instruction hands lane i column i of them.
+            const int i = lane & 15;
+            const int r = base + 4 * h + (i >> 2);
+            const int c = 4 * block + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);
+            const T* const a = tile + r * PITCH + ((c ^ swizzle(r)) * 8) + (i & 1) * 4;
+            const T* const b = tile + (r + 8) * PITCH + ((c ^ swizzle(r + 8)) * 8) + (i & 1) * 4;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(a));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(b));
+            s16x8 both;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                both[e] = lo[e];
+                both[4 + e] = hi[e];
+            }
+            return __builtin_bit_cast(Frag<T>, both);
+        } else {
+            const int d = 32 * block + (lane & 31);
+            Frag<T> f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int r = base + 4 * h + (e & 3) + 8 * (e >> 2);
+                f[e] = tile[r * PITCH + (((d >> 2) ^ swizzle(r)) * 4) + (d & 3)];
+            }
+            return f;
+        }
+    }
+};
+
+// Copies ROWS rows into a tile by THREADS threads (thread `gt` of them; whole wavefronts).  Row i comes from
+// base + offset(i), an offset in bytes, or is zeros where offset(i) is kOutside; chunks from element D on are zeros.
+// VEC: 16-byte loads that write LDS themselves (asynchronous: the caller waits); else element by element.
+template <typename T, int PITCH, int ROWS, int THREADS, bool VEC, typename F>
+static __device__ __forceinline__ void stage(T* tile, const T* base, int gt, int d, F&& offset)
+{
+    typedef Tile<T, PITCH> L;
+    constexpr int kChunks = ROWS * L::kChunks;
+    static_assert(kChunks % THREADS == 0, "every thread copies as many chunks");
+    if constexpr (VEC) {
+        const __amdgpu_buffer_rsrc_t rsrc =
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, 0x7fffffff, kBufferFlags);
+#pragma unroll
+        for (int i = 0; i < kChunks / THREADS; i++) {
+            const int at = i * THREADS + gt;
+            const int r = at / L::kChunks, c = (at % L::kChunks) ^ L::swizzle(r);
+            const uint32_t from = offset(r);
+            const uint32_t off = (from == kOutside || c * L::kPerChunk >= d) ? kOutside : from + (uint32_t)c * 16u;
+            T* const dst = tile + (i * THREADS + (gt & ~63)) * L::kPerChunk;  // the wavefront's; lanes follow in order
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)dst, 16, (int)off, 0, 0, 0);
+        }
+    } else {
+#pragma unroll 1
+        for (int i = 0; i < kChunks / THREADS; i++) {
+            const int at = i * THREADS + gt;
+            const int r = at / L::kChunks, c = (at % L::kChunks) ^ L::swizzle(r);
+            const uint32_t from = offset(r);
+            alignas(16) T x[L::kPerChunk];
+#pragma unroll
+            for (int e = 0; e < L::kPerChunk; e++) {
+                const int el = c * L::kPerChunk + e;
+                x[e] = (from == kOutside || el >= d)
+                           ? (T)0.0f
+                           : *reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + from + (uint32_t)el * sizeof(T));
+            }
+            typedef float f32x4 __attribute__((ext_vector_type(4)));
+            *reinterpret_cast<f32x4*>(tile + at * L::kPerChunk) = *reinterpret_cast<const f32x4*>(x);
+        }
+    }
+}
+
+// Eight elements from element `first` of a row on, zeros from element d on.
+template <typename T, bool VEC>
+static __device__ __forceinline__ Frag<T> global_row(const T* row, int first, int d)
+{
+    Frag<T> f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        f[e] = (T)0.0f;
+    }
+    if constexpr (VEC) {
+        // d is a multiple of the 16-byte vector: four elements of FLOAT, eight of the others
+        if constexpr (sizeof(T) == 2) {
+            if (first < d) {
+                f = *reinterpret_cast<const Frag<T>*>(row + first);
+            }
+        } else {
+            typedef float f32x4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                if (first + 4 * i < d) {
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(row + first + 4 * i);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        f[4 * i + e] = x[e];
+                    }
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            if (first + e < d) {
+                f[e] = row[first + e];
+            }
+        }
+    }
+    return f;
+}
+
+// Writes four neighbouring elements of a row from `first` on, none from element d on.
+template <typename T, bool VEC>
+static __device__ __forceinline__ void put4(T* row, int first, int d, float a, float b, float c, float e)
+{
+    const float x[4] = {a, b, c, e};
+    if constexpr (VEC) {
+        if (first < d) {  // d is a multiple of four
+            struct alignas(4 * sizeof(T)) Four {
+                T v[4];
+            } k;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                k.v[i] = (T)x[i];
+            }
+            *reinterpret_cast<Four*>(row + first) = k;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (first + i < d) {
+                row[first + i] = (T)x[i];
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------- visibility
+
+static __device__ __forceinline__ int length_at(const Whole& w, int64_t b, int64_t most)
+{
+    if (w.ptr == nullptr) {
+        return (int)most;
+    }
+    const int64_t v = w.wide != 0 ? ((const int64_t*)w.ptr)[b * w.stride[0]] : (int64_t)((const int32_t*)w.ptr)[b * w.stride[0]];
+    return (int)(v < 0 ? 0 : (v > most ? most : v));
+}
+
+// One sequence: its lengths and the position of query 0.
+struct Sequence {
+    int q_len, kv_len, first;
+};
+
+static __device__ __forceinline__ Sequence sequence_at(const AttentionArgs& a, int64_t b)
+{
+    Sequence s;
+    s.q_len = length_at(a.q_lengths, b, a.tokens);
+    s.kv_len = length_at(a.kv_lengths, b, a.kv_tokens);
+    s.first = s.kv_len - s.q_len;
+    return s;
+}
+
+// Whether a query at position p sees key j < kv_len.
+static __device__ __forceinline__ bool sees(int p, int j, int left, int right, int sinks)
+{
+    return j <= p + right && (j >= p - left || j < sinks);
+}
+
+}  // namespace att
+}  // namespace opscv

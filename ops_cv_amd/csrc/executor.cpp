@@ -183,6 +183,10 @@ aclnnStatus execute_plan(void* workspace, const aclOpExecutor* ex, aclrtStream s
             return ACLNN_ERR_PARAM_NULLPTR;
         }
         e = launch_resize_grad(a, s);
+    } else if (ex->kind >= OpKind::ResidualNorm) {
+        if (const aclnnStatus st = execute_token_plan(workspace, ex, s, api, &e); st != ACLNN_SUCCESS) {
+            return st;
+        }
     } else {
         ResizeArgs a = ex->rs;
         a.x = resolve(ex->in0, workspace);

@@ -30,6 +30,10 @@ inline void* resolve(const PlannedPtr& p, void* workspace)
     return p.in_workspace ? (void*)((char*)workspace + p.ws_offset) : p.direct;
 }
 
+// Launches the operators on token sequences (opscv_tokens.cpp); the launch's own status goes to `e`.
+aclnnStatus execute_token_plan(void* workspace, const aclOpExecutor* ex, hipStream_t stream, const char* api,
+                               hipError_t* e);
+
 // Second phase common to every operator: checks the executor and the workspace, gathers packed inputs,
 // launches the operator, scatters the packed output, frees the executor (always, also on failure).
 aclnnStatus run_executor(void* workspace, uint64_t workspace_size, aclOpExecutor* ex, aclrtStream stream,

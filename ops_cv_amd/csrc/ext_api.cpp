@@ -8,6 +8,7 @@
 #include "acl_types.hpp"
 #include "kernels.hpp"
 #include "options.hpp"
+#include "token_kernels.hpp"
 
 using namespace opscv;
 
@@ -118,6 +119,12 @@ const char* opscvExecutorVariant(const aclOpExecutor* executor)
                 return executor->gs3.interp == 0 ? "gs3d_ndhwc_bilinear" : "gs3d_ndhwc_nearest";
             }
             return executor->gs3.interp == 0 ? "gs3d_bilinear" : "gs3d_nearest";
+        case OpKind::ResidualNorm: return executor->norm.int8 != 0 ? "residual_norm_int8" : "residual_norm";
+        case OpKind::ResidualNormGrad: return "residual_norm_grad";
+        case OpKind::RotaryTable: return "rotary_table";
+        case OpKind::Rotary: return executor->rotary.interleaved != 0 ? "rotary_interleaved" : "rotary_halves";
+        case OpKind::WindowAttention: return attention_variant(executor->attention);
+        case OpKind::WindowAttentionGrad: return "attention_grad";
         default: break;
     }
     return "";

@@ -1,0 +1,550 @@
+// Root-mean-square norm of rows with the residual's addition, its result also in 8 bits, and its gradients.
+//
+//   h = x + r,  rstd = 1 / sqrt(mean(h^2) + eps),  y = h rstd w
+//   8 bits: t = h w, m = max|t|, y = round(t (127 / m)), scale = m rstd / 127
+//
+// rstd cancels in the 8-bit numbers, so they do not depend on the order of the sum of squares; h stays in 32 bits between
+// the addition and the norm (only the `sum` that is handed on is rounded to its type).
+//
+// Bound by memory: every element is read once and written once, so a row stays in registers between its sum and its
+// scaling.  A row belongs to one wavefront (up to 32 elements a lane), to 256 threads, or to 1024; longer rows are read
+// twice.  Statistics are 32-bit sums over a lane's elements, then over lanes, then over wavefronts.
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "token_elem.hpp"
+#include "token_kernels.hpp"
+
+namespace opscv {
+
+using namespace tok;
+
+namespace {
+
+constexpr int kMostPerLane = 32;   // elements of a row that a thread keeps in registers
+constexpr int64_t kMostBlocks = 1 << 20;  // more rows than these take are walked
+constexpr int kPartialRows = 512;  // rows of partial sums of the weight's gradient: two workgroups per CU
+
+dim3 grid(int64_t blocks) { return dim3((unsigned)(blocks < kMostBlocks ? blocks : kMostBlocks)); }
+
+// Sum (and, with `most`, largest value) over the threads of a row: THREADS of them, 64 or a whole workgroup.  `slot`
+// alternates between calls, so that one barrier a call is enough.
+template <int THREADS>
+__device__ __forceinline__ void row_reduce(float& sum, float* most, float (*shared)[2][16], int slot)
+{
+    sum = wave_sum(sum);
+    if (most != nullptr) {
+        *most = wave_larger(*most);
+    }
+    if constexpr (THREADS > 64) {
+        const int wave = (int)threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) {
+            shared[slot][0][wave] = sum;
+            if (most != nullptr) {
+                shared[slot][1][wave] = *most;
+            }
+        }
+        __syncthreads();
+        sum = 0.0f;
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < THREADS / 64; i++) {
+            sum += shared[slot][0][i];
+            if (most != nullptr) {
+                m = larger(m, shared[slot][1][i]);
+            }
+        }
+        if (most != nullptr) {
+            *most = m;
+        }
+    }
+}
+
+template <typename T, typename W, bool INT8, int VEC>
+__device__ __forceinline__ void put_row_part(const NormArgs& a, int64_t row, int64_t c, const float (&h)[VEC], float rstd,
+                                             float step)
+{
+    float w[VEC], y[VEC];
+    load<W, VEC>((const W*)a.weight + c, w);
+    if constexpr (INT8) {
+        Pack<int8_t, VEC> k;
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+            // step is 0 for rows without a finite range; |t * step| is at most 127 and a rounding
+            const float q = rintf(h[i] * w[i] * step);
+            k.v[i] = step == 0.0f ? (int8_t)0 : (int8_t)(int)fminf(fmaxf(q, -127.0f), 127.0f);
+        }
+        *reinterpret_cast<Pack<int8_t, VEC>*>((int8_t*)a.y.ptr + row * a.y.row_stride + c) = k;
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+            y[i] = h[i] * w[i] * rstd;
+        }
+        store<T, VEC>((T*)a.y.ptr + row * a.y.row_stride + c, y);
+    }
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void get_row_part(const NormArgs& a, int64_t row, int64_t c, float (&h)[VEC])
+{
+    load<T, VEC>((const T*)a.x.ptr + row * a.x.row_stride + c, h);
+    if (a.residual.ptr != nullptr) {
+        float r[VEC];
+        load<T, VEC>((const T*)a.residual.ptr + row * a.residual.row_stride + c, r);
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+            h[i] += r[i];
+        }
+    }
+}
+
+// step of the 8-bit numbers and what a row's scale is; 0 and NaN where the row holds a NaN or an infinity
+__device__ __forceinline__ float int8_step(float most, float rstd, float* scale)
+{
+    const bool finite = most < INFINITY;  // false for NaN too
+    *scale = finite ? most * rstd / 127.0f : NAN;
+    return (finite && most > 0.0f) ? 127.0f / most : 0.0f;
+}
+
+// THREADS per row; a workgroup is 256 threads, or THREADS where that is more.  NV vectors of VEC elements a thread.
+template <typename T, typename W, bool INT8, int THREADS, int NV, int VEC>
+__global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void norm_kernel(NormArgs a)
+{
+    constexpr int kRows = THREADS >= 256 ? 1 : 256 / THREADS;
+    __shared__ float shared[2][2][16];
+    const int lane = (int)threadIdx.x % THREADS;
+    int slot = 0;
+    // where a barrier follows (THREADS >= 256), a workgroup has one row and all its threads make as many turns
+    for (int64_t row = (int64_t)blockIdx.x * kRows + (int)threadIdx.x / THREADS; row < a.rows;
+         row += (int64_t)gridDim.x * kRows) {
+        float h[NV][VEC], sum = 0.0f, most = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const int64_t c = ((int64_t)j * THREADS + lane) * VEC;
+            if (c < a.width) {
+                get_row_part<T, VEC>(a, row, c, h[j]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; i++) {
+                    h[j][i] = 0.0f;
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const int64_t c = ((int64_t)j * THREADS + lane) * VEC;
+#pragma unroll
+            for (int i = 0; i < VEC; i++) {
+                sum += h[j][i] * h[j][i];
+            }
+            if (c < a.width) {
+                if (a.sum.ptr != nullptr) {
+                    store<T, VEC>((T*)a.sum.ptr + row * a.sum.row_stride + c, h[j]);
+                }
+                if constexpr (INT8) {
+                    float w[VEC];
+                    load<W, VEC>((const W*)a.weight + c, w);
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) {
+                        most = larger(most, fabsf(h[j][i] * w[i]));
+                    }
+                }
+            }
+        }
+        row_reduce<THREADS>(sum, INT8 ? &most : nullptr, shared, slot);
+        slot ^= 1;
+        const float rstd = 1.0f / sqrtf(sum / (float)a.width + a.eps);
+        float scale = 0.0f;
+        const float step = INT8 ? int8_step(most, rstd, &scale) : 0.0f;
+        if (lane == 0) {
+            if (a.rstd != nullptr) {
+                a.rstd[row] = rstd;
+            }
+            if (INT8) {
+                a.scale[row] = scale;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const int64_t c = ((int64_t)j * THREADS + lane) * VEC;
+            if (c < a.width) {
+                put_row_part<T, W, INT8, VEC>(a, row, c, h[j], rstd, step);
+            }
+        }
+    }
+}
+
+// Rows longer than 1024 threads hold: read once for the statistics and once more for the result (`sum` is written in the
+// second pass, since it may be x).
+template <typename T, typename W, bool INT8, int VEC>
+__global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a)
+{
+    __shared__ float shared[2][2][16];
+    int slot = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    float sum = 0.0f, most = 0.0f;
+    for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.width; c += 1024 * VEC) {
+        float h[VEC], w[VEC];
+        get_row_part<T, VEC>(a, row, c, h);
+        load<W, VEC>((const W*)a.weight + c, w);
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+            sum += h[i] * h[i];
+            most = larger(most, fabsf(h[i] * w[i]));
+        }
+    }
+    row_reduce<1024>(sum, INT8 ? &most : nullptr, shared, slot);
+    slot ^= 1;
+    const float rstd = 1.0f / sqrtf(sum / (float)a.width + a.eps);
+    float scale = 0.0f;
+    const float step = INT8 ? int8_step(most, rstd, &scale) : 0.0f;
+    if (threadIdx.x == 0) {
+        if (a.rstd != nullptr) {
+            a.rstd[row] = rstd;
+        }
+        if (INT8) {
+            a.scale[row] = scale;
+        }
+    }
+    for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.width; c += 1024 * VEC) {
+        float h[VEC];
+        get_row_part<T, VEC>(a, row, c, h);
+        if (a.sum.ptr != nullptr) {
+            store<T, VEC>((T*)a.sum.ptr + row * a.sum.row_stride + c, h);
+        }
+        put_row_part<T, W, INT8, VEC>(a, row, c, h, rstd, step);
+    }
+    }
+}
+
+template <typename T, typename W, bool INT8, int VEC>
+hipError_t run_norm(const NormArgs& a, hipStream_t stream)
+{
+    constexpr int kVectors = kMostPerLane / VEC;
+    const int64_t vectors = (a.width + VEC - 1) / VEC;
+    if (vectors <= 64 * kVectors / 2) {
+        hipLaunchKernelGGL((norm_kernel<T, W, INT8, 64, kVectors / 2, VEC>), grid((a.rows + 3) / 4), dim3(256),
+                           0, stream, a);
+    } else if (vectors <= 256 * kVectors / 2) {
+        hipLaunchKernelGGL((norm_kernel<T, W, INT8, 256, kVectors / 2, VEC>), grid(a.rows), dim3(256), 0, stream,
+                           a);
+    } else if (vectors <= 256 * kVectors) {
+        hipLaunchKernelGGL((norm_kernel<T, W, INT8, 256, kVectors, VEC>), grid(a.rows), dim3(256), 0, stream, a);
+    } else if (vectors <= 1024 * kVectors) {
+        hipLaunchKernelGGL((norm_kernel<T, W, INT8, 1024, kVectors, VEC>), grid(a.rows), dim3(1024), 0, stream,
+                           a);
+    } else {
+        hipLaunchKernelGGL((norm_long_kernel<T, W, INT8, VEC>), grid(a.rows), dim3(1024), 0, stream, a);
+    }
+    return hipGetLastError();
+}
+
+template <typename T, typename W>
+hipError_t run_norm_type(const NormArgs& a, hipStream_t stream)
+{
+    constexpr int kVec = 16 / (int)sizeof(T);
+    const int e = (int)sizeof(T), ye = a.int8 != 0 ? 1 : e;
+    // vectors where every row starts on one, single elements otherwise
+    const bool vectors = a.width % kVec == 0 && aligned(a.x.ptr, a.x.row_stride, e, 16) &&
+                         aligned(a.residual.ptr, a.residual.row_stride, e, 16) &&
+                         aligned(a.sum.ptr, a.sum.row_stride, e, 16) &&
+                         aligned(a.y.ptr, a.y.row_stride, ye, kVec * ye) &&
+                         aligned(a.weight, 0, 1, kVec * (int)sizeof(W));
+    if (a.int8 != 0) {
+        return vectors ? run_norm<T, W, true, kVec>(a, stream) : run_norm<T, W, true, 1>(a, stream);
+    }
+    return vectors ? run_norm<T, W, false, kVec>(a, stream) : run_norm<T, W, false, 1>(a, stream);
+}
+
+// ------------------------------------------------------------------------------------------------------ gradients
+
+// Gradient of the rows, and of the weight's columns over the rows of one workgroup, which it adds up in registers and
+// leaves in its row of `partial`.  THREADS per row; wavefronts of 64-thread rows join their sums through LDS.
+template <typename T, typename W, int THREADS, int NV, int VEC, bool WEIGHT>
+__global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void norm_grad_kernel(NormGradArgs a)
+{
+    constexpr int kRows = THREADS >= 256 ? 1 : 256 / THREADS;
+    __shared__ float shared[2][2][16];
+    const int lane = (int)threadIdx.x % THREADS;
+    float w[NV][VEC], total[NV][VEC];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int64_t c = ((int64_t)j * THREADS + lane) * VEC;
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+            total[j][i] = w[j][i] = 0.0f;
+        }
+        if (c < a.width) {
+            load<W, VEC>((const W*)a.weight + c, w[j]);
+        }
+    }
+    int slot = 0;
+    // every thread of a workgroup makes as many turns: the barrier of row_reduce is met by all (THREADS >= 256: one row
+    // a turn; 64: no barrier)
+    for (int64_t row = (int64_t)blockIdx.x * kRows + (int)threadIdx.x / THREADS; row < a.rows;
+         row += (int64_t)gridDim.x * kRows) {
+        const float rstd = a.rstd[row];
+        float n[NV][VEC], g[NV][VEC], along = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const int64_t c = ((int64_t)j * THREADS + lane) * VEC;
+            if (c < a.width) {
+                load<T, VEC>((const T*)a.sum.ptr + row * a.sum.row_stride + c, n[j]);
+                load<T, VEC>((const T*)a.grad_y.ptr + row * a.grad_y.row_stride + c, g[j]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; i++) {
+                    n[j][i] = g[j][i] = 0.0f;
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+#pragma unroll
+            for (int i = 0; i < VEC; i++) {
+                n[j][i] *= rstd;
+                if (WEIGHT) {
+                    total[j][i] += g[j][i] * n[j][i];
+                }
+                g[j][i] *= w[j][i];
+                along += g[j][i] * n[j][i];
+            }
+        }
+        row_reduce<THREADS>(along, nullptr, shared, slot);
+        slot ^= 1;
+        along /= (float)a.width;
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const int64_t c = ((int64_t)j * THREADS + lane) * VEC;
+            if (c < a.width) {
+                float s[VEC] = {0.0f};
+                if (a.grad_sum.ptr != nullptr) {
+                    load<T, VEC>((const T*)a.grad_sum.ptr + row * a.grad_sum.row_stride + c, s);
+                }
+#pragma unroll
+                for (int i = 0; i < VEC; i++) {
+                    s[i] += (g[j][i] - n[j][i] * along) * rstd;
+                }
+                store<T, VEC>((T*)a.grad_x.ptr + row * a.grad_x.row_stride + c, s);
+            }
+        }
+    }
+    if constexpr (WEIGHT) {
+        __shared__ float joined[kRows > 1 ? THREADS * VEC : 1];
+        float* const out = a.partial + (int64_t)blockIdx.x * a.width;
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const int64_t c = ((int64_t)j * THREADS + lane) * VEC;
+            if constexpr (kRows > 1) {
+                for (int turn = 0; turn < kRows; turn++) {  // the wavefronts add in order
+                    if ((int)threadIdx.x / THREADS == turn) {
+#pragma unroll
+                        for (int i = 0; i < VEC; i++) {
+                            float& slot_sum = joined[i * THREADS + lane];
+                            slot_sum = turn == 0 ? total[j][i] : slot_sum + total[j][i];
+                            if (turn == kRows - 1 && c + i < a.width) {
+                                out[c + i] = slot_sum;
+                            }
+                        }
+                    }
+                    __syncthreads();
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; i++) {
+                    if (c + i < a.width) {
+                        out[c + i] = total[j][i];
+                    }
+                }
+            }
+        }
+    }
+}
+
+// Rows longer than 1024 threads hold, read twice: the sum along the row, then the gradient.  The weight's gradient comes
+// from norm_weight_long_kernel.
+template <typename T, typename W, int VEC>
+__global__ __launch_bounds__(1024) void norm_grad_long_kernel(NormGradArgs a)
+{
+    __shared__ float shared[2][2][16];
+    int slot = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const float rstd = a.rstd[row];
+    const T* const sum = (const T*)a.sum.ptr + row * a.sum.row_stride;
+    const T* const gy = (const T*)a.grad_y.ptr + row * a.grad_y.row_stride;
+    float along = 0.0f;
+    for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.width; c += 1024 * VEC) {
+        float n[VEC], g[VEC], w[VEC];
+        load<T, VEC>(sum + c, n);
+        load<T, VEC>(gy + c, g);
+        load<W, VEC>((const W*)a.weight + c, w);
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+            along += g[i] * w[i] * (n[i] * rstd);
+        }
+    }
+    row_reduce<1024>(along, nullptr, shared, slot);
+    slot ^= 1;
+    along /= (float)a.width;
+    for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.width; c += 1024 * VEC) {
+        float n[VEC], g[VEC], w[VEC], s[VEC] = {0.0f};
+        load<T, VEC>(sum + c, n);
+        load<T, VEC>(gy + c, g);
+        load<W, VEC>((const W*)a.weight + c, w);
+        if (a.grad_sum.ptr != nullptr) {
+            load<T, VEC>((const T*)a.grad_sum.ptr + row * a.grad_sum.row_stride + c, s);
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; i++) {
+            s[i] += (g[i] * w[i] - n[i] * rstd * along) * rstd;
+        }
+        store<T, VEC>((T*)a.grad_x.ptr + row * a.grad_x.row_stride + c, s);
+    }
+    }
+}
+
+// One column a thread, every gridDim.y-th row: before the rows' gradient is written, since that may be gradY itself.
+template <typename T>
+__global__ __launch_bounds__(256) void norm_weight_long_kernel(NormGradArgs a)
+{
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c >= a.width) {
+        return;
+    }
+    float total = 0.0f;
+    for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+        total += (float)((const T*)a.grad_y.ptr)[row * a.grad_y.row_stride + c] *
+                 ((float)((const T*)a.sum.ptr)[row * a.sum.row_stride + c] * a.rstd[row]);
+    }
+    a.partial[(int64_t)blockIdx.y * a.width + c] = total;
+}
+
+// Sum of the rows of `partial`: 32 columns a workgroup, every eighth row a thread, joined in order.
+template <typename W>
+__global__ __launch_bounds__(256) void norm_weight_kernel(const float* __restrict__ partial, int64_t rows, int64_t width,
+                                                          W* __restrict__ out)
+{
+    __shared__ float shared[8][32];
+    const int column = (int)threadIdx.x & 31, part = (int)threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 32 + column;
+    float total = 0.0f;
+    if (c < width) {
+#pragma unroll 8
+        for (int64_t r = part; r < rows; r += 8) {
+            total += partial[r * width + c];
+        }
+    }
+    shared[part][column] = total;
+    __syncthreads();
+    if (part == 0 && c < width) {
+#pragma unroll
+        for (int i = 1; i < 8; i++) {
+            total += shared[i][column];
+        }
+        out[c] = (W)total;
+    }
+}
+
+template <typename T, typename W, int THREADS, int NV, int VEC>
+void launch_norm_grad(const NormGradArgs& a, int64_t blocks, hipStream_t stream)
+{
+    if (a.grad_weight != nullptr) {
+        hipLaunchKernelGGL((norm_grad_kernel<T, W, THREADS, NV, VEC, true>), dim3((unsigned)blocks),
+                           dim3(THREADS > 256 ? THREADS : 256), 0, stream, a);
+    } else {
+        hipLaunchKernelGGL((norm_grad_kernel<T, W, THREADS, NV, VEC, false>), dim3((unsigned)blocks),
+                           dim3(THREADS > 256 ? THREADS : 256), 0, stream, a);
+    }
+}
+
+template <typename T, typename W, int VEC>
+hipError_t run_norm_grad(const NormGradArgs& a, hipStream_t stream)
+{
+    constexpr int kVectors = kMostPerLane / VEC;
+    const int64_t vectors = (a.width + VEC - 1) / VEC;
+    const int64_t partials = norm_grad_partials(a);
+    const auto blocks = [&](int64_t rows_each) {
+        const int64_t most = (a.rows + rows_each - 1) / rows_each;
+        return a.grad_weight != nullptr ? partials : (most < kMostBlocks ? most : kMostBlocks);
+    };
+    if (a.rows > 0 || a.grad_weight != nullptr) {
+        if (vectors <= 64 * kVectors / 2) {
+            launch_norm_grad<T, W, 64, kVectors / 2, VEC>(a, blocks(4), stream);
+        } else if (vectors <= 256 * kVectors / 2) {
+            launch_norm_grad<T, W, 256, kVectors / 2, VEC>(a, blocks(1), stream);
+        } else if (vectors <= 256 * kVectors) {
+            launch_norm_grad<T, W, 256, kVectors, VEC>(a, blocks(1), stream);
+        } else if (vectors <= 1024 * kVectors) {
+            launch_norm_grad<T, W, 1024, kVectors, VEC>(a, blocks(1), stream);
+        } else {
+            if (a.grad_weight != nullptr) {
+                hipLaunchKernelGGL((norm_weight_long_kernel<T>), dim3((unsigned)((a.width + 255) / 256), (unsigned)partials),
+                                   dim3(256), 0, stream, a);
+            }
+            if (a.rows > 0) {
+                hipLaunchKernelGGL((norm_grad_long_kernel<T, W, VEC>), grid(a.rows), dim3(1024), 0, stream, a);
+            }
+        }
+    }
+    if (a.grad_weight != nullptr) {
+        hipLaunchKernelGGL((norm_weight_kernel<W>), dim3((unsigned)((a.width + 31) / 32)), dim3(256), 0, stream, a.partial,
+                           partials, a.width, (W*)a.grad_weight);
+    }
+    return hipGetLastError();
+}
+
+template <typename T, typename W>
+hipError_t run_norm_grad_type(const NormGradArgs& a, hipStream_t stream)
+{
+    constexpr int kVec = 16 / (int)sizeof(T);
+    const int e = (int)sizeof(T);
+    const bool vectors = a.width % kVec == 0 && aligned(a.grad_y.ptr, a.grad_y.row_stride, e, 16) &&
+                         aligned(a.grad_sum.ptr, a.grad_sum.row_stride, e, 16) &&
+                         aligned(a.sum.ptr, a.sum.row_stride, e, 16) &&
+                         aligned(a.grad_x.ptr, a.grad_x.row_stride, e, 16) &&
+                         aligned(a.weight, 0, 1, kVec * (int)sizeof(W));
+    return vectors ? run_norm_grad<T, W, kVec>(a, stream) : run_norm_grad<T, W, 1>(a, stream);
+}
+
+// f(T, W) by the operands' types
+template <typename F>
+hipError_t by_type(int elem, int weight_float, F&& f)
+{
+    switch ((Elem)elem) {
+        case Elem::F32: return f((float*)nullptr, (float*)nullptr);
+        case Elem::F16: return weight_float != 0 ? f((_Float16*)nullptr, (float*)nullptr) : f((_Float16*)nullptr, (_Float16*)nullptr);
+        default: return weight_float != 0 ? f((__bf16*)nullptr, (float*)nullptr) : f((__bf16*)nullptr, (__bf16*)nullptr);
+    }
+}
+
+}  // namespace
+
+int64_t norm_grad_partials(const NormGradArgs& a)
+{
+    // a workgroup takes four rows at a time at most; one row of partial sums even where there are no rows
+    const int64_t groups = (a.rows + 3) / 4;
+    return groups < 1 ? 1 : (groups < kPartialRows ? groups : kPartialRows);
+}
+
+hipError_t launch_residual_norm(const NormArgs& a, hipStream_t stream)
+{
+    if (a.rows < 1 || a.width < 1) {
+        return hipErrorInvalidValue;
+    }
+    return by_type(a.elem, a.weight_float, [&](auto* t, auto* w) {
+        return run_norm_type<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(w)>>(a, stream);
+    });
+}
+
+hipError_t launch_residual_norm_grad(const NormGradArgs& a, hipStream_t stream)
+{
+    if (a.width < 1 || (a.grad_weight != nullptr && a.partial == nullptr)) {
+        return hipErrorInvalidValue;
+    }
+    return by_type(a.elem, a.weight_float, [&](auto* t, auto* w) {
+        return run_norm_grad_type<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(w)>>(a, stream);
+    });
+}
+
+}  // namespace opscv

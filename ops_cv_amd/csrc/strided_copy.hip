@@ -83,6 +83,9 @@ hipError_t launch_strided_copy(const StridedView& v, void* contiguous, int elem_
     if (elem_bytes == 2) {
         return run<uint16_t>(v, contiguous, gather, stream);
     }
+    if (elem_bytes == 1) {
+        return run<uint8_t>(v, contiguous, gather, stream);
+    }
     return hipErrorInvalidValue;
 }
 

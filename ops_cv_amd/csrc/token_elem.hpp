@@ -1,0 +1,65 @@
+// Elements of the operators on token sequences: vectors of up to 16 bytes, read and written whole, computed in 32 bits.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace opscv {
+namespace tok {
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Pack {
+    T v[N];
+};
+
+template <typename T, int N>
+static __device__ __forceinline__ void load(const T* p, float (&x)[N])
+{
+    const Pack<T, N> k = *reinterpret_cast<const Pack<T, N>*>(p);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        x[i] = (float)k.v[i];
+    }
+}
+
+template <typename T, int N>
+static __device__ __forceinline__ void store(T* p, const float (&x)[N])
+{
+    Pack<T, N> k;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        k.v[i] = (T)x[i];
+    }
+    *reinterpret_cast<Pack<T, N>*>(p) = k;
+}
+
+static __device__ __forceinline__ float wave_sum(float v)
+{
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        v += __shfl_xor(v, d, 64);
+    }
+    return v;
+}
+
+// the larger one; NaN where either is
+static __device__ __forceinline__ float larger(float a, float b) { return (a > b || a != a) ? a : b; }
+
+static __device__ __forceinline__ float wave_larger(float v)
+{
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        v = larger(v, __shfl_xor(v, d, 64));
+    }
+    return v;
+}
+
+// whether `p` and a step of `stride` elements keep vectors of `bytes` aligned
+inline bool aligned(const void* p, int64_t stride, int elem_bytes, int bytes)
+{
+    return reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes == 0 && stride * elem_bytes % bytes == 0;
+}
+
+}  // namespace tok
+}  // namespace opscv

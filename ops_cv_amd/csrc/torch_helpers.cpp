@@ -26,6 +26,7 @@
 #include "aclnn_resize.h"
 #include "aclnn_upsample_bilinear_2d.h"
 #include "aclnn_upsample_bilinear_2d_backward.h"
+#include "opscv_tokens.h"
 
 namespace {
 
@@ -220,8 +221,9 @@ public:
     // the call allocated
     aclTensor* handle(const at::Tensor& t, aclFormat fmt = ACL_FORMAT_ND, bool made = false)
     {
-        if (!t.is_cuda()) {
-            PyErr_SetString(PyExc_RuntimeError, "ops_cv_amd needs device tensors: there is no CPU path");
+        if (!t.is_cuda() || count_ == kMost) {
+            PyErr_SetString(PyExc_RuntimeError, t.is_cuda() ? "more tensors than a call holds"
+                                                            : "ops_cv_amd needs device tensors: there is no CPU path");
             throw Raised();
         }
         // a copy-on-write tensor gets memory of its own first: an output must not be written through into the tensor it
@@ -239,7 +241,8 @@ public:
 
 private:
     const Queue& queue_;
-    aclTensor* handles_[5];
+    static constexpr int kMost = 16;
+    aclTensor* handles_[kMost];
     int count_ = 0;
 };
 
@@ -537,6 +540,230 @@ PyObject* upsample_bilinear2d_backward(PyObject*, PyObject* const* a, Py_ssize_t
     });
 }
 
+// ------------------------------------------------------------------------------------- operators on token sequences
+
+// The caller's tensor, or nothing where it is None.
+at::Tensor optional_arg(PyObject* o) { return o == Py_None ? at::Tensor() : tensor_arg(o); }
+
+aclTensor* optional_handle(Call& c, const at::Tensor& t, bool made = false)
+{
+    return t.defined() ? c.handle(t, ACL_FORMAT_ND, made) : nullptr;
+}
+
+// The caller's output, or a new one; nothing where it is neither given nor wanted.
+at::Tensor wanted_out(PyObject* out, bool wanted, const at::Tensor& like, at::IntArrayRef sizes, at::ScalarType type)
+{
+    if (out != Py_None) {
+        return tensor_arg(out);
+    }
+    return wanted ? at::empty(sizes, like.options().memory_format(at::MemoryFormat::Contiguous).dtype(type))
+                  : at::Tensor();
+}
+
+PyObject* wrapped(const at::Tensor& t)
+{
+    if (!t.defined()) {
+        Py_RETURN_NONE;
+    }
+    return THPVariable_Wrap(t);
+}
+
+template <typename... T>
+PyObject* tuple_of(const T&... tensors)
+{
+    PyObject* all = PyTuple_New(sizeof...(tensors));
+    if (all == nullptr) {
+        throw Raised();
+    }
+    Py_ssize_t i = 0;
+    (PyTuple_SET_ITEM(all, i++, wrapped(tensors)), ...);
+    return all;
+}
+
+at::IntArrayRef leading(const at::Tensor& x)
+{
+    if (x.dim() < 1) {
+        PyErr_SetString(PyExc_ValueError, "rows have one dimension or more");
+        throw Raised();
+    }
+    return x.sizes().slice(0, x.dim() - 1);
+}
+
+// (x, weight, residual, eps, int8, need_rstd, out, scale, sum, rstd, workspace, stream)
+PyObject* residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    return guarded(n, 12, [&]() -> PyObject* {
+        const at::Tensor& x = tensor_arg(a[0]);
+        const at::Tensor& w = tensor_arg(a[1]);
+        const at::Tensor r = optional_arg(a[2]);
+        const double eps = float_arg(a[3]);
+        const bool int8 = bool_arg(a[4]), need_rstd = bool_arg(a[5]);
+        const Queue queue(a[11], x);
+        const at::Tensor y = wanted_out(a[6], true, x, x.sizes(), int8 ? at::kChar : x.scalar_type());
+        const at::Tensor scale = wanted_out(a[7], int8, x, leading(x), at::kFloat);
+        const at::Tensor sum = wanted_out(a[8], r.defined(), x, x.sizes(), x.scalar_type());
+        const at::Tensor rstd = wanted_out(a[9], need_rstd, x, leading(x), at::kFloat);
+        Call c(queue);
+        aclTensor *hx = c.handle(x), *hr = optional_handle(c, r), *hw = c.handle(w),
+                  *hy = c.handle(y, ACL_FORMAT_ND, a[6] == Py_None), *hs = optional_handle(c, scale, a[7] == Py_None),
+                  *hh = optional_handle(c, sum, a[8] == Py_None), *hv = optional_handle(c, rstd, a[9] == Py_None);
+        uint64_t ws = 0;
+        aclOpExecutor* ex = nullptr;
+        const aclnnStatus st = opscvResidualNormGetWorkspaceSize(hx, hr, hw, eps, hy, hs, hh, hv, &ws, &ex);
+        if (st != ACLNN_SUCCESS) {
+            raise_status("opscvResidualNormGetWorkspaceSize", st);
+        }
+        launch("opscvResidualNorm", opscvResidualNorm, ws, ex, x, a[10], queue);
+        return int8 ? tuple_of(y, scale, sum, rstd) : tuple_of(y, sum, rstd);
+    });
+}
+
+// (grad_y, sum, weight, rstd, grad_sum, need_weight, grad_x, grad_weight, workspace, stream)
+PyObject* residual_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    return guarded(n, 10, [&]() -> PyObject* {
+        const at::Tensor& gy = tensor_arg(a[0]);
+        const at::Tensor& h = tensor_arg(a[1]);
+        const at::Tensor& w = tensor_arg(a[2]);
+        const at::Tensor& rstd = tensor_arg(a[3]);
+        const at::Tensor gs = optional_arg(a[4]);
+        const Queue queue(a[9], h);
+        const at::Tensor gx = wanted_out(a[6], true, h, h.sizes(), h.scalar_type());
+        const at::Tensor gw = wanted_out(a[7], bool_arg(a[5]), w, w.sizes(), w.scalar_type());
+        Call c(queue);
+        aclTensor *hgy = c.handle(gy), *hgs = optional_handle(c, gs), *hh = c.handle(h), *hw = c.handle(w),
+                  *hr = c.handle(rstd), *hgx = c.handle(gx, ACL_FORMAT_ND, a[6] == Py_None),
+                  *hgw = optional_handle(c, gw, a[7] == Py_None);
+        uint64_t ws = 0;
+        aclOpExecutor* ex = nullptr;
+        const aclnnStatus st = opscvResidualNormBackwardGetWorkspaceSize(hgy, hgs, hh, hw, hr, hgx, hgw, &ws, &ex);
+        if (st != ACLNN_SUCCESS) {
+            raise_status("opscvResidualNormBackwardGetWorkspaceSize", st);
+        }
+        launch("opscvResidualNormBackward", opscvResidualNormBackward, ws, ex, h, a[8], queue);
+        return tuple_of(gx, gw);
+    });
+}
+
+// (like, positions, rot, base, scaling, factor, original_length, magnitude, out, workspace, stream): `like` is any tensor
+// on the table's device
+PyObject* rotary_table(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    return guarded(n, 11, [&]() -> PyObject* {
+        const at::Tensor& like = tensor_arg(a[0]);
+        const int64_t sizes[2] = {int_arg(a[1]), int_arg(a[2])};
+        const Queue queue(a[10], like);
+        const at::Tensor table = wanted_out(a[8], true, like, sizes, at::kFloat);
+        Call c(queue);
+        aclTensor* ht = c.handle(table, ACL_FORMAT_ND, a[8] == Py_None);
+        uint64_t ws = 0;
+        aclOpExecutor* ex = nullptr;
+        const aclnnStatus st = opscvRotaryTableGetWorkspaceSize(float_arg(a[3]), int_arg(a[4]), float_arg(a[5]),
+                                                                int_arg(a[6]), float_arg(a[7]), ht, &ws, &ex);
+        if (st != ACLNN_SUCCESS) {
+            raise_status("opscvRotaryTableGetWorkspaceSize", st);
+        }
+        launch("opscvRotaryTable", opscvRotaryTable, ws, ex, like, a[9], queue);
+        return wrapped(table);
+    });
+}
+
+// (query, key, table, positions, interleaved, inverse, query_out, key_out, workspace, stream)
+PyObject* rotary(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    return guarded(n, 10, [&]() -> PyObject* {
+        const at::Tensor& q = tensor_arg(a[0]);
+        const at::Tensor k = optional_arg(a[1]);
+        const at::Tensor& table = tensor_arg(a[2]);
+        const at::Tensor positions = optional_arg(a[3]);
+        const bool interleaved = bool_arg(a[4]), inverse = bool_arg(a[5]);
+        const Queue queue(a[9], q);
+        const at::Tensor qo = wanted_out(a[6], true, q, q.sizes(), q.scalar_type());
+        const at::Tensor ko = wanted_out(a[7], k.defined(), q, k.defined() ? k.sizes() : q.sizes(), q.scalar_type());
+        Call c(queue);
+        aclTensor *hq = c.handle(q), *hk = optional_handle(c, k), *hp = optional_handle(c, positions),
+                  *ht = c.handle(table), *hqo = c.handle(qo, ACL_FORMAT_ND, a[6] == Py_None),
+                  *hko = optional_handle(c, ko, a[7] == Py_None);
+        uint64_t ws = 0;
+        aclOpExecutor* ex = nullptr;
+        const aclnnStatus st = opscvRotaryGetWorkspaceSize(hq, hk, hp, ht, interleaved, inverse, hqo, hko, &ws, &ex);
+        if (st != ACLNN_SUCCESS) {
+            raise_status("opscvRotaryGetWorkspaceSize", st);
+        }
+        launch("opscvRotary", opscvRotary, ws, ex, q, a[8], queue);
+        return tuple_of(qo, ko);
+    });
+}
+
+// (query, key, value, scale, left, right, sinks, q_lengths, kv_lengths, need_lse, out, lse, workspace, stream)
+PyObject* window_attention(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    return guarded(n, 14, [&]() -> PyObject* {
+        const at::Tensor& q = tensor_arg(a[0]);
+        const at::Tensor& k = tensor_arg(a[1]);
+        const at::Tensor& v = tensor_arg(a[2]);
+        const double scale = float_arg(a[3]);
+        const int64_t left = int_arg(a[4]), right = int_arg(a[5]), sinks = int_arg(a[6]);
+        const at::Tensor ql = optional_arg(a[7]), kl = optional_arg(a[8]);
+        const bool need_lse = bool_arg(a[9]);
+        const Queue queue(a[13], q);
+        const at::Tensor out = wanted_out(a[10], true, q, q.sizes(), q.scalar_type());
+        at::Tensor lse;
+        if (need_lse || a[11] != Py_None) {
+            lse = wanted_out(a[11], true, q, Sizes{size_of(q, 0), size_of(q, 2), size_of(q, 1)}, at::kFloat);
+        }
+        Call c(queue);
+        aclTensor *hq = c.handle(q), *hk = c.handle(k), *hv = c.handle(v), *hql = optional_handle(c, ql),
+                  *hkl = optional_handle(c, kl), *ho = c.handle(out, ACL_FORMAT_ND, a[10] == Py_None),
+                  *hl = optional_handle(c, lse, a[11] == Py_None);
+        uint64_t ws = 0;
+        aclOpExecutor* ex = nullptr;
+        const aclnnStatus st =
+            opscvWindowAttentionGetWorkspaceSize(hq, hk, hv, hql, hkl, scale, left, right, sinks, ho, hl, &ws, &ex);
+        if (st != ACLNN_SUCCESS) {
+            raise_status("opscvWindowAttentionGetWorkspaceSize", st);
+        }
+        launch("opscvWindowAttention", opscvWindowAttention, ws, ex, q, a[12], queue);
+        return tuple_of(out, lse);
+    });
+}
+
+// (grad_out, query, key, value, out, lse, scale, left, right, sinks, q_lengths, kv_lengths, grad_query, grad_key,
+// grad_value, workspace, stream)
+PyObject* window_attention_backward(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    return guarded(n, 17, [&]() -> PyObject* {
+        const at::Tensor& go = tensor_arg(a[0]);
+        const at::Tensor& q = tensor_arg(a[1]);
+        const at::Tensor& k = tensor_arg(a[2]);
+        const at::Tensor& v = tensor_arg(a[3]);
+        const at::Tensor& out = tensor_arg(a[4]);
+        const at::Tensor& lse = tensor_arg(a[5]);
+        const double scale = float_arg(a[6]);
+        const int64_t left = int_arg(a[7]), right = int_arg(a[8]), sinks = int_arg(a[9]);
+        const at::Tensor ql = optional_arg(a[10]), kl = optional_arg(a[11]);
+        const Queue queue(a[16], q);
+        const at::Tensor gq = wanted_out(a[12], true, q, q.sizes(), q.scalar_type());
+        const at::Tensor gk = wanted_out(a[13], true, k, k.sizes(), k.scalar_type());
+        const at::Tensor gv = wanted_out(a[14], true, v, v.sizes(), v.scalar_type());
+        Call c(queue);
+        aclTensor *hgo = c.handle(go), *hq = c.handle(q), *hk = c.handle(k), *hv = c.handle(v), *ho = c.handle(out),
+                  *hl = c.handle(lse), *hql = optional_handle(c, ql), *hkl = optional_handle(c, kl),
+                  *hgq = c.handle(gq, ACL_FORMAT_ND, a[12] == Py_None),
+                  *hgk = c.handle(gk, ACL_FORMAT_ND, a[13] == Py_None),
+                  *hgv = c.handle(gv, ACL_FORMAT_ND, a[14] == Py_None);
+        uint64_t ws = 0;
+        aclOpExecutor* ex = nullptr;
+        const aclnnStatus st = opscvWindowAttentionBackwardGetWorkspaceSize(
+            hgo, hq, hk, hv, ho, hl, hql, hkl, scale, left, right, sinks, hgq, hgk, hgv, &ws, &ex);
+        if (st != ACLNN_SUCCESS) {
+            raise_status("opscvWindowAttentionBackwardGetWorkspaceSize", st);
+        }
+        launch("opscvWindowAttentionBackward", opscvWindowAttentionBackward, ws, ex, q, a[15], queue);
+        return tuple_of(gq, gk, gv);
+    });
+}
+
 // (AclnnError): the class of the errors raised for a status other than success
 PyObject* set_error_class(PyObject*, PyObject* cls)
 {
@@ -553,6 +780,12 @@ PyMethodDef kMethods[] = {OPSCV_FAST(grid_sampler2d),
                           OPSCV_FAST(upsample_bilinear2d),
                           OPSCV_FAST(upsample_bilinear2d_backward),
                           OPSCV_FAST(resize),
+                          OPSCV_FAST(residual_norm),
+                          OPSCV_FAST(residual_norm_backward),
+                          OPSCV_FAST(rotary_table),
+                          OPSCV_FAST(rotary),
+                          OPSCV_FAST(window_attention),
+                          OPSCV_FAST(window_attention_backward),
                           {"set_error_class", set_error_class, METH_O, nullptr},
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_torch_helpers", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
