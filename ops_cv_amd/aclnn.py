@@ -128,6 +128,26 @@ def load_library():
                                                                   ctypes.POINTER(vp)]
     L.aclnnUpsampleBilinear2dBackward.restype = i32
     L.aclnnUpsampleBilinear2dBackward.argtypes = [vp, u64, vp, vp]
+    L.opscvResidualNormGetWorkspaceSize.restype = i32
+    L.opscvResidualNormGetWorkspaceSize.argtypes = [vp, vp, vp, ctypes.c_double, vp, vp, vp, vp, p_u64, p_vp]
+    L.opscvResidualNormBackwardGetWorkspaceSize.restype = i32
+    L.opscvResidualNormBackwardGetWorkspaceSize.argtypes = [vp, vp, vp, vp, vp, vp, vp, p_u64, p_vp]
+    L.opscvRotaryTableGetWorkspaceSize.restype = i32
+    L.opscvRotaryTableGetWorkspaceSize.argtypes = [ctypes.c_double, i64, ctypes.c_double, i64, ctypes.c_double, vp, p_u64,
+                                                   p_vp]
+    L.opscvRotaryGetWorkspaceSize.restype = i32
+    L.opscvRotaryGetWorkspaceSize.argtypes = [vp, vp, vp, vp, ctypes.c_bool, ctypes.c_bool, vp, vp, p_u64, p_vp]
+    L.opscvWindowAttentionGetWorkspaceSize.restype = i32
+    L.opscvWindowAttentionGetWorkspaceSize.argtypes = [vp, vp, vp, vp, vp, ctypes.c_double, i64, i64, i64, vp, vp, p_u64,
+                                                       p_vp]
+    L.opscvWindowAttentionBackwardGetWorkspaceSize.restype = i32
+    L.opscvWindowAttentionBackwardGetWorkspaceSize.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_double, i64, i64,
+                                                               i64, vp, vp, vp, p_u64, p_vp]
+    for name in ("ResidualNorm", "ResidualNormBackward", "RotaryTable", "Rotary", "WindowAttention",
+                 "WindowAttentionBackward"):
+        phase2 = getattr(L, "opscv" + name)
+        phase2.restype = i32
+        phase2.argtypes = [vp, u64, vp, vp]
     L.opscvGridSampler2DTaps.restype = i32
     L.opscvGridSampler2DTaps.argtypes = [vp, ctypes.c_int, i64, i64, i64, i64, i64, i64, i64, ctypes.c_bool, vp, vp]
     L.opscvGridSampler2DBicubicTaps.restype = i32

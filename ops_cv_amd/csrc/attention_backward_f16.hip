@@ -1,0 +1,12 @@
+#include <hip/hip_runtime.h>
+
+#include "attention_backward_kernel.hpp"
+
+namespace opscv {
+
+hipError_t run_attention_grad_f16(const AttentionArgs& a, bool vectors, hipStream_t stream)
+{
+    return vectors ? att::run_backward<_Float16, true>(a, stream) : att::run_backward<_Float16, false>(a, stream);
+}
+
+}  // namespace opscv

@@ -1,0 +1,586 @@
+// Gradients of attention, in three kernels and a join:
+//
+//   statistics  per row i: lse_i log2 e (infinity where the row sees nothing), D_i = sum gO_i O_i, and for FLOAT16 a power
+//               of two near the largest |gO_i|
+//   queries     as the forward pass walks keys:  P' = exp2(K Q' c - lse),  dP' = V gO',  dS' = P' (dP' - D),
+//               gQ' += K' dS'
+//   keys        a wavefront keeps 32 keys and walks the queries that see them:  P, dS as above with rows and columns
+//               exchanged,  gV' += gO' P,  gK' += Q' dS
+//   join        where the queries of a tile of keys were cut into parts, their 32-bit sums in order
+//
+// Everything but the operands of the products is in 32 bits: P and dS are rounded to the type as the matrix instructions
+// want them.  P and dS are computed twice, once for each direction: seven products instead of five, but every sum has one
+// owner and a fixed order, and no gradient is added up by atomics.
+//
+// dS of FLOAT16: P of a long row times a small gradient falls among the numbers that FLOAT16 has few bits or none for, so dS
+// is divided by a power of two of the size of the row's (of the rows' walked so far) gradient before it is rounded, and
+// the sum multiplied by it.
+#pragma once
+
+#include <atomic>
+#include <type_traits>
+
+#include "attention_plan.hpp"
+#include "attention_tile.hpp"
+#include "fast_div.hpp"
+#include "kernels.hpp"
+
+namespace opscv {
+namespace att {
+
+struct GradLaunch {
+    AttentionArgs a;
+    FastDiv group;
+    uint32_t rows, tiles, kv_heads;
+    uint32_t key_tiles, sink_tiles, sink_parts, parts;
+    uint32_t query_blocks, key_blocks;
+    float* stats;          // (batch, heads, 3, tokens)
+    float* sink_partials;  // (batch * kv_heads, sink_tiles, sink_parts, 2, kGradKeys, d rounded up to four)
+    float* partials;       // the same of the other tiles
+};
+
+static __device__ __forceinline__ int64_t stats_row(const AttentionArgs& a, int64_t b, int64_t head)
+{
+    return (b * a.heads + head) * 3 * a.tokens;
+}
+
+// Statistics of the rows: sixteen lanes a row.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void attention_stats_kernel(GradLaunch p, uint32_t rows)
+{
+    const AttentionArgs& a = p.a;
+    const uint32_t row = (blockIdx.x * 256u + threadIdx.x) / 16;
+    const int lane = (int)threadIdx.x & 15, d = (int)a.d;
+    if (row >= rows) {
+        return;  // sixteen lanes together
+    }
+    // heads fastest: neighbouring rows lie side by side where heads do
+    const uint32_t head = row % (uint32_t)a.heads, rest = row / (uint32_t)a.heads;
+    const uint32_t token = rest % (uint32_t)a.tokens, b = rest / (uint32_t)a.tokens;
+    const T* const go = (const T*)a.grad_out.ptr + (int64_t)b * a.grad_out.stride[0] +
+                        (int64_t)token * a.grad_out.stride[1] + (int64_t)head * a.grad_out.stride[2];
+    const T* const o = (const T*)a.out.ptr + (int64_t)b * a.out.stride[0] + (int64_t)token * a.out.stride[1] +
+                       (int64_t)head * a.out.stride[2];
+    float sum = 0.0f, most = 0.0f;
+    for (int c = lane * 8; c < d; c += 128) {
+        const Frag<T> x = global_row<T, VEC>(go, c, d), y = global_row<T, VEC>(o, c, d);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            sum += (float)x[e] * (float)y[e];
+            most = fmaxf(most, fabsf((float)x[e]));
+        }
+    }
+#pragma unroll
+    for (int w = 8; w > 0; w >>= 1) {
+        sum += __shfl_xor(sum, w, 64);
+        most = fmaxf(most, __shfl_xor(most, w, 64));
+    }
+    if (lane == 0) {
+        const Sequence seq = sequence_at(a, b);
+        const float lse = ((const float*)a.lse.ptr)[(int64_t)b * a.lse.stride[0] + (int64_t)head * a.lse.stride[1] +
+                                                    (int64_t)token * a.lse.stride[2]];
+        const bool live = (int)token < seq.q_len && lse != -INFINITY;
+        float* const to = p.stats + stats_row(a, b, head) + token;
+        to[0] = live ? lse * kLog2e : INFINITY;
+        to[a.tokens] = live ? sum : 0.0f;
+        // 2^floor(log2 most) by its exponent bits; 0 for rows of zeros
+        const uint32_t bits = __float_as_uint(most) & 0x7f800000u;
+        to[2 * a.tokens] = !live ? 0.0f : (bits == 0x7f800000u ? 1.0f : __uint_as_float(bits));
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------- queries' gradients
+
+constexpr ForwardShape query_grad_shape(int elem_bytes, int pitch) { return forward_shape(elem_bytes, pitch, false); }
+
+template <typename T, int NB, bool VEC>
+__global__ __launch_bounds__(256, 1) void attention_query_grad_kernel(GradLaunch p)
+{
+    constexpr int kPitch = pitch_of(NB);
+    constexpr ForwardShape kShape = query_grad_shape(sizeof(T), kPitch);
+    constexpr int kKeys = kShape.keys, kSubs = kKeys / kBlock, kThreads = 256;
+    constexpr bool kUnits = std::is_same<T, _Float16>::value;
+    typedef Tile<T, kPitch> L;
+    extern __shared__ __align__(16) char lds[];
+
+    const AttentionArgs& a = p.a;
+    const uint32_t index = xcd_order(blockIdx.x, p.query_blocks);
+    if (index >= p.query_blocks) {
+        return;
+    }
+    const uint32_t tile = index % p.tiles, bh = index / p.tiles;
+    const uint32_t b = bh / p.kv_heads, kv_head = bh % p.kv_heads;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
+    const int h = lane >> 5, own = lane & 31, gt = wave * 64 + lane;
+    const int d = (int)a.d, left = (int)a.left, right = (int)a.right, sinks = (int)a.sinks;
+    const Sequence seq = sequence_at(a, b);
+
+    const uint32_t row0 = tile * kShape.rows(), wave_row0 = row0 + wave * kBlock;
+    const uint32_t row = min(wave_row0 + own, p.rows - 1);
+    const int query = (int)fast_div(row, p.group);
+    const int head = (int)(kv_head * p.group.div) + (int)(row - (uint32_t)query * p.group.div);
+    const int pos = query < seq.q_len ? seq.first + query : INT32_MIN / 2;
+    const auto query_of = [&](uint32_t r) { return (int)fast_div(min(r, p.rows - 1), p.group); };
+    const int block_low = query_of(row0), block_high = min(query_of(row0 + kShape.rows() - 1), seq.q_len - 1);
+    KeyRange range = key_range<kKeys>(seq.first + block_low, seq.first + block_high, seq.kv_len, left, right, sinks);
+    if (block_high < block_low) {
+        range.tiles = 0;
+    }
+    const int wave_low = seq.first + query_of(wave_row0), wave_high = seq.first + query_of(wave_row0 + kBlock - 1);
+    const bool wave_whole = query_of(wave_row0 + kBlock - 1) < seq.q_len;
+
+    Frag<T> q[2 * NB], go[2 * NB];
+    {
+        const T* const src = (const T*)a.q.ptr + (int64_t)b * a.q.stride[0] + (int64_t)query * a.q.stride[1] +
+                             (int64_t)head * a.q.stride[2];
+        const T* const gsrc = (const T*)a.grad_out.ptr + (int64_t)b * a.grad_out.stride[0] +
+                              (int64_t)query * a.grad_out.stride[1] + (int64_t)head * a.grad_out.stride[2];
+#pragma unroll
+        for (int i = 0; i < 2 * NB; i++) {
+            q[i] = global_row<T, VEC>(src, 16 * i + 8 * h, d);
+            go[i] = global_row<T, VEC>(gsrc, 16 * i + 8 * h, d);
+        }
+    }
+    const float* const stat = p.stats + stats_row(a, b, head) + query;
+    const float lse = stat[0], along = stat[a.tokens];
+    const float unit = kUnits ? stat[2 * a.tokens] : 1.0f, per_unit = unit > 0.0f ? 1.0f / unit : 0.0f;
+
+    const T* const k_base = (const T*)a.k.ptr + (int64_t)b * a.k.stride[0] + (int64_t)kv_head * a.k.stride[2];
+    const T* const v_base = (const T*)a.v.ptr + (int64_t)b * a.v.stride[0] + (int64_t)kv_head * a.v.stride[2];
+    const uint32_t k_pitch = (uint32_t)(a.k.stride[1] * (int64_t)sizeof(T));
+    const uint32_t v_pitch = (uint32_t)(a.v.stride[1] * (int64_t)sizeof(T));
+    T* const ring = reinterpret_cast<T*>(lds);
+    const auto fetch = [&](int t, int buffer) {
+        const int key0 = range.key_of(t, kKeys);
+        T* const k_tile = ring + buffer * (2 * kKeys * kPitch);
+        stage<T, kPitch, kKeys, kThreads, VEC>(k_tile, k_base + (int64_t)key0 * a.k.stride[1], gt, d, [&](int r) {
+            return range.holds(t, key0 + r) ? (uint32_t)r * k_pitch : kOutside;
+        });
+        stage<T, kPitch, kKeys, kThreads, VEC>(k_tile + kKeys * kPitch, v_base + (int64_t)key0 * a.v.stride[1], gt, d,
+                                               [&](int r) { return range.holds(t, key0 + r) ? (uint32_t)r * v_pitch : kOutside; });
+    };
+    constexpr int kInFlight = 2 * kKeys * L::kChunks / kThreads;
+
+    const float c = a.scale * kLog2e;
+    acc_t gq[NB];
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        gq[i] = zeros();
+    }
+    int buffer = 0;
+    if (range.tiles > 0) {
+        fetch(0, 0);
+    }
+    for (int t = 0; t < range.tiles; t++) {
+        const bool more = t + 1 < range.tiles;
+        if (kShape.stages == 2 && more) {
+            fetch(t + 1, buffer ^ 1);
+            if constexpr (VEC) {
+                __builtin_amdgcn_s_waitcnt(wait_for_loads(kInFlight));
+            }
+        } else if constexpr (VEC) {
+            __builtin_amdgcn_s_waitcnt(wait_for_loads(0));
+        }
+        __syncthreads();
+        const T* const k_tile = ring + buffer * (2 * kKeys * kPitch);
+        const T* const v_tile = k_tile + kKeys * kPitch;
+        const int key0 = range.key_of(t, kKeys), end = range.end_of(t);
+        const bool all_seen = wave_whole && key0 + kKeys <= end && key0 + kKeys - 1 <= wave_low + right &&
+                              (key0 >= wave_high - left || key0 + kKeys <= sinks);
+#pragma unroll
+        for (int j = 0; j < kSubs; j++) {
+            acc_t s = zeros(), dp = zeros();
+#pragma unroll
+            for (int i = 0; i < 2 * NB; i++) {
+                s = Mma<T>::mul(L::row(k_tile, j * kBlock + own, 2 * i + h), q[i], s);
+                dp = Mma<T>::mul(L::row(v_tile, j * kBlock + own, 2 * i + h), go[i], dp);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -lse)) * ((dp[r] - along) * per_unit);
+                if (!all_seen) {
+                    const int key = key0 + j * kBlock + 8 * (r / 4) + 4 * h + r % 4;
+                    s[r] = (key < end && sees(pos, key, left, right, sinks)) ? x : 0.0f;
+                } else {
+                    s[r] = x;
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+                const Frag<T> w = operand<T>(s, g);
+#pragma unroll
+                for (int i = 0; i < NB; i++) {
+                    gq[i] = Mma<T>::mul(L::column(k_tile, j * kBlock + 16 * g, i, lane), w, gq[i]);
+                }
+            }
+        }
+        __syncthreads();
+        if (kShape.stages == 1 && more) {
+            fetch(t + 1, 0);
+        }
+        buffer ^= kShape.stages - 1;
+    }
+    if (wave_row0 + own >= p.rows) {
+        return;
+    }
+    const float f = a.scale * unit;
+    // a row that sees nothing has the gradient 0, also where its unit is one of an infinite gradient
+    T* const to = (T*)a.grad_q.ptr + (int64_t)b * a.grad_q.stride[0] + (int64_t)query * a.grad_q.stride[1] +
+                  (int64_t)head * a.grad_q.stride[2];
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            put4<T, VEC>(to, i * kBlock + 8 * (r / 4) + 4 * h, d, gq[i][r] * f, gq[i][r + 1] * f, gq[i][r + 2] * f,
+                         gq[i][r + 3] * f);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------- keys' gradients
+
+constexpr int key_grad_stages(int elem_bytes, int pitch) { return elem_bytes * pitch <= 512 ? 2 : 1; }
+
+template <typename T, int NB, bool VEC>
+__global__ __launch_bounds__(64 * kKeyWaves, 1) void attention_key_grad_kernel(GradLaunch p)
+{
+    constexpr int kPitch = pitch_of(NB), kThreads = 64 * kKeyWaves, kStages = key_grad_stages(sizeof(T), kPitch);
+    constexpr bool kUnits = std::is_same<T, _Float16>::value;
+    constexpr int kStatRows = kUnits ? 4 : 2;  // of 32 floats each, a wavefront and stage
+    constexpr int kTile = kBlock * kPitch;     // elements
+    typedef Tile<T, kPitch> L;
+    extern __shared__ __align__(16) char lds[];
+
+    const AttentionArgs& a = p.a;
+    uint32_t index = xcd_order(blockIdx.x, p.key_blocks);
+    if (index >= p.key_blocks) {
+        return;
+    }
+    // of a key head: the parts of the sinks' tiles, then those of the others
+    const uint32_t sink_items = p.sink_tiles * p.sink_parts;
+    const uint32_t items = sink_items + (p.key_tiles - p.sink_tiles) * p.parts;
+    const uint32_t bh = index / items, item = index % items;
+    const bool sink_tile = item < sink_items;
+    const uint32_t of = sink_tile ? p.sink_parts : p.parts, at = sink_tile ? item : item - sink_items;
+    const uint32_t part = at % of, local_tile = at / of, tile = local_tile + (sink_tile ? 0 : p.sink_tiles);
+    const uint32_t b = bh / p.kv_heads, kv_head = bh % p.kv_heads;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
+    const int h = lane >> 5, own = lane & 31, gt = wave * 64 + lane;
+    const int d = (int)a.d, left = (int)a.left, right = (int)a.right, sinks = (int)a.sinks;
+    const Sequence seq = sequence_at(a, b);
+
+    const int key0 = (int)tile * kGradKeys, wave_key0 = key0 + wave * kBlock, key = wave_key0 + own;
+    // queries that see a key of the tile
+    const int last = min(key0 + kGradKeys, seq.kv_len) - 1;
+    int low = max(key0 - right - seq.first, 0);
+    int high = key0 < sinks ? seq.q_len : min(seq.q_len, last + left + 1 - seq.first);
+    if (last < key0) {
+        high = low;
+    }
+    const int row_tiles = high > low ? (high - low + kBlock - 1) / kBlock : 0;
+    const int steps = row_tiles * (int)p.group.div;
+    const int s_begin = (int)((int64_t)steps * part / of), s_end = (int)((int64_t)steps * (part + 1) / of);
+
+    Frag<T> k[2 * NB], v[2 * NB];
+    {
+        const int64_t from = min(key, (int)a.kv_tokens - 1);
+        const T* const ks = (const T*)a.k.ptr + (int64_t)b * a.k.stride[0] + from * a.k.stride[1] + (int64_t)kv_head * a.k.stride[2];
+        const T* const vs = (const T*)a.v.ptr + (int64_t)b * a.v.stride[0] + from * a.v.stride[1] + (int64_t)kv_head * a.v.stride[2];
+#pragma unroll
+        for (int i = 0; i < 2 * NB; i++) {
+            k[i] = global_row<T, VEC>(ks, 16 * i + 8 * h, d);
+            v[i] = global_row<T, VEC>(vs, 16 * i + 8 * h, d);
+        }
+    }
+    T* const ring = reinterpret_cast<T*>(lds);
+    float* const stat_ring = reinterpret_cast<float*>(lds + (size_t)kStages * 2 * kTile * sizeof(T)) +
+                             wave * (kStages * kStatRows * kBlock);
+    const uint32_t q_pitch = (uint32_t)(a.q.stride[1] * (int64_t)sizeof(T));
+    const uint32_t go_pitch = (uint32_t)(a.grad_out.stride[1] * (int64_t)sizeof(T));
+    // step s: head s / row_tiles of the group, queries from low + 32 (s % row_tiles) on
+    const auto fetch = [&](int s, int buffer) {
+        const int g = s / row_tiles, i0 = low + (s - g * row_tiles) * kBlock;
+        const int64_t head = (int64_t)kv_head * p.group.div + g;
+        const T* const q_base = (const T*)a.q.ptr + (int64_t)b * a.q.stride[0] + i0 * a.q.stride[1] + head * a.q.stride[2];
+        const T* const go_base = (const T*)a.grad_out.ptr + (int64_t)b * a.grad_out.stride[0] + i0 * a.grad_out.stride[1] +
+                                 head * a.grad_out.stride[2];
+        const int rows = seq.q_len - i0;
+        T* const q_tile = ring + buffer * (2 * kTile);
+        stage<T, kPitch, kBlock, kThreads, VEC>(q_tile, q_base, gt, d, [&](int r) { return r < rows ? (uint32_t)r * q_pitch : kOutside; });
+        stage<T, kPitch, kBlock, kThreads, VEC>(q_tile + kTile, go_base, gt, d,
+                                                [&](int r) { return r < rows ? (uint32_t)r * go_pitch : kOutside; });
+        // statistics: lanes of the lower half read one kind, of the upper half the next; rows past the end read zeros,
+        // which meet rows of zeros
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+            p.stats + stats_row(a, b, head) + i0, 0, 0x7fffffff, kBufferFlags);
+        float* const to = stat_ring + buffer * (kStatRows * kBlock);
+#pragma unroll
+        for (int n = 0; n < kStatRows / 2; n++) {
+            const int kind = 2 * n + h;
+            const uint32_t off = (own < rows && kind < 3) ? (uint32_t)(kind * (int)a.tokens + own) * 4u : kOutside;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)(to + n * 2 * kBlock), 4, (int)off, 0, 0, 0);
+        }
+    };
+    constexpr int kInFlight = (VEC ? 2 * kBlock * L::kChunks / kThreads : 0) + kStatRows / 2;
+
+    const float c = a.scale * kLog2e;
+    acc_t gk[NB], gv[NB];
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        gk[i] = zeros();
+        gv[i] = zeros();
+    }
+    float unit = 0.0f, per_unit = kUnits ? 0.0f : 1.0f;
+    int buffer = 0;
+    if (s_begin < s_end) {
+        fetch(s_begin, 0);
+    }
+    for (int step = s_begin; step < s_end; step++) {
+        const bool more = step + 1 < s_end;
+        if (kStages == 2 && more) {
+            fetch(step + 1, buffer ^ 1);
+            __builtin_amdgcn_s_waitcnt(wait_for_loads(kInFlight));
+        } else {
+            __builtin_amdgcn_s_waitcnt(wait_for_loads(0));
+        }
+        __syncthreads();
+        const T* const q_tile = ring + buffer * (2 * kTile);
+        const T* const go_tile = q_tile + kTile;
+        const float* const stat = stat_ring + buffer * (kStatRows * kBlock);
+        const int i0 = low + (step % row_tiles) * kBlock;
+        const int p_low = seq.first + i0, p_high = seq.first + min(i0 + kBlock, seq.q_len) - 1;
+        // whether the wavefront's keys are seen by any of the rows, and by all of them
+        const bool any = wave_key0 < seq.kv_len && wave_key0 <= p_high + right &&
+                         (wave_key0 + kBlock - 1 >= p_low - left || wave_key0 < sinks);
+        const bool all_seen = wave_key0 + kBlock <= seq.kv_len && wave_key0 + kBlock - 1 <= p_low + right &&
+                              (wave_key0 >= p_high - left || wave_key0 + kBlock <= sinks);
+        if (any) {
+            if constexpr (kUnits) {
+                float most = stat[2 * kBlock + own];
+#pragma unroll
+                for (int w = 16; w > 0; w >>= 1) {
+                    most = fmaxf(most, __shfl_xor(most, w, 64));
+                }
+                if (__any(most > unit)) {
+                    const float fade = unit / most;
+#pragma unroll
+                    for (int i = 0; i < NB; i++) {
+#pragma unroll
+                        for (int r = 0; r < 16; r++) {
+                            gk[i][r] *= fade;
+                        }
+                    }
+                    unit = most;
+                    per_unit = 1.0f / most;
+                }
+            }
+            acc_t s = zeros(), dp = zeros();
+#pragma unroll
+            for (int i = 0; i < 2 * NB; i++) {
+                s = Mma<T>::mul(L::row(q_tile, own, 2 * i + h), k[i], s);
+                dp = Mma<T>::mul(L::row(go_tile, own, 2 * i + h), v[i], dp);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int n = 8 * (r / 4) + 4 * h + r % 4;
+                float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -stat[n]));
+                float y = x * ((dp[r] - stat[kBlock + n]) * per_unit);
+                if (!all_seen) {
+                    const bool seen = key < seq.kv_len && sees(p_low + n, key, left, right, sinks);
+                    x = seen ? x : 0.0f;
+                    y = seen ? y : 0.0f;
+                }
+                s[r] = x;
+                dp[r] = y;
+            }
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+                const Frag<T> w = operand<T>(s, g), x = operand<T>(dp, g);
+#pragma unroll
+                for (int i = 0; i < NB; i++) {
+                    gv[i] = Mma<T>::mul(L::column(go_tile, 16 * g, i, lane), w, gv[i]);
+                    gk[i] = Mma<T>::mul(L::column(q_tile, 16 * g, i, lane), x, gk[i]);
+                }
+            }
+        }
+        __syncthreads();
+        if (kStages == 1 && more) {
+            fetch(step + 1, 0);
+        }
+        buffer ^= kStages - 1;
+    }
+    const float f = a.scale * (kUnits ? unit : 1.0f);
+    if (of > 1) {
+        const int64_t tile_index = sink_tile ? (int64_t)bh * p.sink_tiles + local_tile
+                                             : (int64_t)bh * (p.key_tiles - p.sink_tiles) + local_tile;
+        const int row_floats = (d + 3) / 4 * 4;
+        float* const to = (sink_tile ? p.sink_partials : p.partials) +
+                          ((tile_index * of + part) * 2 * kGradKeys + wave * kBlock + own) * row_floats;
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int el = i * kBlock + 8 * (r / 4) + 4 * h;
+                if (el < d) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        to[el + e] = gk[i][r + e] * f;
+                        to[(int64_t)kGradKeys * row_floats + el + e] = gv[i][r + e];
+                    }
+                }
+            }
+        }
+        return;
+    }
+    if (key >= (int)a.kv_tokens) {
+        return;
+    }
+    T* const to_k = (T*)a.grad_k.ptr + (int64_t)b * a.grad_k.stride[0] + (int64_t)key * a.grad_k.stride[1] +
+                    (int64_t)kv_head * a.grad_k.stride[2];
+    T* const to_v = (T*)a.grad_v.ptr + (int64_t)b * a.grad_v.stride[0] + (int64_t)key * a.grad_v.stride[1] +
+                    (int64_t)kv_head * a.grad_v.stride[2];
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const int el = i * kBlock + 8 * (r / 4) + 4 * h;
+            put4<T, VEC>(to_k, el, d, gk[i][r] * f, gk[i][r + 1] * f, gk[i][r + 2] * f, gk[i][r + 3] * f);
+            put4<T, VEC>(to_v, el, d, gv[i][r], gv[i][r + 1], gv[i][r + 2], gv[i][r + 3]);
+        }
+    }
+}
+
+// Sums of the parts of `tiles` tiles of every key head, from tile `first` on: four features of a key a thread.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void attention_grad_join_kernel(GradLaunch p, const float* __restrict__ partials,
+                                                                  uint32_t first, uint32_t tiles, uint32_t parts,
+                                                                  uint32_t quads, uint32_t total)
+{
+    const AttentionArgs& a = p.a;
+    const uint32_t index = blockIdx.x * 256u + threadIdx.x;
+    if (index >= total) {
+        return;
+    }
+    const uint32_t quad = index % quads;
+    uint32_t rest = index / quads;
+    const uint32_t local_key = rest % kGradKeys;
+    rest /= kGradKeys;
+    const uint32_t value = rest & 1, tile_index = rest >> 1;
+    const uint32_t tile = first + tile_index % tiles, bh = tile_index / tiles;
+    const int64_t key = (int64_t)tile * kGradKeys + local_key;
+    if (key >= a.kv_tokens) {
+        return;
+    }
+    const int row_floats = (int)quads * 4;
+    const float* const from =
+        partials + (((int64_t)tile_index * parts * 2 + value) * kGradKeys + local_key) * row_floats + quad * 4;
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t i = 0; i < parts; i++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            x[e] += from[(int64_t)i * 2 * kGradKeys * row_floats + e];
+        }
+    }
+    const Strided& out = value != 0 ? a.grad_v : a.grad_k;
+    T* const to = (T*)out.ptr + (int64_t)(bh / p.kv_heads) * out.stride[0] + key * out.stride[1] +
+                  (int64_t)(bh % p.kv_heads) * out.stride[2];
+    put4<T, VEC>(to, (int)quad * 4, (int)a.d, x[0], x[1], x[2], x[3]);
+}
+
+template <typename T, int NB, bool VEC>
+hipError_t run_backward_shape(const GradLaunch& p, hipStream_t stream)
+{
+    constexpr int kPitch = pitch_of(NB);
+    constexpr ForwardShape kShape = query_grad_shape(sizeof(T), kPitch);
+    constexpr int kQueryBytes = kShape.stages * 2 * kShape.keys * kPitch * (int)sizeof(T);
+    constexpr int kStages = key_grad_stages(sizeof(T), kPitch);
+    constexpr int kKeyBytes = kStages * 2 * kBlock * kPitch * (int)sizeof(T) +
+                              kKeyWaves * kStages * (std::is_same<T, _Float16>::value ? 4 : 2) * kBlock * 4;
+    static_assert(kQueryBytes <= 160 * 1024 && kKeyBytes <= 160 * 1024, "LDS of a CU");
+    static std::atomic<uint32_t> query_done{0}, key_done{0};
+    const auto query_kernel = attention_query_grad_kernel<T, NB, VEC>;
+    const auto key_kernel = attention_key_grad_kernel<T, NB, VEC>;
+    hipError_t e = hipSuccess;
+    if (kQueryBytes > 64 * 1024) {
+        e = allow_dynamic_lds((const void*)query_kernel, kQueryBytes, query_done);
+    }
+    if (e == hipSuccess && kKeyBytes > 64 * 1024) {
+        e = allow_dynamic_lds((const void*)key_kernel, kKeyBytes, key_done);
+    }
+    if (e != hipSuccess) {
+        return e;
+    }
+    if (p.query_blocks > 0) {
+        hipLaunchKernelGGL(query_kernel, dim3((p.query_blocks + 7) / 8 * 8), dim3(kShape.threads()), kQueryBytes, stream, p);
+    }
+    if (p.key_blocks > 0) {
+        hipLaunchKernelGGL(key_kernel, dim3((p.key_blocks + 7) / 8 * 8), dim3(64 * kKeyWaves), kKeyBytes, stream, p);
+    }
+    return hipGetLastError();
+}
+
+template <typename T, bool VEC>
+hipError_t run_backward(const AttentionArgs& a, hipStream_t stream)
+{
+    const GradPlan plan = plan_grad(a);
+    const int64_t bh = a.batch * a.kv_heads, stat_rows = a.batch * a.heads * a.tokens;
+    const int64_t query_blocks = bh * plan.tiles;
+    const int64_t key_blocks = bh * (plan.sink_tiles * plan.sink_parts + (plan.key_tiles - plan.sink_tiles) * plan.parts);
+    const int64_t quads = (a.d + 3) / 4;
+    const int64_t sink_joins = plan.sink_parts > 1 ? bh * plan.sink_tiles * 2 * kGradKeys * quads : 0;
+    const int64_t joins = plan.parts > 1 ? bh * (plan.key_tiles - plan.sink_tiles) * 2 * kGradKeys * quads : 0;
+    // 3 * tokens * 4 bytes of statistics are reached with 32-bit offsets
+    if (query_blocks > INT32_MAX / 1024 || key_blocks > INT32_MAX / 1024 || stat_rows > INT32_MAX / 16 ||
+        a.tokens > INT32_MAX / 12 || sink_joins > INT32_MAX || joins > INT32_MAX ||
+        (a.scratch == nullptr && plan.stats > 0)) {
+        return hipErrorInvalidValue;
+    }
+    GradLaunch p;
+    p.a = a;
+    p.group = make_fast_div((uint32_t)(a.heads / a.kv_heads));
+    p.rows = (uint32_t)plan.rows;
+    p.tiles = (uint32_t)plan.tiles;
+    p.kv_heads = (uint32_t)a.kv_heads;
+    p.key_tiles = (uint32_t)plan.key_tiles;
+    p.sink_tiles = (uint32_t)plan.sink_tiles;
+    p.sink_parts = (uint32_t)plan.sink_parts;
+    p.parts = (uint32_t)plan.parts;
+    p.query_blocks = (uint32_t)query_blocks;
+    p.key_blocks = (uint32_t)key_blocks;
+    p.stats = a.scratch;
+    p.sink_partials = a.scratch + (plan.stats + 3) / 4 * 4;
+    p.partials = p.sink_partials + plan.sink_partials;
+    if (stat_rows > 0) {
+        hipLaunchKernelGGL((attention_stats_kernel<T, VEC>), dim3((unsigned)((stat_rows + 15) / 16)), dim3(256), 0, stream, p,
+                           (uint32_t)stat_rows);
+    }
+    hipError_t e = hipErrorInvalidValue;
+    switch (blocks_of(a.d)) {
+        case 8: e = run_backward_shape<T, 8, VEC>(p, stream); break;
+        case 4: e = run_backward_shape<T, 4, VEC>(p, stream); break;
+        case 3: e = run_backward_shape<T, 3, VEC>(p, stream); break;
+        default: e = run_backward_shape<T, 2, VEC>(p, stream); break;
+    }
+    if (e != hipSuccess) {
+        return e;
+    }
+    if (sink_joins > 0) {
+        hipLaunchKernelGGL((attention_grad_join_kernel<T, VEC>), dim3((unsigned)((sink_joins + 255) / 256)), dim3(256), 0,
+                           stream, p, p.sink_partials, 0u, p.sink_tiles, p.sink_parts, (uint32_t)quads, (uint32_t)sink_joins);
+    }
+    if (joins > 0) {
+        hipLaunchKernelGGL((attention_grad_join_kernel<T, VEC>), dim3((unsigned)((joins + 255) / 256)), dim3(256), 0, stream,
+                           p, p.partials, p.sink_tiles, p.key_tiles - p.sink_tiles, p.parts, (uint32_t)quads,
+                           (uint32_t)joins);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace att
+
+// one translation unit a type
+hipError_t run_attention_grad_f32(const AttentionArgs& a, bool vectors, hipStream_t stream);
+hipError_t run_attention_grad_f16(const AttentionArgs& a, bool vectors, hipStream_t stream);
+hipError_t run_attention_grad_bf16(const AttentionArgs& a, bool vectors, hipStream_t stream);
+
+}  // namespace opscv

@@ -11,6 +11,7 @@
 #pragma once
 
 #include <atomic>
+#include <type_traits>
 
 #include "attention_plan.hpp"
 #include "attention_tile.hpp"
@@ -28,35 +29,63 @@ struct ForwardLaunch {
     uint32_t blocks;  // workgroups with work
 };
 
-// Workgroups go round the eight XCDs; this gives every XCD a run of neighbouring numbers, so that the tiles of rows that
-// read the same keys share an L2.
-static __device__ __forceinline__ uint32_t xcd_order(uint32_t index, uint32_t count)
+// Where some rows do not see some keys of a tile, a value that is not finite must not reach them through its product with
+// their weight 0.  odd_values: whether the tile holds such values (wave-uniform); tiles that all rows see whole are not
+// asked.
+template <typename T, int PITCH, int KEYS, int NB>
+static __device__ __forceinline__ bool odd_values(const T* tile, int lane)
 {
-    const uint32_t each = (count + 7) / 8;
-    return (index & 7u) * each + (index >> 3);
+    bool odd = false;
+#pragma unroll
+    for (int base = 0; base < KEYS; base += 16) {
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+            const Frag<T> f = Tile<T, PITCH>::column(tile, base, i, lane);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                odd = odd || !__builtin_isfinite((float)f[e]);
+            }
+        }
+    }
+    return __any(odd);
 }
 
-// Keys that a range of rows sees, as tiles: the first `sink_tiles` start at key 0, the others at `first`.
-struct KeyRange {
-    int first, end;  // window
-    int sink_end;    // sinks in front of it
-    int sink_tiles, tiles;
-};
-
-template <int KEYS>
-static __device__ __forceinline__ KeyRange key_range(int p_low, int p_high, int kv_len, int left, int right, int sinks)
+// O' += V' P with such values: the finite ones as ever; of the others, which kinds each row gives weight to is counted by
+// products of ones and zeros.
+template <typename T, int PITCH, int SUBS, int NB>
+static __device__ __forceinline__ void add_odd_values(acc_t (&o)[NB], const acc_t (&s)[SUBS], const T* tile, int lane)
 {
-    KeyRange k;
-    k.end = min(max(p_high + right + 1, 0), kv_len);
-    k.first = min(max(p_low - left, 0), k.end);
-    k.sink_end = min(sinks, k.first);
-    k.sink_tiles = (k.sink_end + KEYS - 1) / KEYS;
-    if (k.sink_tiles > 0 && k.first <= k.sink_tiles * KEYS) {  // the window starts among them: one run of tiles
-        k.first = 0;
-        k.sink_tiles = 0;
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        acc_t up = zeros(), down = zeros(), none = zeros();
+#pragma unroll
+        for (int j = 0; j < SUBS; j++) {
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+                const Frag<T> w = operand<T>(s[j], g), f = Tile<T, PITCH>::column(tile, j * kBlock + 16 * g, i, lane);
+                Frag<T> finite, is_up, is_down, is_none, has;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float x = (float)f[e];
+                    finite[e] = __builtin_isfinite(x) ? f[e] : (T)0.0f;
+                    is_up[e] = (T)(x == INFINITY ? 1.0f : 0.0f);
+                    is_down[e] = (T)(x == -INFINITY ? 1.0f : 0.0f);
+                    is_none[e] = (T)(x != x ? 1.0f : 0.0f);
+                    has[e] = (T)(s[j][8 * g + e] > 0.0f ? 1.0f : 0.0f);
+                }
+                o[i] = Mma<T>::mul(finite, w, o[i]);
+                up = Mma<T>::mul(is_up, has, up);
+                down = Mma<T>::mul(is_down, has, down);
+                none = Mma<T>::mul(is_none, has, none);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            o[i][r] += up[r] > 0.0f ? INFINITY : 0.0f;
+            o[i][r] += down[r] > 0.0f ? -INFINITY : 0.0f;
+            o[i][r] += none[r] > 0.0f ? NAN : 0.0f;
+        }
     }
-    k.tiles = k.sink_tiles + (k.end - k.first + KEYS - 1) / KEYS;
-    return k;
 }
 
 template <typename T, int NB, bool FEW, bool VEC>
@@ -71,7 +100,7 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
 
     const AttentionArgs& a = p.a;
     const uint32_t index = xcd_order(blockIdx.x, p.blocks);
-    if (index >= p.blocks || (blockIdx.x >> 3) >= (p.blocks + 7) / 8) {
+    if (index >= p.blocks) {
         return;
     }
     const uint32_t tile = index % p.tiles, rest = index / p.tiles;
@@ -118,16 +147,14 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
     const uint32_t v_pitch = (uint32_t)(a.v.stride[1] * (int64_t)sizeof(T));
 
     T* const ring = reinterpret_cast<T*>(lds) + (size_t)key_wave * (kShape.stages * 2 * kKeys * kPitch);
-    const auto key_of = [&](int t) { return t < range.sink_tiles ? t * kKeys : range.first + (t - range.sink_tiles) * kKeys; };
-    const auto end_of = [&](int t) { return t < range.sink_tiles ? range.sink_end : range.end; };
     const auto fetch = [&](int t, int buffer) {
-        const int key0 = key_of(t), rows = end_of(t) - key0;
+        const int key0 = range.key_of(t, kKeys);
         T* const k_tile = ring + buffer * (2 * kKeys * kPitch);
         stage<T, kPitch, kKeys, kGroupThreads, VEC>(k_tile, k_base + (int64_t)key0 * a.k.stride[1], gt, d, [&](int r) {
-            return r < rows ? (uint32_t)r * k_pitch : kOutside;
+            return range.holds(t, key0 + r) ? (uint32_t)r * k_pitch : kOutside;
         });
         stage<T, kPitch, kKeys, kGroupThreads, VEC>(k_tile + kKeys * kPitch, v_base + (int64_t)key0 * a.v.stride[1], gt, d,
-                                                    [&](int r) { return r < rows ? (uint32_t)r * v_pitch : kOutside; });
+                                                    [&](int r) { return range.holds(t, key0 + r) ? (uint32_t)r * v_pitch : kOutside; });
     };
     constexpr int kInFlight = 2 * kKeys * L::kChunks / kGroupThreads;  // loads of one fetch, a wavefront
     const auto group_barrier = [&]() {
@@ -136,7 +163,7 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
         } else {
             // one wavefront: its LDS operations stay in order; what it has read is back before the place is filled again
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+            __builtin_amdgcn_s_waitcnt(kWaitForLds);
         }
     };
 
@@ -157,15 +184,15 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
         if (kShape.stages == 2 && more) {
             fetch(t + kShape.key_waves, buffer ^ 1);
             if constexpr (VEC) {
-                __builtin_amdgcn_s_waitcnt((kInFlight & 15) | ((kInFlight >> 4) << 14) | 0xf70);  // vmcnt(kInFlight)
+                __builtin_amdgcn_s_waitcnt(wait_for_loads(kInFlight));
             }
         } else if constexpr (VEC) {
-            __builtin_amdgcn_s_waitcnt(0xf70);  // vmcnt(0)
+            __builtin_amdgcn_s_waitcnt(wait_for_loads(0));
         }
         group_barrier();
         const T* const k_tile = ring + buffer * (2 * kKeys * kPitch);
         const T* const v_tile = k_tile + kKeys * kPitch;
-        const int key0 = key_of(t), end = end_of(t);
+        const int key0 = range.key_of(t, kKeys), end = range.end_of(t);
 
         acc_t s[kSubs];
 #pragma unroll
@@ -219,14 +246,18 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
                 total += s[j][r];
             }
         }
+        if (!all_seen && odd_values<T, kPitch, kKeys, NB>(v_tile, lane)) {
+            add_odd_values<T, kPitch, kSubs, NB>(o, s, v_tile, lane);
+        } else {
 #pragma unroll
-        for (int j = 0; j < kSubs; j++) {
+            for (int j = 0; j < kSubs; j++) {
 #pragma unroll
-            for (int g = 0; g < 2; g++) {
-                const Frag<T> w = operand<T>(s[j], g);
+                for (int g = 0; g < 2; g++) {
+                    const Frag<T> w = operand<T>(s[j], g);
 #pragma unroll
-                for (int i = 0; i < NB; i++) {
-                    o[i] = Mma<T>::mul(L::column(v_tile, j * kBlock + 16 * g, i, lane), w, o[i]);
+                    for (int i = 0; i < NB; i++) {
+                        o[i] = Mma<T>::mul(L::column(v_tile, j * kBlock + 16 * g, i, lane), w, o[i]);
+                    }
                 }
             }
         }
@@ -411,18 +442,14 @@ hipError_t run_forward(const AttentionArgs& a, hipStream_t stream)
     p.splits = (uint32_t)plan.splits;
     p.kv_heads = (uint32_t)a.kv_heads;
     p.blocks = (uint32_t)plan.blocks;
-    const int nb = VEC ? blocks_of(a.d) : (a.d <= 128 ? 4 : 8);  // odd sizes: two widths serve them all
     hipError_t e = hipErrorInvalidValue;
     const auto pick = [&](auto few) {
         constexpr bool kFew = decltype(few)::value;
-        switch (nb) {
+        switch (blocks_of(a.d)) {
             case 8: e = run_forward_shape<T, 8, kFew, VEC>(p, stream); break;
             case 4: e = run_forward_shape<T, 4, kFew, VEC>(p, stream); break;
-            default:
-                if constexpr (VEC) {
-                    e = nb == 3 ? run_forward_shape<T, 3, kFew, VEC>(p, stream) : run_forward_shape<T, 2, kFew, VEC>(p, stream);
-                }
-                break;
+            case 3: e = run_forward_shape<T, 3, kFew, VEC>(p, stream); break;
+        default: e = run_forward_shape<T, 2, kFew, VEC>(p, stream); break;
         }
     };
     plan.few_rows ? pick(std::true_type()) : pick(std::false_type());

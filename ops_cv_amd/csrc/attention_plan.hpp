@@ -66,5 +66,49 @@ inline ForwardPlan plan_forward(const AttentionArgs& a)
     return p;
 }
 
+// ---------------------------------------------------------------------------------------------------------- gradients
+
+// The keys' gradients: a workgroup has four wavefronts with 32 keys each and walks tiles of 32 queries of one head.
+constexpr int kKeyWaves = 4;
+constexpr int kGradKeys = kKeyWaves * kBlock;
+
+struct GradPlan {
+    int64_t rows = 0, tiles = 0;       // of the queries' gradients, as in the forward pass
+    int64_t key_tiles = 0;             // of a key head
+    int64_t sink_tiles = 0;            // the first of them, seen by queries of any position
+    int64_t sink_parts = 1, parts = 1; // parts that the queries of such a tile, and of the others, are cut into
+    // 32-bit words of the scratch: statistics of the rows, partial gradients of the sinks' tiles and of the others
+    int64_t stats = 0, sink_partials = 0, partials = 0;
+};
+
+inline GradPlan plan_grad(const AttentionArgs& a)
+{
+    GradPlan p;
+    const int64_t group = a.heads / a.kv_heads, bh = a.batch * a.kv_heads;
+    p.rows = a.tokens * group;
+    p.tiles = (p.rows + 4 * kBlock - 1) / (4 * kBlock);
+    p.key_tiles = (a.kv_tokens + kGradKeys - 1) / kGradKeys;
+    const int64_t sinks = a.sinks < a.kv_tokens ? a.sinks : a.kv_tokens;
+    p.sink_tiles = (sinks + kGradKeys - 1) / kGradKeys;
+    // steps (tiles of 32 queries, of every head of the group) of a tile of keys, at most
+    const int64_t all = (a.tokens + kBlock - 1) / kBlock;
+    const int64_t window = (a.left + a.right + kGradKeys + kBlock - 1) / kBlock + 1;
+    const int64_t steps = group * (window < all ? window : all);
+    // two workgroups for every CU where that leaves a part eight steps or more
+    const int64_t whole = bh * p.key_tiles > 0 ? bh * p.key_tiles : 1;
+    int64_t each = (steps * whole + 2 * a.compute_units - 1) / (2 * a.compute_units);
+    each = each < 8 ? 8 : each;
+    each = each < steps ? each : (steps > 0 ? steps : 1);
+    p.parts = (steps + each - 1) / each;
+    p.sink_parts = (group * all + each - 1) / each;
+    p.parts = p.parts < 1 ? 1 : p.parts;
+    p.sink_parts = p.sink_parts < 1 ? 1 : p.sink_parts;
+    p.stats = 3 * a.batch * a.heads * a.tokens;
+    const int64_t tile_floats = 2 * kGradKeys * ((a.d + 3) / 4 * 4);
+    p.sink_partials = p.sink_parts > 1 ? bh * p.sink_tiles * p.sink_parts * tile_floats : 0;
+    p.partials = p.parts > 1 ? bh * (p.key_tiles - p.sink_tiles) * p.parts * tile_floats : 0;
+    return p;
+}
+
 }  // namespace att
 }  // namespace opscv

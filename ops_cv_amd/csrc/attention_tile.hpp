@@ -254,7 +254,13 @@ static __device__ __forceinline__ Frag<T> global_row(const T* row, int first, in
 template <typename T, bool VEC>
 static __device__ __forceinline__ void put4(T* row, int first, int d, float a, float b, float c, float e)
 {
-    const float x[4] = {a, b, c, e};
+    float x[4] = {a, b, c, e};
+    // products are rounded to 32 bits before they are rounded to the type: without this the compiler fuses the two for
+    // FLOAT16 in one of the ways below and not in the other, and results would depend on the strides
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        __asm__("" : "+v"(x[i]));
+    }
     if constexpr (VEC) {
         if (first < d) {  // d is a multiple of four
             struct alignas(4 * sizeof(T)) Four {
@@ -275,6 +281,10 @@ static __device__ __forceinline__ void put4(T* row, int first, int d, float a, f
         }
     }
 }
+
+// operand of s_waitcnt: at most n loads to memory or LDS still under way (gfx9: the count is bits 0-3 and 14-15)
+constexpr int wait_for_loads(int n) { return (n & 15) | ((n >> 4) << 14) | 0xf70; }
+constexpr int kWaitForLds = 0xc07f;  // none of LDS
 
 // ---------------------------------------------------------------------------------------------------------- visibility
 
@@ -305,6 +315,51 @@ static __device__ __forceinline__ Sequence sequence_at(const AttentionArgs& a, i
 static __device__ __forceinline__ bool sees(int p, int j, int left, int right, int sinks)
 {
     return j <= p + right && (j >= p - left || j < sinks);
+}
+
+// Workgroups go round the eight XCDs; this gives every XCD a run of neighbouring numbers, so that the tiles of rows that
+// read the same keys share an L2.
+static __device__ __forceinline__ uint32_t xcd_order(uint32_t index, uint32_t count)
+{
+    const uint32_t each = (count + 7) / 8;
+    return (index & 7u) * each + (index >> 3);
+}
+
+// Keys that a range of rows sees, as tiles: the first `sink_tiles` start at key 0, the others at `first`.
+struct KeyRange {
+    int first, end;  // window
+    int sink_end;    // sinks in front of it
+    int gap_end;     // keys from sink_end to here, in the first tile of a joined run, are seen by none of the rows
+    int sink_tiles, tiles;
+
+    __device__ __forceinline__ int key_of(int t, int keys) const
+    {
+        return t < sink_tiles ? t * keys : first + (t - sink_tiles) * keys;
+    }
+    __device__ __forceinline__ int end_of(int t) const { return t < sink_tiles ? sink_end : end; }
+    // whether tile t has to hold this key: others are staged as zeros, whatever they are
+    __device__ __forceinline__ bool holds(int t, int key) const
+    {
+        return key < end_of(t) && (key < sink_end || key >= gap_end);
+    }
+};
+
+template <int KEYS>
+static __device__ __forceinline__ KeyRange key_range(int p_low, int p_high, int kv_len, int left, int right, int sinks)
+{
+    KeyRange k;
+    k.end = min(max(p_high + right + 1, 0), kv_len);
+    k.first = min(max(p_low - left, 0), k.end);
+    k.sink_end = min(sinks, k.first);
+    k.gap_end = k.sink_end;
+    k.sink_tiles = (k.sink_end + KEYS - 1) / KEYS;
+    if (k.sink_tiles > 0 && k.first <= k.sink_tiles * KEYS) {  // the window starts among them: one run of tiles
+        k.gap_end = k.first;
+        k.first = 0;
+        k.sink_tiles = 0;
+    }
+    k.tiles = k.sink_tiles + (k.end - k.first + KEYS - 1) / KEYS;
+    return k;
 }
 
 }  // namespace att

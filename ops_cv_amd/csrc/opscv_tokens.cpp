@@ -13,8 +13,10 @@ using namespace opscv;
 
 namespace {
 
-constexpr int64_t kMostExtent = (int64_t)1 << 30;  // positions and sums of positions and windows fit 32 bits
+constexpr int64_t kMostExtent = (int64_t)1 << 30;
 constexpr int64_t kMostTokenStride = (int64_t)1 << 22;  // elements
+// tokens of a sequence and reaches of a window: sums of any three fit 32 bits
+constexpr int64_t kMostTokens = (int64_t)1 << 28;
 constexpr int64_t kMostHeadDim = 256;
 constexpr int64_t kMostRotaryDim = 1024;
 
@@ -255,7 +257,8 @@ aclnnStatus check_attention(const char* api, const aclTensor* q, const aclTensor
     if (a->kv_heads < 1 || a->heads < 1 || a->heads % a->kv_heads != 0) {
         return invalid("%s: %lld heads cannot share %lld key heads", api, (long long)a->heads, (long long)a->kv_heads);
     }
-    if (!extents_fit(q) || !extents_fit(k) || a->batch * a->heads > INT32_MAX || a->tokens * a->heads > kMostExtent) {
+    if (!extents_fit(q) || !extents_fit(k) || a->batch * a->heads > INT32_MAX || a->tokens > kMostTokens ||
+        a->kv_tokens > kMostTokens || a->tokens * a->heads > kMostExtent) {
         return invalid("%s: extents too large", api);
     }
     for (const aclTensor* n : {q_lengths, kv_lengths}) {
@@ -270,9 +273,9 @@ aclnnStatus check_attention(const char* api, const aclTensor* q, const aclTensor
     if (!std::isfinite(a->scale) || !(a->scale > 0.0f)) {
         return invalid("%s: scale must be positive and finite", api);
     }
-    a->left = left < kMostExtent ? left : kMostExtent;
-    a->right = right < kMostExtent ? right : kMostExtent;
-    a->sinks = sinks < kMostExtent ? sinks : kMostExtent;
+    a->left = left < kMostTokens ? left : kMostTokens;
+    a->right = right < kMostTokens ? right : kMostTokens;
+    a->sinks = sinks < kMostTokens ? sinks : kMostTokens;
     a->compute_units = compute_unit_count();
     return ACLNN_SUCCESS;
 }

@@ -61,12 +61,12 @@ __device__ __forceinline__ void row_reduce(float& sum, float* most, float (*shar
     }
 }
 
-template <typename T, typename W, bool INT8, int VEC>
+template <typename T, typename W, bool INT8, int VEC, bool WIDE>
 __device__ __forceinline__ void put_row_part(const NormArgs& a, int64_t row, int64_t c, const float (&h)[VEC], float rstd,
                                              float step)
 {
     float w[VEC], y[VEC];
-    load<W, VEC>((const W*)a.weight + c, w);
+    load_part<W, VEC, WIDE>((const W*)a.weight, c, a.width, w);
     if constexpr (INT8) {
         Pack<int8_t, VEC> k;
 #pragma unroll
@@ -75,23 +75,33 @@ __device__ __forceinline__ void put_row_part(const NormArgs& a, int64_t row, int
             const float q = rintf(h[i] * w[i] * step);
             k.v[i] = step == 0.0f ? (int8_t)0 : (int8_t)(int)fminf(fmaxf(q, -127.0f), 127.0f);
         }
-        *reinterpret_cast<Pack<int8_t, VEC>*>((int8_t*)a.y.ptr + row * a.y.row_stride + c) = k;
+        int8_t* const to = (int8_t*)a.y.ptr + row * a.y.row_stride + c;
+        if constexpr (WIDE) {
+            *reinterpret_cast<Pack<int8_t, VEC>*>(to) = k;
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; i++) {
+                if (c + i < a.width) {
+                    to[i] = k.v[i];
+                }
+            }
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < VEC; i++) {
             y[i] = h[i] * w[i] * rstd;
         }
-        store<T, VEC>((T*)a.y.ptr + row * a.y.row_stride + c, y);
+        store_part<T, VEC, WIDE>((T*)a.y.ptr + row * a.y.row_stride, c, a.width, y);
     }
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool WIDE>
 __device__ __forceinline__ void get_row_part(const NormArgs& a, int64_t row, int64_t c, float (&h)[VEC])
 {
-    load<T, VEC>((const T*)a.x.ptr + row * a.x.row_stride + c, h);
+    load_part<T, VEC, WIDE>((const T*)a.x.ptr + row * a.x.row_stride, c, a.width, h);
     if (a.residual.ptr != nullptr) {
         float r[VEC];
-        load<T, VEC>((const T*)a.residual.ptr + row * a.residual.row_stride + c, r);
+        load_part<T, VEC, WIDE>((const T*)a.residual.ptr + row * a.residual.row_stride, c, a.width, r);
 #pragma unroll
         for (int i = 0; i < VEC; i++) {
             h[i] += r[i];
@@ -108,7 +118,7 @@ __device__ __forceinline__ float int8_step(float most, float rstd, float* scale)
 }
 
 // THREADS per row; a workgroup is 256 threads, or THREADS where that is more.  NV vectors of VEC elements a thread.
-template <typename T, typename W, bool INT8, int THREADS, int NV, int VEC>
+template <typename T, typename W, bool INT8, int THREADS, int NV, int VEC, bool WIDE>
 __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void norm_kernel(NormArgs a)
 {
     constexpr int kRows = THREADS >= 256 ? 1 : 256 / THREADS;
@@ -123,7 +133,7 @@ __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void norm_kernel(Nor
         for (int j = 0; j < NV; j++) {
             const int64_t c = ((int64_t)j * THREADS + lane) * VEC;
             if (c < a.width) {
-                get_row_part<T, VEC>(a, row, c, h[j]);
+                get_row_part<T, VEC, WIDE>(a, row, c, h[j]);
             } else {
 #pragma unroll
                 for (int i = 0; i < VEC; i++) {
@@ -140,11 +150,11 @@ __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void norm_kernel(Nor
             }
             if (c < a.width) {
                 if (a.sum.ptr != nullptr) {
-                    store<T, VEC>((T*)a.sum.ptr + row * a.sum.row_stride + c, h[j]);
+                    store_part<T, VEC, WIDE>((T*)a.sum.ptr + row * a.sum.row_stride, c, a.width, h[j]);
                 }
                 if constexpr (INT8) {
                     float w[VEC];
-                    load<W, VEC>((const W*)a.weight + c, w);
+                    load_part<W, VEC, WIDE>((const W*)a.weight, c, a.width, w);
 #pragma unroll
                     for (int i = 0; i < VEC; i++) {
                         most = larger(most, fabsf(h[j][i] * w[i]));
@@ -169,7 +179,7 @@ __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void norm_kernel(Nor
         for (int j = 0; j < NV; j++) {
             const int64_t c = ((int64_t)j * THREADS + lane) * VEC;
             if (c < a.width) {
-                put_row_part<T, W, INT8, VEC>(a, row, c, h[j], rstd, step);
+                put_row_part<T, W, INT8, VEC, WIDE>(a, row, c, h[j], rstd, step);
             }
         }
     }
@@ -177,7 +187,7 @@ __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void norm_kernel(Nor
 
 // Rows longer than 1024 threads hold: read once for the statistics and once more for the result (`sum` is written in the
 // second pass, since it may be x).
-template <typename T, typename W, bool INT8, int VEC>
+template <typename T, typename W, bool INT8, int VEC, bool WIDE>
 __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a)
 {
     __shared__ float shared[2][2][16];
@@ -186,8 +196,8 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a)
     float sum = 0.0f, most = 0.0f;
     for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.width; c += 1024 * VEC) {
         float h[VEC], w[VEC];
-        get_row_part<T, VEC>(a, row, c, h);
-        load<W, VEC>((const W*)a.weight + c, w);
+        get_row_part<T, VEC, WIDE>(a, row, c, h);
+        load_part<W, VEC, WIDE>((const W*)a.weight, c, a.width, w);
 #pragma unroll
         for (int i = 0; i < VEC; i++) {
             sum += h[i] * h[i];
@@ -209,33 +219,33 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a)
     }
     for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.width; c += 1024 * VEC) {
         float h[VEC];
-        get_row_part<T, VEC>(a, row, c, h);
+        get_row_part<T, VEC, WIDE>(a, row, c, h);
         if (a.sum.ptr != nullptr) {
-            store<T, VEC>((T*)a.sum.ptr + row * a.sum.row_stride + c, h);
+            store_part<T, VEC, WIDE>((T*)a.sum.ptr + row * a.sum.row_stride, c, a.width, h);
         }
-        put_row_part<T, W, INT8, VEC>(a, row, c, h, rstd, step);
+        put_row_part<T, W, INT8, VEC, WIDE>(a, row, c, h, rstd, step);
     }
     }
 }
 
-template <typename T, typename W, bool INT8, int VEC>
+template <typename T, typename W, bool INT8, int VEC, bool WIDE>
 hipError_t run_norm(const NormArgs& a, hipStream_t stream)
 {
     constexpr int kVectors = kMostPerLane / VEC;
     const int64_t vectors = (a.width + VEC - 1) / VEC;
     if (vectors <= 64 * kVectors / 2) {
-        hipLaunchKernelGGL((norm_kernel<T, W, INT8, 64, kVectors / 2, VEC>), grid((a.rows + 3) / 4), dim3(256),
+        hipLaunchKernelGGL((norm_kernel<T, W, INT8, 64, kVectors / 2, VEC, WIDE>), grid((a.rows + 3) / 4), dim3(256),
                            0, stream, a);
     } else if (vectors <= 256 * kVectors / 2) {
-        hipLaunchKernelGGL((norm_kernel<T, W, INT8, 256, kVectors / 2, VEC>), grid(a.rows), dim3(256), 0, stream,
+        hipLaunchKernelGGL((norm_kernel<T, W, INT8, 256, kVectors / 2, VEC, WIDE>), grid(a.rows), dim3(256), 0, stream,
                            a);
     } else if (vectors <= 256 * kVectors) {
-        hipLaunchKernelGGL((norm_kernel<T, W, INT8, 256, kVectors, VEC>), grid(a.rows), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((norm_kernel<T, W, INT8, 256, kVectors, VEC, WIDE>), grid(a.rows), dim3(256), 0, stream, a);
     } else if (vectors <= 1024 * kVectors) {
-        hipLaunchKernelGGL((norm_kernel<T, W, INT8, 1024, kVectors, VEC>), grid(a.rows), dim3(1024), 0, stream,
+        hipLaunchKernelGGL((norm_kernel<T, W, INT8, 1024, kVectors, VEC, WIDE>), grid(a.rows), dim3(1024), 0, stream,
                            a);
     } else {
-        hipLaunchKernelGGL((norm_long_kernel<T, W, INT8, VEC>), grid(a.rows), dim3(1024), 0, stream, a);
+        hipLaunchKernelGGL((norm_long_kernel<T, W, INT8, VEC, WIDE>), grid(a.rows), dim3(1024), 0, stream, a);
     }
     return hipGetLastError();
 }
@@ -245,23 +255,23 @@ hipError_t run_norm_type(const NormArgs& a, hipStream_t stream)
 {
     constexpr int kVec = 16 / (int)sizeof(T);
     const int e = (int)sizeof(T), ye = a.int8 != 0 ? 1 : e;
-    // vectors where every row starts on one, single elements otherwise
+    // whole vectors where every row starts on one, their elements one by one otherwise
     const bool vectors = a.width % kVec == 0 && aligned(a.x.ptr, a.x.row_stride, e, 16) &&
                          aligned(a.residual.ptr, a.residual.row_stride, e, 16) &&
                          aligned(a.sum.ptr, a.sum.row_stride, e, 16) &&
                          aligned(a.y.ptr, a.y.row_stride, ye, kVec * ye) &&
                          aligned(a.weight, 0, 1, kVec * (int)sizeof(W));
     if (a.int8 != 0) {
-        return vectors ? run_norm<T, W, true, kVec>(a, stream) : run_norm<T, W, true, 1>(a, stream);
+        return vectors ? run_norm<T, W, true, kVec, true>(a, stream) : run_norm<T, W, true, kVec, false>(a, stream);
     }
-    return vectors ? run_norm<T, W, false, kVec>(a, stream) : run_norm<T, W, false, 1>(a, stream);
+    return vectors ? run_norm<T, W, false, kVec, true>(a, stream) : run_norm<T, W, false, kVec, false>(a, stream);
 }
 
 // ------------------------------------------------------------------------------------------------------ gradients
 
 // Gradient of the rows, and of the weight's columns over the rows of one workgroup, which it adds up in registers and
 // leaves in its row of `partial`.  THREADS per row; wavefronts of 64-thread rows join their sums through LDS.
-template <typename T, typename W, int THREADS, int NV, int VEC, bool WEIGHT>
+template <typename T, typename W, int THREADS, int NV, int VEC, bool WIDE, bool WEIGHT>
 __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void norm_grad_kernel(NormGradArgs a)
 {
     constexpr int kRows = THREADS >= 256 ? 1 : 256 / THREADS;
@@ -276,7 +286,7 @@ __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void norm_grad_kerne
             total[j][i] = w[j][i] = 0.0f;
         }
         if (c < a.width) {
-            load<W, VEC>((const W*)a.weight + c, w[j]);
+            load_part<W, VEC, WIDE>((const W*)a.weight, c, a.width, w[j]);
         }
     }
     int slot = 0;
@@ -290,8 +300,8 @@ __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void norm_grad_kerne
         for (int j = 0; j < NV; j++) {
             const int64_t c = ((int64_t)j * THREADS + lane) * VEC;
             if (c < a.width) {
-                load<T, VEC>((const T*)a.sum.ptr + row * a.sum.row_stride + c, n[j]);
-                load<T, VEC>((const T*)a.grad_y.ptr + row * a.grad_y.row_stride + c, g[j]);
+                load_part<T, VEC, WIDE>((const T*)a.sum.ptr + row * a.sum.row_stride, c, a.width, n[j]);
+                load_part<T, VEC, WIDE>((const T*)a.grad_y.ptr + row * a.grad_y.row_stride, c, a.width, g[j]);
             } else {
 #pragma unroll
                 for (int i = 0; i < VEC; i++) {
@@ -320,13 +330,13 @@ __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void norm_grad_kerne
             if (c < a.width) {
                 float s[VEC] = {0.0f};
                 if (a.grad_sum.ptr != nullptr) {
-                    load<T, VEC>((const T*)a.grad_sum.ptr + row * a.grad_sum.row_stride + c, s);
+                    load_part<T, VEC, WIDE>((const T*)a.grad_sum.ptr + row * a.grad_sum.row_stride, c, a.width, s);
                 }
 #pragma unroll
                 for (int i = 0; i < VEC; i++) {
                     s[i] += (g[j][i] - n[j][i] * along) * rstd;
                 }
-                store<T, VEC>((T*)a.grad_x.ptr + row * a.grad_x.row_stride + c, s);
+                store_part<T, VEC, WIDE>((T*)a.grad_x.ptr + row * a.grad_x.row_stride, c, a.width, s);
             }
         }
     }
@@ -364,7 +374,7 @@ __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void norm_grad_kerne
 
 // Rows longer than 1024 threads hold, read twice: the sum along the row, then the gradient.  The weight's gradient comes
 // from norm_weight_long_kernel.
-template <typename T, typename W, int VEC>
+template <typename T, typename W, int VEC, bool WIDE>
 __global__ __launch_bounds__(1024) void norm_grad_long_kernel(NormGradArgs a)
 {
     __shared__ float shared[2][2][16];
@@ -376,9 +386,9 @@ __global__ __launch_bounds__(1024) void norm_grad_long_kernel(NormGradArgs a)
     float along = 0.0f;
     for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.width; c += 1024 * VEC) {
         float n[VEC], g[VEC], w[VEC];
-        load<T, VEC>(sum + c, n);
-        load<T, VEC>(gy + c, g);
-        load<W, VEC>((const W*)a.weight + c, w);
+        load_part<T, VEC, WIDE>(sum, c, a.width, n);
+        load_part<T, VEC, WIDE>(gy, c, a.width, g);
+        load_part<W, VEC, WIDE>((const W*)a.weight, c, a.width, w);
 #pragma unroll
         for (int i = 0; i < VEC; i++) {
             along += g[i] * w[i] * (n[i] * rstd);
@@ -389,17 +399,17 @@ __global__ __launch_bounds__(1024) void norm_grad_long_kernel(NormGradArgs a)
     along /= (float)a.width;
     for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.width; c += 1024 * VEC) {
         float n[VEC], g[VEC], w[VEC], s[VEC] = {0.0f};
-        load<T, VEC>(sum + c, n);
-        load<T, VEC>(gy + c, g);
-        load<W, VEC>((const W*)a.weight + c, w);
+        load_part<T, VEC, WIDE>(sum, c, a.width, n);
+        load_part<T, VEC, WIDE>(gy, c, a.width, g);
+        load_part<W, VEC, WIDE>((const W*)a.weight, c, a.width, w);
         if (a.grad_sum.ptr != nullptr) {
-            load<T, VEC>((const T*)a.grad_sum.ptr + row * a.grad_sum.row_stride + c, s);
+            load_part<T, VEC, WIDE>((const T*)a.grad_sum.ptr + row * a.grad_sum.row_stride, c, a.width, s);
         }
 #pragma unroll
         for (int i = 0; i < VEC; i++) {
             s[i] += (g[i] * w[i] - n[i] * rstd * along) * rstd;
         }
-        store<T, VEC>((T*)a.grad_x.ptr + row * a.grad_x.row_stride + c, s);
+        store_part<T, VEC, WIDE>((T*)a.grad_x.ptr + row * a.grad_x.row_stride, c, a.width, s);
     }
     }
 }
@@ -446,19 +456,19 @@ __global__ __launch_bounds__(256) void norm_weight_kernel(const float* __restric
     }
 }
 
-template <typename T, typename W, int THREADS, int NV, int VEC>
+template <typename T, typename W, int THREADS, int NV, int VEC, bool WIDE>
 void launch_norm_grad(const NormGradArgs& a, int64_t blocks, hipStream_t stream)
 {
     if (a.grad_weight != nullptr) {
-        hipLaunchKernelGGL((norm_grad_kernel<T, W, THREADS, NV, VEC, true>), dim3((unsigned)blocks),
+        hipLaunchKernelGGL((norm_grad_kernel<T, W, THREADS, NV, VEC, WIDE, true>), dim3((unsigned)blocks),
                            dim3(THREADS > 256 ? THREADS : 256), 0, stream, a);
     } else {
-        hipLaunchKernelGGL((norm_grad_kernel<T, W, THREADS, NV, VEC, false>), dim3((unsigned)blocks),
+        hipLaunchKernelGGL((norm_grad_kernel<T, W, THREADS, NV, VEC, WIDE, false>), dim3((unsigned)blocks),
                            dim3(THREADS > 256 ? THREADS : 256), 0, stream, a);
     }
 }
 
-template <typename T, typename W, int VEC>
+template <typename T, typename W, int VEC, bool WIDE>
 hipError_t run_norm_grad(const NormGradArgs& a, hipStream_t stream)
 {
     constexpr int kVectors = kMostPerLane / VEC;
@@ -470,20 +480,20 @@ hipError_t run_norm_grad(const NormGradArgs& a, hipStream_t stream)
     };
     if (a.rows > 0 || a.grad_weight != nullptr) {
         if (vectors <= 64 * kVectors / 2) {
-            launch_norm_grad<T, W, 64, kVectors / 2, VEC>(a, blocks(4), stream);
+            launch_norm_grad<T, W, 64, kVectors / 2, VEC, WIDE>(a, blocks(4), stream);
         } else if (vectors <= 256 * kVectors / 2) {
-            launch_norm_grad<T, W, 256, kVectors / 2, VEC>(a, blocks(1), stream);
+            launch_norm_grad<T, W, 256, kVectors / 2, VEC, WIDE>(a, blocks(1), stream);
         } else if (vectors <= 256 * kVectors) {
-            launch_norm_grad<T, W, 256, kVectors, VEC>(a, blocks(1), stream);
+            launch_norm_grad<T, W, 256, kVectors, VEC, WIDE>(a, blocks(1), stream);
         } else if (vectors <= 1024 * kVectors) {
-            launch_norm_grad<T, W, 1024, kVectors, VEC>(a, blocks(1), stream);
+            launch_norm_grad<T, W, 1024, kVectors, VEC, WIDE>(a, blocks(1), stream);
         } else {
             if (a.grad_weight != nullptr) {
                 hipLaunchKernelGGL((norm_weight_long_kernel<T>), dim3((unsigned)((a.width + 255) / 256), (unsigned)partials),
                                    dim3(256), 0, stream, a);
             }
             if (a.rows > 0) {
-                hipLaunchKernelGGL((norm_grad_long_kernel<T, W, VEC>), grid(a.rows), dim3(1024), 0, stream, a);
+                hipLaunchKernelGGL((norm_grad_long_kernel<T, W, VEC, WIDE>), grid(a.rows), dim3(1024), 0, stream, a);
             }
         }
     }
@@ -504,7 +514,7 @@ hipError_t run_norm_grad_type(const NormGradArgs& a, hipStream_t stream)
                          aligned(a.sum.ptr, a.sum.row_stride, e, 16) &&
                          aligned(a.grad_x.ptr, a.grad_x.row_stride, e, 16) &&
                          aligned(a.weight, 0, 1, kVec * (int)sizeof(W));
-    return vectors ? run_norm_grad<T, W, kVec>(a, stream) : run_norm_grad<T, W, 1>(a, stream);
+    return vectors ? run_norm_grad<T, W, kVec, true>(a, stream) : run_norm_grad<T, W, kVec, false>(a, stream);
 }
 
 // f(T, W) by the operands' types

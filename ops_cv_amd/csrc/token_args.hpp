@@ -67,7 +67,7 @@ struct RotaryArgs {
 struct AttentionArgs {
     int elem = 0;
     int64_t batch = 0, tokens = 0, kv_tokens = 0, heads = 0, kv_heads = 0, d = 0;
-    int64_t left = 0, right = 0, sinks = 0;  // clamped to 2^30 by the first phase
+    int64_t left = 0, right = 0, sinks = 0;  // clamped to 2^28 by the first phase
     float scale = 0.0f;
     int compute_units = 0;  // of the device that was current in the first phase: how far the keys are split
     Strided q, k, v, out;   // strides of batch, token, head

@@ -34,6 +34,36 @@ static __device__ __forceinline__ void store(T* p, const float (&x)[N])
     *reinterpret_cast<Pack<T, N>*>(p) = k;
 }
 
+// Elements c .. c + N - 1 of a row of `width`: whole vectors (WIDE; c + N <= width), or one by one, zeros from the row's
+// end on.  Both ways a lane owns the same elements, so sums over lanes do not depend on a row's alignment.
+template <typename T, int N, bool WIDE>
+static __device__ __forceinline__ void load_part(const T* row, int64_t c, int64_t width, float (&x)[N])
+{
+    if constexpr (WIDE) {
+        load<T, N>(row + c, x);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            x[i] = c + i < width ? (float)row[c + i] : 0.0f;
+        }
+    }
+}
+
+template <typename T, int N, bool WIDE>
+static __device__ __forceinline__ void store_part(T* row, int64_t c, int64_t width, const float (&x)[N])
+{
+    if constexpr (WIDE) {
+        store<T, N>(row + c, x);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if (c + i < width) {
+                row[c + i] = (T)x[i];
+            }
+        }
+    }
+}
+
 static __device__ __forceinline__ float wave_sum(float v)
 {
 #pragma unroll
