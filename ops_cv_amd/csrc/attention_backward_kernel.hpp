@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256) void attention_stats_kernel(GradLaunch p, uint
 constexpr ForwardShape query_grad_shape(int elem_bytes, int pitch) { return forward_shape(elem_bytes, pitch, false); }
 
 template <typename T, int NB, bool VEC>
-__global__ __launch_bounds__(256, 1) void attention_query_grad_kernel(GradLaunch p)
+__global__ __launch_bounds__(256, sizeof(T) * NB <= 8 ? 2 : 1) void attention_query_grad_kernel(GradLaunch p)
 {
     constexpr int kPitch = pitch_of(NB);
     constexpr ForwardShape kShape = query_grad_shape(sizeof(T), kPitch);
@@ -111,7 +111,7 @@ __global__ __launch_bounds__(256, 1) void attention_query_grad_kernel(GradLaunch
     const uint32_t tile = index % p.tiles, bh = index / p.tiles;
     const uint32_t b = bh / p.kv_heads, kv_head = bh % p.kv_heads;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
-    const int h = lane >> 5, own = lane & 31, gt = wave * 64 + lane;
+    const int h = lane >> 5, own = lane & 31;
     const int d = (int)a.d, left = (int)a.left, right = (int)a.right, sinks = (int)a.sinks;
     const Sequence seq = sequence_at(a, b);
 
@@ -129,6 +129,29 @@ __global__ __launch_bounds__(256, 1) void attention_query_grad_kernel(GradLaunch
     const int wave_low = seq.first + query_of(wave_row0), wave_high = seq.first + query_of(wave_row0 + kBlock - 1);
     const bool wave_whole = query_of(wave_row0 + kBlock - 1) < seq.q_len;
 
+    const T* const k_base = (const T*)a.k.ptr + (int64_t)b * a.k.stride[0] + (int64_t)kv_head * a.k.stride[2];
+    const T* const v_base = (const T*)a.v.ptr + (int64_t)b * a.v.stride[0] + (int64_t)kv_head * a.v.stride[2];
+    const uint32_t k_pitch = (uint32_t)(a.k.stride[1] * (int64_t)sizeof(T));
+    const uint32_t v_pitch = (uint32_t)(a.v.stride[1] * (int64_t)sizeof(T));
+    T* const ring = reinterpret_cast<T*>(lds);
+    const auto fetch = [&](int t, int buffer) {
+        const int key0 = range.key_of(t, kKeys), rows = range.end_of(t) - key0;
+        T* const k_tile = ring + buffer * (2 * kKeys * kPitch);
+        const int gt = wave * 64 + again(lane);
+        stage<T, kPitch, kKeys, kThreads, VEC>(k_tile, k_base + (int64_t)key0 * a.k.stride[1], gt, wave, d, k_pitch, min(rows, kKeys));
+        stage<T, kPitch, kKeys, kThreads, VEC>(k_tile + kKeys * kPitch, v_base + (int64_t)key0 * a.v.stride[1], gt, wave, d, v_pitch,
+                                         min(rows, kKeys));
+    };
+    const float c = a.scale * kLog2e;
+    acc_t gq[NB];
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        gq[i] = zeros();
+    }
+    int buffer = 0;
+    if (range.tiles > 0) {
+        fetch(0, 0);
+    }
     Frag<T> q[2 * NB], go[2 * NB];
     {
         const T* const src = (const T*)a.q.ptr + (int64_t)b * a.q.stride[0] + (int64_t)query * a.q.stride[1] +
@@ -144,44 +167,14 @@ __global__ __launch_bounds__(256, 1) void attention_query_grad_kernel(GradLaunch
     const float* const stat = p.stats + stats_row(a, b, head) + query;
     const float lse = stat[0], along = stat[a.tokens];
     const float unit = kUnits ? stat[2 * a.tokens] : 1.0f, per_unit = unit > 0.0f ? 1.0f / unit : 0.0f;
-
-    const T* const k_base = (const T*)a.k.ptr + (int64_t)b * a.k.stride[0] + (int64_t)kv_head * a.k.stride[2];
-    const T* const v_base = (const T*)a.v.ptr + (int64_t)b * a.v.stride[0] + (int64_t)kv_head * a.v.stride[2];
-    const uint32_t k_pitch = (uint32_t)(a.k.stride[1] * (int64_t)sizeof(T));
-    const uint32_t v_pitch = (uint32_t)(a.v.stride[1] * (int64_t)sizeof(T));
-    T* const ring = reinterpret_cast<T*>(lds);
-    const auto fetch = [&](int t, int buffer) {
-        const int key0 = range.key_of(t, kKeys);
-        T* const k_tile = ring + buffer * (2 * kKeys * kPitch);
-        stage<T, kPitch, kKeys, kThreads, VEC>(k_tile, k_base + (int64_t)key0 * a.k.stride[1], gt, d, [&](int r) {
-            return range.holds(t, key0 + r) ? (uint32_t)r * k_pitch : kOutside;
-        });
-        stage<T, kPitch, kKeys, kThreads, VEC>(k_tile + kKeys * kPitch, v_base + (int64_t)key0 * a.v.stride[1], gt, d,
-                                               [&](int r) { return range.holds(t, key0 + r) ? (uint32_t)r * v_pitch : kOutside; });
-    };
-    constexpr int kInFlight = 2 * kKeys * L::kChunks / kThreads;
-
-    const float c = a.scale * kLog2e;
-    acc_t gq[NB];
-#pragma unroll
-    for (int i = 0; i < NB; i++) {
-        gq[i] = zeros();
-    }
-    int buffer = 0;
-    if (range.tiles > 0) {
-        fetch(0, 0);
-    }
+    wait_for_registers();
     for (int t = 0; t < range.tiles; t++) {
         const bool more = t + 1 < range.tiles;
+        wait_for_loads<0>();  // as in the forward pass
+        barrier();
         if (kShape.stages == 2 && more) {
             fetch(t + 1, buffer ^ 1);
-            if constexpr (VEC) {
-                __builtin_amdgcn_s_waitcnt(wait_for_loads(kInFlight));
-            }
-        } else if constexpr (VEC) {
-            __builtin_amdgcn_s_waitcnt(wait_for_loads(0));
         }
-        __syncthreads();
         const T* const k_tile = ring + buffer * (2 * kKeys * kPitch);
         const T* const v_tile = k_tile + kKeys * kPitch;
         const int key0 = range.key_of(t, kKeys), end = range.end_of(t);
@@ -190,32 +183,41 @@ __global__ __launch_bounds__(256, 1) void attention_query_grad_kernel(GradLaunch
 #pragma unroll
         for (int j = 0; j < kSubs; j++) {
             acc_t s = zeros(), dp = zeros();
+            const int ln = again(lane);
 #pragma unroll
             for (int i = 0; i < 2 * NB; i++) {
-                s = Mma<T>::mul(L::row(k_tile, j * kBlock + own, 2 * i + h), q[i], s);
-                dp = Mma<T>::mul(L::row(v_tile, j * kBlock + own, 2 * i + h), go[i], dp);
+                s = Mma<T>::mul(L::row(k_tile, j * kBlock + (ln & 31), 2 * i + (ln >> 5)), q[i], s);
+                dp = Mma<T>::mul(L::row(v_tile, j * kBlock + (ln & 31), 2 * i + (ln >> 5)), go[i], dp);
+            }
+            if constexpr (sizeof(T) == 2) {
+                read_ahead<4 * NB, 1, 4>();
             }
 #pragma unroll
             for (int r = 0; r < 16; r++) {
-                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -lse)) * ((dp[r] - along) * per_unit);
-                if (!all_seen) {
-                    const int key = key0 + j * kBlock + 8 * (r / 4) + 4 * h + r % 4;
-                    s[r] = (key < end && sees(pos, key, left, right, sinks)) ? x : 0.0f;
-                } else {
-                    s[r] = x;
+                s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -lse)) * ((dp[r] - along) * per_unit);
+            }
+            if (__builtin_expect(!all_seen, 0)) {
+                const Sight see = sight(pos, key0 + j * kBlock + 4 * h, end, left, right, sinks);
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    s[r] = see.sees(8 * (r / 4) + r % 4) ? s[r] : 0.0f;
                 }
             }
+            const int k_lane = again(lane);
 #pragma unroll
             for (int g = 0; g < 2; g++) {
                 const Frag<T> w = operand<T>(s, g);
 #pragma unroll
                 for (int i = 0; i < NB; i++) {
-                    gq[i] = Mma<T>::mul(L::column(k_tile, j * kBlock + 16 * g, i, lane), w, gq[i]);
+                    gq[i] = Mma<T>::mul(L::column(k_tile, j * kBlock + 16 * g, i, k_lane), w, gq[i]);
                 }
             }
+            if constexpr (sizeof(T) == 2) {
+                read_ahead<2 * NB, 2, 3>();
+            }
         }
-        __syncthreads();
         if (kShape.stages == 1 && more) {
+            barrier();
             fetch(t + 1, 0);
         }
         buffer ^= kShape.stages - 1;
@@ -265,7 +267,7 @@ __global__ __launch_bounds__(64 * kKeyWaves, 1) void attention_key_grad_kernel(G
     const uint32_t part = at % of, local_tile = at / of, tile = local_tile + (sink_tile ? 0 : p.sink_tiles);
     const uint32_t b = bh / p.kv_heads, kv_head = bh % p.kv_heads;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
-    const int h = lane >> 5, own = lane & 31, gt = wave * 64 + lane;
+    const int h = lane >> 5, own = lane & 31;
     const int d = (int)a.d, left = (int)a.left, right = (int)a.right, sinks = (int)a.sinks;
     const Sequence seq = sequence_at(a, b);
 
@@ -281,17 +283,6 @@ __global__ __launch_bounds__(64 * kKeyWaves, 1) void attention_key_grad_kernel(G
     const int steps = row_tiles * (int)p.group.div;
     const int s_begin = (int)((int64_t)steps * part / of), s_end = (int)((int64_t)steps * (part + 1) / of);
 
-    Frag<T> k[2 * NB], v[2 * NB];
-    {
-        const int64_t from = min(key, (int)a.kv_tokens - 1);
-        const T* const ks = (const T*)a.k.ptr + (int64_t)b * a.k.stride[0] + from * a.k.stride[1] + (int64_t)kv_head * a.k.stride[2];
-        const T* const vs = (const T*)a.v.ptr + (int64_t)b * a.v.stride[0] + from * a.v.stride[1] + (int64_t)kv_head * a.v.stride[2];
-#pragma unroll
-        for (int i = 0; i < 2 * NB; i++) {
-            k[i] = global_row<T, VEC>(ks, 16 * i + 8 * h, d);
-            v[i] = global_row<T, VEC>(vs, 16 * i + 8 * h, d);
-        }
-    }
     T* const ring = reinterpret_cast<T*>(lds);
     float* const stat_ring = reinterpret_cast<float*>(lds + (size_t)kStages * 2 * kTile * sizeof(T)) +
                              wave * (kStages * kStatRows * kBlock);
@@ -306,23 +297,20 @@ __global__ __launch_bounds__(64 * kKeyWaves, 1) void attention_key_grad_kernel(G
                                  head * a.grad_out.stride[2];
         const int rows = seq.q_len - i0;
         T* const q_tile = ring + buffer * (2 * kTile);
-        stage<T, kPitch, kBlock, kThreads, VEC>(q_tile, q_base, gt, d, [&](int r) { return r < rows ? (uint32_t)r * q_pitch : kOutside; });
-        stage<T, kPitch, kBlock, kThreads, VEC>(q_tile + kTile, go_base, gt, d,
-                                                [&](int r) { return r < rows ? (uint32_t)r * go_pitch : kOutside; });
+        const int gt = wave * 64 + again(lane);
+        stage<T, kPitch, kBlock, kThreads, VEC>(q_tile, q_base, gt, wave, d, q_pitch, min(rows, kBlock));
+        stage<T, kPitch, kBlock, kThreads, VEC>(q_tile + kTile, go_base, gt, wave, d, go_pitch, min(rows, kBlock));
         // statistics: lanes of the lower half read one kind, of the upper half the next; rows past the end read zeros,
         // which meet rows of zeros
-        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
-            p.stats + stats_row(a, b, head) + i0, 0, 0x7fffffff, kBufferFlags);
+        const rsrc_t rsrc = att::buffer(p.stats + stats_row(a, b, head) + i0, 0x7fffffffu);
         float* const to = stat_ring + buffer * (kStatRows * kBlock);
 #pragma unroll
         for (int n = 0; n < kStatRows / 2; n++) {
             const int kind = 2 * n + h;
             const uint32_t off = (own < rows && kind < 3) ? (uint32_t)(kind * (int)a.tokens + own) * 4u : kOutside;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)(to + n * 2 * kBlock), 4, (int)off, 0, 0, 0);
+            load_to_lds<4>(rsrc, to + n * 2 * kBlock, off);
         }
     };
-    constexpr int kInFlight = (VEC ? 2 * kBlock * L::kChunks / kThreads : 0) + kStatRows / 2;
-
     const float c = a.scale * kLog2e;
     acc_t gk[NB], gv[NB];
 #pragma unroll
@@ -335,15 +323,25 @@ __global__ __launch_bounds__(64 * kKeyWaves, 1) void attention_key_grad_kernel(G
     if (s_begin < s_end) {
         fetch(s_begin, 0);
     }
+    Frag<T> k[2 * NB], v[2 * NB];
+    {
+        const int64_t from = min(key, (int)a.kv_tokens - 1);
+        const T* const ks = (const T*)a.k.ptr + (int64_t)b * a.k.stride[0] + from * a.k.stride[1] + (int64_t)kv_head * a.k.stride[2];
+        const T* const vs = (const T*)a.v.ptr + (int64_t)b * a.v.stride[0] + from * a.v.stride[1] + (int64_t)kv_head * a.v.stride[2];
+#pragma unroll
+        for (int i = 0; i < 2 * NB; i++) {
+            k[i] = global_row<T, VEC>(ks, 16 * i + 8 * h, d);
+            v[i] = global_row<T, VEC>(vs, 16 * i + 8 * h, d);
+        }
+    }
+    wait_for_registers();
     for (int step = s_begin; step < s_end; step++) {
         const bool more = step + 1 < s_end;
+        wait_for_loads<0>();
+        barrier();
         if (kStages == 2 && more) {
             fetch(step + 1, buffer ^ 1);
-            __builtin_amdgcn_s_waitcnt(wait_for_loads(kInFlight));
-        } else {
-            __builtin_amdgcn_s_waitcnt(wait_for_loads(0));
         }
-        __syncthreads();
         const T* const q_tile = ring + buffer * (2 * kTile);
         const T* const go_tile = q_tile + kTile;
         const float* const stat = stat_ring + buffer * (kStatRows * kBlock);
@@ -375,36 +373,49 @@ __global__ __launch_bounds__(64 * kKeyWaves, 1) void attention_key_grad_kernel(G
                 }
             }
             acc_t s = zeros(), dp = zeros();
+            const int ln = again(lane);
 #pragma unroll
             for (int i = 0; i < 2 * NB; i++) {
-                s = Mma<T>::mul(L::row(q_tile, own, 2 * i + h), k[i], s);
-                dp = Mma<T>::mul(L::row(go_tile, own, 2 * i + h), v[i], dp);
+                s = Mma<T>::mul(L::row(q_tile, ln & 31, 2 * i + (ln >> 5)), k[i], s);
+                dp = Mma<T>::mul(L::row(go_tile, ln & 31, 2 * i + (ln >> 5)), v[i], dp);
+            }
+            if constexpr (sizeof(T) == 2) {
+                read_ahead<4 * NB, 1, 6>();
             }
 #pragma unroll
             for (int r = 0; r < 16; r++) {
                 const int n = 8 * (r / 4) + 4 * h + r % 4;
-                float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -stat[n]));
-                float y = x * ((dp[r] - stat[kBlock + n]) * per_unit);
-                if (!all_seen) {
-                    const bool seen = key < seq.kv_len && sees(p_low + n, key, left, right, sinks);
-                    x = seen ? x : 0.0f;
-                    y = seen ? y : 0.0f;
-                }
-                s[r] = x;
-                dp[r] = y;
+                s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -stat[n]));
+                dp[r] = s[r] * ((dp[r] - stat[kBlock + n]) * per_unit);
             }
+            if (__builtin_expect(!all_seen, 0)) {
+                // query p_low + n sees the key: n >= first, n <= last or the key a sink, the key within the sequence
+                const int first = key - right - p_low - 4 * h;
+                const int last = key >= seq.kv_len ? -1 : key < sinks ? kBlock : key + left - p_low - 4 * h;
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int n = 8 * (r / 4) + r % 4;
+                    const bool seen = (n >= first) & (n <= last);
+                    s[r] = seen ? s[r] : 0.0f;
+                    dp[r] = seen ? dp[r] : 0.0f;
+                }
+            }
+            const int c_lane = again(lane);
 #pragma unroll
             for (int g = 0; g < 2; g++) {
                 const Frag<T> w = operand<T>(s, g), x = operand<T>(dp, g);
 #pragma unroll
                 for (int i = 0; i < NB; i++) {
-                    gv[i] = Mma<T>::mul(L::column(go_tile, 16 * g, i, lane), w, gv[i]);
-                    gk[i] = Mma<T>::mul(L::column(q_tile, 16 * g, i, lane), x, gk[i]);
+                    gv[i] = Mma<T>::mul(L::column(go_tile, 16 * g, i, c_lane), w, gv[i]);
+                    gk[i] = Mma<T>::mul(L::column(q_tile, 16 * g, i, c_lane), x, gk[i]);
                 }
             }
+            if constexpr (sizeof(T) == 2) {
+                read_ahead<4 * NB, 2, 4>();
+            }
         }
-        __syncthreads();
         if (kStages == 1 && more) {
+            barrier();
             fetch(step + 1, 0);
         }
         buffer ^= kStages - 1;

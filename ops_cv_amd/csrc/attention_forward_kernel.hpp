@@ -29,67 +29,65 @@ struct ForwardLaunch {
     uint32_t blocks;  // workgroups with work
 };
 
-// Where some rows do not see some keys of a tile, a value that is not finite must not reach them through its product with
-// their weight 0.  odd_values: whether the tile holds such values (wave-uniform); tiles that all rows see whole are not
-// asked.
-template <typename T, int PITCH, int KEYS, int NB>
-static __device__ __forceinline__ bool odd_values(const T* tile, int lane)
+// One block of features of V' P for a tile that some rows do not see whole.  A value that is not finite must not reach
+// those rows through its product with their weight 0: its presence shows in the sums (0 times it is NaN), and then the
+// finite values are multiplied as ever, and which kinds of the others each row gives weight to is counted by products of
+// ones and zeros.  Sums of finite values come out the same either way.
+template <typename T, int PITCH, int SUBS>
+static __device__ __forceinline__ acc_t add_seen_values(acc_t o, const Frag<T> (&w)[2 * SUBS], const T* tile, int block, int lane)
 {
-    bool odd = false;
+    acc_t x = zeros();
 #pragma unroll
-    for (int base = 0; base < KEYS; base += 16) {
-#pragma unroll
-        for (int i = 0; i < NB; i++) {
-            const Frag<T> f = Tile<T, PITCH>::column(tile, base, i, lane);
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                odd = odd || !__builtin_isfinite((float)f[e]);
-            }
-        }
+    for (int n = 0; n < 2 * SUBS; n++) {
+        x = Mma<T>::mul(Tile<T, PITCH>::column(tile, 16 * n, block, lane), w[n], x);
     }
-    return __any(odd);
-}
-
-// O' += V' P with such values: the finite ones as ever; of the others, which kinds each row gives weight to is counted by
-// products of ones and zeros.
-template <typename T, int PITCH, int SUBS, int NB>
-static __device__ __forceinline__ void add_odd_values(acc_t (&o)[NB], const acc_t (&s)[SUBS], const T* tile, int lane)
-{
+    float check = 0.0f;  // NaN where a sum is not finite
 #pragma unroll
-    for (int i = 0; i < NB; i++) {
-        acc_t up = zeros(), down = zeros(), none = zeros();
+    for (int r = 0; r < 16; r++) {
+        check = __builtin_fmaf(x[r], 0.0f, check);
+    }
+    if (__builtin_expect(__any(check != 0.0f) != 0, 0)) {
+        x = zeros();
+        // the finite ones, then +infinity, -infinity and NaN, one class at a time
+#pragma unroll 1
+        for (int kind = 0; kind < 4; kind++) {
+            const int mask = kind == 0 ? 0x1f8 : kind == 1 ? 0x200 : kind == 2 ? 0x004 : 0x003;
+            const float special = kind == 0 ? 0.0f : kind == 1 ? INFINITY : kind == 2 ? -INFINITY : NAN;
+            lane = again(lane);  // the values are read again for every class: held through the loop they cost registers
+            acc_t count = zeros();
+#pragma unroll 1
+            for (int n = 0; n < 2 * SUBS; n++) {
+                Frag<T> f = Tile<T, PITCH>::column(tile, 16 * n, block, lane), has = w[0];
 #pragma unroll
-        for (int j = 0; j < SUBS; j++) {
-#pragma unroll
-            for (int g = 0; g < 2; g++) {
-                const Frag<T> w = operand<T>(s[j], g), f = Tile<T, PITCH>::column(tile, j * kBlock + 16 * g, i, lane);
-                Frag<T> finite, is_up, is_down, is_none, has;
+                for (int m = 1; m < 2 * SUBS; m++) {
+                    has = n == m ? w[m] : has;
+                }
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const float x = (float)f[e];
-                    finite[e] = __builtin_isfinite(x) ? f[e] : (T)0.0f;
-                    is_up[e] = (T)(x == INFINITY ? 1.0f : 0.0f);
-                    is_down[e] = (T)(x == -INFINITY ? 1.0f : 0.0f);
-                    is_none[e] = (T)(x != x ? 1.0f : 0.0f);
-                    has[e] = (T)(s[j][8 * g + e] > 0.0f ? 1.0f : 0.0f);
+                    const float v = (float)f[e];
+                    f[e] = (T)(__builtin_amdgcn_classf(v, mask) ? (kind == 0 ? v : 1.0f) : 0.0f);
+                    has[e] = (kind == 0 || !((float)has[e] > 0.0f)) ? has[e] : (T)1.0f;
                 }
-                o[i] = Mma<T>::mul(finite, w, o[i]);
-                up = Mma<T>::mul(is_up, has, up);
-                down = Mma<T>::mul(is_down, has, down);
-                none = Mma<T>::mul(is_none, has, none);
+                count = Mma<T>::mul(f, has, count);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                x[r] += kind == 0 ? count[r] : (count[r] > 0.0f ? special : 0.0f);
             }
         }
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-            o[i][r] += up[r] > 0.0f ? INFINITY : 0.0f;
-            o[i][r] += down[r] > 0.0f ? -INFINITY : 0.0f;
-            o[i][r] += none[r] > 0.0f ? NAN : 0.0f;
-        }
     }
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+        o[r] += x[r];
+    }
+    return o;
 }
 
+// Two wavefronts a SIMD (256 registers each) where a row's share fits: 16-bit heads of up to 128 features, FLOAT of up to 64.
+constexpr int waves_per_simd(int elem_bytes, int nb) { return elem_bytes * nb <= 8 ? 2 : 1; }
+
 template <typename T, int NB, bool FEW, bool VEC>
-__global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads(), 1) void attention_kernel(
+__global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads(), waves_per_simd(sizeof(T), NB)) void attention_kernel(
     ForwardLaunch p)
 {
     constexpr int kPitch = pitch_of(NB);
@@ -109,7 +107,6 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
     const int h = lane >> 5, own = lane & 31;
     const int row_wave = wave % kShape.row_waves, key_wave = wave / kShape.row_waves;
-    const int gt = row_wave * 64 + lane;
     const int d = (int)a.d, left = (int)a.left, right = (int)a.right, sinks = (int)a.sinks;
     const Sequence seq = sequence_at(a, b);
 
@@ -127,20 +124,11 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
     if (block_high < block_low) {
         range.tiles = 0;
     }
-    const int wave_low = seq.first + query_of(wave_row0), wave_high = seq.first + query_of(wave_row0 + kBlock - 1);
-    const bool wave_whole = query_of(wave_row0 + kBlock - 1) < seq.q_len;
+    const int block_first = seq.first + block_low, block_last = seq.first + block_high;
+    const bool rows_whole = query_of(row0 + kShape.rows() - 1) < seq.q_len;
     const int t_begin = (int)((int64_t)range.tiles * split / p.splits);
     const int t_end = (int)((int64_t)range.tiles * (split + 1) / p.splits);
 
-    Frag<T> q[2 * NB];
-    {
-        const T* const src = (const T*)a.q.ptr + (int64_t)b * a.q.stride[0] + (int64_t)query * a.q.stride[1] +
-                             (int64_t)head * a.q.stride[2];
-#pragma unroll
-        for (int i = 0; i < 2 * NB; i++) {
-            q[i] = global_row<T, VEC>(src, 16 * i + 8 * h, d);
-        }
-    }
     const T* const k_base = (const T*)a.k.ptr + (int64_t)b * a.k.stride[0] + (int64_t)kv_head * a.k.stride[2];
     const T* const v_base = (const T*)a.v.ptr + (int64_t)b * a.v.stride[0] + (int64_t)kv_head * a.v.stride[2];
     const uint32_t k_pitch = (uint32_t)(a.k.stride[1] * (int64_t)sizeof(T));
@@ -148,24 +136,15 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
 
     T* const ring = reinterpret_cast<T*>(lds) + (size_t)key_wave * (kShape.stages * 2 * kKeys * kPitch);
     const auto fetch = [&](int t, int buffer) {
-        const int key0 = range.key_of(t, kKeys);
+        const int key0 = range.key_of(t, kKeys), rows = range.end_of(t) - key0;
         T* const k_tile = ring + buffer * (2 * kKeys * kPitch);
-        stage<T, kPitch, kKeys, kGroupThreads, VEC>(k_tile, k_base + (int64_t)key0 * a.k.stride[1], gt, d, [&](int r) {
-            return range.holds(t, key0 + r) ? (uint32_t)r * k_pitch : kOutside;
-        });
-        stage<T, kPitch, kKeys, kGroupThreads, VEC>(k_tile + kKeys * kPitch, v_base + (int64_t)key0 * a.v.stride[1], gt, d,
-                                                    [&](int r) { return range.holds(t, key0 + r) ? (uint32_t)r * v_pitch : kOutside; });
+        const int thread = row_wave * 64 + again(lane);
+        stage<T, kPitch, kKeys, kGroupThreads, VEC>(k_tile, k_base + (int64_t)key0 * a.k.stride[1], thread, row_wave, d,
+                                                    k_pitch, min(rows, kKeys));
+        stage<T, kPitch, kKeys, kGroupThreads, VEC>(k_tile + kKeys * kPitch, v_base + (int64_t)key0 * a.v.stride[1], thread,
+                                                    row_wave, d, v_pitch, min(rows, kKeys));
     };
     constexpr int kInFlight = 2 * kKeys * L::kChunks / kGroupThreads;  // loads of one fetch, a wavefront
-    const auto group_barrier = [&]() {
-        if constexpr (kShape.row_waves > 1) {
-            __syncthreads();
-        } else {
-            // one wavefront: its LDS operations stay in order; what it has read is back before the place is filled again
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_s_waitcnt(kWaitForLds);
-        }
-    };
 
     const float c = a.scale * kLog2e;
     float most = -INFINITY, total = 0.0f;  // `total`: of this lane's keys only
@@ -175,24 +154,49 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
         o[i] = zeros();
     }
 
-    int buffer = 0;
-    if (t_begin + key_wave < t_end) {
-        fetch(t_begin + key_wave, 0);
+    int t = t_begin + key_wave, buffer = 0;
+    if (t < t_end) {
+        fetch(t, 0);
     }
-    for (int t = t_begin + key_wave; t < t_end; t += kShape.key_waves) {
-        const bool more = t + kShape.key_waves < t_end;
-        if (kShape.stages == 2 && more) {
-            fetch(t + kShape.key_waves, buffer ^ 1);
-            if constexpr (VEC) {
-                __builtin_amdgcn_s_waitcnt(wait_for_loads(kInFlight));
-            }
-        } else if constexpr (VEC) {
-            __builtin_amdgcn_s_waitcnt(wait_for_loads(0));
+    Frag<T> q[2 * NB];
+    {
+        const T* const src = (const T*)a.q.ptr + (int64_t)b * a.q.stride[0] + (int64_t)query * a.q.stride[1] +
+                             (int64_t)head * a.q.stride[2];
+#pragma unroll
+        for (int i = 0; i < 2 * NB; i++) {
+            q[i] = global_row<T, VEC>(src, 16 * i + 8 * h, d);
         }
-        group_barrier();
+    }
+    wait_for_registers();
+    // whether all rows of the workgroup see all keys of a tile
+    const auto whole = [&](int tile_index) {
+        const int key0 = range.key_of(tile_index, kKeys);
+        return rows_whole && key0 + kKeys <= range.end_of(tile_index) && key0 + kKeys - 1 <= block_first + right &&
+               (key0 >= block_last - left || key0 + kKeys <= sinks);
+    };
+    // one tile; PART: some rows may not see some keys
+    const auto work = [&](auto part, const Rows32<T, kPitch, NB>& k_rows, const Columns32<T, kPitch, NB>& v_columns) {
+        constexpr bool PART = decltype(part)::value;
+        const bool more = t + kShape.key_waves < t_end;
+        if constexpr (kShape.row_waves > 1) {
+            // tile t is there for all wavefronts, and all have done with the tile before it, whose place is filled again
+            // while they work on this one
+            wait_for_loads<0>();
+            barrier();
+            if (kShape.stages == 2 && more) {
+                fetch(t + 1, buffer ^ 1);
+            }
+        } else {
+            // a ring of its own: the next tile is asked for before this one has come
+            if (kShape.stages == 2 && more) {
+                fetch(t + kShape.key_waves, buffer ^ 1);
+                wait_for_loads<VEC ? kInFlight : 0>();
+            } else {
+                wait_for_loads<0>();
+            }
+        }
         const T* const k_tile = ring + buffer * (2 * kKeys * kPitch);
         const T* const v_tile = k_tile + kKeys * kPitch;
-        const int key0 = range.key_of(t, kKeys), end = range.end_of(t);
 
         acc_t s[kSubs];
 #pragma unroll
@@ -200,33 +204,34 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
             s[j] = zeros();
 #pragma unroll
             for (int i = 0; i < 2 * NB; i++) {
-                s[j] = Mma<T>::mul(L::row(k_tile, j * kBlock + own, 2 * i + h), q[i], s[j]);
+                s[j] = Mma<T>::mul(k_rows(k_tile, j * kBlock, i), q[i], s[j]);
             }
         }
-        const bool all_seen = wave_whole && key0 + kKeys <= end && key0 + kKeys - 1 <= wave_low + right &&
-                              (key0 >= wave_high - left || key0 + kKeys <= sinks);
-        if (!all_seen) {
+        if constexpr (sizeof(T) == 2) {
+            read_ahead<2 * NB * kSubs, 1, 4>();
+        }
+        if constexpr (PART) {
+            const Sight see = sight(pos, range.key_of(t, kKeys) + 4 * h, range.end_of(t), left, right, sinks);
 #pragma unroll
             for (int j = 0; j < kSubs; j++) {
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
-                    const int key = key0 + j * kBlock + 8 * (r / 4) + 4 * h + r % 4;
-                    s[j][r] = (key < end && sees(pos, key, left, right, sinks)) ? s[j][r] : -INFINITY;
+                    s[j][r] = see.sees(j * kBlock + 8 * (r / 4) + r % 4) ? s[j][r] : -INFINITY;
                 }
             }
         }
-        float high = s[0][0];
+        float high = -INFINITY;
 #pragma unroll
         for (int j = 0; j < kSubs; j++) {
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                high = fmaxf(high, s[j][r]);
+            for (int r = 0; r < 16; r += 2) {
+                high = largest(high, s[j][r], s[j][r + 1]);
             }
         }
-        high = fmaxf(high, other_half(high)) * c;
-        const float now = fmaxf(most, high);
+        high = larger_of_halves(high) * c;
+        const float now = __builtin_elementwise_maximum(most, high);
         const float base = now == -INFINITY ? 0.0f : now;  // rows that have seen nothing yet: exp2(-inf - 0) = 0
-        if (__any(now > most)) {
+        if (__any(!(now <= most))) {
             const float fade = exp2f(most - base);
             total *= fade;
 #pragma unroll
@@ -238,34 +243,56 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
             }
         }
         most = now;
+        Frag<T> w[2 * kSubs];
 #pragma unroll
-        for (int j = 0; j < kSubs; j++) {
+        for (int n = 0; n < 2 * kSubs; n++) {
+            acc_t& x = s[n / 2];
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                s[j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][r], c, -base));
-                total += s[j][r];
+            for (int e = 0; e < 8; e++) {
+                const int r = 8 * (n % 2) + e;
+                x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], c, -base));
+                total += x[r];
             }
+            w[n] = operand<T>(x, n % 2);
         }
-        if (!all_seen && odd_values<T, kPitch, kKeys, NB>(v_tile, lane)) {
-            add_odd_values<T, kPitch, kSubs, NB>(o, s, v_tile, lane);
+        if constexpr (PART) {
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+                o[i] = add_seen_values<T, kPitch, kSubs>(o[i], w, v_tile, i, again(lane));
+            }
         } else {
 #pragma unroll
-            for (int j = 0; j < kSubs; j++) {
+            for (int n = 0; n < 2 * kSubs; n++) {
 #pragma unroll
-                for (int g = 0; g < 2; g++) {
-                    const Frag<T> w = operand<T>(s[j], g);
-#pragma unroll
-                    for (int i = 0; i < NB; i++) {
-                        o[i] = Mma<T>::mul(L::column(v_tile, j * kBlock + 16 * g, i, lane), w, o[i]);
-                    }
+                for (int i = 0; i < NB; i++) {
+                    o[i] = Mma<T>::mul(v_columns(v_tile, 16 * n, i), w[n], o[i]);
                 }
             }
+            if constexpr (sizeof(T) == 2) {
+                read_ahead<2 * NB * kSubs, 2, 3>();
+            }
         }
-        group_barrier();
         if (kShape.stages == 1 && more) {
+            if constexpr (kShape.row_waves > 1) {
+                barrier();
+            } else {
+                wait_for_lds();  // what was read of the tile is back before its place is filled again
+            }
             fetch(t + kShape.key_waves, 0);
         }
         buffer ^= kShape.stages - 1;
+        t += kShape.key_waves;
+    };
+    // two loops, so that the one for whole tiles has its registers to itself
+    while (t < t_end) {
+        while (t < t_end && !whole(t)) {
+            work(std::true_type(), Rows32<T, kPitch, NB>(again(lane)), Columns32<T, kPitch, NB>(again(lane)));
+        }
+        const Rows32<T, kPitch, NB> k_rows(again(lane));
+        const Columns32<T, kPitch, NB> v_columns(again(lane));
+        while (t < t_end && whole(t)) {
+            work(std::false_type(), k_rows, v_columns);
+        }
     }
     total += other_half(total);
 

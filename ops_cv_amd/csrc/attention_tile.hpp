@@ -94,7 +94,77 @@ static __device__ __forceinline__ Frag<T> operand(const acc_t& x, int g)
 }
 
 // x of the other half's lane with the same l % 32
-static __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+static __device__ __forceinline__ float other_half(float x)
+{
+    const uint32_t u = __float_as_uint(x);
+    const auto both = __builtin_amdgcn_permlane32_swap(u, u, false, false);  // halves: lower twice, upper twice
+    return __uint_as_float((threadIdx.x & 32) != 0 ? both[0] : both[1]);
+}
+
+// the larger of x and of the other half's lane, for both
+static __device__ __forceinline__ float larger_of_halves(float x)
+{
+    const uint32_t u = __float_as_uint(x);
+    const auto both = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __builtin_elementwise_maximum(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
+
+// the largest of three, NaN where any is
+static __device__ __forceinline__ float largest(float a, float b, float c)
+{
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
+}
+
+// ---------------------------------------------------------------------------------------------------- loads into LDS
+
+typedef int rsrc_t __attribute__((ext_vector_type(4)));
+
+// Descriptor of `bytes` bytes from an address that the wavefront shares.
+static __device__ __forceinline__ rsrc_t buffer(const void* base, uint32_t bytes)
+{
+    const uint64_t at = (uint64_t)base;
+    rsrc_t r;
+    r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)at);
+    r[1] = __builtin_amdgcn_readfirstlane((int)((uint32_t)(at >> 32) & 0xffffu));
+    r[2] = __builtin_amdgcn_readfirstlane((int)bytes);
+    r[3] = kBufferFlags;
+    // the loads that use it are not instructions whose hazards the compiler looks after: five wait states between a vector
+    // instruction that writes a scalar register and a load that reads it
+    __asm__ volatile("s_nop 4" : "+s"(r));
+    return r;
+}
+
+// BYTES bytes a lane from offset `off` of a buffer into LDS, the wavefront's first at `dst` and the lanes in order; lanes
+// whose offset is out of range write zeros.  It has no result for the compiler to wait for, and as an instruction that the
+// compiler does not look into it makes it wait for nothing: with the builtin, every transposed read of LDS is preceded by
+// a wait for all loads under way, which takes a prompt's attention from 180 to 210 us.  The caller waits.
+template <int BYTES>
+static __device__ __forceinline__ void load_to_lds(rsrc_t rsrc, void* dst, uint32_t off)
+{
+    const uint32_t at = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(lds_ptr_t)dst);
+    if constexpr (BYTES == 16) {
+        __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(rsrc)
+                         : "memory", "m0");
+    } else {
+        __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(rsrc)
+                         : "memory", "m0");
+    }
+}
+
+// Order of the instructions around it: AHEAD products' reads of LDS (READS each) first, then a product and the reads of
+// the one AHEAD behind it in turn.  Left alone, the compiler reads, waits and multiplies in turn.
+template <int PRODUCTS, int READS, int AHEAD>
+static __device__ __forceinline__ void read_ahead()
+{
+    constexpr int kAhead = AHEAD < PRODUCTS ? AHEAD : PRODUCTS;
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead * READS, 0);
+#pragma unroll
+    for (int i = 0; i < PRODUCTS - kAhead; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+}
 
 // ---------------------------------------------------------------------------------------------------------------- LDS
 //
@@ -170,43 +240,118 @@ struct Tile {
     }
 };
 
-// Copies ROWS rows into a tile by THREADS threads (thread `gt` of them; whole wavefronts).  Row i comes from
-// base + offset(i), an offset in bytes, or is zeros where offset(i) is kOutside; chunks from element D on are zeros.
-// VEC: 16-byte loads that write LDS themselves (asynchronous: the caller waits); else element by element.
-template <typename T, int PITCH, int ROWS, int THREADS, bool VEC, typename F>
-static __device__ __forceinline__ void stage(T* tile, const T* base, int gt, int d, F&& offset)
+// Where a lane reads whole rows (row base + l % 32) or columns of a tile: places that a loop computes once.  NB blocks of
+// 32 elements.  FLOAT has eight places a column and computes them as it goes: its products take eight times as long.
+template <typename T, int PITCH, int NB>
+struct Rows32 {
+    int at[2 * NB];
+    __device__ __forceinline__ explicit Rows32(int lane)
+    {
+        const int r = lane & 31, h = lane >> 5;
+#pragma unroll
+        for (int i = 0; i < 2 * NB; i++) {
+            constexpr int kPer8 = 8 / Tile<T, PITCH>::kPerChunk;  // chunks of eight elements: 1, FLOAT 2
+            at[i] = r * PITCH * (int)sizeof(T) + (((kPer8 * (2 * i + h)) ^ Tile<T, PITCH>::swizzle(r)) * 16);
+        }
+    }
+    // operand i (elements 16 i .. 16 i + 15) of rows base + l % 32, base a multiple of 32
+    __device__ __forceinline__ Frag<T> operator()(const T* tile, int base, int i) const
+    {
+        const char* const from = reinterpret_cast<const char*>(tile) + at[i] + base * PITCH * (int)sizeof(T);
+        if constexpr (sizeof(T) == 2) {
+            return *reinterpret_cast<const Frag<T>*>(from);
+        } else {
+            typedef float f32x4 __attribute__((ext_vector_type(4)));
+            const f32x4 a = *reinterpret_cast<const f32x4*>(from);
+            const f32x4 b = *reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(tile) + (at[i] ^ 16) +
+                                                            base * PITCH * (int)sizeof(T));
+            Frag<T> f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                f[e] = a[e];
+                f[4 + e] = b[e];
+            }
+            return f;
+        }
+    }
+};
+
+template <typename T, int PITCH, int NB>
+struct Columns32 {
+    int at[sizeof(T) == 2 ? 2 * NB : 1];
+    __device__ __forceinline__ explicit Columns32(int lane)
+    {
+        if constexpr (sizeof(T) == 2) {
+            const int i = lane & 15, r = 4 * (lane >> 5) + (i >> 2);
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+                const int c = 4 * n + ((lane >> 4) & 1) * 2 + ((i & 3) >> 1);
+                at[2 * n] = r * PITCH * 2 + ((c ^ Tile<T, PITCH>::swizzle(r)) * 16) + (i & 1) * 8;
+                at[2 * n + 1] = (r + 8) * PITCH * 2 + ((c ^ Tile<T, PITCH>::swizzle(r + 8)) * 16) + (i & 1) * 8;
+            }
+        } else {
+            at[0] = lane;
+        }
+    }
+    // block n of the sixteen rows from base on, a multiple of 16
+    __device__ __forceinline__ Frag<T> operator()(const T* tile, int base, int n) const
+    {
+        if constexpr (sizeof(T) == 2) {
+            typedef __attribute__((address_space(3))) s16x4* place;
+            const char* const from = reinterpret_cast<const char*>(tile) + base * PITCH * 2;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((place)(from + at[2 * n]));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((place)(from + at[2 * n + 1]));
+            s16x8 both;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                both[e] = lo[e];
+                both[4 + e] = hi[e];
+            }
+            return __builtin_bit_cast(Frag<T>, both);
+        } else {
+            return Tile<T, PITCH>::column(tile, base, n, at[0]);
+        }
+    }
+};
+
+// Copies ROWS rows into a tile by THREADS threads (thread `gt` of them, in their wavefront `wave`): row r from base + r * pitch
+// bytes, rows from `rows` (one or more) on and elements from d on as zeros.  VEC: 16-byte loads that write LDS themselves (asynchronous:
+// the caller waits), pitch at least the row's own bytes; else element by element.
+template <typename T, int PITCH, int ROWS, int THREADS, bool VEC>
+static __device__ __forceinline__ void stage(T* tile, const T* base, int gt, int wave, int d, uint32_t pitch, int rows)
 {
     typedef Tile<T, PITCH> L;
     constexpr int kChunks = ROWS * L::kChunks;
-    static_assert(kChunks % THREADS == 0, "every thread copies as many chunks");
+    constexpr int kStep = THREADS / L::kChunks;  // rows between a thread's chunks
+    static_assert(kChunks % THREADS == 0 && THREADS % L::kChunks == 0, "every thread copies as many chunks");
+    const int r0 = gt / L::kChunks, place = gt % L::kChunks;
     if constexpr (VEC) {
-        const __amdgpu_buffer_rsrc_t rsrc =
-            __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, 0x7fffffff, kBufferFlags);
+        // What lies behind the last row's last element is out of the buffer's range, and such loads return zeros; so do
+        // chunks behind the head's end, by an offset that no range holds.
+        const uint32_t bytes = (uint32_t)(rows - 1) * pitch + (uint32_t)d * (uint32_t)sizeof(T);
+        const rsrc_t rsrc = buffer(base, bytes);
+        const uint32_t row0 = (uint32_t)r0 * pitch;
 #pragma unroll
         for (int i = 0; i < kChunks / THREADS; i++) {
-            const int at = i * THREADS + gt;
-            const int r = at / L::kChunks, c = (at % L::kChunks) ^ L::swizzle(r);
-            const uint32_t from = offset(r);
-            const uint32_t off = (from == kOutside || c * L::kPerChunk >= d) ? kOutside : from + (uint32_t)c * 16u;
-            T* const dst = tile + (i * THREADS + (gt & ~63)) * L::kPerChunk;  // the wavefront's; lanes follow in order
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)dst, 16, (int)off, 0, 0, 0);
+            const int c = place ^ L::swizzle(r0 + i * kStep);
+            const uint32_t off = (c * L::kPerChunk >= d ? kOutside : row0 + (uint32_t)c * 16u) + (uint32_t)(i * kStep) * pitch;
+            T* const dst = tile + (i * THREADS + wave * 64) * L::kPerChunk;  // the wavefront's; lanes follow in order
+            load_to_lds<16>(rsrc, dst, off);
         }
     } else {
 #pragma unroll 1
         for (int i = 0; i < kChunks / THREADS; i++) {
-            const int at = i * THREADS + gt;
-            const int r = at / L::kChunks, c = (at % L::kChunks) ^ L::swizzle(r);
-            const uint32_t from = offset(r);
+            const int r = r0 + i * kStep, c = place ^ L::swizzle(r);
             alignas(16) T x[L::kPerChunk];
 #pragma unroll
             for (int e = 0; e < L::kPerChunk; e++) {
                 const int el = c * L::kPerChunk + e;
-                x[e] = (from == kOutside || el >= d)
-                           ? (T)0.0f
-                           : *reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + from + (uint32_t)el * sizeof(T));
+                x[e] = (r >= rows || el >= d) ? (T)0.0f
+                                              : *reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) +
+                                                                            ((uint32_t)r * pitch + (uint32_t)el * (uint32_t)sizeof(T)));
             }
             typedef float f32x4 __attribute__((ext_vector_type(4)));
-            *reinterpret_cast<f32x4*>(tile + at * L::kPerChunk) = *reinterpret_cast<const f32x4*>(x);
+            *reinterpret_cast<f32x4*>(tile + (i * THREADS + gt) * L::kPerChunk) = *reinterpret_cast<const f32x4*>(x);
         }
     }
 }
@@ -282,9 +427,24 @@ static __device__ __forceinline__ void put4(T* row, int first, int d, float a, f
     }
 }
 
-// operand of s_waitcnt: at most n loads to memory or LDS still under way (gfx9: the count is bits 0-3 and 14-15)
-constexpr int wait_for_loads(int n) { return (n & 15) | ((n >> 4) << 14) | 0xf70; }
-constexpr int kWaitForLds = 0xc07f;  // none of LDS
+// Waits until at most N loads to memory or LDS are under way, or none of LDS; nothing that follows is moved before it.
+template <int N>
+static __device__ __forceinline__ void wait_for_loads()
+{
+    __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// Waits for all loads, in a way that the compiler knows: it has then no reason to wait for registers loaded before a loop
+// inside the loop, where such a wait would be one for the loop's own loads.
+static __device__ __forceinline__ void wait_for_registers() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+static __device__ __forceinline__ void wait_for_lds() { __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// The same number, which the compiler takes for another: what is computed from it inside a loop is computed there, in a few
+// instructions, and holds no registers through the rest of the loop.
+static __device__ __forceinline__ int again(int x)
+{
+    __asm__ volatile("" : "+v"(x));
+    return x;
+}
 
 // ---------------------------------------------------------------------------------------------------------- visibility
 
@@ -311,11 +471,21 @@ static __device__ __forceinline__ Sequence sequence_at(const AttentionArgs& a, i
     return s;
 }
 
-// Whether a query at position p sees key j < kv_len.
-static __device__ __forceinline__ bool sees(int p, int j, int left, int right, int sinks)
+// What a query at position p sees of 64 keys from key0 on, of which those before `end` count: key key0 + n for
+// n <= last and (n >= first or n < sinks).
+struct Sight {
+    int first, last, sinks;
+    __device__ __forceinline__ bool sees(int n) const { return (n <= last) & ((n >= first) | (n < sinks)); }
+};
+
+static __device__ __forceinline__ Sight sight(int p, int key0, int end, int left, int right, int sinks)
 {
-    return j <= p + right && (j >= p - left || j < sinks);
+    return Sight{p - left - key0, min(p + right, end - 1) - key0, sinks - key0};
 }
+
+// Barrier of the workgroup that waits for the wavefront's LDS operations, but not for loads under way into LDS, as
+// __syncthreads would.
+static __device__ __forceinline__ void barrier() { __asm__ volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // Workgroups go round the eight XCDs; this gives every XCD a run of neighbouring numbers, so that the tiles of rows that
 // read the same keys share an L2.
@@ -325,11 +495,11 @@ static __device__ __forceinline__ uint32_t xcd_order(uint32_t index, uint32_t co
     return (index & 7u) * each + (index >> 3);
 }
 
-// Keys that a range of rows sees, as tiles: the first `sink_tiles` start at key 0, the others at `first`.
+// Keys that a range of rows sees, as tiles: the first `sink_tiles` start at key 0, the others at `first`.  Tiles hold
+// nothing between the sinks and the window: what lies there is seen by none of the rows, and may be anything.
 struct KeyRange {
     int first, end;  // window
     int sink_end;    // sinks in front of it
-    int gap_end;     // keys from sink_end to here, in the first tile of a joined run, are seen by none of the rows
     int sink_tiles, tiles;
 
     __device__ __forceinline__ int key_of(int t, int keys) const
@@ -337,11 +507,6 @@ struct KeyRange {
         return t < sink_tiles ? t * keys : first + (t - sink_tiles) * keys;
     }
     __device__ __forceinline__ int end_of(int t) const { return t < sink_tiles ? sink_end : end; }
-    // whether tile t has to hold this key: others are staged as zeros, whatever they are
-    __device__ __forceinline__ bool holds(int t, int key) const
-    {
-        return key < end_of(t) && (key < sink_end || key >= gap_end);
-    }
 };
 
 template <int KEYS>
@@ -351,13 +516,10 @@ static __device__ __forceinline__ KeyRange key_range(int p_low, int p_high, int 
     k.end = min(max(p_high + right + 1, 0), kv_len);
     k.first = min(max(p_low - left, 0), k.end);
     k.sink_end = min(sinks, k.first);
-    k.gap_end = k.sink_end;
-    k.sink_tiles = (k.sink_end + KEYS - 1) / KEYS;
-    if (k.sink_tiles > 0 && k.first <= k.sink_tiles * KEYS) {  // the window starts among them: one run of tiles
-        k.gap_end = k.first;
-        k.first = 0;
-        k.sink_tiles = 0;
+    if (k.sink_end == k.first) {  // the window follows the sinks: one run of tiles
+        k.sink_end = k.first = 0;
     }
+    k.sink_tiles = (k.sink_end + KEYS - 1) / KEYS;
     k.tiles = k.sink_tiles + (k.end - k.first + KEYS - 1) / KEYS;
     return k;
 }

@@ -93,9 +93,10 @@ void plan_strided(aclOpExecutor* ex, int slot, const aclTensor* t, int elem_byte
 {
     const int last = (int)t->ndim - 1;
     bool in_place = t->dims[last] == 1 || t->strides[last] == 1;
-    // kernels walk up to 64 tokens from a 64-bit address with 32-bit offsets in bytes
+    // kernels walk up to 64 tokens, of which none begins inside another, from a 64-bit address with 32-bit offsets in bytes
     for (int i = 0; i < last; i++) {
-        in_place = in_place && (t->dims[i] <= 1 || (t->strides[i] >= 0 && (i != 1 || t->strides[i] <= kMostTokenStride)));
+        in_place = in_place && (t->dims[i] <= 1 || (t->strides[i] >= 0 && (i != 1 || (t->strides[i] >= t->dims[last] &&
+                                                                                       t->strides[i] <= kMostTokenStride))));
     }
     if (in_place) {
         PlannedPtr p;
@@ -103,7 +104,7 @@ void plan_strided(aclOpExecutor* ex, int slot, const aclTensor* t, int elem_byte
         ex->operands[slot] = p;
         ex->required |= t->empty() ? 0u : 1u << slot;
         for (int i = 0; i < last; i++) {
-            s->stride[i] = t->dims[i] > 1 ? t->strides[i] : 0;
+            s->stride[i] = t->dims[i] > 1 ? t->strides[i] : (i == 1 ? t->dims[last] : 0);
         }
         return;
     }
