@@ -4,8 +4,8 @@
 // so a tile of keys and values in LDS serves them all, and their windows span few keys beyond one query's.  A wavefront
 // has 32 rows, one per lane of a half:
 //   S' = K Q'        (32 keys x 32 rows; K from LDS in "row" order, Q in registers)
-//   m, l             running maximum of a row and sum of exp2(S c - m), c = scale log2 e; a row's keys are spread over two
-//                    lanes, which exchange their maxima
+//   m, l             running reference of a row (near its largest score) and sum of exp2(S c - m), c = scale log2 e; a
+//                    row's keys are spread over two lanes, which exchange their maxima
 //   O' = O' f + V' P (head features x 32 rows; V from LDS in "column" order, P are S's registers, rounded to the type)
 // m, l and O stay in 32 bits; P is rounded to the type as the matrix instructions want it.
 #pragma once
@@ -29,56 +29,38 @@ struct ForwardLaunch {
     uint32_t blocks;  // workgroups with work
 };
 
-// One block of features of V' P for a tile that some rows do not see whole.  A value that is not finite must not reach
-// those rows through its product with their weight 0: its presence shows in the sums (0 times it is NaN), and then the
-// finite values are multiplied as ever, and which kinds of the others each row gives weight to is counted by products of
-// ones and zeros.  Sums of finite values come out the same either way.
+// O' += V' P for one block of features of a tile that some rows do not see whole and that holds values that are not finite.
+// Such a value must not reach the rows that do not see it through its product with their weight 0: the finite values are
+// multiplied as ever, and which kinds of the others each row gives weight to is counted by products of ones and zeros.
 template <typename T, int PITCH, int SUBS>
 static __device__ __forceinline__ acc_t add_seen_values(acc_t o, const Frag<T> (&w)[2 * SUBS], const T* tile, int block, int lane)
 {
-    acc_t x = zeros();
-#pragma unroll
-    for (int n = 0; n < 2 * SUBS; n++) {
-        x = Mma<T>::mul(Tile<T, PITCH>::column(tile, 16 * n, block, lane), w[n], x);
-    }
-    float check = 0.0f;  // NaN where a sum is not finite
-#pragma unroll
-    for (int r = 0; r < 16; r++) {
-        check = __builtin_fmaf(x[r], 0.0f, check);
-    }
-    if (__builtin_expect(__any(check != 0.0f) != 0, 0)) {
-        x = zeros();
-        // the finite ones, then +infinity, -infinity and NaN, one class at a time
+    // the finite ones, then +infinity, -infinity and NaN, one class at a time
 #pragma unroll 1
-        for (int kind = 0; kind < 4; kind++) {
-            const int mask = kind == 0 ? 0x1f8 : kind == 1 ? 0x200 : kind == 2 ? 0x004 : 0x003;
-            const float special = kind == 0 ? 0.0f : kind == 1 ? INFINITY : kind == 2 ? -INFINITY : NAN;
-            lane = again(lane);  // the values are read again for every class: held through the loop they cost registers
-            acc_t count = zeros();
+    for (int kind = 0; kind < 4; kind++) {
+        const int mask = kind == 0 ? 0x1f8 : kind == 1 ? 0x200 : kind == 2 ? 0x004 : 0x003;
+        const float special = kind == 1 ? INFINITY : kind == 2 ? -INFINITY : NAN;
+        lane = again(lane);  // the values are read again for every class: held through the loop they cost registers
+        acc_t count = kind == 0 ? o : zeros();
 #pragma unroll 1
-            for (int n = 0; n < 2 * SUBS; n++) {
-                Frag<T> f = Tile<T, PITCH>::column(tile, 16 * n, block, lane), has = w[0];
+        for (int n = 0; n < 2 * SUBS; n++) {
+            Frag<T> f = Tile<T, PITCH>::column(tile, 16 * n, block, lane), has = w[0];
 #pragma unroll
-                for (int m = 1; m < 2 * SUBS; m++) {
-                    has = n == m ? w[m] : has;
-                }
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float v = (float)f[e];
-                    f[e] = (T)(__builtin_amdgcn_classf(v, mask) ? (kind == 0 ? v : 1.0f) : 0.0f);
-                    has[e] = (kind == 0 || !((float)has[e] > 0.0f)) ? has[e] : (T)1.0f;
-                }
-                count = Mma<T>::mul(f, has, count);
+            for (int m = 1; m < 2 * SUBS; m++) {
+                has = n == m ? w[m] : has;
             }
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                x[r] += kind == 0 ? count[r] : (count[r] > 0.0f ? special : 0.0f);
+            for (int e = 0; e < 8; e++) {
+                const float v = (float)f[e];
+                f[e] = (T)(__builtin_amdgcn_classf(v, mask) ? (kind == 0 ? v : 1.0f) : 0.0f);
+                has[e] = (kind == 0 || !((float)has[e] > 0.0f)) ? has[e] : (T)1.0f;
             }
+            count = Mma<T>::mul(f, has, count);
         }
-    }
 #pragma unroll
-    for (int r = 0; r < 16; r++) {
-        o[r] += x[r];
+        for (int r = 0; r < 16; r++) {
+            o[r] = kind == 0 ? count[r] : (count[r] > 0.0f ? o[r] + special : o[r]);
+        }
     }
     return o;
 }
@@ -147,12 +129,11 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
     constexpr int kInFlight = 2 * kKeys * L::kChunks / kGroupThreads;  // loads of one fetch, a wavefront
 
     const float c = a.scale * kLog2e;
-    float most = -INFINITY, total = 0.0f;  // `total`: of this lane's keys only
+    // Scores are taken relative to `base`, a score of the row: not its largest, but at most kSlack (in powers of two) below,
+    // so that sums seldom have to be scaled again.  -infinity: the row has seen nothing.
+    constexpr float kSlack = 8.0f;
+    float base, total;  // `total`: of this lane's keys only
     acc_t o[NB];
-#pragma unroll
-    for (int i = 0; i < NB; i++) {
-        o[i] = zeros();
-    }
 
     int t = t_begin + key_wave, buffer = 0;
     if (t < t_end) {
@@ -168,6 +149,7 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
         }
     }
     wait_for_registers();
+    bool careful = false;  // a second pass, for values that are not finite
     // whether all rows of the workgroup see all keys of a tile
     const auto whole = [&](int tile_index) {
         const int key0 = range.key_of(tile_index, kKeys);
@@ -220,19 +202,20 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
                 }
             }
         }
-        float high = -INFINITY;
+        float highs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four chains: one would wait for itself
 #pragma unroll
         for (int j = 0; j < kSubs; j++) {
 #pragma unroll
             for (int r = 0; r < 16; r += 2) {
-                high = largest(high, s[j][r], s[j][r + 1]);
+                highs[r / 2 % 4] = largest(highs[r / 2 % 4], s[j][r], s[j][r + 1]);
             }
         }
-        high = larger_of_halves(high) * c;
-        const float now = __builtin_elementwise_maximum(most, high);
-        const float base = now == -INFINITY ? 0.0f : now;  // rows that have seen nothing yet: exp2(-inf - 0) = 0
-        if (__any(!(now <= most))) {
-            const float fade = exp2f(most - base);
+        const float high = larger_of_halves(largest(highs[0], highs[1], largest(highs[2], highs[3], highs[3]))) * c;
+        const bool grows = !(high <= base + kSlack);
+        if (__any(grows)) {
+            // each row by its own scores alone: what it sees beside it does not change its result
+            const float now = grows ? __builtin_elementwise_maximum(base, high) : base;
+            const float fade = base == -INFINITY ? 0.0f : exp2f(base - now);
             total *= fade;
 #pragma unroll
             for (int i = 0; i < NB; i++) {
@@ -241,21 +224,24 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
                     o[i][r] *= fade;
                 }
             }
+            base = now;
         }
-        most = now;
+        const float from = base == -INFINITY ? 0.0f : base;  // exp2(-inf - 0) = 0
         Frag<T> w[2 * kSubs];
+        float sums[4] = {total, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int n = 0; n < 2 * kSubs; n++) {
             acc_t& x = s[n / 2];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const int r = 8 * (n % 2) + e;
-                x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], c, -base));
-                total += x[r];
+                x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], c, -from));
+                sums[e % 4] += x[r];
             }
             w[n] = operand<T>(x, n % 2);
         }
-        if constexpr (PART) {
+        total = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        if (PART && __builtin_expect(careful, 0)) {
 #pragma unroll
             for (int i = 0; i < NB; i++) {
                 o[i] = add_seen_values<T, kPitch, kSubs>(o[i], w, v_tile, i, again(lane));
@@ -283,15 +269,47 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
         buffer ^= kShape.stages - 1;
         t += kShape.key_waves;
     };
-    // two loops, so that the one for whole tiles has its registers to itself
-    while (t < t_end) {
-        while (t < t_end && !whole(t)) {
-            work(std::true_type(), Rows32<T, kPitch, NB>(again(lane)), Columns32<T, kPitch, NB>(again(lane)));
+    while (true) {
+        base = -INFINITY;
+        total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+            o[i] = zeros();
         }
-        const Rows32<T, kPitch, NB> k_rows(again(lane));
-        const Columns32<T, kPitch, NB> v_columns(again(lane));
-        while (t < t_end && whole(t)) {
-            work(std::false_type(), k_rows, v_columns);
+        // two loops, so that the one for whole tiles has its registers to itself
+        while (t < t_end) {
+            {
+                const Rows32<T, kPitch, NB> k_rows(again(lane));
+                const Columns32<T, kPitch, NB> v_columns(again(lane));
+                while (t < t_end && !whole(t)) {
+                    work(std::true_type(), k_rows, v_columns);
+                }
+            }
+            const Rows32<T, kPitch, NB> k_rows(again(lane));
+            const Columns32<T, kPitch, NB> v_columns(again(lane));
+            while (t < t_end && whole(t)) {
+                work(std::false_type(), k_rows, v_columns);
+            }
+        }
+        // Sums that are not finite may come from values that a row does not see, through their products with its weight 0
+        // (0 times infinity is NaN): then all is done once more, and tiles that not all rows see whole with care.
+        float check = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                check = __builtin_fmaf(o[i][r], 0.0f, check);
+            }
+        }
+        const bool odd = !careful && check != 0.0f;
+        if (!(kShape.row_waves > 1 ? __syncthreads_or(odd) : __any(odd))) {
+            break;
+        }
+        careful = true;
+        t = t_begin + key_wave;
+        buffer = 0;
+        if (t < t_end) {
+            fetch(t, 0);
         }
     }
     total += other_half(total);
@@ -305,7 +323,7 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
         __syncthreads();
         float* const mine = sums + wave * kWaveFloats;
         if (h == 0) {
-            mine[own] = most;
+            mine[own] = base;
             mine[kBlock + own] = total;
         }
 #pragma unroll
@@ -321,13 +339,13 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
         for (int w = 0; w < kJoin; w++) {
             high = fmaxf(high, sums[w * kWaveFloats + own]);
         }
-        const float base = high == -INFINITY ? 0.0f : high;
+        const float from = high == -INFINITY ? 0.0f : high;
         float share[kJoin];
         total = 0.0f;
-        most = high;
+        base = high;
 #pragma unroll
         for (int w = 0; w < kJoin; w++) {
-            share[w] = exp2f(sums[w * kWaveFloats + own] - base);
+            share[w] = exp2f(sums[w * kWaveFloats + own] - from);
             total += share[w] * sums[w * kWaveFloats + kBlock + own];
         }
 #pragma unroll
@@ -353,7 +371,7 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
     if (p.splits > 1) {
         float* const part = a.scratch + (((int64_t)bh * p.splits + split) * p.rows + row) * partial_floats(d);
         if (first_wave && h == 0) {
-            part[0] = most;
+            part[0] = base;
             part[1] = total;
         }
 #pragma unroll
@@ -377,7 +395,7 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
     if (first_wave && h == 0 && a.lse.ptr != nullptr) {
         ((float*)a.lse.ptr)[(int64_t)b * a.lse.stride[0] + (int64_t)head * a.lse.stride[1] +
                             (int64_t)query * a.lse.stride[2]] =
-            total == 0.0f ? -INFINITY : (most + log2f(total)) * kLn2;
+            total == 0.0f ? -INFINITY : (base + log2f(total)) * kLn2;
     }
     T* const out = (T*)a.out.ptr + (int64_t)b * a.out.stride[0] + (int64_t)query * a.out.stride[1] +
                    (int64_t)head * a.out.stride[2];
