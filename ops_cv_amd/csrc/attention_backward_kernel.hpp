@@ -100,7 +100,6 @@ __global__ __launch_bounds__(256, sizeof(T) * NB <= 8 ? 2 : 1) void attention_qu
     constexpr ForwardShape kShape = query_grad_shape(sizeof(T), kPitch);
     constexpr int kKeys = kShape.keys, kSubs = kKeys / kBlock, kThreads = 256;
     constexpr bool kUnits = std::is_same<T, _Float16>::value;
-    typedef Tile<T, kPitch> L;
     extern __shared__ __align__(16) char lds[];
 
     const AttentionArgs& a = p.a;
@@ -138,8 +137,8 @@ __global__ __launch_bounds__(256, sizeof(T) * NB <= 8 ? 2 : 1) void attention_qu
         const int key0 = range.key_of(t, kKeys), rows = range.end_of(t) - key0;
         T* const k_tile = ring + buffer * (2 * kKeys * kPitch);
         const int gt = wave * 64 + again(lane);
-        stage<T, kPitch, kKeys, kThreads, VEC>(k_tile, k_base + (int64_t)key0 * a.k.stride[1], gt, wave, d, k_pitch, min(rows, kKeys));
-        stage<T, kPitch, kKeys, kThreads, VEC>(k_tile + kKeys * kPitch, v_base + (int64_t)key0 * a.v.stride[1], gt, wave, d, v_pitch,
+        stage<T, kPitch, kKeys, kThreads, VEC>(k_tile, at_bytes(k_base, (uint32_t)key0, k_pitch), gt, wave, d, k_pitch, min(rows, kKeys));
+        stage<T, kPitch, kKeys, kThreads, VEC>(k_tile + kKeys * kPitch, at_bytes(v_base, (uint32_t)key0, v_pitch), gt, wave, d, v_pitch,
                                          min(rows, kKeys));
     };
     const float c = a.scale * kLog2e;
@@ -168,6 +167,8 @@ __global__ __launch_bounds__(256, sizeof(T) * NB <= 8 ? 2 : 1) void attention_qu
     const float lse = stat[0], along = stat[a.tokens];
     const float unit = kUnits ? stat[2 * a.tokens] : 1.0f, per_unit = unit > 0.0f ? 1.0f / unit : 0.0f;
     wait_for_registers();
+    const Rows32<T, kPitch, NB> rows(lane);
+    const Columns32<T, kPitch, NB> columns(lane);
     for (int t = 0; t < range.tiles; t++) {
         const bool more = t + 1 < range.tiles;
         wait_for_loads<0>();  // as in the forward pass
@@ -183,11 +184,10 @@ __global__ __launch_bounds__(256, sizeof(T) * NB <= 8 ? 2 : 1) void attention_qu
 #pragma unroll
         for (int j = 0; j < kSubs; j++) {
             acc_t s = zeros(), dp = zeros();
-            const int ln = again(lane);
 #pragma unroll
             for (int i = 0; i < 2 * NB; i++) {
-                s = Mma<T>::mul(L::row(k_tile, j * kBlock + (ln & 31), 2 * i + (ln >> 5)), q[i], s);
-                dp = Mma<T>::mul(L::row(v_tile, j * kBlock + (ln & 31), 2 * i + (ln >> 5)), go[i], dp);
+                s = Mma<T>::mul(rows(k_tile, j * kBlock, i), q[i], s);
+                dp = Mma<T>::mul(rows(v_tile, j * kBlock, i), go[i], dp);
             }
             if constexpr (sizeof(T) == 2) {
                 read_ahead<4 * NB, 1, 4>();
@@ -203,13 +203,12 @@ __global__ __launch_bounds__(256, sizeof(T) * NB <= 8 ? 2 : 1) void attention_qu
                     s[r] = see.sees(8 * (r / 4) + r % 4) ? s[r] : 0.0f;
                 }
             }
-            const int k_lane = again(lane);
 #pragma unroll
             for (int g = 0; g < 2; g++) {
                 const Frag<T> w = operand<T>(s, g);
 #pragma unroll
                 for (int i = 0; i < NB; i++) {
-                    gq[i] = Mma<T>::mul(L::column(k_tile, j * kBlock + 16 * g, i, k_lane), w, gq[i]);
+                    gq[i] = Mma<T>::mul(columns(k_tile, j * kBlock + 16 * g, i), w, gq[i]);
                 }
             }
             if constexpr (sizeof(T) == 2) {
@@ -242,15 +241,20 @@ __global__ __launch_bounds__(256, sizeof(T) * NB <= 8 ? 2 : 1) void attention_qu
 // ------------------------------------------------------------------------------------------------------- keys' gradients
 
 constexpr int key_grad_stages(int elem_bytes, int pitch) { return elem_bytes * pitch <= 512 ? 2 : 1; }
+// The values of the 128 keys are read from LDS for every product, which leaves 16-bit heads of up to 128 features within
+// the 256 registers of two wavefronts a SIMD (with the values in registers too, one: the accumulators then lie in the other
+// half of the register file and are copied to and fro; 4096 tokens, 32 heads on 8, window 1024: 366 us against 187).
+constexpr bool key_grad_values_in_lds(int elem_bytes, int pitch) { return elem_bytes * pitch <= 512; }
+constexpr int key_grad_waves(int elem_bytes, int nb) { return elem_bytes * nb <= 8 ? 2 : 1; }
 
 template <typename T, int NB, bool VEC>
-__global__ __launch_bounds__(64 * kKeyWaves, 1) void attention_key_grad_kernel(GradLaunch p)
+__global__ __launch_bounds__(64 * kKeyWaves, key_grad_waves(sizeof(T), NB)) void attention_key_grad_kernel(GradLaunch p)
 {
     constexpr int kPitch = pitch_of(NB), kThreads = 64 * kKeyWaves, kStages = key_grad_stages(sizeof(T), kPitch);
     constexpr bool kUnits = std::is_same<T, _Float16>::value;
     constexpr int kStatRows = kUnits ? 4 : 2;  // of 32 floats each, a wavefront and stage
     constexpr int kTile = kBlock * kPitch;     // elements
-    typedef Tile<T, kPitch> L;
+    constexpr bool kValuesInLds = key_grad_values_in_lds(sizeof(T), kPitch);
     extern __shared__ __align__(16) char lds[];
 
     const AttentionArgs& a = p.a;
@@ -286,31 +290,44 @@ __global__ __launch_bounds__(64 * kKeyWaves, 1) void attention_key_grad_kernel(G
     T* const ring = reinterpret_cast<T*>(lds);
     float* const stat_ring = reinterpret_cast<float*>(lds + (size_t)kStages * 2 * kTile * sizeof(T)) +
                              wave * (kStages * kStatRows * kBlock);
+    T* const v_tile = reinterpret_cast<T*>(lds + (size_t)kStages * 2 * kTile * sizeof(T) +
+                                           kKeyWaves * kStages * kStatRows * kBlock * sizeof(float));
     const uint32_t q_pitch = (uint32_t)(a.q.stride[1] * (int64_t)sizeof(T));
     const uint32_t go_pitch = (uint32_t)(a.grad_out.stride[1] * (int64_t)sizeof(T));
-    // step s: head s / row_tiles of the group, queries from low + 32 (s % row_tiles) on
-    const auto fetch = [&](int s, int buffer) {
-        const int g = s / row_tiles, i0 = low + (s - g * row_tiles) * kBlock;
-        const int64_t head = (int64_t)kv_head * p.group.div + g;
-        const T* const q_base = (const T*)a.q.ptr + (int64_t)b * a.q.stride[0] + i0 * a.q.stride[1] + head * a.q.stride[2];
-        const T* const go_base = (const T*)a.grad_out.ptr + (int64_t)b * a.grad_out.stride[0] + i0 * a.grad_out.stride[1] +
-                                 head * a.grad_out.stride[2];
-        const int rows = seq.q_len - i0;
+    const int64_t head0 = (int64_t)kv_head * p.group.div;
+    const T* const q_base = (const T*)a.q.ptr + (int64_t)b * a.q.stride[0] + head0 * a.q.stride[2];
+    const T* const go_base = (const T*)a.grad_out.ptr + (int64_t)b * a.grad_out.stride[0] + head0 * a.grad_out.stride[2];
+    const float* const stat_base = p.stats + stats_row(a, b, head0);
+    // steps go through the tiles of one head's queries, then the next head's; `f_`: the step that is fetched next
+    int f_head = row_tiles > 0 ? s_begin / row_tiles : 0, f_query = low + (s_begin - f_head * row_tiles) * kBlock;
+    int c_query = f_query;
+    const auto fetch = [&](int buffer) {
+        const int rows = min(seq.q_len - f_query, kBlock);
         T* const q_tile = ring + buffer * (2 * kTile);
-        const int gt = wave * 64 + again(lane);
-        stage<T, kPitch, kBlock, kThreads, VEC>(q_tile, q_base, gt, wave, d, q_pitch, min(rows, kBlock));
-        stage<T, kPitch, kBlock, kThreads, VEC>(q_tile + kTile, go_base, gt, wave, d, go_pitch, min(rows, kBlock));
+        const int thread = wave * 64 + again(lane);
+        stage<T, kPitch, kBlock, kThreads, VEC>(q_tile, at_bytes(q_base + f_head * a.q.stride[2], (uint32_t)f_query, q_pitch),
+                                                thread, wave, d, q_pitch, rows);
+        stage<T, kPitch, kBlock, kThreads, VEC>(q_tile + kTile,
+                                                at_bytes(go_base + f_head * a.grad_out.stride[2], (uint32_t)f_query, go_pitch),
+                                                thread, wave, d, go_pitch, rows);
         // statistics: lanes of the lower half read one kind, of the upper half the next; rows past the end read zeros,
         // which meet rows of zeros
-        const rsrc_t rsrc = att::buffer(p.stats + stats_row(a, b, head) + i0, 0x7fffffffu);
-        float* const to = stat_ring + buffer * (kStatRows * kBlock);
-#pragma unroll
-        for (int n = 0; n < kStatRows / 2; n++) {
-            const int kind = 2 * n + h;
-            const uint32_t off = (own < rows && kind < 3) ? (uint32_t)(kind * (int)a.tokens + own) * 4u : kOutside;
-            load_to_lds<4>(rsrc, to + n * 2 * kBlock, off);
+        const rsrc_t rsrc = att::buffer(stat_base + f_head * (3 * a.tokens) + f_query, 0x7fffffffu);
+        const uint32_t to = lds_place(stat_ring + buffer * (kStatRows * kBlock));
+        const auto stat_offset = [&](int kind) {
+            return (own < rows && kind < 3) ? (uint32_t)(kind * (int)a.tokens + own) * 4u : kOutside;
+        };
+        load_to_lds<4, 0>(rsrc, to, stat_offset(h));
+        if constexpr (kUnits) {
+            load_to_lds<4, 2 * kBlock * 4>(rsrc, to, stat_offset(2 + h));
+        }
+        f_query += kBlock;
+        if (f_query >= high) {
+            f_query = low;
+            f_head++;
         }
     };
+
     const float c = a.scale * kLog2e;
     acc_t gk[NB], gv[NB];
 #pragma unroll
@@ -321,17 +338,26 @@ __global__ __launch_bounds__(64 * kKeyWaves, 1) void attention_key_grad_kernel(G
     float unit = 0.0f, per_unit = kUnits ? 0.0f : 1.0f;
     int buffer = 0;
     if (s_begin < s_end) {
-        fetch(s_begin, 0);
+        fetch(0);
     }
-    Frag<T> k[2 * NB], v[2 * NB];
+    Frag<T> k[2 * NB], v[kValuesInLds ? 1 : 2 * NB];
     {
         const int64_t from = min(key, (int)a.kv_tokens - 1);
-        const T* const ks = (const T*)a.k.ptr + (int64_t)b * a.k.stride[0] + from * a.k.stride[1] + (int64_t)kv_head * a.k.stride[2];
-        const T* const vs = (const T*)a.v.ptr + (int64_t)b * a.v.stride[0] + from * a.v.stride[1] + (int64_t)kv_head * a.v.stride[2];
+        const T* const k_first = (const T*)a.k.ptr + (int64_t)b * a.k.stride[0] + (int64_t)kv_head * a.k.stride[2];
+        const T* const v_first = (const T*)a.v.ptr + (int64_t)b * a.v.stride[0] + (int64_t)kv_head * a.v.stride[2];
+        if constexpr (kValuesInLds) {
+            if (last >= key0) {
+                const uint32_t v_pitch = (uint32_t)(a.v.stride[1] * (int64_t)sizeof(T));
+                stage<T, kPitch, kGradKeys, kThreads, VEC>(v_tile, at_bytes(v_first, (uint32_t)key0, v_pitch), wave * 64 + lane,
+                                                           wave, d, v_pitch, last + 1 - key0);
+            }
+        }
 #pragma unroll
         for (int i = 0; i < 2 * NB; i++) {
-            k[i] = global_row<T, VEC>(ks, 16 * i + 8 * h, d);
-            v[i] = global_row<T, VEC>(vs, 16 * i + 8 * h, d);
+            k[i] = global_row<T, VEC>(k_first + from * a.k.stride[1], 16 * i + 8 * h, d);
+            if constexpr (!kValuesInLds) {
+                v[i] = global_row<T, VEC>(v_first + from * a.v.stride[1], 16 * i + 8 * h, d);
+            }
         }
     }
     wait_for_registers();
@@ -340,12 +366,13 @@ __global__ __launch_bounds__(64 * kKeyWaves, 1) void attention_key_grad_kernel(G
         wait_for_loads<0>();
         barrier();
         if (kStages == 2 && more) {
-            fetch(step + 1, buffer ^ 1);
+            fetch(buffer ^ 1);
         }
         const T* const q_tile = ring + buffer * (2 * kTile);
         const T* const go_tile = q_tile + kTile;
         const float* const stat = stat_ring + buffer * (kStatRows * kBlock);
-        const int i0 = low + (step % row_tiles) * kBlock;
+        const int i0 = c_query;
+        c_query = c_query + kBlock < high ? c_query + kBlock : low;
         const int p_low = seq.first + i0, p_high = seq.first + min(i0 + kBlock, seq.q_len) - 1;
         // whether the wavefront's keys are seen by any of the rows, and by all of them
         const bool any = wave_key0 < seq.kv_len && wave_key0 <= p_high + right &&
@@ -373,14 +400,25 @@ __global__ __launch_bounds__(64 * kKeyWaves, 1) void attention_key_grad_kernel(G
                 }
             }
             acc_t s = zeros(), dp = zeros();
-            const int ln = again(lane);
+            const Rows32<T, kPitch, NB> rows(again(lane));
 #pragma unroll
             for (int i = 0; i < 2 * NB; i++) {
-                s = Mma<T>::mul(L::row(q_tile, ln & 31, 2 * i + (ln >> 5)), k[i], s);
-                dp = Mma<T>::mul(L::row(go_tile, ln & 31, 2 * i + (ln >> 5)), v[i], dp);
+                s = Mma<T>::mul(rows(q_tile, 0, i), k[i], s);
             }
             if constexpr (sizeof(T) == 2) {
-                read_ahead<4 * NB, 1, 6>();
+                read_ahead<2 * NB, 1, 4>();
+            }
+#pragma unroll
+            for (int i = 0; i < 2 * NB; i++) {
+                const Frag<T> g = rows(go_tile, 0, i);
+                if constexpr (kValuesInLds) {
+                    dp = Mma<T>::mul(g, rows(v_tile, wave * kBlock, i), dp);
+                } else {
+                    dp = Mma<T>::mul(g, v[i], dp);
+                }
+            }
+            if constexpr (sizeof(T) == 2) {
+                read_ahead<2 * NB, 2, 3>();
             }
 #pragma unroll
             for (int r = 0; r < 16; r++) {
@@ -400,14 +438,14 @@ __global__ __launch_bounds__(64 * kKeyWaves, 1) void attention_key_grad_kernel(G
                     dp[r] = seen ? dp[r] : 0.0f;
                 }
             }
-            const int c_lane = again(lane);
+            const Columns32<T, kPitch, NB> columns(again(lane));
 #pragma unroll
             for (int g = 0; g < 2; g++) {
                 const Frag<T> w = operand<T>(s, g), x = operand<T>(dp, g);
 #pragma unroll
                 for (int i = 0; i < NB; i++) {
-                    gv[i] = Mma<T>::mul(L::column(go_tile, 16 * g, i, c_lane), w, gv[i]);
-                    gk[i] = Mma<T>::mul(L::column(q_tile, 16 * g, i, c_lane), x, gk[i]);
+                    gv[i] = Mma<T>::mul(columns(go_tile, 16 * g, i), w, gv[i]);
+                    gk[i] = Mma<T>::mul(columns(q_tile, 16 * g, i), x, gk[i]);
                 }
             }
             if constexpr (sizeof(T) == 2) {
@@ -416,7 +454,7 @@ __global__ __launch_bounds__(64 * kKeyWaves, 1) void attention_key_grad_kernel(G
         }
         if (kStages == 1 && more) {
             barrier();
-            fetch(step + 1, 0);
+            fetch(0);
         }
         buffer ^= kStages - 1;
     }
@@ -506,7 +544,8 @@ hipError_t run_backward_shape(const GradLaunch& p, hipStream_t stream)
     constexpr int kQueryBytes = kShape.stages * 2 * kShape.keys * kPitch * (int)sizeof(T);
     constexpr int kStages = key_grad_stages(sizeof(T), kPitch);
     constexpr int kKeyBytes = kStages * 2 * kBlock * kPitch * (int)sizeof(T) +
-                              kKeyWaves * kStages * (std::is_same<T, _Float16>::value ? 4 : 2) * kBlock * 4;
+                              kKeyWaves * kStages * (std::is_same<T, _Float16>::value ? 4 : 2) * kBlock * 4 +
+                              (key_grad_values_in_lds(sizeof(T), kPitch) ? kGradKeys * kPitch * (int)sizeof(T) : 0);
     static_assert(kQueryBytes <= 160 * 1024 && kKeyBytes <= 160 * 1024, "LDS of a CU");
     static std::atomic<uint32_t> query_done{0}, key_done{0};
     const auto query_kernel = attention_query_grad_kernel<T, NB, VEC>;

@@ -121,9 +121,9 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
         const int key0 = range.key_of(t, kKeys), rows = range.end_of(t) - key0;
         T* const k_tile = ring + buffer * (2 * kKeys * kPitch);
         const int thread = row_wave * 64 + again(lane);
-        stage<T, kPitch, kKeys, kGroupThreads, VEC>(k_tile, k_base + (int64_t)key0 * a.k.stride[1], thread, row_wave, d,
+        stage<T, kPitch, kKeys, kGroupThreads, VEC>(k_tile, at_bytes(k_base, (uint32_t)key0, k_pitch), thread, row_wave, d,
                                                     k_pitch, min(rows, kKeys));
-        stage<T, kPitch, kKeys, kGroupThreads, VEC>(k_tile + kKeys * kPitch, v_base + (int64_t)key0 * a.v.stride[1], thread,
+        stage<T, kPitch, kKeys, kGroupThreads, VEC>(k_tile + kKeys * kPitch, at_bytes(v_base, (uint32_t)key0, v_pitch), thread,
                                                     row_wave, d, v_pitch, min(rows, kKeys));
     };
     constexpr int kInFlight = 2 * kKeys * L::kChunks / kGroupThreads;  // loads of one fetch, a wavefront

@@ -14,6 +14,8 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
+#include <utility>
 
 #include "acl_types.hpp"
 
@@ -125,7 +127,7 @@ static __device__ __forceinline__ rsrc_t buffer(const void* base, uint32_t bytes
     const uint64_t at = (uint64_t)base;
     rsrc_t r;
     r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)at);
-    r[1] = __builtin_amdgcn_readfirstlane((int)((uint32_t)(at >> 32) & 0xffffu));
+    r[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32));  // addresses have 48 bits: no stride, no swizzle
     r[2] = __builtin_amdgcn_readfirstlane((int)bytes);
     r[3] = kBufferFlags;
     // the loads that use it are not instructions whose hazards the compiler looks after: five wait states between a vector
@@ -134,21 +136,28 @@ static __device__ __forceinline__ rsrc_t buffer(const void* base, uint32_t bytes
     return r;
 }
 
-// BYTES bytes a lane from offset `off` of a buffer into LDS, the wavefront's first at `dst` and the lanes in order; lanes
+// BYTES bytes a lane from offset `off` of a buffer into LDS, the wavefront's first at place dst + AT and the lanes in order; lanes
 // whose offset is out of range write zeros.  It has no result for the compiler to wait for, and as an instruction that the
 // compiler does not look into it makes it wait for nothing: with the builtin, every transposed read of LDS is preceded by
-// a wait for all loads under way, which takes a prompt's attention from 180 to 210 us.  The caller waits.
-template <int BYTES>
-static __device__ __forceinline__ void load_to_lds(rsrc_t rsrc, void* dst, uint32_t off)
+// a wait for all loads under way, which takes the attention of a prompt of 8192 tokens from 193 to 203 us.  The caller waits.
+template <int BYTES, int AT>
+static __device__ __forceinline__ void load_to_lds(rsrc_t rsrc, uint32_t dst, uint32_t off)
 {
-    const uint32_t at = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(lds_ptr_t)dst);
     if constexpr (BYTES == 16) {
-        __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(rsrc)
-                         : "memory", "m0");
+        __asm__ volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(off),
+                         "s"(rsrc), "n"(AT)
+                         : "memory", "m0", "scc");
     } else {
-        __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(rsrc)
-                         : "memory", "m0");
+        __asm__ volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(dst), "v"(off),
+                         "s"(rsrc), "n"(AT)
+                         : "memory", "m0", "scc");
     }
+}
+
+// where a place in LDS begins, for load_to_lds
+static __device__ __forceinline__ uint32_t lds_place(const void* at)
+{
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(lds_ptr_t)const_cast<void*>(at));
 }
 
 // Order of the instructions around it: AHEAD products' reads of LDS (READS each) first, then a product and the reads of
@@ -314,6 +323,21 @@ struct Columns32 {
     }
 };
 
+// the loads of stage(): chunk `place` (swizzled) of rows r0, r0 + STEP, ..., BYTES apart in LDS
+template <typename T, int PITCH, int STEP, int BYTES, int... I>
+static __device__ __forceinline__ void stage_chunks(rsrc_t rsrc, uint32_t dst, int r0, int place, int d, uint32_t pitch,
+                                                    uint32_t row0, std::integer_sequence<int, I...>)
+{
+    typedef Tile<T, PITCH> L;
+    const auto one = [&](auto i) {
+        constexpr int kI = decltype(i)::value;
+        const int c = place ^ L::swizzle(r0 + kI * STEP);
+        const uint32_t off = (c * L::kPerChunk >= d ? kOutside : row0 + (uint32_t)c * 16u) + (uint32_t)(kI * STEP) * pitch;
+        load_to_lds<16, kI * BYTES>(rsrc, dst, off);
+    };
+    (one(std::integral_constant<int, I>()), ...);
+}
+
 // Copies ROWS rows into a tile by THREADS threads (thread `gt` of them, in their wavefront `wave`): row r from base + r * pitch
 // bytes, rows from `rows` (one or more) on and elements from d on as zeros.  VEC: 16-byte loads that write LDS themselves (asynchronous:
 // the caller waits), pitch at least the row's own bytes; else element by element.
@@ -331,13 +355,9 @@ static __device__ __forceinline__ void stage(T* tile, const T* base, int gt, int
         const uint32_t bytes = (uint32_t)(rows - 1) * pitch + (uint32_t)d * (uint32_t)sizeof(T);
         const rsrc_t rsrc = buffer(base, bytes);
         const uint32_t row0 = (uint32_t)r0 * pitch;
-#pragma unroll
-        for (int i = 0; i < kChunks / THREADS; i++) {
-            const int c = place ^ L::swizzle(r0 + i * kStep);
-            const uint32_t off = (c * L::kPerChunk >= d ? kOutside : row0 + (uint32_t)c * 16u) + (uint32_t)(i * kStep) * pitch;
-            T* const dst = tile + (i * THREADS + wave * 64) * L::kPerChunk;  // the wavefront's; lanes follow in order
-            load_to_lds<16>(rsrc, dst, off);
-        }
+        const uint32_t dst = lds_place(tile + wave * 64 * L::kPerChunk);  // the wavefront's; lanes follow in order
+        stage_chunks<T, PITCH, kStep, THREADS * 16>(rsrc, dst, r0, place, d, pitch, row0,
+                                                    std::make_integer_sequence<int, kChunks / THREADS>());
     } else {
 #pragma unroll 1
         for (int i = 0; i < kChunks / THREADS; i++) {
@@ -354,6 +374,13 @@ static __device__ __forceinline__ void stage(T* tile, const T* base, int gt, int
             *reinterpret_cast<f32x4*>(tile + (i * THREADS + gt) * L::kPerChunk) = *reinterpret_cast<const f32x4*>(x);
         }
     }
+}
+
+// the address `n` rows of `pitch` bytes behind another
+template <typename T>
+static __device__ __forceinline__ const T* at_bytes(const T* base, uint32_t n, uint32_t pitch)
+{
+    return reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + (uint64_t)n * pitch);
 }
 
 // Eight elements from element `first` of a row on, zeros from element d on.
