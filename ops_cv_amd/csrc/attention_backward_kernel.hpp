@@ -32,10 +32,10 @@ struct GradLaunch {
     AttentionArgs a;
     FastDiv group;
     uint32_t rows, tiles, kv_heads;
-    uint32_t key_tiles, sink_tiles, sink_parts, parts;
+    uint32_t keys, key_tiles, sink_tiles, sink_parts, parts;
     uint32_t query_blocks, key_blocks;
     float* stats;          // (batch, heads, 3, tokens)
-    float* sink_partials;  // (batch * kv_heads, sink_tiles, sink_parts, 2, kGradKeys, d rounded up to four)
+    float* sink_partials;  // (batch * kv_heads, sink_tiles, sink_parts, 2, keys, d rounded up to four)
     float* partials;       // the same of the other tiles
 };
 
@@ -91,14 +91,13 @@ __global__ __launch_bounds__(256) void attention_stats_kernel(GradLaunch p, uint
 
 // ---------------------------------------------------------------------------------------------------- queries' gradients
 
-constexpr ForwardShape query_grad_shape(int elem_bytes, int pitch) { return forward_shape(elem_bytes, pitch, false); }
-
-template <typename T, int NB, bool VEC>
-__global__ __launch_bounds__(256, sizeof(T) * NB <= 8 ? 2 : 1) void attention_query_grad_kernel(GradLaunch p)
+template <typename T, int NB, bool FEW, bool VEC>
+__global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads(),
+                             sizeof(T) * NB <= 8 ? 2 : 1) void attention_query_grad_kernel(GradLaunch p)
 {
     constexpr int kPitch = pitch_of(NB);
-    constexpr ForwardShape kShape = query_grad_shape(sizeof(T), kPitch);
-    constexpr int kKeys = kShape.keys, kSubs = kKeys / kBlock, kThreads = 256;
+    constexpr ForwardShape kShape = forward_shape(sizeof(T), kPitch, FEW);
+    constexpr int kKeys = kShape.keys, kSubs = kKeys / kBlock, kThreads = 64 * kShape.row_waves, kJoin = kShape.key_waves;
     constexpr bool kUnits = std::is_same<T, _Float16>::value;
     extern __shared__ __align__(16) char lds[];
 
@@ -114,7 +113,8 @@ __global__ __launch_bounds__(256, sizeof(T) * NB <= 8 ? 2 : 1) void attention_qu
     const int d = (int)a.d, left = (int)a.left, right = (int)a.right, sinks = (int)a.sinks;
     const Sequence seq = sequence_at(a, b);
 
-    const uint32_t row0 = tile * kShape.rows(), wave_row0 = row0 + wave * kBlock;
+    const int row_wave = wave % kShape.row_waves, key_wave = wave / kShape.row_waves;
+    const uint32_t row0 = tile * kShape.rows(), wave_row0 = row0 + row_wave * kBlock;
     const uint32_t row = min(wave_row0 + own, p.rows - 1);
     const int query = (int)fast_div(row, p.group);
     const int head = (int)(kv_head * p.group.div) + (int)(row - (uint32_t)query * p.group.div);
@@ -132,13 +132,15 @@ __global__ __launch_bounds__(256, sizeof(T) * NB <= 8 ? 2 : 1) void attention_qu
     const T* const v_base = (const T*)a.v.ptr + (int64_t)b * a.v.stride[0] + (int64_t)kv_head * a.v.stride[2];
     const uint32_t k_pitch = (uint32_t)(a.k.stride[1] * (int64_t)sizeof(T));
     const uint32_t v_pitch = (uint32_t)(a.v.stride[1] * (int64_t)sizeof(T));
-    T* const ring = reinterpret_cast<T*>(lds);
+    T* const ring = reinterpret_cast<T*>(lds) + (size_t)key_wave * (kShape.stages * 2 * kKeys * kPitch);
     const auto fetch = [&](int t, int buffer) {
         const int key0 = range.key_of(t, kKeys), rows = range.end_of(t) - key0;
         T* const k_tile = ring + buffer * (2 * kKeys * kPitch);
-        const int gt = wave * 64 + again(lane);
-        stage<T, kPitch, kKeys, kThreads, VEC>(k_tile, at_bytes(k_base, (uint32_t)key0, k_pitch), gt, wave, d, k_pitch, min(rows, kKeys));
-        stage<T, kPitch, kKeys, kThreads, VEC>(k_tile + kKeys * kPitch, at_bytes(v_base, (uint32_t)key0, v_pitch), gt, wave, d, v_pitch,
+        const int gt = row_wave * 64 + again(lane);
+        stage<T, kPitch, kKeys, kThreads, VEC>(k_tile, at_bytes(k_base, (uint32_t)key0, k_pitch), gt, row_wave, d, k_pitch,
+                                               min(rows, kKeys));
+        stage<T, kPitch, kKeys, kThreads, VEC>(k_tile + kKeys * kPitch, at_bytes(v_base, (uint32_t)key0, v_pitch), gt, row_wave, d,
+                                               v_pitch,
                                          min(rows, kKeys));
     };
     const float c = a.scale * kLog2e;
@@ -148,8 +150,9 @@ __global__ __launch_bounds__(256, sizeof(T) * NB <= 8 ? 2 : 1) void attention_qu
         gq[i] = zeros();
     }
     int buffer = 0;
-    if (range.tiles > 0) {
-        fetch(0, 0);
+    constexpr int kInFlight = 2 * kKeys * Tile<T, kPitch>::kChunks / kThreads;  // loads of one fetch, a wavefront
+    if (key_wave < range.tiles) {
+        fetch(key_wave, 0);
     }
     Frag<T> q[2 * NB], go[2 * NB];
     {
@@ -169,12 +172,21 @@ __global__ __launch_bounds__(256, sizeof(T) * NB <= 8 ? 2 : 1) void attention_qu
     wait_for_registers();
     const Rows32<T, kPitch, NB> rows(lane);
     const Columns32<T, kPitch, NB> columns(lane);
-    for (int t = 0; t < range.tiles; t++) {
-        const bool more = t + 1 < range.tiles;
-        wait_for_loads<0>();  // as in the forward pass
-        barrier();
-        if (kShape.stages == 2 && more) {
-            fetch(t + 1, buffer ^ 1);
+    for (int t = key_wave; t < range.tiles; t += kJoin) {
+        const bool more = t + kJoin < range.tiles;
+        if constexpr (kJoin == 1) {  // as in the forward pass
+            wait_for_loads<0>();
+            barrier();
+            if (kShape.stages == 2 && more) {
+                fetch(t + 1, buffer ^ 1);
+            }
+        } else {
+            if (kShape.stages == 2 && more) {
+                fetch(t + kJoin, buffer ^ 1);
+                wait_for_loads<VEC ? kInFlight : 0>();
+            } else {
+                wait_for_loads<0>();
+            }
         }
         const T* const k_tile = ring + buffer * (2 * kKeys * kPitch);
         const T* const v_tile = k_tile + kKeys * kPitch;
@@ -216,45 +228,85 @@ __global__ __launch_bounds__(256, sizeof(T) * NB <= 8 ? 2 : 1) void attention_qu
             }
         }
         if (kShape.stages == 1 && more) {
-            barrier();
-            fetch(t + 1, 0);
+            if constexpr (kJoin == 1) {
+                barrier();
+            } else {
+                wait_for_lds();
+            }
+            fetch(t + kJoin, 0);
         }
         buffer ^= kShape.stages - 1;
+    }
+    if constexpr (kJoin > 1) {
+        // sums of the wavefronts that shared the keys, [feature][row]; every one adds up a share of the features
+        constexpr int kWaveFloats = NB * kBlock * kBlock;
+        float* const sums = reinterpret_cast<float*>(lds);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                sums[wave * kWaveFloats + (i * kBlock + 8 * (r / 4) + 4 * h + r % 4) * kBlock + own] = gq[i][r];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+            if (i % kJoin == wave) {
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    float x = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < kJoin; w++) {
+                        x += sums[w * kWaveFloats + (i * kBlock + 8 * (r / 4) + 4 * h + r % 4) * kBlock + own];
+                    }
+                    gq[i][r] = x;
+                }
+            }
+        }
     }
     if (wave_row0 + own >= p.rows) {
         return;
     }
     const float f = a.scale * unit;
-    // a row that sees nothing has the gradient 0, also where its unit is one of an infinite gradient
     T* const to = (T*)a.grad_q.ptr + (int64_t)b * a.grad_q.stride[0] + (int64_t)query * a.grad_q.stride[1] +
                   (int64_t)head * a.grad_q.stride[2];
 #pragma unroll
     for (int i = 0; i < NB; i++) {
+        if (kJoin == 1 || i % kJoin == wave) {
 #pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            put4<T, VEC>(to, i * kBlock + 8 * (r / 4) + 4 * h, d, gq[i][r] * f, gq[i][r + 1] * f, gq[i][r + 2] * f,
-                         gq[i][r + 3] * f);
+            for (int r = 0; r < 16; r += 4) {
+                put4<T, VEC>(to, i * kBlock + 8 * (r / 4) + 4 * h, d, gq[i][r] * f, gq[i][r + 1] * f, gq[i][r + 2] * f,
+                             gq[i][r + 3] * f);
+            }
         }
     }
 }
 
 // ------------------------------------------------------------------------------------------------------- keys' gradients
 
-constexpr int key_grad_stages(int elem_bytes, int pitch) { return elem_bytes * pitch <= 512 ? 2 : 1; }
-// The values of the 128 keys are read from LDS for every product, which leaves 16-bit heads of up to 128 features within
-// the 256 registers of two wavefronts a SIMD (with the values in registers too, one: the accumulators then lie in the other
+// Both gradients in one pass, or, for heads of more than 128 features, whose two sums would not fit the registers, one after
+// the other (the scores' product is done twice: five products instead of four).
+enum KeyGradPass : int { kBothGrads = 0, kValueGrad = 1, kKeyGrad = 2 };
+
+// The values of the keys are read from LDS for every product, which leaves 16-bit heads of up to 128 features within the
+// 256 registers of two wavefronts a SIMD (with the values in registers too, one: the accumulators then lie in the other
 // half of the register file and are copied to and fro; 4096 tokens, 32 heads on 8, window 1024: 366 us against 187).
-constexpr bool key_grad_values_in_lds(int elem_bytes, int pitch) { return elem_bytes * pitch <= 512; }
+// FLOAT keeps them in registers: LDS then holds four workgroups a CU.
+constexpr bool key_grad_values_in_lds(int elem_bytes) { return elem_bytes == 2; }
+constexpr int key_grad_stages(int elem_bytes) { return elem_bytes == 2 ? 2 : 1; }
 constexpr int key_grad_waves(int elem_bytes, int nb) { return elem_bytes * nb <= 8 ? 2 : 1; }
 
-template <typename T, int NB, bool VEC>
-__global__ __launch_bounds__(64 * kKeyWaves, key_grad_waves(sizeof(T), NB)) void attention_key_grad_kernel(GradLaunch p)
+template <typename T, int NB, int PASS, bool VEC>
+__global__ __launch_bounds__(64 * grad_key_waves(sizeof(T) == 4, NB), key_grad_waves(sizeof(T), NB)) void
+attention_key_grad_kernel(GradLaunch p)
 {
-    constexpr int kPitch = pitch_of(NB), kThreads = 64 * kKeyWaves, kStages = key_grad_stages(sizeof(T), kPitch);
+    constexpr int kKeyWaves = grad_key_waves(sizeof(T) == 4, NB), kGradKeys = kBlock * kKeyWaves;
+    constexpr int kPitch = pitch_of(NB), kThreads = 64 * kKeyWaves, kStages = key_grad_stages(sizeof(T));
     constexpr bool kUnits = std::is_same<T, _Float16>::value;
     constexpr int kStatRows = kUnits ? 4 : 2;  // of 32 floats each, a wavefront and stage
     constexpr int kTile = kBlock * kPitch;     // elements
-    constexpr bool kValuesInLds = key_grad_values_in_lds(sizeof(T), kPitch);
+    constexpr bool kValuesInLds = key_grad_values_in_lds(sizeof(T)), kWithKeys = PASS != kValueGrad, kWithValues = PASS != kKeyGrad;
     extern __shared__ __align__(16) char lds[];
 
     const AttentionArgs& a = p.a;
@@ -340,12 +392,12 @@ __global__ __launch_bounds__(64 * kKeyWaves, key_grad_waves(sizeof(T), NB)) void
     if (s_begin < s_end) {
         fetch(0);
     }
-    Frag<T> k[2 * NB], v[kValuesInLds ? 1 : 2 * NB];
+    Frag<T> k[2 * NB], v[kValuesInLds || !kWithKeys ? 1 : 2 * NB];
     {
         const int64_t from = min(key, (int)a.kv_tokens - 1);
         const T* const k_first = (const T*)a.k.ptr + (int64_t)b * a.k.stride[0] + (int64_t)kv_head * a.k.stride[2];
         const T* const v_first = (const T*)a.v.ptr + (int64_t)b * a.v.stride[0] + (int64_t)kv_head * a.v.stride[2];
-        if constexpr (kValuesInLds) {
+        if constexpr (kValuesInLds && kWithKeys) {
             if (last >= key0) {
                 const uint32_t v_pitch = (uint32_t)(a.v.stride[1] * (int64_t)sizeof(T));
                 stage<T, kPitch, kGradKeys, kThreads, VEC>(v_tile, at_bytes(v_first, (uint32_t)key0, v_pitch), wave * 64 + lane,
@@ -355,7 +407,7 @@ __global__ __launch_bounds__(64 * kKeyWaves, key_grad_waves(sizeof(T), NB)) void
 #pragma unroll
         for (int i = 0; i < 2 * NB; i++) {
             k[i] = global_row<T, VEC>(k_first + from * a.k.stride[1], 16 * i + 8 * h, d);
-            if constexpr (!kValuesInLds) {
+            if constexpr (!kValuesInLds && kWithKeys) {
                 v[i] = global_row<T, VEC>(v_first + from * a.v.stride[1], 16 * i + 8 * h, d);
             }
         }
@@ -380,7 +432,7 @@ __global__ __launch_bounds__(64 * kKeyWaves, key_grad_waves(sizeof(T), NB)) void
         const bool all_seen = wave_key0 + kBlock <= seq.kv_len && wave_key0 + kBlock - 1 <= p_low + right &&
                               (wave_key0 >= p_high - left || wave_key0 + kBlock <= sinks);
         if (any) {
-            if constexpr (kUnits) {
+            if constexpr (kUnits && kWithKeys) {
                 float most = stat[2 * kBlock + own];
 #pragma unroll
                 for (int w = 16; w > 0; w >>= 1) {
@@ -408,23 +460,27 @@ __global__ __launch_bounds__(64 * kKeyWaves, key_grad_waves(sizeof(T), NB)) void
             if constexpr (sizeof(T) == 2) {
                 read_ahead<2 * NB, 1, 4>();
             }
+            if constexpr (kWithKeys) {
 #pragma unroll
-            for (int i = 0; i < 2 * NB; i++) {
-                const Frag<T> g = rows(go_tile, 0, i);
-                if constexpr (kValuesInLds) {
-                    dp = Mma<T>::mul(g, rows(v_tile, wave * kBlock, i), dp);
-                } else {
-                    dp = Mma<T>::mul(g, v[i], dp);
+                for (int i = 0; i < 2 * NB; i++) {
+                    const Frag<T> g = rows(go_tile, 0, i);
+                    if constexpr (kValuesInLds) {
+                        dp = Mma<T>::mul(g, rows(v_tile, wave * kBlock, i), dp);
+                    } else {
+                        dp = Mma<T>::mul(g, v[i], dp);
+                    }
                 }
-            }
-            if constexpr (sizeof(T) == 2) {
-                read_ahead<2 * NB, 2, 3>();
+                if constexpr (sizeof(T) == 2) {
+                    read_ahead<2 * NB, 2, 3>();
+                }
             }
 #pragma unroll
             for (int r = 0; r < 16; r++) {
                 const int n = 8 * (r / 4) + 4 * h + r % 4;
                 s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -stat[n]));
-                dp[r] = s[r] * ((dp[r] - stat[kBlock + n]) * per_unit);
+                if constexpr (kWithKeys) {
+                    dp[r] = s[r] * ((dp[r] - stat[kBlock + n]) * per_unit);
+                }
             }
             if (__builtin_expect(!all_seen, 0)) {
                 // query p_low + n sees the key: n >= first, n <= last or the key a sink, the key within the sequence
@@ -444,12 +500,16 @@ __global__ __launch_bounds__(64 * kKeyWaves, key_grad_waves(sizeof(T), NB)) void
                 const Frag<T> w = operand<T>(s, g), x = operand<T>(dp, g);
 #pragma unroll
                 for (int i = 0; i < NB; i++) {
-                    gv[i] = Mma<T>::mul(columns(go_tile, 16 * g, i), w, gv[i]);
-                    gk[i] = Mma<T>::mul(columns(q_tile, 16 * g, i), x, gk[i]);
+                    if constexpr (kWithValues) {
+                        gv[i] = Mma<T>::mul(columns(go_tile, 16 * g, i), w, gv[i]);
+                    }
+                    if constexpr (kWithKeys) {
+                        gk[i] = Mma<T>::mul(columns(q_tile, 16 * g, i), x, gk[i]);
+                    }
                 }
             }
             if constexpr (sizeof(T) == 2) {
-                read_ahead<4 * NB, 2, 4>();
+                read_ahead<(PASS == kBothGrads ? 4 : 2) * NB, 2, 4>();
             }
         }
         if (kStages == 1 && more) {
@@ -473,8 +533,12 @@ __global__ __launch_bounds__(64 * kKeyWaves, key_grad_waves(sizeof(T), NB)) void
                 if (el < d) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        to[el + e] = gk[i][r + e] * f;
-                        to[(int64_t)kGradKeys * row_floats + el + e] = gv[i][r + e];
+                        if constexpr (kWithKeys) {
+                            to[el + e] = gk[i][r + e] * f;
+                        }
+                        if constexpr (kWithValues) {
+                            to[(int64_t)kGradKeys * row_floats + el + e] = gv[i][r + e];
+                        }
                     }
                 }
             }
@@ -493,8 +557,12 @@ __global__ __launch_bounds__(64 * kKeyWaves, key_grad_waves(sizeof(T), NB)) void
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
             const int el = i * kBlock + 8 * (r / 4) + 4 * h;
-            put4<T, VEC>(to_k, el, d, gk[i][r] * f, gk[i][r + 1] * f, gk[i][r + 2] * f, gk[i][r + 3] * f);
-            put4<T, VEC>(to_v, el, d, gv[i][r], gv[i][r + 1], gv[i][r + 2], gv[i][r + 3]);
+            if constexpr (kWithKeys) {
+                put4<T, VEC>(to_k, el, d, gk[i][r] * f, gk[i][r + 1] * f, gk[i][r + 2] * f, gk[i][r + 3] * f);
+            }
+            if constexpr (kWithValues) {
+                put4<T, VEC>(to_v, el, d, gv[i][r], gv[i][r + 1], gv[i][r + 2], gv[i][r + 3]);
+            }
         }
     }
 }
@@ -512,22 +580,22 @@ __global__ __launch_bounds__(256) void attention_grad_join_kernel(GradLaunch p, 
     }
     const uint32_t quad = index % quads;
     uint32_t rest = index / quads;
-    const uint32_t local_key = rest % kGradKeys;
-    rest /= kGradKeys;
+    const uint32_t local_key = rest % p.keys;
+    rest /= p.keys;
     const uint32_t value = rest & 1, tile_index = rest >> 1;
     const uint32_t tile = first + tile_index % tiles, bh = tile_index / tiles;
-    const int64_t key = (int64_t)tile * kGradKeys + local_key;
+    const int64_t key = (int64_t)tile * p.keys + local_key;
     if (key >= a.kv_tokens) {
         return;
     }
     const int row_floats = (int)quads * 4;
     const float* const from =
-        partials + (((int64_t)tile_index * parts * 2 + value) * kGradKeys + local_key) * row_floats + quad * 4;
+        partials + (((int64_t)tile_index * parts * 2 + value) * p.keys + local_key) * row_floats + quad * 4;
     float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (uint32_t i = 0; i < parts; i++) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            x[e] += from[(int64_t)i * 2 * kGradKeys * row_floats + e];
+            x[e] += from[(int64_t)i * 2 * p.keys * row_floats + e];
         }
     }
     const Strided& out = value != 0 ? a.grad_v : a.grad_k;
@@ -536,37 +604,66 @@ __global__ __launch_bounds__(256) void attention_grad_join_kernel(GradLaunch p, 
     put4<T, VEC>(to, (int)quad * 4, (int)a.d, x[0], x[1], x[2], x[3]);
 }
 
-template <typename T, int NB, bool VEC>
-hipError_t run_backward_shape(const GradLaunch& p, hipStream_t stream)
+template <typename T, int NB, bool FEW, bool VEC>
+hipError_t launch_query_grad(const GradLaunch& p, hipStream_t stream)
 {
-    constexpr int kPitch = pitch_of(NB);
-    constexpr ForwardShape kShape = query_grad_shape(sizeof(T), kPitch);
-    constexpr int kQueryBytes = kShape.stages * 2 * kShape.keys * kPitch * (int)sizeof(T);
-    constexpr int kStages = key_grad_stages(sizeof(T), kPitch);
-    constexpr int kKeyBytes = kStages * 2 * kBlock * kPitch * (int)sizeof(T) +
-                              kKeyWaves * kStages * (std::is_same<T, _Float16>::value ? 4 : 2) * kBlock * 4 +
-                              (key_grad_values_in_lds(sizeof(T), kPitch) ? kGradKeys * kPitch * (int)sizeof(T) : 0);
-    static_assert(kQueryBytes <= 160 * 1024 && kKeyBytes <= 160 * 1024, "LDS of a CU");
-    static std::atomic<uint32_t> query_done{0}, key_done{0};
-    const auto query_kernel = attention_query_grad_kernel<T, NB, VEC>;
-    const auto key_kernel = attention_key_grad_kernel<T, NB, VEC>;
-    hipError_t e = hipSuccess;
-    if (kQueryBytes > 64 * 1024) {
-        e = allow_dynamic_lds((const void*)query_kernel, kQueryBytes, query_done);
+    constexpr ForwardShape kShape = forward_shape(sizeof(T), pitch_of(NB), FEW);
+    constexpr int kTiles = kShape.key_waves * kShape.stages * 2 * kShape.keys * pitch_of(NB) * (int)sizeof(T);
+    constexpr int kJoin = kShape.key_waves > 1 ? kShape.key_waves * NB * kBlock * kBlock * 4 : 0;
+    constexpr int kBytes = kTiles > kJoin ? kTiles : kJoin;
+    static_assert(kBytes <= 160 * 1024, "LDS of a CU");
+    static std::atomic<uint32_t> done{0};
+    const auto kernel = attention_query_grad_kernel<T, NB, FEW, VEC>;
+    if (kBytes > 64 * 1024) {
+        if (const hipError_t e = allow_dynamic_lds((const void*)kernel, kBytes, done); e != hipSuccess) {
+            return e;
+        }
     }
-    if (e == hipSuccess && kKeyBytes > 64 * 1024) {
-        e = allow_dynamic_lds((const void*)key_kernel, kKeyBytes, key_done);
-    }
-    if (e != hipSuccess) {
-        return e;
-    }
-    if (p.query_blocks > 0) {
-        hipLaunchKernelGGL(query_kernel, dim3((p.query_blocks + 7) / 8 * 8), dim3(kShape.threads()), kQueryBytes, stream, p);
-    }
-    if (p.key_blocks > 0) {
-        hipLaunchKernelGGL(key_kernel, dim3((p.key_blocks + 7) / 8 * 8), dim3(64 * kKeyWaves), kKeyBytes, stream, p);
-    }
+    hipLaunchKernelGGL(kernel, dim3((p.query_blocks + 7) / 8 * 8), dim3(kShape.threads()), kBytes, stream, p);
     return hipGetLastError();
+}
+
+template <typename T, int NB, int PASS, bool VEC>
+hipError_t launch_key_grad(const GradLaunch& p, hipStream_t stream)
+{
+    constexpr int kPitch = pitch_of(NB), kStages = key_grad_stages(sizeof(T)), kWaves = grad_key_waves(sizeof(T) == 4, NB);
+    constexpr int kBytes = kStages * 2 * kBlock * kPitch * (int)sizeof(T) +
+                           kWaves * kStages * (std::is_same<T, _Float16>::value ? 4 : 2) * kBlock * 4 +
+                           (key_grad_values_in_lds(sizeof(T)) ? kWaves * kBlock * kPitch * (int)sizeof(T) : 0);
+    static_assert(kBytes <= 160 * 1024, "LDS of a CU");
+    static std::atomic<uint32_t> done{0};
+    const auto kernel = attention_key_grad_kernel<T, NB, PASS, VEC>;
+    if (kBytes > 64 * 1024) {
+        if (const hipError_t e = allow_dynamic_lds((const void*)kernel, kBytes, done); e != hipSuccess) {
+            return e;
+        }
+    }
+    hipLaunchKernelGGL(kernel, dim3((p.key_blocks + 7) / 8 * 8), dim3(64 * kWaves), kBytes, stream, p);
+    return hipGetLastError();
+}
+
+template <typename T, int NB, bool VEC>
+hipError_t run_backward_shape(const GradLaunch& p, bool few, hipStream_t stream)
+{
+    hipError_t e = hipSuccess;
+    if (p.query_blocks > 0) {
+        if constexpr (sizeof(T) == 2) {
+            e = few ? launch_query_grad<T, NB, true, VEC>(p, stream) : launch_query_grad<T, NB, false, VEC>(p, stream);
+        } else {
+            e = few ? launch_query_grad<T, NB, true, VEC>(p, stream) : hipErrorInvalidValue;
+        }
+    }
+    if (e == hipSuccess && p.key_blocks > 0) {
+        if constexpr (NB <= 4) {
+            e = launch_key_grad<T, NB, kBothGrads, VEC>(p, stream);
+        } else {
+            e = launch_key_grad<T, NB, kValueGrad, VEC>(p, stream);
+            if (e == hipSuccess) {
+                e = launch_key_grad<T, NB, kKeyGrad, VEC>(p, stream);
+            }
+        }
+    }
+    return e;
 }
 
 template <typename T, bool VEC>
@@ -577,8 +674,8 @@ hipError_t run_backward(const AttentionArgs& a, hipStream_t stream)
     const int64_t query_blocks = bh * plan.tiles;
     const int64_t key_blocks = bh * (plan.sink_tiles * plan.sink_parts + (plan.key_tiles - plan.sink_tiles) * plan.parts);
     const int64_t quads = (a.d + 3) / 4;
-    const int64_t sink_joins = plan.sink_parts > 1 ? bh * plan.sink_tiles * 2 * kGradKeys * quads : 0;
-    const int64_t joins = plan.parts > 1 ? bh * (plan.key_tiles - plan.sink_tiles) * 2 * kGradKeys * quads : 0;
+    const int64_t sink_joins = plan.sink_parts > 1 ? bh * plan.sink_tiles * 2 * plan.keys * quads : 0;
+    const int64_t joins = plan.parts > 1 ? bh * (plan.key_tiles - plan.sink_tiles) * 2 * plan.keys * quads : 0;
     // 3 * tokens * 4 bytes of statistics are reached with 32-bit offsets
     if (query_blocks > INT32_MAX / 1024 || key_blocks > INT32_MAX / 1024 || stat_rows > INT32_MAX / 16 ||
         a.tokens > INT32_MAX / 12 || sink_joins > INT32_MAX || joins > INT32_MAX ||
@@ -591,6 +688,7 @@ hipError_t run_backward(const AttentionArgs& a, hipStream_t stream)
     p.rows = (uint32_t)plan.rows;
     p.tiles = (uint32_t)plan.tiles;
     p.kv_heads = (uint32_t)a.kv_heads;
+    p.keys = (uint32_t)plan.keys;
     p.key_tiles = (uint32_t)plan.key_tiles;
     p.sink_tiles = (uint32_t)plan.sink_tiles;
     p.sink_parts = (uint32_t)plan.sink_parts;
@@ -606,10 +704,10 @@ hipError_t run_backward(const AttentionArgs& a, hipStream_t stream)
     }
     hipError_t e = hipErrorInvalidValue;
     switch (blocks_of(a.d)) {
-        case 8: e = run_backward_shape<T, 8, VEC>(p, stream); break;
-        case 4: e = run_backward_shape<T, 4, VEC>(p, stream); break;
-        case 3: e = run_backward_shape<T, 3, VEC>(p, stream); break;
-        default: e = run_backward_shape<T, 2, VEC>(p, stream); break;
+        case 8: e = run_backward_shape<T, 8, VEC>(p, plan.few_rows, stream); break;
+        case 4: e = run_backward_shape<T, 4, VEC>(p, plan.few_rows, stream); break;
+        case 3: e = run_backward_shape<T, 3, VEC>(p, plan.few_rows, stream); break;
+        default: e = run_backward_shape<T, 2, VEC>(p, plan.few_rows, stream); break;
     }
     if (e != hipSuccess) {
         return e;

@@ -497,7 +497,11 @@ hipError_t run_forward(const AttentionArgs& a, hipStream_t stream)
         default: e = run_forward_shape<T, 2, kFew, VEC>(p, stream); break;
         }
     };
-    plan.few_rows ? pick(std::true_type()) : pick(std::false_type());
+    if (plan.few_rows) {
+        pick(std::true_type());
+    } else if constexpr (sizeof(T) == 2) {
+        pick(std::false_type());
+    }
     if (e != hipSuccess || plan.splits == 1) {
         return e;
     }

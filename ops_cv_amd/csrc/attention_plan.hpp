@@ -14,24 +14,24 @@ constexpr int kBlock = 32;
 constexpr int blocks_of(int64_t d) { return d <= 64 ? 2 : d <= 96 ? 3 : d <= 128 ? 4 : 8; }
 constexpr int pitch_of(int blocks) { return blocks <= 2 ? 64 : blocks <= 4 ? 128 : 256; }
 
-// Shape of a forward workgroup: kRowWaves wavefronts with 32 rows each (a row is a query of one of the heads that share
-// a key head) that read the same tiles, or one row wavefront's worth of rows with kKeyWaves wavefronts that take tiles of
-// their own in turn.
+// Shape of a workgroup that walks keys: row_waves wavefronts with 32 rows each (a row is a query of one of the heads that
+// share a key head) that read the same tiles, or few rows: 32 of them, and key_waves wavefronts that take tiles of their own
+// in turn.
 struct ForwardShape {
     int row_waves, key_waves, keys, stages;
     constexpr int threads() const { return 64 * row_waves * key_waves; }
     constexpr int rows() const { return kBlock * row_waves; }
 };
 
-// LDS decides: a tile of keys and one of values per stage and group of wavefronts, of at most 160 KB in all, so that two
-// workgroups fit a CU where rows are shared.
+// LDS decides: a tile of keys and one of values per stage and group of wavefronts.  Two workgroups of shared rows fit a CU's
+// 160 KB; of few rows, one of four wavefronts with two tiles each under way, or, where a tile is larger, five of one.
 constexpr ForwardShape forward_shape(int elem_bytes, int pitch, bool few_rows)
 {
     const int row = elem_bytes * pitch;  // bytes
-    if (!few_rows) {
-        return ForwardShape{4, 1, row <= 256 ? 64 : 32, row <= 512 ? 2 : 1};
+    if (few_rows) {
+        return row <= 256 ? ForwardShape{1, 4, 32, 2} : ForwardShape{1, 1, 32, 1};
     }
-    return row <= 256 ? ForwardShape{1, 4, 32, 2} : row <= 512 ? ForwardShape{1, 4, 32, 1} : ForwardShape{1, 2, 32, 1};
+    return ForwardShape{4, 1, row <= 256 ? 64 : 32, row <= 512 ? 2 : 1};
 }
 
 struct ForwardPlan {
@@ -45,12 +45,22 @@ struct ForwardPlan {
 // Partial results of a split: per row the largest score, the sum, and the weighted values.
 constexpr int64_t partial_floats(int64_t d) { return 2 + (d + 3) / 4 * 4; }
 
+// Tiles of 32 rows instead of tiles of 128: where those would leave CUs without work, where there are no more rows, and for
+// FLOAT, whose products take sixteen times as long as those of 16-bit types: what it costs that every 32 rows read their
+// keys themselves does not show, and no wavefront waits for another.
+inline bool few_rows(const AttentionArgs& a)
+{
+    const int64_t rows = a.tokens * (a.heads / a.kv_heads);
+    return a.elem == 0 || rows <= kBlock ||
+           a.batch * a.kv_heads * ((rows + 4 * kBlock - 1) / (4 * kBlock)) < a.compute_units;
+}
+
 inline ForwardPlan plan_forward(const AttentionArgs& a)
 {
     ForwardPlan p;
     const int64_t group = a.heads / a.kv_heads;
     p.rows = a.tokens * group;
-    p.few_rows = p.rows <= kBlock;
+    p.few_rows = few_rows(a);
     const ForwardShape s = forward_shape(a.elem == 0 ? 4 : 2, pitch_of(blocks_of(a.d)), p.few_rows);
     p.tiles = (p.rows + s.rows() - 1) / s.rows();
     const int64_t whole = a.batch * a.kv_heads * p.tiles;
@@ -58,8 +68,9 @@ inline ForwardPlan plan_forward(const AttentionArgs& a)
     const int64_t window = a.left + a.right + s.rows() / group + 2;
     const int64_t keys = a.kv_tokens < window + a.sinks ? a.kv_tokens : window + a.sinks;
     const int64_t key_tiles = (keys + s.keys - 1) / s.keys;
-    // two workgroups for every CU where that many parts leave each wavefront four tiles or more
-    const int64_t want = (2 * (int64_t)a.compute_units + whole - 1) / whole, most = key_tiles / (4 * s.key_waves);
+    // eight wavefronts for every CU where that many parts leave each four tiles or more
+    const int64_t waves = s.row_waves * s.key_waves;
+    const int64_t want = (8 * (int64_t)a.compute_units / waves + whole - 1) / whole, most = key_tiles / (4 * s.key_waves);
     p.splits = want < most ? want : most;
     p.splits = p.splits < 1 ? 1 : (p.splits > 64 ? 64 : p.splits);
     p.blocks = whole * p.splits;
@@ -68,12 +79,14 @@ inline ForwardPlan plan_forward(const AttentionArgs& a)
 
 // ---------------------------------------------------------------------------------------------------------- gradients
 
-// The keys' gradients: a workgroup has four wavefronts with 32 keys each and walks tiles of 32 queries of one head.
-constexpr int kKeyWaves = 4;
-constexpr int kGradKeys = kKeyWaves * kBlock;
+// The keys' gradients: a wavefront has 32 keys and walks tiles of 32 queries of one head.  16-bit types: four wavefronts walk
+// together, so that a tile of queries is loaded once for 128 keys.  FLOAT: each by itself, for the same reason as above.
+constexpr int grad_key_waves(bool is_float, int nb) { return is_float && nb <= 4 ? 1 : 4; }
 
 struct GradPlan {
+    bool few_rows = false;
     int64_t rows = 0, tiles = 0;       // of the queries' gradients, as in the forward pass
+    int64_t keys = 0;                  // of a tile
     int64_t key_tiles = 0;             // of a key head
     int64_t sink_tiles = 0;            // the first of them, seen by queries of any position
     int64_t sink_parts = 1, parts = 1; // parts that the queries of such a tile, and of the others, are cut into
@@ -86,25 +99,41 @@ inline GradPlan plan_grad(const AttentionArgs& a)
     GradPlan p;
     const int64_t group = a.heads / a.kv_heads, bh = a.batch * a.kv_heads;
     p.rows = a.tokens * group;
-    p.tiles = (p.rows + 4 * kBlock - 1) / (4 * kBlock);
-    p.key_tiles = (a.kv_tokens + kGradKeys - 1) / kGradKeys;
+    p.few_rows = few_rows(a);
+    const int64_t tile_rows = p.few_rows ? kBlock : 4 * kBlock;
+    p.tiles = (p.rows + tile_rows - 1) / tile_rows;
+    p.keys = kBlock * grad_key_waves(a.elem == 0, blocks_of(a.d));
+    p.key_tiles = (a.kv_tokens + p.keys - 1) / p.keys;
     const int64_t sinks = a.sinks < a.kv_tokens ? a.sinks : a.kv_tokens;
-    p.sink_tiles = (sinks + kGradKeys - 1) / kGradKeys;
+    p.sink_tiles = (sinks + p.keys - 1) / p.keys;
     // steps (tiles of 32 queries, of every head of the group) of a tile of keys, at most
     const int64_t all = (a.tokens + kBlock - 1) / kBlock;
-    const int64_t window = (a.left + a.right + kGradKeys + kBlock - 1) / kBlock + 1;
+    const int64_t window = (a.left + a.right + p.keys + kBlock - 1) / kBlock + 1;
     const int64_t steps = group * (window < all ? window : all);
-    // two workgroups for every CU where that leaves a part eight steps or more
-    const int64_t whole = bh * p.key_tiles > 0 ? bh * p.key_tiles : 1;
-    int64_t each = (steps * whole + 2 * a.compute_units - 1) / (2 * a.compute_units);
-    each = each < 8 ? 8 : each;
-    each = each < steps ? each : (steps > 0 ? steps : 1);
-    p.parts = (steps + each - 1) / each;
-    p.sink_parts = (group * all + each - 1) / each;
+    // As few parts as fill the card with one round of workgroups, the shorter ones last: ten wavefronts for every CU, of
+    // which eight run at a time, where a part has eight steps or more (4096 tokens, 32 heads of 128 on 8, window 1024, bf16:
+    // 302 us for the whole backward call, with eight 348, with fourteen 323).  FLOAT: one step or more, and four wavefronts,
+    // which is what its registers leave room for from three blocks of features on.
+    const int64_t sink_steps = group * all;
+    const int64_t room = a.compute_units * (a.elem != 0 ? 10 : blocks_of(a.d) > 2 ? 4 : 8) * kBlock / p.keys;
+    const auto items = [&](int64_t each) {
+        return bh * (p.sink_tiles * ((sink_steps + each - 1) / each) + (p.key_tiles - p.sink_tiles) * ((steps + each - 1) / each));
+    };
+    int64_t low = a.elem == 0 ? 1 : 8, high = steps > low ? steps : low;  // the fewest steps whose parts fit, or all
+    while (low < high) {
+        const int64_t middle = (low + high) / 2;
+        if (items(middle) <= room) {
+            high = middle;
+        } else {
+            low = middle + 1;
+        }
+    }
+    p.parts = (steps + low - 1) / low;
+    p.sink_parts = (sink_steps + low - 1) / low;
     p.parts = p.parts < 1 ? 1 : p.parts;
     p.sink_parts = p.sink_parts < 1 ? 1 : p.sink_parts;
     p.stats = 3 * a.batch * a.heads * a.tokens;
-    const int64_t tile_floats = 2 * kGradKeys * ((a.d + 3) / 4 * 4);
+    const int64_t tile_floats = 2 * p.keys * ((a.d + 3) / 4 * 4);
     p.sink_partials = p.sink_parts > 1 ? bh * p.sink_tiles * p.sink_parts * tile_floats : 0;
     p.partials = p.parts > 1 ? bh * (p.key_tiles - p.sink_tiles) * p.parts * tile_floats : 0;
     return p;
