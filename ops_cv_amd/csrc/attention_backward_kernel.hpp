@@ -33,6 +33,7 @@ struct GradLaunch {
     FastDiv group;
     uint32_t rows, tiles, kv_heads;
     uint32_t keys, key_tiles, sink_tiles, sink_parts, parts;
+    int32_t each;  // steps of a part; the last one has the rest
     uint32_t query_blocks, key_blocks;
     float* stats;          // (batch, heads, 3, tokens)
     float* sink_partials;  // (batch * kv_heads, sink_tiles, sink_parts, 2, keys, d rounded up to four)
@@ -302,7 +303,8 @@ __global__ __launch_bounds__(64 * grad_key_waves(sizeof(T) == 4, NB), key_grad_w
 attention_key_grad_kernel(GradLaunch p)
 {
     constexpr int kKeyWaves = grad_key_waves(sizeof(T) == 4, NB), kGradKeys = kBlock * kKeyWaves;
-    constexpr int kPitch = pitch_of(NB), kThreads = 64 * kKeyWaves, kStages = key_grad_stages(sizeof(T));
+    constexpr int kPitch = pitch_of(NB), kThreads = 64 * kKeyWaves;
+    constexpr int kStages = key_grad_stages(sizeof(T));
     constexpr bool kUnits = std::is_same<T, _Float16>::value;
     constexpr int kStatRows = kUnits ? 4 : 2;  // of 32 floats each, a wavefront and stage
     constexpr int kTile = kBlock * kPitch;     // elements
@@ -337,7 +339,7 @@ attention_key_grad_kernel(GradLaunch p)
     }
     const int row_tiles = high > low ? (high - low + kBlock - 1) / kBlock : 0;
     const int steps = row_tiles * (int)p.group.div;
-    const int s_begin = (int)((int64_t)steps * part / of), s_end = (int)((int64_t)steps * (part + 1) / of);
+    const int s_begin = min((int)part * p.each, steps), s_end = part + 1 == of ? steps : min(s_begin + p.each, steps);
 
     T* const ring = reinterpret_cast<T*>(lds);
     float* const stat_ring = reinterpret_cast<float*>(lds + (size_t)kStages * 2 * kTile * sizeof(T)) +
@@ -351,7 +353,7 @@ attention_key_grad_kernel(GradLaunch p)
     const T* const go_base = (const T*)a.grad_out.ptr + (int64_t)b * a.grad_out.stride[0] + head0 * a.grad_out.stride[2];
     const float* const stat_base = p.stats + stats_row(a, b, head0);
     // steps go through the tiles of one head's queries, then the next head's; `f_`: the step that is fetched next
-    int f_head = row_tiles > 0 ? s_begin / row_tiles : 0, f_query = low + (s_begin - f_head * row_tiles) * kBlock;
+    int f_head = s_begin < s_end ? s_begin / row_tiles : 0, f_query = low + (s_begin - f_head * row_tiles) * kBlock;
     int c_query = f_query;
     const auto fetch = [&](int buffer) {
         const int rows = min(seq.q_len - f_query, kBlock);
@@ -626,7 +628,8 @@ hipError_t launch_query_grad(const GradLaunch& p, hipStream_t stream)
 template <typename T, int NB, int PASS, bool VEC>
 hipError_t launch_key_grad(const GradLaunch& p, hipStream_t stream)
 {
-    constexpr int kPitch = pitch_of(NB), kStages = key_grad_stages(sizeof(T)), kWaves = grad_key_waves(sizeof(T) == 4, NB);
+    constexpr int kPitch = pitch_of(NB);
+    constexpr int kStages = key_grad_stages(sizeof(T)), kWaves = grad_key_waves(sizeof(T) == 4, NB);
     constexpr int kBytes = kStages * 2 * kBlock * kPitch * (int)sizeof(T) +
                            kWaves * kStages * (std::is_same<T, _Float16>::value ? 4 : 2) * kBlock * 4 +
                            (key_grad_values_in_lds(sizeof(T)) ? kWaves * kBlock * kPitch * (int)sizeof(T) : 0);
@@ -693,6 +696,7 @@ hipError_t run_backward(const AttentionArgs& a, hipStream_t stream)
     p.sink_tiles = (uint32_t)plan.sink_tiles;
     p.sink_parts = (uint32_t)plan.sink_parts;
     p.parts = (uint32_t)plan.parts;
+    p.each = (int32_t)plan.each;
     p.query_blocks = (uint32_t)query_blocks;
     p.key_blocks = (uint32_t)key_blocks;
     p.stats = a.scratch;
@@ -707,7 +711,8 @@ hipError_t run_backward(const AttentionArgs& a, hipStream_t stream)
         case 8: e = run_backward_shape<T, 8, VEC>(p, plan.few_rows, stream); break;
         case 4: e = run_backward_shape<T, 4, VEC>(p, plan.few_rows, stream); break;
         case 3: e = run_backward_shape<T, 3, VEC>(p, plan.few_rows, stream); break;
-        default: e = run_backward_shape<T, 2, VEC>(p, plan.few_rows, stream); break;
+        case 2: e = run_backward_shape<T, 2, VEC>(p, plan.few_rows, stream); break;
+        default: e = run_backward_shape<T, 1, VEC>(p, plan.few_rows, stream); break;
     }
     if (e != hipSuccess) {
         return e;

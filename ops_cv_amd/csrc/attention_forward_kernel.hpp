@@ -494,7 +494,8 @@ hipError_t run_forward(const AttentionArgs& a, hipStream_t stream)
             case 8: e = run_forward_shape<T, 8, kFew, VEC>(p, stream); break;
             case 4: e = run_forward_shape<T, 4, kFew, VEC>(p, stream); break;
             case 3: e = run_forward_shape<T, 3, kFew, VEC>(p, stream); break;
-        default: e = run_forward_shape<T, 2, kFew, VEC>(p, stream); break;
+        case 2: e = run_forward_shape<T, 2, kFew, VEC>(p, stream); break;
+        default: e = run_forward_shape<T, 1, kFew, VEC>(p, stream); break;
         }
     };
     if (plan.few_rows) {

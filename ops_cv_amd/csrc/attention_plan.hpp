@@ -11,7 +11,7 @@ namespace att {
 // A product's result is 32 x 32; heads are cut into blocks of 32 features, and a tile's row has room for PITCH.
 constexpr int kBlock = 32;
 
-constexpr int blocks_of(int64_t d) { return d <= 64 ? 2 : d <= 96 ? 3 : d <= 128 ? 4 : 8; }
+constexpr int blocks_of(int64_t d) { return d <= 32 ? 1 : d <= 64 ? 2 : d <= 96 ? 3 : d <= 128 ? 4 : 8; }
 constexpr int pitch_of(int blocks) { return blocks <= 2 ? 64 : blocks <= 4 ? 128 : 256; }
 
 // Shape of a workgroup that walks keys: row_waves wavefronts with 32 rows each (a row is a query of one of the heads that
@@ -24,7 +24,8 @@ struct ForwardShape {
 };
 
 // LDS decides: a tile of keys and one of values per stage and group of wavefronts.  Two workgroups of shared rows fit a CU's
-// 160 KB; of few rows, one of four wavefronts with two tiles each under way, or, where a tile is larger, five of one.
+// 160 KB; of few rows, one of four wavefronts with two tiles each under way, or, where a tile is larger, five of one
+// wavefront and one tile.
 constexpr ForwardShape forward_shape(int elem_bytes, int pitch, bool few_rows)
 {
     const int row = elem_bytes * pitch;  // bytes
@@ -89,7 +90,8 @@ struct GradPlan {
     int64_t keys = 0;                  // of a tile
     int64_t key_tiles = 0;             // of a key head
     int64_t sink_tiles = 0;            // the first of them, seen by queries of any position
-    int64_t sink_parts = 1, parts = 1; // parts that the queries of such a tile, and of the others, are cut into
+    int64_t each = 1;                  // steps of a part
+    int64_t sink_parts = 1, parts = 1; // parts that the queries of such a tile, and of the others, are cut into at most
     // 32-bit words of the scratch: statistics of the rows, partial gradients of the sinks' tiles and of the others
     int64_t stats = 0, sink_partials = 0, partials = 0;
 };
@@ -112,10 +114,11 @@ inline GradPlan plan_grad(const AttentionArgs& a)
     const int64_t steps = group * (window < all ? window : all);
     // As few parts as fill the card with one round of workgroups, the shorter ones last: ten wavefronts for every CU, of
     // which eight run at a time, where a part has eight steps or more (4096 tokens, 32 heads of 128 on 8, window 1024, bf16:
-    // 302 us for the whole backward call, with eight 348, with fourteen 323).  FLOAT: one step or more, and four wavefronts,
-    // which is what its registers leave room for from three blocks of features on.
+    // 302 us for the whole backward call, with eight 348, with fourteen 323).  FLOAT: one step or more, and as many
+    // wavefronts as its registers leave room for: four from three blocks of features on, eight of two, and of one block many
+    // short parts (3 x 1024 tokens, 64 heads of 32 on 8: 732 us with 32, with eight 937).
     const int64_t sink_steps = group * all;
-    const int64_t room = a.compute_units * (a.elem != 0 ? 10 : blocks_of(a.d) > 2 ? 4 : 8) * kBlock / p.keys;
+    const int64_t room = a.compute_units * (a.elem != 0 ? 10 : blocks_of(a.d) > 2 ? 4 : blocks_of(a.d) == 2 ? 8 : 32) * kBlock / p.keys;
     const auto items = [&](int64_t each) {
         return bh * (p.sink_tiles * ((sink_steps + each - 1) / each) + (p.key_tiles - p.sink_tiles) * ((steps + each - 1) / each));
     };
@@ -128,6 +131,7 @@ inline GradPlan plan_grad(const AttentionArgs& a)
             low = middle + 1;
         }
     }
+    p.each = low;
     p.parts = (steps + low - 1) / low;
     p.sink_parts = (sink_steps + low - 1) / low;
     p.parts = p.parts < 1 ? 1 : p.parts;
