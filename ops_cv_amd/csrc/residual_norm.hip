@@ -91,7 +91,7 @@ __device__ __forceinline__ void put_row_part(const NormArgs& a, int64_t row, int
         for (int i = 0; i < VEC; i++) {
             y[i] = h[i] * w[i] * rstd;
         }
-        store_part<T, VEC, WIDE>((T*)a.y.ptr + row * a.y.row_stride, c, a.width, y);
+        store_part<T, VEC, WIDE>((T*)a.y.ptr + row * a.y.row_stride, c, a.width, y, a.streaming != 0);
     }
 }
 
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void norm_kernel(Nor
             }
             if (c < a.width) {
                 if (a.sum.ptr != nullptr) {
-                    store_part<T, VEC, WIDE>((T*)a.sum.ptr + row * a.sum.row_stride, c, a.width, h[j]);
+                    store_part<T, VEC, WIDE>((T*)a.sum.ptr + row * a.sum.row_stride, c, a.width, h[j], a.streaming != 0);
                 }
                 if constexpr (INT8) {
                     float w[VEC];
@@ -221,7 +221,7 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a)
         float h[VEC];
         get_row_part<T, VEC, WIDE>(a, row, c, h);
         if (a.sum.ptr != nullptr) {
-            store_part<T, VEC, WIDE>((T*)a.sum.ptr + row * a.sum.row_stride, c, a.width, h);
+            store_part<T, VEC, WIDE>((T*)a.sum.ptr + row * a.sum.row_stride, c, a.width, h, a.streaming != 0);
         }
         put_row_part<T, W, INT8, VEC, WIDE>(a, row, c, h, rstd, step);
     }
@@ -269,13 +269,43 @@ hipError_t run_norm_type(const NormArgs& a, hipStream_t stream)
 
 // ------------------------------------------------------------------------------------------------------ gradients
 
+// Sums over the threads of `R` rows at once, as row_reduce.
+template <int THREADS, int R>
+__device__ __forceinline__ void rows_reduce(float (&sum)[R], float (*shared)[R][16], int slot)
+{
+#pragma unroll
+    for (int k = 0; k < R; k++) {
+        sum[k] = wave_sum(sum[k]);
+    }
+    if constexpr (THREADS > 64) {
+        const int wave = (int)threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+            for (int k = 0; k < R; k++) {
+                shared[slot][k][wave] = sum[k];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < R; k++) {
+            sum[k] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < THREADS / 64; i++) {
+                sum[k] += shared[slot][k][i];
+            }
+        }
+    }
+}
+
 // Gradient of the rows, and of the weight's columns over the rows of one workgroup, which it adds up in registers and
-// leaves in its row of `partial`.  THREADS per row; wavefronts of 64-thread rows join their sums through LDS.
-template <typename T, typename W, int THREADS, int NV, int VEC, bool WIDE, bool WEIGHT>
+// leaves in its row of `partial`.  THREADS per row; wavefronts of 64-thread rows join their sums through LDS.  R rows at a
+// time, as many as a thread's registers hold, so that enough loads are under way with two workgroups a CU (more of them
+// would write more partial sums): 16384 rows of 2048 bf16 74 us with one row, 68 with four.
+template <typename T, typename W, int THREADS, int NV, int VEC, bool WIDE, bool WEIGHT, int R>
 __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void norm_grad_kernel(NormGradArgs a)
 {
-    constexpr int kRows = THREADS >= 256 ? 1 : 256 / THREADS;
-    __shared__ float shared[2][2][16];
+    constexpr int kGroups = THREADS >= 256 ? 1 : 256 / THREADS;
+    __shared__ float shared[2][R][16];
     const int lane = (int)threadIdx.x % THREADS;
     float w[NV][VEC], total[NV][VEC];
 #pragma unroll
@@ -290,71 +320,94 @@ __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void norm_grad_kerne
         }
     }
     int slot = 0;
-    // every thread of a workgroup makes as many turns: the barrier of row_reduce is met by all (THREADS >= 256: one row
-    // a turn; 64: no barrier)
-    for (int64_t row = (int64_t)blockIdx.x * kRows + (int)threadIdx.x / THREADS; row < a.rows;
-         row += (int64_t)gridDim.x * kRows) {
-        const float rstd = a.rstd[row];
-        float n[NV][VEC], g[NV][VEC], along = 0.0f;
+    // every thread of a workgroup makes as many turns: the barrier of rows_reduce is met by all (THREADS >= 256: the same
+    // rows; 64: no barrier)
+    for (int64_t row0 = ((int64_t)blockIdx.x * kGroups + (int)threadIdx.x / THREADS) * R; row0 < a.rows;
+         row0 += (int64_t)gridDim.x * kGroups * R) {
+        float n[R][NV][VEC], g[R][NV][VEC], rstd[R], along[R];
 #pragma unroll
-        for (int j = 0; j < NV; j++) {
-            const int64_t c = ((int64_t)j * THREADS + lane) * VEC;
-            if (c < a.width) {
-                load_part<T, VEC, WIDE>((const T*)a.sum.ptr + row * a.sum.row_stride, c, a.width, n[j]);
-                load_part<T, VEC, WIDE>((const T*)a.grad_y.ptr + row * a.grad_y.row_stride, c, a.width, g[j]);
-            } else {
+        for (int k = 0; k < R; k++) {
+            const int64_t row = row0 + k;
+            const bool live = row < a.rows;
+            rstd[k] = live ? a.rstd[row] : 0.0f;
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                const int64_t c = ((int64_t)j * THREADS + lane) * VEC;
+                if (live && c < a.width) {
+                    load_part<T, VEC, WIDE>((const T*)a.sum.ptr + row * a.sum.row_stride, c, a.width, n[k][j]);
+                    load_part<T, VEC, WIDE>((const T*)a.grad_y.ptr + row * a.grad_y.row_stride, c, a.width, g[k][j]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) {
+                        n[k][j][i] = g[k][j][i] = 0.0f;
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < R; k++) {
+            along[k] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
 #pragma unroll
                 for (int i = 0; i < VEC; i++) {
-                    n[j][i] = g[j][i] = 0.0f;
+                    n[k][j][i] *= rstd[k];
+                    if (WEIGHT) {
+                        total[j][i] += g[k][j][i] * n[k][j][i];
+                    }
+                    g[k][j][i] *= w[j][i];
+                    along[k] += g[k][j][i] * n[k][j][i];
                 }
             }
         }
-#pragma unroll
-        for (int j = 0; j < NV; j++) {
-#pragma unroll
-            for (int i = 0; i < VEC; i++) {
-                n[j][i] *= rstd;
-                if (WEIGHT) {
-                    total[j][i] += g[j][i] * n[j][i];
-                }
-                g[j][i] *= w[j][i];
-                along += g[j][i] * n[j][i];
-            }
-        }
-        row_reduce<THREADS>(along, nullptr, shared, slot);
+        rows_reduce<THREADS, R>(along, shared, slot);
         slot ^= 1;
-        along /= (float)a.width;
 #pragma unroll
-        for (int j = 0; j < NV; j++) {
-            const int64_t c = ((int64_t)j * THREADS + lane) * VEC;
-            if (c < a.width) {
-                float s[VEC] = {0.0f};
-                if (a.grad_sum.ptr != nullptr) {
-                    load_part<T, VEC, WIDE>((const T*)a.grad_sum.ptr + row * a.grad_sum.row_stride, c, a.width, s);
-                }
+        for (int k = 0; k < R; k++) {
+            const int64_t row = row0 + k;
+            if (row >= a.rows) {
+                break;
+            }
+            const float mean = along[k] / (float)a.width;
 #pragma unroll
-                for (int i = 0; i < VEC; i++) {
-                    s[i] += (g[j][i] - n[j][i] * along) * rstd;
+            for (int j = 0; j < NV; j++) {
+                const int64_t c = ((int64_t)j * THREADS + lane) * VEC;
+                if (c < a.width) {
+                    float s[VEC] = {0.0f};
+                    if (a.grad_sum.ptr != nullptr) {
+                        load_part<T, VEC, WIDE>((const T*)a.grad_sum.ptr + row * a.grad_sum.row_stride, c, a.width, s);
+                    }
+#pragma unroll
+                    for (int i = 0; i < VEC; i++) {
+                        s[i] += (g[k][j][i] - n[k][j][i] * mean) * rstd[k];
+                    }
+                    store_part<T, VEC, WIDE>((T*)a.grad_x.ptr + row * a.grad_x.row_stride, c, a.width, s, false);
                 }
-                store_part<T, VEC, WIDE>((T*)a.grad_x.ptr + row * a.grad_x.row_stride, c, a.width, s);
             }
         }
     }
     if constexpr (WEIGHT) {
-        __shared__ float joined[kRows > 1 ? THREADS * VEC : 1];
-        float* const out = a.partial + (int64_t)blockIdx.x * a.width;
+        // the one workgroup of few rows writes the gradient itself
+        __shared__ float joined[kGroups > 1 ? THREADS * VEC : 1];
+        const auto put = [&](int64_t c, float x) {
+            if (gridDim.x == 1) {
+                ((W*)a.grad_weight)[c] = (W)x;
+            } else {
+                a.partial[(int64_t)blockIdx.x * a.width + c] = x;
+            }
+        };
 #pragma unroll
         for (int j = 0; j < NV; j++) {
             const int64_t c = ((int64_t)j * THREADS + lane) * VEC;
-            if constexpr (kRows > 1) {
-                for (int turn = 0; turn < kRows; turn++) {  // the wavefronts add in order
+            if constexpr (kGroups > 1) {
+                for (int turn = 0; turn < kGroups; turn++) {  // the wavefronts add in order
                     if ((int)threadIdx.x / THREADS == turn) {
 #pragma unroll
                         for (int i = 0; i < VEC; i++) {
                             float& slot_sum = joined[i * THREADS + lane];
                             slot_sum = turn == 0 ? total[j][i] : slot_sum + total[j][i];
-                            if (turn == kRows - 1 && c + i < a.width) {
-                                out[c + i] = slot_sum;
+                            if (turn == kGroups - 1 && c + i < a.width) {
+                                put(c + i, slot_sum);
                             }
                         }
                     }
@@ -364,7 +417,7 @@ __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void norm_grad_kerne
 #pragma unroll
                 for (int i = 0; i < VEC; i++) {
                     if (c + i < a.width) {
-                        out[c + i] = total[j][i];
+                        put(c + i, total[j][i]);
                     }
                 }
             }
@@ -409,7 +462,7 @@ __global__ __launch_bounds__(1024) void norm_grad_long_kernel(NormGradArgs a)
         for (int i = 0; i < VEC; i++) {
             s[i] += (g[i] * w[i] - n[i] * rstd * along) * rstd;
         }
-        store_part<T, VEC, WIDE>((T*)a.grad_x.ptr + row * a.grad_x.row_stride, c, a.width, s);
+        store_part<T, VEC, WIDE>((T*)a.grad_x.ptr + row * a.grad_x.row_stride, c, a.width, s, false);
     }
     }
 }
@@ -457,14 +510,17 @@ __global__ __launch_bounds__(256) void norm_weight_kernel(const float* __restric
 }
 
 template <typename T, typename W, int THREADS, int NV, int VEC, bool WIDE>
-void launch_norm_grad(const NormGradArgs& a, int64_t blocks, hipStream_t stream)
+void launch_norm_grad(const NormGradArgs& a, hipStream_t stream)
 {
+    constexpr int kThreads = THREADS > 256 ? THREADS : 256;
+    constexpr int kRowsATime = THREADS > 256 ? 1 : kMostPerLane / (NV * VEC);
+    constexpr int64_t kRowsABlock = (THREADS >= 256 ? 1 : 256 / THREADS) * kRowsATime;
     if (a.grad_weight != nullptr) {
-        hipLaunchKernelGGL((norm_grad_kernel<T, W, THREADS, NV, VEC, WIDE, true>), dim3((unsigned)blocks),
-                           dim3(THREADS > 256 ? THREADS : 256), 0, stream, a);
+        hipLaunchKernelGGL((norm_grad_kernel<T, W, THREADS, NV, VEC, WIDE, true, kRowsATime>),
+                           dim3((unsigned)norm_grad_partials(a)), dim3(kThreads), 0, stream, a);
     } else {
-        hipLaunchKernelGGL((norm_grad_kernel<T, W, THREADS, NV, VEC, WIDE, false>), dim3((unsigned)blocks),
-                           dim3(THREADS > 256 ? THREADS : 256), 0, stream, a);
+        hipLaunchKernelGGL((norm_grad_kernel<T, W, THREADS, NV, VEC, WIDE, false, kRowsATime>),
+                           grid((a.rows + kRowsABlock - 1) / kRowsABlock), dim3(kThreads), 0, stream, a);
     }
 }
 
@@ -472,32 +528,29 @@ template <typename T, typename W, int VEC, bool WIDE>
 hipError_t run_norm_grad(const NormGradArgs& a, hipStream_t stream)
 {
     constexpr int kVectors = kMostPerLane / VEC;
-    const int64_t vectors = (a.width + VEC - 1) / VEC;
-    const int64_t partials = norm_grad_partials(a);
-    const auto blocks = [&](int64_t rows_each) {
-        const int64_t most = (a.rows + rows_each - 1) / rows_each;
-        return a.grad_weight != nullptr ? partials : (most < kMostBlocks ? most : kMostBlocks);
-    };
-    if (a.rows > 0 || a.grad_weight != nullptr) {
-        if (vectors <= 64 * kVectors / 2) {
-            launch_norm_grad<T, W, 64, kVectors / 2, VEC, WIDE>(a, blocks(4), stream);
-        } else if (vectors <= 256 * kVectors / 2) {
-            launch_norm_grad<T, W, 256, kVectors / 2, VEC, WIDE>(a, blocks(1), stream);
-        } else if (vectors <= 256 * kVectors) {
-            launch_norm_grad<T, W, 256, kVectors, VEC, WIDE>(a, blocks(1), stream);
-        } else if (vectors <= 1024 * kVectors) {
-            launch_norm_grad<T, W, 1024, kVectors, VEC, WIDE>(a, blocks(1), stream);
-        } else {
-            if (a.grad_weight != nullptr) {
-                hipLaunchKernelGGL((norm_weight_long_kernel<T>), dim3((unsigned)((a.width + 255) / 256), (unsigned)partials),
-                                   dim3(256), 0, stream, a);
-            }
-            if (a.rows > 0) {
-                hipLaunchKernelGGL((norm_grad_long_kernel<T, W, VEC, WIDE>), grid(a.rows), dim3(1024), 0, stream, a);
-            }
+    const int64_t vectors = (a.width + VEC - 1) / VEC, partials = norm_grad_partials(a);
+    bool joined = partials == 1;  // the kernel of short rows writes a single partial sum where it belongs
+    if (vectors <= 64 * kVectors / 2) {
+        launch_norm_grad<T, W, 64, kVectors / 2, VEC, WIDE>(a, stream);
+    } else if (vectors <= 256 * kVectors / 4) {
+        launch_norm_grad<T, W, 256, kVectors / 4, VEC, WIDE>(a, stream);
+    } else if (vectors <= 256 * kVectors / 2) {
+        launch_norm_grad<T, W, 256, kVectors / 2, VEC, WIDE>(a, stream);
+    } else if (vectors <= 256 * kVectors) {
+        launch_norm_grad<T, W, 256, kVectors, VEC, WIDE>(a, stream);
+    } else if (vectors <= 1024 * kVectors) {
+        launch_norm_grad<T, W, 1024, kVectors, VEC, WIDE>(a, stream);
+    } else {
+        joined = false;
+        if (a.grad_weight != nullptr) {
+            hipLaunchKernelGGL((norm_weight_long_kernel<T>), dim3((unsigned)((a.width + 255) / 256), (unsigned)partials),
+                               dim3(256), 0, stream, a);
+        }
+        if (a.rows > 0) {
+            hipLaunchKernelGGL((norm_grad_long_kernel<T, W, VEC, WIDE>), grid(a.rows), dim3(1024), 0, stream, a);
         }
     }
-    if (a.grad_weight != nullptr) {
+    if (a.grad_weight != nullptr && !joined) {
         hipLaunchKernelGGL((norm_weight_kernel<W>), dim3((unsigned)((a.width + 31) / 32)), dim3(256), 0, stream, a.partial,
                            partials, a.width, (W*)a.grad_weight);
     }
@@ -532,16 +585,18 @@ hipError_t by_type(int elem, int weight_float, F&& f)
 
 int64_t norm_grad_partials(const NormGradArgs& a)
 {
-    // a workgroup takes four rows at a time at most; one row of partial sums even where there are no rows
-    const int64_t groups = (a.rows + 3) / 4;
+    // a workgroup takes up to eight rows at a time; one row of partial sums even where there are no rows
+    const int64_t groups = (a.rows + 7) / 8;
     return groups < 1 ? 1 : (groups < kPartialRows ? groups : kPartialRows);
 }
 
-hipError_t launch_residual_norm(const NormArgs& a, hipStream_t stream)
+hipError_t launch_residual_norm(const NormArgs& args, hipStream_t stream)
 {
-    if (a.rows < 1 || a.width < 1) {
+    if (args.rows < 1 || args.width < 1) {
         return hipErrorInvalidValue;
     }
+    NormArgs a = args;
+    a.streaming = a.rows * a.width * elem_size((Elem)a.elem) >= kStreamBytes ? 1 : 0;
     return by_type(a.elem, a.weight_float, [&](auto* t, auto* w) {
         return run_norm_type<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(w)>>(a, stream);
     });

@@ -68,6 +68,8 @@ struct RotaryPlan {
     RotaryArgs a;
     FastDiv units, groups, tokens;  // units of a head, groups of heads, tokens of a sequence
     uint32_t turned;                // units that turn; the others copy
+    int wide_table;                 // the table's rows start on 16 bytes
+    int streaming;
     uint32_t total;                 // threads with work
 };
 
@@ -104,10 +106,34 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryPlan p)
         const int64_t at = a.position.ptr != nullptr ? whole_at(a.position, b, t) : (int64_t)t;
         if (at >= 0 && at < a.positions) {
             const float* const row = a.table + at * a.table_stride + pair;
+            bool read = false;
+            if constexpr (kPairs % 4 == 0) {
+                if (p.wide_table != 0) {
+                    read = true;
 #pragma unroll
-            for (int i = 0; i < kPairs; i++) {
-                cosine[i] = row[i];
-                sine[i] = a.inverse != 0 ? -row[half + i] : row[half + i];
+                    for (int i = 0; i < kPairs; i += 4) {
+                        const Pack<float, 4> x = *reinterpret_cast<const Pack<float, 4>*>(row + i);
+                        const Pack<float, 4> y = *reinterpret_cast<const Pack<float, 4>*>(row + half + i);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            cosine[i + e] = x.v[e];
+                            sine[i + e] = y.v[e];
+                        }
+                    }
+                }
+            }
+            if (!read) {
+#pragma unroll
+                for (int i = 0; i < kPairs; i++) {
+                    cosine[i] = row[i];
+                    sine[i] = row[half + i];
+                }
+            }
+            if (a.inverse != 0) {
+#pragma unroll
+                for (int i = 0; i < kPairs; i++) {
+                    sine[i] = -sine[i];
+                }
             }
         } else {
 #pragma unroll
@@ -153,10 +179,10 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryPlan p)
                 u = s;
             }
             if (!INTERLEAVED) {
-                store<T, VEC>(to[i] + second, y[i]);
+                store<T, VEC>(to[i] + second, y[i], p.streaming != 0);
             }
         }
-        store<T, VEC>(to[i] + first, x[i]);
+        store<T, VEC>(to[i] + first, x[i], p.streaming != 0);
     }
 }
 
@@ -203,6 +229,8 @@ hipError_t run(const RotaryArgs& a, hipStream_t stream)
             p.groups = make_fast_div((uint32_t)groups);
             p.tokens = make_fast_div((uint32_t)p.a.tokens);
             p.turned = (uint32_t)turned;
+            p.streaming = tokens * heads * a.d * (int64_t)sizeof(T) >= kStreamBytes ? 1 : 0;
+            p.wide_table = aligned(p.a.table, a.table_stride, 4, 16) && a.rot / 2 % 4 == 0 ? 1 : 0;
             p.total = (uint32_t)(p.a.batch * p.a.tokens * per_token);
             const dim3 grid((p.total + kThreads - 1) / kThreads);
             if (each == 8) {

@@ -28,6 +28,7 @@ struct NormArgs {
     int elem = 0;         // Elem of x, residual, sum and y
     int weight_float = 0;  // weight (and its gradient) in FLOAT where elem is another type
     int int8 = 0;         // y in 8 bits, with scale
+    int streaming = 0;    // set by the launcher
     int64_t rows = 0, width = 0;
     float eps = 0.0f;
     Rows x, residual, y, sum;  // residual and sum: ptr may be null
