@@ -126,7 +126,8 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
     if (block_high < block_low) {
         range.tiles = 0;
     }
-    const int wave_low = seq.first + query_of(wave_row0), wave_high = seq.first + query_of(wave_row0 + kBlock - 1);
+    const int wave_low = seq.first + query_of(wave_row0);
+    const int wave_high = seq.first + min(query_of(wave_row0 + kBlock - 1), seq.q_len - 1);
     const bool wave_whole = query_of(wave_row0 + kBlock - 1) < seq.q_len;
 
     const T* const k_base = (const T*)a.k.ptr + (int64_t)b * a.k.stride[0] + (int64_t)kv_head * a.k.stride[2];
@@ -171,11 +172,55 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
     const float lse = stat[0], along = stat[a.tokens];
     const float unit = kUnits ? stat[2 * a.tokens] : 1.0f, per_unit = unit > 0.0f ? 1.0f / unit : 0.0f;
     wait_for_registers();
-    const Rows32<T, kPitch, NB> rows(lane);
-    const Columns32<T, kPitch, NB> columns(lane);
-    for (int t = key_wave; t < range.tiles; t += kJoin) {
+    // as in the forward pass: 32 keys of a tile, those of tiles that all of the wavefront's rows see whole in a loop of their own
+    const auto whole = [&](int t) {
+        const int key0 = range.key_of(t, kKeys);
+        return wave_whole && key0 + kKeys <= range.end_of(t) && key0 + kKeys - 1 <= wave_low + right &&
+               (key0 >= wave_high - left || key0 + kKeys <= sinks);
+    };
+    const auto unseen = [&](int key0, int end) {
+        return wave_low > wave_high || key0 >= end || key0 > wave_high + right ||
+               (key0 + kBlock - 1 < wave_low - left && key0 >= sinks);
+    };
+    const auto attend = [&](auto part, int key0, int end, const T* k_tile, const T* v_tile, const Rows32<T, kPitch, NB>& rows,
+                            const Columns32<T, kPitch, NB>& columns) {
+        acc_t s = zeros(), dp = zeros();
+#pragma unroll
+        for (int i = 0; i < 2 * NB; i++) {
+            s = Mma<T>::mul(rows(k_tile, 0, i), q[i], s);
+            dp = Mma<T>::mul(rows(v_tile, 0, i), go[i], dp);
+        }
+        if constexpr (sizeof(T) == 2) {
+            read_ahead<4 * NB, 1, 4>();
+        }
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -lse)) * ((dp[r] - along) * per_unit);
+        }
+        if constexpr (decltype(part)::value) {
+            const Sight see = sight(pos, key0 + 4 * h, end, left, right, sinks);
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                s[r] = see.sees(8 * (r / 4) + r % 4) ? s[r] : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+            const Frag<T> w = operand<T>(s, g);
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+                gq[i] = Mma<T>::mul(columns(k_tile, 16 * g, i), w, gq[i]);
+            }
+        }
+        if constexpr (sizeof(T) == 2) {
+            read_ahead<2 * NB, 2, 3>();
+        }
+    };
+    int t = key_wave;
+    const auto work = [&](auto part, const Rows32<T, kPitch, NB>& rows, const Columns32<T, kPitch, NB>& columns) {
+        constexpr bool PART = decltype(part)::value;
         const bool more = t + kJoin < range.tiles;
-        if constexpr (kJoin == 1) {  // as in the forward pass
+        if constexpr (kJoin == 1) {
             wait_for_loads<0>();
             barrier();
             if (kShape.stages == 2 && more) {
@@ -192,40 +237,17 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
         const T* const k_tile = ring + buffer * (2 * kKeys * kPitch);
         const T* const v_tile = k_tile + kKeys * kPitch;
         const int key0 = range.key_of(t, kKeys), end = range.end_of(t);
-        const bool all_seen = wave_whole && key0 + kKeys <= end && key0 + kKeys - 1 <= wave_low + right &&
-                              (key0 >= wave_high - left || key0 + kKeys <= sinks);
-#pragma unroll
-        for (int j = 0; j < kSubs; j++) {
-            acc_t s = zeros(), dp = zeros();
-#pragma unroll
-            for (int i = 0; i < 2 * NB; i++) {
-                s = Mma<T>::mul(rows(k_tile, j * kBlock, i), q[i], s);
-                dp = Mma<T>::mul(rows(v_tile, j * kBlock, i), go[i], dp);
-            }
-            if constexpr (sizeof(T) == 2) {
-                read_ahead<4 * NB, 1, 4>();
-            }
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -lse)) * ((dp[r] - along) * per_unit);
-            }
-            if (__builtin_expect(!all_seen, 0)) {
-                const Sight see = sight(pos, key0 + j * kBlock + 4 * h, end, left, right, sinks);
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    s[r] = see.sees(8 * (r / 4) + r % 4) ? s[r] : 0.0f;
+        if constexpr (PART) {
+#pragma unroll 1
+            for (int j = 0; j < kKeys; j += kBlock) {
+                if (!unseen(key0 + j, end)) {
+                    attend(part, key0 + j, end, k_tile + j * kPitch, v_tile + j * kPitch, rows, columns);
                 }
             }
+        } else {
 #pragma unroll
-            for (int g = 0; g < 2; g++) {
-                const Frag<T> w = operand<T>(s, g);
-#pragma unroll
-                for (int i = 0; i < NB; i++) {
-                    gq[i] = Mma<T>::mul(columns(k_tile, j * kBlock + 16 * g, i), w, gq[i]);
-                }
-            }
-            if constexpr (sizeof(T) == 2) {
-                read_ahead<2 * NB, 2, 3>();
+            for (int j = 0; j < kKeys; j += kBlock) {
+                attend(part, key0 + j, end, k_tile + j * kPitch, v_tile + j * kPitch, rows, columns);
             }
         }
         if (kShape.stages == 1 && more) {
@@ -237,6 +259,21 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
             fetch(t + kJoin, 0);
         }
         buffer ^= kShape.stages - 1;
+        t += kJoin;
+    };
+    while (t < range.tiles) {
+        {
+            const Rows32<T, kPitch, NB> rows(again(lane));
+            const Columns32<T, kPitch, NB> columns(again(lane));
+            while (t < range.tiles && !whole(t)) {
+                work(std::true_type(), rows, columns);
+            }
+        }
+        const Rows32<T, kPitch, NB> rows(again(lane));
+        const Columns32<T, kPitch, NB> columns(again(lane));
+        while (t < range.tiles && whole(t)) {
+            work(std::false_type(), rows, columns);
+        }
     }
     if constexpr (kJoin > 1) {
         // sums of the wavefronts that shared the keys, [feature][row]; every one adds up a share of the features

@@ -106,8 +106,9 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
     if (block_high < block_low) {
         range.tiles = 0;
     }
-    const int block_first = seq.first + block_low, block_last = seq.first + block_high;
-    const bool rows_whole = query_of(row0 + kShape.rows() - 1) < seq.q_len;
+    const int wave_first = seq.first + query_of(wave_row0);
+    const bool rows_whole = query_of(wave_row0 + kBlock - 1) < seq.q_len;
+    const int wave_last = seq.first + min(query_of(wave_row0 + kBlock - 1), seq.q_len - 1);
     const int t_begin = (int)((int64_t)range.tiles * split / p.splits);
     const int t_end = (int)((int64_t)range.tiles * (split + 1) / p.splits);
 
@@ -150,11 +151,100 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
     }
     wait_for_registers();
     bool careful = false;  // a second pass, for values that are not finite
-    // whether all rows of the workgroup see all keys of a tile
+    // whether all rows of the wavefront see all keys of a tile, and whether none of them sees any of 32 keys: wavefronts of a
+    // workgroup meet once a tile, but each spends on it what its own rows see of it
     const auto whole = [&](int tile_index) {
         const int key0 = range.key_of(tile_index, kKeys);
-        return rows_whole && key0 + kKeys <= range.end_of(tile_index) && key0 + kKeys - 1 <= block_first + right &&
-               (key0 >= block_last - left || key0 + kKeys <= sinks);
+        return rows_whole && key0 + kKeys <= range.end_of(tile_index) && key0 + kKeys - 1 <= wave_first + right &&
+               (key0 >= wave_last - left || key0 + kKeys <= sinks);
+    };
+    const auto unseen = [&](int key0, int end) {
+        return wave_first > wave_last || key0 >= end || key0 > wave_last + right ||
+               (key0 + kBlock - 1 < wave_first - left && key0 >= sinks);
+    };
+    // SUBS times 32 keys of a tile; PART: some rows may not see some of them
+    const auto attend = [&](auto part, auto subs, int key0, int end, const T* k_tile, const T* v_tile,
+                            const Rows32<T, kPitch, NB>& k_rows, const Columns32<T, kPitch, NB>& v_columns) {
+        constexpr bool PART = decltype(part)::value;
+        constexpr int SUBS = decltype(subs)::value;
+        acc_t s[SUBS];
+#pragma unroll
+        for (int j = 0; j < SUBS; j++) {
+            s[j] = zeros();
+#pragma unroll
+            for (int i = 0; i < 2 * NB; i++) {
+                s[j] = Mma<T>::mul(k_rows(k_tile, j * kBlock, i), q[i], s[j]);
+            }
+        }
+        if constexpr (sizeof(T) == 2) {
+            read_ahead<2 * NB * SUBS, 1, 4>();
+        }
+        if constexpr (PART) {
+            const Sight see = sight(pos, key0 + 4 * h, end, left, right, sinks);
+#pragma unroll
+            for (int j = 0; j < SUBS; j++) {
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    s[j][r] = see.sees(j * kBlock + 8 * (r / 4) + r % 4) ? s[j][r] : -INFINITY;
+                }
+            }
+        }
+        float highs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four chains: one would wait for itself
+#pragma unroll
+        for (int j = 0; j < SUBS; j++) {
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+                highs[r / 2 % 4] = largest(highs[r / 2 % 4], s[j][r], s[j][r + 1]);
+            }
+        }
+        const float high = larger_of_halves(largest(highs[0], highs[1], largest(highs[2], highs[3], highs[3]))) * c;
+        const bool grows = !(high <= base + kSlack);
+        if (__any(grows)) {
+            // each row by its own scores alone: what it sees beside it does not change its result
+            const float now = grows ? __builtin_elementwise_maximum(base, high) : base;
+            const float fade = base == -INFINITY ? 0.0f : exp2f(base - now);
+            total *= fade;
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    o[i][r] *= fade;
+                }
+            }
+            base = now;
+        }
+        const float from = base == -INFINITY ? 0.0f : base;  // exp2(-inf - 0) = 0
+        Frag<T> w[2 * SUBS];
+        float sums[4] = {total, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int n = 0; n < 2 * SUBS; n++) {
+            acc_t& x = s[n / 2];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int r = 8 * (n % 2) + e;
+                x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], c, -from));
+                sums[e % 4] += x[r];
+            }
+            w[n] = operand<T>(x, n % 2);
+        }
+        total = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        if (PART && __builtin_expect(careful, 0)) {
+#pragma unroll
+            for (int i = 0; i < NB; i++) {
+                o[i] = add_seen_values<T, kPitch, SUBS>(o[i], w, v_tile, i, again(lane));
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < 2 * SUBS; n++) {
+#pragma unroll
+                for (int i = 0; i < NB; i++) {
+                    o[i] = Mma<T>::mul(v_columns(v_tile, 16 * n, i), w[n], o[i]);
+                }
+            }
+            if constexpr (sizeof(T) == 2) {
+                read_ahead<2 * NB * SUBS, 2, 3>();
+            }
+        }
     };
     // one tile; PART: some rows may not see some keys
     const auto work = [&](auto part, const Rows32<T, kPitch, NB>& k_rows, const Columns32<T, kPitch, NB>& v_columns) {
@@ -179,84 +269,17 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
         }
         const T* const k_tile = ring + buffer * (2 * kKeys * kPitch);
         const T* const v_tile = k_tile + kKeys * kPitch;
-
-        acc_t s[kSubs];
-#pragma unroll
-        for (int j = 0; j < kSubs; j++) {
-            s[j] = zeros();
-#pragma unroll
-            for (int i = 0; i < 2 * NB; i++) {
-                s[j] = Mma<T>::mul(k_rows(k_tile, j * kBlock, i), q[i], s[j]);
-            }
-        }
-        if constexpr (sizeof(T) == 2) {
-            read_ahead<2 * NB * kSubs, 1, 4>();
-        }
+        const int key0 = range.key_of(t, kKeys), end = range.end_of(t);
         if constexpr (PART) {
-            const Sight see = sight(pos, range.key_of(t, kKeys) + 4 * h, range.end_of(t), left, right, sinks);
-#pragma unroll
-            for (int j = 0; j < kSubs; j++) {
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    s[j][r] = see.sees(j * kBlock + 8 * (r / 4) + r % 4) ? s[j][r] : -INFINITY;
+#pragma unroll 1
+            for (int j = 0; j < kKeys; j += kBlock) {
+                if (!unseen(key0 + j, end)) {
+                    attend(part, std::integral_constant<int, 1>(), key0 + j, end, k_tile + j * kPitch, v_tile + j * kPitch, k_rows,
+                           v_columns);
                 }
-            }
-        }
-        float highs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // four chains: one would wait for itself
-#pragma unroll
-        for (int j = 0; j < kSubs; j++) {
-#pragma unroll
-            for (int r = 0; r < 16; r += 2) {
-                highs[r / 2 % 4] = largest(highs[r / 2 % 4], s[j][r], s[j][r + 1]);
-            }
-        }
-        const float high = larger_of_halves(largest(highs[0], highs[1], largest(highs[2], highs[3], highs[3]))) * c;
-        const bool grows = !(high <= base + kSlack);
-        if (__any(grows)) {
-            // each row by its own scores alone: what it sees beside it does not change its result
-            const float now = grows ? __builtin_elementwise_maximum(base, high) : base;
-            const float fade = base == -INFINITY ? 0.0f : exp2f(base - now);
-            total *= fade;
-#pragma unroll
-            for (int i = 0; i < NB; i++) {
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    o[i][r] *= fade;
-                }
-            }
-            base = now;
-        }
-        const float from = base == -INFINITY ? 0.0f : base;  // exp2(-inf - 0) = 0
-        Frag<T> w[2 * kSubs];
-        float sums[4] = {total, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int n = 0; n < 2 * kSubs; n++) {
-            acc_t& x = s[n / 2];
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int r = 8 * (n % 2) + e;
-                x[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], c, -from));
-                sums[e % 4] += x[r];
-            }
-            w[n] = operand<T>(x, n % 2);
-        }
-        total = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-        if (PART && __builtin_expect(careful, 0)) {
-#pragma unroll
-            for (int i = 0; i < NB; i++) {
-                o[i] = add_seen_values<T, kPitch, kSubs>(o[i], w, v_tile, i, again(lane));
             }
         } else {
-#pragma unroll
-            for (int n = 0; n < 2 * kSubs; n++) {
-#pragma unroll
-                for (int i = 0; i < NB; i++) {
-                    o[i] = Mma<T>::mul(v_columns(v_tile, 16 * n, i), w[n], o[i]);
-                }
-            }
-            if constexpr (sizeof(T) == 2) {
-                read_ahead<2 * NB * kSubs, 2, 3>();
-            }
+            attend(part, std::integral_constant<int, kSubs>(), key0, end, k_tile, v_tile, k_rows, v_columns);
         }
         if (kShape.stages == 1 && more) {
             if constexpr (kShape.row_waves > 1) {
