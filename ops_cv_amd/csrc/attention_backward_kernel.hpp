@@ -1,9 +1,8 @@
-// Gradients of attention, in three kernels and a join:
+// Gradients of attention, in two kernels and a join:
 //
-//   statistics  per row i: lse_i log2 e (infinity where the row sees nothing), D_i = sum gO_i O_i, and for FLOAT16 a power
-//               of two near the largest |gO_i|
 //   queries     as the forward pass walks keys:  P' = exp2(K Q' c - lse),  dP' = V gO',  dS' = P' (dP' - D),
-//               gQ' += K' dS'
+//               gQ' += K' dS'.  Before that every row i's statistics, which the next kernel reads too: lse_i log2 e (infinity
+//               where the row sees nothing), D_i = sum gO_i O_i, and for FLOAT16 a power of two near the largest |gO_i|
 //   keys        a wavefront keeps 32 keys and walks the queries that see them:  P, dS as above with rows and columns
 //               exchanged,  gV' += gO' P,  gK' += Q' dS
 //   join        where the queries of a tile of keys were cut into parts, their 32-bit sums in order
@@ -33,7 +32,6 @@ struct GradLaunch {
     FastDiv group;
     uint32_t rows, tiles, kv_heads;
     uint32_t keys, key_tiles, sink_tiles, sink_parts, parts;
-    int32_t each;  // steps of a part; the last one has the rest
     uint32_t query_blocks, key_blocks;
     float* stats;          // (batch, heads, 3, tokens)
     float* sink_partials;  // (batch * kv_heads, sink_tiles, sink_parts, 2, keys, d rounded up to four)
@@ -45,51 +43,6 @@ static __device__ __forceinline__ int64_t stats_row(const AttentionArgs& a, int6
     return (b * a.heads + head) * 3 * a.tokens;
 }
 
-// Statistics of the rows: sixteen lanes a row.
-template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void attention_stats_kernel(GradLaunch p, uint32_t rows)
-{
-    const AttentionArgs& a = p.a;
-    const uint32_t row = (blockIdx.x * 256u + threadIdx.x) / 16;
-    const int lane = (int)threadIdx.x & 15, d = (int)a.d;
-    if (row >= rows) {
-        return;  // sixteen lanes together
-    }
-    // heads fastest: neighbouring rows lie side by side where heads do
-    const uint32_t head = row % (uint32_t)a.heads, rest = row / (uint32_t)a.heads;
-    const uint32_t token = rest % (uint32_t)a.tokens, b = rest / (uint32_t)a.tokens;
-    const T* const go = (const T*)a.grad_out.ptr + (int64_t)b * a.grad_out.stride[0] +
-                        (int64_t)token * a.grad_out.stride[1] + (int64_t)head * a.grad_out.stride[2];
-    const T* const o = (const T*)a.out.ptr + (int64_t)b * a.out.stride[0] + (int64_t)token * a.out.stride[1] +
-                       (int64_t)head * a.out.stride[2];
-    float sum = 0.0f, most = 0.0f;
-    for (int c = lane * 8; c < d; c += 128) {
-        const Frag<T> x = global_row<T, VEC>(go, c, d), y = global_row<T, VEC>(o, c, d);
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            sum += (float)x[e] * (float)y[e];
-            most = fmaxf(most, fabsf((float)x[e]));
-        }
-    }
-#pragma unroll
-    for (int w = 8; w > 0; w >>= 1) {
-        sum += __shfl_xor(sum, w, 64);
-        most = fmaxf(most, __shfl_xor(most, w, 64));
-    }
-    if (lane == 0) {
-        const Sequence seq = sequence_at(a, b);
-        const float lse = ((const float*)a.lse.ptr)[(int64_t)b * a.lse.stride[0] + (int64_t)head * a.lse.stride[1] +
-                                                    (int64_t)token * a.lse.stride[2]];
-        const bool live = (int)token < seq.q_len && lse != -INFINITY;
-        float* const to = p.stats + stats_row(a, b, head) + token;
-        to[0] = live ? lse * kLog2e : INFINITY;
-        to[a.tokens] = live ? sum : 0.0f;
-        // 2^floor(log2 most) by its exponent bits; 0 for rows of zeros
-        const uint32_t bits = __float_as_uint(most) & 0x7f800000u;
-        to[2 * a.tokens] = !live ? 0.0f : (bits == 0x7f800000u ? 1.0f : __uint_as_float(bits));
-    }
-}
-
 // ---------------------------------------------------------------------------------------------------- queries' gradients
 
 template <typename T, int NB, bool FEW, bool VEC>
@@ -98,7 +51,7 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
 {
     constexpr int kPitch = pitch_of(NB);
     constexpr ForwardShape kShape = forward_shape(sizeof(T), kPitch, FEW);
-    constexpr int kKeys = kShape.keys, kSubs = kKeys / kBlock, kThreads = 64 * kShape.row_waves, kJoin = kShape.key_waves;
+    constexpr int kKeys = kShape.keys, kThreads = 64 * kShape.row_waves, kJoin = kShape.key_waves;
     constexpr bool kUnits = std::is_same<T, _Float16>::value;
     extern __shared__ __align__(16) char lds[];
 
@@ -168,9 +121,44 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
             go[i] = global_row<T, VEC>(gsrc, 16 * i + 8 * h, d);
         }
     }
-    const float* const stat = p.stats + stats_row(a, b, head) + query;
-    const float lse = stat[0], along = stat[a.tokens];
-    const float unit = kUnits ? stat[2 * a.tokens] : 1.0f, per_unit = unit > 0.0f ? 1.0f / unit : 0.0f;
+    // the row's statistics, left for the keys' gradients too
+    float lse, along, unit = 1.0f;
+    {
+        const T* const out = (const T*)a.out.ptr + (int64_t)b * a.out.stride[0] + (int64_t)query * a.out.stride[1] +
+                             (int64_t)head * a.out.stride[2];
+        float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f}, most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2 * NB; i++) {
+            const Frag<T> y = global_row<T, VEC>(out, 16 * i + 8 * h, d);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                sums[e % 4] += (float)go[i][e] * (float)y[e];
+                most = fmaxf(most, fabsf((float)go[i][e]));
+            }
+        }
+        along = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        along += other_half(along);
+        most = fmaxf(most, other_half(most));
+        lse = ((const float*)a.lse.ptr)[(int64_t)b * a.lse.stride[0] + (int64_t)head * a.lse.stride[1] +
+                                        (int64_t)query * a.lse.stride[2]];
+        const bool live = query < seq.q_len && lse != -INFINITY;
+        lse = live ? lse * kLog2e : INFINITY;
+        along = live ? along : 0.0f;
+        if constexpr (kUnits) {
+            // 2^floor(log2 most) by its exponent bits; 0 for rows of zeros
+            const uint32_t bits = __float_as_uint(most) & 0x7f800000u;
+            unit = !live ? 0.0f : (bits == 0x7f800000u ? 1.0f : __uint_as_float(bits));
+        }
+        if (key_wave == 0 && h == 0 && wave_row0 + own < p.rows) {
+            float* const stat = p.stats + stats_row(a, b, head) + query;
+            stat[0] = lse;
+            stat[a.tokens] = along;
+            if constexpr (kUnits) {
+                stat[2 * a.tokens] = unit;
+            }
+        }
+    }
+    const float per_unit = unit > 0.0f ? 1.0f / unit : 0.0f;
     wait_for_registers();
     // as in the forward pass: 32 keys of a tile, those of tiles that all of the wavefront's rows see whole in a loop of their own
     const auto whole = [&](int t) {
@@ -376,7 +364,7 @@ attention_key_grad_kernel(GradLaunch p)
     }
     const int row_tiles = high > low ? (high - low + kBlock - 1) / kBlock : 0;
     const int steps = row_tiles * (int)p.group.div;
-    const int s_begin = min((int)part * p.each, steps), s_end = part + 1 == of ? steps : min(s_begin + p.each, steps);
+    const int s_begin = (int)((int64_t)steps * part / of), s_end = (int)((int64_t)steps * (part + 1) / of);
 
     T* const ring = reinterpret_cast<T*>(lds);
     float* const stat_ring = reinterpret_cast<float*>(lds + (size_t)kStages * 2 * kTile * sizeof(T)) +
@@ -606,19 +594,21 @@ attention_key_grad_kernel(GradLaunch p)
     }
 }
 
-// Sums of the parts of `tiles` tiles of every key head, from tile `first` on: four features of a key a thread.
+// Sums of the parts, of the sinks' tiles and of the others: four features of a key a thread.
 template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void attention_grad_join_kernel(GradLaunch p, const float* __restrict__ partials,
-                                                                  uint32_t first, uint32_t tiles, uint32_t parts,
-                                                                  uint32_t quads, uint32_t total)
+__global__ __launch_bounds__(256) void attention_grad_join_kernel(GradLaunch p, uint32_t sink_joins, uint32_t quads, uint32_t total)
 {
     const AttentionArgs& a = p.a;
     const uint32_t index = blockIdx.x * 256u + threadIdx.x;
     if (index >= total) {
         return;
     }
-    const uint32_t quad = index % quads;
-    uint32_t rest = index / quads;
+    const bool sinks = index < sink_joins;
+    const float* const partials = sinks ? p.sink_partials : p.partials;
+    const uint32_t first = sinks ? 0 : p.sink_tiles, tiles = sinks ? p.sink_tiles : p.key_tiles - p.sink_tiles;
+    const uint32_t parts = sinks ? p.sink_parts : p.parts, local = sinks ? index : index - sink_joins;
+    const uint32_t quad = local % quads;
+    uint32_t rest = local / quads;
     const uint32_t local_key = rest % p.keys;
     rest /= p.keys;
     const uint32_t value = rest & 1, tile_index = rest >> 1;
@@ -718,7 +708,7 @@ hipError_t run_backward(const AttentionArgs& a, hipStream_t stream)
     const int64_t joins = plan.parts > 1 ? bh * (plan.key_tiles - plan.sink_tiles) * 2 * plan.keys * quads : 0;
     // 3 * tokens * 4 bytes of statistics are reached with 32-bit offsets
     if (query_blocks > INT32_MAX / 1024 || key_blocks > INT32_MAX / 1024 || stat_rows > INT32_MAX / 16 ||
-        a.tokens > INT32_MAX / 12 || sink_joins > INT32_MAX || joins > INT32_MAX ||
+        a.tokens > INT32_MAX / 12 || sink_joins + joins > INT32_MAX ||
         (a.scratch == nullptr && plan.stats > 0)) {
         return hipErrorInvalidValue;
     }
@@ -733,16 +723,11 @@ hipError_t run_backward(const AttentionArgs& a, hipStream_t stream)
     p.sink_tiles = (uint32_t)plan.sink_tiles;
     p.sink_parts = (uint32_t)plan.sink_parts;
     p.parts = (uint32_t)plan.parts;
-    p.each = (int32_t)plan.each;
     p.query_blocks = (uint32_t)query_blocks;
     p.key_blocks = (uint32_t)key_blocks;
     p.stats = a.scratch;
     p.sink_partials = a.scratch + (plan.stats + 3) / 4 * 4;
     p.partials = p.sink_partials + plan.sink_partials;
-    if (stat_rows > 0) {
-        hipLaunchKernelGGL((attention_stats_kernel<T, VEC>), dim3((unsigned)((stat_rows + 15) / 16)), dim3(256), 0, stream, p,
-                           (uint32_t)stat_rows);
-    }
     hipError_t e = hipErrorInvalidValue;
     switch (blocks_of(a.d)) {
         case 8: e = run_backward_shape<T, 8, VEC>(p, plan.few_rows, stream); break;
@@ -754,14 +739,10 @@ hipError_t run_backward(const AttentionArgs& a, hipStream_t stream)
     if (e != hipSuccess) {
         return e;
     }
-    if (sink_joins > 0) {
-        hipLaunchKernelGGL((attention_grad_join_kernel<T, VEC>), dim3((unsigned)((sink_joins + 255) / 256)), dim3(256), 0,
-                           stream, p, p.sink_partials, 0u, p.sink_tiles, p.sink_parts, (uint32_t)quads, (uint32_t)sink_joins);
-    }
-    if (joins > 0) {
-        hipLaunchKernelGGL((attention_grad_join_kernel<T, VEC>), dim3((unsigned)((joins + 255) / 256)), dim3(256), 0, stream,
-                           p, p.partials, p.sink_tiles, p.key_tiles - p.sink_tiles, p.parts, (uint32_t)quads,
-                           (uint32_t)joins);
+    if (sink_joins + joins > 0) {
+        const uint32_t total = (uint32_t)(sink_joins + joins);
+        hipLaunchKernelGGL((attention_grad_join_kernel<T, VEC>), dim3((total + 255) / 256), dim3(256), 0, stream, p,
+                           (uint32_t)sink_joins, (uint32_t)quads, total);
     }
     return hipGetLastError();
 }

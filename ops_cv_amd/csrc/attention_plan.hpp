@@ -90,7 +90,6 @@ struct GradPlan {
     int64_t keys = 0;                  // of a tile
     int64_t key_tiles = 0;             // of a key head
     int64_t sink_tiles = 0;            // the first of them, seen by queries of any position
-    int64_t each = 1;                  // steps of a part
     int64_t sink_parts = 1, parts = 1; // parts that the queries of such a tile, and of the others, are cut into at most
     // 32-bit words of the scratch: statistics of the rows, partial gradients of the sinks' tiles and of the others
     int64_t stats = 0, sink_partials = 0, partials = 0;
@@ -112,11 +111,12 @@ inline GradPlan plan_grad(const AttentionArgs& a)
     const int64_t all = (a.tokens + kBlock - 1) / kBlock;
     const int64_t window = (a.left + a.right + p.keys + kBlock - 1) / kBlock + 1;
     const int64_t steps = group * (window < all ? window : all);
-    // As few parts as fill the card with one round of workgroups, the shorter ones last: ten wavefronts for every CU, of
-    // which eight run at a time, where a part has eight steps or more (4096 tokens, 32 heads of 128 on 8, window 1024, bf16:
-    // 302 us for the whole backward call, with eight 348, with fourteen 323).  FLOAT: one step or more, and as many
-    // wavefronts as its registers leave room for: four from three blocks of features on, eight of two, and of one block many
-    // short parts (3 x 1024 tokens, 64 heads of 32 on 8: 732 us with 32, with eight 937).
+    // As few parts as fill the card with one round of workgroups, every tile's steps in equal parts: ten wavefronts for every
+    // CU, of which eight run at a time, where a part has eight steps or more (4096 tokens, 32 heads of 128 on 8, window 1024,
+    // bf16: 294 us for the whole backward call, with eight 334, with sixteen 314; parts of as many steps each, whose last
+    // is what is left: 325).  FLOAT: one step or more, and as many wavefronts as its registers leave room for: four from
+    // three blocks of features on, eight of two, and of one block many short parts (3 x 1024 tokens, 64 heads of 32 on 8:
+    // 732 us with 32, with eight 937).
     const int64_t sink_steps = group * all;
     const int64_t room = a.compute_units * (a.elem != 0 ? 10 : blocks_of(a.d) > 2 ? 4 : blocks_of(a.d) == 2 ? 8 : 32) * kBlock / p.keys;
     const auto items = [&](int64_t each) {
@@ -131,7 +131,6 @@ inline GradPlan plan_grad(const AttentionArgs& a)
             low = middle + 1;
         }
     }
-    p.each = low;
     p.parts = (steps + low - 1) / low;
     p.sink_parts = (sink_steps + low - 1) / low;
     p.parts = p.parts < 1 ? 1 : p.parts;
