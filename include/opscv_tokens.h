@@ -108,8 +108,8 @@ ACLNN_API aclnnStatus opscvRotary(void* workspace, uint64_t workspaceSize, aclOp
  *       [0, kvTokens].  A sequence's queries are its last tokens: query i < qLength stands at
  *       p = kvLength - qLength + i.
  *   Query i sees key j if j < kvLength, j <= p + right, and (j >= p - left or j < sinks).
- *   out = softmax over the seen keys of (scale * query . key) applied to their values; what a key or value holds that no
- *       query of its head group sees, or from kvLength on, is never read into a result, NaN included.  A query that
+ *   out = softmax over the seen keys of (scale * query . key) applied to their values; what a key or value holds that a
+ *       query does not see, or from kvLength on, is never read into its result, NaN included.  A query that
  *       sees nothing (i >= qLength among them) gives zeros.
  *   lse : NULL, or (batch, heads, tokens), FLOAT: ln of the sum of exp(scale * query . key) over the seen keys, minus
  *       infinity where nothing is seen
@@ -127,6 +127,9 @@ ACLNN_API aclnnStatus opscvWindowAttention(void* workspace, uint64_t workspaceSi
 /*
  * Gradients of the attention.  out and lse are what the forward call wrote for the same arguments; gradQuery, gradKey
  * and gradValue have the shapes of query, key and value and are written whole (zeros where nothing is seen).
+ * What keys, values, queries and gradients hold past the sequences' lengths is never read into a result, nor is a key or
+ * value that a query does not see into that query's gradient.  A query or its gradOut that is not finite reaches the
+ * gradients of the keys that it sees, and may reach those of keys beside them.
  */
 ACLNN_API aclnnStatus opscvWindowAttentionBackwardGetWorkspaceSize(
     const aclTensor* gradOut, const aclTensor* query, const aclTensor* key, const aclTensor* value,

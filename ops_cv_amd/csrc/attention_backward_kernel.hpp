@@ -45,6 +45,34 @@ static __device__ __forceinline__ int64_t stats_row(const AttentionArgs& a, int6
 
 // ---------------------------------------------------------------------------------------------------- queries' gradients
 
+// gQ' += K' dS' for one block of features and 32 keys that some rows do not see and that may hold values that are not finite:
+// the finite ones are multiplied as ever, and the rows that see one of the others (products of ones and zeros count them)
+// get NaN, which is what a score that is not finite makes of them.
+template <typename T, int PITCH>
+static __device__ __forceinline__ acc_t add_seen_keys(acc_t sum, const acc_t& ds, const acc_t& seen, const T* tile, int block,
+                                                      int lane)
+{
+    acc_t count = zeros();
+#pragma unroll
+    for (int g = 0; g < 2; g++) {
+        Frag<T> f = Tile<T, PITCH>::column(tile, 16 * g, block, lane), special;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float v = (float)f[e];
+            const bool finite = __builtin_amdgcn_classf(v, 0x1f8);
+            f[e] = (T)(finite ? v : 0.0f);
+            special[e] = (T)(finite ? 0.0f : 1.0f);
+        }
+        sum = Mma<T>::mul(f, operand<T>(ds, g), sum);
+        count = Mma<T>::mul(special, operand<T>(seen, g), count);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+        sum[r] = count[r] > 0.0f ? NAN : sum[r];
+    }
+    return sum;
+}
+
 template <typename T, int NB, bool FEW, bool VEC>
 __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads(),
                              sizeof(T) * NB <= 8 ? 2 : 1) void attention_query_grad_kernel(GradLaunch p)
@@ -100,10 +128,6 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
     };
     const float c = a.scale * kLog2e;
     acc_t gq[NB];
-#pragma unroll
-    for (int i = 0; i < NB; i++) {
-        gq[i] = zeros();
-    }
     int buffer = 0;
     constexpr int kInFlight = 2 * kKeys * Tile<T, kPitch>::kChunks / kThreads;  // loads of one fetch, a wavefront
     if (key_wave < range.tiles) {
@@ -170,6 +194,7 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
         return wave_low > wave_high || key0 >= end || key0 > wave_high + right ||
                (key0 + kBlock - 1 < wave_low - left && key0 >= sinks);
     };
+    bool careful = false;  // a second pass, for keys that are not finite
     const auto attend = [&](auto part, int key0, int end, const T* k_tile, const T* v_tile, const Rows32<T, kPitch, NB>& rows,
                             const Columns32<T, kPitch, NB>& columns) {
         acc_t s = zeros(), dp = zeros();
@@ -192,16 +217,29 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
                 s[r] = see.sees(8 * (r / 4) + r % 4) ? s[r] : 0.0f;
             }
         }
+        if (decltype(part)::value && __builtin_expect(careful, 0)) {
+            const Sight see = sight(pos, key0 + 4 * h, end, left, right, sinks);
+            acc_t seen;
 #pragma unroll
-        for (int g = 0; g < 2; g++) {
-            const Frag<T> w = operand<T>(s, g);
+            for (int r = 0; r < 16; r++) {
+                seen[r] = see.sees(8 * (r / 4) + r % 4) ? 1.0f : 0.0f;
+            }
 #pragma unroll
             for (int i = 0; i < NB; i++) {
-                gq[i] = Mma<T>::mul(columns(k_tile, 16 * g, i), w, gq[i]);
+                gq[i] = add_seen_keys<T, kPitch>(gq[i], s, seen, k_tile, i, again(lane));
             }
-        }
-        if constexpr (sizeof(T) == 2) {
-            read_ahead<2 * NB, 2, 3>();
+        } else {
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+                const Frag<T> w = operand<T>(s, g);
+#pragma unroll
+                for (int i = 0; i < NB; i++) {
+                    gq[i] = Mma<T>::mul(columns(k_tile, 16 * g, i), w, gq[i]);
+                }
+            }
+            if constexpr (sizeof(T) == 2) {
+                read_ahead<2 * NB, 2, 3>();
+            }
         }
     };
     int t = key_wave;
@@ -249,18 +287,43 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
         buffer ^= kShape.stages - 1;
         t += kJoin;
     };
-    while (t < range.tiles) {
-        {
+    while (true) {
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+            gq[i] = zeros();
+        }
+        while (t < range.tiles) {
+            {
+                const Rows32<T, kPitch, NB> rows(again(lane));
+                const Columns32<T, kPitch, NB> columns(again(lane));
+                while (t < range.tiles && !whole(t)) {
+                    work(std::true_type(), rows, columns);
+                }
+            }
             const Rows32<T, kPitch, NB> rows(again(lane));
             const Columns32<T, kPitch, NB> columns(again(lane));
-            while (t < range.tiles && !whole(t)) {
-                work(std::true_type(), rows, columns);
+            while (t < range.tiles && whole(t)) {
+                work(std::false_type(), rows, columns);
             }
         }
-        const Rows32<T, kPitch, NB> rows(again(lane));
-        const Columns32<T, kPitch, NB> columns(again(lane));
-        while (t < range.tiles && whole(t)) {
-            work(std::false_type(), rows, columns);
+        // as in the forward pass: gradients that are not finite may come from keys that a row does not see
+        float check = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                check = __builtin_fmaf(gq[i][r], 0.0f, check);
+            }
+        }
+        const bool odd = !careful && check != 0.0f;
+        if (!(kShape.row_waves > 1 ? __syncthreads_or(odd) : __any(odd))) {
+            break;
+        }
+        careful = true;
+        t = key_wave;
+        buffer = 0;
+        if (t < range.tiles) {
+            fetch(t, 0);
         }
     }
     if constexpr (kJoin > 1) {

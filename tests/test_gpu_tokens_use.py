@@ -161,3 +161,32 @@ def test_example_block(device):
                        stderr=subprocess.STDOUT, text=True, timeout=110, cwd=ROOT)
     assert p.returncode == 0, p.stdout
     assert "decoded" in p.stdout and "loss" in p.stdout
+
+
+@pytest.mark.parametrize("dtype,sq,heads,d", [(torch.bfloat16, 300, 8, 128), (torch.float16, 7, 2, 64), (torch.float32, 150, 2, 72),
+                                              (torch.float16, 160, 4, 256), (torch.bfloat16, 1500, 64, 32)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_gradients_of_queries_beside_keys_that_are_not_finite(device, aclnn, dtype, sq, heads, d, bad):
+    """A key that is not finite reaches the gradients of the queries that see it, and no other query's, by a single bit."""
+    skv, left, sinks = sq + 90, 40, 3
+    q, go = normal(device, 1, 1, sq, heads, d, dtype=dtype), normal(device, 2, 1, sq, heads, d, dtype=dtype)
+    k, v = normal(device, 3, 1, skv, 2, d, dtype=dtype), normal(device, 4, 1, skv, 2, d, dtype=dtype)
+    masks = dict(left=left, sinks=sinks)
+
+    def grads(k, v):
+        out, lse = aclnn.window_attention(q, k, v, need_lse=True, **masks)
+        return aclnn.window_attention_backward(go, q, k, v, out, lse, **masks)
+    clean = grads(k, v)
+    position = torch.arange(sq, device=device) + skv - sq
+    for key in (20, skv - sq // 2 - 1):  # seen by nobody, and by some
+        for which in (0, 1):
+            pair = [k.clone(), v.clone()]
+            pair[which][0, key, 0, d // 3] = bad
+            got = grads(*pair)
+            sees = (position >= key) & (position - left <= key)
+            half = heads // 2  # heads of the first key head
+            assert torch.equal(got[0][:, ~sees], clean[0][:, ~sees]) and torch.equal(got[0][:, :, half:], clean[0][:, :, half:])
+            reached = got[0][:, sees][:, :, :half]  # a score of minus infinity leaves 0 times infinity, at the key's own feature
+            assert not (reached if which else reached[..., d // 3]).isfinite().any()
+            if not sees.any():
+                assert torch.equal(got[1], clean[1]) and torch.equal(got[2], clean[2])
