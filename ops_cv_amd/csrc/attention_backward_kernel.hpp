@@ -74,13 +74,17 @@ static __device__ __forceinline__ acc_t add_seen_keys(acc_t sum, const acc_t& ds
 }
 
 template <typename T, int NB, bool FEW, bool VEC>
-__global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads(),
+__global__ __launch_bounds__(grad_query_shape(sizeof(T), pitch_of(NB), FEW).threads(),
                              sizeof(T) * NB <= 8 ? 2 : 1) void attention_query_grad_kernel(GradLaunch p)
 {
     constexpr int kPitch = pitch_of(NB);
-    constexpr ForwardShape kShape = forward_shape(sizeof(T), kPitch, FEW);
+    constexpr ForwardShape kShape = grad_query_shape(sizeof(T), kPitch, FEW);
     constexpr int kKeys = kShape.keys, kThreads = 64 * kShape.row_waves, kJoin = kShape.key_waves;
     constexpr bool kUnits = std::is_same<T, _Float16>::value;
+    // FLOAT's products take so long that operands can come from memory as they are needed: the values of wider heads do,
+    // which leaves LDS for the keys of four wavefronts, and gO of the widest, which leaves registers for the rest
+    constexpr bool kDirect = grad_values_direct(sizeof(T), kPitch, FEW), kGradDirect = kDirect && NB > 4;
+    constexpr int kTileElems = (kDirect ? 1 : 2) * kKeys * kPitch;
     extern __shared__ __align__(16) char lds[];
 
     const AttentionArgs& a = p.a;
@@ -115,34 +119,38 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
     const T* const v_base = (const T*)a.v.ptr + (int64_t)b * a.v.stride[0] + (int64_t)kv_head * a.v.stride[2];
     const uint32_t k_pitch = (uint32_t)(a.k.stride[1] * (int64_t)sizeof(T));
     const uint32_t v_pitch = (uint32_t)(a.v.stride[1] * (int64_t)sizeof(T));
-    T* const ring = reinterpret_cast<T*>(lds) + (size_t)key_wave * (kShape.stages * 2 * kKeys * kPitch);
+    T* const ring = reinterpret_cast<T*>(lds) + (size_t)key_wave * (kShape.stages * kTileElems);
     const auto fetch = [&](int t, int buffer) {
         const int key0 = range.key_of(t, kKeys), rows = range.end_of(t) - key0;
-        T* const k_tile = ring + buffer * (2 * kKeys * kPitch);
+        T* const k_tile = ring + buffer * kTileElems;
         const int gt = row_wave * 64 + again(lane);
         stage<T, kPitch, kKeys, kThreads, VEC>(k_tile, at_bytes(k_base, (uint32_t)key0, k_pitch), gt, row_wave, d, k_pitch,
                                                min(rows, kKeys));
-        stage<T, kPitch, kKeys, kThreads, VEC>(k_tile + kKeys * kPitch, at_bytes(v_base, (uint32_t)key0, v_pitch), gt, row_wave, d,
-                                               v_pitch,
-                                         min(rows, kKeys));
+        if constexpr (!kDirect) {
+            stage<T, kPitch, kKeys, kThreads, VEC>(k_tile + kKeys * kPitch, at_bytes(v_base, (uint32_t)key0, v_pitch), gt, row_wave,
+                                                   d, v_pitch, min(rows, kKeys));
+        }
     };
     const float c = a.scale * kLog2e;
     acc_t gq[NB];
     int buffer = 0;
-    constexpr int kInFlight = 2 * kKeys * Tile<T, kPitch>::kChunks / kThreads;  // loads of one fetch, a wavefront
+    constexpr int kInFlight = kTileElems / kPitch * Tile<T, kPitch>::kChunks / kThreads;  // loads of one fetch, a wavefront
     if (key_wave < range.tiles) {
         fetch(key_wave, 0);
     }
-    Frag<T> q[2 * NB], go[2 * NB];
+    Frag<T> q[2 * NB], held[kGradDirect ? 1 : 2 * NB];
+    const T* const grad_row = (const T*)a.grad_out.ptr + (int64_t)b * a.grad_out.stride[0] +
+                              (int64_t)query * a.grad_out.stride[1] + (int64_t)head * a.grad_out.stride[2];
+    const auto go = [&](int i) { return kGradDirect ? global_row<T, VEC>(grad_row, 16 * i + 8 * h, d) : held[kGradDirect ? 0 : i]; };
     {
         const T* const src = (const T*)a.q.ptr + (int64_t)b * a.q.stride[0] + (int64_t)query * a.q.stride[1] +
                              (int64_t)head * a.q.stride[2];
-        const T* const gsrc = (const T*)a.grad_out.ptr + (int64_t)b * a.grad_out.stride[0] +
-                              (int64_t)query * a.grad_out.stride[1] + (int64_t)head * a.grad_out.stride[2];
 #pragma unroll
         for (int i = 0; i < 2 * NB; i++) {
             q[i] = global_row<T, VEC>(src, 16 * i + 8 * h, d);
-            go[i] = global_row<T, VEC>(gsrc, 16 * i + 8 * h, d);
+            if constexpr (!kGradDirect) {
+                held[i] = global_row<T, VEC>(grad_row, 16 * i + 8 * h, d);
+            }
         }
     }
     // the row's statistics, left for the keys' gradients too
@@ -153,11 +161,11 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
         float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f}, most = 0.0f;
 #pragma unroll
         for (int i = 0; i < 2 * NB; i++) {
-            const Frag<T> y = global_row<T, VEC>(out, 16 * i + 8 * h, d);
+            const Frag<T> x = go(i), y = global_row<T, VEC>(out, 16 * i + 8 * h, d);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                sums[e % 4] += (float)go[i][e] * (float)y[e];
-                most = fmaxf(most, fabsf((float)go[i][e]));
+                sums[e % 4] += (float)x[e] * (float)y[e];
+                most = fmaxf(most, fabsf((float)x[e]));
             }
         }
         along = (sums[0] + sums[1]) + (sums[2] + sums[3]);
@@ -198,10 +206,31 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
     const auto attend = [&](auto part, int key0, int end, const T* k_tile, const T* v_tile, const Rows32<T, kPitch, NB>& rows,
                             const Columns32<T, kPitch, NB>& columns) {
         acc_t s = zeros(), dp = zeros();
+        // keys that the lane's value stands in for past the end are not seen
+        const T* const value = kDirect ? at_bytes(v_base, (uint32_t)min(key0 + own, end - 1), v_pitch) : nullptr;
+        if constexpr (kGradDirect) {
+            // the next operands are asked for before a product, and no earlier: their registers are few
+            Frag<T> value_now = global_row<T, VEC>(value, 8 * h, d), grad_now = go(0);
 #pragma unroll
-        for (int i = 0; i < 2 * NB; i++) {
-            s = Mma<T>::mul(rows(k_tile, 0, i), q[i], s);
-            dp = Mma<T>::mul(rows(v_tile, 0, i), go[i], dp);
+            for (int i = 0; i < 2 * NB; i++) {
+                const int next = i + 1 < 2 * NB ? i + 1 : i;
+                const Frag<T> value_next = global_row<T, VEC>(value, 16 * next + 8 * h, d), grad_next = go(next);
+                dp = Mma<T>::mul(value_now, grad_now, dp);
+                s = Mma<T>::mul(rows(k_tile, 0, i), q[i], s);
+                __builtin_amdgcn_sched_barrier(0);
+                value_now = value_next;
+                grad_now = grad_next;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2 * NB; i++) {
+                s = Mma<T>::mul(rows(k_tile, 0, i), q[i], s);
+                if constexpr (kDirect) {
+                    dp = Mma<T>::mul(global_row<T, VEC>(value, 16 * i + 8 * h, d), held[i], dp);
+                } else {
+                    dp = Mma<T>::mul(rows(v_tile, 0, i), held[i], dp);
+                }
+            }
         }
         if constexpr (sizeof(T) == 2) {
             read_ahead<4 * NB, 1, 4>();
@@ -260,7 +289,7 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
                 wait_for_loads<0>();
             }
         }
-        const T* const k_tile = ring + buffer * (2 * kKeys * kPitch);
+        const T* const k_tile = ring + buffer * kTileElems;
         const T* const v_tile = k_tile + kKeys * kPitch;
         const int key0 = range.key_of(t, kKeys), end = range.end_of(t);
         if constexpr (PART) {
@@ -699,8 +728,9 @@ __global__ __launch_bounds__(256) void attention_grad_join_kernel(GradLaunch p, 
 template <typename T, int NB, bool FEW, bool VEC>
 hipError_t launch_query_grad(const GradLaunch& p, hipStream_t stream)
 {
-    constexpr ForwardShape kShape = forward_shape(sizeof(T), pitch_of(NB), FEW);
-    constexpr int kTiles = kShape.key_waves * kShape.stages * 2 * kShape.keys * pitch_of(NB) * (int)sizeof(T);
+    constexpr ForwardShape kShape = grad_query_shape(sizeof(T), pitch_of(NB), FEW);
+    constexpr int kOperands = grad_values_direct(sizeof(T), pitch_of(NB), FEW) ? 1 : 2;
+    constexpr int kTiles = kShape.key_waves * kShape.stages * kOperands * kShape.keys * pitch_of(NB) * (int)sizeof(T);
     constexpr int kJoin = kShape.key_waves > 1 ? kShape.key_waves * NB * kBlock * kBlock * 4 : 0;
     constexpr int kBytes = kTiles > kJoin ? kTiles : kJoin;
     static_assert(kBytes <= 160 * 1024, "LDS of a CU");
@@ -740,7 +770,7 @@ hipError_t run_backward_shape(const GradLaunch& p, bool few, hipStream_t stream)
 {
     hipError_t e = hipSuccess;
     if (p.query_blocks > 0) {
-        if constexpr (sizeof(T) == 2) {
+        if constexpr (sizeof(T) == 2 || NB > 2) {
             e = few ? launch_query_grad<T, NB, true, VEC>(p, stream) : launch_query_grad<T, NB, false, VEC>(p, stream);
         } else {
             e = few ? launch_query_grad<T, NB, true, VEC>(p, stream) : hipErrorInvalidValue;

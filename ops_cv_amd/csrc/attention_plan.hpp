@@ -80,6 +80,22 @@ inline ForwardPlan plan_forward(const AttentionArgs& a)
 
 // ---------------------------------------------------------------------------------------------------------- gradients
 
+// The queries' gradients: as the forward pass, but for FLOAT of more than 64 features, whose tiles fill LDS: 32 rows and one
+// wavefront, or, for few rows, four that share the keys.  There, and for heads of more than 128 features, the values come
+// straight from memory: FLOAT's products take long enough for that (4 x 1024 tokens, 2 heads of 128, causal: four wavefronts
+// 81 us, one 217; 16 x 512, 2 heads of 256 on 1: 205 and 334), and yet from LDS they come sooner (one wavefront: 2 x 777
+// tokens, 12 heads of 72 on 4, window 101: 38 us, with values from memory 42, with four wavefronts 53).
+constexpr bool grad_values_direct(int elem_bytes, int pitch, bool few_rows)
+{
+    return elem_bytes == 4 && (pitch > 128 || (pitch > 64 && few_rows));
+}
+constexpr ForwardShape grad_query_shape(int elem_bytes, int pitch, bool few_rows)
+{
+    return elem_bytes == 2 || pitch <= 64 ? forward_shape(elem_bytes, pitch, few_rows)
+           : few_rows                     ? ForwardShape{1, 4, 32, 1}
+                                          : ForwardShape{1, 1, 32, 1};
+}
+
 // The keys' gradients: a wavefront has 32 keys and walks tiles of 32 queries of one head.  16-bit types: four wavefronts walk
 // together, so that a tile of queries is loaded once for 128 keys.  FLOAT: each by itself, for the same reason as above.
 constexpr int grad_key_waves(bool is_float, int nb) { return is_float && nb <= 4 ? 1 : 4; }
@@ -103,6 +119,9 @@ inline GradPlan plan_grad(const AttentionArgs& a)
     p.few_rows = few_rows(a);
     const int64_t tile_rows = p.few_rows ? kBlock : 4 * kBlock;
     p.tiles = (p.rows + tile_rows - 1) / tile_rows;
+    if (a.elem == 0 && a.d > 64) {
+        p.few_rows = bh * p.tiles <= 2 * a.compute_units;
+    }
     p.keys = kBlock * grad_key_waves(a.elem == 0, blocks_of(a.d));
     p.key_tiles = (a.kv_tokens + p.keys - 1) / p.keys;
     const int64_t sinks = a.sinks < a.kv_tokens ? a.sinks : a.kv_tokens;
