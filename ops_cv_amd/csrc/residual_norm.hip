@@ -585,9 +585,17 @@ hipError_t by_type(int elem, int weight_float, F&& f)
 
 int64_t norm_grad_partials(const NormGradArgs& a)
 {
-    // a workgroup takes up to eight rows at a time; one row of partial sums even where there are no rows
+    // A workgroup takes up to eight rows at a time; one row of partial sums even where there are no rows.  Of wide rows it
+    // takes one or two, and few of them go to as many workgroups as there are CUs (64 rows of 5120 FLOAT: 10.8 us, eight rows
+    // a workgroup 25.8; 419: 16.6 and 28.7), unless one workgroup, which needs no second kernel, is as fast (four rows of
+    // 2048: 6.6 us, of 5120: 14.5).
+    constexpr int64_t kWide = 1024, kWidest = 4096;
     const int64_t groups = (a.rows + 7) / 8;
-    return groups < 1 ? 1 : (groups < kPartialRows ? groups : kPartialRows);
+    if (a.rows <= 1 || (groups == 1 && a.width <= kWidest)) {
+        return 1;
+    }
+    const int64_t spread = a.width <= kWide ? groups : (a.rows < 256 ? a.rows : 256);
+    return groups < spread ? spread : (groups < kPartialRows ? groups : kPartialRows);
 }
 
 hipError_t launch_residual_norm(const NormArgs& args, hipStream_t stream)
