@@ -11,6 +11,12 @@
 // want them.  P and dS are computed twice, once for each direction: seven products instead of five, but every sum has one
 // owner and a fixed order, and no gradient is added up by atomics.
 //
+// 4096 tokens, 32 heads of 128 on 8, window 1024, bf16: 280 to 290 us (520 TFLOP/s of the five products); keys 172 to 200,
+// queries 115 to 140, the join 15.  The keys' kernel reads five operands of 1 KB from LDS for four products, a quarter more
+// than LDS gives in their time, at two wavefronts a SIMD, which is what its accumulators leave room for.  FLOAT (2 x 777
+// tokens, 12 heads of 72 on 4, window 101: 92 us) is bound by its products, which take sixteen times as long, and by tiles
+// of 32 along a window of 101.
+//
 // dS of FLOAT16: P of a long row times a small gradient falls among the numbers that FLOAT16 has few bits or none for, so dS
 // is divided by a power of two of the size of the row's (of the rows' walked so far) gradient before it is rounded, and
 // the sum multiplied by it.
@@ -127,8 +133,8 @@ __global__ __launch_bounds__(grad_query_shape(sizeof(T), pitch_of(NB), FEW).thre
         stage<T, kPitch, kKeys, kThreads, VEC>(k_tile, at_bytes(k_base, (uint32_t)key0, k_pitch), gt, row_wave, d, k_pitch,
                                                min(rows, kKeys));
         if constexpr (!kDirect) {
-            stage<T, kPitch, kKeys, kThreads, VEC>(k_tile + kKeys * kPitch, at_bytes(v_base, (uint32_t)key0, v_pitch), gt, row_wave,
-                                                   d, v_pitch, min(rows, kKeys));
+            stage<T, kPitch, kKeys, kThreads, VEC>(k_tile + kKeys * kPitch, at_bytes(v_base, (uint32_t)key0, v_pitch), gt,
+                                                   row_wave, d, v_pitch, min(rows, kKeys));
         }
     };
     const float c = a.scale * kLog2e;
@@ -141,7 +147,13 @@ __global__ __launch_bounds__(grad_query_shape(sizeof(T), pitch_of(NB), FEW).thre
     Frag<T> q[2 * NB], held[kGradDirect ? 1 : 2 * NB];
     const T* const grad_row = (const T*)a.grad_out.ptr + (int64_t)b * a.grad_out.stride[0] +
                               (int64_t)query * a.grad_out.stride[1] + (int64_t)head * a.grad_out.stride[2];
-    const auto go = [&](int i) { return kGradDirect ? global_row<T, VEC>(grad_row, 16 * i + 8 * h, d) : held[kGradDirect ? 0 : i]; };
+    const auto go = [&](int i) {
+        if constexpr (kGradDirect) {
+            return global_row<T, VEC>(grad_row, 16 * i + 8 * h, d);
+        } else {
+            return held[i];
+        }
+    };
     {
         const T* const src = (const T*)a.q.ptr + (int64_t)b * a.q.stride[0] + (int64_t)query * a.q.stride[1] +
                              (int64_t)head * a.q.stride[2];

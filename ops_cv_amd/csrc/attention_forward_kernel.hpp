@@ -8,6 +8,15 @@
 //                    row's keys are spread over two lanes, which exchange their maxima
 //   O' = O' f + V' P (head features x 32 rows; V from LDS in "column" order, P are S's registers, rounded to the type)
 // m, l and O stay in 32 bits; P is rounded to the type as the matrix instructions want it.
+//
+// Why so: O' in registers, its columns being rows of the product, is scaled by one number a lane, and S' becomes the
+// operand P without leaving the registers.  Bound by memory for single tokens (32 caches of up to 16384 tokens, window
+// 4096, 32 heads of 128 on 8, bf16: 104 us, 5.2 TB/s), where the keys are shared out over wavefronts and workgroups.  Of
+// prompts (8192 tokens, the same heads, window 1024: 163 to 175 us on different machines, 740 to 790 TFLOP/s) by LDS as
+// much as by the matrix cores: 32 rows a wavefront read 1 KB for every product, as much as LDS gives four SIMDs meanwhile.
+// Wavefronts of 64 rows would halve that, but leave the registers of one a SIMD, whose loads and exponentials are then
+// not behind the products (235 us).  Heads of 64 (8 images of 1369 tokens, 16 heads, window 513: 51 us) have half the
+// products to an exponential and are bound by vector instructions and what is left undone while wavefronts wait.
 #pragma once
 
 #include <atomic>

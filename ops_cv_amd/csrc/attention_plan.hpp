@@ -137,9 +137,11 @@ inline GradPlan plan_grad(const AttentionArgs& a)
     // three blocks of features on, eight of two, and of one block many short parts (3 x 1024 tokens, 64 heads of 32 on 8:
     // 732 us with 32, with eight 937).
     const int64_t sink_steps = group * all;
-    const int64_t room = a.compute_units * (a.elem != 0 ? 10 : blocks_of(a.d) > 2 ? 4 : blocks_of(a.d) == 2 ? 8 : 32) * kBlock / p.keys;
+    const int64_t waves = a.elem != 0 ? 10 : blocks_of(a.d) > 2 ? 4 : blocks_of(a.d) == 2 ? 8 : 32;
+    const int64_t room = a.compute_units * waves * kBlock / p.keys;
     const auto items = [&](int64_t each) {
-        return bh * (p.sink_tiles * ((sink_steps + each - 1) / each) + (p.key_tiles - p.sink_tiles) * ((steps + each - 1) / each));
+        return bh * (p.sink_tiles * ((sink_steps + each - 1) / each) +
+                     (p.key_tiles - p.sink_tiles) * ((steps + each - 1) / each));
     };
     int64_t low = a.elem == 0 ? 1 : 8, high = steps > low ? steps : low;  // the fewest steps whose parts fit, or all
     while (low < high) {

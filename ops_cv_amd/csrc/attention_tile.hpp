@@ -195,26 +195,6 @@ struct Tile {
 
     static constexpr int bytes(int rows) { return rows * PITCH * (int)sizeof(T); }
 
-    // eight elements from element 8 c of a row on: an operand in "row" order, m or n = the row
-    static __device__ __forceinline__ Frag<T> row(const T* tile, int r, int c)
-    {
-        const T* const at = tile + r * PITCH;
-        if constexpr (sizeof(T) == 2) {
-            return *reinterpret_cast<const Frag<T>*>(at + ((c ^ swizzle(r)) * 8));
-        } else {
-            typedef float f32x4 __attribute__((ext_vector_type(4)));
-            const f32x4 a = *reinterpret_cast<const f32x4*>(at + (((2 * c) ^ swizzle(r)) * 4));
-            const f32x4 b = *reinterpret_cast<const f32x4*>(at + (((2 * c + 1) ^ swizzle(r)) * 4));
-            Frag<T> f;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                f[e] = a[e];
-                f[4 + e] = b[e];
-            }
-            return f;
-        }
-    }
-
     // element 32 block + l % 32 of rows base + 4 h + {0..3, 8..11}: an operand in "column" order, m or n = the element
     static __device__ __forceinline__ Frag<T> column(const T* tile, int base, int block, int lane)
     {
@@ -323,6 +303,13 @@ struct Columns32 {
     }
 };
 
+// the address `n` rows of `pitch` bytes behind another
+template <typename T>
+static __device__ __forceinline__ const T* at_bytes(const T* base, uint32_t n, uint32_t pitch)
+{
+    return reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + (uint64_t)n * pitch);
+}
+
 // the loads of stage(): chunk `place` (swizzled) of rows r0, r0 + STEP, ..., BYTES apart in LDS
 template <typename T, int PITCH, int STEP, int BYTES, int... I>
 static __device__ __forceinline__ void stage_chunks(rsrc_t rsrc, uint32_t dst, int r0, int place, int d, uint32_t pitch,
@@ -339,8 +326,8 @@ static __device__ __forceinline__ void stage_chunks(rsrc_t rsrc, uint32_t dst, i
 }
 
 // Copies ROWS rows into a tile by THREADS threads (thread `gt` of them, in their wavefront `wave`): row r from base + r * pitch
-// bytes, rows from `rows` (one or more) on and elements from d on as zeros.  VEC: 16-byte loads that write LDS themselves (asynchronous:
-// the caller waits), pitch at least the row's own bytes; else element by element.
+// bytes, rows from `rows` (one or more) on and elements from d on as zeros.  VEC: 16-byte loads that write LDS themselves
+// (asynchronous: the caller waits), pitch at least the row's own bytes; else element by element.
 template <typename T, int PITCH, int ROWS, int THREADS, bool VEC>
 static __device__ __forceinline__ void stage(T* tile, const T* base, int gt, int wave, int d, uint32_t pitch, int rows)
 {
@@ -366,21 +353,12 @@ static __device__ __forceinline__ void stage(T* tile, const T* base, int gt, int
 #pragma unroll
             for (int e = 0; e < L::kPerChunk; e++) {
                 const int el = c * L::kPerChunk + e;
-                x[e] = (r >= rows || el >= d) ? (T)0.0f
-                                              : *reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) +
-                                                                            ((uint32_t)r * pitch + (uint32_t)el * (uint32_t)sizeof(T)));
+                x[e] = (r >= rows || el >= d) ? (T)0.0f : at_bytes(base, (uint32_t)r, pitch)[el];
             }
             typedef float f32x4 __attribute__((ext_vector_type(4)));
             *reinterpret_cast<f32x4*>(tile + (i * THREADS + gt) * L::kPerChunk) = *reinterpret_cast<const f32x4*>(x);
         }
     }
-}
-
-// the address `n` rows of `pitch` bytes behind another
-template <typename T>
-static __device__ __forceinline__ const T* at_bytes(const T* base, uint32_t n, uint32_t pitch)
-{
-    return reinterpret_cast<const T*>(reinterpret_cast<const char*>(base) + (uint64_t)n * pitch);
 }
 
 // Eight elements from element `first` of a row on, zeros from element d on.

@@ -46,7 +46,8 @@ static __device__ __forceinline__ void store(T* p, const float (&x)[N], bool str
 }
 
 // Outputs from the L2 caches' size on (8 x 4 MB) are written with streaming stores.  8192 rows of 4096 bf16 through the norm:
-// 52.7 us without, 48.8 with; two prompts of 4096 tokens through the rotation: 42.2 and 34.2.  (The gradients of the norm get slower by it.)
+// 52.7 us without, 48.8 with; two prompts of 4096 tokens through the rotation: 42.2 and 34.2.  (The gradients of the norm
+// get slower by it.)
 constexpr int64_t kStreamBytes = (int64_t)32 << 20;
 
 // Elements c .. c + N - 1 of a row of `width`: whole vectors (WIDE; c + N <= width), or one by one, zeros from the row's
