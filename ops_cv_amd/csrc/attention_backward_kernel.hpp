@@ -725,6 +725,7 @@ __global__ __launch_bounds__(256) void attention_grad_join_kernel(GradLaunch p, 
     const float* const from =
         partials + (((int64_t)tile_index * parts * 2 + value) * p.keys + local_key) * row_floats + quad * 4;
     float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
     for (uint32_t i = 0; i < parts; i++) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {

@@ -459,11 +459,13 @@ __global__ __launch_bounds__(256) void attention_join_kernel(ForwardLaunch p, ui
     const int64_t step = partial_floats(d) * (int64_t)p.rows;
     const float* const part = a.scratch + ((int64_t)bh * p.splits * p.rows + row) * partial_floats(d);
     float high = -INFINITY;
+#pragma unroll 8
     for (uint32_t s = 0; s < p.splits; s++) {
         high = fmaxf(high, part[s * step]);
     }
     const float base = high == -INFINITY ? 0.0f : high;
     float sum = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
     for (uint32_t s = 0; s < p.splits; s++) {
         const float* const at = part + s * step;
         const float share = exp2f(at[0] - base);

@@ -69,9 +69,11 @@ inline ForwardPlan plan_forward(const AttentionArgs& a)
     const int64_t window = a.left + a.right + s.rows() / group + 2;
     const int64_t keys = a.kv_tokens < window + a.sinks ? a.kv_tokens : window + a.sinks;
     const int64_t key_tiles = (keys + s.keys - 1) / s.keys;
-    // eight wavefronts for every CU where that many parts leave each four tiles or more
-    const int64_t waves = s.row_waves * s.key_waves;
-    const int64_t want = (8 * (int64_t)a.compute_units / waves + whole - 1) / whole, most = key_tiles / (4 * s.key_waves);
+    // Eight wavefronts for every CU where that many parts leave each four tiles or more; single wavefronts of FLOAT, whose
+    // products take sixteen times as long, one tile (one token on a window of 129, 8 heads of 96 on 1: 13 us, 25 with four; five sequences of 256
+    // tokens, a head of 128, window 86: 16 and 26).
+    const int64_t waves = s.row_waves * s.key_waves, least = waves == 1 && a.elem == 0 ? 1 : 4 * s.key_waves;
+    const int64_t want = (8 * (int64_t)a.compute_units / waves + whole - 1) / whole, most = key_tiles / least;
     p.splits = want < most ? want : most;
     p.splits = p.splits < 1 ? 1 : (p.splits > 64 ? 64 : p.splits);
     p.blocks = whole * p.splits;
