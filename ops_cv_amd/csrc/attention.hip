@@ -61,7 +61,7 @@ hipError_t launch_window_attention_grad(const AttentionArgs& a, hipStream_t stre
 int64_t attention_grad_scratch_floats(const AttentionArgs& a)
 {
     const att::GradPlan p = att::plan_grad(a);
-    return (p.stats + 3) / 4 * 4 + p.sink_partials + p.partials;
+    return p.stats + p.sink_partials + p.partials;
 }
 
 const char* attention_variant(const AttentionArgs& a)

@@ -2,7 +2,7 @@
 //
 //   queries     as the forward pass walks keys:  P' = exp2(K Q' c - lse),  dP' = V gO',  dS' = P' (dP' - D),
 //               gQ' += K' dS'.  Before that every row i's statistics, which the next kernel reads too: lse_i log2 e (infinity
-//               where the row sees nothing), D_i = sum gO_i O_i, and for FLOAT16 a power of two near the largest |gO_i|
+//               where the row sees nothing) and D_i = sum gO_i O_i
 //   keys        a wavefront keeps 32 keys and walks the queries that see them:  P, dS as above with rows and columns
 //               exchanged,  gV' += gO' P,  gK' += Q' dS
 //   join        where the queries of a tile of keys were cut into parts, their 32-bit sums in order
@@ -17,9 +17,10 @@
 // tokens, 12 heads of 72 on 4, window 101: 92 us) is bound by its products, which take sixteen times as long, and by tiles
 // of 32 along a window of 101.
 //
-// dS of FLOAT16: P of a long row times a small gradient falls among the numbers that FLOAT16 has few bits or none for, so dS
-// is divided by a power of two of the size of the row's (of the rows' walked so far) gradient before it is rounded, and
-// the sum multiplied by it.
+// dS of FLOAT16 may be anything from P of a long row times a small gradient, for which FLOAT16 has few bits or none, to the
+// products of large gradients and values, which are past its end.  So every sum's dS (of a row in the queries' kernel, of a
+// key in the keys') is divided before it is rounded by a power of two that follows the largest |dS| met so far, and the sum
+// multiplied by it (fit_unit).
 #pragma once
 
 #include <atomic>
@@ -39,14 +40,70 @@ struct GradLaunch {
     uint32_t rows, tiles, kv_heads;
     uint32_t keys, key_tiles, sink_tiles, sink_parts, parts;
     uint32_t query_blocks, key_blocks;
-    float* stats;          // (batch, heads, 3, tokens)
+    int64_t stat_pitch;
+    float* stats;          // (batch, heads, 2, stat_pitch)
     float* sink_partials;  // (batch * kv_heads, sink_tiles, sink_parts, 2, keys, d rounded up to four)
     float* partials;       // the same of the other tiles
 };
 
-static __device__ __forceinline__ int64_t stats_row(const AttentionArgs& a, int64_t b, int64_t head)
+static __device__ __forceinline__ int64_t stats_row(const GradLaunch& p, int64_t b, int64_t head)
 {
-    return (b * a.heads + head) * 3 * a.tokens;
+    return (b * p.a.heads + head) * 2 * p.stat_pitch;
+}
+
+// What dS of FLOAT16 is divided by before it is rounded, its unit: a power of two of the lane's column (a row or a key, whose
+// 32 terms of a tile two lanes hold).  Terms past 2^15 units would not be numbers; those of less than 2^-14 lose bits.
+constexpr float kMostUnits = 32768.0f;
+
+// the column's largest |x| that is finite (a term that is not leaves a sum that is not, whatever the unit)
+static __device__ __forceinline__ float largest_term(const acc_t& x)
+{
+    float highs[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int r = 0; r < 16; r += 2) {
+        highs[r / 2 % 4] = fmaxf(fmaxf(highs[r / 2 % 4], fabsf(x[r])), fabsf(x[r + 1]));
+    }
+    float high = fmaxf(fmaxf(highs[0], highs[1]), fmaxf(highs[2], highs[3]));
+    high = fmaxf(high, other_half(high));
+    return high < INFINITY ? high : 0.0f;
+}
+
+// the unit of which a term of `size` has 2^steps to 2^(steps + 1)
+static __device__ __forceinline__ float unit_of(float size, int steps)
+{
+    const float power = __uint_as_float(__float_as_uint(size) & 0x7f800000u);
+    return size > 0.0f ? fmaxf(__builtin_amdgcn_ldexpf(power, -steps), 0x1p-100f) : 0.0f;
+}
+
+// Lets `unit` grow with the largest of x, what is seen of a tile's terms; `sum` holds what the column has so far, in units.  A
+// new unit is 2^-8 of the largest term, so that it seldom has to grow again.
+template <int NB>
+static __device__ __forceinline__ void fit_unit(const acc_t& x, float& unit, acc_t (&sum)[NB])
+{
+    const float high = largest_term(x);
+    const bool grows = high > unit * kMostUnits;
+    if (__builtin_expect(__any(grows), 0)) {
+        const float now = grows ? unit_of(high, 8) : unit, fade = grows ? unit / now : 1.0f;
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                sum[i][r] *= fade;
+            }
+        }
+        unit = now;
+    }
+}
+
+// x in units
+static __device__ __forceinline__ void to_units(acc_t& x, float unit)
+{
+    // 1 / unit of a power of two; 2^127 of 0, where x holds zeros or what is not finite
+    const float per_unit = __uint_as_float(0x7f000000u - __float_as_uint(unit));
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+        x[r] *= per_unit;
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------- queries' gradients
@@ -86,7 +143,10 @@ __global__ __launch_bounds__(grad_query_shape(sizeof(T), pitch_of(NB), FEW).thre
     constexpr int kPitch = pitch_of(NB);
     constexpr ForwardShape kShape = grad_query_shape(sizeof(T), kPitch, FEW);
     constexpr int kKeys = kShape.keys, kThreads = 64 * kShape.row_waves, kJoin = kShape.key_waves;
-    constexpr bool kUnits = std::is_same<T, _Float16>::value;
+    // Units of dS: sums of up to 128 features are scaled as the unit grows.  Those of more, for which that would cost registers
+    // in the loop (16 x 512 tokens, 2 heads of 256 on 1: 156 us for 119), have the unit of their first term's size, and
+    // where a later one is past its range, all is done once more with the unit of the largest.
+    constexpr bool kUnits = std::is_same<T, _Float16>::value, kOneUnit = kUnits && NB > 4;
     // FLOAT's products take so long that operands can come from memory as they are needed: the values of wider heads do,
     // which leaves LDS for the keys of four wavefronts, and gO of the widest, which leaves registers for the rest
     constexpr bool kDirect = grad_values_direct(sizeof(T), kPitch, FEW), kGradDirect = kDirect && NB > 4;
@@ -166,43 +226,32 @@ __global__ __launch_bounds__(grad_query_shape(sizeof(T), pitch_of(NB), FEW).thre
         }
     }
     // the row's statistics, left for the keys' gradients too
-    float lse, along, unit = 1.0f;
+    float lse, along;
     {
         const T* const out = (const T*)a.out.ptr + (int64_t)b * a.out.stride[0] + (int64_t)query * a.out.stride[1] +
                              (int64_t)head * a.out.stride[2];
-        float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f}, most = 0.0f;
+        float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < 2 * NB; i++) {
             const Frag<T> x = go(i), y = global_row<T, VEC>(out, 16 * i + 8 * h, d);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 sums[e % 4] += (float)x[e] * (float)y[e];
-                most = fmaxf(most, fabsf((float)x[e]));
             }
         }
         along = (sums[0] + sums[1]) + (sums[2] + sums[3]);
         along += other_half(along);
-        most = fmaxf(most, other_half(most));
         lse = ((const float*)a.lse.ptr)[(int64_t)b * a.lse.stride[0] + (int64_t)head * a.lse.stride[1] +
                                         (int64_t)query * a.lse.stride[2]];
         const bool live = query < seq.q_len && lse != -INFINITY;
         lse = live ? lse * kLog2e : INFINITY;
         along = live ? along : 0.0f;
-        if constexpr (kUnits) {
-            // 2^floor(log2 most) by its exponent bits; 0 for rows of zeros
-            const uint32_t bits = __float_as_uint(most) & 0x7f800000u;
-            unit = !live ? 0.0f : (bits == 0x7f800000u ? 1.0f : __uint_as_float(bits));
-        }
         if (key_wave == 0 && h == 0 && wave_row0 + own < p.rows) {
-            float* const stat = p.stats + stats_row(a, b, head) + query;
+            float* const stat = p.stats + stats_row(p, b, head) + query;
             stat[0] = lse;
-            stat[a.tokens] = along;
-            if constexpr (kUnits) {
-                stat[2 * a.tokens] = unit;
-            }
+            stat[p.stat_pitch] = along;
         }
     }
-    const float per_unit = unit > 0.0f ? 1.0f / unit : 0.0f;
     wait_for_registers();
     // as in the forward pass: 32 keys of a tile, those of tiles that all of the wavefront's rows see whole in a loop of their own
     const auto whole = [&](int t) {
@@ -215,6 +264,7 @@ __global__ __launch_bounds__(grad_query_shape(sizeof(T), pitch_of(NB), FEW).thre
                (key0 + kBlock - 1 < wave_low - left && key0 >= sinks);
     };
     bool careful = false;  // a second pass, for keys that are not finite
+    float unit = 0.0f, most = 0.0f, first_unit = 0.0f;
     const auto attend = [&](auto part, int key0, int end, const T* k_tile, const T* v_tile, const Rows32<T, kPitch, NB>& rows,
                             const Columns32<T, kPitch, NB>& columns) {
         acc_t s = zeros(), dp = zeros();
@@ -249,7 +299,7 @@ __global__ __launch_bounds__(grad_query_shape(sizeof(T), pitch_of(NB), FEW).thre
         }
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-            s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -lse)) * ((dp[r] - along) * per_unit);
+            s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -lse)) * (dp[r] - along);
         }
         if constexpr (decltype(part)::value) {
             const Sight see = sight(pos, key0 + 4 * h, end, left, right, sinks);
@@ -257,6 +307,16 @@ __global__ __launch_bounds__(grad_query_shape(sizeof(T), pitch_of(NB), FEW).thre
             for (int r = 0; r < 16; r++) {
                 s[r] = see.sees(8 * (r / 4) + r % 4) ? s[r] : 0.0f;
             }
+        }
+        if constexpr (kOneUnit) {
+            const float high = largest_term(s);
+            most = fmaxf(most, high);
+            unit = unit == 0.0f ? unit_of(high, 0) : unit;
+        } else if constexpr (kUnits) {
+            fit_unit(s, unit, gq);
+        }
+        if constexpr (kUnits) {
+            to_units(s, unit);
         }
         if (decltype(part)::value && __builtin_expect(careful, 0)) {
             const Sight see = sight(pos, key0 + 4 * h, end, left, right, sinks);
@@ -333,6 +393,7 @@ __global__ __launch_bounds__(grad_query_shape(sizeof(T), pitch_of(NB), FEW).thre
         for (int i = 0; i < NB; i++) {
             gq[i] = zeros();
         }
+        unit = first_unit;
         while (t < range.tiles) {
             {
                 const Rows32<T, kPitch, NB> rows(again(lane));
@@ -356,15 +417,28 @@ __global__ __launch_bounds__(grad_query_shape(sizeof(T), pitch_of(NB), FEW).thre
                 check = __builtin_fmaf(gq[i][r], 0.0f, check);
             }
         }
-        const bool odd = !careful && check != 0.0f;
-        if (!(kShape.row_waves > 1 ? __syncthreads_or(odd) : __any(odd))) {
+        const auto any_row = [&](bool x) { return kShape.row_waves > 1 ? __syncthreads_or(x) != 0 : __any(x) != 0; };
+        const bool past = most > unit * kMostUnits;
+        if (kOneUnit && any_row(past)) {
+            first_unit = past ? unit_of(most, 8) : unit;  // each row by its own terms alone
+        } else if (any_row(!careful && check != 0.0f)) {
+            careful = true;
+        } else {
             break;
         }
-        careful = true;
         t = key_wave;
         buffer = 0;
         if (t < range.tiles) {
             fetch(t, 0);
+        }
+    }
+    if constexpr (kUnits) {
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                gq[i][r] *= unit;
+            }
         }
     }
     if constexpr (kJoin > 1) {
@@ -398,7 +472,7 @@ __global__ __launch_bounds__(grad_query_shape(sizeof(T), pitch_of(NB), FEW).thre
     if (wave_row0 + own >= p.rows) {
         return;
     }
-    const float f = a.scale * unit;
+    const float f = a.scale;
     T* const to = (T*)a.grad_q.ptr + (int64_t)b * a.grad_q.stride[0] + (int64_t)query * a.grad_q.stride[1] +
                   (int64_t)head * a.grad_q.stride[2];
 #pragma unroll
@@ -435,7 +509,7 @@ attention_key_grad_kernel(GradLaunch p)
     constexpr int kPitch = pitch_of(NB), kThreads = 64 * kKeyWaves;
     constexpr int kStages = key_grad_stages(sizeof(T));
     constexpr bool kUnits = std::is_same<T, _Float16>::value;
-    constexpr int kStatRows = kUnits ? 4 : 2;  // of 32 floats each, a wavefront and stage
+    constexpr int kStatRows = 2;               // of 32 floats each, a wavefront and stage
     constexpr int kTile = kBlock * kPitch;     // elements
     constexpr bool kValuesInLds = key_grad_values_in_lds(sizeof(T)), kWithKeys = PASS != kValueGrad, kWithValues = PASS != kKeyGrad;
     extern __shared__ __align__(16) char lds[];
@@ -480,7 +554,7 @@ attention_key_grad_kernel(GradLaunch p)
     const int64_t head0 = (int64_t)kv_head * p.group.div;
     const T* const q_base = (const T*)a.q.ptr + (int64_t)b * a.q.stride[0] + head0 * a.q.stride[2];
     const T* const go_base = (const T*)a.grad_out.ptr + (int64_t)b * a.grad_out.stride[0] + head0 * a.grad_out.stride[2];
-    const float* const stat_base = p.stats + stats_row(a, b, head0);
+    const float* const stat_base = p.stats + stats_row(p, b, head0);
     // steps go through the tiles of one head's queries, then the next head's; `f_`: the step that is fetched next
     int f_head = s_begin < s_end ? s_begin / row_tiles : 0, f_query = low + (s_begin - f_head * row_tiles) * kBlock;
     int c_query = f_query;
@@ -493,17 +567,11 @@ attention_key_grad_kernel(GradLaunch p)
         stage<T, kPitch, kBlock, kThreads, VEC>(q_tile + kTile,
                                                 at_bytes(go_base + f_head * a.grad_out.stride[2], (uint32_t)f_query, go_pitch),
                                                 thread, wave, d, go_pitch, rows);
-        // statistics: lanes of the lower half read one kind, of the upper half the next; rows past the end read zeros,
+        // statistics: lanes of the lower half read one kind, of the upper half the other; rows past the end read zeros,
         // which meet rows of zeros
-        const rsrc_t rsrc = att::buffer(stat_base + f_head * (3 * a.tokens) + f_query, 0x7fffffffu);
-        const uint32_t to = lds_place(stat_ring + buffer * (kStatRows * kBlock));
-        const auto stat_offset = [&](int kind) {
-            return (own < rows && kind < 3) ? (uint32_t)(kind * (int)a.tokens + own) * 4u : kOutside;
-        };
-        load_to_lds<4, 0>(rsrc, to, stat_offset(h));
-        if constexpr (kUnits) {
-            load_to_lds<4, 2 * kBlock * 4>(rsrc, to, stat_offset(2 + h));
-        }
+        const rsrc_t rsrc = att::buffer(stat_base + f_head * (2 * p.stat_pitch) + f_query, 0x7fffffffu);
+        load_to_lds<4, 0>(rsrc, lds_place(stat_ring + buffer * (kStatRows * kBlock)),
+                          own < rows ? (uint32_t)(h * (int)p.stat_pitch + own) * 4u : kOutside);
         f_query += kBlock;
         if (f_query >= high) {
             f_query = low;
@@ -518,7 +586,7 @@ attention_key_grad_kernel(GradLaunch p)
         gk[i] = zeros();
         gv[i] = zeros();
     }
-    float unit = 0.0f, per_unit = kUnits ? 0.0f : 1.0f;
+    float unit = 0.0f;
     int buffer = 0;
     if (s_begin < s_end) {
         fetch(0);
@@ -563,25 +631,6 @@ attention_key_grad_kernel(GradLaunch p)
         const bool all_seen = wave_key0 + kBlock <= seq.kv_len && wave_key0 + kBlock - 1 <= p_low + right &&
                               (wave_key0 >= p_high - left || wave_key0 + kBlock <= sinks);
         if (any) {
-            if constexpr (kUnits && kWithKeys) {
-                float most = stat[2 * kBlock + own];
-#pragma unroll
-                for (int w = 16; w > 0; w >>= 1) {
-                    most = fmaxf(most, __shfl_xor(most, w, 64));
-                }
-                if (__any(most > unit)) {
-                    const float fade = unit / most;
-#pragma unroll
-                    for (int i = 0; i < NB; i++) {
-#pragma unroll
-                        for (int r = 0; r < 16; r++) {
-                            gk[i][r] *= fade;
-                        }
-                    }
-                    unit = most;
-                    per_unit = 1.0f / most;
-                }
-            }
             acc_t s = zeros(), dp = zeros();
             const Rows32<T, kPitch, NB> rows(again(lane));
 #pragma unroll
@@ -610,7 +659,7 @@ attention_key_grad_kernel(GradLaunch p)
                 const int n = 8 * (r / 4) + 4 * h + r % 4;
                 s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -stat[n]));
                 if constexpr (kWithKeys) {
-                    dp[r] = s[r] * ((dp[r] - stat[kBlock + n]) * per_unit);
+                    dp[r] = s[r] * (dp[r] - stat[kBlock + n]);
                 }
             }
             if (__builtin_expect(!all_seen, 0)) {
@@ -624,6 +673,10 @@ attention_key_grad_kernel(GradLaunch p)
                     s[r] = seen ? s[r] : 0.0f;
                     dp[r] = seen ? dp[r] : 0.0f;
                 }
+            }
+            if constexpr (kUnits && kWithKeys) {
+                fit_unit(dp, unit, gk);
+                to_units(dp, unit);
             }
             const Columns32<T, kPitch, NB> columns(again(lane));
 #pragma unroll
@@ -764,7 +817,7 @@ hipError_t launch_key_grad(const GradLaunch& p, hipStream_t stream)
     constexpr int kPitch = pitch_of(NB);
     constexpr int kStages = key_grad_stages(sizeof(T)), kWaves = grad_key_waves(sizeof(T) == 4, NB);
     constexpr int kBytes = kStages * 2 * kBlock * kPitch * (int)sizeof(T) +
-                           kWaves * kStages * (std::is_same<T, _Float16>::value ? 4 : 2) * kBlock * 4 +
+                           kWaves * kStages * 2 * kBlock * 4 +
                            (key_grad_values_in_lds(sizeof(T)) ? kWaves * kBlock * kPitch * (int)sizeof(T) : 0);
     static_assert(kBytes <= 160 * 1024, "LDS of a CU");
     static std::atomic<uint32_t> done{0};
@@ -812,7 +865,7 @@ hipError_t run_backward(const AttentionArgs& a, hipStream_t stream)
     const int64_t quads = (a.d + 3) / 4;
     const int64_t sink_joins = plan.sink_parts > 1 ? bh * plan.sink_tiles * 2 * plan.keys * quads : 0;
     const int64_t joins = plan.parts > 1 ? bh * (plan.key_tiles - plan.sink_tiles) * 2 * plan.keys * quads : 0;
-    // 3 * tokens * 4 bytes of statistics are reached with 32-bit offsets
+    // two rows of statistics are reached with 32-bit offsets
     if (query_blocks > INT32_MAX / 1024 || key_blocks > INT32_MAX / 1024 || stat_rows > INT32_MAX / 16 ||
         a.tokens > INT32_MAX / 12 || sink_joins + joins > INT32_MAX ||
         (a.scratch == nullptr && plan.stats > 0)) {
@@ -831,8 +884,9 @@ hipError_t run_backward(const AttentionArgs& a, hipStream_t stream)
     p.parts = (uint32_t)plan.parts;
     p.query_blocks = (uint32_t)query_blocks;
     p.key_blocks = (uint32_t)key_blocks;
+    p.stat_pitch = plan.stat_pitch;
     p.stats = a.scratch;
-    p.sink_partials = a.scratch + (plan.stats + 3) / 4 * 4;
+    p.sink_partials = a.scratch + plan.stats;
     p.partials = p.sink_partials + plan.sink_partials;
     hipError_t e = hipErrorInvalidValue;
     switch (blocks_of(a.d)) {

@@ -110,7 +110,7 @@ struct GradPlan {
     int64_t sink_tiles = 0;            // the first of them, seen by queries of any position
     int64_t sink_parts = 1, parts = 1; // parts that the queries of such a tile, and of the others, are cut into at most
     // 32-bit words of the scratch: statistics of the rows, partial gradients of the sinks' tiles and of the others
-    int64_t stats = 0, sink_partials = 0, partials = 0;
+    int64_t stat_pitch = 0, stats = 0, sink_partials = 0, partials = 0;
 };
 
 inline GradPlan plan_grad(const AttentionArgs& a)
@@ -158,7 +158,8 @@ inline GradPlan plan_grad(const AttentionArgs& a)
     p.sink_parts = (sink_steps + low - 1) / low;
     p.parts = p.parts < 1 ? 1 : p.parts;
     p.sink_parts = p.sink_parts < 1 ? 1 : p.sink_parts;
-    p.stats = 3 * a.batch * a.heads * a.tokens;
+    p.stat_pitch = (a.tokens + 15) / 16 * 16;  // rows of statistics begin on lines of 64 bytes
+    p.stats = 2 * a.batch * a.heads * p.stat_pitch;
     const int64_t tile_floats = 2 * p.keys * ((a.d + 3) / 4 * 4);
     p.sink_partials = p.sink_parts > 1 ? bh * p.sink_tiles * p.sink_parts * tile_floats : 0;
     p.partials = p.parts > 1 ? bh * (p.key_tiles - p.sink_tiles) * p.parts * tile_floats : 0;

@@ -1,0 +1,103 @@
+"""The operators on token sequences at the ends of their types' ranges, against plain implementations in 64 bits."""
+import math
+
+import pytest
+import torch
+
+import token_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+NONE = 2 ** 63 - 1
+
+
+def gen(*key):
+    return torch.Generator().manual_seed(sum((i + 1) * ord(c) for i, c in enumerate(str(key))))
+
+
+def normal(g, *size, dtype="fp16", scale=1.0):
+    return (torch.randn(*size, generator=g, dtype=torch.float64) * scale).to(O.DTYPES[dtype])
+
+
+# -------------------------------------------------------------------------------- gradients of attention in FLOAT16
+
+def gradient_bounds(r, q, k, v, go, scale, dtype):
+    """How far the gradients may be, entry by entry.
+
+    off_ij, the error of the scores' gradient gs_ij = w_ij (go_i . v_j - D_i) as an operand of the products that follow: it is
+    rounded to the type (relative U); the weight and the two terms of the difference carry 32-bit errors (F32), D_i the
+    rounding of `out` (U).  FLOAT16 has 2^-25 of absolute error on top, of whatever the largest operand is divided by: a row's
+    own largest where rows are summed up (gq), a key's own largest where keys are (gk).  Weights as operands (gv): relative U,
+    and nothing absolute that would show, since no weight exceeds 1 and the products have 32 bits."""
+    u, tiny = O.U[dtype], O.TINY[dtype]
+    group = q.shape[2] // k.shape[2]
+    spread = lambda x: x.double().abs().repeat_interleave(group, 2).transpose(1, 2)  # noqa: E731
+    gather = lambda x: x.transpose(1, 2).unflatten(2, (k.shape[2], group)).sum(3)  # noqa: E731
+    w, gs = r["weights"], r["gs"].abs()
+    vs, ks, qs = spread(v), spread(k), q.double().abs().transpose(1, 2)
+    g = go.double().abs().transpose(1, 2)
+    along = (g * r["out"].abs().transpose(1, 2)).sum(-1, keepdim=True)
+    off = gs * (u + O.F32) + w * (g @ vs.transpose(2, 3) + along) * O.F32 + w * along * u
+    low = 2.0 ** -25 if dtype == "fp16" else 0.0
+    off_row = off + low * gs.amax(3, keepdim=True) * (w > 0)
+    # a key's gradient is one sum over the rows of all the heads that share it
+    most = gs.amax(2, keepdim=True).unflatten(1, (-1, group)).amax(2, keepdim=True).expand(-1, -1, group, -1, -1).flatten(1, 2)
+    off_key = off + low * most * (w > 0)
+    return ((off_row @ ks * scale).transpose(1, 2) + u * r["gq"].abs() + tiny,
+            gather(off_key.transpose(2, 3) @ qs) * scale + u * r["gk"].abs() + tiny,
+            gather((w * (u + O.F32)).transpose(2, 3) @ g) + u * r["gv"].abs() + tiny)
+
+
+def check_gradients(device, aclnn, q, k, v, go, dtype, which=("gq", "gk", "gv"), **masks):
+    r = O.attention(q, k, v, grad_out=go, **masks)
+    bounds = gradient_bounds(r, q, k, v, go, masks["scale"], dtype)
+    dev = [t.to(device) for t in (go, q, k, v, r["out"].to(q.dtype), r["lse"].float())]
+    got = aclnn.window_attention_backward(*dev, **masks)
+    for name, x, bound in zip(("gq", "gk", "gv"), got, bounds):
+        assert r[name].abs().max() < 65000  # the results themselves are numbers of the type
+        if name in which:
+            O.within(x, r[name], bound, name)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("b,sq,d", [(1, 40, 64), (1, 40, 128), (1, 70, 256), (2, 300, 80), (130, 140, 32)])
+def test_gradients_of_large_values(device, aclnn, dtype, b, sq, d):
+    """Two keys a query, whose values differ by what makes the score's gradient, over the size of gradOut, pass 65504."""
+    g = gen("large values", dtype, b, sq, d)
+    q, k = normal(g, b, sq, 4, d, dtype=dtype, scale=0.1), normal(g, b, sq, 2, d, dtype=dtype)
+    sign = torch.ones(sq).double()
+    sign[::2] = -1
+    size = 1.1 * 2 * 65504 / d
+    v = (size * sign[None, :, None, None] * (1 + 0.01 * torch.randn(b, sq, 2, d, generator=g, dtype=torch.float64))).to(O.DTYPES[dtype])
+    go = torch.full(q.shape, 2.0 ** -10, dtype=q.dtype)
+    check_gradients(device, aclnn, q, k, v, go, dtype, scale=0.1, left=1, right=0, sinks=0)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("b,sq,heads,d,left", [(1, 300, 1, 64, 100), (2, 200, 4, 128, NONE), (70, 260, 4, 64, 100), (1, 150, 2, 256, 60)])
+def test_gradients_beside_loud_rows(device, aclnn, dtype, b, sq, heads, d, left):
+    """Every eighth query has a gradient 1e5 times as large as the others', and looks at its own key alone: what the other
+    queries leave in the other keys keeps its bits."""
+    g = gen("loud rows", dtype, b, sq, heads, d)
+    q, k = normal(g, b, sq, heads, d, dtype=dtype, scale=0.1), normal(g, b, sq, 1, d, dtype=dtype)
+    v = normal(g, b, sq, 1, d, dtype=dtype)
+    go = normal(g, b, sq, heads, d, dtype=dtype, scale=0.3)
+    loud = torch.arange(sq) % 8 == 3
+    scale = 1 / math.sqrt(d)
+    q[:, loud] = (k[:, loud] * (30 / math.sqrt(d))).expand(-1, -1, heads, -1)  # a score of 30 or so with its own key
+    go[:, loud] = go[:, loud] * 2e4
+    check_gradients(device, aclnn, q, k, v, go, dtype, ("gq", "gk"), scale=scale, left=left, right=0, sinks=0)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("b,sq,heads,d", [(1, 300, 1, 64), (2, 200, 4, 128), (70, 260, 4, 32), (1, 150, 2, 256), (70, 260, 4, 160)])
+def test_gradients_that_grow_along_the_row(device, aclnn, dtype, b, sq, heads, d):
+    """Every other query looks at its own key and the one before it, past many that have a millionth of their weight or less:
+    the gradients of its first scores are a million times smaller than those of its last ones."""
+    g = gen("growing", dtype, b, sq, heads, d)
+    k, v = normal(g, b, sq, 1, d, dtype=dtype), normal(g, b, sq, 1, d, dtype=dtype)
+    q = normal(g, b, sq, heads, d, dtype=dtype, scale=0.1)
+    pair = (k.double() + k.double().roll(1, 1)) * (20 / math.sqrt(d))
+    q[:, ::2] = pair[:, ::2].expand(-1, -1, heads, -1).to(q.dtype)
+    go = normal(g, b, sq, heads, d, dtype=dtype)
+    check_gradients(device, aclnn, q, k, v, go, dtype, ("gq", "gk"), scale=1 / math.sqrt(d), left=NONE, right=0, sinks=0)
