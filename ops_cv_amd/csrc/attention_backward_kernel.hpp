@@ -20,7 +20,8 @@
 // dS of FLOAT16 may be anything from P of a long row times a small gradient, for which FLOAT16 has few bits or none, to the
 // products of large gradients and values, which are past its end.  So every sum's dS (of a row in the queries' kernel, of a
 // key in the keys') is divided before it is rounded by a power of two that follows the largest |dS| met so far, and the sum
-// multiplied by it (fit_unit).
+// multiplied by it (fit_unit).  P of the keys' kernel is never more than 1 and enters its products 2^14 times as large, so that
+// it has its bits down to 2^-28, below which nothing that it is multiplied with makes more than FLOAT16's smallest numbers.
 #pragma once
 
 #include <atomic>
@@ -41,10 +42,14 @@ struct GradLaunch {
     uint32_t keys, key_tiles, sink_tiles, sink_parts, parts;
     uint32_t query_blocks, key_blocks;
     int64_t stat_pitch;
-    float* stats;          // (batch, heads, 2, stat_pitch)
+    float* stats;          // (batch, heads, 2, stat_pitch): lse log2 e - kWeightGain, and D
     float* sink_partials;  // (batch * kv_heads, sink_tiles, sink_parts, 2, keys, d rounded up to four)
     float* partials;       // the same of the other tiles
 };
+
+// binary logarithm of the factor that P of the keys' kernel has
+template <typename T>
+constexpr float kWeightGain = std::is_same<T, _Float16>::value ? 14.0f : 0.0f;
 
 static __device__ __forceinline__ int64_t stats_row(const GradLaunch& p, int64_t b, int64_t head)
 {
@@ -248,7 +253,7 @@ __global__ __launch_bounds__(grad_query_shape(sizeof(T), pitch_of(NB), FEW).thre
         along = live ? along : 0.0f;
         if (key_wave == 0 && h == 0 && wave_row0 + own < p.rows) {
             float* const stat = p.stats + stats_row(p, b, head) + query;
-            stat[0] = lse;
+            stat[0] = lse - kWeightGain<T>;
             stat[p.stat_pitch] = along;
         }
     }
@@ -702,7 +707,18 @@ attention_key_grad_kernel(GradLaunch p)
         }
         buffer ^= kStages - 1;
     }
-    const float f = a.scale * (kUnits ? unit : 1.0f);
+    float f = a.scale;
+    if constexpr (kUnits) {
+        constexpr float kGain = 1.0f / (1 << (int)kWeightGain<T>);
+        f *= unit * kGain;
+#pragma unroll
+        for (int i = 0; i < (kWithValues ? NB : 0); i++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                gv[i][r] *= kGain;
+            }
+        }
+    }
     if (of > 1) {
         const int64_t tile_index = sink_tile ? (int64_t)bh * p.sink_tiles + local_tile
                                              : (int64_t)bh * (p.key_tiles - p.sink_tiles) + local_tile;

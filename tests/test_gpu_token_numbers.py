@@ -75,7 +75,8 @@ def test_gradients_of_large_values(device, aclnn, dtype, b, sq, d):
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 @pytest.mark.parametrize("b,sq,heads,d,left", [(1, 300, 1, 64, 100), (2, 200, 4, 128, NONE), (70, 260, 4, 64, 100), (1, 150, 2, 256, 60)])
-def test_gradients_beside_loud_rows(device, aclnn, dtype, b, sq, heads, d, left):
+@pytest.mark.parametrize("which", [("gq", "gk"), ("gv",)], ids=["scores", "values"])
+def test_gradients_beside_loud_rows(device, aclnn, dtype, b, sq, heads, d, left, which):
     """Every eighth query has a gradient 1e5 times as large as the others', and looks at its own key alone: what the other
     queries leave in the other keys keeps its bits."""
     g = gen("loud rows", dtype, b, sq, heads, d)
@@ -86,7 +87,7 @@ def test_gradients_beside_loud_rows(device, aclnn, dtype, b, sq, heads, d, left)
     scale = 1 / math.sqrt(d)
     q[:, loud] = (k[:, loud] * (30 / math.sqrt(d))).expand(-1, -1, heads, -1)  # a score of 30 or so with its own key
     go[:, loud] = go[:, loud] * 2e4
-    check_gradients(device, aclnn, q, k, v, go, dtype, ("gq", "gk"), scale=scale, left=left, right=0, sinks=0)
+    check_gradients(device, aclnn, q, k, v, go, dtype, which, scale=scale, left=left, right=0, sinks=0)
 
 
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
@@ -101,3 +102,14 @@ def test_gradients_that_grow_along_the_row(device, aclnn, dtype, b, sq, heads, d
     q[:, ::2] = pair[:, ::2].expand(-1, -1, heads, -1).to(q.dtype)
     go = normal(g, b, sq, heads, d, dtype=dtype)
     check_gradients(device, aclnn, q, k, v, go, dtype, ("gq", "gk"), scale=1 / math.sqrt(d), left=NONE, right=0, sinks=0)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("keys", [5000, 104531])
+def test_value_gradients_of_small_weights(device, aclnn, dtype, keys):
+    """Queries that weigh all keys alike: 1 / keys has its bits also below the normal numbers of FLOAT16."""
+    g = gen("small weights", dtype, keys)
+    q = torch.zeros(1, 2, 1, 64, dtype=O.DTYPES[dtype])
+    k, v = normal(g, 1, keys, 1, 64, dtype=dtype), normal(g, 1, keys, 1, 64, dtype=dtype)
+    go = normal(g, 1, 2, 1, 64, dtype=dtype, scale=3000)
+    check_gradients(device, aclnn, q, k, v, go, dtype, scale=0.125, left=NONE, right=NONE, sinks=0)
