@@ -142,6 +142,9 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
     // Scores are taken relative to `base`, a score of the row: not its largest, but at most kSlack (in powers of two) below,
     // so that sums seldom have to be scaled again.  -infinity: the row has seen nothing.
     constexpr float kSlack = 8.0f;
+    // Weights of FLOAT16 are 2^7 times as large, and so at most 2^15: those of 2^-21 of the largest still have all their bits,
+    // for long rows of which a few keys take the most.
+    constexpr float kGain = std::is_same<T, _Float16>::value ? 7.0f : 0.0f;
     float base, total;  // `total`: of this lane's keys only
     acc_t o[NB];
 
@@ -222,7 +225,7 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
             }
             base = now;
         }
-        const float from = base == -INFINITY ? 0.0f : base;  // exp2(-inf - 0) = 0
+        const float from = base == -INFINITY ? 0.0f : base - kGain;  // exp2(-inf - 0) = 0
         Frag<T> w[2 * SUBS];
         float sums[4] = {total, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -345,6 +348,7 @@ __global__ __launch_bounds__(forward_shape(sizeof(T), pitch_of(NB), FEW).threads
         }
     }
     total += other_half(total);
+    base -= kGain;  // what the sums are relative to
 
     // join the wavefronts that shared the keys: every one leaves its sums in LDS, [feature][row], and takes a share of
     // the features for all of them

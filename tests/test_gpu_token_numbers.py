@@ -113,3 +113,28 @@ def test_value_gradients_of_small_weights(device, aclnn, dtype, keys):
     k, v = normal(g, 1, keys, 1, 64, dtype=dtype), normal(g, 1, keys, 1, 64, dtype=dtype)
     go = normal(g, 1, 2, 1, 64, dtype=dtype, scale=3000)
     check_gradients(device, aclnn, q, k, v, go, dtype, scale=0.125, left=NONE, right=NONE, sinks=0)
+
+
+# ------------------------------------------------------------------------------------------------- forward, weights
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("sq", [1, 16384])
+def test_many_small_weights_beside_a_large_one(device, aclnn, dtype, sq):
+    """A first token that takes most of the weight, and a quarter of a million others that share the rest: each has a
+    millionth of the largest weight, and they add up to a fifth of the whole.  All queries are the same one."""
+    g = gen("small", dtype)
+    n, d = 262144, 64
+    q, k = torch.zeros(1, 1, 2, d, dtype=O.DTYPES[dtype]), torch.zeros(1, n, 1, d, dtype=O.DTYPES[dtype])
+    q[..., 0], k[:, 0, :, 0] = 1, 14
+    v = (3 + 0.1 * torch.randn(1, n, 1, d, generator=g, dtype=torch.float64)).to(O.DTYPES[dtype])
+    v[:, 0] = 0
+    # exp(-13.8352) is 16.45 steps of FLOAT16's smallest numbers
+    masks = dict(scale=13.8352 / 14, left=NONE, right=NONE, sinks=0)
+    out, lse = aclnn.window_attention(q.expand(1, sq, 2, d).to(device), k.to(device), v.to(device), need_lse=True, **masks)
+    want = O.attention(q, k, v, **masks)
+    # weights are rounded to the type (relative U); a running sum of the weights takes up to nine additions for 64 keys and
+    # one of the weighted values one for 16, each of which rounds by 2^-24 of the sum
+    sums = (n / 64 * 9 + n / 16) * 2.0 ** -24
+    u = O.U[dtype]
+    O.within(out, want["out"].expand(1, sq, 2, d), (2 * u + sums) * want["out"].abs(), "out")
+    O.within(lse, want["lse"].expand(1, 2, sq), sums + 1e-5, "lse")
