@@ -62,9 +62,24 @@ __device__ __forceinline__ void row_reduce(float& sum, float* most, float (*shar
     }
 }
 
+// How a row's products become 8-bit numbers: q = round((t * lift) * step).
+struct Int8Steps {
+    float lift, step;
+};
+
+// 127 / m is no number of 32 bits where m is less than 3.7e-37; there both are taken 2^64 times as large, which rounds nothing.
+// step 0, and scale NaN, where the row holds a NaN or an infinity.
+__device__ __forceinline__ Int8Steps int8_steps(float most, float rstd, float* scale)
+{
+    const bool finite = most < INFINITY;  // false for NaN too
+    *scale = finite ? most * rstd / 127.0f : NAN;
+    const float lift = most < 0x1p-100f ? 0x1p64f : 1.0f;
+    return {lift, (finite && most > 0.0f) ? 127.0f / (most * lift) : 0.0f};
+}
+
 template <typename T, typename W, bool INT8, int VEC, bool WIDE>
 __device__ __forceinline__ void put_row_part(const NormArgs& a, int64_t row, int64_t c, const float (&h)[VEC], float rstd,
-                                             float step)
+                                             Int8Steps steps)
 {
     float w[VEC], y[VEC];
     load_part<W, VEC, WIDE>((const W*)a.weight, c, a.width, w);
@@ -73,8 +88,8 @@ __device__ __forceinline__ void put_row_part(const NormArgs& a, int64_t row, int
 #pragma unroll
         for (int i = 0; i < VEC; i++) {
             // step is 0 for rows without a finite range; |t * step| is at most 127 and a rounding
-            const float q = rintf(h[i] * w[i] * step);
-            k.v[i] = step == 0.0f ? (int8_t)0 : (int8_t)(int)fminf(fmaxf(q, -127.0f), 127.0f);
+            const float q = rintf(h[i] * w[i] * steps.lift * steps.step);
+            k.v[i] = steps.step == 0.0f ? (int8_t)0 : (int8_t)(int)fminf(fmaxf(q, -127.0f), 127.0f);
         }
         int8_t* const to = (int8_t*)a.y.ptr + row * a.y.row_stride + c;
         if constexpr (WIDE) {
@@ -108,14 +123,6 @@ __device__ __forceinline__ void get_row_part(const NormArgs& a, int64_t row, int
             h[i] += r[i];
         }
     }
-}
-
-// step of the 8-bit numbers and what a row's scale is; 0 and NaN where the row holds a NaN or an infinity
-__device__ __forceinline__ float int8_step(float most, float rstd, float* scale)
-{
-    const bool finite = most < INFINITY;  // false for NaN too
-    *scale = finite ? most * rstd / 127.0f : NAN;
-    return (finite && most > 0.0f) ? 127.0f / most : 0.0f;
 }
 
 // THREADS per row; a workgroup is 256 threads, or THREADS where that is more.  NV vectors of VEC elements a thread.
@@ -167,7 +174,7 @@ __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void norm_kernel(Nor
         slot ^= 1;
         const float rstd = 1.0f / sqrtf(sum / (float)a.width + a.eps);
         float scale = 0.0f;
-        const float step = INT8 ? int8_step(most, rstd, &scale) : 0.0f;
+        const Int8Steps steps = INT8 ? int8_steps(most, rstd, &scale) : Int8Steps{};
         if (lane == 0) {
             if (a.rstd != nullptr) {
                 a.rstd[row] = rstd;
@@ -180,7 +187,7 @@ __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void norm_kernel(Nor
         for (int j = 0; j < NV; j++) {
             const int64_t c = ((int64_t)j * THREADS + lane) * VEC;
             if (c < a.width) {
-                put_row_part<T, W, INT8, VEC, WIDE>(a, row, c, h[j], rstd, step);
+                put_row_part<T, W, INT8, VEC, WIDE>(a, row, c, h[j], rstd, steps);
             }
         }
     }
@@ -209,7 +216,7 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a)
     slot ^= 1;
     const float rstd = 1.0f / sqrtf(sum / (float)a.width + a.eps);
     float scale = 0.0f;
-    const float step = INT8 ? int8_step(most, rstd, &scale) : 0.0f;
+    const Int8Steps steps = INT8 ? int8_steps(most, rstd, &scale) : Int8Steps{};
     if (threadIdx.x == 0) {
         if (a.rstd != nullptr) {
             a.rstd[row] = rstd;
@@ -224,7 +231,7 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a)
         if (a.sum.ptr != nullptr) {
             store_part<T, VEC, WIDE>((T*)a.sum.ptr + row * a.sum.row_stride, c, a.width, h, a.streaming != 0);
         }
-        put_row_part<T, W, INT8, VEC, WIDE>(a, row, c, h, rstd, step);
+        put_row_part<T, W, INT8, VEC, WIDE>(a, row, c, h, rstd, steps);
     }
     }
 }

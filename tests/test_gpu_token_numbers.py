@@ -138,3 +138,25 @@ def test_many_small_weights_beside_a_large_one(device, aclnn, dtype, sq):
     u = O.U[dtype]
     O.within(out, want["out"].expand(1, sq, 2, d), (2 * u + sums) * want["out"].abs(), "out")
     O.within(lse, want["lse"].expand(1, 2, sq), sums + 1e-5, "lse")
+
+
+# ------------------------------------------------------------------------------------------------------ 8-bit norm
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("width", [8, 100, 2048, 40000])
+def test_8_bit_norm_of_tiny_rows(device, aclnn, dtype, width):
+    """Rows whose largest product is too small for 127 / m to be a number of 32 bits: m below 3.7e-37."""
+    x = torch.zeros(6, width, dtype=O.DTYPES[dtype])
+    x[0, :4] = torch.tensor([1e-38, 0.0, 5.1e-39, -2.3e-39])
+    x[1, :4] = torch.tensor([-3e-37, 1e-37, 0.0, 2e-38])
+    x[2, 1], x[3, 0] = 1e-40, 3.8e-37
+    x[4, :3] = torch.tensor([1.0, 1e-38, 0.0])
+    w = torch.ones(width, dtype=O.DTYPES[dtype])
+    q, scale, _, _ = aclnn.residual_norm_int8(x.to(device), w.to(device))
+    t = x.double()
+    most = t.abs().amax(1, keepdim=True)
+    want = torch.where(most > 0, t * 127 / torch.where(most > 0, most, 1), 0)
+    assert ((want - want.floor()) - 0.5).abs().min() > 1e-3  # no ties
+    assert torch.equal(q.cpu().double(), want.round())
+    rstd = 1 / torch.sqrt(t.square().mean(1) + 1e-6)
+    O.within(scale, most[:, 0] * rstd / 127, O.F32 * most[:, 0] * rstd / 127 + 2.0 ** -149, "scale")
