@@ -68,11 +68,12 @@ struct Int8Steps {
 };
 
 // 127 / m is no number of 32 bits where m is less than 3.7e-37; there both are taken 2^64 times as large, which rounds nothing.
-// step 0, and scale NaN, where the row holds a NaN or an infinity.
+// step 0 for a row of zeros, whose scale is 0 also where eps is and rstd infinite, and, with scale NaN, where the row holds a
+// NaN or an infinity.
 __device__ __forceinline__ Int8Steps int8_steps(float most, float rstd, float* scale)
 {
     const bool finite = most < INFINITY;  // false for NaN too
-    *scale = finite ? most * rstd / 127.0f : NAN;
+    *scale = !finite ? NAN : most > 0.0f ? most * rstd / 127.0f : 0.0f;
     const float lift = most < 0x1p-100f ? 0x1p64f : 1.0f;
     return {lift, (finite && most > 0.0f) ? 127.0f / (most * lift) : 0.0f};
 }

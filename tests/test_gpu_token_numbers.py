@@ -160,3 +160,12 @@ def test_8_bit_norm_of_tiny_rows(device, aclnn, dtype, width):
     assert torch.equal(q.cpu().double(), want.round())
     rstd = 1 / torch.sqrt(t.square().mean(1) + 1e-6)
     O.within(scale, most[:, 0] * rstd / 127, O.F32 * most[:, 0] * rstd / 127 + 2.0 ** -149, "scale")
+
+
+def test_8_bit_norm_of_zeros_without_eps(device, aclnn):
+    for width in (16, 40000):
+        x, w = torch.zeros(3, width), torch.ones(width)
+        x[1] = 2
+        q, scale, _, _ = aclnn.residual_norm_int8(x.to(device), w.to(device), eps=0.0)
+        assert (q[0] == 0).all() and (q[1] == 127).all() and (q[2] == 0).all()
+        assert scale[0] == 0 and scale[2] == 0 and abs(scale[1].item() - 1 / 127) < 1e-7
