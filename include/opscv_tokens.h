@@ -115,6 +115,9 @@ ACLNN_API aclnnStatus opscvRotary(void* workspace, uint64_t workspaceSize, aclOp
  *       infinity where nothing is seen
  *   left, right, sinks >= 0 (right = 0: causal; left = INT64_MAX: no window), scale > 0 and finite.
  * Prompts (many queries), chunks on a cache and single tokens take the same call.
+ *   sizes : up to 2^28 tokens and kvTokens, 2^30 rows (tokens * heads) of a sequence, 2^31 - 1 batch * heads.  A sequence
+ *       whose workgroups one launch does not hold is refused (161002): FLOAT over 2^29 rows of a key head, and, in the
+ *       gradients, kvTokens * kvHeads from 2^31 on.  Batches of any size take as many launches as they need.
  */
 ACLNN_API aclnnStatus opscvWindowAttentionGetWorkspaceSize(const aclTensor* query, const aclTensor* key,
                                                            const aclTensor* value, const aclTensor* qLengths,

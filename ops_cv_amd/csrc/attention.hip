@@ -24,6 +24,31 @@ bool vectors(const AttentionArgs& a, const S&... operands)
     return fits;
 }
 
+// run(a, plan, vectors, stream) for every launch of the call
+template <typename Plan, typename Run>
+hipError_t run_launches(const AttentionArgs& a, Plan&& plan_of, bool fits, Run&& run, hipStream_t stream)
+{
+    hipError_t e = hipSuccess;
+    int64_t done = 0;
+    att::by_launches(a, plan_of, [&](const AttentionArgs& s, const auto& plan) {
+        e = e == hipSuccess ? run(s, plan, fits, stream) : e;
+        done += s.batch;
+    });
+    return done == a.batch ? e : hipErrorInvalidValue;
+}
+
+// the most that floats(a, plan) is over the launches of the call; -1 where not one sequence fits a launch
+template <typename Plan, typename Floats>
+int64_t most_scratch(const AttentionArgs& a, Plan&& plan_of, Floats&& floats)
+{
+    int64_t most = -1;
+    att::by_launches(a, plan_of, [&](const AttentionArgs& s, const auto& plan) {
+        const int64_t n = plan.fits ? floats(s, plan) : -1;
+        most = n > most ? n : most;
+    });
+    return most;
+}
+
 }  // namespace
 
 hipError_t launch_window_attention(const AttentionArgs& a, hipStream_t stream)
@@ -31,18 +56,17 @@ hipError_t launch_window_attention(const AttentionArgs& a, hipStream_t stream)
     if (a.batch < 1 || a.tokens < 1 || a.kv_heads < 1 || a.heads % a.kv_heads != 0 || a.d < 1 || a.d > 256) {
         return hipErrorInvalidValue;
     }
-    const bool fits = vectors(a, a.q, a.k, a.v, a.out);
-    switch ((Elem)a.elem) {
-        case Elem::F32: return run_attention_f32(a, fits, stream);
-        case Elem::F16: return run_attention_f16(a, fits, stream);
-        default: return run_attention_bf16(a, fits, stream);
-    }
+    const auto run = a.elem == (int)Elem::F32   ? run_attention_f32
+                     : a.elem == (int)Elem::F16 ? run_attention_f16
+                                                : run_attention_bf16;
+    return run_launches(a, att::plan_forward, vectors(a, a.q, a.k, a.v, a.out), run, stream);
 }
 
 int64_t attention_scratch_floats(const AttentionArgs& a)
 {
-    const att::ForwardPlan p = att::plan_forward(a);
-    return p.splits > 1 ? a.batch * a.kv_heads * p.splits * p.rows * att::partial_floats(a.d) : 0;
+    return most_scratch(a, att::plan_forward, [](const AttentionArgs& s, const att::ForwardPlan& p) {
+        return p.splits > 1 ? s.batch * s.kv_heads * p.splits * p.rows * att::partial_floats(s.d) : 0;
+    });
 }
 
 hipError_t launch_window_attention_grad(const AttentionArgs& a, hipStream_t stream)
@@ -50,18 +74,18 @@ hipError_t launch_window_attention_grad(const AttentionArgs& a, hipStream_t stre
     if (a.batch < 1 || a.kv_heads < 1 || a.heads % a.kv_heads != 0 || a.d < 1 || a.d > 256) {
         return hipErrorInvalidValue;
     }
-    const bool fits = vectors(a, a.q, a.k, a.v, a.out, a.grad_out, a.grad_q, a.grad_k, a.grad_v);
-    switch ((Elem)a.elem) {
-        case Elem::F32: return run_attention_grad_f32(a, fits, stream);
-        case Elem::F16: return run_attention_grad_f16(a, fits, stream);
-        default: return run_attention_grad_bf16(a, fits, stream);
-    }
+    const auto run = a.elem == (int)Elem::F32   ? run_attention_grad_f32
+                     : a.elem == (int)Elem::F16 ? run_attention_grad_f16
+                                                : run_attention_grad_bf16;
+    return run_launches(a, att::plan_grad, vectors(a, a.q, a.k, a.v, a.out, a.grad_out, a.grad_q, a.grad_k, a.grad_v), run,
+                        stream);
 }
 
 int64_t attention_grad_scratch_floats(const AttentionArgs& a)
 {
-    const att::GradPlan p = att::plan_grad(a);
-    return p.stats + p.sink_partials + p.partials;
+    return most_scratch(a, att::plan_grad, [](const AttentionArgs&, const att::GradPlan& p) {
+        return p.stats + p.sink_partials + p.partials;
+    });
 }
 
 const char* attention_variant(const AttentionArgs& a)

@@ -4,9 +4,9 @@
 
 namespace opscv {
 
-hipError_t run_attention_grad_bf16(const AttentionArgs& a, bool vectors, hipStream_t stream)
+hipError_t run_attention_grad_bf16(const AttentionArgs& a, const att::GradPlan& plan, bool vectors, hipStream_t stream)
 {
-    return vectors ? att::run_backward<__bf16, true>(a, stream) : att::run_backward<__bf16, false>(a, stream);
+    return vectors ? att::run_backward<__bf16, true>(a, plan, stream) : att::run_backward<__bf16, false>(a, plan, stream);
 }
 
 }  // namespace opscv

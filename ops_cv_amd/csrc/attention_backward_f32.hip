@@ -4,9 +4,9 @@
 
 namespace opscv {
 
-hipError_t run_attention_grad_f32(const AttentionArgs& a, bool vectors, hipStream_t stream)
+hipError_t run_attention_grad_f32(const AttentionArgs& a, const att::GradPlan& plan, bool vectors, hipStream_t stream)
 {
-    return vectors ? att::run_backward<float, true>(a, stream) : att::run_backward<float, false>(a, stream);
+    return vectors ? att::run_backward<float, true>(a, plan, stream) : att::run_backward<float, false>(a, plan, stream);
 }
 
 }  // namespace opscv

@@ -823,7 +823,7 @@ hipError_t launch_query_grad(const GradLaunch& p, hipStream_t stream)
             return e;
         }
     }
-    hipLaunchKernelGGL(kernel, dim3((p.query_blocks + 7) / 8 * 8), dim3(kShape.threads()), kBytes, stream, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)launched(p.query_blocks)), dim3(kShape.threads()), kBytes, stream, p);
     return hipGetLastError();
 }
 
@@ -843,7 +843,7 @@ hipError_t launch_key_grad(const GradLaunch& p, hipStream_t stream)
             return e;
         }
     }
-    hipLaunchKernelGGL(kernel, dim3((p.key_blocks + 7) / 8 * 8), dim3(64 * kWaves), kBytes, stream, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)launched(p.key_blocks)), dim3(64 * kWaves), kBytes, stream, p);
     return hipGetLastError();
 }
 
@@ -872,19 +872,10 @@ hipError_t run_backward_shape(const GradLaunch& p, bool few, hipStream_t stream)
 }
 
 template <typename T, bool VEC>
-hipError_t run_backward(const AttentionArgs& a, hipStream_t stream)
+hipError_t run_backward(const AttentionArgs& a, const GradPlan& plan, hipStream_t stream)
 {
-    const GradPlan plan = plan_grad(a);
-    const int64_t bh = a.batch * a.kv_heads, stat_rows = a.batch * a.heads * a.tokens;
-    const int64_t query_blocks = bh * plan.tiles;
-    const int64_t key_blocks = bh * (plan.sink_tiles * plan.sink_parts + (plan.key_tiles - plan.sink_tiles) * plan.parts);
-    const int64_t quads = (a.d + 3) / 4;
-    const int64_t sink_joins = plan.sink_parts > 1 ? bh * plan.sink_tiles * 2 * plan.keys * quads : 0;
-    const int64_t joins = plan.parts > 1 ? bh * (plan.key_tiles - plan.sink_tiles) * 2 * plan.keys * quads : 0;
-    // two rows of statistics are reached with 32-bit offsets
-    if (query_blocks > INT32_MAX / 1024 || key_blocks > INT32_MAX / 1024 || stat_rows > INT32_MAX / 16 ||
-        a.tokens > INT32_MAX / 12 || sink_joins + joins > INT32_MAX ||
-        (a.scratch == nullptr && plan.stats > 0)) {
+    // two rows of statistics are reached with 32-bit offsets in bytes
+    if (!plan.fits || plan.stat_pitch > ((int64_t)1 << 28) || (a.scratch == nullptr && plan.stats > 0)) {
         return hipErrorInvalidValue;
     }
     GradLaunch p;
@@ -898,8 +889,8 @@ hipError_t run_backward(const AttentionArgs& a, hipStream_t stream)
     p.sink_tiles = (uint32_t)plan.sink_tiles;
     p.sink_parts = (uint32_t)plan.sink_parts;
     p.parts = (uint32_t)plan.parts;
-    p.query_blocks = (uint32_t)query_blocks;
-    p.key_blocks = (uint32_t)key_blocks;
+    p.query_blocks = (uint32_t)plan.query_blocks;
+    p.key_blocks = (uint32_t)plan.key_blocks;
     p.stat_pitch = plan.stat_pitch;
     p.stats = a.scratch;
     p.sink_partials = a.scratch + plan.stats;
@@ -915,10 +906,10 @@ hipError_t run_backward(const AttentionArgs& a, hipStream_t stream)
     if (e != hipSuccess) {
         return e;
     }
-    if (sink_joins + joins > 0) {
-        const uint32_t total = (uint32_t)(sink_joins + joins);
+    if (plan.sink_joins + plan.joins > 0) {
+        const uint32_t total = (uint32_t)(plan.sink_joins + plan.joins);
         hipLaunchKernelGGL((attention_grad_join_kernel<T, VEC>), dim3((total + 255) / 256), dim3(256), 0, stream, p,
-                           (uint32_t)sink_joins, (uint32_t)quads, total);
+                           (uint32_t)plan.sink_joins, (uint32_t)((a.d + 3) / 4), total);
     }
     return hipGetLastError();
 }
@@ -926,8 +917,8 @@ hipError_t run_backward(const AttentionArgs& a, hipStream_t stream)
 }  // namespace att
 
 // one translation unit a type
-hipError_t run_attention_grad_f32(const AttentionArgs& a, bool vectors, hipStream_t stream);
-hipError_t run_attention_grad_f16(const AttentionArgs& a, bool vectors, hipStream_t stream);
-hipError_t run_attention_grad_bf16(const AttentionArgs& a, bool vectors, hipStream_t stream);
+hipError_t run_attention_grad_f32(const AttentionArgs& a, const att::GradPlan& plan, bool vectors, hipStream_t stream);
+hipError_t run_attention_grad_f16(const AttentionArgs& a, const att::GradPlan& plan, bool vectors, hipStream_t stream);
+hipError_t run_attention_grad_bf16(const AttentionArgs& a, const att::GradPlan& plan, bool vectors, hipStream_t stream);
 
 }  // namespace opscv

@@ -4,9 +4,9 @@
 
 namespace opscv {
 
-hipError_t run_attention_f32(const AttentionArgs& a, bool vectors, hipStream_t stream)
+hipError_t run_attention_f32(const AttentionArgs& a, const att::ForwardPlan& plan, bool vectors, hipStream_t stream)
 {
-    return vectors ? att::run_forward<float, true>(a, stream) : att::run_forward<float, false>(a, stream);
+    return vectors ? att::run_forward<float, true>(a, plan, stream) : att::run_forward<float, false>(a, plan, stream);
 }
 
 }  // namespace opscv

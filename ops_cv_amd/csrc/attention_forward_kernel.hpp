@@ -506,15 +506,14 @@ hipError_t run_forward_shape(const ForwardLaunch& p, hipStream_t stream)
             return e;
         }
     }
-    hipLaunchKernelGGL(kernel, dim3((p.blocks + 7) / 8 * 8), dim3(kShape.threads()), kBytes, stream, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)launched(p.blocks)), dim3(kShape.threads()), kBytes, stream, p);
     return hipGetLastError();
 }
 
 template <typename T, bool VEC>
-hipError_t run_forward(const AttentionArgs& a, hipStream_t stream)
+hipError_t run_forward(const AttentionArgs& a, const ForwardPlan& plan, hipStream_t stream)
 {
-    const ForwardPlan plan = plan_forward(a);
-    if (plan.blocks > INT32_MAX / 1024 || (plan.splits > 1 && a.scratch == nullptr)) {
+    if (!plan.fits || (plan.splits > 1 && a.scratch == nullptr)) {
         return hipErrorInvalidValue;
     }
     ForwardLaunch p;
@@ -544,20 +543,16 @@ hipError_t run_forward(const AttentionArgs& a, hipStream_t stream)
     if (e != hipSuccess || plan.splits == 1) {
         return e;
     }
-    const int64_t quads = (a.d + 3) / 4, total = a.batch * a.kv_heads * plan.rows * quads;
-    if (total > INT32_MAX) {
-        return hipErrorInvalidValue;
-    }
-    hipLaunchKernelGGL((attention_join_kernel<T, VEC>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, stream, p,
-                       (uint32_t)quads, (uint32_t)total);
+    hipLaunchKernelGGL((attention_join_kernel<T, VEC>), dim3((unsigned)((plan.joins + 255) / 256)), dim3(256), 0, stream, p,
+                       (uint32_t)((a.d + 3) / 4), (uint32_t)plan.joins);
     return hipGetLastError();
 }
 
 }  // namespace att
 
 // one translation unit a type
-hipError_t run_attention_f32(const AttentionArgs& a, bool vectors, hipStream_t stream);
-hipError_t run_attention_f16(const AttentionArgs& a, bool vectors, hipStream_t stream);
-hipError_t run_attention_bf16(const AttentionArgs& a, bool vectors, hipStream_t stream);
+hipError_t run_attention_f32(const AttentionArgs& a, const att::ForwardPlan& plan, bool vectors, hipStream_t stream);
+hipError_t run_attention_f16(const AttentionArgs& a, const att::ForwardPlan& plan, bool vectors, hipStream_t stream);
+hipError_t run_attention_bf16(const AttentionArgs& a, const att::ForwardPlan& plan, bool vectors, hipStream_t stream);
 
 }  // namespace opscv

@@ -4,6 +4,7 @@
 #include <cstdint>
 
 #include "acl_types.hpp"
+#include "launch_limits.hpp"
 
 namespace opscv {
 namespace att {
@@ -41,7 +42,12 @@ struct ForwardPlan {
     int64_t tiles = 0;  // workgroups' worth of rows
     int64_t splits = 1; // parts that the keys of a tile are cut into
     int64_t blocks = 0; // workgroups
+    int64_t joins = 0;  // threads that join the parts, one for four features of a row
+    bool fits = false;  // one launch
 };
+
+// Workgroups with work, as they are launched: as many for every XCD.
+constexpr int64_t launched(int64_t blocks) { return (blocks + 7) / 8 * 8; }
 
 // Partial results of a split: per row the largest score, the sum, and the weighted values.
 constexpr int64_t partial_floats(int64_t d) { return 2 + (d + 3) / 4 * 4; }
@@ -77,6 +83,8 @@ inline ForwardPlan plan_forward(const AttentionArgs& a)
     p.splits = want < most ? want : most;
     p.splits = p.splits < 1 ? 1 : (p.splits > 64 ? 64 : p.splits);
     p.blocks = whole * p.splits;
+    p.joins = p.splits > 1 ? a.batch * a.kv_heads * p.rows * ((a.d + 3) / 4) : 0;
+    p.fits = fits_launch(launched(p.blocks), s.threads()) && p.joins <= INT32_MAX;
     return p;
 }
 
@@ -111,6 +119,9 @@ struct GradPlan {
     int64_t sink_parts = 1, parts = 1; // parts that the queries of such a tile, and of the others, are cut into at most
     // 32-bit words of the scratch: statistics of the rows, partial gradients of the sinks' tiles and of the others
     int64_t stat_pitch = 0, stats = 0, sink_partials = 0, partials = 0;
+    // workgroups of the two kernels, and threads of the join, for the sinks' tiles and for the others
+    int64_t query_blocks = 0, key_blocks = 0, sink_joins = 0, joins = 0;
+    bool fits = false;  // one launch each
 };
 
 inline GradPlan plan_grad(const AttentionArgs& a)
@@ -158,12 +169,57 @@ inline GradPlan plan_grad(const AttentionArgs& a)
     p.sink_parts = (sink_steps + low - 1) / low;
     p.parts = p.parts < 1 ? 1 : p.parts;
     p.sink_parts = p.sink_parts < 1 ? 1 : p.sink_parts;
-    p.stat_pitch = (a.tokens + 15) / 16 * 16;  // rows of statistics begin on lines of 64 bytes
+    p.stat_pitch = (a.tokens + 7) / 8 * 8;  // rows of statistics begin on sectors of 32 bytes
     p.stats = 2 * a.batch * a.heads * p.stat_pitch;
     const int64_t tile_floats = 2 * p.keys * ((a.d + 3) / 4 * 4);
     p.sink_partials = p.sink_parts > 1 ? bh * p.sink_tiles * p.sink_parts * tile_floats : 0;
     p.partials = p.parts > 1 ? bh * (p.key_tiles - p.sink_tiles) * p.parts * tile_floats : 0;
+    p.query_blocks = bh * p.tiles;
+    p.key_blocks = bh * (p.sink_tiles * p.sink_parts + (p.key_tiles - p.sink_tiles) * p.parts);
+    const int64_t tile_joins = 2 * p.keys * ((a.d + 3) / 4);
+    p.sink_joins = p.sink_parts > 1 ? bh * p.sink_tiles * tile_joins : 0;
+    p.joins = p.parts > 1 ? bh * (p.key_tiles - p.sink_tiles) * tile_joins : 0;
+    const int bytes = a.elem == 0 ? 4 : 2;
+    p.fits = fits_launch(launched(p.query_blocks), grad_query_shape(bytes, pitch_of(blocks_of(a.d)), p.few_rows).threads()) &&
+             fits_launch(launched(p.key_blocks), 2 * p.keys) && p.sink_joins + p.joins <= INT32_MAX;
     return p;
+}
+
+// ------------------------------------------------------------------------------------------------------------ large batches
+
+// f(a, plan) for the launches that a call is made of: all sequences, or as many a launch as the half, the quarter, ... of them
+// that fits, and what is left.  None where one sequence alone does not fit.  plan_of(a): plan_forward or plan_grad.
+template <typename Plan, typename F>
+void by_launches(const AttentionArgs& a, Plan&& plan_of, F&& f)
+{
+    AttentionArgs s = a;
+    auto plan = plan_of(s);
+    while (!plan.fits && s.batch > 1) {
+        s.batch /= 2;
+        plan = plan_of(s);
+    }
+    if (!plan.fits) {
+        return;
+    }
+    f(s, plan);
+    const int elem_bytes = a.elem == 0 ? 4 : 2;
+    for (int64_t each = s.batch, b = each; b < a.batch; b += each) {
+        for (Strided* x : {&s.q, &s.k, &s.v, &s.out, &s.grad_out, &s.grad_q, &s.grad_k, &s.grad_v, &s.lse}) {
+            if (x->ptr != nullptr) {
+                x->ptr = (char*)x->ptr + each * x->stride[0] * (x == &s.lse ? 4 : elem_bytes);
+            }
+        }
+        for (Whole* x : {&s.q_lengths, &s.kv_lengths}) {
+            if (x->ptr != nullptr) {
+                x->ptr = (const char*)x->ptr + each * x->stride[0] * (x->wide != 0 ? 8 : 4);
+            }
+        }
+        if (a.batch - b < each) {
+            s.batch = a.batch - b;
+            plan = plan_of(s);
+        }
+        f(s, plan);
+    }
 }
 
 }  // namespace att

@@ -658,6 +658,10 @@ aclnnStatus opscvWindowAttentionGetWorkspaceSize(const aclTensor* query, const a
     if (a.batch == 0 || a.tokens == 0) {
         return finish(api, ex, workspaceSize, executor);
     }
+    const int64_t scratch = attention_scratch_floats(a);
+    if (scratch < 0) {
+        return invalid("%s: more rows of a sequence than a launch holds", api);
+    }
     ex->kind = OpKind::WindowAttention;
     const int bytes = elem_size((Elem)a.elem);
     plan_strided(ex.get(), kAtQ, query, bytes, false, &a.q);
@@ -673,7 +677,7 @@ aclnnStatus opscvWindowAttentionGetWorkspaceSize(const aclTensor* query, const a
     if (lse != nullptr) {
         plan_lse(ex.get(), kAtLse, lse, &a.lse);
     }
-    plan_scratch(ex.get(), kAtScratch, attention_scratch_floats(a));
+    plan_scratch(ex.get(), kAtScratch, scratch);
     return finish(api, ex, workspaceSize, executor);
 }
 
@@ -706,6 +710,10 @@ aclnnStatus opscvWindowAttentionBackwardGetWorkspaceSize(
     if (query->empty() && key->empty()) {
         return finish(api, ex, workspaceSize, executor);
     }
+    const int64_t scratch = attention_grad_scratch_floats(a);
+    if (scratch < 0) {
+        return invalid("%s: more rows or keys of a sequence than a launch holds", api);
+    }
     ex->kind = OpKind::WindowAttentionGrad;
     const int bytes = elem_size((Elem)a.elem);
     plan_strided(ex.get(), kAtQ, query, bytes, false, &a.q);
@@ -723,7 +731,7 @@ aclnnStatus opscvWindowAttentionBackwardGetWorkspaceSize(
         plan_whole(ex.get(), kAtKvLengths, kvLengths, &a.kv_lengths);
     }
     plan_lse(ex.get(), kAtLse, lse, &a.lse);
-    plan_scratch(ex.get(), kAtScratch, attention_grad_scratch_floats(a));
+    plan_scratch(ex.get(), kAtScratch, scratch);
     return finish(api, ex, workspaceSize, executor);
 }
 
