@@ -294,6 +294,29 @@ hipError_t launch_rotary(const RotaryArgs& a, hipStream_t stream)
     if (a.rot < 2 || a.rot % 2 != 0 || a.rot > a.d || a.batch < 1 || a.tokens < 1) {
         return hipErrorInvalidValue;
     }
+    // a launch takes one token at least, whose threads have 31-bit numbers: more heads than those reach go span by span, keys
+    // as queries of their own
+    constexpr int64_t kMostHeads = (int64_t)1 << 20;
+    if (a.heads + a.kv_heads > kMostHeads) {
+        const int64_t e = a.elem == (int)Elem::F32 ? 4 : 2;
+        for (const bool keys : {false, true}) {
+            const int64_t heads = keys ? a.kv_heads : a.heads;
+            for (int64_t h = 0; h < heads; h += kMostHeads) {
+                RotaryArgs s = a;
+                s.heads = heads - h < kMostHeads ? heads - h : kMostHeads;
+                s.kv_heads = 0;
+                s.query = keys ? a.key : a.query;
+                s.query_out = keys ? a.key_out : a.query_out;
+                s.key = s.key_out = Strided();
+                s.query.ptr = (char*)s.query.ptr + h * s.query.stride[2] * e;
+                s.query_out.ptr = (char*)s.query_out.ptr + h * s.query_out.stride[2] * e;
+                if (const hipError_t status = launch_rotary(s, stream); status != hipSuccess) {
+                    return status;
+                }
+            }
+        }
+        return hipSuccess;
+    }
     switch ((Elem)a.elem) {
         case Elem::F32: return run_type<float>(a, stream);
         case Elem::F16: return run_type<_Float16>(a, stream);

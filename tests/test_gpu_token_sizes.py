@@ -52,3 +52,25 @@ def test_tokens_of_hundreds_of_thousands_of_sequences(device, aclnn, dtype):
 def test_tokens_of_more_sequences_than_a_launch_holds(device, aclnn):
     """2^24 workgroups of 256 threads and a few: two launches."""
     check_tokens(aclnn, device, torch.bfloat16, (1 << 21) + 3, 8, 2, 8)
+
+
+@pytest.mark.parametrize("heads,kv_heads,d,rot,interleaved", [
+    ((1 << 20) + 5, (1 << 20) + 3, 6, 6, False), ((1 << 20) + 5, 2, 8, 8, True), (3, (2 << 20) + 1, 4, 2, False),
+    ((1 << 24) + (1 << 16), 0, 1023, 2, False)])
+def test_rotary_of_very_many_heads(device, aclnn, heads, kv_heads, d, rot, interleaved):
+    """More heads of a token than the threads of a launch have numbers for, or than one launch takes: as a few of them alone."""
+    table = aclnn.rotary_table(torch.empty(0, device=device), 3, rot)
+    positions = torch.tensor([[2]], device=device)
+    made = []
+    for n in (heads, kv_heads):
+        x = torch.empty(1, 1, n, d, dtype=torch.bfloat16, device=device)
+        for part in x[0, 0].split(1 << 22):
+            part.normal_()
+        made.append(x if n else None)
+    # the first, the last, and those where spans of heads meet
+    places = [[slice(a, a + 70) for a in (0, (1 << 20) - 20, (1 << 21) - 30, (1 << 24) - 40, max(0, n - 70)) if a < n] for n in (heads, kv_heads)]
+    kept = [[x[:, :, p].clone() for p in ps] if x is not None else [] for x, ps in zip(made, places)]
+    aclnn.rotary(made[0], made[1], table, positions=positions, interleaved=interleaved, query_out=made[0], key_out=made[1])
+    for x, ps, before in zip(made, places, kept):
+        for p, b in zip(ps, before):
+            assert torch.equal(x[:, :, p], aclnn.rotary(b, None, table, positions=positions, interleaved=interleaved)[0]), p
