@@ -499,7 +499,7 @@ __global__ __launch_bounds__(256) void norm_weight_kernel(const float* __restric
 {
     __shared__ float shared[8][32];
     const int column = (int)threadIdx.x & 31, part = (int)threadIdx.x >> 5;
-    const int64_t c = (int64_t)blockIdx.x * 32 + column;
+    const int64_t c = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 32 + column;
     float total = 0.0f;
     if (c < width) {
 #pragma unroll 8
@@ -560,8 +560,12 @@ hipError_t run_norm_grad(const NormGradArgs& a, hipStream_t stream)
         }
     }
     if (a.grad_weight != nullptr && !joined) {
-        hipLaunchKernelGGL((norm_weight_kernel<W>), dim3((unsigned)((a.width + 31) / 32)), dim3(256), 0, stream, a.partial,
-                           partials, a.width, (W*)a.grad_weight);
+        // rows of more than 2^25 columns take more than one row of workgroups: 2^24 of 256 threads are more than a launch holds
+        // in one
+        const int64_t blocks = (a.width + 31) / 32;
+        const dim3 columns((unsigned)(blocks < kMostBlocks ? blocks : kMostBlocks), (unsigned)((blocks + kMostBlocks - 1) / kMostBlocks));
+        hipLaunchKernelGGL((norm_weight_kernel<W>), columns, dim3(256), 0, stream, a.partial, partials, a.width,
+                           (W*)a.grad_weight);
     }
     return hipGetLastError();
 }

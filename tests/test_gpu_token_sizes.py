@@ -74,3 +74,22 @@ def test_rotary_of_very_many_heads(device, aclnn, heads, kv_heads, d, rot, inter
     for x, ps, before in zip(made, places, kept):
         for p, b in zip(ps, before):
             assert torch.equal(x[:, :, p], aclnn.rotary(b, None, table, positions=positions, interleaved=interleaved)[0]), p
+
+
+@pytest.mark.parametrize("rows,width", [(3, (1 << 25) + 33), (1, (1 << 29) + 33)])
+def test_norm_gradients_of_very_long_rows(device, aclnn, rows, width):
+    """Rows whose columns are more than a launch of the weight's gradient holds side by side."""
+    h, gy = (normal(device, s, rows, width, dtype=torch.bfloat16) for s in (1, 2))
+    w = normal(device, 3, width, dtype=torch.bfloat16)
+    rstd = torch.full((rows,), 0.75, device=device)
+    gx, gw = aclnn.residual_norm_backward(gy, h, w, rstd)
+    mean = torch.zeros(rows, dtype=torch.float64, device=device)
+    parts = [slice(i, min(i + (1 << 24), width)) for i in range(0, width, 1 << 24)]
+    for p in parts:
+        mean += (gy[:, p].double() * w[p].double() * h[:, p].double() * 0.75).sum(1) / width
+    for p in parts:
+        n, g = h[:, p].double() * 0.75, gy[:, p].double()
+        want = (g * w[p].double() - n * mean[:, None]) * 0.75
+        assert ((gx[:, p].double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-5 * ((g * w[p].double()).abs() + n.abs())).all()
+        want = (g * n).sum(0)
+        assert ((gw[p].double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-5 * (g * n).abs().sum(0)).all()
