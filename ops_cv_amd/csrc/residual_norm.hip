@@ -202,38 +202,38 @@ __global__ __launch_bounds__(1024) void norm_long_kernel(NormArgs a)
     __shared__ float shared[2][2][16];
     int slot = 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    float sum = 0.0f, most = 0.0f;
-    for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.width; c += 1024 * VEC) {
-        float h[VEC], w[VEC];
-        get_row_part<T, VEC, WIDE>(a, row, c, h);
-        load_part<W, VEC, WIDE>((const W*)a.weight, c, a.width, w);
+        float sum = 0.0f, most = 0.0f;
+        for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.width; c += 1024 * VEC) {
+            float h[VEC], w[VEC];
+            get_row_part<T, VEC, WIDE>(a, row, c, h);
+            load_part<W, VEC, WIDE>((const W*)a.weight, c, a.width, w);
 #pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            sum += h[i] * h[i];
-            most = larger(most, fabsf(h[i] * w[i]));
+            for (int i = 0; i < VEC; i++) {
+                sum += h[i] * h[i];
+                most = larger(most, fabsf(h[i] * w[i]));
+            }
         }
-    }
-    row_reduce<1024>(sum, INT8 ? &most : nullptr, shared, slot);
-    slot ^= 1;
-    const float rstd = 1.0f / sqrtf(sum / (float)a.width + a.eps);
-    float scale = 0.0f;
-    const Int8Steps steps = INT8 ? int8_steps(most, rstd, &scale) : Int8Steps{};
-    if (threadIdx.x == 0) {
-        if (a.rstd != nullptr) {
-            a.rstd[row] = rstd;
+        row_reduce<1024>(sum, INT8 ? &most : nullptr, shared, slot);
+        slot ^= 1;
+        const float rstd = 1.0f / sqrtf(sum / (float)a.width + a.eps);
+        float scale = 0.0f;
+        const Int8Steps steps = INT8 ? int8_steps(most, rstd, &scale) : Int8Steps{};
+        if (threadIdx.x == 0) {
+            if (a.rstd != nullptr) {
+                a.rstd[row] = rstd;
+            }
+            if (INT8) {
+                a.scale[row] = scale;
+            }
         }
-        if (INT8) {
-            a.scale[row] = scale;
+        for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.width; c += 1024 * VEC) {
+            float h[VEC];
+            get_row_part<T, VEC, WIDE>(a, row, c, h);
+            if (a.sum.ptr != nullptr) {
+                store_part<T, VEC, WIDE>((T*)a.sum.ptr + row * a.sum.row_stride, c, a.width, h, a.streaming != 0);
+            }
+            put_row_part<T, W, INT8, VEC, WIDE>(a, row, c, h, rstd, steps);
         }
-    }
-    for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.width; c += 1024 * VEC) {
-        float h[VEC];
-        get_row_part<T, VEC, WIDE>(a, row, c, h);
-        if (a.sum.ptr != nullptr) {
-            store_part<T, VEC, WIDE>((T*)a.sum.ptr + row * a.sum.row_stride, c, a.width, h, a.streaming != 0);
-        }
-        put_row_part<T, W, INT8, VEC, WIDE>(a, row, c, h, rstd, steps);
-    }
     }
 }
 
@@ -442,37 +442,37 @@ __global__ __launch_bounds__(1024) void norm_grad_long_kernel(NormGradArgs a)
     __shared__ float shared[2][2][16];
     int slot = 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const float rstd = a.rstd[row];
-    const T* const sum = (const T*)a.sum.ptr + row * a.sum.row_stride;
-    const T* const gy = (const T*)a.grad_y.ptr + row * a.grad_y.row_stride;
-    float along = 0.0f;
-    for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.width; c += 1024 * VEC) {
-        float n[VEC], g[VEC], w[VEC];
-        load_part<T, VEC, WIDE>(sum, c, a.width, n);
-        load_part<T, VEC, WIDE>(gy, c, a.width, g);
-        load_part<W, VEC, WIDE>((const W*)a.weight, c, a.width, w);
+        const float rstd = a.rstd[row];
+        const T* const sum = (const T*)a.sum.ptr + row * a.sum.row_stride;
+        const T* const gy = (const T*)a.grad_y.ptr + row * a.grad_y.row_stride;
+        float along = 0.0f;
+        for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.width; c += 1024 * VEC) {
+            float n[VEC], g[VEC], w[VEC];
+            load_part<T, VEC, WIDE>(sum, c, a.width, n);
+            load_part<T, VEC, WIDE>(gy, c, a.width, g);
+            load_part<W, VEC, WIDE>((const W*)a.weight, c, a.width, w);
 #pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            along += g[i] * w[i] * (n[i] * rstd);
+            for (int i = 0; i < VEC; i++) {
+                along += g[i] * w[i] * (n[i] * rstd);
+            }
         }
-    }
-    row_reduce<1024>(along, nullptr, shared, slot);
-    slot ^= 1;
-    along /= (float)a.width;
-    for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.width; c += 1024 * VEC) {
-        float n[VEC], g[VEC], w[VEC], s[VEC] = {0.0f};
-        load_part<T, VEC, WIDE>(sum, c, a.width, n);
-        load_part<T, VEC, WIDE>(gy, c, a.width, g);
-        load_part<W, VEC, WIDE>((const W*)a.weight, c, a.width, w);
-        if (a.grad_sum.ptr != nullptr) {
-            load_part<T, VEC, WIDE>((const T*)a.grad_sum.ptr + row * a.grad_sum.row_stride, c, a.width, s);
-        }
+        row_reduce<1024>(along, nullptr, shared, slot);
+        slot ^= 1;
+        along /= (float)a.width;
+        for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.width; c += 1024 * VEC) {
+            float n[VEC], g[VEC], w[VEC], s[VEC] = {0.0f};
+            load_part<T, VEC, WIDE>(sum, c, a.width, n);
+            load_part<T, VEC, WIDE>(gy, c, a.width, g);
+            load_part<W, VEC, WIDE>((const W*)a.weight, c, a.width, w);
+            if (a.grad_sum.ptr != nullptr) {
+                load_part<T, VEC, WIDE>((const T*)a.grad_sum.ptr + row * a.grad_sum.row_stride, c, a.width, s);
+            }
 #pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            s[i] += (g[i] * w[i] - n[i] * rstd * along) * rstd;
+            for (int i = 0; i < VEC; i++) {
+                s[i] += (g[i] * w[i] - n[i] * rstd * along) * rstd;
+            }
+            store_part<T, VEC, WIDE>((T*)a.grad_x.ptr + row * a.grad_x.row_stride, c, a.width, s, false);
         }
-        store_part<T, VEC, WIDE>((T*)a.grad_x.ptr + row * a.grad_x.row_stride, c, a.width, s, false);
-    }
     }
 }
 
