@@ -7,7 +7,9 @@
  * the executor.
  *
  *   dtypes  : FLOAT, FLOAT16, BF16; the operands of one call have one type unless stated otherwise.  Sums, softmax
- *             statistics and norms are held in 32 bits.
+ *             statistics and norms are held in 32 bits.  The matrix products of attention take operands of the tensors'
+ *             type: its weights, and in the gradients weights and gradients of the scores, are rounded to it (to nearest,
+ *             a relative 2^-11 at most for FLOAT16, 2^-8 for BF16) before they are multiplied and summed up in 32 bits.
  *   formats : any (the order of the dimensions is fixed by the operator)
  *   views   : arbitrary strides and offsets are honoured.  Attention and rotary operands whose last dimension is dense
  *             are used in place whatever the strides of the others; other views are packed through the workspace.
@@ -27,7 +29,8 @@ extern "C" {
 /*
  * Root-mean-square norm with the residual's addition:
  *   h = x + residual,  rstd = 1 / sqrt(mean(h^2) + eps),  y = h * rstd * weight
- * x, residual, y, sum : (..., width), one to five dimensions; weight : (width), of x's type or FLOAT.
+ * x, residual, y, sum : (..., width), one to five dimensions; weight : (width), of x's type or FLOAT.  h, its squares and
+ * h * weight are numbers of 32 bits: their range is FLOAT's.
  *   residual : NULL: h = x
  *   y        : of x's type, or INT8.  INT8: y = round(h * weight * (127 / m)) to the nearest, ties to even, with
  *              m = max |h * weight| over the row, and `scale` (FLOAT, the leading dimensions) = m * rstd / 127, so that
@@ -64,7 +67,7 @@ ACLNN_API aclnnStatus opscvResidualNormBackward(void* workspace, uint64_t worksp
 
 /* How opscvRotaryTable stretches its angles to contexts longer than a model was trained on. */
 typedef enum {
-    OPSCV_ROTARY_PLAIN = 0,    /* frequency i: base^(-2i/rot) turns of 2 pi per 2 pi positions */
+    OPSCV_ROTARY_PLAIN = 0,    /* pair i turns by base^(-2i/rot) radians from one position to the next */
     OPSCV_ROTARY_LINEAR = 1,   /* every frequency divided by factor */
     OPSCV_ROTARY_BASE = 2,     /* base * factor^(rot / (rot - 2)): the lowest frequency is divided by factor, the
                                   highest kept */
@@ -116,8 +119,8 @@ ACLNN_API aclnnStatus opscvRotary(void* workspace, uint64_t workspaceSize, aclOp
  *   left, right, sinks >= 0 (right = 0: causal; left = INT64_MAX: no window), scale > 0 and finite.
  * Prompts (many queries), chunks on a cache and single tokens take the same call.
  *   sizes : up to 2^28 tokens and kvTokens, 2^30 rows (tokens * heads) of a sequence, 2^31 - 1 batch * heads.  A sequence
- *       whose workgroups one launch does not hold is refused (161002): FLOAT over 2^29 rows of a key head, and, in the
- *       gradients, kvTokens * kvHeads from 2^31 on.  Batches of any size take as many launches as they need.
+ *       whose workgroups one launch does not hold is refused (161002): FLOAT heads of up to 64 features from 2^29
+ *       rows on, and, in the gradients, kvTokens * kvHeads from 2^31 on.  Batches of any size take as many launches as they need.
  */
 ACLNN_API aclnnStatus opscvWindowAttentionGetWorkspaceSize(const aclTensor* query, const aclTensor* key,
                                                            const aclTensor* value, const aclTensor* qLengths,

@@ -7,15 +7,17 @@
 //               exchanged,  gV' += gO' P,  gK' += Q' dS
 //   join        where the queries of a tile of keys were cut into parts, their 32-bit sums in order
 //
-// Everything but the operands of the products is in 32 bits: P and dS are rounded to the type as the matrix instructions
-// want them.  P and dS are computed twice, once for each direction: seven products instead of five, but every sum has one
-// owner and a fixed order, and no gradient is added up by atomics.
+// Everything but the operands of the products is in 32 bits: P and dS are rounded to the type, because the matrix instructions
+// take operands of one type (as in the forward pass).  P and dS are computed twice, once for each direction: seven products
+// instead of five, but every sum has one owner and a fixed order, and no gradient is added up by atomics.
 //
-// 4096 tokens, 32 heads of 128 on 8, window 1024, bf16: 280 to 290 us (520 TFLOP/s of the five products); keys 172 to 200,
-// queries 115 to 140, the join 15.  The keys' kernel reads five operands of 1 KB from LDS for four products, a quarter more
-// than LDS gives in their time, at two wavefronts a SIMD, which is what its accumulators leave room for.  FLOAT (2 x 777
-// tokens, 12 heads of 72 on 4, window 101: 92 us) is bound by its products, which take sixteen times as long, and by tiles
-// of 32 along a window of 101.
+// 4096 tokens, 32 heads of 128 on 8, window 1024, bf16: 284 to 288 us (525 TFLOP/s of the five products); keys 160 to 167,
+// queries 115 to 125, the join 15.  In both kernels 35 % of a SIMD's cycles are products and 30 % vector instructions,
+// which two wavefronts a SIMD, all that the accumulators leave room for, cover in part; LDS is busy for 26 % in the keys'.
+// FLOAT (2 x 777 tokens, 12 heads of 72 on 4, window 101: 91 us, queries 37, keys 50) is bound by single wavefronts that walk
+// five or six tiles one after another: products, which take sixteen times as many cycles as those of 16-bit types, are half
+// of a wavefront's time and loads that nothing covers a quarter (keys) to a third (queries), while fewer than half of the
+// SIMDs have a wavefront at all.
 //
 // dS of FLOAT16 may be anything from P of a long row times a small gradient, for which FLOAT16 has few bits or none, to the
 // products of large gradients and values, which are past its end.  So every sum's dS (of a row in the queries' kernel, of a

@@ -7,16 +7,20 @@
 //   m, l             running reference of a row (near its largest score) and sum of exp2(S c - m), c = scale log2 e; a
 //                    row's keys are spread over two lanes, which exchange their maxima
 //   O' = O' f + V' P (head features x 32 rows; V from LDS in "column" order, P are S's registers, rounded to the type)
-// m, l and O stay in 32 bits; P is rounded to the type as the matrix instructions want it.
+// m, l and O stay in 32 bits; P is rounded to the type, because the matrix instructions take operands of one type: with it in
+// two parts of 16 bits the second product would be done twice.  Against 64 bits that makes results 1.4 times as far off as
+// the rounding of the result alone does (bf16 0.0023 for 0.0017, FLOAT16 0.00029 for 0.00021, on heads of 64 and 128).
 //
 // Why so: O' in registers, its columns being rows of the product, is scaled by one number a lane, and S' becomes the
 // operand P without leaving the registers.  Bound by memory for single tokens (32 caches of up to 16384 tokens, window
 // 4096, 32 heads of 128 on 8, bf16: 104 us, 5.2 TB/s), where the keys are shared out over wavefronts and workgroups.  Of
-// prompts (8192 tokens, the same heads, window 1024: 163 to 175 us on different machines, 740 to 790 TFLOP/s) by LDS as
-// much as by the matrix cores: 32 rows a wavefront read 1 KB for every product, as much as LDS gives four SIMDs meanwhile.
-// Wavefronts of 64 rows would halve that, but leave the registers of one a SIMD, whose loads and exponentials are then
-// not behind the products (235 us).  Heads of 64 (8 images of 1369 tokens, 16 heads, window 513: 51 us) have half the
-// products to an exponential and are bound by vector instructions and what is left undone while wavefronts wait.
+// prompts (8192 tokens, the same heads, window 1024: 165 to 172 us, 750 to 785 TFLOP/s) by the issue of vector instructions
+// and products: of a SIMD's cycles 40 % go to vector instructions (a fifth of those to exponentials) and 35 % to products,
+// and two wavefronts a SIMD cover each other only in part.  LDS is busy for 18 %: 1 KB for every product is half of the
+// 256 bytes a cycle that it gives.  Wavefronts of 64 rows read half as much, but leave the registers of one a SIMD, whose
+// loads and exponentials are then not behind the products (235 us).  Heads of 64 (8 images of 1369 tokens, 16 heads, window
+// 513: 51 us) have twice the exponentials to a product: vector instructions 40 %, products 16 %, and for 29 % of the time a
+// CU has no work (start and end, and 1408 workgroups are five and a half for each).
 #pragma once
 
 #include <atomic>
@@ -531,8 +535,8 @@ hipError_t run_forward(const AttentionArgs& a, const ForwardPlan& plan, hipStrea
             case 8: e = run_forward_shape<T, 8, kFew, VEC>(p, stream); break;
             case 4: e = run_forward_shape<T, 4, kFew, VEC>(p, stream); break;
             case 3: e = run_forward_shape<T, 3, kFew, VEC>(p, stream); break;
-        case 2: e = run_forward_shape<T, 2, kFew, VEC>(p, stream); break;
-        default: e = run_forward_shape<T, 1, kFew, VEC>(p, stream); break;
+            case 2: e = run_forward_shape<T, 2, kFew, VEC>(p, stream); break;
+            default: e = run_forward_shape<T, 1, kFew, VEC>(p, stream); break;
         }
     };
     if (plan.few_rows) {

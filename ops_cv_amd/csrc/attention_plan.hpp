@@ -53,8 +53,16 @@ constexpr int64_t launched(int64_t blocks) { return (blocks + 7) / 8 * 8; }
 constexpr int64_t partial_floats(int64_t d) { return 2 + (d + 3) / 4 * 4; }
 
 // Tiles of 32 rows instead of tiles of 128: where those would leave CUs without work, where there are no more rows, and for
-// FLOAT, whose products take sixteen times as long as those of 16-bit types: what it costs that every 32 rows read their
-// keys themselves does not show, and no wavefront waits for another.
+// FLOAT.  On both sides of the line, us with tiles of 32 and of 128 (tiles of 128 in brackets), forward and gradients:
+//   8 heads of 128 on 8, window 1024, bf16    [128] 30 and 35, 80 and 89   [224] 54 and 52, 124 and 106
+//                                             [256] 56 and 45, 135 and 112   [512] 112 and 52, 253 and 185
+//   pictures of 1369 tokens, heads of 64      [176] 18 and 26, 58 and 58   [264] 23 and 29, 68 and 65
+//                                             [352] 28 and 33, 76 and 73
+//   2048 tokens, 8 heads of 256 on 8, fp16    [128] 98 and 104, 323 and 282   [256] 155 and 163, 389 and 342
+// FLOAT, forward: pictures of 1369 tokens, 16 heads of 64, one 56 and 67, four 197 and 173; 4096 tokens, 32 heads of 128 on 8
+// 672 and 692; 2 x 4096, 16 of 96 on 4 550 and 541.  Tiles of 128 would be the faster ones of many tiles of narrow heads
+// (8192 tokens, 16 heads of 64 on 4: 481 and 310; 5 x 911, 16 of 32 on 2: 129 and 78) and of heads of 256 (2048 tokens, 8
+// heads: 748 and 620); there is no such kernel.
 inline bool few_rows(const AttentionArgs& a)
 {
     const int64_t rows = a.tokens * (a.heads / a.kv_heads);
@@ -76,8 +84,8 @@ inline ForwardPlan plan_forward(const AttentionArgs& a)
     const int64_t keys = a.kv_tokens < window + a.sinks ? a.kv_tokens : window + a.sinks;
     const int64_t key_tiles = (keys + s.keys - 1) / s.keys;
     // Eight wavefronts for every CU where that many parts leave each four tiles or more; single wavefronts of FLOAT, whose
-    // products take sixteen times as long, one tile (one token on a window of 129, 8 heads of 96 on 1: 13 us, 25 with four; five sequences of 256
-    // tokens, a head of 128, window 86: 16 and 26).
+    // products take sixteen times as many cycles, one tile (one token on a window of 129, 8 heads of 96 on 1: 13 us, 25 with
+    // four; five sequences of 256 tokens, a head of 128, window 86: 16 and 26).
     const int64_t waves = s.row_waves * s.key_waves, least = waves == 1 && a.elem == 0 ? 1 : 4 * s.key_waves;
     const int64_t want = (8 * (int64_t)a.compute_units / waves + whole - 1) / whole, most = key_tiles / least;
     p.splits = want < most ? want : most;
@@ -91,7 +99,11 @@ inline ForwardPlan plan_forward(const AttentionArgs& a)
 // ---------------------------------------------------------------------------------------------------------- gradients
 
 // The queries' gradients: as the forward pass, but for FLOAT of more than 64 features, whose tiles fill LDS: 32 rows and one
-// wavefront, or, for few rows, four that share the keys.  There, and for heads of more than 128 features, the values come
+// wavefront, or, where there are at most two tiles of 32 rows for every CU, four that share the keys.  That line on both
+// sides, the whole backward call with one wavefront and with four: 4 x 1024 tokens, heads of 128, causal, 2 on 1 (256 tiles)
+// 311 and 177, 4 on 2 (512) 388 and 289, 8 on 8 (1024) 554 and 548; 2048 tokens, 8 heads of 96 on 2, window 512 (512) 208 and
+// 186, two such (1024) 317 and 365; 2 x 777, 12 of 72 on 4, window 101 (584) 92 and 107.
+//  There, and for heads of more than 128 features, the values come
 // straight from memory: FLOAT's products take long enough for that (4 x 1024 tokens, 2 heads of 128, causal: four wavefronts
 // 81 us, one 217; 16 x 512, 2 heads of 256 on 1: 205 and 334), and yet from LDS they come sooner (one wavefront: 2 x 777
 // tokens, 12 heads of 72 on 4, window 101: 38 us, with values from memory 42, with four wavefronts 53).
@@ -144,11 +156,14 @@ inline GradPlan plan_grad(const AttentionArgs& a)
     const int64_t window = (a.left + a.right + p.keys + kBlock - 1) / kBlock + 1;
     const int64_t steps = group * (window < all ? window : all);
     // As few parts as fill the card with one round of workgroups, every tile's steps in equal parts: ten wavefronts for every
-    // CU, of which eight run at a time, where a part has eight steps or more (4096 tokens, 32 heads of 128 on 8, window 1024,
-    // bf16: 294 us for the whole backward call, with eight 334, with sixteen 314; parts of as many steps each, whose last
-    // is what is left: 325).  FLOAT: one step or more, and as many wavefronts as its registers leave room for: four from
-    // three blocks of features on, eight of two, and of one block many short parts (3 x 1024 tokens, 64 heads of 32 on 8:
-    // 732 us with 32, with eight 937).
+    // CU, of which eight run at a time, where a part has eight steps or more.  The whole backward call with 8, 10 and 16:
+    // 4096 tokens, 32 heads of 128 on 8, window 1024, bf16 317, 284 and 299 us (parts of as many steps each, whose last is
+    // what is left: 325 at the time, for 294); 8 pictures of 1369 tokens, 16 heads of 64 174, 174, 174; 2 x 2048, 16 heads of
+    // 64, causal 143, 143, 134; 4 x 1024, 8 of 128 on 2 83, 89, 101; 8192 tokens, 8 of 128 on 1, window 512 128, 150, 152.
+    // FLOAT: one step or more, and as many wavefronts as its registers leave room for: four from three blocks of features on,
+    // eight of two, and of one block many short parts.  With 4, 8 and 32: 4 x 1024, 2 heads of 128 on 1 177, 178, 262; 2 x
+    // 2048, 8 of 96 on 2, window 512 319, 301, 344; 2 x 777, 12 of 72 on 4 93, 92, 108; 16 x 512, 2 of 256 on 1 468, 432, 768;
+    // 4 x 512, 8 of 64 128, 98, 120; 3 x 1024, 64 of 32 on 8, window 256 610, 469, 456; 5 x 911, 16 of 32 on 2 504, 346, 305.
     const int64_t sink_steps = group * all;
     const int64_t waves = a.elem != 0 ? 10 : blocks_of(a.d) > 2 ? 4 : blocks_of(a.d) == 2 ? 8 : 32;
     const int64_t room = a.compute_units * waves * kBlock / p.keys;

@@ -139,7 +139,8 @@ static __device__ __forceinline__ rsrc_t buffer(const void* base, uint32_t bytes
 // BYTES bytes a lane from offset `off` of a buffer into LDS, the wavefront's first at place dst + AT and the lanes in order; lanes
 // whose offset is out of range write zeros.  It has no result for the compiler to wait for, and as an instruction that the
 // compiler does not look into it makes it wait for nothing: with the builtin, every transposed read of LDS is preceded by
-// a wait for all loads under way, which takes the attention of a prompt of 8192 tokens from 193 to 203 us.  The caller waits.
+// a wait for all loads under way (a prompt of 8192 tokens took 203 us so where it took 193 without, before later steps).  The
+// caller waits.
 template <int BYTES, int AT>
 static __device__ __forceinline__ void load_to_lds(rsrc_t rsrc, uint32_t dst, uint32_t off)
 {
@@ -230,7 +231,7 @@ struct Tile {
 };
 
 // Where a lane reads whole rows (row base + l % 32) or columns of a tile: places that a loop computes once.  NB blocks of
-// 32 elements.  FLOAT has eight places a column and computes them as it goes: its products take eight times as long.
+// 32 elements.  FLOAT has eight places a column and computes them as it goes: its products take sixteen times as many cycles.
 template <typename T, int PITCH, int NB>
 struct Rows32 {
     int at[2 * NB];
