@@ -145,6 +145,137 @@ ACLNN_API aclnnStatus opscvWindowAttentionBackwardGetWorkspaceSize(
 ACLNN_API aclnnStatus opscvWindowAttentionBackward(void* workspace, uint64_t workspaceSize, aclOpExecutor* executor,
                                                    aclrtStream stream);
 
+/*
+ * Layer norm with the residual's addition:
+ *   h = x + residual,  rstd = 1 / sqrt(mean((h - mean(h))^2) + eps),  y = (h - mean(h)) * rstd * weight + bias
+ * x, residual, y, sum : (..., width), one to five dimensions; weight, bias : (width), both of x's type or both FLOAT.
+ *   residual   : NULL: h = x
+ *   weight     : NULL: ones
+ *   bias       : NULL: zeros
+ *   sum        : NULL, or h rounded to x's type.  The norm is taken of h before that rounding.
+ *   mean, rstd : NULL, or FLOAT, the leading dimensions: what the backward pass reads
+ * The squares are taken of h minus its mean, so a mean that is large beside the spread costs no more than its own rounding.
+ * sum may be x or residual (the same view): the addition in place.
+ */
+ACLNN_API aclnnStatus opscvLayerNormGetWorkspaceSize(const aclTensor* x, const aclTensor* residual,
+                                                     const aclTensor* weight, const aclTensor* bias, double eps,
+                                                     aclTensor* y, aclTensor* sum, aclTensor* mean, aclTensor* rstd,
+                                                     uint64_t* workspaceSize, aclOpExecutor** executor);
+ACLNN_API aclnnStatus opscvLayerNorm(void* workspace, uint64_t workspaceSize, aclOpExecutor* executor,
+                                     aclrtStream stream);
+
+/*
+ * Gradients of the layer norm.  n = (sum - mean) * rstd, g = gradY * weight:
+ *   gradX = (g - mean(g) - n * mean(g * n)) * rstd + gradSum
+ *   gradWeight = sum over rows of gradY * n,   gradBias = sum over rows of gradY
+ * gradX is the gradient of x and of the residual alike.
+ *   sum, mean, rstd : what the forward pass wrote (sum = x where there was no residual)
+ *   gradSum         : NULL, or the gradient that reaches `sum` on its other way
+ *   weight          : NULL: ones
+ *   gradWeight      : NULL, or (width), of weight's type (of sum's or FLOAT without a weight)
+ *   gradBias        : NULL, or (width), of gradWeight's or weight's type (of sum's or FLOAT without them)
+ * gradX may be gradY or gradSum (the same view).
+ */
+ACLNN_API aclnnStatus opscvLayerNormBackwardGetWorkspaceSize(const aclTensor* gradY, const aclTensor* gradSum,
+                                                             const aclTensor* sum, const aclTensor* weight,
+                                                             const aclTensor* mean, const aclTensor* rstd,
+                                                             aclTensor* gradX, aclTensor* gradWeight,
+                                                             aclTensor* gradBias, uint64_t* workspaceSize,
+                                                             aclOpExecutor** executor);
+ACLNN_API aclnnStatus opscvLayerNormBackward(void* workspace, uint64_t workspaceSize, aclOpExecutor* executor,
+                                             aclrtStream stream);
+
+/* Which pairs of features opscvRotaryAxes turns by which axis, and by which columns of the table. */
+typedef enum {
+    OPSCV_AXES_CONSECUTIVE = 0, /* the first sections[0] pairs by axis 0, the next sections[1] by axis 1, ...; pair i by
+                                   column i */
+    OPSCV_AXES_RESTART = 1,     /* the same pairs; those of each axis by columns 0, 1, ...: every axis has all frequencies */
+    OPSCV_AXES_DEALT = 2        /* one pair to each axis in turn, passing over axes that have all theirs; pair i by column i */
+} opscvAxesLayout;
+
+/*
+ * Rotary positions with several axes, such as time, height and width of a video's patches: opscvRotary where every pair is
+ * turned by the token's position on the pair's own axis.
+ *   positions : (axes, batch, tokens), INT32 or INT64, one to four axes.  A pair whose position is not a row of the table
+ *               becomes NaN.
+ *   sections  : one number of pairs, zero or more, per axis; the rotated features are rot = 2 * their sum, 2 <= rot <= d
+ *   table     : (positions, 2 * columns), FLOAT, as opscvRotaryTable writes it: columns cosines and behind them columns
+ *               sines.  columns = rot / 2, with OPSCV_AXES_RESTART the largest section.
+ *   others    : as opscvRotary.  inverse is the gradient's way back; the outputs may be the inputs (the same views).
+ */
+ACLNN_API aclnnStatus opscvRotaryAxesGetWorkspaceSize(const aclTensor* query, const aclTensor* key,
+                                                      const aclTensor* positions, const aclTensor* table,
+                                                      const aclIntArray* sections, int64_t layout, bool interleaved,
+                                                      bool inverse, aclTensor* queryOut, aclTensor* keyOut,
+                                                      uint64_t* workspaceSize, aclOpExecutor** executor);
+ACLNN_API aclnnStatus opscvRotaryAxes(void* workspace, uint64_t workspaceSize, aclOpExecutor* executor,
+                                      aclrtStream stream);
+
+/*
+ * Dropout with the residual's addition; which elements are kept is computed, never stored:
+ *   y = residual + (keep ? x * 65536 / (65536 - threshold) : 0),   threshold = 65536 p rounded to the nearest
+ * Element e (its number in the order of the dimensions, whatever the strides) is kept if its 16-bit number is not less than
+ * threshold.  The numbers of elements 8 c .. 8 c + 7 are the halves, low one first, of the four words that Philox 4x32 with
+ * ten rounds (Salmon, Moraes, Dror and Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011) makes of the counter (c's
+ * low word, c's high word, offset's low word, offset's high word) under the key (seed's low word, its high word).
+ * x, residual, y : (..., width), one to five dimensions, one type
+ *   residual     : NULL: nothing is added
+ *   state        : (2), INT64: seed and offset, read when the kernel runs.  A caller adds one to the offset (any number: every
+ *                  offset is another mask) between calls, in a recorded graph by a kernel of its own.
+ *   p            : 0 to 1; the mean of y is exact for the p that the threshold stands for.  p = 1 (or what rounds to it)
+ *                  keeps nothing.
+ * What x holds where it is dropped is never read into a result, NaN included.
+ * The gradient's way: gradX is the same call with gradY as x and no residual; the residual's gradient is gradY.
+ * y may be x or residual (the same view).
+ */
+ACLNN_API aclnnStatus opscvDropoutGetWorkspaceSize(const aclTensor* x, const aclTensor* residual, const aclTensor* state,
+                                                   double p, aclTensor* y, uint64_t* workspaceSize,
+                                                   aclOpExecutor** executor);
+ACLNN_API aclnnStatus opscvDropout(void* workspace, uint64_t workspaceSize, aclOpExecutor* executor,
+                                   aclrtStream stream);
+
+/* The activation of a gated projection. */
+typedef enum {
+    OPSCV_GATE_SILU = 0,     /* g / (1 + exp(-g)) */
+    OPSCV_GATE_GELU = 1,     /* g / 2 * (1 + erf(g / sqrt(2))) */
+    OPSCV_GATE_GELU_TANH = 2 /* g / 2 * (1 + tanh(sqrt(2 / pi) * (g + 0.044715 g^3))) */
+} opscvGateActivation;
+
+/*
+ * Gated projections, the first half of a gated feed-forward block, in one kernel:
+ *   gate = x gateWeight^T + gateBias,  up = x upWeight^T + upBias,  y = activation(gate) * up
+ * x : (..., width), y, gate, up : (..., inner), one to five dimensions; gateWeight, upWeight : (inner, width); gateBias,
+ * upBias : (inner), both or neither; all of one type.  Products are summed up in 32 bits, and y is computed from those sums.
+ *   gate, up : NULL (both), or the sums rounded to the type: what the backward pass reads
+ *   sizes    : width and inner up to 2^20, rows (the product of the leading dimensions) up to 2^30
+ */
+ACLNN_API aclnnStatus opscvGatedProjectionGetWorkspaceSize(const aclTensor* x, const aclTensor* gateWeight,
+                                                           const aclTensor* upWeight, const aclTensor* gateBias,
+                                                           const aclTensor* upBias, int64_t activation, aclTensor* y,
+                                                           aclTensor* gate, aclTensor* up, uint64_t* workspaceSize,
+                                                           aclOpExecutor** executor);
+ACLNN_API aclnnStatus opscvGatedProjection(void* workspace, uint64_t workspaceSize, aclOpExecutor* executor,
+                                           aclrtStream stream);
+
+/*
+ * Gradients of the gated projections.  dGate = gradY * up * activation'(gate), dUp = gradY * activation(gate):
+ *   gradX = dGate gateWeight + dUp upWeight
+ *   gradGateWeight = dGate^T x,  gradUpWeight = dUp^T x;   gradGateBias, gradUpBias = sums over rows of dGate, dUp
+ *   gate, up : what the forward call wrote
+ *   gradX, the weights' gradients (both or neither), the biases' (both or neither) : NULL where they are not wanted
+ * dGate and dUp are rounded to the type before they are multiplied (to nearest, relative 2^-11 at most for FLOAT16, 2^-8 for
+ * BF16), not before the biases' sums.  FLOAT16: times a power of two for each row, and for the weights' gradients each
+ * column, so that their largest is near 2^14; what is 2^28 times less than that largest loses bits.
+ *   sizes : width, inner and rows up to 2^20
+ */
+ACLNN_API aclnnStatus opscvGatedProjectionBackwardGetWorkspaceSize(
+    const aclTensor* gradY, const aclTensor* x, const aclTensor* gateWeight, const aclTensor* upWeight,
+    const aclTensor* gate, const aclTensor* up, int64_t activation, aclTensor* gradX, aclTensor* gradGateWeight,
+    aclTensor* gradUpWeight, aclTensor* gradGateBias, aclTensor* gradUpBias, uint64_t* workspaceSize,
+    aclOpExecutor** executor);
+ACLNN_API aclnnStatus opscvGatedProjectionBackward(void* workspace, uint64_t workspaceSize, aclOpExecutor* executor,
+                                                   aclrtStream stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -143,8 +143,17 @@ def load_library():
     L.opscvWindowAttentionBackwardGetWorkspaceSize.restype = i32
     L.opscvWindowAttentionBackwardGetWorkspaceSize.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_double, i64, i64,
                                                                i64, vp, vp, vp, p_u64, p_vp]
+    f64, flag = ctypes.c_double, ctypes.c_bool
+    for name, args in (("LayerNorm", [vp, vp, vp, vp, f64, vp, vp, vp, vp]), ("LayerNormBackward", [vp] * 9),
+                       ("RotaryAxes", [vp, vp, vp, vp, vp, i64, flag, flag, vp, vp]), ("Dropout", [vp, vp, vp, f64, vp]),
+                       ("GatedProjection", [vp, vp, vp, vp, vp, i64, vp, vp, vp]),
+                       ("GatedProjectionBackward", [vp] * 6 + [i64] + [vp] * 5)):
+        phase1 = getattr(L, "opscv" + name + "GetWorkspaceSize")
+        phase1.restype = i32
+        phase1.argtypes = args + [p_u64, p_vp]
     for name in ("ResidualNorm", "ResidualNormBackward", "RotaryTable", "Rotary", "WindowAttention",
-                 "WindowAttentionBackward"):
+                 "WindowAttentionBackward", "LayerNorm", "LayerNormBackward", "RotaryAxes", "Dropout", "GatedProjection",
+                 "GatedProjectionBackward"):
         phase2 = getattr(L, "opscv" + name)
         phase2.restype = i32
         phase2.argtypes = [vp, u64, vp, vp]
@@ -481,6 +490,8 @@ def upsample_bilinear2d_backward(grad_out, input_size, align_corners=False, scal
 # ----------------------------------------------------------------------------------------------------
 
 ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_BASE, ROTARY_BY_PARTS = 0, 1, 2, 3
+AXES_CONSECUTIVE, AXES_RESTART, AXES_DEALT = 0, 1, 2
+GATE_SILU, GATE_GELU, GATE_GELU_TANH = 0, 1, 2
 NO_WINDOW = 2 ** 63 - 1
 
 
@@ -547,6 +558,62 @@ def window_attention_backward(grad_out, query, key, value, out, lse, scale=None,
     return (_helpers or _native()).window_attention_backward(grad_out, query, key, value, out, lse, _scale(scale, query),
                                                              left, right, sinks, q_lengths, kv_lengths, grad_query,
                                                              grad_key, grad_value, workspace, _raw(stream))
+
+
+def layer_norm(x, weight=None, bias=None, residual=None, eps=1e-5, need_stats=False, out=None, sum_out=None, mean_out=None,
+               rstd_out=None, stream=None, workspace=None):
+    """Both phases of opscvLayerNorm: layer norm of x, or of x + residual, times weight plus bias (ones and zeros where they
+    are None), over the last dimension.  Returns (out, sum, mean, rstd): sum is x + residual (None without a residual), mean
+    and rstd what the backward call reads (None unless need_stats)."""
+    return (_helpers or _native()).layer_norm(x, weight, bias, residual, eps, need_stats, out, sum_out, mean_out, rstd_out,
+                                              workspace, _raw(stream))
+
+
+def layer_norm_backward(grad_y, sum_in, weight, mean, rstd, grad_sum=None, need_weight=True, need_bias=True, grad_x=None,
+                        grad_weight=None, grad_bias=None, stream=None, workspace=None):
+    """Both phases of opscvLayerNormBackward; returns (grad_x, grad_weight, grad_bias).  sum_in, mean and rstd are what the
+    forward call returned (sum_in = x without a residual), grad_sum the gradient that reaches the sum on its other way.
+    grad_x is the gradient of x and of the residual alike; grad_weight is None without a weight or need_weight, grad_bias
+    unless need_bias."""
+    return (_helpers or _native()).layer_norm_backward(grad_y, sum_in, weight, mean, rstd, grad_sum, need_weight, need_bias,
+                                                       grad_x, grad_weight, grad_bias, workspace, _raw(stream))
+
+
+def rotary_axes(query, key, table, positions, sections, layout=AXES_CONSECUTIVE, interleaved=False, inverse=False,
+                query_out=None, key_out=None, stream=None, workspace=None):
+    """Both phases of opscvRotaryAxes: rotary with positions on several axes, (axes, batch, tokens); sections holds the number
+    of pairs of each axis, layout how pairs are shared out.  Returns (query_out, key_out).  key may be None.  The outputs may
+    be the inputs.  inverse gives the gradient's way back.  The table is rotary_table's, of 2 * sum(sections) columns, with
+    AXES_RESTART of 2 * max(sections)."""
+    return (_helpers or _native()).rotary_axes(query, key, table, positions, sections, layout, interleaved, inverse,
+                                               query_out, key_out, workspace, _raw(stream))
+
+
+def dropout(x, state, p, residual=None, out=None, stream=None, workspace=None):
+    """Both phases of opscvDropout; returns residual + x / (1 - p) where an element is kept, residual (or 0) where not.  state
+    is an int64 tensor of seed and offset on x's device, read when the kernel runs: the same state gives the same mask, so the
+    gradient of x is dropout(grad, state, p).  Add to state[1] for another mask."""
+    return (_helpers or _native()).dropout(x, state, p, residual, out, workspace, _raw(stream))
+
+
+def gated_projection(x, gate_weight, up_weight, gate_bias=None, up_bias=None, activation=GATE_SILU, need_sums=False, out=None,
+                     gate_out=None, up_out=None, stream=None, workspace=None):
+    """Both phases of opscvGatedProjection: activation(x @ gate_weight.T + gate_bias) * (x @ up_weight.T + up_bias).  Returns
+    (out, gate, up): gate and up are the two sums before the activation, what the backward call reads (None unless
+    need_sums)."""
+    return (_helpers or _native()).gated_projection(x, gate_weight, up_weight, gate_bias, up_bias, activation, need_sums, out,
+                                                    gate_out, up_out, workspace, _raw(stream))
+
+
+def gated_projection_backward(grad_y, x, gate_weight, up_weight, gate, up, activation=GATE_SILU, need_x=True,
+                              need_weights=True, need_bias=False, grad_x=None, grad_gate_weight=None, grad_up_weight=None,
+                              grad_gate_bias=None, grad_up_bias=None, stream=None, workspace=None):
+    """Both phases of opscvGatedProjectionBackward; returns (grad_x, grad_gate_weight, grad_up_weight, grad_gate_bias,
+    grad_up_bias), None for those not wanted.  gate and up are what the forward call returned."""
+    return (_helpers or _native()).gated_projection_backward(grad_y, x, gate_weight, up_weight, gate, up, activation, need_x,
+                                                             need_weights, need_bias, grad_x, grad_gate_weight,
+                                                             grad_up_weight, grad_gate_bias, grad_up_bias, workspace,
+                                                             _raw(stream))
 
 
 def grid_sampler2d_taps(grid, h_in, w_in, interpolation_mode=0, padding_mode=0, align_corners=False, stream=None):

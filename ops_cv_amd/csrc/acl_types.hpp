@@ -83,7 +83,8 @@ struct StridedView {
 
 enum class OpKind : int { Nop = 0, GridSampler2D = 1, Resize = 2, ResizeGrad = 3, GridSampler3D = 4, GridSampler2DGrad = 5,
                           GridSampler3DGrad = 6, ResidualNorm = 7, ResidualNormGrad = 8, RotaryTable = 9, Rotary = 10,
-                          WindowAttention = 11, WindowAttentionGrad = 12 };
+                          WindowAttention = 11, WindowAttentionGrad = 12, LayerNorm = 13, LayerNormGrad = 14, Dropout = 15,
+                          Gated = 16, GatedGrad = 17, RotaryAxes = 18 };
 
 // Where a kernel operand lives: the tensor's own memory (contiguous view) or a slice of the caller's
 // workspace, known only as an offset until the second phase receives the workspace address.
@@ -224,6 +225,10 @@ struct aclOpExecutor {
     opscv::RotaryTableArgs rotary_table;
     opscv::RotaryArgs rotary;
     opscv::AttentionArgs attention;
+    opscv::LayerNormArgs layer_norm;
+    opscv::LayerNormGradArgs layer_norm_grad;
+    opscv::DropoutArgs dropout;
+    opscv::GatedArgs gated;
     int want_out0 = 1, want_out1 = 0;  // which outputs the operator produces (backward output mask)
     opscv::PlannedPtr in0, in1, out0;  // input/self, grid, out
     opscv::PlannedPtr in2, out1;       // third input and second output of the operators that have them
@@ -239,9 +244,9 @@ struct aclOpExecutor {
         uint64_t ws_offset = 0;
         int elem_bytes = 0;
     };
-    // at most five inputs and four outputs per operator; fixed storage, so that planning never touches the heap
+    // at most six inputs and five outputs per operator; fixed storage, so that planning never touches the heap
     struct PackList {
-        static constexpr int kCapacity = 5;
+        static constexpr int kCapacity = 6;
         Pack items[kCapacity];
         int count = 0;
         // false when the list is full (the entry is dropped: the caller must fail the plan)

@@ -125,6 +125,12 @@ const char* opscvExecutorVariant(const aclOpExecutor* executor)
         case OpKind::Rotary: return executor->rotary.interleaved != 0 ? "rotary_interleaved" : "rotary_halves";
         case OpKind::WindowAttention: return attention_variant(executor->attention);
         case OpKind::WindowAttentionGrad: return "attention_grad";
+        case OpKind::RotaryAxes: return "rotary_axes";
+        case OpKind::LayerNorm: return "layer_norm";
+        case OpKind::LayerNormGrad: return "layer_norm_grad";
+        case OpKind::Dropout: return "dropout";
+        case OpKind::Gated: return "gated_projection";
+        case OpKind::GatedGrad: return "gated_projection_grad";
         default: break;
     }
     return "";

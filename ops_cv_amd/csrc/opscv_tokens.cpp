@@ -1,234 +1,16 @@
 // Operators on token sequences: parameter validation, planning and the second-phase entries (include/opscv_tokens.h).
-#include <cmath>
-#include <cstring>
-#include <memory>
-#include <new>
-
-#include "executor.hpp"
-#include "kernels.hpp"
 #include "opscv_tokens.h"
 #include "token_kernels.hpp"
+#include "token_plan.hpp"
 
 using namespace opscv;
+using namespace opscv::tokplan;
 
 namespace {
 
-constexpr int64_t kMostExtent = (int64_t)1 << 30;
-constexpr int64_t kMostTokenStride = (int64_t)1 << 22;  // elements
 // tokens of a sequence and reaches of a window: sums of any three fit 32 bits
 constexpr int64_t kMostTokens = (int64_t)1 << 28;
 constexpr int64_t kMostHeadDim = 256;
-constexpr int64_t kMostRotaryDim = 1024;
-
-typedef std::unique_ptr<aclOpExecutor> Executor;
-
-// What both arguments that return something are checked for, and the executor of the call.
-aclnnStatus begin(const char* api, uint64_t* workspaceSize, aclOpExecutor** executor, Executor* ex)
-{
-    if (workspaceSize == nullptr || executor == nullptr) {
-        set_error("%s: workspaceSize and executor must not be NULL", api);
-        return ACLNN_ERR_PARAM_NULLPTR;
-    }
-    ex->reset(new (std::nothrow) aclOpExecutor());
-    if (!*ex) {
-        set_error("%s: cannot allocate the executor", api);
-        return ACLNN_ERR_INNER_CREATE_EXECUTOR;
-    }
-    return ACLNN_SUCCESS;
-}
-
-aclnnStatus finish(const char* api, Executor& ex, uint64_t* workspaceSize, aclOpExecutor** executor)
-{
-    if (const aclnnStatus ps = plan_status(ex.get(), api); ps != ACLNN_SUCCESS) {
-        return ps;
-    }
-    *workspaceSize = ex->workspace_bytes;
-    *executor = ex.release();
-    return ACLNN_SUCCESS;
-}
-
-aclnnStatus missing(const char* api, const char* names)
-{
-    set_error("%s: %s must not be NULL", api, names);
-    return ACLNN_ERR_PARAM_NULLPTR;
-}
-
-template <typename... A>
-aclnnStatus invalid(const char* format, A... a)
-{
-    set_error(format, a...);
-    return ACLNN_ERR_PARAM_INVALID;
-}
-
-bool same_dims(const aclTensor* a, const aclTensor* b)
-{
-    return a->ndim == b->ndim && memcmp(a->dims, b->dims, sizeof(int64_t) * (size_t)a->ndim) == 0;
-}
-
-// the leading dimensions of `t`, one value per row
-bool per_row(const aclTensor* r, const aclTensor* t)
-{
-    return r->ndim == t->ndim - 1 && memcmp(r->dims, t->dims, sizeof(int64_t) * (size_t)r->ndim) == 0;
-}
-
-bool extents_fit(const aclTensor* t)
-{
-    for (int64_t i = 0; i < t->ndim; i++) {
-        if (t->dims[i] > kMostExtent) {
-            return false;
-        }
-    }
-    return true;
-}
-
-// Operand `slot` of the executor: the tensor packed dense.
-void plan_dense(aclOpExecutor* ex, int slot, const aclTensor* t, int elem_bytes, bool output)
-{
-    ex->operands[slot] = plan_view(ex, t, elem_bytes, output);
-    ex->required |= t->empty() ? 0u : 1u << slot;
-}
-
-// Operand `slot`, used in place where its last dimension is dense, packed otherwise; the strides that the kernel walks.
-void plan_strided(aclOpExecutor* ex, int slot, const aclTensor* t, int elem_bytes, bool output, Strided* s)
-{
-    const int last = (int)t->ndim - 1;
-    bool in_place = t->dims[last] == 1 || t->strides[last] == 1;
-    // kernels walk up to 64 tokens, of which none begins inside another, from a 64-bit address with 32-bit offsets in bytes
-    for (int i = 0; i < last; i++) {
-        in_place = in_place && (t->dims[i] <= 1 || (t->strides[i] >= 0 && (i != 1 || (t->strides[i] >= t->dims[last] &&
-                                                                                       t->strides[i] <= kMostTokenStride))));
-    }
-    if (in_place) {
-        PlannedPtr p;
-        p.direct = (t->data == nullptr) ? nullptr : (char*)t->data + t->offset * (int64_t)elem_bytes;
-        ex->operands[slot] = p;
-        ex->required |= t->empty() ? 0u : 1u << slot;
-        for (int i = 0; i < last; i++) {
-            s->stride[i] = t->dims[i] > 1 ? t->strides[i] : (i == 1 ? t->dims[last] : 0);
-        }
-        return;
-    }
-    plan_dense(ex, slot, t, elem_bytes, output);
-    int64_t stride = t->dims[last];
-    for (int i = last - 1; i >= 0; i--) {
-        s->stride[i] = stride;
-        stride *= t->dims[i];
-    }
-}
-
-// Operand `slot` as rows of its last dimension: in place where the leading dimensions are evenly spaced rows.
-void plan_rows(aclOpExecutor* ex, int slot, const aclTensor* t, int elem_bytes, bool output, Rows* r)
-{
-    const int last = (int)t->ndim - 1;
-    bool even = t->dims[last] == 1 || t->strides[last] == 1;
-    int64_t stride = 0, expect = 0;  // of the innermost dimension of more than one row; of the next one outwards
-    for (int i = last - 1; i >= 0 && even; i--) {
-        if (t->dims[i] == 1) {
-            continue;
-        }
-        if (expect == 0) {
-            stride = t->strides[i];
-            expect = stride * t->dims[i];
-            even = stride > 0 || !output;
-        } else {
-            even = t->strides[i] == expect;
-            expect *= t->dims[i];
-        }
-        even = even && expect != 0;
-    }
-    if (even) {
-        PlannedPtr p;
-        p.direct = (t->data == nullptr) ? nullptr : (char*)t->data + t->offset * (int64_t)elem_bytes;
-        ex->operands[slot] = p;
-        ex->required |= t->empty() ? 0u : 1u << slot;
-        r->row_stride = stride;
-        return;
-    }
-    plan_dense(ex, slot, t, elem_bytes, output);
-    r->row_stride = t->dims[last];
-}
-
-// A vector or matrix of whole numbers, always read in place.
-void plan_whole(aclOpExecutor* ex, int slot, const aclTensor* t, Whole* w)
-{
-    w->wide = t->dtype == ACL_INT64 ? 1 : 0;
-    for (int i = 0; i < t->ndim; i++) {
-        w->stride[i] = t->strides[i];
-    }
-    ex->operands[slot].direct = (t->data == nullptr) ? nullptr : (char*)t->data + t->offset * (w->wide ? 8 : 4);
-    ex->required |= t->empty() ? 0u : 1u << slot;
-}
-
-void plan_scratch(aclOpExecutor* ex, int slot, int64_t floats)
-{
-    if (floats > 0) {
-        PlannedPtr p;
-        p.in_workspace = true;
-        p.ws_offset = (ex->workspace_bytes + 255) / 256 * 256;
-        ex->workspace_bytes = p.ws_offset + (uint64_t)floats * 4;
-        ex->operands[slot] = p;
-    }
-}
-
-bool whole_type(const aclTensor* t) { return t->dtype == ACL_INT32 || t->dtype == ACL_INT64; }
-
-// Weight of a norm: (width), of the activations' type or FLOAT.
-aclnnStatus check_weight(const char* api, const char* name, const aclTensor* w, const aclTensor* x)
-{
-    if (w->ndim != 1 || w->dims[0] != x->dims[x->ndim - 1]) {
-        return invalid("%s: %s must have one dimension, the width of the rows", api, name);
-    }
-    if (w->dtype != x->dtype && w->dtype != ACL_FLOAT) {
-        return invalid("%s: %s must have the type of the rows or FLOAT", api, name);
-    }
-    return ACLNN_SUCCESS;
-}
-
-// Rows of one type and shape
-aclnnStatus check_rows(const char* api, const char* name, const aclTensor* t, const aclTensor* like, bool dtype = true)
-{
-    if (!same_dims(t, like)) {
-        return invalid("%s: %s has another shape than the other rows", api, name);
-    }
-    if (dtype && t->dtype != like->dtype) {
-        return invalid("%s: %s has another type than the other rows", api, name);
-    }
-    return ACLNN_SUCCESS;
-}
-
-aclnnStatus check_row_values(const char* api, const char* name, const aclTensor* t, const aclTensor* like)
-{
-    if (!per_row(t, like) || t->dtype != ACL_FLOAT) {
-        return invalid("%s: %s must hold one FLOAT per row", api, name);
-    }
-    return ACLNN_SUCCESS;
-}
-
-#define OPSCV_CHECK(call)                                    \
-    if (const aclnnStatus st_ = (call); st_ != ACLNN_SUCCESS) { \
-        return st_;                                          \
-    }
-
-// What the rows of a norm must be; their number and width.
-aclnnStatus norm_rows(const char* api, const aclTensor* x, Elem* e, int64_t* rows, int64_t* width)
-{
-    if (x->ndim < 1 || x->ndim > kViewDims) {
-        return invalid("%s: rows have one to %d dimensions, got %lld", api, kViewDims, (long long)x->ndim);
-    }
-    if (!elem_of(x->dtype, e)) {
-        return invalid("%s: dtype %d is not in {FLOAT, FLOAT16, BF16}", api, (int)x->dtype);
-    }
-    *width = x->dims[x->ndim - 1];
-    *rows = 1;
-    for (int i = 0; i + 1 < x->ndim; i++) {
-        *rows *= x->dims[i];
-    }
-    if (*width < 1 || *width > kMostExtent || *rows > INT32_MAX) {
-        return invalid("%s: rows of 1 to 2^30 elements and fewer than 2^31 rows, got %lld by %lld", api, (long long)*rows,
-                       (long long)*width);
-    }
-    return ACLNN_SUCCESS;
-}
 
 // The operands that attention's two directions share.
 aclnnStatus check_attention(const char* api, const aclTensor* q, const aclTensor* k, const aclTensor* v,
@@ -306,6 +88,118 @@ enum RotarySlot { kRoQuery, kRoKey, kRoPositions, kRoTable, kRoQueryOut, kRoKeyO
 enum AttentionSlot { kAtQ, kAtK, kAtV, kAtQLengths, kAtKvLengths, kAtOut, kAtLse, kAtGradOut, kAtGradQ, kAtGradK, kAtGradV,
                      kAtScratch };
 
+// Sections and layout of opscvRotaryAxes, and the columns of its table.
+aclnnStatus rotary_axes(const char* api, const aclIntArray* sections, int64_t layout, const aclTensor* table, RotaryArgs* a)
+{
+    if (sections->v.empty() || sections->v.size() > 4) {
+        return invalid("%s: one to four axes, got %lld sections", api, (long long)sections->v.size());
+    }
+    if (layout < OPSCV_AXES_CONSECUTIVE || layout > OPSCV_AXES_DEALT) {
+        return invalid("%s: unknown layout %lld", api, (long long)layout);
+    }
+    a->axes = (int)sections->v.size();
+    a->layout = (int)layout;
+    int64_t pairs = 0, most = 0;
+    for (int i = 0; i < a->axes; i++) {
+        const int64_t n = sections->v[(size_t)i];
+        if (n < 0 || n > kMostRotaryDim / 2) {
+            return invalid("%s: sections of 0 to %lld pairs, got %lld", api, (long long)(kMostRotaryDim / 2), (long long)n);
+        }
+        a->sections[i] = n;
+        pairs += n;
+        most = n > most ? n : most;
+    }
+    a->rot = 2 * pairs;
+    a->columns = layout == OPSCV_AXES_RESTART ? most : pairs;
+    if (table->dims[1] != 2 * a->columns) {
+        return invalid("%s: table must have %lld columns, got %lld", api, (long long)(2 * a->columns),
+                       (long long)table->dims[1]);
+    }
+    return ACLNN_SUCCESS;
+}
+
+// First phase of opscvRotary, and with `sections` of opscvRotaryAxes.
+aclnnStatus rotary_plan(const char* api, OpKind kind, const aclTensor* query, const aclTensor* key,
+                        const aclTensor* positions, const aclTensor* table, const aclIntArray* sections, int64_t layout,
+                        bool interleaved, bool inverse, aclTensor* queryOut, aclTensor* keyOut, uint64_t* workspaceSize,
+                        aclOpExecutor** executor)
+{
+    Executor ex;
+    OPSCV_CHECK(begin(api, workspaceSize, executor, &ex));
+    if (query == nullptr || table == nullptr || queryOut == nullptr || (key == nullptr) != (keyOut == nullptr)) {
+        return missing(api, "query, table and queryOut, and one of key and keyOut beside the other,");
+    }
+    if (kind == OpKind::RotaryAxes && (sections == nullptr || positions == nullptr)) {
+        return missing(api, "positions and sections");
+    }
+    Elem e;
+    if (query->ndim != 4 || !elem_of(query->dtype, &e)) {
+        return invalid("%s: query must be (batch, tokens, heads, d) of {FLOAT, FLOAT16, BF16}", api);
+    }
+    OPSCV_CHECK(check_rows(api, "queryOut", queryOut, query));
+    RotaryArgs& a = ex->rotary;
+    a.elem = (int)e;
+    a.batch = query->dims[0];
+    a.tokens = query->dims[1];
+    a.heads = query->dims[2];
+    a.d = query->dims[3];
+    if (key != nullptr) {
+        if (key->ndim != 4 || key->dtype != query->dtype || key->dims[0] != a.batch || key->dims[1] != a.tokens ||
+            key->dims[3] != a.d) {
+            return invalid("%s: key must have query's type, batch, tokens and head size", api);
+        }
+        OPSCV_CHECK(check_rows(api, "keyOut", keyOut, key));
+        a.kv_heads = key->dims[2];
+    }
+    if (table->ndim != 2 || table->dtype != ACL_FLOAT) {
+        return invalid("%s: table must be FLOAT (positions, rot)", api);
+    }
+    a.positions = table->dims[0];
+    a.rot = table->dims[1];
+    a.columns = a.rot / 2;
+    if (kind == OpKind::RotaryAxes) {
+        OPSCV_CHECK(rotary_axes(api, sections, layout, table, &a));
+    }
+    if (a.d < 1 || a.d > kMostRotaryDim || a.rot % 2 != 0 || a.rot < 2 || a.rot > a.d) {
+        return invalid("%s: an even number of rotated features out of 2 to %lld, got %lld of %lld", api,
+                       (long long)kMostRotaryDim, (long long)a.rot, (long long)a.d);
+    }
+    const int lead = kind == OpKind::RotaryAxes ? 1 : 0;
+    if (positions != nullptr &&
+        (positions->ndim != 2 + lead || (lead != 0 && positions->dims[0] != a.axes) ||
+         positions->dims[lead] != a.batch || positions->dims[lead + 1] != a.tokens || !whole_type(positions))) {
+        return invalid("%s: positions must be INT32 or INT64 (%sbatch, tokens)", api, lead != 0 ? "axes, " : "");
+    }
+    if (!extents_fit(query) || !extents_fit(table) || a.kv_heads > kMostExtent || a.batch * a.tokens > INT32_MAX) {
+        return invalid("%s: extents too large", api);
+    }
+    if (a.batch == 0 || a.tokens == 0 || a.heads + a.kv_heads == 0) {
+        return finish(api, ex, workspaceSize, executor);
+    }
+    ex->kind = kind;
+    a.interleaved = interleaved ? 1 : 0;
+    a.inverse = inverse ? 1 : 0;
+    const int bytes = elem_size(e);
+    plan_strided(ex.get(), kRoQuery, query, bytes, false, &a.query);
+    plan_strided(ex.get(), kRoQueryOut, queryOut, bytes, true, &a.query_out);
+    if (key != nullptr) {
+        plan_strided(ex.get(), kRoKey, key, bytes, false, &a.key);
+        plan_strided(ex.get(), kRoKeyOut, keyOut, bytes, true, &a.key_out);
+    }
+    if (positions != nullptr) {
+        plan_whole(ex.get(), kRoPositions, positions, &a.position);
+        if (lead != 0) {
+            a.position.axis_stride = positions->strides[0];
+            a.position.stride[0] = positions->strides[1];
+            a.position.stride[1] = positions->strides[2];
+        }
+    }
+    Rows r;
+    plan_rows(ex.get(), kRoTable, table, 4, false, &r);
+    a.table_stride = r.row_stride;
+    return finish(api, ex, workspaceSize, executor);
+}
+
 }  // namespace
 
 namespace opscv {
@@ -352,7 +246,8 @@ aclnnStatus execute_token_plan(void* workspace, const aclOpExecutor* ex, hipStre
             *e = launch_rotary_table(a, stream);
             break;
         }
-        case OpKind::Rotary: {
+        case OpKind::Rotary:
+        case OpKind::RotaryAxes: {
             RotaryArgs a = ex->rotary;
             a.query.ptr = at(kRoQuery);
             a.key.ptr = at(kRoKey);
@@ -363,6 +258,11 @@ aclnnStatus execute_token_plan(void* workspace, const aclOpExecutor* ex, hipStre
             *e = launch_rotary(a, stream);
             break;
         }
+        case OpKind::LayerNorm:
+        case OpKind::LayerNormGrad:
+        case OpKind::Dropout:
+        case OpKind::Gated:
+        case OpKind::GatedGrad: *e = launch_block_plan(workspace, ex, stream); break;
         default: {
             AttentionArgs a = ex->attention;
             a.q.ptr = at(kAtQ);
@@ -570,72 +470,27 @@ aclnnStatus opscvRotaryGetWorkspaceSize(const aclTensor* query, const aclTensor*
                                         const aclTensor* table, bool interleaved, bool inverse, aclTensor* queryOut,
                                         aclTensor* keyOut, uint64_t* workspaceSize, aclOpExecutor** executor)
 {
-    const char* const api = "opscvRotary";
-    Executor ex;
-    OPSCV_CHECK(begin(api, workspaceSize, executor, &ex));
-    if (query == nullptr || table == nullptr || queryOut == nullptr || (key == nullptr) != (keyOut == nullptr)) {
-        return missing(api, "query, table and queryOut, and one of key and keyOut beside the other,");
-    }
-    Elem e;
-    if (query->ndim != 4 || !elem_of(query->dtype, &e)) {
-        return invalid("%s: query must be (batch, tokens, heads, d) of {FLOAT, FLOAT16, BF16}", api);
-    }
-    OPSCV_CHECK(check_rows(api, "queryOut", queryOut, query));
-    RotaryArgs& a = ex->rotary;
-    a.elem = (int)e;
-    a.batch = query->dims[0];
-    a.tokens = query->dims[1];
-    a.heads = query->dims[2];
-    a.d = query->dims[3];
-    if (key != nullptr) {
-        if (key->ndim != 4 || key->dtype != query->dtype || key->dims[0] != a.batch || key->dims[1] != a.tokens ||
-            key->dims[3] != a.d) {
-            return invalid("%s: key must have query's type, batch, tokens and head size", api);
-        }
-        OPSCV_CHECK(check_rows(api, "keyOut", keyOut, key));
-        a.kv_heads = key->dims[2];
-    }
-    if (table->ndim != 2 || table->dtype != ACL_FLOAT) {
-        return invalid("%s: table must be FLOAT (positions, rot)", api);
-    }
-    a.positions = table->dims[0];
-    a.rot = table->dims[1];
-    if (a.d < 1 || a.d > kMostRotaryDim || a.rot % 2 != 0 || a.rot < 2 || a.rot > a.d) {
-        return invalid("%s: an even number of rotated features out of 2 to %lld, got %lld of %lld", api,
-                       (long long)kMostRotaryDim, (long long)a.rot, (long long)a.d);
-    }
-    if (positions != nullptr && (positions->ndim != 2 || positions->dims[0] != a.batch || positions->dims[1] != a.tokens ||
-                                 !whole_type(positions))) {
-        return invalid("%s: positions must be INT32 or INT64 (batch, tokens)", api);
-    }
-    if (!extents_fit(query) || !extents_fit(table) || a.kv_heads > kMostExtent || a.batch * a.tokens > INT32_MAX) {
-        return invalid("%s: extents too large", api);
-    }
-    if (a.batch == 0 || a.tokens == 0 || a.heads + a.kv_heads == 0) {
-        return finish(api, ex, workspaceSize, executor);
-    }
-    ex->kind = OpKind::Rotary;
-    a.interleaved = interleaved ? 1 : 0;
-    a.inverse = inverse ? 1 : 0;
-    const int bytes = elem_size(e);
-    plan_strided(ex.get(), kRoQuery, query, bytes, false, &a.query);
-    plan_strided(ex.get(), kRoQueryOut, queryOut, bytes, true, &a.query_out);
-    if (key != nullptr) {
-        plan_strided(ex.get(), kRoKey, key, bytes, false, &a.key);
-        plan_strided(ex.get(), kRoKeyOut, keyOut, bytes, true, &a.key_out);
-    }
-    if (positions != nullptr) {
-        plan_whole(ex.get(), kRoPositions, positions, &a.position);
-    }
-    Rows r;
-    plan_rows(ex.get(), kRoTable, table, 4, false, &r);
-    a.table_stride = r.row_stride;
-    return finish(api, ex, workspaceSize, executor);
+    return rotary_plan("opscvRotary", OpKind::Rotary, query, key, positions, table, nullptr, 0, interleaved, inverse,
+                       queryOut, keyOut, workspaceSize, executor);
 }
 
 aclnnStatus opscvRotary(void* workspace, uint64_t workspaceSize, aclOpExecutor* executor, aclrtStream stream)
 {
     return run_executor(workspace, workspaceSize, executor, stream, OpKind::Rotary, "opscvRotary");
+}
+
+aclnnStatus opscvRotaryAxesGetWorkspaceSize(const aclTensor* query, const aclTensor* key, const aclTensor* positions,
+                                            const aclTensor* table, const aclIntArray* sections, int64_t layout,
+                                            bool interleaved, bool inverse, aclTensor* queryOut, aclTensor* keyOut,
+                                            uint64_t* workspaceSize, aclOpExecutor** executor)
+{
+    return rotary_plan("opscvRotaryAxes", OpKind::RotaryAxes, query, key, positions, table, sections, layout, interleaved,
+                       inverse, queryOut, keyOut, workspaceSize, executor);
+}
+
+aclnnStatus opscvRotaryAxes(void* workspace, uint64_t workspaceSize, aclOpExecutor* executor, aclrtStream stream)
+{
+    return run_executor(workspace, workspaceSize, executor, stream, OpKind::RotaryAxes, "opscvRotaryAxes");
 }
 
 aclnnStatus opscvWindowAttentionGetWorkspaceSize(const aclTensor* query, const aclTensor* key, const aclTensor* value,

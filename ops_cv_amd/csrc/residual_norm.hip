@@ -16,6 +16,7 @@
 
 #include "token_elem.hpp"
 #include "token_kernels.hpp"
+#include "token_rows.hpp"
 
 namespace opscv {
 
@@ -23,11 +24,7 @@ using namespace tok;
 
 namespace {
 
-constexpr int kMostPerLane = 32;   // elements of a row that a thread keeps in registers
-constexpr int64_t kMostBlocks = 1 << 20;  // more rows than these take are walked
 constexpr int kPartialRows = 512;  // rows of partial sums of the weight's gradient: two workgroups per CU
-
-dim3 grid(int64_t blocks) { return dim3((unsigned)(blocks < kMostBlocks ? blocks : kMostBlocks)); }
 
 // Sum (and, with `most`, largest value) over the threads of a row: THREADS of them, 64 or a whole workgroup.  `slot`
 // alternates between calls, so that one barrier a call is enough.
@@ -278,34 +275,6 @@ hipError_t run_norm_type(const NormArgs& a, hipStream_t stream)
 
 // ------------------------------------------------------------------------------------------------------ gradients
 
-// Sums over the threads of `R` rows at once, as row_reduce.
-template <int THREADS, int R>
-__device__ __forceinline__ void rows_reduce(float (&sum)[R], float (*shared)[R][16], int slot)
-{
-#pragma unroll
-    for (int k = 0; k < R; k++) {
-        sum[k] = wave_sum(sum[k]);
-    }
-    if constexpr (THREADS > 64) {
-        const int wave = (int)threadIdx.x >> 6;
-        if ((threadIdx.x & 63) == 0) {
-#pragma unroll
-            for (int k = 0; k < R; k++) {
-                shared[slot][k][wave] = sum[k];
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < R; k++) {
-            sum[k] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < THREADS / 64; i++) {
-                sum[k] += shared[slot][k][i];
-            }
-        }
-    }
-}
-
 // Gradient of the rows, and of the weight's columns over the rows of one workgroup, which it adds up in registers and
 // leaves in its row of `partial`.  THREADS per row; wavefronts of 64-thread rows join their sums through LDS.  R rows at a
 // time, as many as a thread's registers hold, so that enough loads are under way with two workgroups a CU (more of them
@@ -492,32 +461,6 @@ __global__ __launch_bounds__(256) void norm_weight_long_kernel(NormGradArgs a)
     a.partial[(int64_t)blockIdx.y * a.width + c] = total;
 }
 
-// Sum of the rows of `partial`: 32 columns a workgroup, every eighth row a thread, joined in order.
-template <typename W>
-__global__ __launch_bounds__(256) void norm_weight_kernel(const float* __restrict__ partial, int64_t rows, int64_t width,
-                                                          W* __restrict__ out)
-{
-    __shared__ float shared[8][32];
-    const int column = (int)threadIdx.x & 31, part = (int)threadIdx.x >> 5;
-    const int64_t c = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 32 + column;
-    float total = 0.0f;
-    if (c < width) {
-#pragma unroll 8
-        for (int64_t r = part; r < rows; r += 8) {
-            total += partial[r * width + c];
-        }
-    }
-    shared[part][column] = total;
-    __syncthreads();
-    if (part == 0 && c < width) {
-#pragma unroll
-        for (int i = 1; i < 8; i++) {
-            total += shared[i][column];
-        }
-        out[c] = (W)total;
-    }
-}
-
 template <typename T, typename W, int THREADS, int NV, int VEC, bool WIDE>
 void launch_norm_grad(const NormGradArgs& a, hipStream_t stream)
 {
@@ -560,12 +503,7 @@ hipError_t run_norm_grad(const NormGradArgs& a, hipStream_t stream)
         }
     }
     if (a.grad_weight != nullptr && !joined) {
-        // rows of more than 2^25 columns take more than one row of workgroups: 2^24 of 256 threads are more than a launch holds
-        // in one
-        const int64_t blocks = (a.width + 31) / 32;
-        const dim3 columns((unsigned)(blocks < kMostBlocks ? blocks : kMostBlocks), (unsigned)((blocks + kMostBlocks - 1) / kMostBlocks));
-        hipLaunchKernelGGL((norm_weight_kernel<W>), columns, dim3(256), 0, stream, a.partial, partials, a.width,
-                           (W*)a.grad_weight);
+        launch_column_sums<W>(a.partial, partials, a.width, (W*)a.grad_weight, stream);
     }
     return hipGetLastError();
 }
@@ -581,17 +519,6 @@ hipError_t run_norm_grad_type(const NormGradArgs& a, hipStream_t stream)
                          aligned(a.grad_x.ptr, a.grad_x.row_stride, e, 16) &&
                          aligned(a.weight, 0, 1, kVec * (int)sizeof(W));
     return vectors ? run_norm_grad<T, W, kVec, true>(a, stream) : run_norm_grad<T, W, kVec, false>(a, stream);
-}
-
-// f(T, W) by the operands' types
-template <typename F>
-hipError_t by_type(int elem, int weight_float, F&& f)
-{
-    switch ((Elem)elem) {
-        case Elem::F32: return f((float*)nullptr, (float*)nullptr);
-        case Elem::F16: return weight_float != 0 ? f((_Float16*)nullptr, (float*)nullptr) : f((_Float16*)nullptr, (_Float16*)nullptr);
-        default: return weight_float != 0 ? f((__bf16*)nullptr, (float*)nullptr) : f((__bf16*)nullptr, (__bf16*)nullptr);
-    }
 }
 
 }  // namespace

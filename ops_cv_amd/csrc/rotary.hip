@@ -6,7 +6,8 @@
 // positions, because a 32-bit product of a position and a frequency loses the angle's fraction far into a long context
 // (position 100000: a hundredth of a radian); the table is computed in 64 bits and costs rot * 4 bytes a token against
 // the heads' 4 d bytes each.  A thread owns a few features (16 bytes, or two halves of a pair group of 16 bytes each) of
-// up to eight heads of one token, so that it reads its cosines and sines once for them.  Two prompts of 4096 tokens, 32 and
+// up to eight heads of one token, so that it reads its cosines and sines once for them.  With positions on several axes a
+// thread's pairs take theirs from the row of their axis: whole vectors where all are of one, else pair by pair.  Two prompts of 4096 tokens, 32 and
 // 8 heads of 128, bf16: 34.4 us, 5.0 TB/s; one token of each of 64 sequences: 6.3, the launch.
 #include <hip/hip_runtime.h>
 
@@ -25,6 +26,7 @@ using namespace tok;
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kMostPairs = 512;  // rot <= 1024
 
 // Frequency of pair i: the angle of position 1.
 double rotary_frequency(const RotaryTableArgs& a, int64_t i)
@@ -45,8 +47,6 @@ double rotary_frequency(const RotaryTableArgs& a, int64_t i)
     return f;
 }
 
-constexpr int kMostPairs = 512;  // rot <= 1024
-
 struct Frequencies {
     double f[kMostPairs];
 };
@@ -65,6 +65,15 @@ __global__ __launch_bounds__(kThreads) void rotary_table_kernel(RotaryTableArgs 
     }
 }
 
+// How the pairs of a head are shared out to several axes.
+struct AxesPlan {
+    int uniform = 0;                         // every thread's pairs are of one axis and side by side in the table
+    uint16_t column[kMostPairs] = {0};       // of the table, for every pair
+    uint8_t axis[kMostPairs] = {0};
+};
+struct NoAxes {};
+
+template <bool AXES>
 struct RotaryPlan {
     RotaryArgs a;
     FastDiv units, groups, tokens;  // units of a head, groups of heads, tokens of a sequence
@@ -72,19 +81,73 @@ struct RotaryPlan {
     int wide_table;                 // the table's rows start on 16 bytes
     int streaming;
     uint32_t total;                 // threads with work
+    std::conditional_t<AXES, AxesPlan, NoAxes> axes;
 };
 
-__device__ __forceinline__ int64_t whole_at(const Whole& w, int64_t i, int64_t j)
+// The axis and the table's column of every pair (opscvAxesLayout).
+AxesPlan share_out(const RotaryArgs& a, int64_t pairs_a_thread)
 {
-    const int64_t at = i * w.stride[0] + j * w.stride[1];
+    AxesPlan p;
+    int64_t done[4] = {0, 0, 0, 0}, pair = 0;
+    for (int64_t turn = 0; pair < a.rot / 2; turn++) {
+        for (int axis = 0; axis < a.axes; axis++) {
+            const int64_t take = a.layout == OPSCV_AXES_DEALT ? (done[axis] < a.sections[axis] ? 1 : 0)
+                                                              : (turn == 0 ? a.sections[axis] : 0);
+            for (int64_t i = 0; i < take; i++, pair++, done[axis]++) {
+                p.axis[pair] = (uint8_t)axis;
+                p.column[pair] = (uint16_t)(a.layout == OPSCV_AXES_RESTART ? done[axis] : pair);
+            }
+        }
+    }
+    p.uniform = 1;
+    for (int64_t i = 0; i < pair; i++) {
+        const int64_t first = i / pairs_a_thread * pairs_a_thread;
+        if (p.axis[i] != p.axis[first] || p.column[i] != p.column[first] + (i - first) ||
+            p.column[first] % pairs_a_thread != 0) {
+            p.uniform = 0;
+        }
+    }
+    return p;
+}
+
+__device__ __forceinline__ int64_t whole_at(const Whole& w, int64_t i, int64_t j, int64_t axis = 0)
+{
+    const int64_t at = i * w.stride[0] + j * w.stride[1] + axis * w.axis_stride;
     return w.wide != 0 ? ((const int64_t*)w.ptr)[at] : (int64_t)((const int32_t*)w.ptr)[at];
+}
+
+// Cosines and sines of PAIRS pairs from `pair` on, side by side in a row of the table.
+template <int PAIRS>
+__device__ __forceinline__ void read_angles(const float* row, int64_t columns, bool wide, float (&cosine)[PAIRS],
+                                            float (&sine)[PAIRS])
+{
+    if constexpr (PAIRS % 4 == 0) {
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < PAIRS; i += 4) {
+                const Pack<float, 4> x = *reinterpret_cast<const Pack<float, 4>*>(row + i);
+                const Pack<float, 4> y = *reinterpret_cast<const Pack<float, 4>*>(row + columns + i);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    cosine[i + e] = x.v[e];
+                    sine[i + e] = y.v[e];
+                }
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < PAIRS; i++) {
+        cosine[i] = row[i];
+        sine[i] = row[columns + i];
+    }
 }
 
 // HEADS heads a thread, VEC features a vector.  A unit that turns is VEC / 2 interleaved pairs (one vector), or VEC pairs
 // of features half a rotation apart (two vectors); a unit that copies is one vector.  Single elements (VEC 1) serve both
 // orders as two vectors.
-template <typename T, int VEC, int HEADS, bool INTERLEAVED>
-__global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryPlan p)
+template <typename T, int VEC, int HEADS, bool INTERLEAVED, bool AXES>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryPlan<AXES> p)
 {
     constexpr int kPairs = INTERLEAVED ? VEC / 2 : VEC;
     const RotaryArgs& a = p.a;
@@ -104,42 +167,51 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryPlan p)
         const bool neighbours = INTERLEAVED || (VEC == 1 && a.interleaved != 0);
         first = neighbours ? 2 * pair : pair;
         second = neighbours ? first + 1 : half + pair;
-        const int64_t at = a.position.ptr != nullptr ? whole_at(a.position, b, t) : (int64_t)t;
-        if (at >= 0 && at < a.positions) {
-            const float* const row = a.table + at * a.table_stride + pair;
-            bool read = false;
-            if constexpr (kPairs % 4 == 0) {
-                if (p.wide_table != 0) {
-                    read = true;
+        if constexpr (AXES) {
+            if (p.axes.uniform != 0) {
+                const int64_t at = whole_at(a.position, b, t, p.axes.axis[pair]);
+                if (at >= 0 && at < a.positions) {
+                    read_angles<kPairs>(a.table + at * a.table_stride + p.axes.column[pair], a.columns, p.wide_table != 0,
+                                        cosine, sine);
+                } else {
 #pragma unroll
-                    for (int i = 0; i < kPairs; i += 4) {
-                        const Pack<float, 4> x = *reinterpret_cast<const Pack<float, 4>*>(row + i);
-                        const Pack<float, 4> y = *reinterpret_cast<const Pack<float, 4>*>(row + half + i);
+                    for (int i = 0; i < kPairs; i++) {
+                        cosine[i] = sine[i] = NAN;
+                    }
+                }
+            } else {
+                int64_t at[4];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            cosine[i + e] = x.v[e];
-                            sine[i + e] = y.v[e];
-                        }
+                for (int i = 0; i < 4; i++) {
+                    at[i] = i < a.axes ? whole_at(a.position, b, t, i) : 0;
+                }
+#pragma unroll
+                for (int i = 0; i < kPairs; i++) {
+                    const int axis = p.axes.axis[pair + i];
+                    const int64_t own = axis == 0 ? at[0] : axis == 1 ? at[1] : axis == 2 ? at[2] : at[3];
+                    cosine[i] = sine[i] = NAN;
+                    if (own >= 0 && own < a.positions) {
+                        const float* const from = a.table + own * a.table_stride + p.axes.column[pair + i];
+                        cosine[i] = from[0];
+                        sine[i] = from[a.columns];
                     }
                 }
             }
-            if (!read) {
-#pragma unroll
-                for (int i = 0; i < kPairs; i++) {
-                    cosine[i] = row[i];
-                    sine[i] = row[half + i];
-                }
-            }
-            if (a.inverse != 0) {
-#pragma unroll
-                for (int i = 0; i < kPairs; i++) {
-                    sine[i] = -sine[i];
-                }
-            }
         } else {
+            const int64_t at = a.position.ptr != nullptr ? whole_at(a.position, b, t) : (int64_t)t;
+            if (at >= 0 && at < a.positions) {
+                read_angles<kPairs>(a.table + at * a.table_stride + pair, half, p.wide_table != 0, cosine, sine);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kPairs; i++) {
+                    cosine[i] = sine[i] = NAN;
+                }
+            }
+        }
+        if (a.inverse != 0) {
 #pragma unroll
             for (int i = 0; i < kPairs; i++) {
-                cosine[i] = sine[i] = NAN;
+                sine[i] = -sine[i];
             }
         }
     } else {
@@ -187,7 +259,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryPlan p)
     }
 }
 
-template <typename T, int VEC, bool INTERLEAVED>
+template <typename T, int VEC, bool INTERLEAVED, bool AXES>
 hipError_t run(const RotaryArgs& a, hipStream_t stream)
 {
     const int64_t pairs = INTERLEAVED ? VEC / 2 : VEC;
@@ -212,7 +284,7 @@ hipError_t run(const RotaryArgs& a, hipStream_t stream)
     };
     for (int64_t b = 0; b < a.batch; b += sequences) {
         for (int64_t t = 0; t < a.tokens; t += span) {
-            RotaryPlan p;
+            RotaryPlan<AXES> p;
             p.a = a;
             p.a.batch = a.batch - b < sequences ? a.batch - b : sequences;
             p.a.tokens = a.tokens - t < span ? a.tokens - t : span;
@@ -231,17 +303,20 @@ hipError_t run(const RotaryArgs& a, hipStream_t stream)
             p.tokens = make_fast_div((uint32_t)p.a.tokens);
             p.turned = (uint32_t)turned;
             p.streaming = tokens * heads * a.d * (int64_t)sizeof(T) >= kStreamBytes ? 1 : 0;
-            p.wide_table = aligned(p.a.table, a.table_stride, 4, 16) && a.rot / 2 % 4 == 0 ? 1 : 0;
+            p.wide_table = aligned(p.a.table, a.table_stride, 4, 16) && a.columns % 4 == 0 ? 1 : 0;
+            if constexpr (AXES) {
+                p.axes = share_out(a, pairs);
+            }
             p.total = (uint32_t)(p.a.batch * p.a.tokens * per_token);
             const dim3 grid((p.total + kThreads - 1) / kThreads);
             if (each == 8) {
-                hipLaunchKernelGGL((rotary_kernel<T, VEC, 8, INTERLEAVED>), grid, dim3(kThreads), 0, stream, p);
+                hipLaunchKernelGGL((rotary_kernel<T, VEC, 8, INTERLEAVED, AXES>), grid, dim3(kThreads), 0, stream, p);
             } else if (each == 4) {
-                hipLaunchKernelGGL((rotary_kernel<T, VEC, 4, INTERLEAVED>), grid, dim3(kThreads), 0, stream, p);
+                hipLaunchKernelGGL((rotary_kernel<T, VEC, 4, INTERLEAVED, AXES>), grid, dim3(kThreads), 0, stream, p);
             } else if (each == 2) {
-                hipLaunchKernelGGL((rotary_kernel<T, VEC, 2, INTERLEAVED>), grid, dim3(kThreads), 0, stream, p);
+                hipLaunchKernelGGL((rotary_kernel<T, VEC, 2, INTERLEAVED, AXES>), grid, dim3(kThreads), 0, stream, p);
             } else {
-                hipLaunchKernelGGL((rotary_kernel<T, VEC, 1, INTERLEAVED>), grid, dim3(kThreads), 0, stream, p);
+                hipLaunchKernelGGL((rotary_kernel<T, VEC, 1, INTERLEAVED, AXES>), grid, dim3(kThreads), 0, stream, p);
             }
         }
     }
@@ -259,9 +334,10 @@ hipError_t run_widest(const RotaryArgs& a, hipStream_t stream)
             fits = fits && aligned(s->ptr, s->stride[0], e, bytes) && aligned(s->ptr, s->stride[1], e, bytes) &&
                    aligned(s->ptr, s->stride[2], e, bytes);
         }
-        return fits ? run<T, VEC, INTERLEAVED>(a, stream) : run_widest<T, INTERLEAVED, VEC / 2>(a, stream);
+        return fits ? (a.axes != 0 ? run<T, VEC, INTERLEAVED, true>(a, stream) : run<T, VEC, INTERLEAVED, false>(a, stream))
+                    : run_widest<T, INTERLEAVED, VEC / 2>(a, stream);
     } else {
-        return run<T, 1, false>(a, stream);
+        return a.axes != 0 ? run<T, 1, false, true>(a, stream) : run<T, 1, false, false>(a, stream);
     }
 }
 

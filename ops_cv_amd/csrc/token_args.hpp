@@ -11,10 +11,11 @@ struct Strided {
     int64_t stride[3] = {0, 0, 0};
 };
 
-// A vector of whole numbers (lengths), or a matrix of them (positions).
+// A vector of whole numbers (lengths), or a matrix of them (positions; by axes first, if there are several).
 struct Whole {
     const void* ptr = nullptr;
     int64_t stride[2] = {0, 0};
+    int64_t axis_stride = 0;
     int wide = 0;  // 1: 64 bits, 0: 32 bits
 };
 
@@ -48,6 +49,66 @@ struct NormGradArgs {
     float* partial = nullptr;     // norm_grad_partials() rows of `width` sums, with grad_weight only
 };
 
+struct LayerNormArgs {
+    int elem = 0;          // Elem of x, residual, sum and y
+    int weight_float = 0;  // weight and bias in FLOAT where elem is another type
+    int streaming = 0;     // set by the launcher
+    int64_t rows = 0, width = 0;
+    float eps = 0.0f;
+    Rows x, residual, y, sum;  // residual and sum: ptr may be null
+    const void* weight = nullptr;  // may be null: ones
+    const void* bias = nullptr;    // may be null: zeros
+    float* mean = nullptr;
+    float* rstd = nullptr;
+};
+
+struct LayerNormGradArgs {
+    int elem = 0;
+    int weight_float = 0;
+    int64_t rows = 0, width = 0;
+    Rows grad_y, grad_sum, sum, grad_x;  // grad_sum: ptr may be null
+    const void* weight = nullptr;        // may be null: ones
+    const float* mean = nullptr;
+    const float* rstd = nullptr;
+    void* grad_weight = nullptr;  // may be null
+    void* grad_bias = nullptr;    // may be null
+    float* partial = nullptr;     // layer_norm_grad_partials() rows of `width` sums for each of the two
+};
+
+struct DropoutArgs {
+    int elem = 0;
+    int64_t rows = 0, width = 0;
+    uint32_t threshold = 0;  // of 65536
+    float scale = 0.0f;
+    Rows x, residual, y;     // residual: ptr may be null
+    const int64_t* state = nullptr;
+    int64_t state_stride = 0;
+};
+
+// One operand of a matrix product: rows of `terms` elements, dense inside.
+struct Operand {
+    const void* ptr = nullptr;
+    int64_t row_stride = 0;
+};
+
+struct GatedArgs {
+    int elem = 0;
+    int activation = 0;
+    int64_t rows = 0, width = 0, inner = 0;
+    int compute_units = 0;  // of the device that was current in the first phase
+    Rows x, gate_weight, up_weight;
+    const void* gate_bias = nullptr;  // both or neither
+    const void* up_bias = nullptr;
+    Rows y, gate, up;  // forward: outputs, gate and up may be null; backward: inputs
+    // backward
+    Rows grad_y, grad_x;                   // grad_x: ptr may be null
+    Rows grad_gate_weight, grad_up_weight;  // both or neither
+    void* grad_gate_bias = nullptr;        // both or neither
+    void* grad_up_bias = nullptr;
+    int want_x = 0, want_weights = 0, want_biases = 0;
+    char* scratch = nullptr;  // gated_scratch_bytes() / gated_grad_scratch_bytes()
+};
+
 struct RotaryTableArgs {
     int64_t positions = 0, rot = 0, row_stride = 0;
     int64_t scaling = 0, original_length = 0;
@@ -63,6 +124,11 @@ struct RotaryArgs {
     Whole position;
     const float* table = nullptr;
     int64_t table_stride = 0;
+    // positions of several axes: their number (0: plain positions), how pairs are shared out (opscvAxesLayout), the pairs of
+    // each axis, cosines of a row of the table
+    int axes = 0, layout = 0;
+    int64_t sections[4] = {0, 0, 0, 0};
+    int64_t columns = 0;
 };
 
 struct AttentionArgs {

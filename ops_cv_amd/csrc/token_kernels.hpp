@@ -20,6 +20,19 @@ hipError_t launch_window_attention(const AttentionArgs& a, hipStream_t stream);
 int64_t attention_scratch_floats(const AttentionArgs& a);
 hipError_t launch_window_attention_grad(const AttentionArgs& a, hipStream_t stream);
 int64_t attention_grad_scratch_floats(const AttentionArgs& a);
+hipError_t launch_layer_norm(const LayerNormArgs& a, hipStream_t stream);
+hipError_t launch_layer_norm_grad(const LayerNormGradArgs& a, hipStream_t stream);
+// rows of each half of LayerNormGradArgs::partial
+int64_t layer_norm_grad_partials(const LayerNormGradArgs& a);
+hipError_t launch_dropout(const DropoutArgs& a, hipStream_t stream);
+hipError_t launch_gated(const GatedArgs& a, hipStream_t stream);
+hipError_t launch_gated_grad(const GatedArgs& a, hipStream_t stream);
+// bytes of GatedArgs::scratch.  The addresses of the operands that are used in place have to be set; those of packed ones are
+// on 256 bytes (null stands for one).
+int64_t gated_scratch_bytes(const GatedArgs& a);
+int64_t gated_grad_scratch_bytes(const GatedArgs& a);
+// the operators of opscv_blocks.cpp, whose operands have been checked (execute_token_plan)
+hipError_t launch_block_plan(void* workspace, const aclOpExecutor* ex, hipStream_t stream);
 // names for opscvExecutorVariant
 const char* attention_variant(const AttentionArgs& a);
 

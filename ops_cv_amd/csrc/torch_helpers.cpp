@@ -764,6 +764,197 @@ PyObject* window_attention_backward(PyObject*, PyObject* const* a, Py_ssize_t n)
     });
 }
 
+// (x, weight, bias, residual, eps, need_stats, out, sum, mean, rstd, workspace, stream)
+PyObject* layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    return guarded(n, 12, [&]() -> PyObject* {
+        const at::Tensor& x = tensor_arg(a[0]);
+        const at::Tensor w = optional_arg(a[1]), b = optional_arg(a[2]), r = optional_arg(a[3]);
+        const double eps = float_arg(a[4]);
+        const bool need_stats = bool_arg(a[5]);
+        const Queue queue(a[11], x);
+        const at::Tensor y = wanted_out(a[6], true, x, x.sizes(), x.scalar_type());
+        const at::Tensor sum = wanted_out(a[7], r.defined(), x, x.sizes(), x.scalar_type());
+        const at::Tensor mean = wanted_out(a[8], need_stats, x, leading(x), at::kFloat);
+        const at::Tensor rstd = wanted_out(a[9], need_stats, x, leading(x), at::kFloat);
+        Call c(queue);
+        aclTensor *hx = c.handle(x), *hr = optional_handle(c, r), *hw = optional_handle(c, w), *hb = optional_handle(c, b),
+                  *hy = c.handle(y, ACL_FORMAT_ND, a[6] == Py_None), *hh = optional_handle(c, sum, a[7] == Py_None),
+                  *hm = optional_handle(c, mean, a[8] == Py_None), *hv = optional_handle(c, rstd, a[9] == Py_None);
+        uint64_t ws = 0;
+        aclOpExecutor* ex = nullptr;
+        const aclnnStatus st = opscvLayerNormGetWorkspaceSize(hx, hr, hw, hb, eps, hy, hh, hm, hv, &ws, &ex);
+        if (st != ACLNN_SUCCESS) {
+            raise_status("opscvLayerNormGetWorkspaceSize", st);
+        }
+        launch("opscvLayerNorm", opscvLayerNorm, ws, ex, x, a[10], queue);
+        return tuple_of(y, sum, mean, rstd);
+    });
+}
+
+// (grad_y, sum, weight, mean, rstd, grad_sum, need_weight, need_bias, grad_x, grad_weight, grad_bias, workspace, stream)
+PyObject* layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    return guarded(n, 13, [&]() -> PyObject* {
+        const at::Tensor& gy = tensor_arg(a[0]);
+        const at::Tensor& h = tensor_arg(a[1]);
+        const at::Tensor w = optional_arg(a[2]);
+        const at::Tensor& mean = tensor_arg(a[3]);
+        const at::Tensor& rstd = tensor_arg(a[4]);
+        const at::Tensor gs = optional_arg(a[5]);
+        const Queue queue(a[12], h);
+        const at::Tensor gx = wanted_out(a[8], true, h, h.sizes(), h.scalar_type());
+        leading(h);
+        const Sizes columns{h.size(-1)};
+        const at::ScalarType type = w.defined() ? w.scalar_type() : h.scalar_type();
+        const at::Tensor gw = wanted_out(a[9], bool_arg(a[6]) && w.defined(), h, columns, type);
+        const at::Tensor gb = wanted_out(a[10], bool_arg(a[7]), h, columns, type);
+        Call c(queue);
+        aclTensor *hgy = c.handle(gy), *hgs = optional_handle(c, gs), *hh = c.handle(h), *hw = optional_handle(c, w),
+                  *hm = c.handle(mean), *hr = c.handle(rstd), *hgx = c.handle(gx, ACL_FORMAT_ND, a[8] == Py_None),
+                  *hgw = optional_handle(c, gw, a[9] == Py_None), *hgb = optional_handle(c, gb, a[10] == Py_None);
+        uint64_t ws = 0;
+        aclOpExecutor* ex = nullptr;
+        const aclnnStatus st = opscvLayerNormBackwardGetWorkspaceSize(hgy, hgs, hh, hw, hm, hr, hgx, hgw, hgb, &ws, &ex);
+        if (st != ACLNN_SUCCESS) {
+            raise_status("opscvLayerNormBackwardGetWorkspaceSize", st);
+        }
+        launch("opscvLayerNormBackward", opscvLayerNormBackward, ws, ex, h, a[11], queue);
+        return tuple_of(gx, gw, gb);
+    });
+}
+
+// (query, key, table, positions, sections, layout, interleaved, inverse, query_out, key_out, workspace, stream)
+PyObject* rotary_axes(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    return guarded(n, 12, [&]() -> PyObject* {
+        const at::Tensor& q = tensor_arg(a[0]);
+        const at::Tensor k = optional_arg(a[1]);
+        const at::Tensor& table = tensor_arg(a[2]);
+        const at::Tensor& positions = tensor_arg(a[3]);
+        const auto sections = sequence_arg<int64_t>(a[4], int_arg);
+        const int64_t layout = int_arg(a[5]);
+        const bool interleaved = bool_arg(a[6]), inverse = bool_arg(a[7]);
+        const Queue queue(a[11], q);
+        const at::Tensor qo = wanted_out(a[8], true, q, q.sizes(), q.scalar_type());
+        const at::Tensor ko = wanted_out(a[9], k.defined(), q, k.defined() ? k.sizes() : q.sizes(), q.scalar_type());
+        Call c(queue);
+        aclTensor *hq = c.handle(q), *hk = optional_handle(c, k), *hp = c.handle(positions), *ht = c.handle(table),
+                  *hqo = c.handle(qo, ACL_FORMAT_ND, a[8] == Py_None), *hko = optional_handle(c, ko, a[9] == Py_None);
+        aclIntArray* hs = aclCreateIntArray(sections.data(), sections.size());
+        uint64_t ws = 0;
+        aclOpExecutor* ex = nullptr;
+        const aclnnStatus st = opscvRotaryAxesGetWorkspaceSize(hq, hk, hp, ht, hs, layout, interleaved, inverse, hqo, hko, &ws,
+                                                               &ex);
+        aclDestroyIntArray(hs);
+        if (st != ACLNN_SUCCESS) {
+            raise_status("opscvRotaryAxesGetWorkspaceSize", st);
+        }
+        launch("opscvRotaryAxes", opscvRotaryAxes, ws, ex, q, a[10], queue);
+        return tuple_of(qo, ko);
+    });
+}
+
+// (x, state, p, residual, out, workspace, stream)
+PyObject* dropout(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    return guarded(n, 7, [&]() -> PyObject* {
+        const at::Tensor& x = tensor_arg(a[0]);
+        const at::Tensor& state = tensor_arg(a[1]);
+        const double p = float_arg(a[2]);
+        const at::Tensor r = optional_arg(a[3]);
+        const Queue queue(a[6], x);
+        const at::Tensor y = wanted_out(a[4], true, x, x.sizes(), x.scalar_type());
+        Call c(queue);
+        aclTensor *hx = c.handle(x), *hr = optional_handle(c, r), *hs = c.handle(state),
+                  *hy = c.handle(y, ACL_FORMAT_ND, a[4] == Py_None);
+        uint64_t ws = 0;
+        aclOpExecutor* ex = nullptr;
+        const aclnnStatus st = opscvDropoutGetWorkspaceSize(hx, hr, hs, p, hy, &ws, &ex);
+        if (st != ACLNN_SUCCESS) {
+            raise_status("opscvDropoutGetWorkspaceSize", st);
+        }
+        launch("opscvDropout", opscvDropout, ws, ex, x, a[5], queue);
+        return wrapped(y);
+    });
+}
+
+// The leading dimensions of `x` and the rows of the weight.
+Sizes inner_sizes(const at::Tensor& x, const at::Tensor& weight)
+{
+    const at::IntArrayRef lead = leading(x);
+    Sizes sizes(lead.begin(), lead.end());
+    sizes.push_back(size_of(weight, 0));
+    return sizes;
+}
+
+// (x, gate_weight, up_weight, gate_bias, up_bias, activation, need_sums, out, gate, up, workspace, stream)
+PyObject* gated_projection(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    return guarded(n, 12, [&]() -> PyObject* {
+        const at::Tensor& x = tensor_arg(a[0]);
+        const at::Tensor& wg = tensor_arg(a[1]);
+        const at::Tensor& wu = tensor_arg(a[2]);
+        const at::Tensor bg = optional_arg(a[3]), bu = optional_arg(a[4]);
+        const int64_t activation = int_arg(a[5]);
+        const bool need_sums = bool_arg(a[6]);
+        const Queue queue(a[11], x);
+        const Sizes sizes = inner_sizes(x, wg);
+        const at::Tensor y = wanted_out(a[7], true, x, sizes, x.scalar_type());
+        const at::Tensor gate = wanted_out(a[8], need_sums, x, sizes, x.scalar_type());
+        const at::Tensor up = wanted_out(a[9], need_sums, x, sizes, x.scalar_type());
+        Call c(queue);
+        aclTensor *hx = c.handle(x), *hwg = c.handle(wg), *hwu = c.handle(wu), *hbg = optional_handle(c, bg),
+                  *hbu = optional_handle(c, bu), *hy = c.handle(y, ACL_FORMAT_ND, a[7] == Py_None),
+                  *hg = optional_handle(c, gate, a[8] == Py_None), *hu = optional_handle(c, up, a[9] == Py_None);
+        uint64_t ws = 0;
+        aclOpExecutor* ex = nullptr;
+        const aclnnStatus st = opscvGatedProjectionGetWorkspaceSize(hx, hwg, hwu, hbg, hbu, activation, hy, hg, hu, &ws, &ex);
+        if (st != ACLNN_SUCCESS) {
+            raise_status("opscvGatedProjectionGetWorkspaceSize", st);
+        }
+        launch("opscvGatedProjection", opscvGatedProjection, ws, ex, x, a[10], queue);
+        return tuple_of(y, gate, up);
+    });
+}
+
+// (grad_y, x, gate_weight, up_weight, gate, up, activation, need_x, need_weights, need_bias, grad_x, grad_gate_weight,
+// grad_up_weight, grad_gate_bias, grad_up_bias, workspace, stream)
+PyObject* gated_projection_backward(PyObject*, PyObject* const* a, Py_ssize_t n)
+{
+    return guarded(n, 17, [&]() -> PyObject* {
+        const at::Tensor& gy = tensor_arg(a[0]);
+        const at::Tensor& x = tensor_arg(a[1]);
+        const at::Tensor& wg = tensor_arg(a[2]);
+        const at::Tensor& wu = tensor_arg(a[3]);
+        const at::Tensor& gate = tensor_arg(a[4]);
+        const at::Tensor& up = tensor_arg(a[5]);
+        const int64_t activation = int_arg(a[6]);
+        const bool need_x = bool_arg(a[7]), need_weights = bool_arg(a[8]), need_bias = bool_arg(a[9]);
+        const Queue queue(a[16], x);
+        const Sizes inner{size_of(wg, 0)};
+        const at::Tensor gx = wanted_out(a[10], need_x, x, x.sizes(), x.scalar_type());
+        const at::Tensor gwg = wanted_out(a[11], need_weights, x, wg.sizes(), x.scalar_type());
+        const at::Tensor gwu = wanted_out(a[12], need_weights, x, wu.sizes(), x.scalar_type());
+        const at::Tensor gbg = wanted_out(a[13], need_bias, x, inner, x.scalar_type());
+        const at::Tensor gbu = wanted_out(a[14], need_bias, x, inner, x.scalar_type());
+        Call c(queue);
+        aclTensor *hgy = c.handle(gy), *hx = c.handle(x), *hwg = c.handle(wg), *hwu = c.handle(wu), *hg = c.handle(gate),
+                  *hu = c.handle(up), *hgx = optional_handle(c, gx, a[10] == Py_None),
+                  *hgwg = optional_handle(c, gwg, a[11] == Py_None), *hgwu = optional_handle(c, gwu, a[12] == Py_None),
+                  *hgbg = optional_handle(c, gbg, a[13] == Py_None), *hgbu = optional_handle(c, gbu, a[14] == Py_None);
+        uint64_t ws = 0;
+        aclOpExecutor* ex = nullptr;
+        const aclnnStatus st = opscvGatedProjectionBackwardGetWorkspaceSize(hgy, hx, hwg, hwu, hg, hu, activation, hgx, hgwg,
+                                                                            hgwu, hgbg, hgbu, &ws, &ex);
+        if (st != ACLNN_SUCCESS) {
+            raise_status("opscvGatedProjectionBackwardGetWorkspaceSize", st);
+        }
+        launch("opscvGatedProjectionBackward", opscvGatedProjectionBackward, ws, ex, x, a[15], queue);
+        return tuple_of(gx, gwg, gwu, gbg, gbu);
+    });
+}
+
 // (AclnnError): the class of the errors raised for a status other than success
 PyObject* set_error_class(PyObject*, PyObject* cls)
 {
@@ -786,6 +977,12 @@ PyMethodDef kMethods[] = {OPSCV_FAST(grid_sampler2d),
                           OPSCV_FAST(rotary),
                           OPSCV_FAST(window_attention),
                           OPSCV_FAST(window_attention_backward),
+                          OPSCV_FAST(layer_norm),
+                          OPSCV_FAST(layer_norm_backward),
+                          OPSCV_FAST(rotary_axes),
+                          OPSCV_FAST(dropout),
+                          OPSCV_FAST(gated_projection),
+                          OPSCV_FAST(gated_projection_backward),
                           {"set_error_class", set_error_class, METH_O, nullptr},
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_torch_helpers", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
