@@ -247,7 +247,7 @@ typedef enum {
  * x : (..., width), y, gate, up : (..., inner), one to five dimensions; gateWeight, upWeight : (inner, width); gateBias,
  * upBias : (inner), both or neither; all of one type.  Products are summed up in 32 bits, and y is computed from those sums.
  *   gate, up : NULL (both), or the sums rounded to the type: what the backward pass reads
- *   sizes    : width and inner up to 2^20, rows (the product of the leading dimensions) up to 2^30
+ *   sizes    : width and inner up to 2^19, rows (the product of the leading dimensions) up to 2^30
  */
 ACLNN_API aclnnStatus opscvGatedProjectionGetWorkspaceSize(const aclTensor* x, const aclTensor* gateWeight,
                                                            const aclTensor* upWeight, const aclTensor* gateBias,
@@ -266,7 +266,7 @@ ACLNN_API aclnnStatus opscvGatedProjection(void* workspace, uint64_t workspaceSi
  * dGate and dUp are rounded to the type before they are multiplied (to nearest, relative 2^-11 at most for FLOAT16, 2^-8 for
  * BF16), not before the biases' sums.  FLOAT16: times a power of two for each row, and for the weights' gradients each
  * column, so that their largest is near 2^14; what is 2^28 times less than that largest loses bits.
- *   sizes : width, inner and rows up to 2^20
+ *   sizes : width and inner up to 2^19, rows up to 2^20
  */
 ACLNN_API aclnnStatus opscvGatedProjectionBackwardGetWorkspaceSize(
     const aclTensor* gradY, const aclTensor* x, const aclTensor* gateWeight, const aclTensor* upWeight,

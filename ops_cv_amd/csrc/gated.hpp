@@ -10,17 +10,17 @@ namespace prod {
 
 struct ProductArgs;
 
-hipError_t launch_product_f32(const ProductArgs& a, int kind, int tile, hipStream_t stream);
-hipError_t launch_product_f16(const ProductArgs& a, int kind, int tile, hipStream_t stream);
-hipError_t launch_product_bf16(const ProductArgs& a, int kind, int tile, hipStream_t stream);
+// the gated forward product, and both products of the gradients (one may be null)
+hipError_t launch_products_f32(const ProductArgs& a, bool large, hipStream_t stream);
+hipError_t launch_products_f16(const ProductArgs& a, bool large, hipStream_t stream);
+hipError_t launch_products_bf16(const ProductArgs& a, bool large, hipStream_t stream);
+hipError_t launch_gradients_f32(const ProductArgs* x, const ProductArgs* weights, bool large, hipStream_t stream);
+hipError_t launch_gradients_f16(const ProductArgs* x, const ProductArgs* weights, bool large, hipStream_t stream);
+hipError_t launch_gradients_bf16(const ProductArgs* x, const ProductArgs* weights, bool large, hipStream_t stream);
 
 // Rows of `width` elements, copied to rows of `to_stride`, zeros from `width` to `padded` on.
 hipError_t launch_pad_rows(Elem e, const void* from, int64_t from_stride, int64_t rows, int64_t width, void* to,
                            int64_t to_stride, int64_t padded, hipStream_t stream);
-
-// to[c][r] = from[r][c], zeros for r from `rows` to `padded` on.
-hipError_t launch_transpose(Elem e, const void* from, int64_t from_stride, int64_t rows, int64_t width, void* to,
-                            int64_t to_stride, int64_t padded, hipStream_t stream);
 
 // Gradients of gate and up, as the products want them (gated_layout.hip).
 struct GateGradArgs {
@@ -28,32 +28,23 @@ struct GateGradArgs {
     int64_t rows = 0, inner = 0;
     const void *grad_y = nullptr, *gate = nullptr, *up = nullptr;
     int64_t grad_y_stride = 0, gate_stride = 0, up_stride = 0;
-    // (rows, 2 padded_inner): dGate, zeros, dUp, zeros; may be null
+    // (rows, 2 padded): dGate, zeros, dUp, zeros; FLOAT16: in the scale of each row.  May be null.
     void* by_rows = nullptr;
-    int64_t padded_inner = 0;
-    // (2 inner, padded_rows): the transposed dGate and dUp, zeros behind; may be null
+    // FLOAT16: the same in the scale of each column.  May be null.
     void* by_columns = nullptr;
-    int64_t padded_rows = 0;
-    // sums over the rows of each tile of kGateTile rows: (tiles, 2 inner); may be null
+    int64_t padded = 0;
+    // sums over the rows of each tile of kGateRows rows: (tiles, 2 inner); may be null
     float* sums = nullptr;
     // FLOAT16: largest absolute values as bits, by rows and by columns (2 inner), and the factors that undo the scales
     uint32_t *row_most = nullptr, *column_most = nullptr;
     float *row_factor = nullptr, *column_factor = nullptr;
 };
-constexpr int kGateTile = 64;
+constexpr int kGateRows = 64;
 
 hipError_t launch_gate_grad(const GateGradArgs& a, hipStream_t stream);
 
-// out[t][f] = factor[t] * sum of the parts
-struct JoinArgs {
-    const float* parts = nullptr;
-    int64_t count = 0, tokens = 0, features = 0;
-    void* out[2] = {nullptr, nullptr};
-    int64_t out_stride[2] = {0, 0};
-    int64_t turn = 0;
-    const float* token_scale = nullptr;
-};
-hipError_t launch_join(Elem e, const JoinArgs& a, hipStream_t stream);
+// The sum of a product's parts in the places of its results (product_tile.hpp).
+hipError_t launch_join(Elem e, const ProductArgs& a, hipStream_t stream);
 
 // Sums of the rows of (rows, 2 inner): the first inner to `gate`, the others to `up`.
 hipError_t launch_bias_sums(Elem e, const float* sums, int64_t rows, int64_t inner, void* gate, void* up, hipStream_t stream);

@@ -1,13 +1,13 @@
-// Around the matrix products of the gated projections: operands laid out as rows of their terms, the gradients of gate and up,
-// sums of partial products and of the biases' gradients.  All bound by memory.
+// Around the matrix products of the gated projections: operands copied to whole vectors, the gradients of gate and up, sums of
+// partial products and of the biases' gradients.  All bound by memory.
 //
 //   dGate = gy up act'(gate),  dUp = gy act(gate)
 //
-// Both are needed by rows (gradient of x: sums over the inner features) and by columns (gradients of the weights: sums over
-// the rows), so a tile of 64 x 64 is computed once and written both ways, through LDS.  FLOAT16 has a range of 2^5 over and
-// 2^14 under the values that gradients have when they are well scaled, and sums of products of gy, up and a slope leave it on
-// both sides: there every row and column is multiplied by the power of two that takes its largest value to 2^14..2^15, found
-// by a first pass, and the products' results are divided by it.
+// They are written once, rounded to the type, and both products read them.  FLOAT16 has a range of 2^5 over and 2^14 under the
+// values that gradients have when they are well scaled, and products of gy, up and a slope leave it on both sides: there every
+// row is multiplied by the power of two that takes its largest value to 2^14..2^15, found by a first pass, and its results of
+// the product, the gradient of x, are divided by it.  The weights' gradients sum over the rows, so they read the same numbers
+// in a scale of every column.
 #include <hip/hip_runtime.h>
 
 #include "gated.hpp"
@@ -24,7 +24,7 @@ using namespace tok;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTile = kGateTile;
+constexpr int kRows = kGateRows;
 
 template <typename T>
 constexpr int kVec = 16 / (int)sizeof(T);
@@ -43,69 +43,6 @@ __global__ __launch_bounds__(kThreads) void pad_rows_kernel(const T* from, int64
         }
         *reinterpret_cast<Pack<T, kVec<T>>*>(to + r * to_stride + c) = k;
     }
-}
-
-// A tile of 64 x 64 in LDS, written by rows and read by columns; four bytes more a row keep a column off one bank.
-template <typename T>
-struct Turn {
-    T v[kTile][kTile + 4 / (int)sizeof(T)];
-};
-
-// Column c of the tile, rows r..: one vector of the transposed rows.
-template <typename T>
-__device__ __forceinline__ void put_turned(const Turn<T>& tile, T* to, int64_t to_stride, int64_t column0, int64_t columns,
-                                           int64_t row0, int64_t padded)
-{
-    constexpr int kParts = kTile / kVec<T>;  // vectors of a column
-    for (int i = (int)threadIdx.x; i < kTile * kParts; i += kThreads) {
-        const int c = i / kParts, r = i % kParts * kVec<T>;
-        if (column0 + c < columns && row0 + r < padded) {
-            Pack<T, kVec<T>> k;
-#pragma unroll
-            for (int e = 0; e < kVec<T>; e++) {
-                k.v[e] = tile.v[r + e][c];
-            }
-            *reinterpret_cast<Pack<T, kVec<T>>*>(to + (column0 + c) * to_stride + row0 + r) = k;
-        }
-    }
-}
-
-template <typename T, bool WIDE>
-__global__ __launch_bounds__(kThreads) void transpose_kernel(const T* from, int64_t from_stride, int64_t rows, int64_t width,
-                                                             T* to, int64_t to_stride, int64_t padded)
-{
-    __shared__ Turn<T> tile;
-    constexpr int kParts = kTile / kVec<T>, kRows = kThreads / kParts;
-    const int64_t row0 = (int64_t)blockIdx.y * kTile, column0 = (int64_t)blockIdx.x * kTile;
-    const int c = (int)threadIdx.x % kParts * kVec<T>;
-#pragma unroll
-    for (int i = 0; i < kTile / kRows; i++) {
-        const int r = i * kRows + (int)threadIdx.x / kParts;
-        const T* const row = from + (row0 + r) * from_stride + column0 + c;
-        Pack<T, kVec<T>> k;
-#pragma unroll
-        for (int e = 0; e < kVec<T>; e++) {
-            k.v[e] = (T)0.0f;
-        }
-        if (row0 + r < rows) {
-            if (WIDE && column0 + c + kVec<T> <= width) {
-                k = *reinterpret_cast<const Pack<T, kVec<T>>*>(row);
-            } else {
-#pragma unroll
-                for (int e = 0; e < kVec<T>; e++) {
-                    if (column0 + c + e < width) {
-                        k.v[e] = row[e];
-                    }
-                }
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < kVec<T>; e++) {
-            tile.v[r][c + e] = k.v[e];
-        }
-    }
-    __syncthreads();
-    put_turned<T>(tile, to, to_stride, column0, width, row0, padded);
 }
 
 // ------------------------------------------------------------------------------------------- gradients of gate and up
@@ -169,22 +106,26 @@ __device__ __forceinline__ uint32_t size_of(float x)
     return u < 0x7F800000u ? u : 0u;
 }
 
+// A workgroup's part: kRows rows of kThreads / 8 vectors; a thread's vectors are those of every eighth row.
+template <typename T>
+constexpr int kColumns = kThreads / 8 * kVec<T>;
+
 // Largest values of rows and columns.  The order of the atomic maxima does not matter.
 template <typename T, bool WIDE>
 __global__ __launch_bounds__(kThreads) void gate_most_kernel(GateGradArgs a)
 {
-    constexpr int N = kVec<T>, kParts = kTile / N, kRows = kThreads / kParts;
-    __shared__ uint32_t rows[kTile], columns[2][kTile];
-    for (int i = (int)threadIdx.x; i < 3 * kTile; i += kThreads) {
-        (i < kTile ? rows[i] : columns[i / kTile - 1][i % kTile]) = 0;
+    constexpr int N = kVec<T>;
+    __shared__ uint32_t rows[kRows], columns[2][kColumns<T>];
+    for (int i = (int)threadIdx.x; i < kRows + 2 * kColumns<T>; i += kThreads) {
+        (i < kRows ? rows[i] : columns[(i - kRows) / kColumns<T>][(i - kRows) % kColumns<T>]) = 0;
     }
     __syncthreads();
-    const int64_t row0 = (int64_t)blockIdx.y * kTile, column0 = (int64_t)blockIdx.x * kTile;
-    const int c = (int)threadIdx.x % kParts * N;
+    const int64_t row0 = (int64_t)blockIdx.y * kRows, column0 = (int64_t)blockIdx.x * kColumns<T>;
+    const int c = (int)threadIdx.x % 32 * N;
     uint32_t most[2][N] = {{0}};
 #pragma unroll
-    for (int i = 0; i < kTile / kRows; i++) {
-        const int r = i * kRows + (int)threadIdx.x / kParts;
+    for (int i = 0; i < kRows / 8; i++) {
+        const int r = i * 8 + (int)threadIdx.x / 32;
         float dg[N], du[N];
         gate_values<T, WIDE>(a, row0 + r, column0 + c, dg, du);
         uint32_t row = 0;
@@ -196,7 +137,14 @@ __global__ __launch_bounds__(kThreads) void gate_most_kernel(GateGradArgs a)
             row = row > g ? row : g;
             row = row > u ? row : u;
         }
-        atomicMax(&rows[r], row);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) {
+            const uint32_t other = (uint32_t)__shfl_xor((int)row, d, 64);
+            row = row > other ? row : other;
+        }
+        if (c == 0) {
+            rows[r] = row;
+        }
     }
 #pragma unroll
     for (int e = 0; e < N; e++) {
@@ -204,95 +152,103 @@ __global__ __launch_bounds__(kThreads) void gate_most_kernel(GateGradArgs a)
         atomicMax(&columns[1][c + e], most[1][e]);
     }
     __syncthreads();
-    for (int i = (int)threadIdx.x; i < 3 * kTile; i += kThreads) {
-        const int at = i % kTile;
-        if (i < kTile) {
-            if (row0 + at < a.rows) {
-                atomicMax(&a.row_most[row0 + at], rows[at]);
+    for (int i = (int)threadIdx.x; i < kRows + 2 * kColumns<T>; i += kThreads) {
+        if (i < kRows) {
+            if (row0 + i < a.rows) {
+                atomicMax(&a.row_most[row0 + i], rows[i]);
             }
-        } else if (column0 + at < a.inner) {
-            atomicMax(&a.column_most[(i / kTile - 1) * a.inner + column0 + at], columns[i / kTile - 1][at]);
+        } else {
+            const int half = (i - kRows) / kColumns<T>, at = (i - kRows) % kColumns<T>;
+            if (column0 + at < a.inner) {
+                atomicMax(&a.column_most[half * a.inner + column0 + at], columns[half][at]);
+            }
         }
     }
 }
 
-template <typename T, bool WIDE, bool SCALED>
+template <typename T, bool WIDE>
 __global__ __launch_bounds__(kThreads) void gate_grad_kernel(GateGradArgs a)
 {
-    constexpr int N = kVec<T>, kParts = kTile / N, kRows = kThreads / kParts;
-    __shared__ Turn<T> tile[2];
-    __shared__ float sums[2][kRows][kTile];
-    const int64_t row0 = (int64_t)blockIdx.y * kTile, column0 = (int64_t)blockIdx.x * kTile;
-    const int c = (int)threadIdx.x % kParts * N, thread_row = (int)threadIdx.x / kParts;
-    float by_column[2][N], total[2][N];
+    constexpr int N = kVec<T>;
+    constexpr bool kScaled = std::is_same_v<T, _Float16>;
+    __shared__ float sums[2][8][kColumns<T>];
+    const int64_t row0 = (int64_t)blockIdx.y * kRows, column0 = (int64_t)blockIdx.x * kColumns<T>;
+    const int c = (int)threadIdx.x % 32 * N, part = (int)threadIdx.x / 32;
+    float by_column[2][kScaled ? N : 1], total[2][N];
 #pragma unroll
     for (int e = 0; e < N; e++) {
-        by_column[0][e] = by_column[1][e] = 1.0f;
         total[0][e] = total[1][e] = 0.0f;
-        if (SCALED && column0 + c + e < a.inner) {
-            by_column[0][e] = lift(a.column_most[column0 + c + e]);
-            by_column[1][e] = lift(a.column_most[a.inner + column0 + c + e]);
-            if (blockIdx.y == 0 && thread_row == 0) {
-                a.column_factor[column0 + c + e] = 1.0f / by_column[0][e];
-                a.column_factor[a.inner + column0 + c + e] = 1.0f / by_column[1][e];
+        if constexpr (kScaled) {
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                by_column[half][e] = 1.0f;
+                if (column0 + c + e < a.inner) {
+                    by_column[half][e] = lift(a.column_most[half * a.inner + column0 + c + e]);
+                    if (blockIdx.y == 0 && part == 0) {
+                        a.column_factor[half * a.inner + column0 + c + e] = 1.0f / by_column[half][e];
+                    }
+                }
             }
         }
     }
-#pragma unroll
-    for (int i = 0; i < kTile / kRows; i++) {
-        const int r = i * kRows + thread_row;
-        const int64_t row = row0 + r;
-        float dg[N], du[N];
+#pragma unroll 2
+    for (int i = 0; i < kRows / 8; i++) {
+        const int64_t row = row0 + i * 8 + part;
+        float dg[N], du[N], x[N];
         gate_values<T, WIDE>(a, row, column0 + c, dg, du);
         float by_row = 1.0f;
-        if (SCALED && row < a.rows) {
+        if (kScaled && row < a.rows) {
             by_row = lift(a.row_most[row]);
             if (blockIdx.x == 0 && c == 0) {
                 a.row_factor[row] = 1.0f / by_row;
             }
         }
-        if (a.by_rows != nullptr && row < a.rows && column0 + c < a.padded_inner) {
-            float x[N];
-            T* const to = (T*)a.by_rows + row * 2 * a.padded_inner + column0 + c;
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                x[e] = dg[e] * by_row;
-            }
-            store<T, N>(to, x, false);
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                x[e] = du[e] * by_row;
-            }
-            store<T, N>(to + a.padded_inner, x, false);
-        }
 #pragma unroll
         for (int e = 0; e < N; e++) {
             total[0][e] += dg[e];
             total[1][e] += du[e];
-            tile[0].v[r][c + e] = (T)(dg[e] * by_column[0][e]);
-            tile[1].v[r][c + e] = (T)(du[e] * by_column[1][e]);
+        }
+        if (row < a.rows && column0 + c < a.padded) {
+            const int64_t at = row * 2 * a.padded + column0 + c;
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                const float(&d)[N] = half == 0 ? dg : du;
+                if (a.by_rows != nullptr) {
+#pragma unroll
+                    for (int e = 0; e < N; e++) {
+                        x[e] = d[e] * by_row;
+                    }
+                    store<T, N>((T*)a.by_rows + at + half * a.padded, x, false);
+                }
+                if constexpr (kScaled) {
+                    if (a.by_columns != nullptr) {
+#pragma unroll
+                        for (int e = 0; e < N; e++) {
+                            x[e] = d[e] * by_column[half][e];
+                        }
+                        store<T, N>((T*)a.by_columns + at + half * a.padded, x, false);
+                    }
+                }
+            }
         }
     }
     if (a.sums != nullptr) {
 #pragma unroll
         for (int e = 0; e < N; e++) {
-            sums[0][thread_row][c + e] = total[0][e];
-            sums[1][thread_row][c + e] = total[1][e];
+            sums[0][part][c + e] = total[0][e];
+            sums[1][part][c + e] = total[1][e];
         }
-    }
-    __syncthreads();
-    if (a.by_columns != nullptr) {
-        put_turned<T>(tile[0], (T*)a.by_columns, a.padded_rows, column0, a.inner, row0, a.padded_rows);
-        put_turned<T>(tile[1], (T*)a.by_columns + a.inner * a.padded_rows, a.padded_rows, column0, a.inner, row0, a.padded_rows);
-    }
-    if (a.sums != nullptr && threadIdx.x < 2 * kTile) {
-        const int half = (int)threadIdx.x / kTile, at = (int)threadIdx.x % kTile;
-        float sum = 0.0f;
-        for (int r = 0; r < kRows; r++) {
-            sum += sums[half][r][at];
-        }
-        if (column0 + at < a.inner) {
-            a.sums[(int64_t)blockIdx.y * 2 * a.inner + half * a.inner + column0 + at] = sum;
+        __syncthreads();
+        for (int i = (int)threadIdx.x; i < 2 * kColumns<T>; i += kThreads) {
+            const int half = i / kColumns<T>, at = i % kColumns<T>;
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                sum += sums[half][k][at];
+            }
+            if (column0 + at < a.inner) {
+                a.sums[(int64_t)blockIdx.y * 2 * a.inner + half * a.inner + column0 + at] = sum;
+            }
         }
     }
 }
@@ -300,16 +256,15 @@ __global__ __launch_bounds__(kThreads) void gate_grad_kernel(GateGradArgs a)
 template <typename T>
 hipError_t run_gate_grad(const GateGradArgs& a, hipStream_t stream)
 {
-    const int64_t columns = (a.inner + kTile - 1) / kTile, rows = (a.rows + kTile - 1) / kTile;
-    if (columns > 65535 || rows > 65535) {
+    const int64_t columns = (a.padded + kColumns<T> - 1) / kColumns<T>, rows = (a.rows + kRows - 1) / kRows;
+    if (columns > 65535 || rows > 65535 || a.padded % kVec<T> != 0 || a.padded < a.inner) {
         return hipErrorInvalidValue;
     }
     const int e = (int)sizeof(T);
     const bool wide = aligned(a.grad_y, a.grad_y_stride, e, 16) && aligned(a.gate, a.gate_stride, e, 16) &&
                       aligned(a.up, a.up_stride, e, 16);
     const dim3 grid((unsigned)columns, (unsigned)rows);
-    constexpr bool kScaled = std::is_same_v<T, _Float16>;
-    if (kScaled) {
+    if constexpr (std::is_same_v<T, _Float16>) {
         const int64_t words = a.rows + 2 * a.inner, blocks = (words + kThreads - 1) / kThreads;
         hipLaunchKernelGGL(clear_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(kThreads), 0, stream, a.row_most,
                            words);  // the columns' follow the rows'
@@ -320,28 +275,32 @@ hipError_t run_gate_grad(const GateGradArgs& a, hipStream_t stream)
         }
     }
     if (wide) {
-        hipLaunchKernelGGL((gate_grad_kernel<T, true, kScaled>), grid, dim3(kThreads), 0, stream, a);
+        hipLaunchKernelGGL((gate_grad_kernel<T, true>), grid, dim3(kThreads), 0, stream, a);
     } else {
-        hipLaunchKernelGGL((gate_grad_kernel<T, false, kScaled>), grid, dim3(kThreads), 0, stream, a);
+        hipLaunchKernelGGL((gate_grad_kernel<T, false>), grid, dim3(kThreads), 0, stream, a);
     }
     return hipGetLastError();
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void join_kernel(JoinArgs a)
+__global__ __launch_bounds__(kThreads) void join_kernel(ProductArgs a)
 {
     const int64_t total = a.tokens * a.features;
     for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
         const int64_t t = i / a.features, f = i - t * a.features;
+        const bool second = t >= a.turn;
+        const int64_t row = second ? t - a.turn : t;
+        if (row >= a.rows || f >= a.columns) {
+            continue;
+        }
         float sum = 0.0f;
-        for (int64_t k = 0; k < a.count; k++) {
-            sum += a.parts[k * total + i];
+        for (int64_t k = 0; k < a.parts; k++) {
+            sum += a.partial[k * total + i];
         }
         if (a.token_scale != nullptr) {
-            sum *= a.token_scale[t];
+            sum *= a.token_scale[second ? a.rows + row : row];
         }
-        const bool second = t >= a.turn;
-        ((T*)a.out[second])[(second ? t - a.turn : t) * a.out_stride[second] + f] = (T)sum;
+        ((T*)a.out[second])[row * a.out_stride[second] + f] = (T)sum;
     }
 }
 
@@ -377,30 +336,6 @@ hipError_t launch_pad_rows(Elem e, const void* from, int64_t from_stride, int64_
     });
 }
 
-hipError_t launch_transpose(Elem e, const void* from, int64_t from_stride, int64_t rows, int64_t width, void* to,
-                            int64_t to_stride, int64_t padded, hipStream_t stream)
-{
-    return typed(e, [&](auto* t) {
-        typedef std::remove_pointer_t<decltype(t)> T;
-        const int64_t columns = (width + kTile - 1) / kTile, row_tiles = (rows + kTile - 1) / kTile;
-        if (rows < 1) {
-            return hipSuccess;
-        }
-        if (padded % kVec<T> != 0 || to_stride % kVec<T> != 0 || columns > 65535 || row_tiles > 65535) {
-            return hipErrorInvalidValue;
-        }
-        const dim3 grid((unsigned)columns, (unsigned)row_tiles);
-        if (aligned(from, from_stride, (int)sizeof(T), 16)) {
-            hipLaunchKernelGGL((transpose_kernel<T, true>), grid, dim3(kThreads), 0, stream, (const T*)from, from_stride, rows,
-                               width, (T*)to, to_stride, padded);
-        } else {
-            hipLaunchKernelGGL((transpose_kernel<T, false>), grid, dim3(kThreads), 0, stream, (const T*)from, from_stride, rows,
-                               width, (T*)to, to_stride, padded);
-        }
-        return hipGetLastError();
-    });
-}
-
 hipError_t launch_gate_grad(const GateGradArgs& a, hipStream_t stream)
 {
     if (a.rows < 1) {
@@ -409,7 +344,7 @@ hipError_t launch_gate_grad(const GateGradArgs& a, hipStream_t stream)
     return typed((Elem)a.elem, [&](auto* t) { return run_gate_grad<std::remove_pointer_t<decltype(t)>>(a, stream); });
 }
 
-hipError_t launch_join(Elem e, const JoinArgs& a, hipStream_t stream)
+hipError_t launch_join(Elem e, const ProductArgs& a, hipStream_t stream)
 {
     return typed(e, [&](auto* t) {
         typedef std::remove_pointer_t<decltype(t)> T;

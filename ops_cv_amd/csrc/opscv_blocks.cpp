@@ -9,7 +9,8 @@ using namespace opscv::tokplan;
 
 namespace {
 
-constexpr int64_t kMostGated = (int64_t)1 << 20;  // width, inner; backward: rows
+constexpr int64_t kMostGated = (int64_t)1 << 19;      // width, inner
+constexpr int64_t kMostGatedRows = (int64_t)1 << 20;  // backward
 
 // slots of aclOpExecutor::operands
 enum LayerNormSlot { kLnX, kLnResidual, kLnWeight, kLnBias, kLnY, kLnSum, kLnMean, kLnRstd };
@@ -78,7 +79,7 @@ aclnnStatus check_gated(const char* api, const aclTensor* x, const aclTensor* ga
     OPSCV_CHECK(check_matrix(api, "gateWeight", gate_weight, *a, x->dtype));
     OPSCV_CHECK(check_matrix(api, "upWeight", up_weight, *a, x->dtype));
     if (a->inner < 1 || a->inner > kMostGated || a->width > kMostGated || a->rows > most_rows) {
-        return invalid("%s: width and inner of 1 to 2^20 and up to %lld rows, got %lld, %lld and %lld", api,
+        return invalid("%s: width and inner of 1 to 2^19 and up to %lld rows, got %lld, %lld and %lld", api,
                        (long long)most_rows, (long long)a->width, (long long)a->inner, (long long)a->rows);
     }
     if (activation < OPSCV_GATE_SILU || activation > OPSCV_GATE_GELU_TANH) {
@@ -421,7 +422,7 @@ aclnnStatus opscvGatedProjectionBackwardGetWorkspaceSize(const aclTensor* gradY,
         return missing(api, "gradY, x, both weights and both sums, a gradient, and one weight's or bias's beside the other,");
     }
     GatedArgs& a = ex->gated;
-    OPSCV_CHECK(check_gated(api, x, gateWeight, upWeight, activation, kMostGated, &a));
+    OPSCV_CHECK(check_gated(api, x, gateWeight, upWeight, activation, kMostGatedRows, &a));
     OPSCV_CHECK(check_rows_of(api, "gradY", gradY, x, a.inner));
     OPSCV_CHECK(check_rows_of(api, "gate", gate, x, a.inner));
     OPSCV_CHECK(check_rows_of(api, "up", up, x, a.inner));
@@ -446,11 +447,11 @@ aclnnStatus opscvGatedProjectionBackwardGetWorkspaceSize(const aclTensor* gradY,
     const int bytes = elem_size((Elem)a.elem);
     plan_rows(ex.get(), kGgY, gradY, bytes, false, &a.grad_y);
     if (a.want_weights != 0) {
-        plan_rows(ex.get(), kGgX, x, bytes, false, &a.x);
+        plan_operand(ex.get(), kGgX, x, bytes, false, &a.x);
     }
     if (a.want_x != 0) {
-        plan_rows(ex.get(), kGgGateWeight, gateWeight, bytes, false, &a.gate_weight);
-        plan_rows(ex.get(), kGgUpWeight, upWeight, bytes, false, &a.up_weight);
+        plan_operand(ex.get(), kGgGateWeight, gateWeight, bytes, false, &a.gate_weight);
+        plan_operand(ex.get(), kGgUpWeight, upWeight, bytes, false, &a.up_weight);
     }
     plan_rows(ex.get(), kGgGate, gate, bytes, false, &a.gate);
     plan_rows(ex.get(), kGgUp, up, bytes, false, &a.up);

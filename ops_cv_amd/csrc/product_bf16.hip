@@ -5,9 +5,14 @@
 namespace opscv {
 namespace prod {
 
-hipError_t launch_product_bf16(const ProductArgs& a, int kind, int tile, hipStream_t stream)
+hipError_t launch_products_bf16(const ProductArgs& a, bool large, hipStream_t stream)
 {
-    return launch_typed<__bf16>(a, kind, tile, stream);
+    return launch_gated_typed<__bf16>(a, large, stream);
+}
+
+hipError_t launch_gradients_bf16(const ProductArgs* x, const ProductArgs* weights, bool large, hipStream_t stream)
+{
+    return launch_gradients_typed<__bf16>(x, weights, large, stream);
 }
 
 }  // namespace prod

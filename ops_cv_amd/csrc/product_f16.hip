@@ -5,9 +5,14 @@
 namespace opscv {
 namespace prod {
 
-hipError_t launch_product_f16(const ProductArgs& a, int kind, int tile, hipStream_t stream)
+hipError_t launch_products_f16(const ProductArgs& a, bool large, hipStream_t stream)
 {
-    return launch_typed<_Float16>(a, kind, tile, stream);
+    return launch_gated_typed<_Float16>(a, large, stream);
+}
+
+hipError_t launch_gradients_f16(const ProductArgs* x, const ProductArgs* weights, bool large, hipStream_t stream)
+{
+    return launch_gradients_typed<_Float16>(x, weights, large, stream);
 }
 
 }  // namespace prod

@@ -7,50 +7,97 @@
 
 #include "kernels.hpp"
 #include "launch_limits.hpp"
-#include "product_plan.hpp"
 #include "product_tile.hpp"
 
 namespace opscv {
 namespace prod {
 
-template <typename T, int KIND, int FB, int TB, int WF, int WT>
-hipError_t launch_shape(ProductArgs a, hipStream_t stream)
+// Workgroups of a product, 0 where it does not fit what the kernels assume.
+template <typename T, bool GATED, bool P_TURNED, bool Q_TURNED, typename S>
+int64_t prepare(ProductArgs* a)
 {
-    typedef Shape<T, KIND, FB, TB, WF, WT> S;
-    const int64_t token_tiles = (a.tokens + S::kTokens - 1) / S::kTokens;
-    const int64_t feature_tiles = (a.features + S::kResults - 1) / S::kResults;
-    const int64_t blocks = token_tiles * feature_tiles * a.parts;
-    const int64_t e = (int64_t)sizeof(T), furthest = kInside - kRowBytes - a.terms * e;
-    const int64_t p_rows = KIND == kGated ? S::kFeatures / 2 : S::kFeatures;
-    if (a.tokens < 1 || a.features < 1 || a.terms < 0 || a.terms * e % 16 != 0 || !fits_launch(blocks, S::kThreads) ||
-        S::kTokens * a.q_stride * e > furthest || p_rows * a.p_stride[0] * e > furthest ||
-        p_rows * a.p_stride[1] * e > furthest || a.q_stride < 0 || a.p_stride[0] < 0 || a.p_stride[1] < 0) {
+    constexpr int64_t kE = (int64_t)sizeof(T), kVec = 16 / kE, kTerms = kRowBytes / kE;
+    const int64_t results = GATED ? S::kFeatures / 2 : S::kFeatures;
+    const int64_t furthest = (int64_t)kInside - 2 * kRowBytes - (P_TURNED && Q_TURNED ? 0 : a->terms * kE);
+    const int64_t p_rows = P_TURNED ? kTerms : results, q_rows = Q_TURNED ? kTerms : S::kTokens;
+    bool fits = a->tokens >= 1 && a->features >= 1 && a->terms >= 0 && a->parts >= 1;
+    // vectors of 16 bytes are whole: of terms, or of turned features and tokens, which a row has room for
+    fits = fits && ((P_TURNED && Q_TURNED) || a->terms % kVec == 0);
+    fits = fits && (!P_TURNED || (a->features % kVec == 0 && a->p_turn % kTerms == 0));
+    fits = fits && (!Q_TURNED || a->tokens % kVec == 0);
+    for (const int64_t stride : {a->p_stride[0], a->p_stride[1], a->q_stride}) {
+        fits = fits && stride >= 0 && stride * kE % 16 == 0;
+    }
+    fits = fits && p_rows * a->p_stride[0] * kE <= furthest && p_rows * a->p_stride[1] * kE <= furthest &&
+           q_rows * a->q_stride * kE <= furthest;
+    const int64_t token_tiles = (a->tokens + S::kTokens - 1) / S::kTokens;
+    const int64_t feature_tiles = (a->features + results - 1) / results, blocks = token_tiles * feature_tiles * a->parts;
+    if (!fits || !fits_launch(blocks, S::kThreads)) {
+        return 0;
+    }
+    a->token_tiles = (uint32_t)token_tiles;
+    a->feature_tiles = (uint32_t)feature_tiles;
+    return blocks;
+}
+
+template <typename S, typename... A>
+hipError_t launch_kernel(void (*kernel)(A...), int64_t blocks, hipStream_t stream, std::atomic<uint32_t>& allowed, A... args)
+{
+    if (!fits_launch(blocks, S::kThreads)) {
         return hipErrorInvalidValue;
     }
-    a.token_tiles = (uint32_t)token_tiles;
-    a.feature_tiles = (uint32_t)feature_tiles;
-    static std::atomic<uint32_t> allowed{0};
     if (S::kLds > 65536) {
-        const hipError_t e = allow_dynamic_lds((const void*)product_kernel<T, KIND, FB, TB, WF, WT>, S::kLds, allowed);
+        const hipError_t e = allow_dynamic_lds((const void*)kernel, S::kLds, allowed);
         if (e != hipSuccess) {
             return e;
         }
     }
-    hipLaunchKernelGGL((product_kernel<T, KIND, FB, TB, WF, WT>), dim3((unsigned)blocks), dim3(S::kThreads), S::kLds, stream,
-                       a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(S::kThreads), S::kLds, stream, args...);
     return hipGetLastError();
 }
 
-template <typename T>
-hipError_t launch_typed(const ProductArgs& a, int kind, int tile, hipStream_t stream)
+template <typename T, typename S>
+hipError_t launch_gated_shape(ProductArgs a, hipStream_t stream)
 {
-    if (kind == kGated) {
-        return tile == kTile256 ? launch_shape<T, kGated, 2, 4, 4, 2>(a, stream) : launch_shape<T, kGated, 2, 2, 2, 2>(a, stream);
+    static std::atomic<uint32_t> allowed{0};
+    const int64_t blocks = prepare<T, true, false, false, S>(&a);
+    return blocks < 1 ? hipErrorInvalidValue : launch_kernel<S>(gated_kernel<T, S>, blocks, stream, allowed, a);
+}
+
+// `x` or `weights` may be null: one product alone
+template <typename T, typename S>
+hipError_t launch_gradients_shape(const ProductArgs* x, const ProductArgs* weights, hipStream_t stream)
+{
+    static std::atomic<uint32_t> allowed{0};
+    ProductArgs ax, aw;
+    int64_t first = 0, others = 0;
+    if (x != nullptr) {
+        ax = *x;
+        first = prepare<T, false, true, false, S>(&ax);
     }
-    if (kind == kPlain) {
-        return tile == kTile256 ? launch_shape<T, kPlain, 2, 4, 4, 2>(a, stream) : launch_shape<T, kPlain, 2, 2, 2, 2>(a, stream);
+    if (weights != nullptr) {
+        aw = *weights;
+        others = prepare<T, false, true, true, S>(&aw);
     }
-    return launch_shape<T, kPartial, 2, 2, 2, 2>(a, stream);
+    if ((x != nullptr && first < 1) || (weights != nullptr && others < 1)) {
+        return hipErrorInvalidValue;
+    }
+    if (first + others == 0) {
+        return hipSuccess;
+    }
+    return launch_kernel<S>(gradients_kernel<T, S>, first + others, stream, allowed, ax, aw, (uint32_t)first);
+}
+
+template <typename T>
+hipError_t launch_gated_typed(const ProductArgs& a, bool large, hipStream_t stream)
+{
+    return large ? launch_gated_shape<T, Large>(a, stream) : launch_gated_shape<T, Small>(a, stream);
+}
+
+template <typename T>
+hipError_t launch_gradients_typed(const ProductArgs* x, const ProductArgs* weights, bool large, hipStream_t stream)
+{
+    return large ? launch_gradients_shape<T, Large>(x, weights, stream) : launch_gradients_shape<T, Small>(x, weights, stream);
 }
 
 }  // namespace prod

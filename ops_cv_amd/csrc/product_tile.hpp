@@ -2,19 +2,21 @@
 //
 //   out[t][f] = sum over k of Q[t][k] P[f][k]
 //
-// Both operands are rows of terms that lie side by side ("tokens" Q and "features" P), so one kernel serves every product;
-// where a gradient sums over another dimension, its operands are laid out so first (gated_layout.hip).
+// with "tokens" Q and "features" P.  An operand lies as it comes: as rows whose terms are side by side (t or f outside), or
+// "turned", as rows of tokens or features, one a term (k outside).  Forward both are rows of terms; the gradient of x is a sum
+// over the inner features, which are the weights' rows, and those of the weights sums over the rows of x and of the gradients.
 //
-// A workgroup makes a tile of TOKENS x FEATURES results.  Stages of 128 bytes of terms (64 of 16 bits, 32 FLOAT) of both
-// operands are copied straight to LDS, two stages in turn: while one is multiplied the other is under way.  Features are the
-// rows of the 32 x 32 results and tokens their columns, so that a lane holds four neighbouring features of a token.  In the
-// gated forward product blocks of 32 features alternate between the two weights, so that a lane holds gate and up of the same
-// features, and the activation and the product need no other lane.
+// A workgroup makes a tile of results.  Stages of 128 bytes of terms (64 of 16 bits, 32 FLOAT) of both operands are copied
+// straight to LDS, two stages in turn: while one is multiplied the other is under way.  Features are the rows of the 32 x 32
+// results and tokens their columns, so that a lane holds four neighbouring features of a token.  In the gated forward product
+// blocks of 32 features alternate between the two weights, so that a lane holds gate and up of the same features, and the
+// activation and the product need no other lane.
 #pragma once
 
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "acl_types.hpp"
 #include "attention_tile.hpp"
@@ -25,32 +27,41 @@ namespace prod {
 
 using att::acc_t;
 
-enum Kind { kPlain = 0, kGated = 1, kPartial = 2 };  // kPartial: 32-bit sums over a part of the terms
-
 struct ProductArgs {
-    const void* p[2] = {nullptr, nullptr};  // features' rows; kGated: gate and up
-    int64_t p_stride[2] = {0, 0};           // elements
+    // features' rows of terms: gate and up.  Turned: rows of features, p[1] from term `p_turn` on, `p_terms` of each.
+    const void* p[2] = {nullptr, nullptr};
+    int64_t p_stride[2] = {0, 0};  // elements
+    int64_t p_turn = 0, p_terms = 0;
     const void* q = nullptr;
     int64_t q_stride = 0;
-    int64_t tokens = 0, features = 0;  // results; kGated: features of y
-    int64_t terms = 0;                 // whole vectors of 16 bytes
-    // results of tokens below `turn` go to out[0], the others to out[1] from its first row on; kGated: y, gate and up
+    int64_t tokens = 0, features = 0;  // of the operands; gated: features of y
+    int64_t columns = 0;               // features of the results that are written: turned rows may be padded
+    int64_t terms = 0;                 // rows of terms: whole vectors of 16 bytes
+    // plain: results of tokens below `turn` go to out[0], the others to out[1] from its first row on, `rows` to each;
+    // gated: y, gate and up
     void* out[3] = {nullptr, nullptr, nullptr};
     int64_t out_stride[3] = {0, 0, 0};
-    int64_t turn = 0;
-    const float* token_scale = nullptr;  // factor of every token's results, or null
+    int64_t turn = INT64_MAX, rows = 0;
+    const float* token_scale = nullptr;  // plain: factor of every token's results, or null
     const void* bias[2] = {nullptr, nullptr};
     int activation = 0;
-    int wide[3] = {0, 0, 0};  // the output's rows start on 16 bytes
-    // launch
-    uint32_t token_tiles = 0, feature_tiles = 0, parts = 1;
-    int64_t part_stages = 0;  // kPartial: stages of a part
+    // plain: the terms in parts of `part_stages` stages, whose sums go to `partial`, (parts, tokens, features); or null
+    float* partial = nullptr;
+    uint32_t parts = 1, part_stages = 0;
+    uint32_t token_tiles = 0, feature_tiles = 0;  // set by the launcher
 };
 
 // ------------------------------------------------------------------------------------------------- activations
 
 // silu, gelu (erf) and gelu (tanh) in the order of opscvGateActivation: value, and derivative where wanted.
-__device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
+
+// By the hardware's exponential and reciprocal, a unit in the last place each; the product with log2 e loses |x| 2^-24 of the
+// exponential.  A workgroup has nothing to do beside its results' activations: with expf and a division the product of 4096
+// rows, 4096 to 14336 bf16, takes 838 us.
+__device__ __forceinline__ float sigmoid(float x)
+{
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * x));
+}
 
 __device__ __forceinline__ float activate(float g, int kind)
 {
@@ -145,123 +156,238 @@ __device__ __forceinline__ void load_to_lds(att::rsrc_t rsrc, uint32_t dst, uint
 }
 
 // FB x TB blocks of 32 x 32 results a wavefront (features, tokens), WF x WT wavefronts a workgroup.
-template <typename T, int KIND, int FB, int TB, int WF, int WT>
+template <int FB_, int TB_, int WF_, int WT_>
 struct Shape {
+    static constexpr int FB = FB_, TB = TB_, WF = WF_, WT = WT_;
     static constexpr int kWaves = WF * WT, kThreads = 64 * kWaves;
     static constexpr int kFeatures = 32 * FB * WF, kTokens = 32 * TB * WT;  // rows of the operands in a stage
-    static constexpr int kResults = KIND == kGated ? kFeatures / 2 : kFeatures;  // features of the tile's results
     static constexpr int kStageBytes = (kFeatures + kTokens) * kRowBytes;
     static constexpr int kLds = 2 * kStageBytes;
-    static constexpr int kLoadsP = kFeatures / 8 / kWaves, kLoadsQ = kTokens / 8 / kWaves;  // of a wavefront and stage
-    static constexpr int kPitch = 32 * (KIND == kGated ? 1 : FB) * (int)sizeof(T) + 16;  // of a token's results on their way out
     static_assert(kWaves % 2 == 0 && kFeatures % (8 * kWaves) == 0 && kTokens % (8 * kWaves) == 0, "whole loads");
-    static_assert(KIND != kGated || (FB % 2 == 0 && (kWaves == 4 || kWaves == 8)), "gate and up in turn");
-    static_assert(kWaves * 32 * kPitch <= kLds, "the results' way out fits the stages");
+    static_assert(kWaves * 32 * (32 * FB * 4 + 16) <= kLds, "the results' way out fits the stages");
+};
+typedef Shape<2, 4, 4, 2> Large;  // 256 x 256, eight wavefronts, one workgroup a CU
+typedef Shape<2, 2, 2, 2> Small;  // 128 x 128, four wavefronts, two workgroups a CU
+
+// One operand's part of the stages: WIDTH tokens or features, BLOCKS blocks of 32 a wavefront, WAVES wavefronts.
+template <typename T, bool TURNED, int WIDTH, int BLOCKS, int WAVES>
+struct Side {
+    typedef typename Step<T>::Frag Frag;
+    static constexpr int kE = (int)sizeof(T);
+    static constexpr int kLoads = WIDTH / 8 / WAVES;                      // of a wavefront and stage, 1024 bytes each
+    static constexpr int kTerms = kRowBytes / kE;                         // of a stage
+    static constexpr int kPitch = TURNED ? WIDTH * kE : kRowBytes;        // of a row in LDS
+    static constexpr int kRowsALoad = 1024 / kPitch;                      // turned: 1, 2 or 4
+
+    uint32_t off[kLoads];  // of this lane's vectors from the stage's base; kOutside: past the end of the tokens or features
+    int first;             // rows of terms: the vector's number in its row; turned: the term of the first load
+    int at[TURNED ? BLOCKS : 4];
+
+    // Turned rows: vector c of row k lies at place c ^ turned_swizzle(k), so that what a half wavefront reads together, four
+    // rows of 64 bytes (FLOAT: two of 128, four rows apart), falls on all 64 banks.
+    static __device__ __forceinline__ int turned_swizzle(int k) { return kE == 2 ? (k & 3) << 2 : ((k >> 2) & 1) << 3; }
+
+    // `left`: tokens or features from the tile's first on; `row`: which row of the operand row r of the tile is
+    template <typename F>
+    __device__ __forceinline__ void places(int64_t stride, int64_t left, int wave, int lane, F&& row)
+    {
+        if constexpr (TURNED) {
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) {
+                const int byte = (i * WAVES + wave) * 1024 + lane * 16, k = byte / kPitch;
+                const int c = (byte % kPitch / 16) ^ turned_swizzle(k);
+                off[i] = c * (16 / kE) < left ? (uint32_t)(k * stride * kE) + (uint32_t)(c * 16) : att::kOutside;
+            }
+            first = (wave * 1024 + lane * 16) / kPitch;
+        } else {
+            const int row8 = wave * 8 + (lane >> 3);  // of the first load
+            first = (lane & 7) ^ swizzle(row8);       // the same in all loads: WAVES * 8 is a multiple of 16
+#pragma unroll
+            for (int i = 0; i < kLoads; i++) {
+                const int64_t r = row(i * WAVES * 8 + row8);
+                off[i] = r < left ? (uint32_t)(r * stride * kE) + (uint32_t)(first * 16) : att::kOutside;
+            }
+        }
+    }
+
+    // Copies a stage whose first term the buffer, `ahead` bytes on, begins with; `terms` are left from there on, and what is
+    // behind them becomes zeros.  `rsrc` gives the buffer of load i.
+    template <typename F>
+    __device__ __forceinline__ void load(F&& rsrc, uint32_t to, uint32_t ahead, int terms) const
+    {
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) {
+            const int own = TURNED ? first + i * WAVES * kRowsALoad : first * (16 / kE);
+            load_to_lds(rsrc(i), to + (uint32_t)(i * WAVES * 1024), own < terms ? off[i] : att::kOutside, ahead);
+        }
+    }
+
+    // Where this lane reads the blocks from `block` on.
+    __device__ __forceinline__ void reads(int block, int lane)
+    {
+        if constexpr (!TURNED) {
+            // row l % 32 of a block, vector 2 j + h of step j
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                at[j] = (block * 32 + (lane & 31)) * kRowBytes + (((2 * j + (lane >> 5)) ^ swizzle(lane & 31)) << 4);
+            }
+        } else {
+            const int h = lane >> 5, i = lane & 15;
+#pragma unroll
+            for (int b = 0; b < BLOCKS; b++) {
+                if constexpr (kE == 2) {
+                    // Sixteen lanes together read four rows of sixteen elements, eight bytes a lane (row i / 4, elements
+                    // 4 (i % 4) .. + 3), and the instruction hands lane i column i of them.
+                    const int r = 8 * h + (i >> 2);
+                    at[b] = r * kPitch + (((block + b) * 64) ^ (turned_swizzle(r) * 16)) + ((lane >> 4) & 1) * 32 + (i & 3) * 8;
+                } else {
+                    at[b] = 4 * h * kPitch + (((block + b) * 128) ^ (h * 128)) + (lane & 31) * 4;
+                }
+            }
+        }
+    }
+
+    // Operand of step j of the stage at `from`, block b: terms 16 j + 8 h .. + 7 (FLOAT: 8 j + 4 h .. + 3) of token or
+    // feature l % 32.
+    __device__ __forceinline__ Frag read(const char* from, int j, int b) const
+    {
+        if constexpr (!TURNED) {
+            return *reinterpret_cast<const Frag*>(from + at[j] + b * 32 * kRowBytes);
+        } else if constexpr (kE == 2) {
+            typedef __attribute__((address_space(3))) att::s16x4* place;
+            const char* const here = from + at[b] + 16 * j * kPitch;
+            const att::s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((place)(here));
+            const att::s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((place)(here + 4 * kPitch));
+            att::s16x8 both;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                both[e] = lo[e];
+                both[4 + e] = hi[e];
+            }
+            return __builtin_bit_cast(Frag, both);
+        } else {
+            const char* const here = from + at[b] + 8 * j * kPitch;
+            Frag f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                f[e] = *reinterpret_cast<const float*>(here + e * kPitch);
+            }
+            return f;
+        }
+    }
 };
 
-template <typename T, int KIND, int FB, int TB, int WF, int WT>
-__global__ __launch_bounds__(64 * WF * WT) void product_kernel(ProductArgs a)
+// Where a workgroup's tile lies.
+struct TileOf {
+    uint32_t t, f, part;
+};
+
+// Workgroups are dealt to the eight XCDs in turn, and each XCD's share is a run of tiles that share operands in its L2: four
+// rows of tiles, column by column.
+__device__ __forceinline__ TileOf tile_of(const ProductArgs& a, uint32_t block)
 {
-    typedef Shape<T, KIND, FB, TB, WF, WT> S;
+    constexpr uint32_t kGroup = 4;
+    const uint32_t tiles = a.token_tiles * a.feature_tiles, total = tiles * a.parts;
+    const uint32_t xcd = block & 7, each = total >> 3, more = total & 7;
+    uint32_t id = xcd * each + (xcd < more ? xcd : more) + (block >> 3);
+    TileOf tile;
+    tile.part = id / tiles;
+    id -= tile.part * tiles;
+    const uint32_t run = kGroup * a.feature_tiles, group = id / run, first = group * kGroup;
+    const uint32_t high = a.token_tiles - first < kGroup ? a.token_tiles - first : kGroup;
+    id -= group * run;
+    tile.f = id / high;
+    tile.t = first + id - tile.f * high;
+    return tile;
+}
+
+// A vector to memory on any element's boundary: rows of odd lengths are written as fast as memory takes them.
+template <typename T>
+struct Loose {
+    T v[16 / sizeof(T)];
+};
+
+template <typename T, bool GATED, bool P_TURNED, bool Q_TURNED, typename S>
+__device__ __forceinline__ void product(const ProductArgs& a, uint32_t block, char* lds)
+{
     typedef typename Step<T>::Frag Frag;
-    constexpr int kE = (int)sizeof(T);
-    extern __shared__ __align__(16) char lds[];
+    constexpr int kE = (int)sizeof(T), FB = S::FB, TB = S::TB;
+    constexpr int kResults = GATED ? S::kFeatures / 2 : S::kFeatures;  // features of the tile's results
+    static_assert(!GATED || (FB % 2 == 0 && (S::kWaves == 4 || S::kWaves == 8) && !P_TURNED && !Q_TURNED), "gate and up in turn");
     const int lane = (int)threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int wf = wave % WF, wt = wave / WF;
+    const int wf = wave % S::WF, wt = wave / S::WF;
+    const TileOf tile = tile_of(a, block);
+    const int64_t t0 = (int64_t)tile.t * S::kTokens, f0 = (int64_t)tile.f * kResults;
 
-    // Which tile: workgroups are dealt to the eight XCDs in turn, and each XCD's share is a run of tiles that share operands
-    // in its L2: four rows of tiles, column by column.
-    uint32_t tile_t, tile_f, part;
-    {
-        const uint32_t tiles = a.token_tiles * a.feature_tiles, total = tiles * a.parts;
-        const uint32_t xcd = blockIdx.x & 7, each = total >> 3, more = total & 7;
-        uint32_t id = xcd * each + (xcd < more ? xcd : more) + (blockIdx.x >> 3);
-        part = id / tiles;
-        id -= part * tiles;
-        constexpr uint32_t kGroup = 4;
-        const uint32_t run = kGroup * a.feature_tiles, group = id / run, first = group * kGroup;
-        const uint32_t high = a.token_tiles - first < kGroup ? a.token_tiles - first : kGroup;
-        id -= group * run;
-        tile_f = id / high;
-        tile_t = first + id - tile_f * high;
-    }
-    const int64_t t0 = (int64_t)tile_t * S::kTokens, f0 = (int64_t)tile_f * S::kResults;
-
-    // What this lane copies of every stage: vector `chunk` of some rows; rows past the end become zeros.
-    const int row8 = wave * 8 + (lane >> 3);  // of the first load
-    const int chunk = (lane & 7) ^ swizzle(row8);  // the same in all loads: kWaves * 8 is a multiple of 16
-    uint32_t off_p[S::kLoadsP], off_q[S::kLoadsQ];
-    att::rsrc_t rsrc_p[2], rsrc_q;
-    {
-        const int64_t left = a.tokens - t0;
+    typedef Side<T, P_TURNED, S::kFeatures, FB, S::kWaves> SideP;
+    typedef Side<T, Q_TURNED, S::kTokens, TB, S::kWaves> SideQ;
+    SideP side_p;
+    SideQ side_q;
+    // gate or up, rows of 32 features in turn: with eight wavefronts by the wavefront, with four by the load
+    const int own = GATED && S::kWaves == 8 ? (wave >> 2) & 1 : 0;
+    const int64_t own_stride = own != 0 ? a.p_stride[1] : a.p_stride[0];
+    side_p.places(own_stride, a.features - f0, wave, lane, [](int r) { return GATED ? (r >> 6) * 32 + (r & 31) : r; });
+    if constexpr (GATED && S::kWaves == 4) {
 #pragma unroll
-        for (int i = 0; i < S::kLoadsQ; i++) {
-            const int r = i * S::kWaves * 8 + row8;
-            off_q[i] = r < left ? (uint32_t)(r * a.q_stride * kE) + (uint32_t)(chunk * 16) : att::kOutside;
+        for (int i = 1; i < SideP::kLoads; i += 2) {  // of up, whose stride is its own
+            const int r = i * 32 + wave * 8 + (lane >> 3);
+            const int64_t f = (r >> 6) * 32 + (r & 31);
+            side_p.off[i] = f < a.features - f0 ? (uint32_t)(f * a.p_stride[1] * kE) + (uint32_t)(side_p.first * 16) : att::kOutside;
         }
+    }
+    side_q.places(a.q_stride, a.tokens - t0, wave, lane, [](int r) { return r; });
+    att::rsrc_t rsrc_p[2], rsrc_q;  // rows of terms: once; turned rows: stage by stage, further than 32 bits
+    if constexpr (!P_TURNED) {
+        rsrc_p[0] = att::buffer((const char*)(own != 0 ? a.p[1] : a.p[0]) + f0 * own_stride * kE, kInside);
+        rsrc_p[1] = GATED && S::kWaves == 4 ? att::buffer((const char*)a.p[1] + f0 * a.p_stride[1] * kE, kInside) : rsrc_p[0];
+    }
+    if constexpr (!Q_TURNED) {
         rsrc_q = att::buffer((const char*)a.q + t0 * a.q_stride * kE, kInside);
     }
-    {
-        const int64_t left = a.features - f0;
-#pragma unroll
-        for (int i = 0; i < S::kLoadsP; i++) {
-            const int r = i * S::kWaves * 8 + row8;
-            const int f = KIND == kGated ? (r >> 6) * 32 + (r & 31) : r;
-            const int half = KIND == kGated ? (r >> 5) & 1 : 0;
-            off_p[i] = f < left ? (uint32_t)(f * a.p_stride[half] * kE) + (uint32_t)(chunk * 16) : att::kOutside;
-        }
-        // gate or up: with eight wavefronts by the wavefront, with four by the load
-        const int own = KIND == kGated && S::kWaves == 8 ? (wave >> 2) & 1 : 0;
-        const void* const base = own != 0 ? a.p[1] : a.p[0];
-        const int64_t stride = own != 0 ? a.p_stride[1] : a.p_stride[0];
-        rsrc_p[0] = att::buffer((const char*)base + f0 * stride * kE, kInside);
-        rsrc_p[1] = KIND == kGated && S::kWaves == 4
-                        ? att::buffer((const char*)a.p[1] + f0 * a.p_stride[1] * kE, kInside)
-                        : rsrc_p[0];
+    constexpr int kTerms = kRowBytes / kE;
+    uint32_t first_stage = 0, stages = (uint32_t)((a.terms + kTerms - 1) / kTerms);
+    if (!GATED && a.parts > 1) {
+        first_stage = tile.part * a.part_stages;
+        const uint32_t left = stages > first_stage ? stages - first_stage : 0;
+        stages = left < a.part_stages ? left : a.part_stages;
     }
     const uint32_t lds0 = att::lds_place(lds);
-    const uint32_t term_bytes = (uint32_t)(a.terms * kE);
-    uint32_t first_stage = 0, stages = (term_bytes + kRowBytes - 1) / kRowBytes;
-    if (KIND == kPartial) {
-        first_stage = part * (uint32_t)a.part_stages;
-        const uint32_t left = stages > first_stage ? stages - first_stage : 0;
-        stages = left < (uint32_t)a.part_stages ? left : (uint32_t)a.part_stages;
-    }
     const auto load_stage = [&](uint32_t stage, int buffer) {
-        const uint32_t at = (first_stage + stage) * kRowBytes;
-        const bool there = at + (uint32_t)chunk * 16 < term_bytes;  // the last stage may end early: zeros, on both sides
+        const int64_t term = (int64_t)(first_stage + stage) * kTerms;
         const uint32_t to = lds0 + (uint32_t)(buffer * S::kStageBytes + wave * 1024);
-#pragma unroll
-        for (int i = 0; i < S::kLoadsP; i++) {
-            load_to_lds(rsrc_p[S::kWaves == 4 ? i & 1 : 0], to + (uint32_t)(i * S::kWaves * 1024),
-                        there ? off_p[i] : att::kOutside, at);
+        const int left = (int)(a.terms - term < kTerms ? a.terms - term : kTerms);
+        if constexpr (P_TURNED) {
+            const int half = term >= a.p_turn ? 1 : 0;
+            const int64_t row = half != 0 ? term - a.p_turn : term;
+            const int64_t there = a.p_terms - row;  // none or less where only zeros stand for the padding of the other operand
+            const int64_t stride = half != 0 ? a.p_stride[1] : a.p_stride[0];
+            const att::rsrc_t rsrc = att::buffer((const char*)(half != 0 ? a.p[1] : a.p[0]) + (row * stride + f0) * kE, kInside);
+            side_p.load([&](int) { return rsrc; }, to, 0, there < left ? (int)there : left);
+        } else {
+            side_p.load([&](int i) { return rsrc_p[S::kWaves == 4 ? i & 1 : 0]; }, to, (uint32_t)(term * kE), left);
         }
-#pragma unroll
-        for (int i = 0; i < S::kLoadsQ; i++) {
-            load_to_lds(rsrc_q, to + (uint32_t)(S::kFeatures * kRowBytes + i * S::kWaves * 1024),
-                        there ? off_q[i] : att::kOutside, at);
+        const uint32_t to_q = to + S::kFeatures * kRowBytes;
+        if constexpr (Q_TURNED) {
+            const att::rsrc_t rsrc = att::buffer((const char*)a.q + (term * a.q_stride + t0) * kE, kInside);
+            side_q.load([&](int) { return rsrc; }, to_q, 0, left);
+        } else {
+            side_q.load([&](int) { return rsrc_q; }, to_q, (uint32_t)(term * kE), left);
         }
     };
 
-    // Where this lane reads: row l % 32 of a block, vector 2 j + h of step j.
-    int at_step[4];
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        at_step[j] = (lane & 31) * kRowBytes + (((2 * j + (lane >> 5)) ^ swizzle(lane & 31)) << 4);
-    }
-    const char* const from_p = lds + wf * FB * 32 * kRowBytes;
-    const char* const from_q = lds + (S::kFeatures + wt * TB * 32) * kRowBytes;
+    side_p.reads(wf * FB, lane);
+    side_q.reads(wt * TB, lane);
     Frag fp[2][FB], fq[2][TB];
     const auto read_step = [&](int j, int buffer, int slot) {
-        const int at = at_step[j] + buffer * S::kStageBytes;
+        const char* const from = lds + buffer * S::kStageBytes;
 #pragma unroll
         for (int b = 0; b < FB; b++) {
-            fp[slot][b] = *reinterpret_cast<const Frag*>(from_p + at + b * 32 * kRowBytes);
+            fp[slot][b] = side_p.read(from, j, b);
         }
 #pragma unroll
         for (int b = 0; b < TB; b++) {
-            fq[slot][b] = *reinterpret_cast<const Frag*>(from_q + at + b * 32 * kRowBytes);
+            fq[slot][b] = side_q.read(from + S::kFeatures * kRowBytes, j, b);
         }
     };
     acc_t acc[FB][TB];
@@ -288,7 +414,7 @@ __global__ __launch_bounds__(64 * WF * WT) void product_kernel(ProductArgs a)
         load_stage(0, 0);
         if (stages > 1) {
             load_stage(1, 1);
-            __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(S::kLoadsP + S::kLoadsQ) : "memory");
+            __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(SideP::kLoads + SideQ::kLoads) : "memory");
         } else {
             __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
@@ -319,8 +445,9 @@ __global__ __launch_bounds__(64 * WF * WT) void product_kernel(ProductArgs a)
     // A wavefront's results go out by way of a place of its own in LDS, 32 tokens at a time, so that neighbouring lanes write
     // neighbouring vectors of a token.  Register r of a block is feature 8 (r / 4) + 4 h + r % 4 of token l % 32.
     const int h = lane >> 5, n = lane & 31;
-    if constexpr (KIND == kPartial) {
-        float* const to = (float*)a.out[0] + ((int64_t)part * a.tokens) * a.features;
+    const bool partial = !GATED && a.partial != nullptr;
+    if (partial) {
+        float* const to = a.partial + (int64_t)tile.part * a.tokens * a.features;
 #pragma unroll
         for (int c = 0; c < TB; c++) {
             const int64_t t = t0 + (wt * TB + c) * 32 + n;
@@ -336,115 +463,141 @@ __global__ __launch_bounds__(64 * WF * WT) void product_kernel(ProductArgs a)
             }
         }
         return;
-    } else {
-        constexpr int kBlocks = KIND == kGated ? FB / 2 : FB;  // of results, a row of them; gated: one at a time
-        constexpr int kRow = KIND == kGated ? 1 : FB;          // blocks of 32 features that go out together
-        constexpr int kVec = 16 / kE;
-        constexpr int kChunks = 32 * kRow * kE / 16;           // vectors of a token
-        __syncthreads();  // all have read their last stage
-        char* const own = lds + wave * 32 * S::kPitch;
-        // Writes out what lies in `own`: tokens t.. , features f..
-        const auto put = [&](int which, int64_t t, int64_t f) {
-            __asm__ volatile("" ::: "memory");  // the compiler keeps the order; LDS does for one wavefront
+    }
+    constexpr int kRow = GATED ? 1 : FB;             // blocks of 32 features that go out together
+    constexpr int kPitch = 32 * kRow * kE + 16;      // of a token on its way
+    constexpr int kVec = 16 / kE, kChunks = 32 * kRow * kE / 16;  // vectors of a token
+    __syncthreads();  // all have read their last stage
+    char* const place = lds + wave * 32 * kPitch;
+    // Writes out what lies there: tokens t.. , features f..
+    const auto put = [&](int which, int64_t t, int64_t f) {
+        __asm__ volatile("" ::: "memory");  // the compiler keeps the order; LDS does for one wavefront
 #pragma unroll
-            for (int i = 0; i < 32 * kChunks / 64; i++) {
-                const int token = (i * 64 + lane) / kChunks, c = (i * 64 + lane) % kChunks;
-                const Pack16 v = *reinterpret_cast<const Pack16*>(own + token * S::kPitch + c * 16);
-                if (t + token < a.tokens) {
-                    const bool second = KIND == kPlain && t + token >= a.turn;
-                    const int64_t row = second ? t + token - a.turn : t + token;
-                    const int64_t stride = second ? a.out_stride[1] : a.out_stride[which];
-                    T* const to = (T*)(second ? a.out[1] : a.out[which]) + row * stride + f + c * kVec;
-                    const int64_t left = a.features - (f + c * kVec);
-                    if ((second ? a.wide[1] : a.wide[which]) != 0 && left >= kVec) {
-                        *reinterpret_cast<Pack16*>(to) = v;
-                    } else {
-                        const T* const each = reinterpret_cast<const T*>(&v);
+        for (int i = 0; i < 32 * kChunks / 64; i++) {
+            const int token = (i * 64 + lane) / kChunks, c = (i * 64 + lane) % kChunks;
+            const Pack16 v = *reinterpret_cast<const Pack16*>(place + token * kPitch + c * 16);
+            const bool second = !GATED && t + token >= a.turn;
+            const int64_t row = second ? t + token - a.turn : t + token;
+            const int64_t left = a.columns - (f + c * kVec);
+            if (row < a.rows && left > 0) {
+                T* const to = (T*)(second ? a.out[1] : a.out[which]) + row * (second ? a.out_stride[1] : a.out_stride[which]) + f +
+                              c * kVec;
+                if (left >= kVec) {
+                    *reinterpret_cast<Loose<T>*>(to) = __builtin_bit_cast(Loose<T>, v);
+                } else {
+                    const Loose<T> each = __builtin_bit_cast(Loose<T>, v);
 #pragma unroll
-                        for (int e = 0; e < kVec; e++) {
-                            if (e < left) {
-                                to[e] = each[e];
-                            }
-                        }
-                    }
-                }
-            }
-            __asm__ volatile("" ::: "memory");
-        };
-        const auto hold = [&](int block, int quarter, const float (&x)[4]) {
-            tok::Pack<T, 4> k;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                k.v[e] = (T)x[e];
-            }
-            *reinterpret_cast<tok::Pack<T, 4>*>(own + n * S::kPitch + (block * 32 + 8 * quarter + 4 * h) * kE) = k;
-        };
-#pragma unroll
-        for (int c = 0; c < TB; c++) {
-            const int64_t t = t0 + (wt * TB + c) * 32;
-            if (t >= a.tokens) {
-                break;
-            }
-            if constexpr (KIND == kPlain) {
-                float scale = 1.0f;
-                if (a.token_scale != nullptr && t + n < a.tokens) {
-                    scale = a.token_scale[t + n];
-                }
-#pragma unroll
-                for (int b = 0; b < FB; b++) {
-#pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        float x[4];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            x[e] = acc[b][c][4 * q + e] * scale;
-                        }
-                        hold(b, q, x);
-                    }
-                }
-                put(0, t, f0 + wf * FB * 32);
-            } else {
-#pragma unroll
-                for (int b = 0; b < kBlocks; b++) {
-                    const int64_t f = f0 + (wf * kBlocks + b) * 32;
-                    if (a.bias[0] != nullptr) {
-#pragma unroll
-                        for (int r = 0; r < 16; r++) {
-                            const int64_t own_f = f + 8 * (r / 4) + 4 * h + r % 4;
-                            if (own_f < a.features) {
-                                acc[2 * b][c][r] += (float)((const T*)a.bias[0])[own_f];
-                                acc[2 * b + 1][c][r] += (float)((const T*)a.bias[1])[own_f];
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        float x[4];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            x[e] = activate(acc[2 * b][c][4 * q + e], a.activation) * acc[2 * b + 1][c][4 * q + e];
-                        }
-                        hold(0, q, x);
-                    }
-                    put(0, t, f);
-                    if (a.out[1] != nullptr) {
-#pragma unroll
-                        for (int which = 0; which < 2; which++) {
-#pragma unroll
-                            for (int q = 0; q < 4; q++) {
-                                float x[4];
-#pragma unroll
-                                for (int e = 0; e < 4; e++) {
-                                    x[e] = acc[2 * b + which][c][4 * q + e];
-                                }
-                                hold(0, q, x);
-                            }
-                            put(1 + which, t, f);
+                    for (int e = 0; e < kVec; e++) {
+                        if (e < left) {
+                            to[e] = each.v[e];
                         }
                     }
                 }
             }
         }
+        __asm__ volatile("" ::: "memory");
+    };
+    const auto hold = [&](int b, int quarter, const float (&x)[4]) {
+        tok::Pack<T, 4> k;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            k.v[e] = (T)x[e];
+        }
+        *reinterpret_cast<tok::Pack<T, 4>*>(place + n * kPitch + (b * 32 + 8 * quarter + 4 * h) * kE) = k;
+    };
+#pragma unroll
+    for (int c = 0; c < TB; c++) {
+        const int64_t t = t0 + (wt * TB + c) * 32;
+        if constexpr (!GATED) {
+            float scale = 1.0f;
+            if (a.token_scale != nullptr) {
+                const bool second = t + n >= a.turn;
+                const int64_t row = second ? t + n - a.turn : t + n;
+                scale = row < a.rows ? a.token_scale[second ? a.rows + row : row] : 1.0f;
+            }
+#pragma unroll
+            for (int b = 0; b < FB; b++) {
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    float x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        x[e] = acc[b][c][4 * q + e] * scale;
+                    }
+                    hold(b, q, x);
+                }
+            }
+            put(0, t, f0 + wf * FB * 32);
+        } else {
+#pragma unroll
+            for (int b = 0; b < FB / 2; b++) {
+                const int64_t f = f0 + (wf * FB / 2 + b) * 32;
+                if (a.bias[0] != nullptr) {
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        const int64_t own_f = f + 8 * (r / 4) + 4 * h + r % 4;
+                        if (own_f < a.features) {
+                            acc[2 * b][c][r] += (float)((const T*)a.bias[0])[own_f];
+                            acc[2 * b + 1][c][r] += (float)((const T*)a.bias[1])[own_f];
+                        }
+                    }
+                }
+                const auto put_values = [&](auto kind) {
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        float x[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            x[e] = activate(acc[2 * b][c][4 * q + e], kind.value) * acc[2 * b + 1][c][4 * q + e];
+                        }
+                        hold(0, q, x);
+                    }
+                };
+                if (a.activation == 0) {
+                    put_values(std::integral_constant<int, 0>());
+                } else if (a.activation == 1) {
+                    put_values(std::integral_constant<int, 1>());
+                } else {
+                    put_values(std::integral_constant<int, 2>());
+                }
+                put(0, t, f);
+                if (a.out[1] != nullptr) {
+#pragma unroll
+                    for (int which = 0; which < 2; which++) {
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            float x[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                x[e] = acc[2 * b + which][c][4 * q + e];
+                            }
+                            hold(0, q, x);
+                        }
+                        put(1 + which, t, f);
+                    }
+                }
+            }
+        }
+    }
+}
+
+template <typename T, typename S>
+__global__ __launch_bounds__(S::kThreads) void gated_kernel(ProductArgs a)
+{
+    extern __shared__ __align__(16) char lds[];
+    product<T, true, false, false, S>(a, blockIdx.x, lds);
+}
+
+// The gradients of x (`first` workgroups) and of the weights, in one launch: the long sums over the inner features first, so
+// that the short ones over the rows fill up the CUs that are done.
+template <typename T, typename S>
+__global__ __launch_bounds__(S::kThreads) void gradients_kernel(ProductArgs x, ProductArgs weights, uint32_t first)
+{
+    extern __shared__ __align__(16) char lds[];
+    if (blockIdx.x < first) {
+        product<T, false, true, false, S>(x, blockIdx.x, lds);
+    } else {
+        product<T, false, true, true, S>(weights, blockIdx.x - first, lds);
     }
 }
 

@@ -85,12 +85,6 @@ struct DropoutArgs {
     int64_t state_stride = 0;
 };
 
-// One operand of a matrix product: rows of `terms` elements, dense inside.
-struct Operand {
-    const void* ptr = nullptr;
-    int64_t row_stride = 0;
-};
-
 struct GatedArgs {
     int elem = 0;
     int activation = 0;

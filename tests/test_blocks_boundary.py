@@ -133,7 +133,7 @@ SHARED = [
     (dict(bg=None), NULLPTR), (dict(bu=None), NULLPTR), (dict(y=None), NULLPTR), (dict(bg=((41,), BF16)), INVALID),
     (dict(bu=((40,), F32)), INVALID), (dict(y=((6, 64), BF16)), INVALID), (dict(y=((2, 3, 40), BF16)), INVALID),
     (dict(wg=((0, 64), BF16), wu=((0, 64), BF16), bg=None, bu=None, y=((6, 0), BF16), gate=None, up=None), INVALID),
-    (dict(x=((6, 2 ** 20 + 1), BF16), wg=((40, 2 ** 20 + 1), BF16), wu=((40, 2 ** 20 + 1), BF16)), INVALID),
+    (dict(x=((6, 2 ** 19 + 1), BF16), wg=((40, 2 ** 19 + 1), BF16), wu=((40, 2 ** 19 + 1), BF16)), INVALID),
     (dict(x=((2 ** 30 + 1, 64), BF16), y=((2 ** 30 + 1, 40), BF16), gate=None, up=None), INVALID)] + SHARED)
 def test_gated(phase1, kw, status):
     st, ws, variant = phase1("opscvGatedProjection", *changed(GATED, **kw))
