@@ -395,6 +395,7 @@ aclnnStatus opscvGatedProjectionGetWorkspaceSize(const aclTensor* x, const aclTe
         plan_rows(ex.get(), kGaGate, gate, bytes, true, &a.gate);
         plan_rows(ex.get(), kGaUp, up, bytes, true, &a.up);
     }
+    plan_gated(&a);
     plan_bytes(ex.get(), kGaScratch, gated_scratch_bytes(a));
     return finish(api, ex, workspaceSize, executor);
 }
@@ -466,6 +467,7 @@ aclnnStatus opscvGatedProjectionBackwardGetWorkspaceSize(const aclTensor* gradY,
         plan_dense(ex.get(), kGgGradGateBias, gradGateBias, bytes, true);
         plan_dense(ex.get(), kGgGradUpBias, gradUpBias, bytes, true);
     }
+    plan_gated_grad(&a);
     plan_bytes(ex.get(), kGgScratch, gated_grad_scratch_bytes(a));
     return finish(api, ex, workspaceSize, executor);
 }

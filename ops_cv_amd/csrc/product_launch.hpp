@@ -7,7 +7,8 @@
 
 #include "kernels.hpp"
 #include "launch_limits.hpp"
-#include "product_tile.hpp"
+#include "product_few.hpp"
+#include "product_plan.hpp"
 
 namespace opscv {
 namespace prod {
@@ -88,10 +89,25 @@ hipError_t launch_gradients_shape(const ProductArgs* x, const ProductArgs* weigh
     return launch_kernel<S>(gradients_kernel<T, S>, first + others, stream, allowed, ax, aw, (uint32_t)first);
 }
 
+template <typename T, int TB, int AHEAD>
+hipError_t launch_few(const ProductArgs& a, hipStream_t stream)
+{
+    const int64_t e = (int64_t)sizeof(T), blocks = (a.features + kFewFeatures - 1) / kFewFeatures;
+    if (a.tokens < 1 || a.tokens > TB * 16 || a.features < 1 || a.terms < 1 || a.terms * e % 16 != 0 ||
+        !fits_launch(blocks, 64 * kFewWaves)) {
+        return hipErrorInvalidValue;
+    }
+    hipLaunchKernelGGL((gated_few_kernel<T, TB, AHEAD>), dim3((unsigned)blocks), dim3(64 * kFewWaves), 0, stream, a);
+    return hipGetLastError();
+}
+
 template <typename T>
 hipError_t launch_gated_typed(const ProductArgs& a, bool large, hipStream_t stream)
 {
-    return large ? launch_gated_shape<T, Large>(a, stream) : launch_gated_shape<T, Small>(a, stream);
+    if (a.tokens <= kFewRows) {
+        return a.tokens <= 16 ? launch_few<T, 1, 4>(a, stream) : a.tokens <= 32 ? launch_few<T, 2, 2>(a, stream) : launch_few<T, 4, 1>(a, stream);
+    }
+    return large ? launch_gated_shape<T, LargeGated>(a, stream) : launch_gated_shape<T, Small>(a, stream);
 }
 
 template <typename T>

@@ -85,6 +85,12 @@ struct DropoutArgs {
     int64_t state_stride = 0;
 };
 
+// How the matrix products of a call are made (product_plan.hpp).
+struct ProductPlan {
+    bool large = false;                                  // tiles of 256 x 256, else of 128 x 128
+    int64_t parts[2] = {1, 1}, part_stages[2] = {0, 0};  // of the terms; more than one part: a second kernel joins their sums
+};
+
 struct GatedArgs {
     int elem = 0;
     int activation = 0;
@@ -100,6 +106,7 @@ struct GatedArgs {
     void* grad_gate_bias = nullptr;        // both or neither
     void* grad_up_bias = nullptr;
     int want_x = 0, want_weights = 0, want_biases = 0;
+    ProductPlan plan;  // by plan_gated() / plan_gated_grad()
     char* scratch = nullptr;  // gated_scratch_bytes() / gated_grad_scratch_bytes()
 };
 
