@@ -42,14 +42,12 @@ bool in_place(const Rows& r, int64_t rows, int64_t width, int e)
            (rows == 1 || r.row_stride <= (int64_t)1 << 20);
 }
 
-// A stage of a large tile on one CU: 8.4 MFLOP of 16 bits at 5 TFLOP/s, 4.2 of FLOAT at 0.53
-double stage_us(const GatedArgs& a) { return a.elem == (int)Elem::F32 ? 8.0 : 1.7; }
-
 // ------------------------------------------------------------------------------------------------------------ forward
 
 struct ForwardLayout {
     int64_t terms = 0;                       // width in whole vectors
     int64_t x = -1, gate = -1, up = -1;      // offsets of padded copies; -1: in place
+    int64_t parts = -1;
     int64_t bytes = 0;
 };
 
@@ -68,8 +66,25 @@ ForwardLayout forward_layout(const GatedArgs& a)
     if (!in_place(a.up_weight, a.inner, a.width, e)) {
         l.up = s.take(a.inner * l.terms * e);
     }
+    if (a.plan.parts[0] > 1) {
+        l.parts = s.take(a.plan.parts[0] * a.rows * 2 * a.inner * 4);
+    }
     l.bytes = s.bytes;
     return l;
+}
+
+// An operand where it lies, or its place among the copies that are to be made.
+void lay_out(const Rows& r, int64_t rows, char* copy, const void** ptr, int64_t* stride, PadArgs* pads)
+{
+    *ptr = copy == nullptr ? r.ptr : copy;
+    *stride = copy == nullptr ? r.row_stride : pads->padded;
+    if (copy != nullptr) {
+        PadArgs::Copy& c = pads->copy[pads->count++];
+        c.from = r.ptr;
+        c.from_stride = r.row_stride;
+        c.rows = rows;
+        c.to = copy;
+    }
 }
 
 // ----------------------------------------------------------------------------------------------------------- backward
@@ -140,7 +155,11 @@ void plan_gated(GatedArgs* a)
 {
     const int e = elem_size((Elem)a->elem);
     const ProductSize size{a->rows, 2 * a->inner, (a->width * e + kRowBytes - 1) / kRowBytes};
-    a->plan = plan_products(&size, 1, false, stage_us(*a), a->compute_units);
+    a->plan = plan_products(&size, 1, e, a->compute_units);
+    if (a->rows <= kFewRows && few_us(a->rows, 2 * a->inner * a->width * e, e) <= a->plan.us) {
+        a->plan = ProductPlan();
+        a->plan.tile = kTileFew;
+    }
 }
 
 void plan_gated_grad(GatedArgs* a)
@@ -156,7 +175,7 @@ void plan_gated_grad(GatedArgs* a)
         size[count++] = {2 * padded, width, (a->rows * e + kRowBytes - 1) / kRowBytes};
     }
     if (count > 0) {
-        a->plan = plan_products(size, count, true, stage_us(*a), a->compute_units);
+        a->plan = plan_products(size, count, e, a->compute_units);
     }
 }
 
@@ -171,16 +190,15 @@ hipError_t launch_gated(const GatedArgs& a, hipStream_t stream)
     if (a.rows < 1 || a.width < 1 || a.inner < 1 || (l.bytes > 0 && a.scratch == nullptr)) {
         return hipErrorInvalidValue;
     }
-    const auto laid_out = [&](const Rows& r, int64_t rows, int64_t copy, const void** ptr, int64_t* stride) {
-        *ptr = copy < 0 ? r.ptr : a.scratch + copy;
-        *stride = copy < 0 ? r.row_stride : l.terms;
-        return copy < 0 ? hipSuccess
-                        : launch_pad_rows(elem, r.ptr, r.row_stride, rows, a.width, a.scratch + copy, l.terms, l.terms, stream);
-    };
+    const auto at = [&](int64_t offset) { return offset < 0 ? nullptr : a.scratch + offset; };
     ProductArgs p;
-    OPSCV_LAUNCH(laid_out(a.x, a.rows, l.x, &p.q, &p.q_stride));
-    OPSCV_LAUNCH(laid_out(a.gate_weight, a.inner, l.gate, &p.p[0], &p.p_stride[0]));
-    OPSCV_LAUNCH(laid_out(a.up_weight, a.inner, l.up, &p.p[1], &p.p_stride[1]));
+    PadArgs pads;
+    pads.width = a.width;
+    pads.padded = l.terms;
+    lay_out(a.x, a.rows, at(l.x), &p.q, &p.q_stride, &pads);
+    lay_out(a.gate_weight, a.inner, at(l.gate), &p.p[0], &p.p_stride[0], &pads);
+    lay_out(a.up_weight, a.inner, at(l.up), &p.p[1], &p.p_stride[1], &pads);
+    OPSCV_LAUNCH(launch_pad_rows(elem, pads, stream));
     p.tokens = p.rows = a.rows;
     p.features = p.columns = a.inner;
     p.terms = l.terms;
@@ -192,12 +210,15 @@ hipError_t launch_gated(const GatedArgs& a, hipStream_t stream)
     p.bias[0] = a.gate_bias;
     p.bias[1] = a.up_bias;
     p.activation = a.activation;
-    const bool large = a.plan.large;
+    p.partial = (float*)at(l.parts);
+    p.parts = (uint32_t)a.plan.parts[0];
+    p.part_stages = (uint32_t)a.plan.part_stages[0];
     switch (elem) {
-        case Elem::F32: return launch_products_f32(p, large, stream);
-        case Elem::F16: return launch_products_f16(p, large, stream);
-        default: return launch_products_bf16(p, large, stream);
+        case Elem::F32: OPSCV_LAUNCH(launch_products_f32(p, a.plan.tile, stream)); break;
+        case Elem::F16: OPSCV_LAUNCH(launch_products_f16(p, a.plan.tile, stream)); break;
+        default: OPSCV_LAUNCH(launch_products_bf16(p, a.plan.tile, stream)); break;
     }
+    return p.partial != nullptr ? launch_join(elem, p, true, stream) : hipSuccess;
 }
 
 hipError_t launch_gated_grad(const GatedArgs& a, hipStream_t stream)
@@ -230,16 +251,13 @@ hipError_t launch_gated_grad(const GatedArgs& a, hipStream_t stream)
         g.column_factor = g.row_factor + a.rows;
     }
     OPSCV_LAUNCH(launch_gate_grad(g, stream));
-    const auto laid_out = [&](const Rows& r, int64_t rows, int64_t copy, const void** ptr, int64_t* stride) {
-        *ptr = copy < 0 ? r.ptr : a.scratch + copy;
-        *stride = copy < 0 ? r.row_stride : l.width;
-        return copy < 0 ? hipSuccess
-                        : launch_pad_rows(elem, r.ptr, r.row_stride, rows, a.width, a.scratch + copy, l.width, l.width, stream);
-    };
+    PadArgs pads;
+    pads.width = a.width;
+    pads.padded = l.width;
     ProductArgs x, weights;
     if (a.want_x != 0) {
-        OPSCV_LAUNCH(laid_out(a.gate_weight, a.inner, l.gate, &x.p[0], &x.p_stride[0]));
-        OPSCV_LAUNCH(laid_out(a.up_weight, a.inner, l.up, &x.p[1], &x.p_stride[1]));
+        lay_out(a.gate_weight, a.inner, at(l.gate), &x.p[0], &x.p_stride[0], &pads);
+        lay_out(a.up_weight, a.inner, at(l.up), &x.p[1], &x.p_stride[1], &pads);
         x.p_turn = l.padded;
         x.p_terms = a.inner;
         x.q = g.by_rows;
@@ -257,7 +275,7 @@ hipError_t launch_gated_grad(const GatedArgs& a, hipStream_t stream)
     }
     if (a.want_weights != 0) {
         const int own = a.want_x != 0 ? 1 : 0;
-        OPSCV_LAUNCH(laid_out(a.x, a.rows, l.x, &weights.p[0], &weights.p_stride[0]));
+        lay_out(a.x, a.rows, at(l.x), &weights.p[0], &weights.p_stride[0], &pads);
         weights.p[1] = weights.p[0];
         weights.p_stride[1] = weights.p_stride[0];
         weights.p_turn = rounded(a.rows, kRowBytes);  // all terms are of the first
@@ -279,20 +297,21 @@ hipError_t launch_gated_grad(const GatedArgs& a, hipStream_t stream)
         weights.parts = (uint32_t)a.plan.parts[own];
         weights.part_stages = (uint32_t)a.plan.part_stages[own];
     }
+    OPSCV_LAUNCH(launch_pad_rows(elem, pads, stream));
     if (a.want_x != 0 || a.want_weights != 0) {
         const ProductArgs* const px = a.want_x != 0 ? &x : nullptr;
         const ProductArgs* const pw = a.want_weights != 0 ? &weights : nullptr;
         switch (elem) {
-            case Elem::F32: OPSCV_LAUNCH(launch_gradients_f32(px, pw, a.plan.large, stream)); break;
-            case Elem::F16: OPSCV_LAUNCH(launch_gradients_f16(px, pw, a.plan.large, stream)); break;
-            default: OPSCV_LAUNCH(launch_gradients_bf16(px, pw, a.plan.large, stream)); break;
+            case Elem::F32: OPSCV_LAUNCH(launch_gradients_f32(px, pw, a.plan.tile, stream)); break;
+            case Elem::F16: OPSCV_LAUNCH(launch_gradients_f16(px, pw, a.plan.tile, stream)); break;
+            default: OPSCV_LAUNCH(launch_gradients_bf16(px, pw, a.plan.tile, stream)); break;
         }
     }
     if (x.partial != nullptr) {
-        OPSCV_LAUNCH(launch_join(elem, x, stream));
+        OPSCV_LAUNCH(launch_join(elem, x, false, stream));
     }
     if (weights.partial != nullptr) {
-        OPSCV_LAUNCH(launch_join(elem, weights, stream));
+        OPSCV_LAUNCH(launch_join(elem, weights, false, stream));
     }
     if (a.want_biases != 0) {
         OPSCV_LAUNCH(launch_bias_sums(elem, g.sums, (a.rows + kGateRows - 1) / kGateRows, a.inner, a.grad_gate_bias,

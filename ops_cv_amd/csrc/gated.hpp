@@ -11,16 +11,25 @@ namespace prod {
 struct ProductArgs;
 
 // the gated forward product, and both products of the gradients (one may be null)
-hipError_t launch_products_f32(const ProductArgs& a, bool large, hipStream_t stream);
-hipError_t launch_products_f16(const ProductArgs& a, bool large, hipStream_t stream);
-hipError_t launch_products_bf16(const ProductArgs& a, bool large, hipStream_t stream);
-hipError_t launch_gradients_f32(const ProductArgs* x, const ProductArgs* weights, bool large, hipStream_t stream);
-hipError_t launch_gradients_f16(const ProductArgs* x, const ProductArgs* weights, bool large, hipStream_t stream);
-hipError_t launch_gradients_bf16(const ProductArgs* x, const ProductArgs* weights, bool large, hipStream_t stream);
+hipError_t launch_products_f32(const ProductArgs& a, int tile, hipStream_t stream);
+hipError_t launch_products_f16(const ProductArgs& a, int tile, hipStream_t stream);
+hipError_t launch_products_bf16(const ProductArgs& a, int tile, hipStream_t stream);
+hipError_t launch_gradients_f32(const ProductArgs* x, const ProductArgs* weights, int tile, hipStream_t stream);
+hipError_t launch_gradients_f16(const ProductArgs* x, const ProductArgs* weights, int tile, hipStream_t stream);
+hipError_t launch_gradients_bf16(const ProductArgs* x, const ProductArgs* weights, int tile, hipStream_t stream);
 
-// Rows of `width` elements, copied to rows of `to_stride`, zeros from `width` to `padded` on.
-hipError_t launch_pad_rows(Elem e, const void* from, int64_t from_stride, int64_t rows, int64_t width, void* to,
-                           int64_t to_stride, int64_t padded, hipStream_t stream);
+// Rows of `width` elements, copied to rows of `padded` with zeros behind them.
+struct PadArgs {
+    struct Copy {
+        const void* from = nullptr;
+        int64_t from_stride = 0, rows = 0;
+        void* to = nullptr;
+    };
+    Copy copy[3];
+    int count = 0;
+    int64_t width = 0, padded = 0;
+};
+hipError_t launch_pad_rows(Elem e, const PadArgs& a, hipStream_t stream);
 
 // Gradients of gate and up, as the products want them (gated_layout.hip).
 struct GateGradArgs {
@@ -43,8 +52,8 @@ constexpr int kGateRows = 64;
 
 hipError_t launch_gate_grad(const GateGradArgs& a, hipStream_t stream);
 
-// The sum of a product's parts in the places of its results (product_tile.hpp).
-hipError_t launch_join(Elem e, const ProductArgs& a, hipStream_t stream);
+// The sums of a product's parts, in the places of its results (product_tile.hpp).
+hipError_t launch_join(Elem e, const ProductArgs& a, bool gated, hipStream_t stream);
 
 // Sums of the rows of (rows, 2 inner): the first inner to `gate`, the others to `up`.
 hipError_t launch_bias_sums(Elem e, const float* sums, int64_t rows, int64_t inner, void* gate, void* up, hipStream_t stream);

@@ -29,26 +29,32 @@ constexpr int kRows = kGateRows;
 template <typename T>
 constexpr int kVec = 16 / (int)sizeof(T);
 
+// One copy for every blockIdx.y.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void pad_rows_kernel(const T* from, int64_t from_stride, int64_t rows, int64_t width,
-                                                            T* to, int64_t to_stride, int64_t padded)
+__global__ __launch_bounds__(kThreads) void pad_rows_kernel(PadArgs a)
 {
-    const int64_t vectors = padded / kVec<T>, total = rows * vectors;
+    const PadArgs::Copy& copy = a.copy[blockIdx.y];
+    const int64_t vectors = a.padded / kVec<T>, total = copy.rows * vectors;
     for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
         const int64_t r = i / vectors, c = (i - r * vectors) * kVec<T>;
-        Pack<T, kVec<T>> k;
+        const T* const from = (const T*)copy.from + r * copy.from_stride + c;
+        Loose<T> k;
+        if (c + kVec<T> <= a.width) {
+            k = *reinterpret_cast<const Loose<T>*>(from);
+        } else {
 #pragma unroll
-        for (int e = 0; e < kVec<T>; e++) {
-            k.v[e] = c + e < width ? from[r * from_stride + c + e] : (T)0.0f;
+            for (int e = 0; e < kVec<T>; e++) {
+                k.v[e] = c + e < a.width ? from[e] : (T)0.0f;
+            }
         }
-        *reinterpret_cast<Pack<T, kVec<T>>*>(to + r * to_stride + c) = k;
+        *reinterpret_cast<Pack16*>((T*)copy.to + r * a.padded + c) = __builtin_bit_cast(Pack16, k);
     }
 }
 
 // ------------------------------------------------------------------------------------------- gradients of gate and up
 
 // Values of a thread: kVec columns of one row; zeros outside.
-template <typename T, bool WIDE>
+template <typename T>
 __device__ __forceinline__ void gate_values(const GateGradArgs& a, int64_t row, int64_t c, float (&dg)[kVec<T>],
                                             float (&du)[kVec<T>])
 {
@@ -62,12 +68,7 @@ __device__ __forceinline__ void gate_values(const GateGradArgs& a, int64_t row, 
     }
     float gy[N], gate[N], up[N];
     const auto get = [&](const void* from, int64_t stride, float (&x)[N]) {
-        const T* const at = (const T*)from + row * stride;
-        if (WIDE && c + N <= a.inner) {
-            load<T, N>(at + c, x);
-        } else {
-            load_part<T, N, false>(at, c, a.inner, x);
-        }
+        load_part<T, N, false>((const T*)from + row * stride, c, a.inner, x);
     };
     get(a.grad_y, a.grad_y_stride, gy);
     get(a.gate, a.gate_stride, gate);
@@ -111,7 +112,7 @@ template <typename T>
 constexpr int kColumns = kThreads / 8 * kVec<T>;
 
 // Largest values of rows and columns.  The order of the atomic maxima does not matter.
-template <typename T, bool WIDE>
+template <typename T>
 __global__ __launch_bounds__(kThreads) void gate_most_kernel(GateGradArgs a)
 {
     constexpr int N = kVec<T>;
@@ -127,7 +128,7 @@ __global__ __launch_bounds__(kThreads) void gate_most_kernel(GateGradArgs a)
     for (int i = 0; i < kRows / 8; i++) {
         const int r = i * 8 + (int)threadIdx.x / 32;
         float dg[N], du[N];
-        gate_values<T, WIDE>(a, row0 + r, column0 + c, dg, du);
+        gate_values<T>(a, row0 + r, column0 + c, dg, du);
         uint32_t row = 0;
 #pragma unroll
         for (int e = 0; e < N; e++) {
@@ -166,7 +167,7 @@ __global__ __launch_bounds__(kThreads) void gate_most_kernel(GateGradArgs a)
     }
 }
 
-template <typename T, bool WIDE>
+template <typename T>
 __global__ __launch_bounds__(kThreads) void gate_grad_kernel(GateGradArgs a)
 {
     constexpr int N = kVec<T>;
@@ -195,7 +196,7 @@ __global__ __launch_bounds__(kThreads) void gate_grad_kernel(GateGradArgs a)
     for (int i = 0; i < kRows / 8; i++) {
         const int64_t row = row0 + i * 8 + part;
         float dg[N], du[N], x[N];
-        gate_values<T, WIDE>(a, row, column0 + c, dg, du);
+        gate_values<T>(a, row, column0 + c, dg, du);
         float by_row = 1.0f;
         if (kScaled && row < a.rows) {
             by_row = lift(a.row_most[row]);
@@ -260,47 +261,85 @@ hipError_t run_gate_grad(const GateGradArgs& a, hipStream_t stream)
     if (columns > 65535 || rows > 65535 || a.padded % kVec<T> != 0 || a.padded < a.inner) {
         return hipErrorInvalidValue;
     }
-    const int e = (int)sizeof(T);
-    const bool wide = aligned(a.grad_y, a.grad_y_stride, e, 16) && aligned(a.gate, a.gate_stride, e, 16) &&
-                      aligned(a.up, a.up_stride, e, 16);
     const dim3 grid((unsigned)columns, (unsigned)rows);
     if constexpr (std::is_same_v<T, _Float16>) {
         const int64_t words = a.rows + 2 * a.inner, blocks = (words + kThreads - 1) / kThreads;
         hipLaunchKernelGGL(clear_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(kThreads), 0, stream, a.row_most,
                            words);  // the columns' follow the rows'
-        if (wide) {
-            hipLaunchKernelGGL((gate_most_kernel<T, true>), grid, dim3(kThreads), 0, stream, a);
-        } else {
-            hipLaunchKernelGGL((gate_most_kernel<T, false>), grid, dim3(kThreads), 0, stream, a);
-        }
+        hipLaunchKernelGGL((gate_most_kernel<T>), grid, dim3(kThreads), 0, stream, a);
     }
-    if (wide) {
-        hipLaunchKernelGGL((gate_grad_kernel<T, true>), grid, dim3(kThreads), 0, stream, a);
-    } else {
-        hipLaunchKernelGGL((gate_grad_kernel<T, false>), grid, dim3(kThreads), 0, stream, a);
-    }
+    hipLaunchKernelGGL((gate_grad_kernel<T>), grid, dim3(kThreads), 0, stream, a);
     return hipGetLastError();
 }
+
+// Sums of a vector's parts.
+template <int N>
+__device__ __forceinline__ void join_parts(const float* from, int64_t part, uint32_t parts, int64_t c, int64_t width, float (&x)[N])
+{
+    load_part<float, N, false>(from, c, width, x);
+    for (uint32_t k = 1; k < parts; k++) {
+        float y[N];
+        load_part<float, N, false>(from + k * part, c, width, y);
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            x[e] += y[e];
+        }
+    }
+}
+
+constexpr int kJoin = 4;  // features of a thread
 
 template <typename T>
 __global__ __launch_bounds__(kThreads) void join_kernel(ProductArgs a)
 {
-    const int64_t total = a.tokens * a.features;
+    const int64_t vectors = (a.columns + kJoin - 1) / kJoin, total = a.tokens * vectors;
     for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
-        const int64_t t = i / a.features, f = i - t * a.features;
+        const int64_t t = i / vectors, f = (i - t * vectors) * kJoin;
         const bool second = t >= a.turn;
         const int64_t row = second ? t - a.turn : t;
-        if (row >= a.rows || f >= a.columns) {
+        if (row >= a.rows) {
             continue;
         }
-        float sum = 0.0f;
-        for (int64_t k = 0; k < a.parts; k++) {
-            sum += a.partial[k * total + i];
-        }
+        float x[kJoin];
+        join_parts<kJoin>(a.partial + t * a.features, a.tokens * a.features, a.parts, f, a.features, x);
         if (a.token_scale != nullptr) {
-            sum *= a.token_scale[second ? a.rows + row : row];
+            const float scale = a.token_scale[second ? a.rows + row : row];
+#pragma unroll
+            for (int e = 0; e < kJoin; e++) {
+                x[e] *= scale;
+            }
         }
-        ((T*)a.out[second])[row * a.out_stride[second] + f] = (T)sum;
+        store_part<T, kJoin, false>((T*)a.out[second] + row * a.out_stride[second], f, a.columns, x, false);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_gated_kernel(ProductArgs a)
+{
+    const int64_t vectors = (a.columns + kJoin - 1) / kJoin, total = a.tokens * vectors;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
+        const int64_t t = i / vectors, f = (i - t * vectors) * kJoin;
+        float x[2][kJoin], y[kJoin];
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            join_parts<kJoin>(a.partial + (2 * t + half) * a.features, a.tokens * 2 * a.features, a.parts, f, a.features, x[half]);
+            if (a.bias[half] != nullptr) {
+                load_part<T, kJoin, false>((const T*)a.bias[half], f, a.features, y);
+#pragma unroll
+                for (int e = 0; e < kJoin; e++) {
+                    x[half][e] += y[e];
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < kJoin; e++) {
+            y[e] = activate(x[0][e], a.activation) * x[1][e];
+        }
+        store_part<T, kJoin, false>((T*)a.out[0] + t * a.out_stride[0], f, a.columns, y, false);
+        if (a.out[1] != nullptr) {
+            store_part<T, kJoin, false>((T*)a.out[1] + t * a.out_stride[1], f, a.columns, x[0], false);
+            store_part<T, kJoin, false>((T*)a.out[2] + t * a.out_stride[2], f, a.columns, x[1], false);
+        }
     }
 }
 
@@ -319,19 +358,22 @@ unsigned blocks_of(int64_t items)
 
 }  // namespace
 
-hipError_t launch_pad_rows(Elem e, const void* from, int64_t from_stride, int64_t rows, int64_t width, void* to,
-                           int64_t to_stride, int64_t padded, hipStream_t stream)
+hipError_t launch_pad_rows(Elem e, const PadArgs& a, hipStream_t stream)
 {
+    int64_t rows = 0;
+    for (int i = 0; i < a.count; i++) {
+        rows = a.copy[i].rows > rows ? a.copy[i].rows : rows;
+    }
     if (rows < 1) {
         return hipSuccess;
     }
     return typed(e, [&](auto* t) {
         typedef std::remove_pointer_t<decltype(t)> T;
-        if (padded % kVec<T> != 0 || to_stride % kVec<T> != 0) {
+        if (a.padded % kVec<T> != 0 || a.padded < a.width) {
             return hipErrorInvalidValue;
         }
-        hipLaunchKernelGGL((pad_rows_kernel<T>), dim3(blocks_of(rows * (padded / kVec<T>))), dim3(kThreads), 0, stream,
-                           (const T*)from, from_stride, rows, width, (T*)to, to_stride, padded);
+        hipLaunchKernelGGL((pad_rows_kernel<T>), dim3(blocks_of(rows * (a.padded / kVec<T>)), (unsigned)a.count), dim3(kThreads),
+                           0, stream, a);
         return hipGetLastError();
     });
 }
@@ -344,11 +386,16 @@ hipError_t launch_gate_grad(const GateGradArgs& a, hipStream_t stream)
     return typed((Elem)a.elem, [&](auto* t) { return run_gate_grad<std::remove_pointer_t<decltype(t)>>(a, stream); });
 }
 
-hipError_t launch_join(Elem e, const ProductArgs& a, hipStream_t stream)
+hipError_t launch_join(Elem e, const ProductArgs& a, bool gated, hipStream_t stream)
 {
     return typed(e, [&](auto* t) {
         typedef std::remove_pointer_t<decltype(t)> T;
-        hipLaunchKernelGGL((join_kernel<T>), dim3(blocks_of(a.tokens * a.features)), dim3(kThreads), 0, stream, a);
+        const dim3 grid(blocks_of(a.tokens * ((a.columns + kJoin - 1) / kJoin)));
+        if (gated) {
+            hipLaunchKernelGGL((join_gated_kernel<T>), grid, dim3(kThreads), 0, stream, a);
+        } else {
+            hipLaunchKernelGGL((join_kernel<T>), grid, dim3(kThreads), 0, stream, a);
+        }
         return hipGetLastError();
     });
 }
@@ -357,8 +404,7 @@ hipError_t launch_bias_sums(Elem e, const float* sums, int64_t rows, int64_t inn
 {
     return typed(e, [&](auto* t) {
         typedef std::remove_pointer_t<decltype(t)> T;
-        launch_column_sums<T>(sums, rows, inner, (T*)gate, stream, 2 * inner);
-        launch_column_sums<T>(sums + inner, rows, inner, (T*)up, stream, 2 * inner);
+        launch_column_sums<T>(sums, sums + inner, rows, inner, (T*)gate, (T*)up, stream, 2 * inner);
         return hipGetLastError();
     });
 }

@@ -5,14 +5,14 @@
 namespace opscv {
 namespace prod {
 
-hipError_t launch_products_f32(const ProductArgs& a, bool large, hipStream_t stream)
+hipError_t launch_products_f32(const ProductArgs& a, int tile, hipStream_t stream)
 {
-    return launch_gated_typed<float>(a, large, stream);
+    return launch_gated_typed<float>(a, tile, stream);
 }
 
-hipError_t launch_gradients_f32(const ProductArgs* x, const ProductArgs* weights, bool large, hipStream_t stream)
+hipError_t launch_gradients_f32(const ProductArgs* x, const ProductArgs* weights, int tile, hipStream_t stream)
 {
-    return launch_gradients_typed<float>(x, weights, large, stream);
+    return launch_gradients_typed<float>(x, weights, tile, stream);
 }
 
 }  // namespace prod

@@ -102,18 +102,20 @@ hipError_t launch_few(const ProductArgs& a, hipStream_t stream)
 }
 
 template <typename T>
-hipError_t launch_gated_typed(const ProductArgs& a, bool large, hipStream_t stream)
+hipError_t launch_gated_typed(const ProductArgs& a, int tile, hipStream_t stream)
 {
-    if (a.tokens <= kFewRows) {
-        return a.tokens <= 16 ? launch_few<T, 1, 4>(a, stream) : a.tokens <= 32 ? launch_few<T, 2, 2>(a, stream) : launch_few<T, 4, 1>(a, stream);
+    if (tile == kTileFew) {
+        return a.tokens <= 16   ? launch_few<T, 1, 4>(a, stream)
+               : a.tokens <= 32 ? launch_few<T, 2, 2>(a, stream)
+                                : launch_few<T, 4, 1>(a, stream);
     }
-    return large ? launch_gated_shape<T, LargeGated>(a, stream) : launch_gated_shape<T, Small>(a, stream);
+    return tile == kTile256 ? launch_gated_shape<T, LargeGated>(a, stream) : launch_gated_shape<T, Small>(a, stream);
 }
 
 template <typename T>
-hipError_t launch_gradients_typed(const ProductArgs* x, const ProductArgs* weights, bool large, hipStream_t stream)
+hipError_t launch_gradients_typed(const ProductArgs* x, const ProductArgs* weights, int tile, hipStream_t stream)
 {
-    return large ? launch_gradients_shape<T, Large>(x, weights, stream) : launch_gradients_shape<T, Small>(x, weights, stream);
+    return tile == kTile256 ? launch_gradients_shape<T, Large>(x, weights, stream) : launch_gradients_shape<T, Small>(x, weights, stream);
 }
 
 }  // namespace prod

@@ -2,13 +2,18 @@
 #pragma once
 
 #include <cstdint>
+#include <initializer_list>
 
 #include "token_args.hpp"
 
 namespace opscv {
 namespace prod {
 
-constexpr int64_t kFewRows = 64;  // up to these, gated projections are product_few.hpp's
+constexpr int kTile128 = 0;  // four wavefronts, two workgroups a CU
+constexpr int kTile256 = 1;  // eight wavefronts, one workgroup a CU
+constexpr int kTileFew = 2;  // product_few.hpp: the gated projections of few rows
+
+constexpr int64_t kFewRows = 64;
 
 // One product: rows of its operands in tiles (gated: features of both weights together), stages of 128 bytes of terms.
 struct ProductSize {
@@ -56,51 +61,65 @@ inline int64_t last_end(const int64_t* count, const int64_t* length, int64_t slo
     return last;
 }
 
-// Time of up to two products in one launch, in stages of a large tile on one CU (about a microsecond of 16-bit numbers).  A CU
-// takes one large tile, or two small ones, of a quarter of the work each, at 0.85 of the rate (8192 terms squared bf16: 877 us
-// in large tiles, 1035 in small ones).  Parts, of eight stages at least, so that the workgroups end together: their sums are
-// written and read again, 4 MB a microsecond.  777 rows, 1001 to 2731 FLOAT, both gradients: 247 us with parts of the longer
-// sum alone, sized by the total.
-inline ProductPlan plan_products(const ProductSize* size, int count, bool split, double stage_us, int units)
+// Up to two products in one launch, by the time that each way would take:
+//   - a CU makes a stage of a 256 tile in 1.7 us (8.4 MFLOP of 16 bits at 5 TFLOP/s; FLOAT 8.0), one of a 128 tile in a quarter of
+//     that, 16 bits at 0.85 of the rate (8192 terms squared bf16: 877 us in large tiles, 1035 in small ones; FLOAT 139 and 132
+//     TFLOP/s); alone on a CU not under 1 us, what a stage takes to come from memory, which gives 5 TB/s to all;
+//   - the terms in parts, of four stages at least, so that there is a workgroup for every CU and they end together: the parts'
+//     sums are written and read again, 4 MB a microsecond, by a kernel of 8 us, start and end of it and of the other's among
+//     them.
+// 256 rows, 1024 to 4096 FLOAT: 71 us in one part.  777 rows, 1001 to 2731 FLOAT, both gradients: 247 us where parts were sized
+// by the total alone.
+inline ProductPlan plan_products(const ProductSize* size, int count, int elem_bytes, int units)
 {
     ProductPlan best;
-    double best_cost = 0.0;
-    for (int large = 0; large < 2; large++) {
-        const int64_t side = large != 0 ? 256 : 128, slots = large != 0 ? units : 2 * units;
-        const double each = (large != 0 ? 1.0 : 0.5 / 0.85) * stage_us;
+    for (const int tile : {kTile128, kTile256}) {
+        const int64_t side = tile == kTile256 ? 256 : 128;
+        const double full = elem_bytes == 4 ? 8.0 : 1.7, alone = tile == kTile256 ? full : full / 4.0 / (elem_bytes == 4 ? 1.0 : 0.85);
         int64_t tiles[2] = {0, 0}, most[2] = {1, 1};
+        double from_memory = 0.0;
         for (int i = 0; i < count; i++) {
             tiles[i] = size[i].tiles(side);
-            // four rounds of workgroups at most: after that, parts have nothing to even out
-            most[i] = !split ? 1 : size[i].stages / 8 < 16 ? size[i].stages / 8 : 16;
-            most[i] = most[i] * tiles[i] <= 4 * slots ? most[i] : 4 * slots / tiles[i];
+            from_memory += (double)((size[i].tokens + size[i].features) * size[i].stages * 128) / 5e6;
+            // eight rounds of workgroups at most: after that, parts have nothing to even out
+            most[i] = size[i].stages / 4 < 16 ? size[i].stages / 4 : 16;
+            most[i] = most[i] * tiles[i] <= 8 * units ? most[i] : 8 * units / tiles[i];
             most[i] = most[i] > 1 ? most[i] : 1;
         }
         for (int64_t first = 1; first <= most[0]; first++) {
             for (int64_t second = 1; second <= most[1]; second++) {
                 ProductPlan p;
-                p.large = large != 0;
+                p.tile = tile;
                 const int64_t wanted[2] = {first, second};
                 int64_t groups[2] = {0, 0};
-                double joined = 0.0;
                 for (int i = 0; i < count; i++) {
                     const int64_t stages = size[i].stages > 0 ? size[i].stages : 1;
                     p.part_stages[i] = (stages + wanted[i] - 1) / wanted[i];
                     p.parts[i] = (stages + p.part_stages[i] - 1) / p.part_stages[i];
                     groups[i] = tiles[i] * p.parts[i];
                     if (p.parts[i] > 1) {
-                        joined += 4.0 + (double)(2 * p.parts[i] * size[i].tokens * size[i].features * 4) / 4e6;
+                        p.us += 8.0 + (double)(2 * p.parts[i] * size[i].tokens * size[i].features * 4) / 4e6;
                     }
                 }
-                const double cost = (double)last_end(groups, p.part_stages, slots) * each + joined;
-                if (best_cost == 0.0 || cost < best_cost) {
+                const int64_t share = tile == kTile128 && groups[0] + groups[1] > units ? 2 : 1;  // workgroups of a CU
+                const double stage = (double)share * alone > 1.0 ? (double)share * alone : 1.0;
+                const double last = (double)last_end(groups, p.part_stages, share * units) * stage;
+                p.us += last > from_memory ? last : from_memory;
+                if (best.us == 0.0 || p.us < best.us) {
                     best = p;
-                    best_cost = cost;
                 }
             }
         }
     }
     return best;
+}
+
+// Time of the kernel of few rows: the weights at 5 TB/s, and more for more rows (4096 to 14336 bf16, 1, 8, 16, 32 and 64 rows: 47,
+// 51, 61, 71 and 94 us, where tiles in two parts take 58 with 8 and 62 with 64; FLOAT 96, 105, 118, 129 and 245).
+inline double few_us(int64_t rows, int64_t weight_bytes, int elem_bytes)
+{
+    const double more = elem_bytes == 4 && rows > 32 ? 2.5 : 1.0 + (double)rows / 64.0;
+    return (double)weight_bytes / 5e6 * more;
 }
 
 }  // namespace prod

@@ -45,7 +45,8 @@ struct ProductArgs {
     const float* token_scale = nullptr;  // plain: factor of every token's results, or null
     const void* bias[2] = {nullptr, nullptr};
     int activation = 0;
-    // plain: the terms in parts of `part_stages` stages, whose sums go to `partial`, (parts, tokens, features); or null
+    // the terms in parts of `part_stages` stages, whose sums go to `partial`, (parts, tokens, features), gated: gate's features
+    // and then up's; or null
     float* partial = nullptr;
     uint32_t parts = 1, part_stages = 0;
     uint32_t token_tiles = 0, feature_tiles = 0;  // set by the launcher
@@ -323,14 +324,12 @@ __device__ __forceinline__ TileOf tile_of(const ProductArgs& a, uint32_t block)
     id -= group * run;
     tile.f = id / high;
     tile.t = first + id - tile.f * high;
+    // the same for all lanes: in scalar registers, which the loads' bases have to be in
+    tile.t = (uint32_t)__builtin_amdgcn_readfirstlane((int)tile.t);
+    tile.f = (uint32_t)__builtin_amdgcn_readfirstlane((int)tile.f);
+    tile.part = (uint32_t)__builtin_amdgcn_readfirstlane((int)tile.part);
     return tile;
 }
-
-// A vector to memory on any element's boundary: rows of odd lengths are written as fast as memory takes them.
-template <typename T>
-struct Loose {
-    T v[16 / sizeof(T)];
-};
 
 template <typename T, bool GATED, bool P_TURNED, bool Q_TURNED, typename S>
 __device__ __forceinline__ void product(const ProductArgs& a, uint32_t block, char* lds)
@@ -372,7 +371,7 @@ __device__ __forceinline__ void product(const ProductArgs& a, uint32_t block, ch
     }
     constexpr int kTerms = kRowBytes / kE;
     uint32_t first_stage = 0, stages = (uint32_t)((a.terms + kTerms - 1) / kTerms);
-    if (!GATED && a.parts > 1) {
+    if (a.parts > 1) {
         first_stage = tile.part * a.part_stages;
         const uint32_t left = stages > first_stage ? stages - first_stage : 0;
         stages = left < a.part_stages ? left : a.part_stages;
@@ -415,12 +414,31 @@ __device__ __forceinline__ void product(const ProductArgs& a, uint32_t block, ch
             fq[slot][b] = side_q.read(from + S::kFeatures * kRowBytes, j, b);
         }
     };
+    // Register r of a block is feature 8 (r / 4) + 4 h + r % 4 of token l % 32.  The sums begin with the biases, whose loads are
+    // under way together with the first stages' (10952 rows of 1280 to 3413 fp16: 232 us, added at the end 28 more).
+    const int h = lane >> 5, n = lane & 31;
+    constexpr int kRow = GATED ? FB / 2 : FB;  // blocks of 32 features of the results
     acc_t acc[FB][TB];
 #pragma unroll
     for (int b = 0; b < FB; b++) {
+        acc[b][0] = att::zeros();
+        if constexpr (GATED) {
+            if (a.bias[0] != nullptr && a.partial == nullptr) {
 #pragma unroll
-        for (int c = 0; c < TB; c++) {
-            acc[b][c] = att::zeros();
+                for (int q = 0; q < 4; q++) {
+                    float x[4];
+                    const int64_t f = f0 + (wf * kRow + b / 2) * 32 + 8 * q + 4 * h;
+                    tok::load_part<T, 4, false>((const T*)a.bias[b % 2], f, a.features, x);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        acc[b][0][4 * q + e] = x[e];
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int c = 1; c < TB; c++) {
+            acc[b][c] = acc[b][0];
         }
     }
     const auto multiply = [&](int slot) {
@@ -468,28 +486,43 @@ __device__ __forceinline__ void product(const ProductArgs& a, uint32_t block, ch
 
     // ---------------------------------------------------------------------------------------------- results
     // A wavefront's results go out by way of a place of its own in LDS, 32 tokens at a time, so that neighbouring lanes write
-    // neighbouring vectors of a token.  Register r of a block is feature 8 (r / 4) + 4 h + r % 4 of token l % 32.
-    const int h = lane >> 5, n = lane & 31;
-    const bool partial = !GATED && a.partial != nullptr;
-    if (partial) {
-        float* const to = a.partial + (int64_t)tile.part * a.tokens * a.features;
+    // neighbouring vectors of a token.
+    if (a.partial != nullptr) {
+        const int64_t pitch = GATED ? 2 * a.features : a.features;
+        float* const to = a.partial + (int64_t)tile.part * a.tokens * pitch;
 #pragma unroll
         for (int c = 0; c < TB; c++) {
             const int64_t t = t0 + (wt * TB + c) * 32 + n;
+            if (t >= a.tokens) {
+                continue;
+            }
 #pragma unroll
             for (int b = 0; b < FB; b++) {
+                const int64_t first = f0 + (wf * kRow + (GATED ? b / 2 : b)) * 32;
+                float* const row = to + t * pitch + (GATED && b % 2 != 0 ? a.features : 0);
 #pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int64_t f = f0 + (wf * FB + b) * 32 + 8 * (r / 4) + 4 * h + r % 4;
-                    if (t < a.tokens && f < a.features) {
-                        to[t * a.features + f] = acc[b][c][r];
+                for (int q = 0; q < 4; q++) {
+                    const int64_t f = first + 8 * q + 4 * h;
+                    if (f + 4 <= a.features) {
+                        tok::Loose<float> v;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            v.v[e] = acc[b][c][4 * q + e];
+                        }
+                        *reinterpret_cast<tok::Loose<float>*>(row + f) = v;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            if (f + e < a.features) {
+                                row[f + e] = acc[b][c][4 * q + e];
+                            }
+                        }
                     }
                 }
             }
         }
         return;
     }
-    constexpr int kRow = GATED ? FB / 2 : FB;        // blocks of 32 features that go out together
     constexpr int kPitch = 32 * kRow * kE + 16;      // of a token on its way
     static_assert(S::kWaves * 32 * kPitch <= S::kLds, "the results' way out fits the stages");
     constexpr int kVec = 16 / kE, kChunks = 32 * kRow * kE / 16;  // vectors of a token
@@ -509,9 +542,9 @@ __device__ __forceinline__ void product(const ProductArgs& a, uint32_t block, ch
                 T* const to = (T*)(second ? a.out[1] : a.out[which]) + row * (second ? a.out_stride[1] : a.out_stride[which]) + f +
                               c * kVec;
                 if (left >= kVec) {
-                    *reinterpret_cast<Loose<T>*>(to) = __builtin_bit_cast(Loose<T>, v);
+                    *reinterpret_cast<tok::Loose<T>*>(to) = __builtin_bit_cast(tok::Loose<T>, v);
                 } else {
-                    const Loose<T> each = __builtin_bit_cast(Loose<T>, v);
+                    const tok::Loose<T> each = __builtin_bit_cast(tok::Loose<T>, v);
 #pragma unroll
                     for (int e = 0; e < kVec; e++) {
                         if (e < left) {
@@ -556,19 +589,6 @@ __device__ __forceinline__ void product(const ProductArgs& a, uint32_t block, ch
             put(0, t, f0 + wf * FB * 32);
         } else {
 const int64_t f = f0 + wf * kRow * 32;
-            if (a.bias[0] != nullptr) {
-#pragma unroll
-                for (int b = 0; b < kRow; b++) {
-#pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const int64_t own_f = f + b * 32 + 8 * (r / 4) + 4 * h + r % 4;
-                        if (own_f < a.features) {
-                            acc[2 * b][c][r] += (float)((const T*)a.bias[0])[own_f];
-                            acc[2 * b + 1][c][r] += (float)((const T*)a.bias[1])[own_f];
-                        }
-                    }
-                }
-            }
             const auto hold_all = [&](auto value) {
 #pragma unroll
                 for (int b = 0; b < kRow; b++) {

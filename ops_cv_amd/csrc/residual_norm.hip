@@ -503,7 +503,7 @@ hipError_t run_norm_grad(const NormGradArgs& a, hipStream_t stream)
         }
     }
     if (a.grad_weight != nullptr && !joined) {
-        launch_column_sums<W>(a.partial, partials, a.width, (W*)a.grad_weight, stream);
+        launch_column_sums<W>(a.partial, nullptr, partials, a.width, (W*)a.grad_weight, nullptr, stream);
     }
     return hipGetLastError();
 }

@@ -50,6 +50,12 @@ static __device__ __forceinline__ void store(T* p, const float (&x)[N], bool str
 // get slower by it.)
 constexpr int64_t kStreamBytes = (int64_t)32 << 20;
 
+// A vector on any element's boundary: memory takes it whole, where single elements would be as many instructions.
+template <typename T, int N = 16 / (int)sizeof(T)>
+struct Loose {
+    T v[N];
+};
+
 // Elements c .. c + N - 1 of a row of `width`: whole vectors (WIDE; c + N <= width), or one by one, zeros from the row's
 // end on.  Both ways a lane owns the same elements, so sums over lanes do not depend on a row's alignment.
 template <typename T, int N, bool WIDE>
@@ -57,6 +63,12 @@ static __device__ __forceinline__ void load_part(const T* row, int64_t c, int64_
 {
     if constexpr (WIDE) {
         load<T, N>(row + c, x);
+    } else if (c + N <= width) {
+        const Loose<T, N> k = *reinterpret_cast<const Loose<T, N>*>(row + c);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            x[i] = (float)k.v[i];
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < N; i++) {
@@ -70,6 +82,13 @@ static __device__ __forceinline__ void store_part(T* row, int64_t c, int64_t wid
 {
     if constexpr (WIDE) {
         store<T, N>(row + c, x, streaming);
+    } else if (c + N <= width) {
+        Loose<T, N> k;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            k.v[i] = (T)x[i];
+        }
+        *reinterpret_cast<Loose<T, N>*>(row + c) = k;
     } else {
 #pragma unroll
         for (int i = 0; i < N; i++) {

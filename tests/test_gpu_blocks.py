@@ -359,14 +359,15 @@ def test_gated_gradients(device, aclnn, dtype, rows, width, inner):
     kind = (rows + width + inner) % 3
     want, off = B.gated_grad(gy, x, wg, wu, gate, up, kind, dtype)
     dev = on(device, gy, x, wg, wu, gate, up)
-    got = aclnn.gated_projection_backward(*dev, activation=kind, need_bias=True)
-    for t, w, e, what in zip(got, want, off, ("x", "gate weight", "up weight", "gate bias", "up bias")):
-        close(t, w, e, dtype, "gradient of the " + what)
-    for need_x, need_weights, need_bias in ((True, False, False), (False, True, False), (False, False, True), (True, True, False)):
-        some = aclnn.gated_projection_backward(*dev, activation=kind, need_x=need_x, need_weights=need_weights,
-                                               need_bias=need_bias)
-        assert [t is not None for t in some] == [need_x, need_weights, need_weights, need_bias, need_bias]
-        assert all(s is None or torch.equal(s, t) for s, t in zip(some, got))
+    # which gradients are wanted decides how the sums are split: the bounds hold for any order of them
+    for need_x, need_weights, need_bias in ((True, True, True), (True, False, False), (False, True, False), (False, False, True),
+                                            (True, True, False)):
+        got = aclnn.gated_projection_backward(*dev, activation=kind, need_x=need_x, need_weights=need_weights,
+                                              need_bias=need_bias)
+        assert [t is not None for t in got] == [need_x, need_weights, need_weights, need_bias, need_bias]
+        for t, w, e, what in zip(got, want, off, ("x", "gate weight", "up weight", "gate bias", "up bias")):
+            if t is not None:
+                close(t, w, e, dtype, "gradient of the " + what)
 
 
 @pytest.mark.parametrize("kind", [0, 1, 2])
