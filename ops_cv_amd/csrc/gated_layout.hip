@@ -53,34 +53,52 @@ __global__ __launch_bounds__(kThreads) void pad_rows_kernel(PadArgs a)
 
 // ------------------------------------------------------------------------------------------- gradients of gate and up
 
-// Values of a thread: kVec columns of one row; zeros outside.
+// What a thread reads of a row: kVec columns.
+struct GateRead {
+    Pack16 grad_y, gate, up;
+};
+
 template <typename T>
-__device__ __forceinline__ void gate_values(const GateGradArgs& a, int64_t row, int64_t c, float (&dg)[kVec<T>],
-                                            float (&du)[kVec<T>])
+__device__ __forceinline__ Pack16 read_columns(const T* row, int64_t c, int64_t width)
 {
-    constexpr int N = kVec<T>;
-    if (row >= a.rows || c >= a.inner) {
-#pragma unroll
-        for (int e = 0; e < N; e++) {
-            dg[e] = du[e] = 0.0f;
-        }
-        return;
+    if (c + kVec<T> <= width) {
+        return __builtin_bit_cast(Pack16, *reinterpret_cast<const Loose<T>*>(row + c));
     }
-    float gy[N], gate[N], up[N];
-    const auto get = [&](const void* from, int64_t stride, float (&x)[N]) {
-        load_part<T, N, false>((const T*)from + row * stride, c, a.inner, x);
-    };
-    get(a.grad_y, a.grad_y_stride, gy);
-    get(a.gate, a.gate_stride, gate);
-    get(a.up, a.up_stride, up);
+    Loose<T> k;
 #pragma unroll
-    for (int e = 0; e < N; e++) {
+    for (int e = 0; e < kVec<T>; e++) {
+        k.v[e] = c + e < width ? row[c + e] : (T)0.0f;
+    }
+    return __builtin_bit_cast(Pack16, k);
+}
+
+// Rows past the end are read as the last one, columns past it are zeros.
+template <typename T>
+__device__ __forceinline__ GateRead gate_read(const GateGradArgs& a, int64_t row, int64_t c)
+{
+    const int64_t r = row < a.rows ? row : a.rows - 1;
+    return {read_columns((const T*)a.grad_y + r * a.grad_y_stride, c, a.inner),
+            read_columns((const T*)a.gate + r * a.gate_stride, c, a.inner),
+            read_columns((const T*)a.up + r * a.up_stride, c, a.inner)};
+}
+
+// dGate and dUp of what was read; zeros where `live` is false.
+template <typename T, int KIND>
+__device__ __forceinline__ void gate_values(const GateRead& x, bool live, float (&dg)[kVec<T>], float (&du)[kVec<T>])
+{
+    const Loose<T> grad_y = __builtin_bit_cast(Loose<T>, x.grad_y), gate = __builtin_bit_cast(Loose<T>, x.gate),
+                   up = __builtin_bit_cast(Loose<T>, x.up);
+#pragma unroll
+    for (int e = 0; e < kVec<T>; e++) {
         float value, slope;
-        activate_both(gate[e], a.activation, &value, &slope);
-        dg[e] = c + e < a.inner ? gy[e] * up[e] * slope : 0.0f;
-        du[e] = c + e < a.inner ? gy[e] * value : 0.0f;
+        activate_both((float)gate.v[e], KIND, &value, &slope);
+        const float gy = (float)grad_y.v[e];
+        dg[e] = live ? gy * (float)up.v[e] * slope : 0.0f;
+        du[e] = live ? gy * value : 0.0f;
     }
 }
+
+constexpr int kAhead = 4;  // rows of a thread that are read together
 
 // The power of two that takes `most` (bits of an absolute value) to 2^14..2^15, at most 2^100.
 __device__ __forceinline__ float lift(uint32_t most)
@@ -112,7 +130,7 @@ template <typename T>
 constexpr int kColumns = kThreads / 8 * kVec<T>;
 
 // Largest values of rows and columns.  The order of the atomic maxima does not matter.
-template <typename T>
+template <typename T, int KIND>
 __global__ __launch_bounds__(kThreads) void gate_most_kernel(GateGradArgs a)
 {
     constexpr int N = kVec<T>;
@@ -124,11 +142,18 @@ __global__ __launch_bounds__(kThreads) void gate_most_kernel(GateGradArgs a)
     const int64_t row0 = (int64_t)blockIdx.y * kRows, column0 = (int64_t)blockIdx.x * kColumns<T>;
     const int c = (int)threadIdx.x % 32 * N;
     uint32_t most[2][N] = {{0}};
+    GateRead x[kAhead];
 #pragma unroll
     for (int i = 0; i < kRows / 8; i++) {
+        if (i % kAhead == 0) {
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) {
+                x[k] = gate_read<T>(a, row0 + (i + k) * 8 + (int)threadIdx.x / 32, column0 + c);
+            }
+        }
         const int r = i * 8 + (int)threadIdx.x / 32;
         float dg[N], du[N];
-        gate_values<T>(a, row0 + r, column0 + c, dg, du);
+        gate_values<T, KIND>(x[i % kAhead], row0 + r < a.rows, dg, du);
         uint32_t row = 0;
 #pragma unroll
         for (int e = 0; e < N; e++) {
@@ -167,7 +192,7 @@ __global__ __launch_bounds__(kThreads) void gate_most_kernel(GateGradArgs a)
     }
 }
 
-template <typename T>
+template <typename T, int KIND>
 __global__ __launch_bounds__(kThreads) void gate_grad_kernel(GateGradArgs a)
 {
     constexpr int N = kVec<T>;
@@ -192,11 +217,18 @@ __global__ __launch_bounds__(kThreads) void gate_grad_kernel(GateGradArgs a)
             }
         }
     }
-#pragma unroll 2
+    GateRead read[kAhead];
+#pragma unroll
     for (int i = 0; i < kRows / 8; i++) {
+        if (i % kAhead == 0) {
+#pragma unroll
+            for (int k = 0; k < kAhead; k++) {
+                read[k] = gate_read<T>(a, row0 + (i + k) * 8 + part, column0 + c);
+            }
+        }
         const int64_t row = row0 + i * 8 + part;
         float dg[N], du[N], x[N];
-        gate_values<T>(a, row, column0 + c, dg, du);
+        gate_values<T, KIND>(read[i % kAhead], row < a.rows, dg, du);
         float by_row = 1.0f;
         if (kScaled && row < a.rows) {
             by_row = lift(a.row_most[row]);
@@ -254,7 +286,7 @@ __global__ __launch_bounds__(kThreads) void gate_grad_kernel(GateGradArgs a)
     }
 }
 
-template <typename T>
+template <typename T, int KIND>
 hipError_t run_gate_grad(const GateGradArgs& a, hipStream_t stream)
 {
     const int64_t columns = (a.padded + kColumns<T> - 1) / kColumns<T>, rows = (a.rows + kRows - 1) / kRows;
@@ -266,9 +298,9 @@ hipError_t run_gate_grad(const GateGradArgs& a, hipStream_t stream)
         const int64_t words = a.rows + 2 * a.inner, blocks = (words + kThreads - 1) / kThreads;
         hipLaunchKernelGGL(clear_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(kThreads), 0, stream, a.row_most,
                            words);  // the columns' follow the rows'
-        hipLaunchKernelGGL((gate_most_kernel<T>), grid, dim3(kThreads), 0, stream, a);
+        hipLaunchKernelGGL((gate_most_kernel<T, KIND>), grid, dim3(kThreads), 0, stream, a);
     }
-    hipLaunchKernelGGL((gate_grad_kernel<T>), grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((gate_grad_kernel<T, KIND>), grid, dim3(kThreads), 0, stream, a);
     return hipGetLastError();
 }
 
@@ -383,7 +415,14 @@ hipError_t launch_gate_grad(const GateGradArgs& a, hipStream_t stream)
     if (a.rows < 1) {
         return hipSuccess;
     }
-    return typed((Elem)a.elem, [&](auto* t) { return run_gate_grad<std::remove_pointer_t<decltype(t)>>(a, stream); });
+    return typed((Elem)a.elem, [&](auto* t) {
+        typedef std::remove_pointer_t<decltype(t)> T;
+        switch (a.activation) {
+            case 0: return run_gate_grad<T, 0>(a, stream);
+            case 1: return run_gate_grad<T, 1>(a, stream);
+            default: return run_gate_grad<T, 2>(a, stream);
+        }
+    });
 }
 
 hipError_t launch_join(Elem e, const ProductArgs& a, bool gated, hipStream_t stream)
