@@ -151,34 +151,6 @@ BackwardLayout backward_layout(const GatedArgs& a)
 
 }  // namespace
 
-void plan_gated(GatedArgs* a)
-{
-    const int e = elem_size((Elem)a->elem);
-    const ProductSize size{a->rows, 2 * a->inner, (a->width * e + kRowBytes - 1) / kRowBytes};
-    a->plan = plan_products(&size, 1, e, a->compute_units);
-    if (a->rows <= kFewRows && few_us(a->rows, 2 * a->inner * a->width * e, e) <= a->plan.us) {
-        a->plan = ProductPlan();
-        a->plan.tile = kTileFew;
-    }
-}
-
-void plan_gated_grad(GatedArgs* a)
-{
-    const int e = elem_size((Elem)a->elem);
-    const int64_t padded = rounded(a->inner, kRowBytes / e), width = rounded(a->width, 16 / e);
-    ProductSize size[2];  // of x's gradient and of the weights', those that are wanted
-    int count = 0;
-    if (a->want_x != 0) {
-        size[count++] = {a->rows, width, 2 * padded * e / kRowBytes};
-    }
-    if (a->want_weights != 0) {
-        size[count++] = {2 * padded, width, (a->rows * e + kRowBytes - 1) / kRowBytes};
-    }
-    if (count > 0) {
-        a->plan = plan_products(size, count, e, a->compute_units);
-    }
-}
-
 int64_t gated_scratch_bytes(const GatedArgs& a) { return forward_layout(a).bytes; }
 
 int64_t gated_grad_scratch_bytes(const GatedArgs& a) { return backward_layout(a).bytes; }

@@ -7,7 +7,7 @@
 // rows whose mean is large beside their spread; h stays in 32 bits between the addition and the norm.
 //
 // Bound by memory: every element is read once and written once, so a row stays in registers between its sums and its
-// result.  A row belongs to one wavefront (up to 32 elements a lane), to 256 threads, or to 1024; longer rows are read three
+// result.  A row belongs to one wavefront (up to 16 elements a lane, or 24), to 256 threads, or to 1024; longer rows are read three
 // times.  Sums are 32-bit, over a thread's elements, then over lanes, then over wavefronts, in a fixed order.
 #include <hip/hip_runtime.h>
 
@@ -192,6 +192,11 @@ hipError_t run_layer_norm(const LayerNormArgs& a, hipStream_t stream)
     if (vectors <= 64 * kVectors / 2) {
         hipLaunchKernelGGL((layer_norm_kernel<T, W, 64, kVectors / 2, VEC, WIDE>), grid((a.rows + 3) / 4), dim3(256), 0,
                            stream, a);
+    } else if (sizeof(T) == 2 && vectors <= 64 * 3 && a.rows >= 4096) {
+        // Little more than 1024 elements leave many of 256 threads without any: 10952 rows of 1280 bf16 23 us here and 27
+        // with 256 threads, of 1025 26 and 41.  Rows of 2048, and of floats, are slower here (35 us and 34; 45 and 42), and
+        // 2048 rows of 1280 want the threads (8 us and 11).
+        hipLaunchKernelGGL((layer_norm_kernel<T, W, 64, 3, VEC, WIDE>), grid((a.rows + 3) / 4), dim3(256), 0, stream, a);
     } else if (vectors <= 256 * kVectors / 2) {
         hipLaunchKernelGGL((layer_norm_kernel<T, W, 256, kVectors / 2, VEC, WIDE>), grid(a.rows), dim3(256), 0, stream, a);
     } else if (vectors <= 256 * kVectors) {

@@ -1,6 +1,7 @@
 // Layer norm, dropout and gated projections: parameter validation, planning and the second-phase entries
 // (include/opscv_tokens.h).
 #include "opscv_tokens.h"
+#include "product_plan.hpp"
 #include "token_kernels.hpp"
 #include "token_plan.hpp"
 
@@ -87,6 +88,17 @@ aclnnStatus check_gated(const char* api, const aclTensor* x, const aclTensor* ga
     }
     a->activation = (int)activation;
     a->compute_units = compute_unit_count();
+    return ACLNN_SUCCESS;
+}
+
+// How the products are made, planned before their scratch memory.
+aclnnStatus check_plan(const char* api, const ProductPlan& plan, GatedArgs* a)
+{
+    if (plan.us == 0.0) {
+        return invalid("%s: %lld rows of %lld and %lld features are more workgroups than a launch holds", api, (long long)a->rows,
+                       (long long)a->width, (long long)a->inner);
+    }
+    a->plan = plan;
     return ACLNN_SUCCESS;
 }
 
@@ -382,6 +394,7 @@ aclnnStatus opscvGatedProjectionGetWorkspaceSize(const aclTensor* x, const aclTe
         return finish(api, ex, workspaceSize, executor);
     }
     ex->kind = OpKind::Gated;
+    OPSCV_CHECK(check_plan(api, prod::gated_plan(a), &a));
     const int bytes = elem_size((Elem)a.elem);
     plan_operand(ex.get(), kGaX, x, bytes, false, &a.x);
     plan_operand(ex.get(), kGaGateWeight, gateWeight, bytes, false, &a.gate_weight);
@@ -395,7 +408,6 @@ aclnnStatus opscvGatedProjectionGetWorkspaceSize(const aclTensor* x, const aclTe
         plan_rows(ex.get(), kGaGate, gate, bytes, true, &a.gate);
         plan_rows(ex.get(), kGaUp, up, bytes, true, &a.up);
     }
-    plan_gated(&a);
     plan_bytes(ex.get(), kGaScratch, gated_scratch_bytes(a));
     return finish(api, ex, workspaceSize, executor);
 }
@@ -445,6 +457,9 @@ aclnnStatus opscvGatedProjectionBackwardGetWorkspaceSize(const aclTensor* gradY,
     a.want_x = gradX != nullptr && a.rows > 0 ? 1 : 0;
     a.want_weights = gradGateWeight != nullptr ? 1 : 0;
     a.want_biases = gradGateBias != nullptr ? 1 : 0;
+    if (a.want_x != 0 || a.want_weights != 0) {
+        OPSCV_CHECK(check_plan(api, prod::gated_grad_plan(a), &a));
+    }
     const int bytes = elem_size((Elem)a.elem);
     plan_rows(ex.get(), kGgY, gradY, bytes, false, &a.grad_y);
     if (a.want_weights != 0) {
@@ -467,7 +482,6 @@ aclnnStatus opscvGatedProjectionBackwardGetWorkspaceSize(const aclTensor* gradY,
         plan_dense(ex.get(), kGgGradGateBias, gradGateBias, bytes, true);
         plan_dense(ex.get(), kGgGradUpBias, gradUpBias, bytes, true);
     }
-    plan_gated_grad(&a);
     plan_bytes(ex.get(), kGgScratch, gated_grad_scratch_bytes(a));
     return finish(api, ex, workspaceSize, executor);
 }

@@ -25,7 +25,7 @@ int64_t prepare(ProductArgs* a)
     // vectors of 16 bytes are whole: of terms, or of turned features and tokens, which a row has room for
     fits = fits && ((P_TURNED && Q_TURNED) || a->terms % kVec == 0);
     fits = fits && (!P_TURNED || (a->features % kVec == 0 && a->p_turn % kTerms == 0));
-    fits = fits && (!Q_TURNED || a->tokens % kVec == 0);
+    fits = fits && (!Q_TURNED || a->tokens % kVec == 0) && (a->turn % 32 == 0 || a->turn > a->tokens);
     for (const int64_t stride : {a->p_stride[0], a->p_stride[1], a->q_stride}) {
         fits = fits && stride >= 0 && stride * kE % 16 == 0;
     }

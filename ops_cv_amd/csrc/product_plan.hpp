@@ -4,6 +4,8 @@
 #include <cstdint>
 #include <initializer_list>
 
+#include "acl_types.hpp"
+#include "launch_limits.hpp"
 #include "token_args.hpp"
 
 namespace opscv {
@@ -14,6 +16,8 @@ constexpr int kTile256 = 1;  // eight wavefronts, one workgroup a CU
 constexpr int kTileFew = 2;  // product_few.hpp: the gated projections of few rows
 
 constexpr int64_t kFewRows = 64;
+
+constexpr int kRowBytes = 128;  // of a row in a stage: eight vectors of 16 bytes
 
 // One product: rows of its operands in tiles (gated: features of both weights together), stages of 128 bytes of terms.
 struct ProductSize {
@@ -70,6 +74,7 @@ inline int64_t last_end(const int64_t* count, const int64_t* length, int64_t slo
 //     them.
 // 256 rows, 1024 to 4096 FLOAT: 71 us in one part.  777 rows, 1001 to 2731 FLOAT, both gradients: 247 us where parts were sized
 // by the total alone.
+// `us` is 0 where no way fits a launch.
 inline ProductPlan plan_products(const ProductSize* size, int count, int elem_bytes, int units)
 {
     ProductPlan best;
@@ -101,6 +106,9 @@ inline ProductPlan plan_products(const ProductSize* size, int count, int elem_by
                         p.us += 8.0 + (double)(2 * p.parts[i] * size[i].tokens * size[i].features * 4) / 4e6;
                     }
                 }
+                if (!fits_launch(groups[0] + groups[1], tile == kTile128 ? 256 : 512)) {
+                    continue;
+                }
                 const int64_t share = tile == kTile128 && groups[0] + groups[1] > units ? 2 : 1;  // workgroups of a CU
                 const double stage = (double)share * alone > 1.0 ? (double)share * alone : 1.0;
                 const double last = (double)last_end(groups, p.part_stages, share * units) * stage;
@@ -120,6 +128,38 @@ inline double few_us(int64_t rows, int64_t weight_bytes, int elem_bytes)
 {
     const double more = elem_bytes == 4 && rows > 32 ? 2.5 : 1.0 + (double)rows / 64.0;
     return (double)weight_bytes / 5e6 * more;
+}
+
+// The forward product of the gated projections, y's features in both weights; `us` is 0 where none fits a launch.
+inline ProductPlan gated_plan(const GatedArgs& a)
+{
+    const int e = elem_size((Elem)a.elem);
+    const ProductSize size{a.rows, 2 * a.inner, (a.width * e + kRowBytes - 1) / kRowBytes};
+    ProductPlan p = plan_products(&size, 1, e, a.compute_units);
+    const double few = few_us(a.rows, 2 * a.inner * a.width * e, e);
+    if (a.rows <= kFewRows && (p.us == 0.0 || few <= p.us)) {
+        p = ProductPlan();
+        p.tile = kTileFew;
+        p.us = few;
+    }
+    return p;
+}
+
+// The products of their gradients that are wanted, one at least: x's, then the weights'.
+inline ProductPlan gated_grad_plan(const GatedArgs& a)
+{
+    const int e = elem_size((Elem)a.elem);
+    const auto rounded = [](int64_t n, int64_t to) { return (n + to - 1) / to * to; };
+    const int64_t padded = rounded(a.inner, kRowBytes / e), width = rounded(a.width, 16 / e);
+    ProductSize size[2];
+    int count = 0;
+    if (a.want_x != 0) {
+        size[count++] = {a.rows, width, 2 * padded * e / kRowBytes};
+    }
+    if (a.want_weights != 0) {
+        size[count++] = {2 * padded, width, (a.rows * e + kRowBytes - 1) / kRowBytes};
+    }
+    return plan_products(size, count, e, a.compute_units);
 }
 
 }  // namespace prod

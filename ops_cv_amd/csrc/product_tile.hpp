@@ -20,6 +20,7 @@
 
 #include "acl_types.hpp"
 #include "attention_tile.hpp"
+#include "product_plan.hpp"
 #include "token_elem.hpp"
 
 namespace opscv {
@@ -41,7 +42,7 @@ struct ProductArgs {
     // gated: y, gate and up
     void* out[3] = {nullptr, nullptr, nullptr};
     int64_t out_stride[3] = {0, 0, 0};
-    int64_t turn = INT64_MAX, rows = 0;
+    int64_t turn = INT64_MAX, rows = 0;  // turn: a multiple of 32
     const float* token_scale = nullptr;  // plain: factor of every token's results, or null
     const void* bias[2] = {nullptr, nullptr};
     int activation = 0;
@@ -163,7 +164,6 @@ struct alignas(16) Pack16 {
     uint32_t v[4];
 };
 
-constexpr int kRowBytes = 128;  // of a row in a stage: eight vectors of 16 bytes
 constexpr uint32_t kInside = 0x80000000u;  // size of the descriptors: offsets of rows and terms that are there stay below it
 
 // Vector c of row r lies at place c ^ swizzle(r), so that 16 neighbouring rows' vectors of one number fall on the 16 places of
@@ -528,31 +528,33 @@ __device__ __forceinline__ void product(const ProductArgs& a, uint32_t block, ch
     constexpr int kVec = 16 / kE, kChunks = 32 * kRow * kE / 16;  // vectors of a token
     __syncthreads();  // all have read their last stage
     char* const place = lds + wave * 32 * kPitch;
-    // Writes out what lies there: tokens t.. , features f..
+    // Writes out what lies there: tokens t.. , features f..  The 32 tokens are on one side of `turn`, a multiple of 32.
+    const int put_token = lane / kChunks, put_vector = lane % kChunks;
     const auto put = [&](int which, int64_t t, int64_t f) {
         __asm__ volatile("" ::: "memory");  // the compiler keeps the order; LDS does for one wavefront
+        const bool second = !GATED && t >= a.turn;
+        const int64_t row = second ? t - a.turn : t, stride = second ? a.out_stride[1] : a.out_stride[which];
+        T* to = (T*)(second ? a.out[1] : a.out[which]) + row * stride + f + (int64_t)put_token * stride + put_vector * kVec;
+        const int left = (int)(a.rows - row < 32 ? a.rows - row : 32);
+        const int64_t columns = a.columns - f - put_vector * kVec;
 #pragma unroll
         for (int i = 0; i < 32 * kChunks / 64; i++) {
-            const int token = (i * 64 + lane) / kChunks, c = (i * 64 + lane) % kChunks;
-            const Pack16 v = *reinterpret_cast<const Pack16*>(place + token * kPitch + c * 16);
-            const bool second = !GATED && t + token >= a.turn;
-            const int64_t row = second ? t + token - a.turn : t + token;
-            const int64_t left = a.columns - (f + c * kVec);
-            if (row < a.rows && left > 0) {
-                T* const to = (T*)(second ? a.out[1] : a.out[which]) + row * (second ? a.out_stride[1] : a.out_stride[which]) + f +
-                              c * kVec;
-                if (left >= kVec) {
+            constexpr int kTokens = 64 / kChunks;  // of an instruction
+            const Pack16 v = *reinterpret_cast<const Pack16*>(place + (put_token + i * kTokens) * kPitch + put_vector * 16);
+            if (put_token + i * kTokens < left) {
+                if (columns >= kVec) {
                     *reinterpret_cast<tok::Loose<T>*>(to) = __builtin_bit_cast(tok::Loose<T>, v);
                 } else {
                     const tok::Loose<T> each = __builtin_bit_cast(tok::Loose<T>, v);
 #pragma unroll
                     for (int e = 0; e < kVec; e++) {
-                        if (e < left) {
+                        if (e < columns) {
                             to[e] = each.v[e];
                         }
                     }
                 }
             }
+            to += kTokens * stride;
         }
         __asm__ volatile("" ::: "memory");
     };

@@ -107,7 +107,7 @@ struct GatedArgs {
     void* grad_gate_bias = nullptr;        // both or neither
     void* grad_up_bias = nullptr;
     int want_x = 0, want_weights = 0, want_biases = 0;
-    ProductPlan plan;  // by plan_gated() / plan_gated_grad()
+    ProductPlan plan;  // by gated_plan() / gated_grad_plan()
     char* scratch = nullptr;  // gated_scratch_bytes() / gated_grad_scratch_bytes()
 };
 

@@ -27,9 +27,6 @@ int64_t layer_norm_grad_partials(const LayerNormGradArgs& a);
 hipError_t launch_dropout(const DropoutArgs& a, hipStream_t stream);
 hipError_t launch_gated(const GatedArgs& a, hipStream_t stream);
 hipError_t launch_gated_grad(const GatedArgs& a, hipStream_t stream);
-// how the products are made: before the scratch memory is asked for
-void plan_gated(GatedArgs* a);
-void plan_gated_grad(GatedArgs* a);
 // bytes of GatedArgs::scratch.  The addresses of the operands that are used in place have to be set; those of packed ones are
 // on 256 bytes (null stands for one).
 int64_t gated_scratch_bytes(const GatedArgs& a);

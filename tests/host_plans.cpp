@@ -5,6 +5,7 @@
 #include "gs2d_grad_grid_plan.hpp"
 #include "gs_grad_gather_plan.hpp"
 #include "gs_grad_tiles_plan.hpp"
+#include "product_plan.hpp"
 #include "resize_flat_plan.hpp"
 #include "resize_grad_plan.hpp"
 #include "resize_nearest_plan.hpp"
@@ -246,6 +247,48 @@ int64_t nearest_rows_nanoseconds(int elem, int64_t N, int64_t C, int64_t Hs, int
         least = t < least ? t : least;
     }
     return least;
+}
+
+// How the gated projections are made: kind 0 forward, else 1 for x's gradient plus 2 for the weights'
+int gated_plan(int elem, int64_t kind, int64_t rows, int64_t width, int64_t inner, int64_t units, int64_t* out)
+{
+    GatedArgs a;
+    a.elem = elem;
+    a.rows = rows;
+    a.width = width;
+    a.inner = inner;
+    a.compute_units = (int)units;
+    a.want_x = (int)(kind & 1);
+    a.want_weights = (int)(kind >> 1 & 1);
+    const ProductPlan p = kind == 0 ? prod::gated_plan(a) : prod::gated_grad_plan(a);
+    out[0] = p.tile;
+    for (int i = 0; i < 2; i++) {
+        out[1 + i] = p.parts[i];
+        out[3 + i] = p.part_stages[i];
+    }
+    out[5] = (int64_t)(p.us * 1000.0);
+    return p.us > 0.0 ? 1 : 0;
+}
+
+// nanoseconds that it takes, the least of ten runs of ten
+int64_t gated_plan_nanoseconds(int elem, int64_t kind, int64_t rows, int64_t width, int64_t inner, int64_t units)
+{
+    int64_t least = INT64_MAX, out[6];
+    for (int run = 0; run < 10; run++) {
+        const auto start = std::chrono::steady_clock::now();
+        for (int i = 0; i < 10; i++) {
+            gated_plan(elem, kind, rows, width, inner, units, out);
+        }
+        const int64_t t = std::chrono::duration_cast<std::chrono::nanoseconds>(std::chrono::steady_clock::now() - start).count() / 10;
+        least = t < least ? t : least;
+    }
+    return least;
+}
+
+int64_t product_last_end(int64_t count0, int64_t length0, int64_t count1, int64_t length1, int64_t slots)
+{
+    const int64_t count[2] = {count0, count1}, length[2] = {length0, length1};
+    return prod::last_end(count, length, slots);
 }
 
 }  // extern "C"

@@ -112,3 +112,23 @@ def nearest_rows_nanoseconds(dtype, shape, out, channels_last=False):
     plan = lib().nearest_rows_nanoseconds
     plan.restype = ctypes.c_int64
     return plan(ctypes.c_int(ELEM[dtype]), *[ctypes.c_int64(v) for v in (*shape, *out, int(channels_last))])
+
+
+def gated_plan(dtype, kind, rows, width, inner, units=256):
+    """(tile, parts of both products, stages of their parts, nanoseconds expected) of a gated projection, None where it fits no
+    launch; kind 0 is the forward pass, else 1 for x's gradient plus 2 for the weights'.  Tiles: 0 of 128, 1 of 256, 2 few."""
+    return _call("gated_plan", 6, dtype, kind, rows, width, inner, units)
+
+
+def gated_plan_nanoseconds(dtype, kind, rows, width, inner, units=256):
+    """Host time of that plan."""
+    plan = lib().gated_plan_nanoseconds
+    plan.restype = ctypes.c_int64
+    return plan(ctypes.c_int(ELEM[dtype]), *[ctypes.c_int64(v) for v in (kind, rows, width, inner, units)])
+
+
+def product_last_end(counts, lengths, slots):
+    """When the last of counts[0] workgroups of lengths[0], then counts[1] of lengths[1], ends."""
+    f = lib().product_last_end
+    f.restype = ctypes.c_int64
+    return f(*[ctypes.c_int64(v) for v in (counts[0], lengths[0], counts[1], lengths[1], slots)])

@@ -31,8 +31,8 @@ def on(device, *tensors):
 
 # -------------------------------------------------------------------------------------------------------- layer norm
 
-NORM_SIZES = [(1, 1), (3, 5), (4, 64), (7, 100), (2, 768), (130, 1024), (5, 1001), (3, 2056), (2, 4096), (3, 8192), (2, 9001),
-              (2, 40000), (2, 33001)]
+NORM_SIZES = [(1, 1), (3, 5), (4, 64), (7, 100), (2, 768), (130, 1024), (5, 1001), (4100, 1040), (4099, 1301), (3, 2056),
+              (2, 4096), (3, 8192), (2, 9001), (2, 40000), (2, 33001)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
