@@ -98,6 +98,18 @@ struct BackwardLayout {
     int64_t bytes = 0;
 };
 
+int64_t gate_rows_of(const GatedArgs& a, int64_t padded)
+{
+    return gate_rows(a.rows, padded, elem_size((Elem)a.elem), a.compute_units);
+}
+
+// rows of the biases' partial sums
+int64_t sum_rows(const GatedArgs& a, int64_t padded)
+{
+    const int64_t each = gate_rows_of(a, padded);
+    return (a.rows + each - 1) / each;
+}
+
 BackwardLayout backward_layout(const GatedArgs& a)
 {
     const int e = elem_size((Elem)a.elem);
@@ -131,7 +143,7 @@ BackwardLayout backward_layout(const GatedArgs& a)
         l.factors = s.take((a.rows + 2 * a.inner) * 4);
     }
     if (a.want_biases != 0) {
-        l.sums = s.take((a.rows + kGateRows - 1) / kGateRows * 2 * a.inner * 4);
+        l.sums = s.take(sum_rows(a, l.padded) * 2 * a.inner * 4);
     }
     const int64_t parts_x = a.plan.parts[0], parts_weights = a.plan.parts[want_x ? 1 : 0];
     if (want_x && parts_x > 1) {
@@ -215,6 +227,7 @@ hipError_t launch_gated_grad(const GatedArgs& a, hipStream_t stream)
     g.by_rows = at(l.by_rows);
     g.by_columns = at(l.by_columns);
     g.padded = l.padded;
+    g.rows_each = gate_rows_of(a, l.padded);
     g.sums = (float*)at(l.sums);
     if (l.most >= 0) {
         g.row_most = (uint32_t*)at(l.most);
@@ -286,7 +299,7 @@ hipError_t launch_gated_grad(const GatedArgs& a, hipStream_t stream)
         OPSCV_LAUNCH(launch_join(elem, weights, false, stream));
     }
     if (a.want_biases != 0) {
-        OPSCV_LAUNCH(launch_bias_sums(elem, g.sums, (a.rows + kGateRows - 1) / kGateRows, a.inner, a.grad_gate_bias,
+        OPSCV_LAUNCH(launch_bias_sums(elem, g.sums, sum_rows(a, l.padded), a.inner, a.grad_gate_bias,
                                       a.grad_up_bias, stream));
     }
     return hipSuccess;

@@ -42,13 +42,26 @@ struct GateGradArgs {
     // FLOAT16: the same in the scale of each column.  May be null.
     void* by_columns = nullptr;
     int64_t padded = 0;
-    // sums over the rows of each tile of kGateRows rows: (tiles, 2 inner); may be null
+    int64_t rows_each = 0;  // of a workgroup: gate_rows()
+    // sums over the rows of each workgroup: (rows / rows_each, 2 inner); may be null
     float* sums = nullptr;
     // FLOAT16: largest absolute values as bits, by rows and by columns (2 inner), and the factors that undo the scales
     uint32_t *row_most = nullptr, *column_most = nullptr;
     float *row_factor = nullptr, *column_factor = nullptr;
 };
 constexpr int kGateRows = 64;
+
+// Rows of a workgroup of them: kGateRows, or fewer while that leaves less than four workgroups to a CU (1355 rows of 1792 bf16: 18
+// us with 64, their arithmetic done by one wavefront a SIMD).
+inline int64_t gate_rows(int64_t rows, int64_t padded, int elem_bytes, int compute_units)
+{
+    const int64_t columns = (padded * elem_bytes + 511) / 512;  // workgroups of a row: 32 vectors each
+    int64_t each = kGateRows;
+    while (each > 8 && columns * ((rows + each - 1) / each) < (int64_t)4 * compute_units) {
+        each /= 2;
+    }
+    return each;
+}
 
 hipError_t launch_gate_grad(const GateGradArgs& a, hipStream_t stream);
 

@@ -72,11 +72,11 @@ __device__ __forceinline__ Pack16 read_columns(const T* row, int64_t c, int64_t 
     return __builtin_bit_cast(Pack16, k);
 }
 
-// Rows past the end are read as the last one, columns past it are zeros.
+// Rows from `end` on are read as the last one, columns past the end are zeros.
 template <typename T>
-__device__ __forceinline__ GateRead gate_read(const GateGradArgs& a, int64_t row, int64_t c)
+__device__ __forceinline__ GateRead gate_read(const GateGradArgs& a, int64_t row, int64_t end, int64_t c)
 {
-    const int64_t r = row < a.rows ? row : a.rows - 1;
+    const int64_t r = row < end ? row : end - 1;
     return {read_columns((const T*)a.grad_y + r * a.grad_y_stride, c, a.inner),
             read_columns((const T*)a.gate + r * a.gate_stride, c, a.inner),
             read_columns((const T*)a.up + r * a.up_stride, c, a.inner)};
@@ -125,12 +125,14 @@ __device__ __forceinline__ uint32_t size_of(float x)
     return u < 0x7F800000u ? u : 0u;
 }
 
-// A workgroup's part: kRows rows of kThreads / 8 vectors; a thread's vectors are those of every eighth row.
+// A workgroup's part: rows_each rows (kRows at most) of kThreads / 8 vectors; a thread's vectors are those of every eighth row.
+// SHORT: rows_each is less than kRows, or there are no more rows, and the loops end where the rows do.  Those ends keep the
+// compiler from moving the loads of the next rows up: 4096 rows of 8192 bf16, 56 us without them and 62 with.
 template <typename T>
 constexpr int kColumns = kThreads / 8 * kVec<T>;
 
 // Largest values of rows and columns.  The order of the atomic maxima does not matter.
-template <typename T, int KIND>
+template <typename T, int KIND, bool SHORT>
 __global__ __launch_bounds__(kThreads) void gate_most_kernel(GateGradArgs a)
 {
     constexpr int N = kVec<T>;
@@ -139,21 +141,27 @@ __global__ __launch_bounds__(kThreads) void gate_most_kernel(GateGradArgs a)
         (i < kRows ? rows[i] : columns[(i - kRows) / kColumns<T>][(i - kRows) % kColumns<T>]) = 0;
     }
     __syncthreads();
-    const int64_t row0 = (int64_t)blockIdx.y * kRows, column0 = (int64_t)blockIdx.x * kColumns<T>;
+    const int64_t row0 = (int64_t)blockIdx.y * a.rows_each, column0 = (int64_t)blockIdx.x * kColumns<T>;
+    const int64_t end = row0 + a.rows_each < a.rows ? row0 + a.rows_each : a.rows;
     const int c = (int)threadIdx.x % 32 * N;
     uint32_t most[2][N] = {{0}};
     GateRead x[kAhead];
 #pragma unroll
     for (int i = 0; i < kRows / 8; i++) {
+        if (SHORT && row0 + i * 8 >= end) {
+            break;
+        }
         if (i % kAhead == 0) {
 #pragma unroll
             for (int k = 0; k < kAhead; k++) {
-                x[k] = gate_read<T>(a, row0 + (i + k) * 8 + (int)threadIdx.x / 32, column0 + c);
+                if (!SHORT || row0 + (i + k) * 8 < end) {
+                    x[k] = gate_read<T>(a, row0 + (i + k) * 8 + (int)threadIdx.x / 32, end, column0 + c);
+                }
             }
         }
         const int r = i * 8 + (int)threadIdx.x / 32;
         float dg[N], du[N];
-        gate_values<T, KIND>(x[i % kAhead], row0 + r < a.rows, dg, du);
+        gate_values<T, KIND>(x[i % kAhead], row0 + r < end, dg, du);
         uint32_t row = 0;
 #pragma unroll
         for (int e = 0; e < N; e++) {
@@ -180,7 +188,7 @@ __global__ __launch_bounds__(kThreads) void gate_most_kernel(GateGradArgs a)
     __syncthreads();
     for (int i = (int)threadIdx.x; i < kRows + 2 * kColumns<T>; i += kThreads) {
         if (i < kRows) {
-            if (row0 + i < a.rows) {
+            if (row0 + i < end) {
                 atomicMax(&a.row_most[row0 + i], rows[i]);
             }
         } else {
@@ -192,13 +200,14 @@ __global__ __launch_bounds__(kThreads) void gate_most_kernel(GateGradArgs a)
     }
 }
 
-template <typename T, int KIND>
+template <typename T, int KIND, bool SHORT>
 __global__ __launch_bounds__(kThreads) void gate_grad_kernel(GateGradArgs a)
 {
     constexpr int N = kVec<T>;
     constexpr bool kScaled = std::is_same_v<T, _Float16>;
     __shared__ float sums[2][8][kColumns<T>];
-    const int64_t row0 = (int64_t)blockIdx.y * kRows, column0 = (int64_t)blockIdx.x * kColumns<T>;
+    const int64_t row0 = (int64_t)blockIdx.y * a.rows_each, column0 = (int64_t)blockIdx.x * kColumns<T>;
+    const int64_t end = row0 + a.rows_each < a.rows ? row0 + a.rows_each : a.rows;
     const int c = (int)threadIdx.x % 32 * N, part = (int)threadIdx.x / 32;
     float by_column[2][kScaled ? N : 1], total[2][N];
 #pragma unroll
@@ -220,17 +229,22 @@ __global__ __launch_bounds__(kThreads) void gate_grad_kernel(GateGradArgs a)
     GateRead read[kAhead];
 #pragma unroll
     for (int i = 0; i < kRows / 8; i++) {
+        if (SHORT && row0 + i * 8 >= end) {
+            break;
+        }
         if (i % kAhead == 0) {
 #pragma unroll
             for (int k = 0; k < kAhead; k++) {
-                read[k] = gate_read<T>(a, row0 + (i + k) * 8 + part, column0 + c);
+                if (!SHORT || row0 + (i + k) * 8 < end) {
+                    read[k] = gate_read<T>(a, row0 + (i + k) * 8 + part, end, column0 + c);
+                }
             }
         }
         const int64_t row = row0 + i * 8 + part;
         float dg[N], du[N], x[N];
-        gate_values<T, KIND>(read[i % kAhead], row < a.rows, dg, du);
+        gate_values<T, KIND>(read[i % kAhead], row < end, dg, du);
         float by_row = 1.0f;
-        if (kScaled && row < a.rows) {
+        if (kScaled && row < end) {
             by_row = lift(a.row_most[row]);
             if (blockIdx.x == 0 && c == 0) {
                 a.row_factor[row] = 1.0f / by_row;
@@ -241,7 +255,7 @@ __global__ __launch_bounds__(kThreads) void gate_grad_kernel(GateGradArgs a)
             total[0][e] += dg[e];
             total[1][e] += du[e];
         }
-        if (row < a.rows && column0 + c < a.padded) {
+        if (row < end && column0 + c < a.padded) {
             const int64_t at = row * 2 * a.padded + column0 + c;
 #pragma unroll
             for (int half = 0; half < 2; half++) {
@@ -286,11 +300,14 @@ __global__ __launch_bounds__(kThreads) void gate_grad_kernel(GateGradArgs a)
     }
 }
 
-template <typename T, int KIND>
+template <typename T, int KIND, bool SHORT>
 hipError_t run_gate_grad(const GateGradArgs& a, hipStream_t stream)
 {
-    const int64_t columns = (a.padded + kColumns<T> - 1) / kColumns<T>, rows = (a.rows + kRows - 1) / kRows;
-    if (columns > 65535 || rows > 65535 || a.padded % kVec<T> != 0 || a.padded < a.inner) {
+    if (a.rows_each < 8 || a.rows_each > kRows || a.rows_each % 8 != 0 || a.padded % kVec<T> != 0 || a.padded < a.inner) {
+        return hipErrorInvalidValue;
+    }
+    const int64_t columns = (a.padded + kColumns<T> - 1) / kColumns<T>, rows = (a.rows + a.rows_each - 1) / a.rows_each;
+    if (columns > 65535 || rows > 65535) {
         return hipErrorInvalidValue;
     }
     const dim3 grid((unsigned)columns, (unsigned)rows);
@@ -298,23 +315,33 @@ hipError_t run_gate_grad(const GateGradArgs& a, hipStream_t stream)
         const int64_t words = a.rows + 2 * a.inner, blocks = (words + kThreads - 1) / kThreads;
         hipLaunchKernelGGL(clear_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(kThreads), 0, stream, a.row_most,
                            words);  // the columns' follow the rows'
-        hipLaunchKernelGGL((gate_most_kernel<T, KIND>), grid, dim3(kThreads), 0, stream, a);
+        hipLaunchKernelGGL((gate_most_kernel<T, KIND, SHORT>), grid, dim3(kThreads), 0, stream, a);
     }
-    hipLaunchKernelGGL((gate_grad_kernel<T, KIND>), grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((gate_grad_kernel<T, KIND, SHORT>), grid, dim3(kThreads), 0, stream, a);
     return hipGetLastError();
 }
 
-// Sums of a vector's parts.
+// Sums of a vector's parts, in order; four are read together (7 rows of 1191, 15 parts: 6.5 us one by one).
 template <int N>
 __device__ __forceinline__ void join_parts(const float* from, int64_t part, uint32_t parts, int64_t c, int64_t width, float (&x)[N])
 {
+    constexpr uint32_t kTogether = 4;
     load_part<float, N, false>(from, c, width, x);
-    for (uint32_t k = 1; k < parts; k++) {
-        float y[N];
-        load_part<float, N, false>(from + k * part, c, width, y);
+    for (uint32_t k = 1; k < parts; k += kTogether) {
+        float y[kTogether][N];
 #pragma unroll
-        for (int e = 0; e < N; e++) {
-            x[e] += y[e];
+        for (uint32_t j = 0; j < kTogether; j++) {
+            // parts past the last one are read as it, and left out
+            load_part<float, N, false>(from + (k + j < parts ? k + j : parts - 1) * part, c, width, y[j]);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kTogether; j++) {
+            if (k + j < parts) {
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    x[e] += y[j][e];
+                }
+            }
         }
     }
 }
@@ -417,10 +444,11 @@ hipError_t launch_gate_grad(const GateGradArgs& a, hipStream_t stream)
     }
     return typed((Elem)a.elem, [&](auto* t) {
         typedef std::remove_pointer_t<decltype(t)> T;
+        const bool few = a.rows_each < kRows || a.rows < kRows;
         switch (a.activation) {
-            case 0: return run_gate_grad<T, 0>(a, stream);
-            case 1: return run_gate_grad<T, 1>(a, stream);
-            default: return run_gate_grad<T, 2>(a, stream);
+            case 0: return few ? run_gate_grad<T, 0, true>(a, stream) : run_gate_grad<T, 0, false>(a, stream);
+            case 1: return few ? run_gate_grad<T, 1, true>(a, stream) : run_gate_grad<T, 1, false>(a, stream);
+            default: return few ? run_gate_grad<T, 2, true>(a, stream) : run_gate_grad<T, 2, false>(a, stream);
         }
     });
 }

@@ -41,19 +41,20 @@ int64_t prepare(ProductArgs* a)
     return blocks;
 }
 
-template <typename S, typename... A>
-hipError_t launch_kernel(void (*kernel)(A...), int64_t blocks, hipStream_t stream, std::atomic<uint32_t>& allowed, A... args)
+template <typename... A>
+hipError_t launch_kernel(void (*kernel)(A...), int64_t blocks, int threads, int lds, hipStream_t stream,
+                         std::atomic<uint32_t>& allowed, A... args)
 {
-    if (!fits_launch(blocks, S::kThreads)) {
+    if (!fits_launch(blocks, threads)) {
         return hipErrorInvalidValue;
     }
-    if (S::kLds > 65536) {
-        const hipError_t e = allow_dynamic_lds((const void*)kernel, S::kLds, allowed);
+    if (lds > 65536) {
+        const hipError_t e = allow_dynamic_lds((const void*)kernel, lds, allowed);
         if (e != hipSuccess) {
             return e;
         }
     }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(S::kThreads), S::kLds, stream, args...);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3((unsigned)threads), (unsigned)lds, stream, args...);
     return hipGetLastError();
 }
 
@@ -62,23 +63,24 @@ hipError_t launch_gated_shape(ProductArgs a, hipStream_t stream)
 {
     static std::atomic<uint32_t> allowed{0};
     const int64_t blocks = prepare<T, true, false, false, S>(&a);
-    return blocks < 1 ? hipErrorInvalidValue : launch_kernel<S>(gated_kernel<T, S>, blocks, stream, allowed, a);
+    return blocks < 1 ? hipErrorInvalidValue : launch_kernel(gated_kernel<T, S>, blocks, S::kThreads, S::kLds, stream, allowed, a);
 }
 
 // `x` or `weights` may be null: one product alone
-template <typename T, typename S>
+template <typename T, typename SX, typename SW>
 hipError_t launch_gradients_shape(const ProductArgs* x, const ProductArgs* weights, hipStream_t stream)
 {
+    static_assert(SX::kThreads == SW::kThreads, "one launch");
     static std::atomic<uint32_t> allowed{0};
     ProductArgs ax, aw;
     int64_t first = 0, others = 0;
     if (x != nullptr) {
         ax = *x;
-        first = prepare<T, false, true, false, S>(&ax);
+        first = prepare<T, false, true, false, SX>(&ax);
     }
     if (weights != nullptr) {
         aw = *weights;
-        others = prepare<T, false, true, true, S>(&aw);
+        others = prepare<T, false, true, true, SW>(&aw);
     }
     if ((x != nullptr && first < 1) || (weights != nullptr && others < 1)) {
         return hipErrorInvalidValue;
@@ -86,7 +88,8 @@ hipError_t launch_gradients_shape(const ProductArgs* x, const ProductArgs* weigh
     if (first + others == 0) {
         return hipSuccess;
     }
-    return launch_kernel<S>(gradients_kernel<T, S>, first + others, stream, allowed, ax, aw, (uint32_t)first);
+    constexpr int kLds = SX::kLds > SW::kLds ? SX::kLds : SW::kLds;
+    return launch_kernel(gradients_kernel<T, SX, SW>, first + others, SX::kThreads, kLds, stream, allowed, ax, aw, (uint32_t)first);
 }
 
 template <typename T, int TB, int AHEAD>
@@ -115,7 +118,13 @@ hipError_t launch_gated_typed(const ProductArgs& a, int tile, hipStream_t stream
 template <typename T>
 hipError_t launch_gradients_typed(const ProductArgs* x, const ProductArgs* weights, int tile, hipStream_t stream)
 {
-    return tile == kTile256 ? launch_gradients_shape<T, Large>(x, weights, stream) : launch_gradients_shape<T, Small>(x, weights, stream);
+    if constexpr (sizeof(T) == 4) {
+        if (tile == kTileSlim) {
+            return launch_gradients_shape<T, Slim, Small>(x, weights, stream);
+        }
+    }
+    return tile == kTile256 ? launch_gradients_shape<T, Large, Large>(x, weights, stream)
+                            : launch_gradients_shape<T, Small, Small>(x, weights, stream);
 }
 
 }  // namespace prod

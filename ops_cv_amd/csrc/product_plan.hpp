@@ -14,6 +14,7 @@ namespace prod {
 constexpr int kTile128 = 0;  // four wavefronts, two workgroups a CU
 constexpr int kTile256 = 1;  // eight wavefronts, one workgroup a CU
 constexpr int kTileFew = 2;  // product_few.hpp: the gated projections of few rows
+constexpr int kTileSlim = 3;  // kTile128, but 32 rows by 256 features for the gradient of x, FLOAT
 
 constexpr int64_t kFewRows = 64;
 
@@ -22,7 +23,7 @@ constexpr int kRowBytes = 128;  // of a row in a stage: eight vectors of 16 byte
 // One product: rows of its operands in tiles (gated: features of both weights together), stages of 128 bytes of terms.
 struct ProductSize {
     int64_t tokens = 0, features = 0, stages = 0;
-    int64_t tiles(int64_t side) const { return (tokens + side - 1) / side * ((features + side - 1) / side); }
+    int64_t tiles(int64_t high, int64_t wide) const { return (tokens + high - 1) / high * ((features + wide - 1) / wide); }
 };
 
 // When the last workgroup ends, in its own stages, if each of `slots` takes the next workgroup as soon as it is free:
@@ -75,16 +76,23 @@ inline int64_t last_end(const int64_t* count, const int64_t* length, int64_t slo
 // 256 rows, 1024 to 4096 FLOAT: 71 us in one part.  777 rows, 1001 to 2731 FLOAT, both gradients: 247 us where parts were sized
 // by the total alone.
 // `us` is 0 where no way fits a launch.
-inline ProductPlan plan_products(const ProductSize* size, int count, int elem_bytes, int units)
+// `slim`: the first product, the gradient of x, may be made of slim tiles.
+inline ProductPlan plan_products(const ProductSize* size, int count, int elem_bytes, int units, bool slim)
 {
     ProductPlan best;
-    for (const int tile : {kTile128, kTile256}) {
+    for (const int tile : {kTile128, kTile256, kTileSlim}) {
+        if (tile == kTileSlim && !slim) {
+            continue;
+        }
         const int64_t side = tile == kTile256 ? 256 : 128;
-        const double full = elem_bytes == 4 ? 8.0 : 1.7, alone = tile == kTile256 ? full : full / 4.0 / (elem_bytes == 4 ? 1.0 : 0.85);
+        // a stage of a slim tile takes half of what one of 128 does: `unit`
+        const int64_t units_of[2] = {1, tile == kTileSlim ? 2 : 1};
+        const double full = elem_bytes == 4 ? 8.0 : 1.7, small = full / 4.0 / (elem_bytes == 4 ? 1.0 : 0.85);
+        const double alone = tile == kTile256 ? full : (tile == kTileSlim ? small / 2.0 : small);
         int64_t tiles[2] = {0, 0}, most[2] = {1, 1};
         double from_memory = 0.0;
         for (int i = 0; i < count; i++) {
-            tiles[i] = size[i].tiles(side);
+            tiles[i] = tile == kTileSlim && i == 0 ? size[i].tiles(32, 256) : size[i].tiles(side, side);
             from_memory += (double)((size[i].tokens + size[i].features) * size[i].stages * 128) / 5e6;
             // eight rounds of workgroups at most: after that, parts have nothing to even out
             most[i] = size[i].stages / 4 < 16 ? size[i].stages / 4 : 16;
@@ -106,12 +114,13 @@ inline ProductPlan plan_products(const ProductSize* size, int count, int elem_by
                         p.us += 8.0 + (double)(2 * p.parts[i] * size[i].tokens * size[i].features * 4) / 4e6;
                     }
                 }
-                if (!fits_launch(groups[0] + groups[1], tile == kTile128 ? 256 : 512)) {
+                if (!fits_launch(groups[0] + groups[1], tile == kTile256 ? 512 : 256)) {
                     continue;
                 }
-                const int64_t share = tile == kTile128 && groups[0] + groups[1] > units ? 2 : 1;  // workgroups of a CU
+                const int64_t share = tile != kTile256 && groups[0] + groups[1] > units ? 2 : 1;  // workgroups of a CU
                 const double stage = (double)share * alone > 1.0 ? (double)share * alone : 1.0;
-                const double last = (double)last_end(groups, p.part_stages, share * units) * stage;
+                const int64_t length[2] = {p.part_stages[0] * units_of[0], p.part_stages[1] * units_of[1]};
+                const double last = (double)last_end(groups, length, share * units) * stage;
                 p.us += last > from_memory ? last : from_memory;
                 if (best.us == 0.0 || p.us < best.us) {
                     best = p;
@@ -135,7 +144,7 @@ inline ProductPlan gated_plan(const GatedArgs& a)
 {
     const int e = elem_size((Elem)a.elem);
     const ProductSize size{a.rows, 2 * a.inner, (a.width * e + kRowBytes - 1) / kRowBytes};
-    ProductPlan p = plan_products(&size, 1, e, a.compute_units);
+    ProductPlan p = plan_products(&size, 1, e, a.compute_units, false);
     const double few = few_us(a.rows, 2 * a.inner * a.width * e, e);
     if (a.rows <= kFewRows && (p.us == 0.0 || few <= p.us)) {
         p = ProductPlan();
@@ -159,7 +168,11 @@ inline ProductPlan gated_grad_plan(const GatedArgs& a)
     if (a.want_weights != 0) {
         size[count++] = {2 * padded, width, (a.rows * e + kRowBytes - 1) / kRowBytes};
     }
-    return plan_products(size, count, e, a.compute_units);
+    // Few rows leave most of a tile of 128 empty, and FLOAT is slow enough that it shows: 2048 to 7168, both gradients of 8, 64, 96
+    // and 160 rows 98, 118, 135 and 224 us in tiles of 128 and 63, 95, 126 and 196 in slim ones; of 300 rows of 1064 to 4256 136
+    // and 150.  16 bits read memory all the time either way (38 and 35 us of 8 rows, 54 and 54 of 160).
+    const bool slim = a.want_x != 0 && e == 4 && a.rows <= 160;
+    return plan_products(size, count, e, a.compute_units, slim);
 }
 
 }  // namespace prod

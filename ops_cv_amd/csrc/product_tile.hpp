@@ -194,6 +194,8 @@ typedef Shape<2, 4, 4, 2> Large;
 typedef Shape<4, 2, 2, 4> LargeGated;
 // 128 x 128, four wavefronts, two workgroups a CU
 typedef Shape<2, 2, 2, 2> Small;
+// 256 features of 32 tokens, as many wavefronts and workgroups: the gradient of x of few FLOAT rows
+typedef Shape<2, 1, 4, 1> Slim;
 
 // One operand's part of the stages: WIDTH tokens or features, BLOCKS blocks of 32 a wavefront, WAVES wavefronts.
 template <typename T, bool TURNED, int WIDTH, int BLOCKS, int WAVES>
@@ -590,7 +592,7 @@ __device__ __forceinline__ void product(const ProductArgs& a, uint32_t block, ch
             }
             put(0, t, f0 + wf * FB * 32);
         } else {
-const int64_t f = f0 + wf * kRow * 32;
+            const int64_t f = f0 + wf * kRow * 32;
             const auto hold_all = [&](auto value) {
 #pragma unroll
                 for (int b = 0; b < kRow; b++) {
@@ -632,14 +634,14 @@ __global__ __launch_bounds__(S::kThreads) void gated_kernel(ProductArgs a)
 
 // The gradients of x (`first` workgroups) and of the weights, in one launch: the long sums over the inner features first, so
 // that the short ones over the rows fill up the CUs that are done.
-template <typename T, typename S>
-__global__ __launch_bounds__(S::kThreads) void gradients_kernel(ProductArgs x, ProductArgs weights, uint32_t first)
+template <typename T, typename SX, typename SW>
+__global__ __launch_bounds__(SX::kThreads) void gradients_kernel(ProductArgs x, ProductArgs weights, uint32_t first)
 {
     extern __shared__ __align__(16) char lds[];
     if (blockIdx.x < first) {
-        product<T, false, true, false, S>(x, blockIdx.x, lds);
+        product<T, false, true, false, SX>(x, blockIdx.x, lds);
     } else {
-        product<T, false, true, true, S>(weights, blockIdx.x - first, lds);
+        product<T, false, true, true, SW>(weights, blockIdx.x - first, lds);
     }
 }
 

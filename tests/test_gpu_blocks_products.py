@@ -8,7 +8,7 @@ import host_plans as P
 
 pytestmark = pytest.mark.gpu
 
-TILE = {0: "128", 1: "256", 2: "few"}
+TILE = {0: "128", 1: "256", 2: "few", 3: "slim"}
 
 
 def operands(device, dtype, rows, width, inner):
@@ -59,7 +59,9 @@ BACKWARD = [("bf16", 1, (20, 20, 520), "128", (True, False)), ("bf16", 2, (1030,
             ("bf16", 3, (1030, 4100, 520), "256", (False, False)), ("bf16", 3, (2049, 520, 4200), "256", (True, False)),
             ("fp16", 3, (2049, 520, 4200), "256", (True, False)), ("fp16", 2, (300, 8200, 520), "256", (False, False)),
             ("fp16", 3, (2049, 20, 520), "128", (True, True)),
-            ("fp32", 1, (20, 20, 264), "128", (True, False)), ("fp32", 3, (300, 20, 264), "128", (True, True)),
+            ("fp32", 1, (20, 20, 264), "slim", (True, False)), ("fp32", 1, (161, 20, 264), "128", (True, False)),
+            ("fp32", 3, (33, 300, 200), "slim", (True, False)), ("fp32", 3, (1, 1031, 30), "slim", (False, False)),
+            ("fp32", 3, (160, 516, 1100), "slim", (True, False)), ("fp32", 3, (300, 20, 264), "128", (True, True)),
             ("fp32", 1, (2049, 4104, 1100), "256", (True, False)), ("fp32", 2, (2049, 2056, 2100), "256", (True, False)),
             ("fp32", 3, (4100, 4104, 2100), "256", (False, True))]
 
