@@ -92,6 +92,8 @@ AXES = dict(q=Q, k=K, positions=((3, 2, 5), I64), table=((100, 64), F32), sectio
     (dict(layout=1), INVALID), (dict(table=((100, 62), F32)), INVALID), (dict(table=((100, 65), F32)), INVALID),
     (dict(table=((100, 64), F16)), INVALID), (dict(positions=((2, 2, 5), I64)), INVALID), (dict(positions=((2, 5), I64)), INVALID),
     (dict(positions=((3, 2, 4), I64)), INVALID), (dict(positions=((3, 2, 5), F32)), INVALID),
+    (dict(q=((2, 5, 4, 1040), BF16), qo=((2, 5, 4, 1040), BF16), k=None, ko=None, sections=[520], positions=((1, 2, 5), I64),
+          table=((100, 1040), F32)), INVALID),
     (dict(q=((2, 5, 4, 64), F64)), INVALID), (dict(qo=((2, 5, 4, 63), BF16)), INVALID), (dict(k=((2, 4, 2, 64), BF16)), INVALID)])
 def test_rotary_axes(phase1, kw, status):
     st, ws, variant = phase1("opscvRotaryAxes", *changed(AXES, **kw))
@@ -134,7 +136,11 @@ SHARED = [
     (dict(bu=((40,), F32)), INVALID), (dict(y=((6, 64), BF16)), INVALID), (dict(y=((2, 3, 40), BF16)), INVALID),
     (dict(wg=((0, 64), BF16), wu=((0, 64), BF16), bg=None, bu=None, y=((6, 0), BF16), gate=None, up=None), INVALID),
     (dict(x=((6, 2 ** 19 + 1), BF16), wg=((40, 2 ** 19 + 1), BF16), wu=((40, 2 ** 19 + 1), BF16)), INVALID),
-    (dict(x=((2 ** 30 + 1, 64), BF16), y=((2 ** 30 + 1, 40), BF16), gate=None, up=None), INVALID)] + SHARED)
+    (dict(x=((2 ** 30 + 1, 64), BF16), y=((2 ** 30 + 1, 40), BF16), gate=None, up=None), INVALID),
+    # as many rows and features as are allowed, but not together
+    (dict(x=((2 ** 30, 64), BF16), y=((2 ** 30, 40), BF16), gate=None, up=None), 0),
+    (dict(x=((2 ** 30, 64), BF16), wg=((2 ** 19, 64), BF16), wu=((2 ** 19, 64), BF16), bg=None, bu=None,
+          y=((2 ** 30, 2 ** 19), BF16), gate=None, up=None), INVALID)] + SHARED)
 def test_gated(phase1, kw, status):
     st, ws, variant = phase1("opscvGatedProjection", *changed(GATED, **kw))
     assert st == status
