@@ -590,9 +590,9 @@ def rotary_axes(query, key, table, positions, sections, layout=AXES_CONSECUTIVE,
 
 
 def dropout(x, state, p, residual=None, out=None, stream=None, workspace=None):
-    """Both phases of opscvDropout; returns residual + x / (1 - p) where an element is kept, residual (or 0) where not.  state
-    is an int64 tensor of seed and offset on x's device, read when the kernel runs: the same state gives the same mask, so the
-    gradient of x is dropout(grad, state, p).  Add to state[1] for another mask."""
+    """Both phases of opscvDropout; returns residual + x / (1 - p) where an element is kept, residual (or 0) where not, with p
+    rounded to steps of 2^-16.  state is an int64 tensor of seed and offset on x's device, read when the kernel runs: the same
+    state gives the same mask, so the gradient of x is dropout(grad, state, p).  Add to state[1] for another mask."""
     return (_helpers or _native()).dropout(x, state, p, residual, out, workspace, _raw(stream))
 
 

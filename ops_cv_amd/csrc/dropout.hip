@@ -7,7 +7,9 @@
 // each would be twice as much arithmetic (20 products of 32 by 32 bits for four elements, at a quarter of the rate of other
 // instructions), and a step of 2^-16 in p is exact in the mean, since s belongs to the threshold and not to p.
 //
-// Bound by memory: each element is read once and written once.  A thread owns the eight elements of one counter.
+// Bound by memory: each element is read once and written once.  A thread owns the eight elements of one counter, whose
+// arithmetic hides behind its loads.  16384 rows of 4096 bf16 with a residual 70 us, 5.8 TB/s (part of it stays in the 256 MB
+// cache); 5477 rows of 1283 FLOAT 11.7, 4.8 TB/s.
 #include <hip/hip_runtime.h>
 
 #include "token_elem.hpp"

@@ -11,6 +11,10 @@
 // results and tokens their columns, so that a lane holds four neighbouring features of a token.  In the gated forward product
 // blocks of 32 features alternate between the two weights, so that a lane holds gate and up of the same features, and the
 // activation and the product need no other lane.
+//
+// Bound by the products, at the clock that power allows (1.75 to 1.9 GHz; 63 % of a SIMD's cycles are products, LDS is busy for a
+// quarter).  4096 rows of 4096 to 14336 bf16: 778 us, 1235 TFLOP/s; both gradients of 4096 rows of 2048 to 8192 470 us, 1170
+// TFLOP/s; 10952 rows of 1280 to 3413 fp16 with gate and up 260, of which the results' way out is 80.
 #pragma once
 
 #include <hip/hip_runtime.h>
