@@ -77,3 +77,18 @@ def test_backward(device, aclnn, dtype, which, size, tile, parts):
     for t, w, e, what in zip(got, want, off, ("x", "gate weight", "up weight")):
         if t is not None:
             close(t, w, e, dtype, "gradient of the " + what)
+
+
+@pytest.mark.parametrize("dtype", list(B.DTYPES))
+@pytest.mark.parametrize("size", [(3, 1 << 19, 40), (70, (1 << 19) - 1, 9), (2, 24, 1 << 19), (200, 7, (1 << 19) - 3), (1 << 20, 8, 16),
+                                  ((1 << 20) - 1, 3, 5)])
+def test_ends_of_the_sizes(device, aclnn, dtype, size):
+    x, weights, biases, (gate, up, gy) = operands(device, dtype, *size)
+    want, off = B.gated(x, *weights, *biases, 0)
+    got = aclnn.gated_projection(x, *weights, *biases, need_sums=True)
+    for t, w, e, what in zip(got, want, off, ("y", "gate", "up")):
+        close(t, w, e, dtype, what)
+    want, off = B.gated_grad(gy, x, *weights, gate, up, 0, dtype)
+    got = aclnn.gated_projection_backward(gy, x, *weights, gate, up, need_bias=True)
+    for t, w, e, what in zip(got, want, off, ("x", "gate weight", "up weight", "gate bias", "up bias")):
+        close(t, w, e, dtype, "gradient of the " + what)

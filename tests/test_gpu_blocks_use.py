@@ -383,3 +383,91 @@ def test_example(device):
                        stderr=subprocess.STDOUT, text=True, timeout=110, cwd=ROOT)
     assert p.returncode == 0, p.stdout
     assert "recorded answers" in p.stdout and "loss" in p.stdout
+
+
+@pytest.mark.parametrize("heads,kv_heads,d,sections,layout", [((1 << 20) + 5, 3, 8, (1, 3), 0), (3, (2 << 20) + 1, 6, (1, 1), 2),
+                                                              ((1 << 24) + (1 << 16), 0, 255, (0, 1), 1)])
+def test_rotary_of_very_many_heads(device, aclnn, heads, kv_heads, d, sections, layout):
+    """More heads of a token than one launch takes: as a few of them alone."""
+    table = aclnn.rotary_table(torch.empty(0, device=device), 9, 2 * (max(sections) if layout == 1 else sum(sections)))
+    at = torch.tensor([[[2, 5]], [[7, 3]]], device=device)
+    made = [normal(device, 3, 1, 2, n, d) if n else None for n in (heads, kv_heads)]
+    places_of = [[slice(a, a + 70) for a in (0, (1 << 20) - 20, (1 << 21) - 30, (1 << 24) - 40, max(0, n - 70)) if a < n]
+                 for n in (heads, kv_heads)]
+    kept = [[x[:, :, p].clone() for p in ps] if x is not None else [] for x, ps in zip(made, places_of)]
+    aclnn.rotary_axes(made[0], made[1], table, at, sections, layout=layout, query_out=made[0], key_out=made[1])
+    for x, ps, before in zip(made, places_of, kept):
+        for p, b in zip(ps, before):
+            assert torch.equal(x[:, :, p], aclnn.rotary_axes(b, None, table, at, sections, layout=layout)[0]), p
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_two_threads_call_at_once(device, aclnn, dtype):
+    """First and second phases on two host threads, each on a stream of its own: the results of calls one after the other."""
+    import threading
+
+    def work(seed):
+        x, w = normal(device, seed, 70, 264, dtype=dtype), [normal(device, seed + i, 130, 264, dtype=dtype, scale=0.1) for i in (1, 2)]
+        state = torch.tensor([seed, 1], device=device)
+
+        def calls():
+            y = aclnn.layer_norm(x, None, None, x)[0]
+            g = aclnn.gated_projection(y, *w, need_sums=True)
+            return aclnn.gated_projection_backward(aclnn.dropout(g[0], state, 0.5), y, *w, *g[1:], need_bias=True)
+        return calls
+    jobs = [work(1), work(7)]
+    want = [job() for job in jobs]
+    torch.cuda.synchronize()
+    got, failed = [None, None], []
+
+    def run(i):
+        try:
+            for _ in range(30):
+                got[i] = jobs[i]()
+        except Exception as e:  # handed to the test's own thread
+            failed.append(e)
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(s, t) for s, t in zip(a, b))
+
+
+@pytest.mark.parametrize("dtype", list(B.DTYPES))
+@pytest.mark.parametrize("rows,width", [(3, 1 << 19), (2, (1 << 20) + 24), (2, (1 << 20) + 9)])
+def test_norms_of_very_long_rows(device, aclnn, dtype, rows, width):
+    """Rows that no workgroup keeps in registers, forward and backward."""
+    x, gy, w, b = (normal(device, i, *s, dtype=B.DTYPES[dtype]) for i, s in ((1, (rows, width)), (2, (rows, width)), (3, (width,)), (4, (width,))))
+    want = B.layer_norm(*(t.cpu() for t in (x, x, w, b)), 1e-5)
+    y, total, mean, rstd = aclnn.layer_norm(x, w, b, x, need_stats=True)
+    close(y, want[0], want[4] + B.gamma(width / 1024) * want[1].abs() * want[3][:, None] * w.cpu().double().abs(), dtype, "norm")
+    grads, off = B.layer_norm_grad(gy.cpu(), None, total.cpu(), w.cpu(), mean.cpu(), rstd.cpu())
+    got = aclnn.layer_norm_backward(gy, total, w, mean, rstd)
+    for t, g, o, what in zip(got, grads, off, ("x", "weight", "bias")):
+        close(t, g, o, dtype, "gradient of " + what)
+
+
+@pytest.mark.parametrize("rows,width", [(3, (1 << 25) + 33), (1, (1 << 29) + 33)])
+def test_norm_gradients_of_very_many_columns(device, aclnn, rows, width):
+    """Rows whose columns are more than a launch of the weight's gradient holds side by side."""
+    h, gy, w = (normal(device, i, *s) for i, s in ((1, (rows, width)), (2, (rows, width)), (3, (width,))))
+    mean, rstd = torch.full((rows,), 0.25, device=device), torch.full((rows,), 0.75, device=device)
+    gx, gw, gb = aclnn.layer_norm_backward(gy, h, w, mean, rstd)
+    parts = [slice(i, min(i + (1 << 24), width)) for i in range(0, width, 1 << 24)]
+    along = torch.zeros(2, rows, 1, dtype=torch.float64, device=device)
+
+    def values(p):
+        return (h[:, p].double() - 0.25) * 0.75, gy[:, p].double(), w[p].double()
+    for p in parts:
+        n, g, v = values(p)
+        along += torch.stack([(g * v).sum(1), (g * v * n).sum(1)])[..., None] / width
+    for p in parts:
+        n, g, v = values(p)
+        want = (g * v - along[0] - n * along[1]) * 0.75
+        assert ((gx[:, p].double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-5 * ((g * v).abs() + 1 + n.abs())).all()
+        for got, want, size in ((gw, (g * n).sum(0), (g * n).abs().sum(0)), (gb, g.sum(0), g.abs().sum(0))):
+            assert ((got[p].double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-5 * size).all()
