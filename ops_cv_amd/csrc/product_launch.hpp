@@ -112,6 +112,11 @@ hipError_t launch_gated_typed(const ProductArgs& a, int tile, hipStream_t stream
                : a.tokens <= 32 ? launch_few<T, 2, 2>(a, stream)
                                 : launch_few<T, 4, 1>(a, stream);
     }
+    if constexpr (sizeof(T) == 2) {
+        if (tile == kTileDeep) {
+            return launch_gated_shape<T, Deep>(a, stream);
+        }
+    }
     return tile == kTile256 ? launch_gated_shape<T, LargeGated>(a, stream) : launch_gated_shape<T, Small>(a, stream);
 }
 

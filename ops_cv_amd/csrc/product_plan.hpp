@@ -15,6 +15,7 @@ constexpr int kTile128 = 0;  // four wavefronts, two workgroups a CU
 constexpr int kTile256 = 1;  // eight wavefronts, one workgroup a CU
 constexpr int kTileFew = 2;  // product_few.hpp: the gated projections of few rows
 constexpr int kTileSlim = 3;  // kTile128, but 32 rows by 256 features for the gradient of x, FLOAT
+constexpr int kTileDeep = 4;  // kTile128 with more stages under way and one workgroup a CU, forward, 16 bits
 
 constexpr int64_t kFewRows = 64;
 
@@ -69,19 +70,21 @@ inline int64_t last_end(const int64_t* count, const int64_t* length, int64_t slo
 // Up to two products in one launch, by the time that each way would take:
 //   - a CU makes a stage of a 256 tile in 1.7 us (8.4 MFLOP of 16 bits at 5 TFLOP/s; FLOAT 8.0), one of a 128 tile in a quarter of
 //     that, 16 bits at 0.85 of the rate (8192 terms squared bf16: 877 us in large tiles, 1035 in small ones; FLOAT 139 and 132
-//     TFLOP/s); alone on a CU not under 1 us, what a stage takes to come from memory, which gives 5 TB/s to all;
+//     TFLOP/s); alone on a CU not under 1 us, what a stage takes to come from memory, which gives 5 TB/s to all, or 0.8 where
+//     three more are under way (128 rows of 4096 to 14336 bf16 71 us and 56, 512 of 4096 to 4096 55 and 46; with more tiles than CUs,
+//     768 rows, 64 and 82; FLOAT and the gradients, whose operands take longer out of LDS, gain nothing);
 //   - the terms in parts, of four stages at least, so that there is a workgroup for every CU and they end together: the parts'
 //     sums are written and read again, 4 MB a microsecond, by a kernel of 8 us, start and end of it and of the other's among
 //     them.
 // 256 rows, 1024 to 4096 FLOAT: 71 us in one part.  777 rows, 1001 to 2731 FLOAT, both gradients: 247 us where parts were sized
 // by the total alone.
 // `us` is 0 where no way fits a launch.
-// `slim`: the first product, the gradient of x, may be made of slim tiles.
-inline ProductPlan plan_products(const ProductSize* size, int count, int elem_bytes, int units, bool slim)
+// `slim`: the first product, the gradient of x, may be made of slim tiles.  `deep`: the one product may be made of deep ones.
+inline ProductPlan plan_products(const ProductSize* size, int count, int elem_bytes, int units, bool slim, bool deep)
 {
     ProductPlan best;
-    for (const int tile : {kTile128, kTile256, kTileSlim}) {
-        if (tile == kTileSlim && !slim) {
+    for (const int tile : {kTileDeep, kTile128, kTile256, kTileSlim}) {
+        if ((tile == kTileSlim && !slim) || (tile == kTileDeep && !deep)) {
             continue;
         }
         const int64_t side = tile == kTile256 ? 256 : 128;
@@ -114,11 +117,16 @@ inline ProductPlan plan_products(const ProductSize* size, int count, int elem_by
                         p.us += 8.0 + (double)(2 * p.parts[i] * size[i].tokens * size[i].features * 4) / 4e6;
                     }
                 }
+                if (tile == kTileDeep && (groups[0] > units || p.parts[0] > 1)) {
+                    continue;
+                }
                 if (!fits_launch(groups[0] + groups[1], tile == kTile256 ? 512 : 256)) {
                     continue;
                 }
-                const int64_t share = tile != kTile256 && groups[0] + groups[1] > units ? 2 : 1;  // workgroups of a CU
-                const double stage = (double)share * alone > 1.0 ? (double)share * alone : 1.0;
+                const bool single = tile == kTile256 || tile == kTileDeep;
+                const int64_t share = !single && groups[0] + groups[1] > units ? 2 : 1;  // workgroups of a CU
+                const double least = tile == kTileDeep ? 0.8 : 1.0;
+                const double stage = (double)share * alone > least ? (double)share * alone : least;
                 const int64_t length[2] = {p.part_stages[0] * units_of[0], p.part_stages[1] * units_of[1]};
                 const double last = (double)last_end(groups, length, share * units) * stage;
                 p.us += last > from_memory ? last : from_memory;
@@ -144,7 +152,7 @@ inline ProductPlan gated_plan(const GatedArgs& a)
 {
     const int e = elem_size((Elem)a.elem);
     const ProductSize size{a.rows, 2 * a.inner, (a.width * e + kRowBytes - 1) / kRowBytes};
-    ProductPlan p = plan_products(&size, 1, e, a.compute_units, false);
+    ProductPlan p = plan_products(&size, 1, e, a.compute_units, false, e == 2);
     const double few = few_us(a.rows, 2 * a.inner * a.width * e, e);
     if (a.rows <= kFewRows && (p.us == 0.0 || few <= p.us)) {
         p = ProductPlan();
@@ -172,7 +180,7 @@ inline ProductPlan gated_grad_plan(const GatedArgs& a)
     // and 160 rows 98, 118, 135 and 224 us in tiles of 128 and 63, 95, 126 and 196 in slim ones; of 300 rows of 1064 to 4256 136
     // and 150.  16 bits read memory all the time either way (38 and 35 us of 8 rows, 54 and 54 of 160).
     const bool slim = a.want_x != 0 && e == 4 && a.rows <= 160;
-    return plan_products(size, count, e, a.compute_units, slim);
+    return plan_products(size, count, e, a.compute_units, slim, false);
 }
 
 }  // namespace prod

@@ -7,7 +7,7 @@
 // over the inner features, which are the weights' rows, and those of the weights sums over the rows of x and of the gradients.
 //
 // A workgroup makes a tile of results.  Stages of 128 bytes of terms (64 of 16 bits, 32 FLOAT) of both operands are copied
-// straight to LDS, two stages in turn: while one is multiplied the other is under way.  Features are the rows of the 32 x 32
+// straight to LDS, two stages in turn or more: while one is multiplied the others are under way.  Features are the rows of the 32 x 32
 // results and tokens their columns, so that a lane holds four neighbouring features of a token.  In the gated forward product
 // blocks of 32 features alternate between the two weights, so that a lane holds gate and up of the same features, and the
 // activation and the product need no other lane.
@@ -182,14 +182,14 @@ __device__ __forceinline__ void load_to_lds(att::rsrc_t rsrc, uint32_t dst, uint
                      : "memory", "m0");
 }
 
-// FB x TB blocks of 32 x 32 results a wavefront (features, tokens), WF x WT wavefronts a workgroup.
-template <int FB_, int TB_, int WF_, int WT_>
+// FB x TB blocks of 32 x 32 results a wavefront (features, tokens), WF x WT wavefronts a workgroup, places for STAGES stages.
+template <int FB_, int TB_, int WF_, int WT_, int STAGES_ = 2>
 struct Shape {
-    static constexpr int FB = FB_, TB = TB_, WF = WF_, WT = WT_;
+    static constexpr int FB = FB_, TB = TB_, WF = WF_, WT = WT_, STAGES = STAGES_;
     static constexpr int kWaves = WF * WT, kThreads = 64 * kWaves;
     static constexpr int kFeatures = 32 * FB * WF, kTokens = 32 * TB * WT;  // rows of the operands in a stage
     static constexpr int kStageBytes = (kFeatures + kTokens) * kRowBytes;
-    static constexpr int kLds = 2 * kStageBytes;
+    static constexpr int kLds = STAGES * kStageBytes;
     static_assert(kWaves % 2 == 0 && kFeatures % (8 * kWaves) == 0 && kTokens % (8 * kWaves) == 0, "whole loads");
 };
 // 256 x 256, eight wavefronts, one workgroup a CU; gated: a wavefront has 64 features of y, so that its tokens leave in runs of
@@ -198,6 +198,8 @@ typedef Shape<2, 4, 4, 2> Large;
 typedef Shape<4, 2, 2, 4> LargeGated;
 // 128 x 128, four wavefronts, two workgroups a CU
 typedef Shape<2, 2, 2, 2> Small;
+// the same with more stages under way, one workgroup a CU: few tiles of the forward product
+typedef Shape<2, 2, 2, 2, 4> Deep;
 // 256 features of 32 tokens, as many wavefronts and workgroups: the gradient of x of few FLOAT rows
 typedef Shape<2, 1, 4, 1> Slim;
 
@@ -459,34 +461,48 @@ __device__ __forceinline__ void product(const ProductArgs& a, uint32_t block, ch
 
     // Steps j of a stage read the operands of step j + 1 before they multiply their own; the last step of a stage first waits
     // for the next stage (all wavefronts have read this one then, so its place is loaded again) and reads its first step.
+    // Loads end in the order in which they were asked for, so the wait counts those of the stages behind the next one.
+    constexpr int kLoads = SideP::kLoads + SideQ::kLoads;
+    static_assert((S::STAGES - 1) * kLoads < 64, "the loads under way can be counted");
     if (stages > 0) {
-        load_stage(0, 0);
-        if (stages > 1) {
-            load_stage(1, 1);
-            __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(SideP::kLoads + SideQ::kLoads) : "memory");
+#pragma unroll
+        for (int i = 0; i < S::STAGES; i++) {
+            if ((uint32_t)i < stages) {
+                load_stage((uint32_t)i, i);
+            }
+        }
+        if (stages >= (uint32_t)S::STAGES) {
+            __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"((S::STAGES - 1) * kLoads) : "memory");
         } else {
             __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
         __builtin_amdgcn_s_barrier();
         __asm__ volatile("" ::: "memory");
         read_step(0, 0, 0);
+        int buffer = 0;
         for (uint32_t stage = 0; stage < stages; stage++) {
-            const int buffer = (int)(stage & 1);
+            const int next = buffer + 1 < S::STAGES ? buffer + 1 : 0;
 #pragma unroll
             for (int j = 0; j < 3; j++) {
                 read_step(j + 1, buffer, (j + 1) & 1);
                 multiply(j & 1);
             }
             if (stage + 1 < stages) {
-                __asm__ volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                // of the stages behind the next one all are under way, or the last ones are waited for together
+                if (S::STAGES > 2 && stage + S::STAGES <= stages) {
+                    __asm__ volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S::STAGES - 2) * kLoads) : "memory");
+                } else {
+                    __asm__ volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                }
                 __builtin_amdgcn_s_barrier();
                 __asm__ volatile("" ::: "memory");
-                if (stage + 2 < stages) {
-                    load_stage(stage + 2, buffer);
+                if (stage + S::STAGES < stages) {
+                    load_stage(stage + S::STAGES, buffer);
                 }
-                read_step(0, buffer ^ 1, 0);
+                read_step(0, next, 0);
             }
             multiply(1);
+            buffer = next;
         }
     }
 

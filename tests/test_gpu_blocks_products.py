@@ -8,7 +8,7 @@ import host_plans as P
 
 pytestmark = pytest.mark.gpu
 
-TILE = {0: "128", 1: "256", 2: "few", 3: "slim"}
+TILE = {0: "128", 1: "256", 2: "few", 3: "slim", 4: "deep"}
 
 
 def operands(device, dtype, rows, width, inner):
@@ -31,7 +31,10 @@ def way(device, dtype, kind, size):
 
 
 # (type, size, tile, parts): the plan is asked, so that a change of its rules does not leave a way without a test
-FORWARD = [("bf16", (65, 20, 30), "128", False), ("bf16", (65, 1032, 30), "128", True), ("bf16", (129, 2056, 257), "128", True),
+FORWARD = [("bf16", (65, 20, 30), "deep", False), ("bf16", (2049, 20, 1000), "128", False), ("fp16", (1030, 200, 2100), "128", False),
+           *[(t, (129, width, 65), "deep", False) for t in ("bf16", "fp16") for width in (64, 128, 192, 250, 300, 640)],
+           ("bf16", (512, 1032, 2000), "deep", False), ("fp16", (700, 383, 511), "deep", False),
+           ("bf16", (65, 1032, 30), "128", True), ("bf16", (129, 2056, 257), "128", True),
            ("bf16", (2049, 1032, 2100), "256", False), ("bf16", (2049, 1031, 2101), "256", False), ("bf16", (4100, 8200, 520), "256", True),
            ("bf16", (20, 1032, 200), "few", False), ("bf16", (40, 520, 33), "few", False), ("bf16", (64, 2050, 4200), "few", False),
            ("fp16", (2049, 1032, 2100), "256", False), ("fp16", (4100, 8200, 520), "256", True), ("fp16", (300, 4100, 200), "128", True),

@@ -6,7 +6,7 @@ import pytest
 
 import host_plans as P
 
-THREADS = {0: 256, 1: 512, 3: 256}
+THREADS = {0: 256, 1: 512, 3: 256, 4: 256}
 VEC = {"fp32": 4, "fp16": 8, "bf16": 8}
 STAGE = {"fp32": 32, "fp16": 64, "bf16": 64}
 
@@ -55,6 +55,7 @@ def test_plans_fit(dtype, kind):
             assert kind == 0 and rows <= 64
             continue
         side, groups = 256 if p[0] == 1 else 128, 0
+        assert p[0] != 4 or (kind == 0 and dtype != "fp32" and p[1] == 1)
         assert p[0] != 3 or (kind & 1 and rows <= 160 and dtype == "fp32")
         for i, (tokens, features, stages) in enumerate(sizes):
             parts, length = p[1 + i], p[3 + i]
@@ -62,7 +63,7 @@ def test_plans_fit(dtype, kind):
             assert parts == 1 or (parts <= 16 and length >= 4)
             high, wide = (32, 256) if p[0] == 3 and i == 0 else (side, side)
             groups += parts * up(tokens, high) * up(features, wide)
-        assert groups * THREADS[p[0]] < 2 ** 32
+        assert groups * THREADS[p[0]] < 2 ** 32 and (p[0] != 4 or groups <= 256)
 
 
 def test_largest_results():
