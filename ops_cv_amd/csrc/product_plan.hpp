@@ -15,7 +15,7 @@ constexpr int kTile128 = 0;  // four wavefronts, two workgroups a CU
 constexpr int kTile256 = 1;  // eight wavefronts, one workgroup a CU
 constexpr int kTileFew = 2;  // product_few.hpp: the gated projections of few rows
 constexpr int kTileSlim = 3;  // kTile128, but 32 rows by 256 features for the gradient of x, FLOAT
-constexpr int kTileDeep = 4;  // kTile128 with more stages under way and one workgroup a CU, forward, 16 bits
+constexpr int kTileDeep = 4;  // kTile128 with more stages under way, eight wavefronts and one workgroup a CU, forward, 16 bits
 
 constexpr int64_t kFewRows = 64;
 
@@ -71,7 +71,7 @@ inline int64_t last_end(const int64_t* count, const int64_t* length, int64_t slo
 //   - a CU makes a stage of a 256 tile in 1.7 us (8.4 MFLOP of 16 bits at 5 TFLOP/s; FLOAT 8.0), one of a 128 tile in a quarter of
 //     that, 16 bits at 0.85 of the rate (8192 terms squared bf16: 877 us in large tiles, 1035 in small ones; FLOAT 139 and 132
 //     TFLOP/s); alone on a CU not under 1 us, what a stage takes to come from memory, which gives 5 TB/s to all, or 0.8 where
-//     three more are under way (128 rows of 4096 to 14336 bf16 71 us and 56, 512 of 4096 to 4096 55 and 46; with more tiles than CUs,
+//     three more are under way (128 rows of 4096 to 14336 bf16 71 us and 56, 512 of 4096 to 4096 55 and 44; with more tiles than CUs,
 //     768 rows, 64 and 82; FLOAT and the gradients, whose operands take longer out of LDS, gain nothing);
 //   - the terms in parts, of four stages at least, so that there is a workgroup for every CU and they end together: the parts'
 //     sums are written and read again, 4 MB a microsecond, by a kernel of 8 us, start and end of it and of the other's among
@@ -91,6 +91,7 @@ inline ProductPlan plan_products(const ProductSize* size, int count, int elem_by
         // a stage of a slim tile takes half of what one of 128 does: `unit`
         const int64_t units_of[2] = {1, tile == kTileSlim ? 2 : 1};
         const double full = elem_bytes == 4 ? 8.0 : 1.7, small = full / 4.0 / (elem_bytes == 4 ? 1.0 : 0.85);
+        const bool single = tile == kTile256 || tile == kTileDeep;  // one workgroup a CU, of eight wavefronts
         const double alone = tile == kTile256 ? full : (tile == kTileSlim ? small / 2.0 : small);
         int64_t tiles[2] = {0, 0}, most[2] = {1, 1};
         double from_memory = 0.0;
@@ -120,10 +121,9 @@ inline ProductPlan plan_products(const ProductSize* size, int count, int elem_by
                 if (tile == kTileDeep && (groups[0] > units || p.parts[0] > 1)) {
                     continue;
                 }
-                if (!fits_launch(groups[0] + groups[1], tile == kTile256 ? 512 : 256)) {
+                if (!fits_launch(groups[0] + groups[1], single ? 512 : 256)) {
                     continue;
                 }
-                const bool single = tile == kTile256 || tile == kTileDeep;
                 const int64_t share = !single && groups[0] + groups[1] > units ? 2 : 1;  // workgroups of a CU
                 const double least = tile == kTileDeep ? 0.8 : 1.0;
                 const double stage = (double)share * alone > least ? (double)share * alone : least;

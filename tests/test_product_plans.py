@@ -6,7 +6,7 @@ import pytest
 
 import host_plans as P
 
-THREADS = {0: 256, 1: 512, 3: 256, 4: 256}
+THREADS = {0: 256, 1: 512, 3: 256, 4: 512}
 VEC = {"fp32": 4, "fp16": 8, "bf16": 8}
 STAGE = {"fp32": 32, "fp16": 64, "bf16": 64}
 
