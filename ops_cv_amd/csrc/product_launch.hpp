@@ -116,6 +116,10 @@ hipError_t launch_gated_typed(const ProductArgs& a, int tile, hipStream_t stream
         if (tile == kTileDeep) {
             return launch_gated_shape<T, Deep>(a, stream);
         }
+    } else {
+        if (tile == kTileSlim) {
+            return launch_gated_shape<T, Slim>(a, stream);
+        }
     }
     return tile == kTile256 ? launch_gated_shape<T, LargeGated>(a, stream) : launch_gated_shape<T, Small>(a, stream);
 }

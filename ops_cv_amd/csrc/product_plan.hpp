@@ -14,7 +14,7 @@ namespace prod {
 constexpr int kTile128 = 0;  // four wavefronts, two workgroups a CU
 constexpr int kTile256 = 1;  // eight wavefronts, one workgroup a CU
 constexpr int kTileFew = 2;  // product_few.hpp: the gated projections of few rows
-constexpr int kTileSlim = 3;  // kTile128, but 32 rows by 256 features for the gradient of x, FLOAT
+constexpr int kTileSlim = 3;  // kTile128, but 32 rows by 256 features for the forward product or the gradient of x, FLOAT
 constexpr int kTileDeep = 4;  // kTile128 with more stages under way, eight wavefronts and one workgroup a CU, forward, 16 bits
 
 constexpr int64_t kFewRows = 64;
@@ -79,7 +79,11 @@ inline int64_t last_end(const int64_t* count, const int64_t* length, int64_t slo
 // 256 rows, 1024 to 4096 FLOAT: 71 us in one part.  777 rows, 1001 to 2731 FLOAT, both gradients: 247 us where parts were sized
 // by the total alone.
 // `us` is 0 where no way fits a launch.
-// `slim`: the first product, the gradient of x, may be made of slim tiles.  `deep`: the one product may be made of deep ones.
+// `slim`: the first product may be made of slim tiles.  Rows that end inside a tile leave a part of it empty, and FLOAT is slow
+// enough that it shows: 2048 to 7168, both gradients of 8, 64, 160 and 777 rows, 98, 118, 224 and 794 us in tiles of 128 and 63, 95,
+// 196 and 841 with slim ones, whose stage takes 7 / 12 of the time for half of the products; forward 389 rows of 1280 to 4480 126
+// and 96, 128 rows 43 and 54.  16 bits read memory all the time either way (gradients of 8 rows 38 and 35, of 160 54 and 54).
+// `deep`: the one product may be made of deep ones.
 inline ProductPlan plan_products(const ProductSize* size, int count, int elem_bytes, int units, bool slim, bool deep)
 {
     ProductPlan best;
@@ -88,11 +92,11 @@ inline ProductPlan plan_products(const ProductSize* size, int count, int elem_by
             continue;
         }
         const int64_t side = tile == kTile256 ? 256 : 128;
-        // a stage of a slim tile takes half of what one of 128 does: `unit`
-        const int64_t units_of[2] = {1, tile == kTileSlim ? 2 : 1};
+        // a stage of a slim tile takes 7 / 12 of what one of 128 does
+        const int64_t weight[2] = {tile == kTileSlim ? 7 : 1, tile == kTileSlim ? 12 : 1};
         const double full = elem_bytes == 4 ? 8.0 : 1.7, small = full / 4.0 / (elem_bytes == 4 ? 1.0 : 0.85);
         const bool single = tile == kTile256 || tile == kTileDeep;  // one workgroup a CU, of eight wavefronts
-        const double alone = tile == kTile256 ? full : (tile == kTileSlim ? small / 2.0 : small);
+        const double alone = tile == kTile256 ? full : (tile == kTileSlim ? small / 12.0 : small);
         int64_t tiles[2] = {0, 0}, most[2] = {1, 1};
         double from_memory = 0.0;
         for (int i = 0; i < count; i++) {
@@ -125,9 +129,9 @@ inline ProductPlan plan_products(const ProductSize* size, int count, int elem_by
                     continue;
                 }
                 const int64_t share = !single && groups[0] + groups[1] > units ? 2 : 1;  // workgroups of a CU
-                const double least = tile == kTileDeep ? 0.8 : 1.0;
+                const double least = tile == kTileDeep ? 0.8 : (tile == kTileSlim ? 1.2 / 7.0 : 1.0);
                 const double stage = (double)share * alone > least ? (double)share * alone : least;
-                const int64_t length[2] = {p.part_stages[0] * units_of[0], p.part_stages[1] * units_of[1]};
+                const int64_t length[2] = {p.part_stages[0] * weight[0], p.part_stages[1] * weight[1]};
                 const double last = (double)last_end(groups, length, share * units) * stage;
                 p.us += last > from_memory ? last : from_memory;
                 if (best.us == 0.0 || p.us < best.us) {
@@ -152,7 +156,7 @@ inline ProductPlan gated_plan(const GatedArgs& a)
 {
     const int e = elem_size((Elem)a.elem);
     const ProductSize size{a.rows, 2 * a.inner, (a.width * e + kRowBytes - 1) / kRowBytes};
-    ProductPlan p = plan_products(&size, 1, e, a.compute_units, false, e == 2);
+    ProductPlan p = plan_products(&size, 1, e, a.compute_units, e == 4, e == 2);
     const double few = few_us(a.rows, 2 * a.inner * a.width * e, e);
     if (a.rows <= kFewRows && (p.us == 0.0 || few <= p.us)) {
         p = ProductPlan();
@@ -176,11 +180,7 @@ inline ProductPlan gated_grad_plan(const GatedArgs& a)
     if (a.want_weights != 0) {
         size[count++] = {2 * padded, width, (a.rows * e + kRowBytes - 1) / kRowBytes};
     }
-    // Few rows leave most of a tile of 128 empty, and FLOAT is slow enough that it shows: 2048 to 7168, both gradients of 8, 64, 96
-    // and 160 rows 98, 118, 135 and 224 us in tiles of 128 and 63, 95, 126 and 196 in slim ones; of 300 rows of 1064 to 4256 136
-    // and 150.  16 bits read memory all the time either way (38 and 35 us of 8 rows, 54 and 54 of 160).
-    const bool slim = a.want_x != 0 && e == 4 && a.rows <= 160;
-    return plan_products(size, count, e, a.compute_units, slim, false);
+    return plan_products(size, count, e, a.compute_units, a.want_x != 0 && e == 4, false);
 }
 
 }  // namespace prod

@@ -201,7 +201,7 @@ typedef Shape<2, 2, 2, 2> Small;
 // 128 x 128, eight wavefronts, more stages under way, one workgroup a CU: few tiles of the forward product (with four wavefronts, which
 // wait for LDS with nothing beside them, 512 rows of 4096 to 4096 47 us, 80 of 1024 to 4096 13; with eight 44 and 12)
 typedef Shape<2, 1, 2, 4, 4> Deep;
-// 256 features of 32 tokens, as many wavefronts and workgroups: the gradient of x of few FLOAT rows
+// 256 features of 32 tokens, four wavefronts, two workgroups a CU: FLOAT rows that would leave larger tiles empty
 typedef Shape<2, 1, 4, 1> Slim;
 
 // One operand's part of the stages: WIDTH tokens or features, BLOCKS blocks of 32 a wavefront, WAVES wavefronts.

@@ -117,7 +117,7 @@ def nearest_rows_nanoseconds(dtype, shape, out, channels_last=False):
 def gated_plan(dtype, kind, rows, width, inner, units=256):
     """(tile, parts of both products, stages of their parts, nanoseconds expected) of a gated projection, None where it fits no
     launch; kind 0 is the forward pass, else 1 for x's gradient plus 2 for the weights'.  Tiles: 0 of 128, 1 of 256, 2 few rows,
-    3 slim ones for x's gradient, 4 deep ones."""
+    3 slim ones, 4 deep ones."""
     return _call("gated_plan", 6, dtype, kind, rows, width, inner, units)
 
 

@@ -38,7 +38,9 @@ FORWARD = [("bf16", (65, 20, 30), "deep", False), ("bf16", (2049, 20, 1000), "12
            ("bf16", (2049, 1032, 2100), "256", False), ("bf16", (2049, 1031, 2101), "256", False), ("bf16", (4100, 8200, 520), "256", True),
            ("bf16", (20, 1032, 200), "few", False), ("bf16", (40, 520, 33), "few", False), ("bf16", (64, 2050, 4200), "few", False),
            ("fp16", (2049, 1032, 2100), "256", False), ("fp16", (4100, 8200, 520), "256", True), ("fp16", (300, 4100, 200), "128", True),
-           ("fp32", (65, 520, 30), "128", True), ("fp32", (300, 72, 520), "128", False), ("fp32", (2049, 2056, 2100), "256", True),
+           ("fp32", (65, 520, 30), "slim", True), ("fp32", (300, 72, 520), "slim", False), ("fp32", (97, 63, 1031), "slim", False),
+           ("fp32", (2049, 20, 520), "128", False), ("fp32", (1030, 2056, 30), "128", True), ("fp32", (389, 640, 1200), "slim", False),
+           ("fp32", (2049, 2056, 2100), "256", True),
            ("fp32", (33, 1030, 70), "few", False), ("fp32", (60, 500, 2100), "few", False)]
 
 
@@ -62,9 +64,11 @@ BACKWARD = [("bf16", 1, (20, 20, 520), "128", (True, False)), ("bf16", 2, (1030,
             ("bf16", 3, (1030, 4100, 520), "256", (False, False)), ("bf16", 3, (2049, 520, 4200), "256", (True, False)),
             ("fp16", 3, (2049, 520, 4200), "256", (True, False)), ("fp16", 2, (300, 8200, 520), "256", (False, False)),
             ("fp16", 3, (2049, 20, 520), "128", (True, True)),
-            ("fp32", 1, (20, 20, 264), "slim", (True, False)), ("fp32", 1, (161, 20, 264), "128", (True, False)),
+            ("fp32", 1, (20, 20, 264), "slim", (True, False)), ("fp32", 1, (2049, 20, 520), "128", (True, False)), ("fp32", 1, (520, 4104, 30), "128", (False, False)),
             ("fp32", 3, (33, 300, 200), "slim", (True, False)), ("fp32", 3, (1, 1031, 30), "slim", (False, False)),
-            ("fp32", 3, (160, 516, 1100), "slim", (True, False)), ("fp32", 3, (300, 20, 264), "128", (True, True)),
+            ("fp32", 3, (160, 516, 1100), "slim", (True, False)), ("fp32", 3, (520, 20, 264), "128", (True, True)),
+            ("fp32", 3, (300, 20, 2100), "slim", (True, True)), ("fp32", 3, (4100, 20, 264), "slim", (False, True)),
+            ("fp32", 3, (65, 20, 30), "128", (False, False)),
             ("fp32", 1, (2049, 4104, 1100), "256", (True, False)), ("fp32", 2, (2049, 2056, 2100), "256", (True, False)),
             ("fp32", 3, (4100, 4104, 2100), "256", (False, True))]
 

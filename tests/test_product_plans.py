@@ -56,7 +56,7 @@ def test_plans_fit(dtype, kind):
             continue
         side, groups = 256 if p[0] == 1 else 128, 0
         assert p[0] != 4 or (kind == 0 and dtype != "fp32" and p[1] == 1)
-        assert p[0] != 3 or (kind & 1 and rows <= 160 and dtype == "fp32")
+        assert p[0] != 3 or (kind != 2 and dtype == "fp32")
         for i, (tokens, features, stages) in enumerate(sizes):
             parts, length = p[1 + i], p[3 + i]
             assert (parts - 1) * length < stages <= parts * length  # none is empty
