@@ -202,7 +202,7 @@ hipError_t launch_gated(const GatedArgs& a, hipStream_t stream)
         case Elem::F16: OPSCV_LAUNCH(launch_products_f16(p, a.plan.tile, stream)); break;
         default: OPSCV_LAUNCH(launch_products_bf16(p, a.plan.tile, stream)); break;
     }
-    return p.partial != nullptr ? launch_join(elem, p, true, stream) : hipSuccess;
+    return p.partial != nullptr ? launch_join_gated(elem, p, stream) : hipSuccess;
 }
 
 hipError_t launch_gated_grad(const GatedArgs& a, hipStream_t stream)
@@ -292,17 +292,17 @@ hipError_t launch_gated_grad(const GatedArgs& a, hipStream_t stream)
             default: OPSCV_LAUNCH(launch_gradients_bf16(px, pw, a.plan.tile, stream)); break;
         }
     }
-    if (x.partial != nullptr) {
-        OPSCV_LAUNCH(launch_join(elem, x, false, stream));
-    }
-    if (weights.partial != nullptr) {
-        OPSCV_LAUNCH(launch_join(elem, weights, false, stream));
-    }
+    FinishArgs f;
+    f.x = &x;
+    f.weights = &weights;
     if (a.want_biases != 0) {
-        OPSCV_LAUNCH(launch_bias_sums(elem, g.sums, sum_rows(a, l.padded), a.inner, a.grad_gate_bias,
-                                      a.grad_up_bias, stream));
+        f.sums = g.sums;
+        f.sum_rows = sum_rows(a, l.padded);
+        f.inner = a.inner;
+        f.gate = a.grad_gate_bias;
+        f.up = a.grad_up_bias;
     }
-    return hipSuccess;
+    return launch_finish(elem, f, stream);
 }
 
 }  // namespace opscv

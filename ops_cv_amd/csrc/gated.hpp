@@ -65,11 +65,18 @@ inline int64_t gate_rows(int64_t rows, int64_t padded, int elem_bytes, int compu
 
 hipError_t launch_gate_grad(const GateGradArgs& a, hipStream_t stream);
 
-// The sums of a product's parts, in the places of its results (product_tile.hpp).
-hipError_t launch_join(Elem e, const ProductArgs& a, bool gated, hipStream_t stream);
+// The sums of the gated product's parts, in the places of its results (product_tile.hpp).
+hipError_t launch_join_gated(Elem e, const ProductArgs& a, hipStream_t stream);
 
-// Sums of the rows of (rows, 2 inner): the first inner to `gate`, the others to `up`.
-hipError_t launch_bias_sums(Elem e, const float* sums, int64_t rows, int64_t inner, void* gate, void* up, hipStream_t stream);
+// What is left of the gradients after their products, in one launch: sums of parts, where there are any (`partial`), and of the
+// biases' rows, (rows, 2 inner), the first inner to `gate`, the others to `up`.
+struct FinishArgs {
+    const ProductArgs *x = nullptr, *weights = nullptr;
+    const float* sums = nullptr;
+    int64_t sum_rows = 0, inner = 0;
+    void *gate = nullptr, *up = nullptr;  // both or neither
+};
+hipError_t launch_finish(Elem e, const FinishArgs& a, hipStream_t stream);
 
 }  // namespace prod
 }  // namespace opscv

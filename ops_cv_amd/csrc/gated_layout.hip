@@ -349,10 +349,10 @@ __device__ __forceinline__ void join_parts(const float* from, int64_t part, uint
 constexpr int kJoin = 4;  // features of a thread
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void join_kernel(ProductArgs a)
+__device__ __forceinline__ void join(const ProductArgs& a, uint32_t block, uint32_t blocks)
 {
     const int64_t vectors = (a.columns + kJoin - 1) / kJoin, total = a.tokens * vectors;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
+    for (int64_t i = (int64_t)block * kThreads + threadIdx.x; i < total; i += (int64_t)blocks * kThreads) {
         const int64_t t = i / vectors, f = (i - t * vectors) * kJoin;
         const bool second = t >= a.turn;
         const int64_t row = second ? t - a.turn : t;
@@ -370,6 +370,29 @@ __global__ __launch_bounds__(kThreads) void join_kernel(ProductArgs a)
         }
         store_part<T, kJoin, false>((T*)a.out[second] + row * a.out_stride[second], f, a.columns, x, false);
     }
+}
+
+// The first workgroups join x's parts, the next ones the weights', the others sum up the biases' rows: launches of their own
+// would each take 4 to 5 us (512 rows of 512 to 2048 bf16, all gradients: 25 us).
+template <typename T>
+__global__ __launch_bounds__(kThreads) void finish_kernel(ProductArgs x, ProductArgs weights, uint32_t x_blocks,
+                                                          uint32_t weight_blocks, const float* sums, int64_t sum_rows,
+                                                          int64_t inner, T* gate, T* up)
+{
+    uint32_t block = blockIdx.x;
+    if (block < x_blocks) {
+        join<T>(x, block, x_blocks);
+        return;
+    }
+    block -= x_blocks;
+    if (block < weight_blocks) {
+        join<T>(weights, block, weight_blocks);
+        return;
+    }
+    block -= weight_blocks;
+    const uint32_t blocks = (uint32_t)((inner + 31) / 32);
+    const bool second = block >= blocks;
+    column_sums<T>(second ? sums + inner : sums, second ? block - blocks : block, sum_rows, inner, 2 * inner, second ? up : gate);
 }
 
 template <typename T>
@@ -453,25 +476,33 @@ hipError_t launch_gate_grad(const GateGradArgs& a, hipStream_t stream)
     });
 }
 
-hipError_t launch_join(Elem e, const ProductArgs& a, bool gated, hipStream_t stream)
+hipError_t launch_join_gated(Elem e, const ProductArgs& a, hipStream_t stream)
 {
     return typed(e, [&](auto* t) {
         typedef std::remove_pointer_t<decltype(t)> T;
-        const dim3 grid(blocks_of(a.tokens * ((a.columns + kJoin - 1) / kJoin)));
-        if (gated) {
-            hipLaunchKernelGGL((join_gated_kernel<T>), grid, dim3(kThreads), 0, stream, a);
-        } else {
-            hipLaunchKernelGGL((join_kernel<T>), grid, dim3(kThreads), 0, stream, a);
-        }
+        hipLaunchKernelGGL((join_gated_kernel<T>), dim3(blocks_of(a.tokens * ((a.columns + kJoin - 1) / kJoin))), dim3(kThreads), 0,
+                           stream, a);
         return hipGetLastError();
     });
 }
 
-hipError_t launch_bias_sums(Elem e, const float* sums, int64_t rows, int64_t inner, void* gate, void* up, hipStream_t stream)
+hipError_t launch_finish(Elem e, const FinishArgs& a, hipStream_t stream)
 {
+    const auto blocks = [](const ProductArgs& p) {
+        return p.partial == nullptr ? 0u : blocks_of(p.tokens * ((p.columns + kJoin - 1) / kJoin));
+    };
+    const uint32_t x = blocks(*a.x), weights = blocks(*a.weights);
+    const uint32_t biases = a.gate == nullptr ? 0u : 2u * (uint32_t)((a.inner + 31) / 32);
+    if (x + weights + biases == 0) {
+        return hipSuccess;
+    }
+    if (a.inner < 0 || a.inner > (int64_t)1 << 24) {
+        return hipErrorInvalidValue;
+    }
     return typed(e, [&](auto* t) {
         typedef std::remove_pointer_t<decltype(t)> T;
-        launch_column_sums<T>(sums, sums + inner, rows, inner, (T*)gate, (T*)up, stream, 2 * inner);
+        hipLaunchKernelGGL((finish_kernel<T>), dim3(x + weights + biases), dim3(kThreads), 0, stream, *a.x, *a.weights, x, weights,
+                           a.sums, a.sum_rows, a.inner, (T*)a.gate, (T*)a.up);
         return hipGetLastError();
     });
 }

@@ -69,8 +69,8 @@ __global__ __launch_bounds__(kThreads) void rotary_table_kernel(RotaryTableArgs 
 // How the pairs of a head are shared out to several axes.
 struct AxesPlan {
     int uniform = 0;                         // every thread's pairs are of one axis and side by side in the table
-    uint16_t column[kMostPairs] = {0};       // of the table, for every pair
-    uint8_t axis[kMostPairs] = {0};
+    alignas(16) uint16_t column[kMostPairs] = {0};  // of the table, for every pair
+    alignas(16) uint8_t axis[kMostPairs] = {0};
 };
 struct NoAxes {};
 
@@ -181,20 +181,30 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryPlan<AXES> p)
                     }
                 }
             } else {
+                // all loads of a step go out together: the pairs' axes and columns with the positions, then the angles, of a
+                // row that is there if the position is not
+                const Pack<uint8_t, kPairs> axes = *reinterpret_cast<const Pack<uint8_t, kPairs>*>(p.axes.axis + pair);
+                const Pack<uint16_t, kPairs> columns = *reinterpret_cast<const Pack<uint16_t, kPairs>*>(p.axes.column + pair);
                 int64_t at[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     at[i] = i < a.axes ? whole_at(a.position, b, t, i) : 0;
                 }
+                if (a.positions > 0) {
 #pragma unroll
-                for (int i = 0; i < kPairs; i++) {
-                    const int axis = p.axes.axis[pair + i];
-                    const int64_t own = axis == 0 ? at[0] : axis == 1 ? at[1] : axis == 2 ? at[2] : at[3];
-                    cosine[i] = sine[i] = NAN;
-                    if (own >= 0 && own < a.positions) {
-                        const float* const from = a.table + own * a.table_stride + p.axes.column[pair + i];
-                        cosine[i] = from[0];
-                        sine[i] = from[a.columns];
+                    for (int i = 0; i < kPairs; i++) {
+                        const int axis = axes.v[i];
+                        const int64_t own = axis == 0 ? at[0] : axis == 1 ? at[1] : axis == 2 ? at[2] : at[3];
+                        const bool there = own >= 0 && own < a.positions;
+                        const float* const from = a.table + (there ? own : 0) * a.table_stride + columns.v[i];
+                        const float c = from[0], s = from[a.columns];
+                        cosine[i] = there ? c : NAN;
+                        sine[i] = there ? s : NAN;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kPairs; i++) {
+                        cosine[i] = sine[i] = NAN;
                     }
                 }
             }

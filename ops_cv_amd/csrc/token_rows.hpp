@@ -44,16 +44,14 @@ static __device__ __forceinline__ void rows_reduce(float (&sum)[R], float (*shar
     }
 }
 
-// Sums of the rows of partial sums, of one or two gradients (blockIdx.z): 32 columns a workgroup, every eighth row a thread,
-// joined in order.
+// Sums of the rows of partial sums: 32 columns a workgroup of 256 threads, every eighth row a thread, joined in order.
 template <typename W>
-static __global__ __launch_bounds__(256) void column_sums_kernel(const float* first, const float* second, int64_t rows,
-                                                                 int64_t width, int64_t stride, W* first_out, W* second_out)
+static __device__ __forceinline__ void column_sums(const float* partial, int64_t block, int64_t rows, int64_t width, int64_t stride,
+                                                   W* out)
 {
     __shared__ float shared[8][32];
-    const float* const partial = blockIdx.z == 0 ? first : second;
     const int column = (int)threadIdx.x & 31, part = (int)threadIdx.x >> 5;
-    const int64_t c = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 32 + column;
+    const int64_t c = block * 32 + column;
     float total = 0.0f;
     if (c < width) {
 #pragma unroll 8
@@ -68,14 +66,23 @@ static __global__ __launch_bounds__(256) void column_sums_kernel(const float* fi
         for (int i = 1; i < 8; i++) {
             total += shared[i][column];
         }
-        (blockIdx.z == 0 ? first_out : second_out)[c] = (W)total;
+        out[c] = (W)total;
     }
 }
 
-// `stride`: of the rows, where they are further apart than their width.  Either output may be null.
+// Of one or two gradients (blockIdx.z).
+template <typename W>
+static __global__ __launch_bounds__(256) void column_sums_kernel(const float* first, const float* second, int64_t rows,
+                                                                 int64_t width, int64_t stride, W* first_out, W* second_out)
+{
+    column_sums<W>(blockIdx.z == 0 ? first : second, (int64_t)blockIdx.y * gridDim.x + blockIdx.x, rows, width, stride,
+                   blockIdx.z == 0 ? first_out : second_out);
+}
+
+// Either output may be null.
 template <typename W>
 void launch_column_sums(const float* first, const float* second, int64_t rows, int64_t width, W* first_out, W* second_out,
-                        hipStream_t stream, int64_t stride = 0)
+                        hipStream_t stream)
 {
     if (first_out == nullptr) {
         first = second;
@@ -87,8 +94,8 @@ void launch_column_sums(const float* first, const float* second, int64_t rows, i
     const int64_t blocks = (width + 31) / 32;
     const dim3 columns((unsigned)(blocks < kMostBlocks ? blocks : kMostBlocks), (unsigned)((blocks + kMostBlocks - 1) / kMostBlocks),
                        second_out != nullptr ? 2 : 1);
-    hipLaunchKernelGGL((column_sums_kernel<W>), columns, dim3(256), 0, stream, first, second, rows, width,
-                       stride > 0 ? stride : width, first_out, second_out);
+    hipLaunchKernelGGL((column_sums_kernel<W>), columns, dim3(256), 0, stream, first, second, rows, width, width,
+                       first_out, second_out);
 }
 
 // f(T, W) by the operands' types
