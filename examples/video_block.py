@@ -5,7 +5,7 @@ Frames are cut into patches, whose positions are (frame, row, column). Each bloc
 through the operators' backward forms; the answers come from a recorded graph. The remaining projections are torch's matrix
 products. Pictures and weights are random.
 
-    python examples/video_block.py [--steps 30]
+    python examples/video_block.py [--steps 400]
 """
 import argparse
 import os
@@ -159,7 +159,7 @@ def videos(pictures, way):
 
 def main():
     p = argparse.ArgumentParser(description=__doc__.splitlines()[0])
-    p.add_argument("--steps", type=int, default=30)
+    p.add_argument("--steps", type=int, default=400)
     a = p.parse_args()
     torch.manual_seed(0)
     dev = torch.device("cuda:0")
