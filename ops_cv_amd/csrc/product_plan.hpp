@@ -132,6 +132,11 @@ inline ProductPlan plan_products(const ProductSize* size, int count, int elem_by
                 const double least = tile == kTileDeep ? 0.8 : (tile == kTileSlim ? 1.2 / 7.0 : 1.0);
                 const double stage = (double)share * alone > least ? (double)share * alone : least;
                 const int64_t length[2] = {p.part_stages[0] * weight[0], p.part_stages[1] * weight[1]};
+                // not before all slots have had an equal share: most ways are ruled out by that
+                const double equal = (double)(groups[0] * length[0] + groups[1] * length[1]) / (double)(share * units) * stage;
+                if (best.us != 0.0 && p.us + (equal > from_memory ? equal : from_memory) >= best.us) {
+                    continue;
+                }
                 const double last = (double)last_end(groups, length, share * units) * stage;
                 p.us += last > from_memory ? last : from_memory;
                 if (best.us == 0.0 || p.us < best.us) {

@@ -75,6 +75,6 @@ def test_largest_results():
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_host_time(dtype):
-    """A part of what a launch takes: 27 us is the most here for sizes of some thousands."""
+    """Some 20 us is the most that random sizes take."""
     for kind, size in ((0, (8, 4096, 14336)), (3, (777, 1001, 2731)), (3, (3000, 3000, 3000)), (3, (64, 8192, 8192))):
         assert P.gated_plan_nanoseconds(dtype, kind, *size) < 500_000
