@@ -15,6 +15,10 @@ PlannedPtr plan_view(aclOpExecutor* ex, const aclTensor* t, int elem_bytes, bool
 {
     PlannedPtr p;
     char* base = (t->data == nullptr) ? nullptr : (char*)t->data + t->offset * (int64_t)elem_bytes;
+    if (t->empty()) {  // nothing to pack, and its address may be null
+        p.direct = base;
+        return p;
+    }
     aclOpExecutor::Pack pk;
     pk.view.base = base;
     const int n = (int)t->ndim;
