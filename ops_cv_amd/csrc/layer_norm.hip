@@ -3,8 +3,11 @@
 //   h = x + r,  m = mean(h),  rstd = 1 / sqrt(mean((h - m)^2) + eps),  y = (h - m) rstd w + b
 //   n = (h - m) rstd, g = gy w:  gx = (g - mean(g) - n mean(g n)) rstd + gs,  gw = sum gy n,  gb = sum gy
 //
-// The squares are taken of h - m in a second round over the registers, not as mean(h^2) - m^2, which loses the variance of
-// rows whose mean is large beside their spread; h stays in 32 bits between the addition and the norm.
+// The squares are taken of h - m0 in a second round over the registers, not as mean(h^2) - m^2, which loses the variance of
+// rows whose mean is large beside their spread; h stays in 32 bits between the addition and the norm.  m0 is the mean as
+// summed up in 32 bits, off by some 2^-24 of the values, which is much of a small spread; the mean of h - m0, from the same
+// round, corrects it:
+//   m = m0 + mean(h - m0),  variance = mean((h - m0)^2) - mean(h - m0)^2
 //
 // Bound by memory: every element is read once and written once, so a row stays in registers between its sums and its
 // result.  A row belongs to one wavefront (up to 16 elements a lane, or 24), to 256 threads, or to 1024; longer rows are read three
@@ -78,12 +81,20 @@ __device__ __forceinline__ void put_statistics(const LayerNormArgs& a, int64_t r
     }
 }
 
+// Mean and rstd from the first mean and the sums of what it leaves of the elements, and of its squares.
+__device__ __forceinline__ void statistics(const LayerNormArgs& a, float first, const float (&left)[2], float* mean, float* rstd)
+{
+    const float more = left[0] / (float)a.width, variance = left[1] / (float)a.width - more * more;
+    *mean = more == more ? first + more : first;  // an infinite mean leaves NaN
+    *rstd = 1.0f / sqrtf((variance < 0.0f ? 0.0f : variance) + a.eps);
+}
+
 // THREADS per row; a workgroup is 256 threads, or THREADS where that is more.  NV vectors of VEC elements a thread.
 template <typename T, typename W, int THREADS, int NV, int VEC, bool WIDE>
 __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void layer_norm_kernel(LayerNormArgs a)
 {
     constexpr int kRows = THREADS >= 256 ? 1 : 256 / THREADS;
-    __shared__ float shared[2][1][16];
+    __shared__ float shared[1][1][16], shared_left[1][2][16];
     const int lane = (int)threadIdx.x % THREADS;
     // where a barrier follows (THREADS >= 256), a workgroup has one row and all its threads make as many turns
     for (int64_t row = (int64_t)blockIdx.x * kRows + (int)threadIdx.x / THREADS; row < a.rows;
@@ -114,21 +125,22 @@ __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void layer_norm_kern
         }
         // two reductions a row, each with places of its own: one barrier a reduction is enough
         rows_reduce<THREADS, 1>(sum, shared, 0);
-        const float mean = sum[0] / (float)a.width;
-        sum[0] = 0.0f;
+        const float first = sum[0] / (float)a.width;
+        float left[2] = {0.0f, 0.0f}, mean, rstd;
 #pragma unroll
         for (int j = 0; j < NV; j++) {
             const int64_t c = ((int64_t)j * THREADS + lane) * VEC;
             if (c < a.width) {
 #pragma unroll
                 for (int i = 0; i < VEC; i++) {
-                    const float d = h[j][i] - mean;
-                    sum[0] += WIDE || c + i < a.width ? d * d : 0.0f;
+                    const float d = WIDE || c + i < a.width ? h[j][i] - first : 0.0f;
+                    left[0] += d;
+                    left[1] += d * d;
                 }
             }
         }
-        rows_reduce<THREADS, 1>(sum, shared, 1);
-        const float rstd = 1.0f / sqrtf(sum[0] / (float)a.width + a.eps);
+        rows_reduce<THREADS, 2>(left, shared_left, 0);
+        statistics(a, first, left, &mean, &rstd);
         if (lane == 0) {
             put_statistics(a, row, mean, rstd);
         }
@@ -143,35 +155,42 @@ __global__ __launch_bounds__(THREADS > 256 ? THREADS : 256) void layer_norm_kern
 }
 
 // Rows longer than 1024 threads hold: read for the mean, for the squares and for the result (`sum` is written in the last
-// round, since it may be x).
+// round, since it may be x).  A thread adds up thousands of numbers here, and the correction of the mean is as good as the
+// first mean is near: its sum is compensated (Kahan, "Further remarks on reducing truncation errors", 1965), a vector at a time.
 template <typename T, typename W, int VEC, bool WIDE>
 __global__ __launch_bounds__(1024) void layer_norm_long_kernel(LayerNormArgs a)
 {
-    __shared__ float shared[2][1][16];
+    __shared__ float shared[1][1][16], shared_left[1][2][16];
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        float sum[1] = {0.0f};
+        float sum[1] = {0.0f}, lost = 0.0f;
         for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.width; c += 1024 * VEC) {
-            float h[VEC];
+            float h[VEC], part = 0.0f;
             get_row_part<T, VEC, WIDE>(a, row, c, h);
 #pragma unroll
             for (int i = 0; i < VEC; i++) {
-                sum[0] += h[i];
+                part += h[i];
             }
+            part -= lost;
+            const float total = sum[0] + part;
+            lost = (total - sum[0]) - part;
+            lost = lost == lost ? lost : 0.0f;  // an infinite sum stays one
+            sum[0] = total;
         }
         rows_reduce<1024, 1>(sum, shared, 0);
-        const float mean = sum[0] / (float)a.width;
-        sum[0] = 0.0f;
+        const float first = sum[0] / (float)a.width;
+        float left[2] = {0.0f, 0.0f}, mean, rstd;
         for (int64_t c = (int64_t)threadIdx.x * VEC; c < a.width; c += 1024 * VEC) {
             float h[VEC];
             get_row_part<T, VEC, WIDE>(a, row, c, h);
 #pragma unroll
             for (int i = 0; i < VEC; i++) {
-                const float d = h[i] - mean;
-                sum[0] += WIDE || c + i < a.width ? d * d : 0.0f;
+                const float d = WIDE || c + i < a.width ? h[i] - first : 0.0f;
+                left[0] += d;
+                left[1] += d * d;
             }
         }
-        rows_reduce<1024, 1>(sum, shared, 1);
-        const float rstd = 1.0f / sqrtf(sum[0] / (float)a.width + a.eps);
+        rows_reduce<1024, 2>(left, shared_left, 0);
+        statistics(a, first, left, &mean, &rstd);
         if (threadIdx.x == 0) {
             put_statistics(a, row, mean, rstd);
         }
