@@ -110,6 +110,9 @@ int64_t sum_rows(const GatedArgs& a, int64_t padded)
     return (a.rows + each - 1) / each;
 }
 
+// FLOAT16: rows and columns that have a scale, of the gradients that are wanted
+int64_t scales(const GatedArgs& a) { return (a.want_x != 0 ? a.rows : 0) + (a.want_weights != 0 ? 2 * a.inner : 0); }
+
 BackwardLayout backward_layout(const GatedArgs& a)
 {
     const int e = elem_size((Elem)a.elem);
@@ -138,9 +141,9 @@ BackwardLayout backward_layout(const GatedArgs& a)
     if (want_weights && scaled) {
         l.by_columns = s.take(a.rows * 2 * l.padded * e);
     }
-    if (scaled) {
-        l.most = s.take((a.rows + 2 * a.inner) * 4);
-        l.factors = s.take((a.rows + 2 * a.inner) * 4);
+    if (scaled && (want_x || want_weights)) {
+        l.most = s.take(scales(a) * 4);
+        l.factors = s.take(scales(a) * 4);
     }
     if (a.want_biases != 0) {
         l.sums = s.take(sum_rows(a, l.padded) * 2 * a.inner * 4);
@@ -230,10 +233,13 @@ hipError_t launch_gated_grad(const GatedArgs& a, hipStream_t stream)
     g.rows_each = gate_rows_of(a, l.padded);
     g.sums = (float*)at(l.sums);
     if (l.most >= 0) {
-        g.row_most = (uint32_t*)at(l.most);
-        g.column_most = g.row_most + a.rows;
-        g.row_factor = (float*)at(l.factors);
-        g.column_factor = g.row_factor + a.rows;
+        const int64_t rows = a.want_x != 0 ? a.rows : 0;
+        uint32_t* const most = (uint32_t*)at(l.most);
+        float* const factors = (float*)at(l.factors);
+        g.row_most = a.want_x != 0 ? most : nullptr;
+        g.row_factor = a.want_x != 0 ? factors : nullptr;
+        g.column_most = a.want_weights != 0 ? most + rows : nullptr;
+        g.column_factor = a.want_weights != 0 ? factors + rows : nullptr;
     }
     OPSCV_LAUNCH(launch_gate_grad(g, stream));
     PadArgs pads;

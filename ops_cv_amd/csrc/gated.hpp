@@ -45,7 +45,8 @@ struct GateGradArgs {
     int64_t rows_each = 0;  // of a workgroup: gate_rows()
     // sums over the rows of each workgroup: (rows / rows_each, 2 inner); may be null
     float* sums = nullptr;
-    // FLOAT16: largest absolute values as bits, by rows and by columns (2 inner), and the factors that undo the scales
+    // FLOAT16: largest absolute values as bits, by rows and by columns (2 inner), and the factors that undo the scales; null
+    // for the direction that is not written
     uint32_t *row_most = nullptr, *column_most = nullptr;
     float *row_factor = nullptr, *column_factor = nullptr;
 };

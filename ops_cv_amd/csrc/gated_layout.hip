@@ -180,18 +180,20 @@ __global__ __launch_bounds__(kThreads) void gate_most_kernel(GateGradArgs a)
             rows[r] = row;
         }
     }
+    if (a.column_most != nullptr) {
 #pragma unroll
-    for (int e = 0; e < N; e++) {
-        atomicMax(&columns[0][c + e], most[0][e]);
-        atomicMax(&columns[1][c + e], most[1][e]);
+        for (int e = 0; e < N; e++) {
+            atomicMax(&columns[0][c + e], most[0][e]);
+            atomicMax(&columns[1][c + e], most[1][e]);
+        }
     }
     __syncthreads();
     for (int i = (int)threadIdx.x; i < kRows + 2 * kColumns<T>; i += kThreads) {
         if (i < kRows) {
-            if (row0 + i < end) {
+            if (a.row_most != nullptr && row0 + i < end) {
                 atomicMax(&a.row_most[row0 + i], rows[i]);
             }
-        } else {
+        } else if (a.column_most != nullptr) {
             const int half = (i - kRows) / kColumns<T>, at = (i - kRows) % kColumns<T>;
             if (column0 + at < a.inner) {
                 atomicMax(&a.column_most[half * a.inner + column0 + at], columns[half][at]);
@@ -217,7 +219,7 @@ __global__ __launch_bounds__(kThreads) void gate_grad_kernel(GateGradArgs a)
 #pragma unroll
             for (int half = 0; half < 2; half++) {
                 by_column[half][e] = 1.0f;
-                if (column0 + c + e < a.inner) {
+                if (a.column_most != nullptr && column0 + c + e < a.inner) {
                     by_column[half][e] = lift(a.column_most[half * a.inner + column0 + c + e]);
                     if (blockIdx.y == 0 && part == 0) {
                         a.column_factor[half * a.inner + column0 + c + e] = 1.0f / by_column[half][e];
@@ -244,7 +246,7 @@ __global__ __launch_bounds__(kThreads) void gate_grad_kernel(GateGradArgs a)
         float dg[N], du[N], x[N];
         gate_values<T, KIND>(read[i % kAhead], row < end, dg, du);
         float by_row = 1.0f;
-        if (kScaled && row < end) {
+        if (kScaled && a.row_most != nullptr && row < end) {
             by_row = lift(a.row_most[row]);
             if (blockIdx.x == 0 && c == 0) {
                 a.row_factor[row] = 1.0f / by_row;
@@ -312,10 +314,17 @@ hipError_t run_gate_grad(const GateGradArgs& a, hipStream_t stream)
     }
     const dim3 grid((unsigned)columns, (unsigned)rows);
     if constexpr (std::is_same_v<T, _Float16>) {
-        const int64_t words = a.rows + 2 * a.inner, blocks = (words + kThreads - 1) / kThreads;
-        hipLaunchKernelGGL(clear_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(kThreads), 0, stream, a.row_most,
-                           words);  // the columns' follow the rows'
-        hipLaunchKernelGGL((gate_most_kernel<T, KIND, SHORT>), grid, dim3(kThreads), 0, stream, a);
+        // the columns' follow the rows'; the biases' sums are of unscaled numbers and need neither
+        const int64_t words = (a.row_most != nullptr ? a.rows : 0) + (a.column_most != nullptr ? 2 * a.inner : 0);
+        const int64_t blocks = (words + kThreads - 1) / kThreads;
+        if ((a.by_rows != nullptr) != (a.row_most != nullptr) || (a.by_columns != nullptr) != (a.column_most != nullptr)) {
+            return hipErrorInvalidValue;
+        }
+        if (words > 0) {
+            hipLaunchKernelGGL(clear_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(kThreads), 0, stream,
+                               a.row_most != nullptr ? a.row_most : a.column_most, words);
+            hipLaunchKernelGGL((gate_most_kernel<T, KIND, SHORT>), grid, dim3(kThreads), 0, stream, a);
+        }
     }
     hipLaunchKernelGGL((gate_grad_kernel<T, KIND, SHORT>), grid, dim3(kThreads), 0, stream, a);
     return hipGetLastError();
