@@ -130,6 +130,8 @@ class Model(torch.nn.Module):
         grid = torch.meshgrid(torch.arange(FRAMES), torch.arange(n), torch.arange(n), indexing="ij")
         self.positions = torch.stack([g.flatten() for g in grid])[:, None].to(device)
         self.state = torch.tensor([1234, 0], device=device)  # seed, offset
+        # the dropouts' offsets from it: made here, since what is copied from the host cannot be recorded
+        self.offsets = torch.tensor([[0, i] for i in range(2 * BLOCKS)], device=device).view(BLOCKS, 2, 2)
 
     def forward(self, frames, p=0.0):
         """(videos, FRAMES, 3, SIZE, SIZE) -> scores of the ways."""
@@ -137,8 +139,8 @@ class Model(torch.nn.Module):
         cut = frames.view(b, FRAMES, 3, n, PATCH, n, PATCH).permute(0, 1, 3, 5, 2, 4, 6).reshape(b, FRAMES * n * n, -1)
         x = cut.bfloat16() @ self.patches.t()
         positions = self.positions.expand(-1, b, -1)
-        # a mask for every dropout and call: the state is a device tensor, so a recorded step would draw new ones as well
-        states = (self.state + torch.tensor([[0, i] for i in range(2 * BLOCKS)], device=x.device)).view(BLOCKS, 2, 2) if p > 0.0 else None
+        # a mask for every dropout and call: the state is a device tensor, so a recorded pass draws new ones as well
+        states = self.state + self.offsets if p > 0.0 else None
         for i, block in enumerate(self.blocks):
             x = block(x, self.table, positions, states[i] if p > 0.0 else (None, None), p)
         if p > 0.0:
