@@ -357,8 +357,16 @@ __device__ __forceinline__ void product(const ProductArgs& a, uint32_t block, ch
     typedef Side<T, Q_TURNED, S::kTokens, TB, S::kWaves> SideQ;
     SideP side_p;
     SideQ side_q;
-    // gate or up, rows of 32 features in turn: with eight wavefronts by the wavefront, with four by the load
-    const int own = GATED && S::kWaves == 8 ? (wave >> 2) & 1 : 0;
+    constexpr int kTerms = kRowBytes / kE;
+    uint32_t first_stage = 0, stages = (uint32_t)((a.terms + kTerms - 1) / kTerms);
+    if (a.parts > 1) {
+        first_stage = tile.part * a.part_stages;
+        const uint32_t left = stages > first_stage ? stages - first_stage : 0;
+        stages = left < a.part_stages ? left : a.part_stages;
+    }
+    // gate or up.  Rows of terms, 32 features of each in turn: with eight wavefronts by the wavefront, with four by the load.
+    // Turned rows: one after the other; `own` is the one that side_p has the offsets of.
+    int own = GATED ? (S::kWaves == 8 ? (wave >> 2) & 1 : 0) : (P_TURNED && (int64_t)first_stage * kTerms >= a.p_turn ? 1 : 0);
     const int64_t own_stride = own != 0 ? a.p_stride[1] : a.p_stride[0];
     side_p.places(own_stride, a.features - f0, wave, lane, [](int r) { return GATED ? (r >> 6) * 32 + (r & 31) : r; });
     if constexpr (GATED && S::kWaves == 4) {
@@ -378,13 +386,6 @@ __device__ __forceinline__ void product(const ProductArgs& a, uint32_t block, ch
     if constexpr (!Q_TURNED) {
         rsrc_q = att::buffer((const char*)a.q + t0 * a.q_stride * kE, kInside);
     }
-    constexpr int kTerms = kRowBytes / kE;
-    uint32_t first_stage = 0, stages = (uint32_t)((a.terms + kTerms - 1) / kTerms);
-    if (a.parts > 1) {
-        first_stage = tile.part * a.part_stages;
-        const uint32_t left = stages > first_stage ? stages - first_stage : 0;
-        stages = left < a.part_stages ? left : a.part_stages;
-    }
     const uint32_t lds0 = att::lds_place(lds);
     const auto load_stage = [&](uint32_t stage, int buffer) {
         const int64_t term = (int64_t)(first_stage + stage) * kTerms;
@@ -395,6 +396,12 @@ __device__ __forceinline__ void product(const ProductArgs& a, uint32_t block, ch
             const int64_t row = half != 0 ? term - a.p_turn : term;
             const int64_t there = a.p_terms - row;  // none or less where only zeros stand for the padding of the other operand
             const int64_t stride = half != 0 ? a.p_stride[1] : a.p_stride[0];
+            if constexpr (!Q_TURNED) {  // the weights' gradients are sums over one operand's rows
+                if (half != own) {      // stages are loaded in their order: once, if at all
+                    own = half;
+                    side_p.places(stride, a.features - f0, wave, lane, [](int r) { return r; });
+                }
+            }
             const att::rsrc_t rsrc = att::buffer((const char*)(half != 0 ? a.p[1] : a.p[0]) + (row * stride + f0) * kE, kInside);
             side_p.load([&](int) { return rsrc; }, to, 0, there < left ? (int)there : left);
         } else {
