@@ -61,8 +61,8 @@ struct ProductArgs {
 
 // silu, gelu (erf) and gelu (tanh) in the order of opscvGateActivation: value, and derivative where wanted.
 
-// By the hardware's exponential and reciprocal, a unit in the last place each; the product with log2 e loses |x| 2^-24 of the
-// exponential.  A workgroup has nothing to do beside its results' activations: with expf and a division the product of 4096
+// By the hardware's exponential and reciprocal, a unit in the last place each; the product with log2 e loses up to 1.5 |x| 2^-24
+// of the exponential (3.7e-6 measured at -80).  A workgroup has nothing to do beside its results' activations: with expf and a division the product of 4096
 // rows, 4096 to 14336 bf16, takes 838 us.
 __device__ __forceinline__ float sigmoid(float x)
 {
@@ -70,8 +70,10 @@ __device__ __forceinline__ float sigmoid(float x)
 }
 
 // The normal distribution's upper tail from a >= 0 on, and exp(-a^2 / 2), as exp(-a^2 / 2) t q(t) with t = 1 / (1 + 0.26 a): q
-// is a polynomial fitted to the tail's relative error over 0 <= a <= 14.5, 3e-8 (from there on both are 0).  Sixteen
-// instructions, where erfc with its branches takes the time of a fifth of a product over 1280 terms.
+// is a polynomial fitted to the tail's relative error over 0 <= a <= 14.5, 3e-8 in exact arithmetic (from there on both are 0).
+// In 32 bits the exponential's argument is rounded, and the tail is off by up to 1.25 a^2 2^-24 of itself more: 1.4e-6 at 5, 7e-6
+// at 13, where it is 1e-38.  Sixteen instructions, where erfc with its branches takes the time of a fifth of a product over 1280
+// terms.
 __device__ __forceinline__ float upper_tail(float a, float* bell)
 {
     const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.26f, a, 1.0f));
