@@ -242,8 +242,10 @@ typedef enum {
 } opscvGateActivation;
 
 /*
- * Gated projections, the first half of a gated feed-forward block, in one kernel:
+ * Gated projections, the first half of a gated feed-forward block:
  *   gate = x gateWeight^T + gateBias,  up = x upWeight^T + upBias,  y = activation(gate) * up
+ * One kernel where x and the weights start on 16 bytes, with rows of whole vectors of 16 bytes, and there are tiles for every CU;
+ * others are copied to the workspace first, and few tiles of long rows are made in parts, whose 32-bit sums go by way of it.
  * x : (..., width), y, gate, up : (..., inner), one to five dimensions; gateWeight, upWeight : (inner, width); gateBias,
  * upBias : (inner), both or neither; all of one type.  Products are summed up in 32 bits, and y is computed from those sums.
  *   gate, up : NULL (both), or the sums rounded to the type: what the backward pass reads

@@ -12,7 +12,7 @@
 // Bound by memory: every element is read once and written once, so a row stays in registers between its sums and its
 // result.  A row belongs to one wavefront (up to 16 elements a lane, or 24), to 256 threads, or to 1024; longer rows are read three
 // times.  Sums are 32-bit, over a thread's elements, then over lanes, then over wavefronts, in a fixed order.  10952 rows of 1280
-// fp16, x, residual, sum and y: 22.7 us, 4.9 TB/s; gradients of 16384 rows of 2048 bf16 with their other gradient 60.4, 4.5 TB/s,
+// fp16, x, residual, sum and y: 23.3 us, 4.8 TB/s (22.7 without the mean's correction); gradients of 16384 rows of 2048 bf16 with their other gradient 60.4, 4.5 TB/s,
 // of which the join of the columns' partial sums is 4.5; eight rows of 4096: 6.3, the launch.
 #include <hip/hip_runtime.h>
 

@@ -74,8 +74,9 @@ inline int64_t last_end(const int64_t* count, const int64_t* length, int64_t slo
 //     three more are under way (128 rows of 4096 to 14336 bf16 71 us and 56, 512 of 4096 to 4096 55 and 44; with more tiles than CUs,
 //     768 rows, 64 and 82; FLOAT and the gradients, whose operands take longer out of LDS, gain nothing);
 //   - the terms in parts, of four stages at least, so that there is a workgroup for every CU and they end together: the parts'
-//     sums are written and read again, 4 MB a microsecond, by a kernel of 8 us, start and end of it and of the other's among
-//     them.
+//     sums are written and read again, 4 MB a microsecond, and 8 us are charged for every product in parts, for the kernel that
+//     joins them and the start and end of workgroups.  That is what a product alone takes; both of the gradients' are joined by
+//     one kernel, of 4 to 6.6 us, and charged for twice.
 // 256 rows, 1024 to 4096 FLOAT: 71 us in one part.  777 rows, 1001 to 2731 FLOAT, both gradients: 247 us where parts were sized
 // by the total alone.
 // `us` is 0 where no way fits a launch.

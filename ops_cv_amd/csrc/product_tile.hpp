@@ -13,7 +13,7 @@
 // activation and the product need no other lane.
 //
 // Bound by the products, at the clock that power allows (1.75 to 1.9 GHz; 63 % of a SIMD's cycles are products, LDS is busy for a
-// quarter).  4096 rows of 4096 to 14336 bf16: 778 us, 1235 TFLOP/s; both gradients of 4096 rows of 2048 to 8192 470 us, 1170
+// quarter).  4096 rows of 4096 to 14336 bf16: 786 us, 1224 TFLOP/s; both gradients of 4096 rows of 2048 to 8192 474 us, 1160
 // TFLOP/s; 10952 rows of 1280 to 3413 fp16 with gate and up 260, of which the results' way out is 80.
 #pragma once
 
@@ -72,7 +72,7 @@ __device__ __forceinline__ float sigmoid(float x)
 // The normal distribution's upper tail from a >= 0 on, and exp(-a^2 / 2), as exp(-a^2 / 2) t q(t) with t = 1 / (1 + 0.26 a): q
 // is a polynomial fitted to the tail's relative error over 0 <= a <= 14.5, 3e-8 in exact arithmetic (from there on both are 0).
 // In 32 bits the exponential's argument is rounded, and the tail is off by up to 1.25 a^2 2^-24 of itself more: 1.4e-6 at 5, 7e-6
-// at 13, where it is 1e-38.  Sixteen instructions, where erfc with its branches takes the time of a fifth of a product over 1280
+// at 13, where it is 6e-39.  Sixteen instructions, where erfc with its branches takes the time of a fifth of a product over 1280
 // terms.
 __device__ __forceinline__ float upper_tail(float a, float* bell)
 {

@@ -87,7 +87,7 @@ struct DropoutArgs {
 
 // How the matrix products of a call are made (product_plan.hpp).
 struct ProductPlan {
-    int tile = 0;                                        // kTile128, kTile256, kTileFew
+    int tile = 0;                                        // kTile128, kTile256, kTileFew, kTileSlim, kTileDeep
     double us = 0.0;                                     // expected time
     int64_t parts[2] = {1, 1}, part_stages[2] = {0, 0};  // of the terms; more than one part: a second kernel joins their sums
 };
